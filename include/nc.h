@@ -256,6 +256,24 @@ NC_API nc_tensor *nc_from_device(nc_ctx *ctx, nc_dtype dt, const void *device_da
  * and persistent tensors.  Constant across steady-state steps, whose temporaries come from the arena. */
 NC_API uint64_t nc_device_alloc_count(const nc_ctx *ctx);
 
+/* ---- attention of this engine (additive; the reference composes it of bmm, masked_fill and softmax) ---- */
+/* Tensors are [batch, tokens, heads, head dim], as a projection's reshape leaves them; strided views (slices of a fused
+ * projection, transposes of head-major tensors) are read in place where their columns are next to each other.
+ * Rotary positions of x [B, L, H, D], D <= 256: n_axes (1 .. 4) sections of axis_dims[a] columns each, whose pairs -- (i, i +
+ * axis_dims[a] / 2), or neighbours where `interleaved` -- are turned by positions[.., a] * base^(-2 i / axis_dims[a]);
+ * positions i32 [L, n_axes] or [B, L, n_axes].  The head's other columns stay. */
+NC_API nc_tensor *nc_rope(nc_tensor *x, nc_tensor *positions, int n_axes, const int64_t *axis_dims, float base,
+                          int interleaved);
+/* The RMS norm of every head of x [B, L, H, D] with the rotation in the same pass: the first q_heads heads are weighted by
+ * q_weight [D], the others by k_weight [D] (NULL: not weighted).  n_axes 0 and positions NULL: the norm alone. */
+NC_API nc_tensor *nc_qk_norm_rope(nc_tensor *x, int64_t q_heads, nc_tensor *q_weight, nc_tensor *k_weight, float eps,
+                                  nc_tensor *positions, int n_axes, const int64_t *axis_dims, float base,
+                                  int interleaved);
+/* softmax(scale q k^T) v of q [B, Lq, Hq, D] over k and v [B, Lk, Hkv, D], Hq a multiple of Hkv (heads of keys are shared), D <=
+ * 256, no causal mask.  key_lengths i32 [B] or NULL: how many of each sequence's keys count; a sequence without keys
+ * gives zeros. */
+NC_API nc_tensor *nc_cross_attention(nc_tensor *q, nc_tensor *k, nc_tensor *v, nc_tensor *key_lengths, float scale);
+
 #ifdef __cplusplus
 }
 #endif

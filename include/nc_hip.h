@@ -297,6 +297,56 @@ NC_HIP_API int nc_hip_linear_int8(int64_t M, int64_t K, int64_t N, const float *
                                   const float *wscale, const float *bias, float *y, void *ws, size_t ws_bytes,
                                   void *stream);
 
+/* Rotary positions.  x [B, L, H, D] (a token's heads, D <= 256 floats each; strides sx[3] of batch, token and head in elements,
+ * columns next to each other) -> y, contiguous.  The head's first columns are n_axes (1 .. 4) sections of axis_dims[a] columns
+ * (even); pair i of section a -- columns i and i + axis_dims[a] / 2 of it, or 2 i and 2 i + 1 where `interleaved` is set -- is
+ * turned by pos[token][a] * base^(-2 i / axis_dims[a]); the columns past the sections are copied.  pos is i32 [L, n_axes], or
+ * [B, L, n_axes] where pos_batched is set; angles are taken in fp64.  Backward: gx (+)= gy turned back (both contiguous).
+ * No counterpart in the reference. */
+NC_HIP_API int nc_hip_rope_fwd(int64_t B, int64_t L, int64_t H, int64_t D, const float *x, const int64_t *sx,
+                               const int32_t *pos, int pos_batched, int n_axes, const int64_t *axis_dims, float base,
+                               int interleaved, float *y, void *stream);
+NC_HIP_API int nc_hip_rope_bwd(int64_t B, int64_t L, int64_t H, int64_t D, const float *gy, const int32_t *pos,
+                               int pos_batched, int n_axes, const int64_t *axis_dims, float base, int interleaved,
+                               float *gx, int accumulate, void *stream);
+/* RMS norm of every head, then the rotation, in one pass: n = x / sqrt(mean(x^2) + eps), y = rope(n w), w = wq [D] for the first
+ * q_heads heads and wk [D] for the others (NULL: ones).  n_axes may be 0 (the norm alone; pos unused).  Backward: gx (+)= ...;
+ * gwq and gwk (+)= the sums over their heads' rows (either may be NULL), in a fixed order, through a workspace of
+ * nc_hip_qk_norm_rope_bwd_workspace bytes; gx, gwq and gwk must not overlap.  No counterpart in the reference. */
+NC_HIP_API int nc_hip_qk_norm_rope_fwd(int64_t B, int64_t L, int64_t H, int64_t D, int64_t q_heads, const float *x,
+                                       const int64_t *sx, const float *wq, const float *wk, float eps,
+                                       const int32_t *pos, int pos_batched, int n_axes, const int64_t *axis_dims,
+                                       float base, int interleaved, float *y, void *stream);
+NC_HIP_API size_t nc_hip_qk_norm_rope_bwd_workspace(int64_t B, int64_t L, int64_t H, int64_t D);
+NC_HIP_API int nc_hip_qk_norm_rope_bwd(int64_t B, int64_t L, int64_t H, int64_t D, int64_t q_heads, const float *x,
+                                       const int64_t *sx, const float *wq, const float *wk, float eps,
+                                       const int32_t *pos, int pos_batched, int n_axes, const int64_t *axis_dims,
+                                       float base, int interleaved, const float *gy, float *gx, float *gwq, float *gwk,
+                                       int acc_x, int acc_wq, int acc_wk, void *ws, size_t ws_bytes, void *stream);
+
+/* Attention of queries q [B, Lq, Hq, D] to keys and values k, v [B, Lk, Hkv, D] of another length, D <= 256, without a causal
+ * mask; strides sq, sk, sv[3] of batch, token and head in elements, columns next to each other.  Query head h reads the keys of
+ * head h / (Hq / Hkv).  key_len i32 [B] (NULL: Lk): a sequence's keys from there on do not count and are not read (values below
+ * 0 or past Lk are taken as 0 and Lk).  o [B, Lq, Hq, D], contiguous: softmax(scale q . k) v, zeros where a sequence has no
+ * keys; lse [B, Hq, Lq] (may be NULL): log sum exp of the scaled products, for the backward.
+ * Backward, from the forward's inputs, o and lse: gq [B, Lq, Hq, D], gk and gv [B, Lk, Hkv, D] (contiguous, not overlapping, each
+ * may be NULL) (+)= ..., zeros for keys that do not count; sums in a fixed order.  No counterpart in the reference (its
+ * attention is bmm, masked_fill, softmax and bmm). */
+NC_HIP_API size_t nc_hip_cross_attention_fwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv,
+                                                       int64_t D);
+NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D,
+                                          float scale, const float *q, const int64_t *sq, const float *k,
+                                          const int64_t *sk, const float *v, const int64_t *sv, const int32_t *key_len,
+                                          float *o, float *lse, void *ws, size_t ws_bytes, void *stream);
+NC_HIP_API size_t nc_hip_cross_attention_bwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv,
+                                                       int64_t D);
+NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D,
+                                          float scale, const float *q, const int64_t *sq, const float *k,
+                                          const int64_t *sk, const float *v, const int64_t *sv, const int32_t *key_len,
+                                          const float *o, const float *lse, const float *go, float *gq, float *gk,
+                                          float *gv, int acc_q, int acc_k, int acc_v, void *ws, size_t ws_bytes,
+                                          void *stream);
+
 #ifdef __cplusplus
 }
 #endif

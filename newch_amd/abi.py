@@ -174,10 +174,17 @@ NC_DEVICE_SIGNATURES: dict[str, tuple] = {
     "nc_device_alloc_count": (c_uint64, [P]),
 }
 
+# Attention functions of this engine (not in the reference ABI).
+NC_ATTENTION_SIGNATURES: dict[str, tuple] = {
+    "nc_rope": (P, [P, P, c_int, I64P, c_float, c_int]),
+    "nc_qk_norm_rope": (P, [P, c_int64, P, P, c_float, P, c_int, I64P, c_float, c_int]),
+    "nc_cross_attention": (P, [P, P, P, P, c_float]),
+}
+
 
 def bind(lib: ctypes.CDLL, strict: bool = True) -> ctypes.CDLL:
     """Sets restype/argtypes for every nc.h function (raises AttributeError on a missing one when
-    strict) and for the device extensions the library has."""
+    strict) and for this engine's additive functions, where the library has them."""
     for name, (res, args) in NC_SIGNATURES.items():
         try:
             fn = getattr(lib, name)
@@ -186,7 +193,7 @@ def bind(lib: ctypes.CDLL, strict: bool = True) -> ctypes.CDLL:
                 raise
             continue
         fn.restype, fn.argtypes = res, args
-    for name, (res, args) in NC_DEVICE_SIGNATURES.items():
+    for name, (res, args) in (NC_DEVICE_SIGNATURES | NC_ATTENTION_SIGNATURES).items():
         if hasattr(lib, name):
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args

@@ -93,6 +93,19 @@ SIGNATURES = {
                                     c_int64, c_int, I64P, I64P, I64P, I64P, P, c_size_t, P]),
     "nc_hip_gemm_s8_nt": (c_int, [c_int64, c_int64, c_int64, P, c_int64, P, c_int64, P, c_int64, P]),
     "nc_hip_linear_int8_workspace": (c_size_t, [c_int64, c_int64]),
+    "nc_hip_rope_fwd": (c_int, [c_int64, c_int64, c_int64, c_int64, P, I64P, P, c_int, c_int, I64P, c_float, c_int, P, P]),
+    "nc_hip_rope_bwd": (c_int, [c_int64, c_int64, c_int64, c_int64, P, P, c_int, c_int, I64P, c_float, c_int, P, c_int,
+                                P]),
+    "nc_hip_qk_norm_rope_fwd": (c_int, [c_int64, c_int64, c_int64, c_int64, c_int64, P, I64P, P, P, c_float, P, c_int,
+                                        c_int, I64P, c_float, c_int, P, P]),
+    "nc_hip_qk_norm_rope_bwd_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    "nc_hip_qk_norm_rope_bwd": (c_int, [c_int64, c_int64, c_int64, c_int64, c_int64, P, I64P, P, P, c_float, P, c_int,
+                                        c_int, I64P, c_float, c_int, P, P, P, P, c_int, c_int, c_int, P, c_size_t, P]),
+    "nc_hip_cross_attention_fwd_workspace": (c_size_t, [c_int64] * 6),
+    "nc_hip_cross_attention_fwd": (c_int, [c_int64] * 6 + [c_float, P, I64P, P, I64P, P, I64P, P, P, P, P, c_size_t, P]),
+    "nc_hip_cross_attention_bwd_workspace": (c_size_t, [c_int64] * 6),
+    "nc_hip_cross_attention_bwd": (c_int, [c_int64] * 6 + [c_float, P, I64P, P, I64P, P, I64P, P, P, P, P, P, P, P, c_int,
+                                                           c_int, c_int, P, c_size_t, P]),
     "nc_hip_linear_int8": (c_int, [c_int64, c_int64, c_int64, P, P, P, P, P, P, c_size_t, P]),
 }
 
@@ -298,3 +311,51 @@ class Kernels:
 
     def linear_int8(self, M, K, N, x, wq, wscale, bias, y, ws, ws_bytes, stream=None):
         self._ok(self.lib.nc_hip_linear_int8(M, K, N, x, wq, wscale, bias, y, ws, ws_bytes, stream), "linear_int8")
+
+    def rope_fwd(self, B, L, H, D, x, sx, pos, pos_batched, axis_dims, base, interleaved, y, stream=None):
+        """axis_dims: the columns of each position axis's section of the head."""
+        self._ok(self.lib.nc_hip_rope_fwd(B, L, H, D, x, _i64(sx), pos, int(pos_batched), len(axis_dims),
+                                          _i64(axis_dims), base, int(interleaved), y, stream), "rope_fwd")
+
+    def rope_bwd(self, B, L, H, D, gy, pos, pos_batched, axis_dims, base, interleaved, gx, accumulate=True, stream=None):
+        self._ok(self.lib.nc_hip_rope_bwd(B, L, H, D, gy, pos, int(pos_batched), len(axis_dims), _i64(axis_dims), base,
+                                          int(interleaved), gx, int(accumulate), stream), "rope_bwd")
+
+    def qk_norm_rope_fwd(self, B, L, H, D, q_heads, x, sx, wq, wk, eps, pos, pos_batched, axis_dims, base, interleaved, y,
+                         stream=None):
+        """The first q_heads heads weighted by wq, the others by wk (None: ones); axis_dims () and pos None: the norm alone."""
+        self._ok(self.lib.nc_hip_qk_norm_rope_fwd(B, L, H, D, q_heads, x, _i64(sx), wq, wk, eps, pos, int(pos_batched),
+                                                  len(axis_dims), _i64(axis_dims), base, int(interleaved), y, stream),
+                 "qk_norm_rope_fwd")
+
+    def qk_norm_rope_bwd_workspace(self, B, L, H, D):
+        return self.lib.nc_hip_qk_norm_rope_bwd_workspace(B, L, H, D)
+
+    def qk_norm_rope_bwd(self, B, L, H, D, q_heads, x, sx, wq, wk, eps, pos, pos_batched, axis_dims, base, interleaved, gy,
+                         gx, gwq, gwk, ws=None, ws_bytes=0, accumulate=True, stream=None):
+        """accumulate: one flag, or one each for gx, gwq and gwk."""
+        ax, aq, ak = accumulate if isinstance(accumulate, tuple) else (accumulate,) * 3
+        self._ok(self.lib.nc_hip_qk_norm_rope_bwd(B, L, H, D, q_heads, x, _i64(sx), wq, wk, eps, pos, int(pos_batched),
+                                                  len(axis_dims), _i64(axis_dims), base, int(interleaved), gy, gx, gwq,
+                                                  gwk, int(ax), int(aq), int(ak), ws, ws_bytes, stream),
+                 "qk_norm_rope_bwd")
+
+    def cross_attention_fwd_workspace(self, B, Lq, Lk, Hq, Hkv, D):
+        return self.lib.nc_hip_cross_attention_fwd_workspace(B, Lq, Lk, Hq, Hkv, D)
+
+    def cross_attention_fwd(self, B, Lq, Lk, Hq, Hkv, D, scale, q, sq, k, sk, v, sv, key_len, o, lse, ws=None, ws_bytes=0,
+                            stream=None):
+        """key_len: i32 [B] or None; lse: [B, Hq, Lq] for the backward, or None."""
+        self._ok(self.lib.nc_hip_cross_attention_fwd(B, Lq, Lk, Hq, Hkv, D, scale, q, _i64(sq), k, _i64(sk), v, _i64(sv),
+                                                     key_len, o, lse, ws, ws_bytes, stream), "cross_attention_fwd")
+
+    def cross_attention_bwd_workspace(self, B, Lq, Lk, Hq, Hkv, D):
+        return self.lib.nc_hip_cross_attention_bwd_workspace(B, Lq, Lk, Hq, Hkv, D)
+
+    def cross_attention_bwd(self, B, Lq, Lk, Hq, Hkv, D, scale, q, sq, k, sk, v, sv, key_len, o, lse, go, gq, gk, gv, ws=None,
+                            ws_bytes=0, accumulate=False, stream=None):
+        """Gradients stored (or, accumulate, added: one flag, or one each for gq, gk and gv); any of the three may be None."""
+        aq, ak, av = accumulate if isinstance(accumulate, tuple) else (accumulate,) * 3
+        self._ok(self.lib.nc_hip_cross_attention_bwd(B, Lq, Lk, Hq, Hkv, D, scale, q, _i64(sq), k, _i64(sk), v, _i64(sv),
+                                                     key_len, o, lse, go, gq, gk, gv, int(aq), int(ak), int(av), ws,
+                                                     ws_bytes, stream), "cross_attention_bwd")
