@@ -6,14 +6,15 @@
 //     dp = go . v,  ds = p (dp - go . o) scale,  gq = ds k,  gk = ds^T q,  gv = p^T go
 //
 // A sequence without keys gives o = 0, lse = -inf and no gradient.  Keys and values past a sequence's length are not read.
-#include "common.hpp"
+//
+// The products run on the fp16 matrix cores with operands in two pieces (attention.hpp), packed once into a workspace.
+#include "attention.hpp"
 
 #include <math.h>
 
 namespace nchip {
 
-constexpr int kAttnD = 256;
-constexpr int kAttnB = 256;
+constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
 
 struct AttnArgs {
     int64_t B, Lq, Lk, Hq, Hkv, D, G;  // G: query heads of a key head
@@ -42,34 +43,331 @@ __device__ __forceinline__ float wg_reduce(float v, float *red, bool max) {
     return max ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// a workgroup a query row, a lane a key
-__global__ __launch_bounds__(kAttnB) void k_attn_fwd_row(AttnArgs a, const float *q, const float *k, const float *v,
-                                                         const int *key_len, float *o, float *lse) {
-    __shared__ float qs[kAttnD], ps[kAttnB], red[4];
-    const int64_t rows = a.B * a.Lq * a.Hq;
-    const int t = threadIdx.x, D = (int)a.D;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const int64_t h = r % a.Hq, i = r / a.Hq % a.Lq, b = r / a.Hq / a.Lq, u = h / a.G, n = attn_keys(a, key_len, b);
-        const float *kb = k + b * a.sk[0] + u * a.sk[2], *vb = v + b * a.sv[0] + u * a.sv[2];
-        __syncthreads();
-        if (t < D) qs[t] = q[b * a.sq[0] + i * a.sq[1] + h * a.sq[2] + t];
-        float m = -INFINITY, l = 0.0f, acc = 0.0f;
-        for (int64_t j0 = 0; j0 < n; j0 += kAttnB) {
-            const int c = (int)min((int64_t)kAttnB, n - j0);
-            __syncthreads();
-            const float s = t < c ? a.scale * dot_row(qs, kb + (j0 + t) * a.sk[1], D) : -INFINITY;
-            const float mn = fmaxf(m, wg_reduce(s, red, true));
-            const float p = t < c ? (mn == -INFINITY ? 0.0f : expf(s - mn)) : 0.0f;
-            const float w = m == mn ? 1.0f : expf(m - mn);
-            ps[t] = p;
-            l = l * w + wg_reduce(p, red, false);
-            acc *= w;
-            m = mn;
-            if (t < D)
-                for (int j = 0; j < c; j++) acc = fma_(ps[j], vb[(j0 + j) * a.sv[1] + t], acc);
+// ------------------------------------------------------------------------------------------------
+// packing: a workgroup a tile of 32 rows, into one or both layouts
+// ------------------------------------------------------------------------------------------------
+// Rows of a (sequence, head of keys) pair: queries' row R is token R / G of query head u G + R % G, keys' are tokens (G = 1).
+struct PackJob {
+    const float *src;
+    int64_t sb, sl, sh;
+    int64_t len, tiles;    // rows and tiles of a pair, before key_len
+    int G, by_len;         // rows are cut by key_len
+    char *rows, *turned;   // [pair][tile][128 DP]; may be NULL
+    float *exps;           // [pair][tile] exponents of the scales
+    int64_t first;         // the job's first workgroup
+};
+struct PackArgs {
+    PackJob job[4];
+    int jobs;
+    int64_t total, Lk, Hkv;
+    int D;
+    const int *key_len;
+};
+
+__device__ __forceinline__ int64_t keys_of(int64_t Lk, const int *key_len, int64_t b) {
+    if (!key_len) return Lk;
+    const int64_t n = key_len[b];
+    return n < 0 ? 0 : n < Lk ? n : Lk;
+}
+
+template <int DP>
+__global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
+    constexpr int C = DP / 8, PER = (C + 7) / 8;  // chunks of a row; of a lane
+    constexpr int LD = DP + 1;
+    __shared__ float tile[kTile * LD];
+    __shared__ float red[kAttnWaves];
+    const int t = threadIdx.x, row = t & 31, cl = t >> 5;
+    for (int64_t w = blockIdx.x; w < a.total; w += gridDim.x) {
+        int jx = 0;
+        while (jx + 1 < a.jobs && w >= a.job[jx + 1].first) jx++;
+        const PackJob &j = a.job[jx];
+        const int64_t pair = (w - j.first) / j.tiles, tl = (w - j.first) - pair * j.tiles;
+        const int64_t b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int64_t n = j.by_len ? keys_of(a.Lk, a.key_len, b) : j.len;
+        const int64_t R = tl * kTile + row;
+        if (tl * kTile >= n) continue;  // no workgroup reads this tile
+        const bool live = R < n;
+        const int64_t i = live ? R / j.G : 0, g = live ? R - i * j.G : 0;
+        const float *src = j.src + b * j.sb + i * j.sl + (u * j.G + g) * j.sh;
+        float x[PER][8], most = 0.0f;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[k][e] = 0.0f;
+            const int c = cl + 8 * k;
+            if (live && c < C) load8(src, 8 * c, a.D, x[k]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[k][e]));
         }
-        if (t < D) o[r * D + t] = n ? acc / l : 0.0f;
-        if (lse && t == 0) lse[(b * a.Hq + h) * a.Lq + i] = n ? m + logf(l) : -INFINITY;
+        most = wave_max_nan_skip(most);
+        __syncthreads();  // the last tile has been read
+        if ((t & 63) == 0) red[t >> 6] = most;
+        if (j.turned) {
+#pragma unroll
+            for (int k = 0; k < PER; k++)
+                if (cl + 8 * k < C)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) tile[row * LD + 8 * (cl + 8 * k) + e] = x[k][e];
+        }
+        __syncthreads();
+        const int ex = tile_exponent(__builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3])));
+        const float inv = pow2i(-ex);
+        const int64_t at = pair * j.tiles + tl;
+        if (t == 0) j.exps[at] = (float)ex;
+        if (j.rows) {
+            char *out = j.rows + at * tile_bytes(DP);
+#pragma unroll
+            for (int k = 0; k < PER; k++)
+                if (cl + 8 * k < C) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[k][e] *= inv;
+                    const Split8 s = split8(x[k]);
+                    h8 *o = (h8 *)out + (cl + 8 * k) * 32 + row;
+                    o[0] = s.hi;
+                    o[4 * DP] = s.lo;
+                }
+        }
+        if (j.turned) {
+            char *out = j.turned + at * tile_bytes(DP);
+            for (int k = t; k < 4 * DP; k += kAttnB) {  // fragment k / 64, its lane k % 64
+                const int f = k >> 6, lane = k & 63, s = f / (DP / 32), col = 32 * (f % (DP / 32)) + (lane & 31);
+                const float *p = tile + (16 * s + 4 * (lane >> 5)) * LD + col;
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = p[(e < 4 ? e : e + 4) * LD] * inv;
+                const Split8 q = split8(y);
+                h8 *o = (h8 *)out + k;
+                o[0] = q.hi;
+                o[4 * DP] = q.lo;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// stages of tiles in LDS
+// ------------------------------------------------------------------------------------------------
+// blocks of 1 KiB dealt over the workgroup's waves, copied straight to LDS; nothing waits for them here
+__device__ __forceinline__ void stage_copy(const char *src, uint32_t lds, int blocks) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    for (int i = wave; i < blocks; i += kAttnWaves) dma16(src + i * 1024 + lane * 16, lds + i * 1024);
+}
+__device__ __forceinline__ void stage_wait() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's copies and LDS reads
+    __builtin_amdgcn_s_barrier();                                // everyone's
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
+}
+
+// Workgroups are dealt round robin over the 8 XCDs: consecutive units of a launch go to one XCD, which then keeps their
+// keys in its L2.
+__device__ __forceinline__ int64_t xcd_unit(int64_t w, int64_t units) {
+    const int64_t each = units / 8, rest = units % 8, x = w % 8, k = w / 8;
+    return x * each + (x < rest ? x : rest) + k;
+}
+
+// ------------------------------------------------------------------------------------------------
+// forward
+// ------------------------------------------------------------------------------------------------
+struct FwdArgs {
+    AttnArgs a;
+    const float *q;
+    const char *kr, *vt;         // packed keys (rows), values (turned)
+    const float *kx, *vx;        // their exponents
+    const int *key_len;
+    float *o, *lse;
+    float *po;                   // splits: [split][pair][row][D] sums, and {reference, sum} of each row
+    f2 *pm;
+    int64_t rows, tiles, units;  // rows of a pair (G Lq), tiles of keys of a pair at most, workgroups' units
+    int qtiles, splits;          // groups of 128 rows of a pair, parts its keys are cut into
+};
+
+// A wave holds 32 rows of queries as columns: s^T = k q^T (A: 32 keys), so that a row's scores lie in the registers of two lanes
+// and its maximum, sum and scale are theirs; p^T is then the operand of o^T = v^T p^T as it lies.  One pass over the keys: the
+// reference m a row's exponents are taken from moves only when a score passes it by 2^4, and o and the sum with it; p is held as
+// 2^10 p (at most 2^14) in two fp16, so a p below 2^-13 loses low bits against an absolute 2^-35.
+constexpr float kPShift = 10.0f, kPSlack = 4.0f;
+
+template <int DP, int TPS, int OCC>
+__global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
+    constexpr int KS = DP / 16, NT = DP / 32;
+    constexpr int TB = 128 * DP;                 // bytes of a packed tile
+    constexpr int STAGE = 2 * TPS * TB;          // keys' tiles, then values'
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const AttnArgs &a = f.a;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const uint32_t lds = lds_address(smem);
+    for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
+        const int64_t unit = xcd_unit(w, f.units);
+        const int qt = (int)(unit % f.qtiles);
+        const int64_t rest = unit / f.qtiles;
+        const int split = (int)(rest % f.splits);
+        const int64_t pair = rest / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int64_t n = keys_of(a.Lk, f.key_len, b), nt = (n + kTile - 1) / kTile;
+        const int64_t t0 = nt * split / f.splits, t1 = nt * (split + 1) / f.splits;
+        const char *kr = f.kr + pair * f.tiles * TB, *vt = f.vt + pair * f.tiles * TB;
+        const float *kx = f.kx + pair * f.tiles, *vx = f.vx + pair * f.tiles;
+
+        auto copy = [&](int64_t t, int buf) {
+            const int c = (int)min((int64_t)TPS, t1 - t) * (TB / 1024);
+            const uint32_t at = __builtin_amdgcn_readfirstlane(lds + buf * STAGE);
+            stage_copy(kr + t * TB, at, c);
+            stage_copy(vt + t * TB, at + TPS * TB, c);
+        };
+        __syncthreads();  // the last unit's stages have been read
+        if (t0 < t1) copy(t0, 0);
+
+        // this lane's row of queries, times scale log2(e), as the second operand
+        const int64_t R = ((int64_t)qt * kAttnWaves + wave) * kTile + (lane & 31);
+        const bool live = R < f.rows;
+        const int64_t i = live ? R / a.G : 0, g = live ? R - i * a.G : 0, h = u * a.G + g;
+        const float *qrow = f.q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2];
+        h8 qh[KS], ql[KS];
+        float cq;
+        {
+            float x[KS][8], most = 0.0f;
+            const float c = a.scale * kLog2e;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                if (live) load8(qrow, 16 * s + 8 * half, (int)a.D, x[s]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[s][e] = live ? x[s][e] * c : 0.0f;
+                    most = __builtin_fmaxf(most, finite_abs(x[s][e]));
+                }
+            }
+            const int e = tile_exponent(halves_max(most));
+            const float inv = pow2i(-e);
+            cq = pow2i(e);
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[s][k] *= inv;
+                const Split8 p = split8(x[s]);
+                qh[s] = p.hi, ql[s] = p.lo;
+            }
+        }
+        f16x o[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
+        float m = -INFINITY, l = 0.0f, E = -1000.0f;
+        for (int64_t t = t0, buf = 0; t < t1; t += TPS, buf ^= 1) {
+            stage_wait();
+            if (t + TPS < t1) copy(t + TPS, (int)buf ^ 1);
+            const char *st = smem + buf * STAGE;
+#pragma unroll
+            for (int x = 0; x < TPS; x++) {
+                if (t + x >= t1) break;
+                const h8 *kf = (const h8 *)(st + x * TB) + lane, *vf = (const h8 *)(st + (TPS + x) * TB) + lane;
+                f16x s;
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KS; k++) s = mfma3(kf[64 * k], kf[64 * k + 4 * DP], qh[k], ql[k], s);
+                const float c = __builtin_fmaxf(cq * pow2i((int)kx[t + x]), 0x1p-126f);  // -inf * c stays -inf
+                const int64_t left = n - (t + x) * kTile;
+                if (left < kTile) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (8 * (r / 4) + 4 * half + r % 4 >= left) s[r] = -INFINITY;
+                }
+                float top = s[0];
+#pragma unroll
+                for (int r = 1; r < 16; r++) top = __builtin_fmaxf(top, s[r]);
+                top = halves_max(top) * c;
+                const float ev = vx[t + x];
+                if (__any(top > m + kPSlack) || ev > E) {
+                    const float mn = top > m + kPSlack ? top : m, En = __builtin_fmaxf(E, ev);
+                    const float al = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                    const float ao = al * __builtin_amdgcn_exp2f(E - En);
+                    l *= al;
+                    m = mn;
+                    E = En;
+#pragma unroll
+                    for (int d = 0; d < NT; d++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) o[d][r] *= ao;
+                }
+                // values of smaller tiles count through smaller p (no smaller than 2^-60: below what o can show)
+                const float dv = __builtin_fmaxf(ev - E, -60.0f), off = kPShift + dv - m;
+                float sum = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[r] = __builtin_amdgcn_exp2f(fma_(s[r], c, off));
+                    sum += s[r];
+                }
+                l = fma_(sum, __builtin_amdgcn_exp2f(-dv), l);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[e] = s[8 * k + e];
+                    const Split8 p = split8(y);
+#pragma unroll
+                    for (int d = 0; d < NT; d++)
+                        o[d] = mfma3(vf[64 * (k * NT + d)], vf[64 * (k * NT + d) + 4 * DP], p.hi, p.lo, o[d]);
+                }
+            }
+        }
+        l = halves_sum(l);
+        if (!live) continue;
+        if (f.splits == 1) {
+            const float inv = l != 0.0f ? pow2i((int)E) / l : 0.0f;  // no keys: o is zero
+            float *row = f.o + ((b * a.Lq + i) * a.Hq + h) * a.D;
+#pragma unroll
+            for (int d = 0; d < NT; d++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    store4(row, 32 * d + 8 * j + 4 * half, (int)a.D,
+                           f4{o[d][4 * j] * inv, o[d][4 * j + 1] * inv, o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv}, 0);
+            if (f.lse && half == 0)
+                f.lse[(b * a.Hq + h) * a.Lq + i] = nt ? fma_(m - kPShift, kLn2, logf(l)) : -INFINITY;
+        } else {
+            const int64_t pr = ((int64_t)split * a.B * a.Hkv + pair) * f.rows + R;
+            const float inv = t0 < t1 ? pow2i((int)E) : 0.0f;
+            float *row = f.po + pr * a.D;
+#pragma unroll
+            for (int d = 0; d < NT; d++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    store4(row, 32 * d + 8 * j + 4 * half, (int)a.D,
+                           f4{o[d][4 * j] * inv, o[d][4 * j + 1] * inv, o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv}, 0);
+            if (half == 0) f.pm[pr] = f2{t0 < t1 ? m - kPShift : -INFINITY, l};
+        }
+    }
+}
+
+// the splits' parts of a row joined: its reference is the largest, parts count by 2^(reference - largest)
+__global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t rows, int splits, const float *po, const f2 *pm,
+                                                      float *o, float *lse) {
+    const int64_t all = a.B * a.Hkv * rows, D4 = (a.D + 3) / 4;
+    for (int64_t x = (int64_t)blockIdx.x * kAttnB + threadIdx.x; x < all * D4; x += (int64_t)gridDim.x * kAttnB) {
+        const int64_t pr = x / D4, pair = pr / rows, R = pr - pair * rows, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int d = (int)(x - pr * D4) * 4;
+        const int64_t i = R / a.G, h = u * a.G + (R - i * a.G);
+        float M = -INFINITY;
+        for (int s = 0; s < splits; s++) {
+            const float m = pm[s * all + pr].x;
+            M = M >= m || M != M ? M : m;  // a NaN part stays
+        }
+        f4 sum = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.0f;
+        for (int s = 0; s < splits; s++) {
+            const f2 ml = pm[s * all + pr];
+            if (ml.x == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(ml.x - M);
+            const float *p = po + (s * all + pr) * a.D + d;
+            l = fma_(w, ml.y, l);
+            for (int e = 0; e < 4; e++)
+                if (d + e < a.D) sum[e] = fma_(w, p[e], sum[e]);
+        }
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        store4(o + ((b * a.Lq + i) * a.Hq + h) * a.D, d, (int)a.D, sum * inv, 0);
+        if (lse && d == 0) lse[(b * a.Hq + h) * a.Lq + i] = M == -INFINITY ? -INFINITY : fma_(M, kLn2, logf(l));
     }
 }
 
@@ -159,10 +457,83 @@ static unsigned row_grid(int64_t rows) { return (unsigned)(rows < (1 << 20) ? ro
 
 using namespace nchip;
 
+namespace nchip {
+
+static int padded(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
+static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// dispatch over the padded columns
+#define NC_ATTN_DP(dp, ...)                                  \
+    do {                                                     \
+        if ((dp) == 32) { constexpr int DP = 32; __VA_ARGS__; }         \
+        else if ((dp) == 64) { constexpr int DP = 64; __VA_ARGS__; }    \
+        else if ((dp) == 96) { constexpr int DP = 96; __VA_ARGS__; }    \
+        else if ((dp) == 128) { constexpr int DP = 128; __VA_ARGS__; }  \
+        else { constexpr int DP = 256; __VA_ARGS__; }                   \
+    } while (0)
+
+struct FwdPlan {
+    int DP, qtiles, splits;
+    int64_t rows, tiles, pairs, units;
+    size_t kr, vt, kx, vx, po, pm, total;  // offsets into the workspace
+};
+
+static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D) {
+    FwdPlan p{};
+    p.DP = padded(D);
+    p.rows = Hq / Hkv * Lq;
+    p.pairs = B * Hkv;
+    p.tiles = (Lk + kTile - 1) / kTile;
+    p.qtiles = (int)((p.rows + kAttnWaves * kTile - 1) / (kAttnWaves * kTile));
+    // keys are cut where there are fewer than two workgroups a CU, into parts of at least four tiles
+    const int64_t whole = p.pairs * p.qtiles;
+    int64_t splits = whole ? 2 * kPlanCUs / whole : 1;
+    if (splits > p.tiles / 4) splits = p.tiles / 4;
+    p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+    p.units = whole * p.splits;
+    const size_t pt = (size_t)(p.pairs * p.tiles);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += up256(bytes);
+        return here;
+    };
+    p.kr = take(pt * tile_bytes(p.DP));
+    p.vt = take(pt * tile_bytes(p.DP));
+    p.kx = take(pt * 4);
+    p.vx = take(pt * 4);
+    if (p.splits > 1) {
+        p.po = take((size_t)p.splits * p.pairs * p.rows * D * 4);
+        p.pm = take((size_t)p.splits * p.pairs * p.rows * 8);
+    }
+    p.total = at;
+    return p;
+}
+
+static unsigned attn_grid(int64_t units) { return (unsigned)(units < kAttnGrid ? units : kAttnGrid); }
+
+template <class F, class A>
+static void attn_launch(F *kernel, int64_t units, size_t lds, hipStream_t st, const A &args) {
+    if (lds > 65536) (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL(kernel, dim3(attn_grid(units)), dim3(kAttnB), lds, st, args);
+}
+
+static void pack_launch(PackArgs &p, int64_t pairs, int DP, hipStream_t st) {
+    p.total = 0;
+    for (int j = 0; j < p.jobs; j++) {
+        p.job[j].first = p.total;
+        p.total += pairs * p.job[j].tiles;
+    }
+    if (!p.total) return;
+    NC_ATTN_DP(DP, hipLaunchKernelGGL((k_attn_pack<DP>), dim3(attn_grid(p.total)), dim3(kAttnB), 0, st, p));
+}
+
+}  // namespace nchip
+
 extern "C" NC_HIP_API size_t nc_hip_cross_attention_fwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv,
                                                                   int64_t D) {
-    (void)B, (void)Lq, (void)Lk, (void)Hq, (void)Hkv, (void)D;
-    return 0;
+    if (B <= 0 || Lq <= 0 || Lk < 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
+    return fwd_plan(B, Lq, Lk, Hq, Hkv, D).total;
 }
 
 extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D,
@@ -175,8 +546,26 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     if (const int rc = attn_args(what, a, B, Lq, Lk, Hq, Hkv, D, scale, sq, sk, sv)) return rc;
     if (B == 0 || Lq == 0) return NC_HIP_OK;
     if (!q || !o || (Lk && (!k || !v))) return set_error(NC_HIP_ERR_ARG, "%s: q, k, v and o are needed", what);
-    (void)ws, (void)ws_bytes;
-    hipLaunchKernelGGL(k_attn_fwd_row, dim3(row_grid(B * Lq * Hq)), kAttnB, 0, as_stream(stream), a, q, k, v, key_len, o, lse);
+    const FwdPlan p = fwd_plan(B, Lq, Lk, Hq, Hkv, D);
+    if (p.total && (!ws || ws_bytes < p.total))
+        return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, p.total);
+    hipStream_t st = as_stream(stream);
+    char *const w = (char *)ws;
+    if (Lk) {
+        PackArgs pk{};
+        pk.Lk = Lk, pk.Hkv = Hkv, pk.D = (int)D, pk.key_len = key_len, pk.jobs = 2;
+        pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, 1, w + p.kr, nullptr, (float *)(w + p.kx), 0};
+        pk.job[1] = {v, sv[0], sv[1], sv[2], Lk, p.tiles, 1, 1, nullptr, w + p.vt, (float *)(w + p.vx), 0};
+        pack_launch(pk, p.pairs, p.DP, st);
+    }
+    FwdArgs f{a, q, w + p.kr, w + p.vt, (float *)(w + p.kx), (float *)(w + p.vx), key_len, o, lse, (float *)(w + p.po), (f2 *)(w + p.pm),
+              p.rows, p.tiles, p.units, p.qtiles, p.splits};
+    NC_ATTN_DP(p.DP, constexpr int TPS = DP <= 64 ? 2 : 1; constexpr int OCC = DP <= 128 ? 2 : 1;
+               attn_launch(&k_attn_fwd<DP, TPS, OCC>, p.units, 2 * 2 * TPS * 128 * DP, st, f));
+    if (p.splits > 1) {
+        const int64_t items = p.pairs * p.rows * ((D + 3) / 4);
+        hipLaunchKernelGGL(k_attn_join, dim3(attn_grid((items + kAttnB - 1) / kAttnB)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, o, lse);
+    }
     return check_launch(what);
 }
 

@@ -69,7 +69,9 @@ def attention64(q, k, v, lens, scale, go=None):
     """Forward, and backward where go is given: {o, lse, gq, gk, gv}: (value, bound).
 
     eps(n) = 2^-20 + n U bounds a product of n terms relative to the sum of their magnitudes: the operands' own roundings where
-    they are held in pieces (at most 2^-22 each, and 2^-22 for the product that is left out) and n additions."""
+    they are held in pieces (at most 2^-22 each, and 2^-22 for the product that is left out) and n additions.  Pieces also have a
+    smallest step: probabilities 2^-35 of the row's largest, values 2^-40 of their tile's largest, their products' gradients 2^-36
+    (2^-25 against a largest of 2^11 at least)."""
     q, k, v = (np.asarray(t, np.float64) for t in (q, k, v))
     B, Lq, Hq, D = q.shape
     Lk, Hkv = k.shape[1:3]
@@ -103,7 +105,7 @@ def attention64(q, k, v, lens, scale, go=None):
             # exp's own error: 4 U, and the argument's rounding relative to the largest magnitudes in the row
             ep = es + es.max(1, keepdims=True) + U * (8 + 2 * np.abs(s) + 2 * np.abs(m))
             o = p @ V
-            eo = (p * (2 * ep.max(1, keepdims=True) + eps(n) + n * U)) @ np.abs(V) + 2.0 ** -39 * np.abs(V).max() * n
+            eo = (p * (2 * ep.max(1, keepdims=True) + eps(n) + n * U)) @ np.abs(V) + 2.0 ** -35 * np.abs(V).max() * n
             add("o", (b, slice(None), h), o, eo)
             lse = (m + np.log(l))[:, 0]
             out["lse"][0][b, h] = lse
@@ -116,7 +118,7 @@ def attention64(q, k, v, lens, scale, go=None):
             ep = ep + out["lse"][1][b, h][:, None]  # p is taken again from the row's log-sum-exp
             ds = p * (dp - delta) * sc
             eds = abs(sc) * p * (eps(D) * (dpm + dm) + (np.abs(g) * eo).sum(1, keepdims=True)
-                                 + np.abs(dp - delta) * (2 * ep + 4 * U)) + 2.0 ** -38 * np.abs(ds).max()
+                                 + np.abs(dp - delta) * (2 * ep + 4 * U)) + 2.0 ** -36 * np.abs(ds).max()
             add("gq", (b, slice(None), h), ds @ K, eds @ np.abs(K) + eps(n) * np.abs(ds) @ np.abs(K))
             add("gk", (b, slice(0, n), u), ds.T @ Q, eds.T @ np.abs(Q) + eps(Lq * G) * np.abs(ds).T @ np.abs(Q))
             add("gv", (b, slice(0, n), u), p.T @ g,
