@@ -22,27 +22,6 @@ struct AttnArgs {
     float scale;
 };
 
-__device__ __forceinline__ int64_t attn_keys(const AttnArgs &a, const int *key_len, int64_t b) {
-    if (!key_len) return a.Lk;
-    const int64_t n = key_len[b];
-    return n < 0 ? 0 : n < a.Lk ? n : a.Lk;
-}
-
-__device__ __forceinline__ float dot_row(const float *a, const float *b, int D) {
-    float s = 0.0f;
-    for (int d = 0; d < D; d++) s = fma_(a[d], b[d], s);
-    return s;
-}
-
-// value of all the workgroup's lanes
-__device__ __forceinline__ float wg_reduce(float v, float *red, bool max) {
-    v = max ? wave_max_nan_skip(v) : wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return max ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
-}
-
 // ------------------------------------------------------------------------------------------------
 // packing: a workgroup a tile of 32 rows, into one or both layouts
 // ------------------------------------------------------------------------------------------------
@@ -55,6 +34,8 @@ struct PackJob {
     char *rows, *turned;   // [pair][tile][128 DP]; may be NULL
     float *exps;           // [pair][tile] exponents of the scales
     int64_t first;         // the job's first workgroup
+    const float *o, *lse;  // the output gradient's job: o (laid out as src), the rows' log-sum-exps [B, Hq, Lq]
+    float *stats;          // [pair][tile][64]: log2-sum-exps (infinite past the rows), src . o of the tile's rows
 };
 struct PackArgs {
     PackJob job[4];
@@ -75,7 +56,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
     constexpr int C = DP / 8, PER = (C + 7) / 8;  // chunks of a row; of a lane
     constexpr int LD = DP + 1;
     __shared__ float tile[kTile * LD];
-    __shared__ float red[kAttnWaves];
+    __shared__ float red[kAttnWaves], dots[8][kTile];
     const int t = threadIdx.x, row = t & 31, cl = t >> 5;
     for (int64_t w = blockIdx.x; w < a.total; w += gridDim.x) {
         int jx = 0;
@@ -88,8 +69,9 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
         if (tl * kTile >= n) continue;  // no workgroup reads this tile
         const bool live = R < n;
         const int64_t i = live ? R / j.G : 0, g = live ? R - i * j.G : 0;
-        const float *src = j.src + b * j.sb + i * j.sl + (u * j.G + g) * j.sh;
-        float x[PER][8], most = 0.0f;
+        const int64_t off = b * j.sb + i * j.sl + (u * j.G + g) * j.sh;
+        const float *src = j.src + off;
+        float x[PER][8], most = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int k = 0; k < PER; k++) {
 #pragma unroll
@@ -98,9 +80,16 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
             if (live && c < C) load8(src, 8 * c, a.D, x[k]);
 #pragma unroll
             for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[k][e]));
+            if (j.stats && live && c < C) {
+                float y[8];
+                load8(j.o + off, 8 * c, a.D, y);
+#pragma unroll
+                for (int e = 0; e < 8; e++) dot = fma_(x[k][e], y[e], dot);
+            }
         }
         most = wave_max_nan_skip(most);
         __syncthreads();  // the last tile has been read
+        if (j.stats) dots[cl][row] = dot;
         if ((t & 63) == 0) red[t >> 6] = most;
         if (j.turned) {
 #pragma unroll
@@ -114,6 +103,13 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
         const float inv = pow2i(-ex);
         const int64_t at = pair * j.tiles + tl;
         if (t == 0) j.exps[at] = (float)ex;
+        if (j.stats && t < kTile) {
+            float d = dots[0][t];
+#pragma unroll
+            for (int e = 1; e < 8; e++) d += dots[e][t];
+            j.stats[at * 64 + t] = live ? j.lse[(b * a.Hkv * j.G + u * j.G + g) * (j.len / j.G) + i] * kLog2e : INFINITY;
+            j.stats[at * 64 + 32 + t] = d;
+        }
         if (j.rows) {
             char *out = j.rows + at * tile_bytes(DP);
 #pragma unroll
@@ -371,71 +367,277 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
     }
 }
 
-__global__ __launch_bounds__(kAttnB) void k_attn_dq_row(AttnArgs a, const float *q, const float *k, const float *v,
-                                                        const int *key_len, const float *o, const float *lse, const float *go,
-                                                        float *gq, int acc_q) {
-    __shared__ float qs[kAttnD], gs[kAttnD], ps[kAttnB], red[4];
-    const int64_t rows = a.B * a.Lq * a.Hq;
-    const int t = threadIdx.x, D = (int)a.D;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const int64_t h = r % a.Hq, i = r / a.Hq % a.Lq, b = r / a.Hq / a.Lq, u = h / a.G, n = attn_keys(a, key_len, b);
-        const float *kb = k + b * a.sk[0] + u * a.sk[2], *vb = v + b * a.sv[0] + u * a.sv[2];
-        __syncthreads();
-        if (t < D) qs[t] = q[b * a.sq[0] + i * a.sq[1] + h * a.sq[2] + t], gs[t] = go[r * D + t];
-        const float delta = wg_reduce(t < D ? go[r * D + t] * o[r * D + t] : 0.0f, red, false);
-        const float ls = lse[(b * a.Hq + h) * a.Lq + i];
-        float acc = 0.0f;
-        for (int64_t j0 = 0; j0 < n; j0 += kAttnB) {
-            const int c = (int)min((int64_t)kAttnB, n - j0);
-            __syncthreads();
-            if (t < c) {
-                const float p = expf(a.scale * dot_row(qs, kb + (j0 + t) * a.sk[1], D) - ls);
-                ps[t] = p * (dot_row(gs, vb + (j0 + t) * a.sv[1], D) - delta) * a.scale;
+// ------------------------------------------------------------------------------------------------
+// backward: two kernels, each with its own recomputed scores, so that every gradient is summed in one place and order
+// ------------------------------------------------------------------------------------------------
+struct BwdArgs {
+    AttnArgs a;
+    const char *kr, *kt, *vr, *qr, *qt, *gr, *gt;  // packed: rows and turned layouts
+    const float *kx, *vx, *qx, *gx, *stats;
+    const int *key_len;
+    float *gq, *gk, *gv;                           // the gradients, or the splits' parts [split][...] where there are any
+    int64_t rows, qtiles, ktiles, units, part_q, part_k;  // rows of a pair, tiles, units; floats of a part
+    int groups, splits;                            // groups of four tiles of a pair, parts the other side is cut into
+    int acc_q, acc_k, acc_v;
+};
+
+// The gradients of the scores have no bound to scale them by beforehand: a lane's column (a key, or a query's row) has a power of
+// two F of its own that puts its largest |x| into [2^11, 2^12) when it first shows or passes 2^15, and its sums are brought along.
+__device__ __forceinline__ bool column_scale(float most, float &F, float &by) {
+    by = 1.0f;
+    const bool over = most * F > 32768.0f;
+    if (over) {
+        int e = (int)(__float_as_uint(most) >> 23);
+        e = e < 12 ? 12 : e;
+        const float f = __uint_as_float((uint32_t)(127 + 11 + 127 - e) << 23);
+        by = f / F;
+        F = f;
+    }
+    return __any(over);
+}
+
+template <int NT>
+__device__ __forceinline__ void scale_acc(f16x (&acc)[NT], float by) {
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[d][r] *= by;
+}
+
+template <int NT>
+__device__ __forceinline__ void store_column(float *row, const f16x (&acc)[NT], float by, int half, int D, int add) {
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            store4(row, 32 * d + 8 * j + 4 * half, D,
+                   f4{acc[d][4 * j] * by, acc[d][4 * j + 1] * by, acc[d][4 * j + 2] * by, acc[d][4 * j + 3] * by}, add);
+}
+
+// gk and gv: a wave holds 32 keys as columns and goes over the tiles of queries: s = q k^T and dp = go v^T, whose rows are queries,
+// then gv^T += go^T p and gk^T += q^T ds with p and ds as they lie.  Padded rows of queries have an infinite log-sum-exp: p = 0.
+template <int DP, int STAGES, int OCC>
+__global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
+    constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, STAGE = 4 * TB + 256;
+    constexpr bool REG = DP <= 128;  // keys and values stay in registers, else they are read again for every tile
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const AttnArgs &a = f.a;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const uint32_t lds = lds_address(smem);
+    for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
+        const int64_t unit = xcd_unit(w, f.units);
+        const int kg = (int)(unit % f.groups);
+        const int64_t rest = unit / f.groups;
+        const int split = (int)(rest % f.splits);
+        const int64_t pair = rest / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int64_t n = keys_of(a.Lk, f.key_len, b);
+        const int64_t kt = (int64_t)kg * kAttnWaves + wave, key = kt * kTile + (lane & 31);
+        const bool any = (int64_t)kg * kAttnWaves * kTile < n, mine = kt * kTile < n, live = key < n;
+        const int64_t t0 = any ? f.qtiles * split / f.splits : 0, t1 = any ? f.qtiles * (split + 1) / f.splits : 0;
+        const int64_t q0 = pair * f.qtiles;
+        auto copy = [&](int64_t t, int buf) {
+            const uint32_t at = __builtin_amdgcn_readfirstlane(lds + buf * STAGE);
+            const int64_t x = (q0 + t) * TB;
+            stage_copy(f.qr + x, at, TB / 1024);
+            stage_copy(f.gr + x, at + TB, TB / 1024);
+            stage_copy(f.qt + x, at + 2 * TB, TB / 1024);
+            stage_copy(f.gt + x, at + 3 * TB, TB / 1024);
+            if (threadIdx.x < 16) dma16(f.stats + (q0 + t) * 64 + threadIdx.x * 4, at + 4 * TB);
+        };
+        __syncthreads();  // the last unit's stages have been read
+        if (STAGES == 2 && t0 < t1) copy(t0, 0);
+        const int64_t tile = pair * f.ktiles + (mine ? kt : 0);
+        const h8 *kf = (const h8 *)(f.kr + tile * TB) + lane, *vf = (const h8 *)(f.vr + tile * TB) + lane;
+        h8 kh[REG ? KS : 1], kl[REG ? KS : 1], vh[REG ? KS : 1], vl[REG ? KS : 1];
+        float ck = 0.0f, cv = 0.0f;
+        if (mine) {
+            ck = pow2i((int)f.kx[tile]) * a.scale * kLog2e;
+            cv = pow2i((int)f.vx[tile]);
+            if constexpr (REG) {
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    kh[s] = kf[64 * s], kl[s] = kf[64 * s + 4 * DP];
+                    vh[s] = vf[64 * s], vl[s] = vf[64 * s + 4 * DP];
+                }
             }
-            __syncthreads();
-            if (t < D)
-                for (int j = 0; j < c; j++) acc = fma_(ps[j], kb[(j0 + j) * a.sk[1] + t], acc);
         }
-        if (t < D) gq[r * D + t] = (acc_q ? gq[r * D + t] : 0.0f) + acc;
+        f16x dk[NT], dv[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) dk[t][r] = dv[t][r] = 0.0f;
+        float F = 0x1p100f, E = -1000.0f;
+        for (int64_t t = t0, buf = 0; t < t1; t++) {
+            if constexpr (STAGES == 1) {
+                __syncthreads();  // the last tile has been read
+                copy(t, 0);
+            }
+            stage_wait();
+            if (STAGES == 2 && t + 1 < t1) copy(t + 1, (int)buf ^ 1);
+            const char *st = smem + buf * STAGE;
+            if (STAGES == 2) buf ^= 1;
+            if (!mine) continue;
+            const h8 *qf = (const h8 *)st + lane, *gf = (const h8 *)(st + TB) + lane;
+            const h8 *qtf = (const h8 *)(st + 2 * TB) + lane, *gtf = (const h8 *)(st + 3 * TB) + lane;
+            const f4 *rows = (const f4 *)(st + 4 * TB) + half;
+            f16x s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) s = mfma3(qf[64 * k], qf[64 * k + 4 * DP], REG ? kh[k] : kf[64 * k], REG ? kl[k] : kf[64 * k + 4 * DP], s);
+#pragma unroll
+            for (int k = 0; k < KS; k++) dp = mfma3(gf[64 * k], gf[64 * k + 4 * DP], REG ? vh[k] : vf[64 * k], REG ? vl[k] : vf[64 * k + 4 * DP], dp);
+            const float ex = f.gx[q0 + t], eq = f.qx[q0 + t];
+            if (ex > E) {
+                scale_acc(dv, __builtin_amdgcn_exp2f(E - ex));
+                E = ex;
+            }
+            // p as 2^14 p, less for tiles of smaller gradients (no less than 2^-60 times: below what gv can show)
+            const float sh = 14.0f + __builtin_fmaxf(ex - E, -60.0f), base = live ? sh : -INFINITY;
+            const float c = ck * pow2i((int)eq), c2 = cv * pow2i((int)ex);
+            float most = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const f4 ls = rows[2 * j], de = rows[8 + 2 * j];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int r = 4 * j + e;
+                    s[r] = __builtin_amdgcn_exp2f(fma_(s[r], c, base - ls[e]));
+                    dp[r] = s[r] * fma_(dp[r], c2, -de[e]);
+                    most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
+                }
+            }
+            const float kap = __builtin_amdgcn_exp2f(eq - sh);
+            float by;
+            if (column_scale(halves_max(most) * kap, F, by)) scale_acc(dk, by);
+            const float kF = kap * F;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                float y[8], z[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = s[8 * k + e], z[e] = dp[8 * k + e] * kF;
+                const Split8 ps = split8(y), ds = split8(z);
+#pragma unroll
+                for (int d = 0; d < NT; d++) {
+                    const int at = 64 * (k * NT + d);
+                    dv[d] = mfma3(gtf[at], gtf[at + 4 * DP], ps.hi, ps.lo, dv[d]);
+                    dk[d] = mfma3(qtf[at], qtf[at + 4 * DP], ds.hi, ds.lo, dk[d]);
+                }
+            }
+        }
+        if (key < a.Lk) {
+            const int64_t at = ((b * a.Lk + key) * a.Hkv + u) * a.D;
+            const bool some = live && t0 < t1;
+            if (f.gk) store_column(f.gk + split * f.part_k + at, dk, some ? a.scale / F : 0.0f, half, (int)a.D, f.acc_k);
+            if (f.gv) store_column(f.gv + split * f.part_k + at, dv, some ? __builtin_amdgcn_exp2f(E - 14.0f) : 0.0f, half, (int)a.D, f.acc_v);
+        }
     }
 }
 
-// a workgroup a key, a lane a query row
-__global__ __launch_bounds__(kAttnB) void k_attn_dkv_row(AttnArgs a, const float *q, const float *k, const float *v,
-                                                         const int *key_len, const float *o, const float *lse,
-                                                         const float *go, float *gk, float *gv, int acc_k, int acc_v) {
-    __shared__ float ks[kAttnD], vs[kAttnD], ps[kAttnB], ds[kAttnB];
-    const int64_t rows = a.B * a.Lk * a.Hkv, nq = a.G * a.Lq;
-    const int t = threadIdx.x, D = (int)a.D;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const int64_t u = r % a.Hkv, j = r / a.Hkv % a.Lk, b = r / a.Hkv / a.Lk, n = attn_keys(a, key_len, b);
-        __syncthreads();
-        float sk = 0.0f, sv = 0.0f;
-        if (j < n) {
-            if (t < D) ks[t] = k[b * a.sk[0] + j * a.sk[1] + u * a.sk[2] + t], vs[t] = v[b * a.sv[0] + j * a.sv[1] + u * a.sv[2] + t];
-            for (int64_t i0 = 0; i0 < nq; i0 += kAttnB) {
-                const int c = (int)min((int64_t)kAttnB, nq - i0);
-                __syncthreads();
-                if (t < c) {
-                    const int64_t i = (i0 + t) / a.G, h = u * a.G + (i0 + t) % a.G;
-                    const float *gr = go + ((b * a.Lq + i) * a.Hq + h) * D, *orow = o + ((b * a.Lq + i) * a.Hq + h) * D;
-                    const float p = expf(a.scale * dot_row(ks, q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2], D) - lse[(b * a.Hq + h) * a.Lq + i]);
-                    ps[t] = p;
-                    ds[t] = p * (dot_row(vs, gr, D) - dot_row(gr, orow, D)) * a.scale;
+// gq: a wave holds 32 rows of queries as columns, as the forward does, and goes over the tiles of keys: s^T = k q^T and
+// dp^T = v go^T, then gq^T += k^T ds^T.
+template <int DP, int STAGES, int OCC>
+__global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
+    constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, STAGE = 3 * TB;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const AttnArgs &a = f.a;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const uint32_t lds = lds_address(smem);
+    for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
+        const int64_t unit = xcd_unit(w, f.units);
+        const int qg = (int)(unit % f.groups);
+        const int64_t rest = unit / f.groups;
+        const int split = (int)(rest % f.splits);
+        const int64_t pair = rest / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int64_t n = keys_of(a.Lk, f.key_len, b), nt = (n + kTile - 1) / kTile;
+        const int64_t t0 = nt * split / f.splits, t1 = nt * (split + 1) / f.splits;
+        const int64_t qt = (int64_t)qg * kAttnWaves + wave, R = qt * kTile + (lane & 31);
+        const bool mine = qt < f.qtiles;
+        const int64_t k0 = pair * f.ktiles;
+        auto copy = [&](int64_t t, int buf) {
+            const uint32_t at = __builtin_amdgcn_readfirstlane(lds + buf * STAGE);
+            const int64_t x = (k0 + t) * TB;
+            stage_copy(f.kr + x, at, TB / 1024);
+            stage_copy(f.vr + x, at + TB, TB / 1024);
+            stage_copy(f.kt + x, at + 2 * TB, TB / 1024);
+        };
+        __syncthreads();  // the last unit's stages have been read
+        if (STAGES == 2 && t0 < t1) copy(t0, 0);
+        const int64_t tile = pair * f.qtiles + (mine ? qt : 0);
+        const h8 *qf = (const h8 *)(f.qr + tile * TB) + lane, *gf = (const h8 *)(f.gr + tile * TB) + lane;
+        h8 qh[KS], ql[KS], gh[KS], gl[KS];
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            qh[s] = qf[64 * s], ql[s] = qf[64 * s + 4 * DP];
+            gh[s] = gf[64 * s], gl[s] = gf[64 * s + 4 * DP];
+        }
+        const float cq = pow2i((int)f.qx[tile]) * a.scale * kLog2e, cg = pow2i((int)f.gx[tile]);
+        const float ls = f.stats[tile * 64 + (lane & 31)], de = f.stats[tile * 64 + 32 + (lane & 31)];
+        f16x dq[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) dq[t][r] = 0.0f;
+        float F = 0x1p100f;
+        for (int64_t t = t0, buf = 0; t < t1; t++) {
+            if constexpr (STAGES == 1) {
+                __syncthreads();  // the last tile has been read
+                copy(t, 0);
+            }
+            stage_wait();
+            if (STAGES == 2 && t + 1 < t1) copy(t + 1, (int)buf ^ 1);
+            const char *st = smem + buf * STAGE;
+            if (STAGES == 2) buf ^= 1;
+            if (!mine) continue;
+            const h8 *kf = (const h8 *)st + lane, *vf = (const h8 *)(st + TB) + lane, *ktf = (const h8 *)(st + 2 * TB) + lane;
+            f16x s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) s = mfma3(kf[64 * k], kf[64 * k + 4 * DP], qh[k], ql[k], s);
+#pragma unroll
+            for (int k = 0; k < KS; k++) dp = mfma3(vf[64 * k], vf[64 * k + 4 * DP], gh[k], gl[k], dp);
+            const float ek = f.kx[k0 + t];
+            const float c = cq * pow2i((int)ek), c2 = cg * pow2i((int)f.vx[k0 + t]);
+            const int64_t left = n - t * kTile;
+            float most = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                float p = __builtin_amdgcn_exp2f(fma_(s[r], c, -ls));
+                if (left < kTile && 8 * (r / 4) + 4 * half + r % 4 >= left) p = 0.0f;
+                dp[r] = p * fma_(dp[r], c2, -de);
+                most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
+            }
+            const float kap = pow2i((int)ek);
+            float by;
+            if (column_scale(halves_max(most) * kap, F, by)) scale_acc(dq, by);
+            const float kF = kap * F;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) z[e] = dp[8 * k + e] * kF;
+                const Split8 ds = split8(z);
+#pragma unroll
+                for (int d = 0; d < NT; d++) {
+                    const int at = 64 * (k * NT + d);
+                    dq[d] = mfma3(ktf[at], ktf[at + 4 * DP], ds.hi, ds.lo, dq[d]);
                 }
-                __syncthreads();
-                if (t < D)
-                    for (int x = 0; x < c; x++) {
-                        const int64_t i = (i0 + x) / a.G, h = u * a.G + (i0 + x) % a.G;
-                        sv = fma_(ps[x], go[((b * a.Lq + i) * a.Hq + h) * D + t], sv);
-                        sk = fma_(ds[x], q[b * a.sq[0] + i * a.sq[1] + h * a.sq[2] + t], sk);
-                    }
             }
         }
-        if (t < D) {
-            if (gk) gk[r * D + t] = (acc_k ? gk[r * D + t] : 0.0f) + sk;
-            if (gv) gv[r * D + t] = (acc_v ? gv[r * D + t] : 0.0f) + sv;
+        if (R < f.rows) {
+            const int64_t i = R / a.G, h = u * a.G + (R - i * a.G);
+            store_column(f.gq + split * f.part_q + ((b * a.Lq + i) * a.Hq + h) * a.D, dq, t0 < t1 ? a.scale / F : 0.0f, half, (int)a.D, f.acc_q);
         }
+    }
+}
+
+// out (+)= the splits' parts, in order
+__global__ __launch_bounds__(kAttnB) void k_attn_sum(int64_t n, int splits, const float *part, float *out, int acc) {
+    for (int64_t i = (int64_t)blockIdx.x * kAttnB + threadIdx.x; i < n; i += (int64_t)gridDim.x * kAttnB) {
+        float s = part[i];
+        for (int k = 1; k < splits; k++) s += part[k * n + i];
+        out[i] = acc ? out[i] + s : s;
     }
 }
 
@@ -450,8 +652,6 @@ static int attn_args(const char *what, AttnArgs &a, int64_t B, int64_t Lq, int64
     a = {B, Lq, Lk, Hq, Hkv, D, Hq / Hkv, {sq[0], sq[1], sq[2]}, {sk[0], sk[1], sk[2]}, {sv[0], sv[1], sv[2]}, scale};
     return NC_HIP_OK;
 }
-
-static unsigned row_grid(int64_t rows) { return (unsigned)(rows < (1 << 20) ? rows : (1 << 20)); }
 
 }  // namespace nchip
 
@@ -554,8 +754,8 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     if (Lk) {
         PackArgs pk{};
         pk.Lk = Lk, pk.Hkv = Hkv, pk.D = (int)D, pk.key_len = key_len, pk.jobs = 2;
-        pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, 1, w + p.kr, nullptr, (float *)(w + p.kx), 0};
-        pk.job[1] = {v, sv[0], sv[1], sv[2], Lk, p.tiles, 1, 1, nullptr, w + p.vt, (float *)(w + p.vx), 0};
+        pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, 1, w + p.kr, nullptr, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
+        pk.job[1] = {v, sv[0], sv[1], sv[2], Lk, p.tiles, 1, 1, nullptr, w + p.vt, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
         pack_launch(pk, p.pairs, p.DP, st);
     }
     FwdArgs f{a, q, w + p.kr, w + p.vt, (float *)(w + p.kx), (float *)(w + p.vx), key_len, o, lse, (float *)(w + p.po), (f2 *)(w + p.pm),
@@ -569,10 +769,61 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     return check_launch(what);
 }
 
+namespace nchip {
+
+struct BwdPlan {
+    int DP, qgroups, kgroups, qsplits, ksplits;  // splits of the keys for gq, of the queries for gk and gv
+    int64_t rows, qtiles, ktiles, pairs, nq, nk;
+    size_t kr, kt, vr, qr, qt, gr, gt, kx, vx, qx, gx, stats, pq, pk, pv, total;
+};
+
+// parts so that there are `want` workgroups, of at least four tiles each
+static int attn_splits(int64_t whole, int64_t tiles, int64_t want) {
+    int64_t s = whole ? want / whole : 1;
+    if (s > tiles / 4) s = tiles / 4;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D) {
+    BwdPlan p{};
+    p.DP = padded(D);
+    p.rows = Hq / Hkv * Lq;
+    p.pairs = B * Hkv;
+    p.qtiles = (p.rows + kTile - 1) / kTile;
+    p.ktiles = (Lk + kTile - 1) / kTile;
+    p.qgroups = (int)((p.qtiles + kAttnWaves - 1) / kAttnWaves);
+    p.kgroups = (int)((p.ktiles + kAttnWaves - 1) / kAttnWaves);
+    const int64_t want = kPlanCUs * (p.DP <= 64 ? 2 : 1);
+    p.qsplits = attn_splits(p.pairs * p.qgroups, p.ktiles, want);
+    p.ksplits = attn_splits(p.pairs * p.kgroups, p.qtiles, want);
+    p.nq = B * Lq * Hq * D;
+    p.nk = B * Lk * Hkv * D;
+    size_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const size_t here = at;
+        at += up256((size_t)bytes);
+        return here;
+    };
+    const int64_t q = p.pairs * p.qtiles, k = p.pairs * p.ktiles, tb = tile_bytes(p.DP);
+    p.kr = take(k * tb), p.kt = take(k * tb), p.vr = take(k * tb);
+    p.qr = take(q * tb), p.qt = take(q * tb), p.gr = take(q * tb), p.gt = take(q * tb);
+    p.kx = take(k * 4), p.vx = take(k * 4), p.qx = take(q * 4), p.gx = take(q * 4), p.stats = take(q * 256);
+    if (p.qsplits > 1) p.pq = take(p.qsplits * p.nq * 4);
+    if (p.ksplits > 1) p.pk = take(p.ksplits * p.nk * 4), p.pv = take(p.ksplits * p.nk * 4);
+    p.total = at;
+    return p;
+}
+
+static void sum_launch(int64_t n, int splits, const float *part, float *out, int acc, hipStream_t st) {
+    hipLaunchKernelGGL(k_attn_sum, dim3(attn_grid((n + kAttnB - 1) / kAttnB)), dim3(kAttnB), 0, st, n, splits, part, out, acc);
+}
+
+}  // namespace nchip
+
 extern "C" NC_HIP_API size_t nc_hip_cross_attention_bwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv,
                                                                   int64_t D) {
-    (void)B, (void)Lq, (void)Lk, (void)Hq, (void)Hkv, (void)D;
-    return 0;
+    if (B <= 0 || Lq < 0 || Lk < 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
+    return bwd_plan(B, Lq, Lk, Hq, Hkv, D).total;
 }
 
 extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D,
@@ -587,10 +838,54 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
     if (B == 0) return NC_HIP_OK;
     if ((Lq && (!q || !o || !lse || !go)) || (Lk && (!k || !v)))
         return set_error(NC_HIP_ERR_ARG, "%s: q, k, v, o, lse and go are needed", what);
-    (void)ws, (void)ws_bytes;
+    const bool want_q = gq && Lq, want_k = (gk || gv) && Lk;
+    if (!want_q && !want_k) return NC_HIP_OK;
+    const BwdPlan p = bwd_plan(B, Lq, Lk, Hq, Hkv, D);
+    if (p.total && (!ws || ws_bytes < p.total))
+        return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, p.total);
     hipStream_t st = as_stream(stream);
-    if (gq && Lq) hipLaunchKernelGGL(k_attn_dq_row, dim3(row_grid(B * Lq * Hq)), kAttnB, 0, st, a, q, k, v, key_len, o, lse, go, gq, acc_q);
-    if ((gk || gv) && Lk)
-        hipLaunchKernelGGL(k_attn_dkv_row, dim3(row_grid(B * Lk * Hkv)), kAttnB, 0, st, a, q, k, v, key_len, o, lse, go, gk, gv, acc_k, acc_v);
+    char *const w = (char *)ws;
+    BwdArgs f{};
+    f.a = a;
+    f.kr = w + p.kr, f.kt = w + p.kt, f.vr = w + p.vr, f.qr = w + p.qr, f.qt = w + p.qt, f.gr = w + p.gr, f.gt = w + p.gt;
+    f.kx = (float *)(w + p.kx), f.vx = (float *)(w + p.vx), f.qx = (float *)(w + p.qx), f.gx = (float *)(w + p.gx);
+    f.stats = (float *)(w + p.stats);
+    f.key_len = key_len;
+    f.rows = p.rows, f.qtiles = p.qtiles, f.ktiles = p.ktiles;
+    PackArgs pk{};
+    pk.Lk = Lk, pk.Hkv = Hkv, pk.D = (int)D, pk.key_len = key_len;
+    const int64_t G = a.G;
+    if (Lk) {
+        pk.job[pk.jobs++] = {k, sk[0], sk[1], sk[2], Lk, p.ktiles, 1, 1, w + p.kr, want_q ? w + p.kt : nullptr, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {v, sv[0], sv[1], sv[2], Lk, p.ktiles, 1, 1, w + p.vr, nullptr, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
+    }
+    if (Lq) {
+        pk.job[pk.jobs++] = {q, sq[0], sq[1], sq[2], p.rows, p.qtiles, (int)G, 0, w + p.qr, want_k ? w + p.qt : nullptr, (float *)(w + p.qx), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {go, Lq * Hq * D, Hq * D, D, p.rows, p.qtiles, (int)G, 0, w + p.gr, want_k ? w + p.gt : nullptr, (float *)(w + p.gx), 0, o, lse, (float *)(w + p.stats)};
+    }
+    pack_launch(pk, p.pairs, p.DP, st);
+    if (want_q) {
+        const bool cut = p.qsplits > 1;
+        f.gq = cut ? (float *)(w + p.pq) : gq;
+        f.acc_q = cut ? 0 : acc_q;
+        f.part_q = p.nq, f.groups = p.qgroups, f.splits = p.qsplits;
+        f.units = p.pairs * p.qgroups * p.qsplits;
+        NC_ATTN_DP(p.DP, constexpr int STAGES = DP <= 128 ? 2 : 1; constexpr int OCC = DP <= 64 ? 2 : 1;
+                   attn_launch(&k_attn_dq<DP, STAGES, OCC>, f.units, STAGES * 3 * 128 * DP, st, f));
+        if (cut) sum_launch(p.nq, p.qsplits, f.gq, gq, acc_q, st);
+    }
+    if (want_k) {
+        const bool cut = p.ksplits > 1;
+        f.gk = cut && gk ? (float *)(w + p.pk) : gk;
+        f.gv = cut && gv ? (float *)(w + p.pv) : gv;
+        f.acc_k = cut ? 0 : acc_k;
+        f.acc_v = cut ? 0 : acc_v;
+        f.part_k = p.nk, f.groups = p.kgroups, f.splits = p.ksplits;
+        f.units = p.pairs * p.kgroups * p.ksplits;
+        NC_ATTN_DP(p.DP, constexpr int STAGES = DP <= 128 ? 2 : 1; constexpr int OCC = DP <= 64 ? 2 : 1;
+                   attn_launch(&k_attn_dkv<DP, STAGES, OCC>, f.units, STAGES * (4 * 128 * DP + 256), st, f));
+        if (cut && gk) sum_launch(p.nk, p.ksplits, f.gk, gk, acc_k, st);
+        if (cut && gv) sum_launch(p.nk, p.ksplits, f.gv, gv, acc_v, st);
+    }
     return check_launch(what);
 }

@@ -83,7 +83,10 @@ __device__ __forceinline__ void load8(const float *row, int d, int D, float *x) 
         *(f4u *)(x + 4) = *(const f4u *)(row + d + 4);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = d + i < D ? row[d + i] : 0.0f;
+        for (int i = 0; i < 8; i++) {
+            const float v = row[d + i < D ? d + i : D - 1];
+            x[i] = d + i < D ? v : 0.0f;
+        }
     }
 }
 
