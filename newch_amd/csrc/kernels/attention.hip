@@ -337,33 +337,206 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
     }
 }
 
-// the splits' parts of a row joined: its reference is the largest, parts count by 2^(reference - largest)
+// ------------------------------------------------------------------------------------------------
+// forward of a few rows: single tokens against long caches
+// ------------------------------------------------------------------------------------------------
+// Bound by reading keys and values once.  LPK lanes hold a key's columns, two 16-byte pieces each, for NR rows of queries at once
+// (the query heads that share the keys); each group of LPK lanes keeps its own running maximum, sum and o over the keys that it
+// sees, U of them in flight, and the groups, waves and parts are joined at the end.  All in fp32 on the vector unit: 8 rows of
+// 128 columns still take less time than the keys' way from memory.
+template <int LPK>
+__device__ __forceinline__ float lanes_sum(float v) {  // over LPK neighbours
+    v += dpp_f32<kDppXor1>(v, 0.0f);
+    v += dpp_f32<kDppXor2>(v, 0.0f);
+    if constexpr (LPK >= 8) v += dpp_f32<kDppHalfMirror>(v, 0.0f);
+    if constexpr (LPK >= 16) v += dpp_f32<kDppMirror>(v, 0.0f);
+    if constexpr (LPK >= 32) v += __shfl_xor(v, 16);
+    return v;
+}
+
+// piece c of a row: four columns, from the row's first where the piece lies past its end; D4: no piece is cut short
+template <bool D4>
+__device__ __forceinline__ f4 row_piece(const float *row, int c, int D) {
+    if constexpr (D4) {
+        return *(const f4u *)(row + (4 * c < D ? 4 * c : 0));
+    } else {
+        f4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = row[4 * c + e < D ? 4 * c + e : 0];
+        return v;
+    }
+}
+
+template <int NR, int LPK, int U, bool D4>
+__global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const float *k, const float *v) {
+    constexpr int NG = kWave / LPK, KEYS = kAttnWaves * U * NG;  // groups of a wave; keys of a round
+    __shared__ float part[kAttnWaves][NR][8 * LPK];
+    __shared__ f2 ml[kAttnWaves][NR];
+    const AttnArgs &a = f.a;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane % LPK, grp = lane / LPK, D = (int)a.D;
+    for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
+        const int split = (int)(w % f.splits);
+        const int64_t pair = w / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int64_t n = keys_of(a.Lk, f.key_len, b), nt = (n + kTile - 1) / kTile;
+        const int64_t j0 = nt * split / f.splits * kTile, j1 = min(n, nt * (split + 1) / f.splits * kTile);
+        const float *kb = k + b * a.sk[0] + u * a.sk[2], *vb = v + b * a.sv[0] + u * a.sv[2];
+        f4 q[NR][2], o[NR][2];
+        float m[NR], l[NR];
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            const int64_t R = r < f.rows ? r : 0, i = R / a.G, h = u * a.G + (R - i * a.G);
+            const float *row = f.q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                q[r][x] = row_piece<D4>(row, ln + x * LPK, D) * (a.scale * kLog2e);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (4 * (ln + x * LPK) + e >= D) q[r][x][e] = 0.0f;
+                o[r][x] = f4{0.f, 0.f, 0.f, 0.f};
+            }
+            m[r] = -INFINITY, l[r] = 0.0f;
+        }
+        for (int64_t j = j0; j < j1; j += KEYS) {
+            f4 kk[U][2], vv[U][2];
+#pragma unroll
+            for (int x = 0; x < U; x++) {
+                const int64_t key = min(j + (wave * U + x) * NG + grp, j1 - 1);
+                const float *kr = kb + key * a.sk[1], *vr = vb + key * a.sv[1];
+#pragma unroll
+                for (int y = 0; y < 2; y++) kk[x][y] = row_piece<D4>(kr, ln + y * LPK, D), vv[x][y] = row_piece<D4>(vr, ln + y * LPK, D);
+            }
+            float s[NR][U];
+#pragma unroll
+            for (int x = 0; x < U; x++) {
+                const bool in = j + (wave * U + x) * NG + grp < j1;
+#pragma unroll
+                for (int r = 0; r < NR; r++) {
+                    float t = 0.0f;
+#pragma unroll
+                    for (int y = 0; y < 2; y++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) t = fma_(q[r][y][e], kk[x][y][e], t);
+                    t = lanes_sum<LPK>(t);
+                    s[r][x] = in ? t : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                float top = m[r];
+#pragma unroll
+                for (int x = 0; x < U; x++) top = __builtin_fmaxf(top, s[r][x]);
+                // no key yet: the reference stays, and every p is 0
+                const float ref = top == -INFINITY ? 0.0f : top, al = __builtin_amdgcn_exp2f(m[r] - ref);
+                m[r] = top;
+                l[r] *= al;
+                o[r][0] *= al;
+                o[r][1] *= al;
+#pragma unroll
+                for (int x = 0; x < U; x++) {
+                    const float p = __builtin_amdgcn_exp2f(s[r][x] - ref);
+                    l[r] += p;
+#pragma unroll
+                    for (int y = 0; y < 2; y++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[r][y][e] = fma_(p, vv[x][y][e], o[r][y][e]);
+                }
+            }
+        }
+        // the wave's groups, then the waves
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            float top = m[r];
+#pragma unroll
+            for (int x = LPK; x < kWave; x *= 2) {
+                const float t = __shfl_xor(top, x);
+                top = top >= t || top != top ? top : t;  // a NaN stays
+            }
+            const float al = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - top);
+            l[r] *= al;
+            o[r][0] *= al;
+            o[r][1] *= al;
+#pragma unroll
+            for (int x = LPK; x < kWave; x *= 2) {
+                l[r] += __shfl_xor(l[r], x);
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[r][y][e] += __shfl_xor(o[r][y][e], x);
+            }
+            m[r] = top;
+        }
+        __syncthreads();  // the last unit's parts have been read
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            if (grp == 0) {
+                *(f4 *)&part[wave][r][4 * ln] = o[r][0];
+                *(f4 *)&part[wave][r][4 * (ln + LPK)] = o[r][1];
+            }
+            if (lane == 0) ml[wave][r] = f2{m[r], l[r]};
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < NR * 8 * LPK; x += kAttnB) {
+            const int r = x / (8 * LPK), d = x - r * 8 * LPK;
+            if (r >= f.rows || d >= D) continue;
+            float top = -INFINITY;
+#pragma unroll
+            for (int y = 0; y < kAttnWaves; y++) {
+                const float t = ml[y][r].x;
+                top = top >= t || top != top ? top : t;
+            }
+            float sum = 0.0f, total = 0.0f;
+#pragma unroll
+            for (int y = 0; y < kAttnWaves; y++) {
+                const f2 t = ml[y][r];
+                const float al = t.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(t.x - top);
+                sum = fma_(al, part[y][r][d], sum);
+                total = fma_(al, t.y, total);
+            }
+            if (f.splits == 1) {
+                const int64_t i = r / a.G, h = u * a.G + (r - i * a.G);
+                f.o[((b * a.Lq + i) * a.Hq + h) * a.D + d] = total != 0.0f ? sum / total : 0.0f;
+                if (f.lse && d == 0) f.lse[(b * a.Hq + h) * a.Lq + i] = n ? fma_(top, kLn2, logf(total)) : -INFINITY;
+            } else {
+                const int64_t pr = ((int64_t)split * a.B * a.Hkv + pair) * f.rows + r;
+                f.po[pr * D + d] = sum;
+                if (d == 0) f.pm[pr] = f2{top, total};
+            }
+        }
+    }
+}
+
+// The splits' parts of a row joined: a part counts by 2^(its reference - the largest).  A wave a row: lane s has part s's
+// reference and sum, then every lane 64th column.
 __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t rows, int splits, const float *po, const f2 *pm,
                                                       float *o, float *lse) {
-    const int64_t all = a.B * a.Hkv * rows, D4 = (a.D + 3) / 4;
-    for (int64_t x = (int64_t)blockIdx.x * kAttnB + threadIdx.x; x < all * D4; x += (int64_t)gridDim.x * kAttnB) {
-        const int64_t pr = x / D4, pair = pr / rows, R = pr - pair * rows, b = pair / a.Hkv, u = pair - b * a.Hkv;
-        const int d = (int)(x - pr * D4) * 4;
+    const int64_t all = a.B * a.Hkv * rows;
+    const int lane = threadIdx.x & 63;
+    for (int64_t pr = (int64_t)blockIdx.x * kAttnWaves + (threadIdx.x >> 6); pr < all; pr += (int64_t)gridDim.x * kAttnWaves) {
+        const int64_t pair = pr / rows, R = pr - pair * rows, b = pair / a.Hkv, u = pair - b * a.Hkv;
         const int64_t i = R / a.G, h = u * a.G + (R - i * a.G);
-        float M = -INFINITY;
-        for (int s = 0; s < splits; s++) {
-            const float m = pm[s * all + pr].x;
-            M = M >= m || M != M ? M : m;  // a NaN part stays
+        const f2 ml = lane < splits ? pm[lane * all + pr] : f2{-INFINITY, 0.0f};
+        const bool nan = __any(ml.x != ml.x);
+        const float M = wave_max_nan_skip(ml.x);
+        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+        const float l = wave_sum(w * ml.y);
+        const float wn = nan ? NAN : l != 0.0f ? w / l : 0.0f;
+        for (int64_t d0 = 0; d0 < a.D; d0 += kWave) {
+            const int64_t d = d0 + lane;
+            const float *p = po + pr * a.D + (d < a.D ? d : 0);
+            float sum = 0.0f;
+            for (int s0 = 0; s0 < splits; s0 += 8) {
+                float x[8];
+#pragma unroll
+                for (int s = 0; s < 8; s++) x[s] = p[min(s0 + s, splits - 1) * all * a.D];
+#pragma unroll
+                for (int s = 0; s < 8; s++) {  // a lane past the parts has weight 0; parts without keys hold nothing that counts
+                    const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wn), s0 + s));
+                    sum = ws != 0.0f ? fma_(ws, x[s], sum) : sum;
+                }
+            }
+            if (d < a.D) o[((b * a.Lq + i) * a.Hq + h) * a.D + d] = sum;
         }
-        f4 sum = {0.f, 0.f, 0.f, 0.f};
-        float l = 0.0f;
-        for (int s = 0; s < splits; s++) {
-            const f2 ml = pm[s * all + pr];
-            if (ml.x == -INFINITY) continue;
-            const float w = __builtin_amdgcn_exp2f(ml.x - M);
-            const float *p = po + (s * all + pr) * a.D + d;
-            l = fma_(w, ml.y, l);
-            for (int e = 0; e < 4; e++)
-                if (d + e < a.D) sum[e] = fma_(w, p[e], sum[e]);
-        }
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        store4(o + ((b * a.Lq + i) * a.Hq + h) * a.D, d, (int)a.D, sum * inv, 0);
-        if (lse && d == 0) lse[(b * a.Hq + h) * a.Lq + i] = M == -INFINITY ? -INFINITY : fma_(M, kLn2, logf(l));
+        if (lse && lane == 0) lse[(b * a.Hq + h) * a.Lq + i] = M == -INFINITY ? -INFINITY : fma_(M, kLn2, logf(l));
     }
 }
 
@@ -672,7 +845,17 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
         else { constexpr int DP = 256; __VA_ARGS__; }                   \
     } while (0)
 
+// parts so that there are `want` workgroups, of at least four tiles each, 64 parts at most
+static int attn_splits(int64_t whole, int64_t tiles, int64_t want) {
+    int64_t s = whole ? want / whole : 1;
+    if (s > tiles / 4) s = tiles / 4;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+constexpr int64_t kTokenRows = 8;  // rows of a pair that k_attn_token takes
+
 struct FwdPlan {
+    bool token;
     int DP, qtiles, splits;
     int64_t rows, tiles, pairs, units;
     size_t kr, vt, kx, vx, po, pm, total;  // offsets into the workspace
@@ -685,11 +868,10 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
     p.pairs = B * Hkv;
     p.tiles = (Lk + kTile - 1) / kTile;
     p.qtiles = (int)((p.rows + kAttnWaves * kTile - 1) / (kAttnWaves * kTile));
-    // keys are cut where there are fewer than two workgroups a CU, into parts of at least four tiles
+    p.token = p.rows <= kTokenRows;
+    if (p.token) p.qtiles = 1;
     const int64_t whole = p.pairs * p.qtiles;
-    int64_t splits = whole ? 2 * kPlanCUs / whole : 1;
-    if (splits > p.tiles / 4) splits = p.tiles / 4;
-    p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+    p.splits = attn_splits(whole, p.tiles, (p.token ? 8 : 2) * kPlanCUs);
     p.units = whole * p.splits;
     const size_t pt = (size_t)(p.pairs * p.tiles);
     size_t at = 0;
@@ -698,10 +880,12 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
         at += up256(bytes);
         return here;
     };
-    p.kr = take(pt * tile_bytes(p.DP));
-    p.vt = take(pt * tile_bytes(p.DP));
-    p.kx = take(pt * 4);
-    p.vx = take(pt * 4);
+    if (!p.token) {
+        p.kr = take(pt * tile_bytes(p.DP));
+        p.vt = take(pt * tile_bytes(p.DP));
+        p.kx = take(pt * 4);
+        p.vx = take(pt * 4);
+    }
     if (p.splits > 1) {
         p.po = take((size_t)p.splits * p.pairs * p.rows * D * 4);
         p.pm = take((size_t)p.splits * p.pairs * p.rows * 8);
@@ -716,6 +900,26 @@ template <class F, class A>
 static void attn_launch(F *kernel, int64_t units, size_t lds, hipStream_t st, const A &args) {
     if (lds > 65536) (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     hipLaunchKernelGGL(kernel, dim3(attn_grid(units)), dim3(kAttnB), lds, st, args);
+}
+
+template <int NR, int LPK>
+static void token_launch2(const FwdArgs &f, const float *k, const float *v, hipStream_t st) {
+    constexpr int U = NR <= 4 ? 4 : 2;
+    if (f.a.D % 4 == 0) hipLaunchKernelGGL((k_attn_token<NR, LPK, U, true>), dim3(attn_grid(f.units)), dim3(kAttnB), 0, st, f, k, v);
+    else hipLaunchKernelGGL((k_attn_token<NR, LPK, U, false>), dim3(attn_grid(f.units)), dim3(kAttnB), 0, st, f, k, v);
+}
+template <int NR>
+static void token_launch1(const FwdArgs &f, const float *k, const float *v, hipStream_t st) {
+    if (f.a.D <= 32) token_launch2<NR, 4>(f, k, v, st);
+    else if (f.a.D <= 64) token_launch2<NR, 8>(f, k, v, st);
+    else if (f.a.D <= 128) token_launch2<NR, 16>(f, k, v, st);
+    else token_launch2<NR, 32>(f, k, v, st);
+}
+static void token_launch(const FwdArgs &f, const float *k, const float *v, hipStream_t st) {
+    if (f.rows == 1) token_launch1<1>(f, k, v, st);
+    else if (f.rows == 2) token_launch1<2>(f, k, v, st);
+    else if (f.rows <= 4) token_launch1<4>(f, k, v, st);
+    else token_launch1<8>(f, k, v, st);
 }
 
 static void pack_launch(PackArgs &p, int64_t pairs, int DP, hipStream_t st) {
@@ -751,7 +955,7 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
         return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, p.total);
     hipStream_t st = as_stream(stream);
     char *const w = (char *)ws;
-    if (Lk) {
+    if (Lk && !p.token) {
         PackArgs pk{};
         pk.Lk = Lk, pk.Hkv = Hkv, pk.D = (int)D, pk.key_len = key_len, pk.jobs = 2;
         pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, 1, w + p.kr, nullptr, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
@@ -760,12 +964,13 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     }
     FwdArgs f{a, q, w + p.kr, w + p.vt, (float *)(w + p.kx), (float *)(w + p.vx), key_len, o, lse, (float *)(w + p.po), (f2 *)(w + p.pm),
               p.rows, p.tiles, p.units, p.qtiles, p.splits};
-    NC_ATTN_DP(p.DP, constexpr int TPS = DP <= 64 ? 2 : 1; constexpr int OCC = DP <= 128 ? 2 : 1;
-               attn_launch(&k_attn_fwd<DP, TPS, OCC>, p.units, 2 * 2 * TPS * 128 * DP, st, f));
-    if (p.splits > 1) {
-        const int64_t items = p.pairs * p.rows * ((D + 3) / 4);
-        hipLaunchKernelGGL(k_attn_join, dim3(attn_grid((items + kAttnB - 1) / kAttnB)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, o, lse);
-    }
+    if (p.token)
+        token_launch(f, k, v, st);
+    else
+        NC_ATTN_DP(p.DP, constexpr int TPS = DP <= 64 ? 2 : 1; constexpr int OCC = DP <= 128 ? 2 : 1;
+                   attn_launch(&k_attn_fwd<DP, TPS, OCC>, p.units, 2 * 2 * TPS * 128 * DP, st, f));
+    if (p.splits > 1)
+        hipLaunchKernelGGL(k_attn_join, dim3(attn_grid((p.pairs * p.rows + kAttnWaves - 1) / kAttnWaves)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, o, lse);
     return check_launch(what);
 }
 
@@ -776,13 +981,6 @@ struct BwdPlan {
     int64_t rows, qtiles, ktiles, pairs, nq, nk;
     size_t kr, kt, vr, qr, qt, gr, gt, kx, vx, qx, gx, stats, pq, pk, pv, total;
 };
-
-// parts so that there are `want` workgroups, of at least four tiles each
-static int attn_splits(int64_t whole, int64_t tiles, int64_t want) {
-    int64_t s = whole ? want / whole : 1;
-    if (s > tiles / 4) s = tiles / 4;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-}
 
 static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D) {
     BwdPlan p{};
