@@ -157,6 +157,24 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
 }
 
+// A value that the launch does not write, through the scalar cache: a vector load here would wait behind the next stage's
+// copies, which share its counter.
+__device__ __forceinline__ float scalar_load(const float *p) {
+    return *(const __attribute__((address_space(4))) float *)(uintptr_t)p;
+}
+
+// The order of a block of N steps, each two fragments from LDS and three products: reads two steps ahead of their products.
+template <int N>
+__device__ __forceinline__ void order_steps() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < N - 2; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+}
+
 // Workgroups are dealt round robin over the 8 XCDs: consecutive units of a launch go to one XCD, which then keeps their
 // keys in its L2.
 __device__ __forceinline__ int64_t xcd_unit(int64_t w, int64_t units) {
@@ -193,7 +211,7 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
     constexpr int STAGE = 2 * TPS * TB;          // keys' tiles, then values'
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lds = lds_address(smem);
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
@@ -223,25 +241,24 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
         h8 qh[KS], ql[KS];
         float cq;
         {
-            float x[KS][8], most = 0.0f;
-            const float c = a.scale * kLog2e;
+            const float c = live ? a.scale * kLog2e : 0.0f;
+            float most = 0.0f, x[8];
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                if (live) load8(qrow, 16 * s + 8 * half, (int)a.D, x[s]);
+                load8(qrow, 16 * s + 8 * half, (int)a.D, x);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    x[s][e] = live ? x[s][e] * c : 0.0f;
-                    most = __builtin_fmaxf(most, finite_abs(x[s][e]));
-                }
+                for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[e] * c));
             }
             const int e = tile_exponent(halves_max(most));
             const float inv = pow2i(-e);
             cq = pow2i(e);
+            asm volatile("" ::: "memory");  // the row is read again (from the caches) rather than held in fp32 as well
 #pragma unroll
             for (int s = 0; s < KS; s++) {
+                load8(qrow, 16 * s + 8 * half, (int)a.D, x);
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[s][k] *= inv;
-                const Split8 p = split8(x[s]);
+                for (int k = 0; k < 8; k++) x[k] = live ? x[k] * c * inv : 0.0f;
+                const Split8 p = split8(x);
                 qh[s] = p.hi, ql[s] = p.lo;
             }
         }
@@ -252,6 +269,9 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
             for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
         float m = -INFINITY, l = 0.0f, E = -1000.0f;
         for (int64_t t = t0, buf = 0; t < t1; t += TPS, buf ^= 1) {
+            float ek[TPS], evs[TPS];
+#pragma unroll
+            for (int x = 0; x < TPS; x++) ek[x] = scalar_load(kx + min(t + x, t1 - 1)), evs[x] = scalar_load(vx + min(t + x, t1 - 1));
             stage_wait();
             if (t + TPS < t1) copy(t + TPS, (int)buf ^ 1);
             const char *st = smem + buf * STAGE;
@@ -264,18 +284,19 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
                 for (int r = 0; r < 16; r++) s[r] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < KS; k++) s = mfma3(kf[64 * k], kf[64 * k + 4 * DP], qh[k], ql[k], s);
-                const float c = __builtin_fmaxf(cq * pow2i((int)kx[t + x]), 0x1p-126f);  // -inf * c stays -inf
-                const int64_t left = n - (t + x) * kTile;
-                if (left < kTile) {
+                order_steps<KS>();
+                const float c = __builtin_fmaxf(cq * pow2i((int)ek[x]), 0x1p-126f);  // -inf * c stays -inf
+                const int left = (int)min(n - (t + x) * kTile, (int64_t)kTile) - 4 * half;
+                if (t + x + 1 == nt) {
 #pragma unroll
                     for (int r = 0; r < 16; r++)
-                        if (8 * (r / 4) + 4 * half + r % 4 >= left) s[r] = -INFINITY;
+                        if (8 * (r / 4) + r % 4 >= left) s[r] = -INFINITY;
                 }
                 float top = s[0];
 #pragma unroll
                 for (int r = 1; r < 16; r++) top = __builtin_fmaxf(top, s[r]);
                 top = halves_max(top) * c;
-                const float ev = vx[t + x];
+                const float ev = evs[x];
                 if (__any(top > m + kPSlack) || ev > E) {
                     const float mn = top > m + kPSlack ? top : m, En = __builtin_fmaxf(E, ev);
                     const float al = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -307,6 +328,7 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
                     for (int d = 0; d < NT; d++)
                         o[d] = mfma3(vf[64 * (k * NT + d)], vf[64 * (k * NT + d) + 4 * DP], p.hi, p.lo, o[d]);
                 }
+                order_steps<2 * NT>();
             }
         }
         l = halves_sum(l);
@@ -595,7 +617,7 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
     constexpr bool REG = DP <= 128;  // keys and values stay in registers, else they are read again for every tile
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lds = lds_address(smem);
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
@@ -645,6 +667,7 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                 __syncthreads();  // the last tile has been read
                 copy(t, 0);
             }
+            const float ex = scalar_load(f.gx + q0 + t), eq = scalar_load(f.qx + q0 + t);
             stage_wait();
             if (STAGES == 2 && t + 1 < t1) copy(t + 1, (int)buf ^ 1);
             const char *st = smem + buf * STAGE;
@@ -657,10 +680,11 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < KS; k++) s = mfma3(qf[64 * k], qf[64 * k + 4 * DP], REG ? kh[k] : kf[64 * k], REG ? kl[k] : kf[64 * k + 4 * DP], s);
-#pragma unroll
-            for (int k = 0; k < KS; k++) dp = mfma3(gf[64 * k], gf[64 * k + 4 * DP], REG ? vh[k] : vf[64 * k], REG ? vl[k] : vf[64 * k + 4 * DP], dp);
-            const float ex = f.gx[q0 + t], eq = f.qx[q0 + t];
+            for (int k = 0; k < KS; k++) {
+                s = mfma3(qf[64 * k], qf[64 * k + 4 * DP], REG ? kh[k] : kf[64 * k], REG ? kl[k] : kf[64 * k + 4 * DP], s);
+                dp = mfma3(gf[64 * k], gf[64 * k + 4 * DP], REG ? vh[k] : vf[64 * k], REG ? vl[k] : vf[64 * k + 4 * DP], dp);
+            }
+            if constexpr (REG) order_steps<2 * KS>();
             if (ex > E) {
                 scale_acc(dv, __builtin_amdgcn_exp2f(E - ex));
                 E = ex;
@@ -697,6 +721,7 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                     dk[d] = mfma3(qtf[at], qtf[at + 4 * DP], ds.hi, ds.lo, dk[d]);
                 }
             }
+            order_steps<4 * NT>();
         }
         if (key < a.Lk) {
             const int64_t at = ((b * a.Lk + key) * a.Hkv + u) * a.D;
@@ -714,7 +739,7 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, STAGE = 3 * TB;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lds = lds_address(smem);
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
@@ -757,6 +782,7 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
                 __syncthreads();  // the last tile has been read
                 copy(t, 0);
             }
+            const float ek = scalar_load(f.kx + k0 + t), ev = scalar_load(f.vx + k0 + t);
             stage_wait();
             if (STAGES == 2 && t + 1 < t1) copy(t + 1, (int)buf ^ 1);
             const char *st = smem + buf * STAGE;
@@ -767,17 +793,18 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < KS; k++) s = mfma3(kf[64 * k], kf[64 * k + 4 * DP], qh[k], ql[k], s);
-#pragma unroll
-            for (int k = 0; k < KS; k++) dp = mfma3(vf[64 * k], vf[64 * k + 4 * DP], gh[k], gl[k], dp);
-            const float ek = f.kx[k0 + t];
-            const float c = cq * pow2i((int)ek), c2 = cg * pow2i((int)f.vx[k0 + t]);
-            const int64_t left = n - t * kTile;
+            for (int k = 0; k < KS; k++) {
+                s = mfma3(kf[64 * k], kf[64 * k + 4 * DP], qh[k], ql[k], s);
+                dp = mfma3(vf[64 * k], vf[64 * k + 4 * DP], gh[k], gl[k], dp);
+            }
+            order_steps<2 * KS>();
+            const float c = cq * pow2i((int)ek), c2 = cg * pow2i((int)ev);
+            const int left = (int)min(n - t * kTile, (int64_t)kTile) - 4 * half;
             float most = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 float p = __builtin_amdgcn_exp2f(fma_(s[r], c, -ls));
-                if (left < kTile && 8 * (r / 4) + 4 * half + r % 4 >= left) p = 0.0f;
+                p = 8 * (r / 4) + r % 4 < left ? p : 0.0f;
                 dp[r] = p * fma_(dp[r], c2, -de);
                 most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
             }
@@ -797,6 +824,7 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
                     dq[d] = mfma3(ktf[at], ktf[at + 4 * DP], ds.hi, ds.lo, dq[d]);
                 }
             }
+            order_steps<2 * NT>();
         }
         if (R < f.rows) {
             const int64_t i = R / a.G, h = u * a.G + (R - i * a.G);

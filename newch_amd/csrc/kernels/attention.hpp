@@ -79,8 +79,9 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 // eight columns of a row from d on, zeros from column D on
 __device__ __forceinline__ void load8(const float *row, int d, int D, float *x) {
     if (d + 8 <= D) {
-        *(f4u *)x = *(const f4u *)(row + d);
-        *(f4u *)(x + 4) = *(const f4u *)(row + d + 4);
+        const f4 p = *(const f4u *)(row + d), q = *(const f4u *)(row + d + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = p[i], x[4 + i] = q[i];
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {

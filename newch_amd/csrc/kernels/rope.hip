@@ -10,8 +10,8 @@
 //
 // Both directions are bound by memory (8 and 12 bytes a value).  The cosines and sines of a group of tokens are computed
 // once, into LDS, for all of its heads: angles in turns in fp64 (a position of 2^31 keeps 2^-22 of a turn), reduced to an
-// eighth of a turn exactly and only then rounded to fp32.  A row is held by 8 to 64 lanes, a unit of V pairs a lane: V = 4
-// where every section's columns fall into whole 16-byte pieces, else single pairs.  Lanes keep their unit for all rows, so
+// eighth of a turn exactly and only then rounded to fp32.  A row is held by 8 to 32 lanes, units of V pairs a lane: V = 4
+// where every section's columns fall into whole 16-byte pieces, else up to 8 single pairs.  Lanes keep their unit for all rows, so
 // that the weights and the weights' gradients stay in registers.
 #include "common.hpp"
 #include "intdiv.hpp"
@@ -47,7 +47,6 @@ __device__ __forceinline__ float group_sum(float v) {
     v += dpp_f32<kDppHalfMirror>(v, 0.0f);
     if constexpr (LPR >= 16) v += dpp_f32<kDppMirror>(v, 0.0f);
     if constexpr (LPR >= 32) v += __shfl_xor(v, 16);
-    if constexpr (LPR >= 64) v += __shfl_xor(v, 32);
     return v;
 }
 
@@ -82,8 +81,11 @@ __device__ __forceinline__ void rope_get(const float *row, const RopeUnit &u, fl
 #pragma unroll
     for (int i = 0; i < 2 * V; i++) e[i] = 0.0f;
     if constexpr (V == 4) {
-        if (u.c1 >= 0) *(f4u *)e = *(const f4u *)(row + u.c1);
-        if (u.c2 >= 0) *(f4u *)(e + 4) = *(const f4u *)(row + u.c2);
+        f4 p = {0.f, 0.f, 0.f, 0.f}, q = p;
+        if (u.c1 >= 0) p = *(const f4u *)(row + u.c1);
+        if (u.c2 >= 0) q = *(const f4u *)(row + u.c2);
+#pragma unroll
+        for (int i = 0; i < 4; i++) e[i] = p[i], e[4 + i] = q[i];
     } else {
         if (u.c1 >= 0) e[0] = row[u.c1];
         if (u.c2 >= 0) e[1] = row[u.c2];
@@ -102,8 +104,8 @@ __device__ __forceinline__ void rope_put(float *row, const RopeUnit &u, const fl
         for (int i = 0; i < 2 * V; i++) o[i] = e[i];
     }
     if constexpr (V == 4) {
-        if (u.c1 >= 0) *(f4u *)(row + u.c1) = *(const f4u *)o;
-        if (u.c2 >= 0) *(f4u *)(row + u.c2) = *(const f4u *)(o + 4);
+        if (u.c1 >= 0) *(f4u *)(row + u.c1) = f4{o[0], o[1], o[2], o[3]};
+        if (u.c2 >= 0) *(f4u *)(row + u.c2) = f4{o[4], o[5], o[6], o[7]};
     } else {
         if (u.c1 >= 0) row[u.c1] = o[0];
         if (u.c2 >= 0) row[u.c2] = o[1];
@@ -114,17 +116,22 @@ __device__ __forceinline__ void rope_put(float *row, const RopeUnit &u, const fl
 template <int V>
 __device__ __forceinline__ void rope_turn(float *e, const float2 *cs, const RopeUnit &u, int inter, float sign) {
     if (u.pair < 0) return;
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        const float2 t = cs[u.pair + i];
-        const float c = t.x, s = sign * t.y;
-        // element i of the first half with i of the second, or neighbours
-        float &p = inter ? e[2 * i] : e[i], &q = inter ? e[2 * i + 1] : e[V + i];
-        const float a = p, b = q;
+    auto turn = [&](float2 t, float &p, float &q) {
+        const float c = t.x, s = sign * t.y, a = p, b = q;
         p = fma_(a, c, -(b * s));
         q = fma_(b, c, a * s);
+    };
+    if (inter) {
+#pragma unroll
+        for (int i = 0; i < V; i++) turn(cs[u.pair + i], e[2 * i], e[2 * i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) turn(cs[u.pair + i], e[i], e[V + i]);
     }
 }
+
+// rows in flight: about 64 bytes of each tensor a lane
+constexpr int rope_rows(int mode, int v, int upl) { return (mode == 2 ? 2 : 4) / (v == 1 && upl > 4 ? 2 : 1); }
 
 // MODE 0: rotation of x (sign 1) or of gy back (sign -1); 1: norm and rotation; 2: their gradient
 template <int V, int LPR, int UPL, int MODE>
@@ -133,6 +140,7 @@ __global__ __launch_bounds__(kRopeB) void k_rope(const RopeArgs a, const float *
                                                  const int *__restrict__ pos, const float *__restrict__ gy,
                                                  float *__restrict__ y, double *__restrict__ part, float sign) {
     constexpr int slots = kRopeB / LPR;
+    constexpr int U = rope_rows(MODE, V, UPL);  // rows a slot holds at once
     __shared__ float2 table[kRopeTable];
     __shared__ float red[MODE == 2 ? kRopeB * 2 * V : 1];
     const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
@@ -157,87 +165,100 @@ __global__ __launch_bounds__(kRopeB) void k_rope(const RopeArgs a, const float *
         const int n = (int)min((int64_t)a.group, a.tokens - t0);
         const int64_t b0 = t0 / a.L;
         const uint32_t l0 = (uint32_t)(t0 - b0 * a.L), L = (uint32_t)a.L;
-        __syncthreads();  // the last group's table has been read
-        for (int j = threadIdx.x; j < n * P; j += kRopeB) {
-            const int t = j / P, p = j - t * P;
-            int ax = 0;
-            while (ax + 1 < a.axes && p >= a.pair0[ax + 1]) ax++;
-            const uint32_t l = l0 + t;
-            const int64_t at = a.batched ? t0 + t : (int64_t)(l < L ? l : l % L);
-            const double turns = (double)pos[at * a.axes + ax] * a.turn[p];
-            const double r = turns - rint(turns);   // -1/2 .. 1/2, exact
-            const double quarter = rint(4.0 * r);   // nearest quarter turn
-            float s, c;
-            sincospif((float)(2.0 * (r - 0.25 * quarter)), &s, &c);  // at most an eighth of a turn
-            const int k = (int)quarter & 3;
-            const float cc = k & 1 ? s : c, ss = k & 1 ? c : s;
-            table[j] = float2{k == 1 || k == 2 ? -cc : cc, k >= 2 ? -ss : ss};
-        }
-        __syncthreads();
         const int rows = n * heads;
-        for (int r0 = 0; r0 < rows; r0 += slots) {  // every lane takes part in the rows' sums
-            const bool live = r0 + slot < rows;
-            const int r = live ? r0 + slot : rows - 1;
-            const int t = heads == a.chunk ? (int)a.heads.div31(r) : r / heads, h = h0 + r - t * heads;
-            const int64_t tok = t0 + t;
-            int64_t b = b0;
-            uint32_t l = l0 + t;
-            if (l >= L) {
-                b += l / L;
-                l %= L;
-            }
-            const float *xr = x + b * a.sb + (int64_t)l * a.sl + h * a.sh;
-            float *yr = y + (tok * a.H + h) * a.D;
-            const float2 *cs = table + t * P;
-            float e[UPL][2 * V];
+        for (int r0 = 0; r0 < rows; r0 += slots * U) {  // every lane takes part in the rows' sums
+            float e[U][UPL][2 * V], g[MODE == 2 ? U : 1][UPL][2 * V];
+            int tok[U], head[U];
 #pragma unroll
-            for (int k = 0; k < UPL; k++) rope_get<V>(xr, un[k], e[k]);
-            if constexpr (MODE == 0) {
-#pragma unroll
-                for (int k = 0; k < UPL; k++) {
-                    rope_turn<V>(e[k], cs, un[k], a.inter, sign);
-                    if (live) rope_put<V>(yr, un[k], e[k], a.acc);
+            for (int k = 0; k < U; k++) {  // all loads first, and before the table
+                if (r0 + k * slots >= rows) break;
+                const int r = min(r0 + k * slots + slot, rows - 1);
+                const int t = heads == a.chunk ? (int)a.heads.div31(r) : r / heads, h = h0 + r - t * heads;
+                tok[k] = t, head[k] = h;
+                int64_t b = b0;
+                uint32_t l = l0 + t;
+                if (l >= L) {
+                    b += l / L;
+                    l %= L;
                 }
-            } else {
-                const bool key = h >= a.q_heads;
-                float ss = 0.0f;
+                const float *xr = x + b * a.sb + (int64_t)l * a.sl + h * a.sh;
 #pragma unroll
-                for (int k = 0; k < UPL; k++)
+                for (int i = 0; i < UPL; i++) rope_get<V>(xr, un[i], e[k][i]);
+                if constexpr (MODE == 2) {
+                    const float *gr = gy + ((t0 + t) * a.H + h) * a.D;
 #pragma unroll
-                    for (int i = 0; i < 2 * V; i++) ss = fma_(e[k][i], e[k][i], ss);
-                if constexpr (MODE == 1) {
-                    const float rn = 1.0f / sqrtf(group_sum<LPR>(ss) / (float)a.D + a.eps);
+                    for (int i = 0; i < UPL; i++) rope_get<V>(gr, un[i], g[k][i]);
+                }
+            }
+            if (r0 == 0) {
+                __syncthreads();  // the last group's table has been read
+                for (int j = threadIdx.x; j < n * P; j += kRopeB) {
+                    const int t = j / P, p = j - t * P;
+                    int ax = 0;
+                    while (ax + 1 < a.axes && p >= a.pair0[ax + 1]) ax++;
+                    const uint32_t l = l0 + t;
+                    const int64_t at = a.batched ? t0 + t : (int64_t)(l < L ? l : l % L);
+                    const double turns = (double)pos[at * a.axes + ax] * a.turn[p];
+                    const double r = turns - rint(turns);   // -1/2 .. 1/2, exact
+                    const double quarter = rint(4.0 * r);   // nearest quarter turn
+                    float s, c;
+                    sincospif((float)(2.0 * (r - 0.25 * quarter)), &s, &c);  // at most an eighth of a turn
+                    const int k = (int)quarter & 3;
+                    const float cc = k & 1 ? s : c, ss = k & 1 ? c : s;
+                    table[j] = float2{k == 1 || k == 2 ? -cc : cc, k >= 2 ? -ss : ss};
+                }
+                __syncthreads();
+            }
 #pragma unroll
-                    for (int k = 0; k < UPL; k++) {
+            for (int k = 0; k < U; k++) {
+                if (r0 + k * slots >= rows) break;
+                const bool live = r0 + k * slots + slot < rows;
+                float *yr = y + ((t0 + tok[k]) * a.H + head[k]) * a.D;
+                const float2 *cs = table + tok[k] * P;
+                if constexpr (MODE == 0) {
 #pragma unroll
-                        for (int i = 0; i < 2 * V; i++) e[k][i] = e[k][i] * rn * (key ? w[1][k][i] : w[0][k][i]);
-                        rope_turn<V>(e[k], cs, un[k], a.inter, 1.0f);
-                        if (live) rope_put<V>(yr, un[k], e[k], 0);
+                    for (int i = 0; i < UPL; i++) {
+                        rope_turn<V>(e[k][i], cs, un[i], a.inter, sign);
+                        if (live) rope_put<V>(yr, un[i], e[k][i], a.acc);
                     }
                 } else {
-                    const float *gr = gy + (tok * a.H + h) * a.D;
-                    float g[UPL][2 * V], dot = 0.0f;
+                    const bool key = head[k] >= a.q_heads;
+                    float ss = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < UPL; k++) {
-                        rope_get<V>(gr, un[k], g[k]);
-                        rope_turn<V>(g[k], cs, un[k], a.inter, -1.0f);
+                    for (int i = 0; i < UPL; i++)
 #pragma unroll
-                        for (int i = 0; i < 2 * V; i++)
-                            dot = fma_(g[k][i] * (key ? w[1][k][i] : w[0][k][i]), e[k][i], dot);
-                    }
+                        for (int c = 0; c < 2 * V; c++) ss = fma_(e[k][i][c], e[k][i][c], ss);
                     const float rn = 1.0f / sqrtf(group_sum<LPR>(ss) / (float)a.D + a.eps);
-                    const float m = group_sum<LPR>(dot) * rn / (float)a.D;
+                    if constexpr (MODE == 1) {
 #pragma unroll
-                    for (int k = 0; k < UPL; k++) {
-                        float o[2 * V];
+                        for (int i = 0; i < UPL; i++) {
 #pragma unroll
-                        for (int i = 0; i < 2 * V; i++) {
-                            const float nv = e[k][i] * rn, term = live ? g[k][i] * nv : 0.0f;
-                            gw[0][k][i] += key ? 0.0f : term;
-                            gw[1][k][i] += key ? term : 0.0f;
-                            o[i] = rn * fma_(-nv, m, g[k][i] * (key ? w[1][k][i] : w[0][k][i]));
+                            for (int c = 0; c < 2 * V; c++) e[k][i][c] = e[k][i][c] * rn * (key ? w[1][i][c] : w[0][i][c]);
+                            rope_turn<V>(e[k][i], cs, un[i], a.inter, 1.0f);
+                            if (live) rope_put<V>(yr, un[i], e[k][i], 0);
                         }
-                        if (live) rope_put<V>(yr, un[k], o, a.acc);
+                    } else {
+                        float dot = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < UPL; i++) {
+                            rope_turn<V>(g[k][i], cs, un[i], a.inter, -1.0f);
+#pragma unroll
+                            for (int c = 0; c < 2 * V; c++)
+                                dot = fma_(g[k][i][c] * (key ? w[1][i][c] : w[0][i][c]), e[k][i][c], dot);
+                        }
+                        const float m = group_sum<LPR>(dot) * rn / (float)a.D;
+#pragma unroll
+                        for (int i = 0; i < UPL; i++) {
+                            float o[2 * V];
+#pragma unroll
+                            for (int c = 0; c < 2 * V; c++) {
+                                const float nv = e[k][i][c] * rn, term = live ? g[k][i][c] * nv : 0.0f;
+                                gw[0][i][c] += key ? 0.0f : term;
+                                gw[1][i][c] += key ? term : 0.0f;
+                                o[c] = rn * fma_(-nv, m, g[k][i][c] * (key ? w[1][i][c] : w[0][i][c]));
+                            }
+                            if (live) rope_put<V>(yr, un[i], o, a.acc);
+                        }
                     }
                 }
             }
@@ -266,23 +287,27 @@ __global__ __launch_bounds__(kRopeB) void k_rope(const RopeArgs a, const float *
     }
 }
 
-// gwq and gwk: the workgroups' partials in a fixed order, 16 columns and 16 runs of partials a workgroup
-__global__ __launch_bounds__(256) void k_rope_weights(const double *__restrict__ part, int n, int D, float *gwq, float *gwk,
-                                                      int acc_q, int acc_k) {
-    __shared__ double red[16][17];
+// gwq and gwk: the workgroups' partials in a fixed order, 16 columns and 64 runs of partials a workgroup
+__global__ __launch_bounds__(1024) void k_rope_weights(const double *__restrict__ part, int n, int D, float *gwq, float *gwk,
+                                                       int acc_q, int acc_k) {
+    __shared__ double red[64][17];
     const int c = threadIdx.x % 16, run = threadIdx.x / 16, col = blockIdx.x * 16 + c, q = blockIdx.y;
     float *out = q ? gwk : gwq;
     if (!out) return;
-    const int each = (n + 15) / 16;
     double s = 0.0;
-    if (col < D)
-        for (int i = run * each; i < min(n, (run + 1) * each); i++) s += part[((int64_t)i * 2 + q) * D + col];
+    if (col < D) {
+#pragma unroll 8
+        for (int i = run; i < n; i += 64) s += part[((int64_t)i * 2 + q) * D + col];
+    }
     red[run][c] = s;
     __syncthreads();
+    for (int h = 32; h; h /= 2) {
+        if (run < h) red[run][c] += red[run + h][c];
+        __syncthreads();
+    }
     if (run == 0 && col < D) {
-        for (int i = 1; i < 16; i++) s += red[i][c];
         const int acc = q ? acc_k : acc_q;
-        out[col] = (acc ? out[col] : 0.0f) + (float)s;
+        out[col] = (acc ? out[col] : 0.0f) + (float)red[0][c];
     }
 }
 
@@ -298,11 +323,11 @@ static RopePlan rope_plan(int64_t tokens, int H, int D, int P, bool wide) {
     p.v = wide ? 4 : 1;
     const int units = (D + 2 * p.v - 1) / (2 * p.v);  // an upper bound: sections end on whole units, the rest on one
     p.lpr = wide ? 8 : 16;
-    while (p.lpr < units && p.lpr < 64) p.lpr *= 2;
+    while (wide && p.lpr < units) p.lpr *= 2;
     p.upl = (units + p.lpr - 1) / p.lpr;
     const int slots = kRopeB / p.lpr;
     // four rounds of rows a group, fewer where the tokens would not make kRopeBlocks groups
-    int64_t g = (4 * slots + H - 1) / H;
+    int64_t g = 4 * slots / H;
     if (P && g > kRopeTable / P) g = kRopeTable / P;
     if (g > tokens / kRopeBlocks) g = tokens / kRopeBlocks;
     p.group = (int)(g < 1 ? 1 : g);
@@ -327,10 +352,11 @@ static int rope_launch(const RopePlan &p, const RopeArgs &a, const float *x, con
         if (p.lpr == 8) NC_ROPE(4, 8, 1);
         else if (p.lpr == 16) NC_ROPE(4, 16, 1);
         else NC_ROPE(4, 32, 1);
-    } else if (p.upl == 2) NC_ROPE(1, 64, 2);
-    else if (p.lpr == 64) NC_ROPE(1, 64, 1);
-    else if (p.lpr == 32) NC_ROPE(1, 32, 1);
-    else NC_ROPE(1, 16, 1);
+    } else if (p.upl == 1) NC_ROPE(1, 16, 1);
+    else if (p.upl == 2) NC_ROPE(1, 16, 2);
+    else if (p.upl == 3) NC_ROPE(1, 16, 3);
+    else if (p.upl == 4) NC_ROPE(1, 16, 4);
+    else NC_ROPE(1, 16, 8);
 #undef NC_ROPE
     return check_launch(what);
 }
@@ -473,7 +499,7 @@ extern "C" NC_HIP_API int nc_hip_qk_norm_rope_bwd(int64_t B, int64_t L, int64_t 
         if (const int rc = rope_launch<2>(p, a, x, wq, wk, pos, gy, gx, cols ? (double *)ws : nullptr, 1.0f, st, what)) return rc;
     }
     if (!cols) return NC_HIP_OK;
-    hipLaunchKernelGGL(k_rope_weights, dim3((unsigned)((D + 15) / 16), 2), 256, 0, st, (const double *)ws, n, (int)D, gwq, gwk,
+    hipLaunchKernelGGL(k_rope_weights, dim3((unsigned)((D + 15) / 16), 2), 1024, 0, st, (const double *)ws, n, (int)D, gwq, gwk,
                        acc_wq, acc_wk);
     return check_launch(what);
 }
