@@ -23,7 +23,7 @@ struct AttnArgs {
 };
 
 // ------------------------------------------------------------------------------------------------
-// packing: a workgroup a tile of 32 rows, into one or both layouts
+// packing: a workgroup a tile of 32 rows
 // ------------------------------------------------------------------------------------------------
 // Rows of a (sequence, head of keys) pair: queries' row R is token R / G of query head u G + R % G, keys' are tokens (G = 1).
 struct PackJob {
@@ -31,7 +31,7 @@ struct PackJob {
     int64_t sb, sl, sh;
     int64_t len, tiles;    // rows and tiles of a pair, before key_len
     int G, by_len;         // rows are cut by key_len
-    char *rows, *turned;   // [pair][tile][128 DP]; may be NULL
+    char *out;             // [pair][tile][128 DP]
     float *exps;           // [pair][tile] exponents of the scales
     int64_t first;         // the job's first workgroup
     const float *o, *lse;  // the output gradient's job: o (laid out as src), the rows' log-sum-exps [B, Hq, Lq]
@@ -54,8 +54,6 @@ __device__ __forceinline__ int64_t keys_of(int64_t Lk, const int *key_len, int64
 template <int DP>
 __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
     constexpr int C = DP / 8, PER = (C + 7) / 8;  // chunks of a row; of a lane
-    constexpr int LD = DP + 1;
-    __shared__ float tile[kTile * LD];
     __shared__ float red[kAttnWaves], dots[8][kTile];
     const int t = threadIdx.x, row = t & 31, cl = t >> 5;
     for (int64_t w = blockIdx.x; w < a.total; w += gridDim.x) {
@@ -91,13 +89,6 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
         __syncthreads();  // the last tile has been read
         if (j.stats) dots[cl][row] = dot;
         if ((t & 63) == 0) red[t >> 6] = most;
-        if (j.turned) {
-#pragma unroll
-            for (int k = 0; k < PER; k++)
-                if (cl + 8 * k < C)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) tile[row * LD + 8 * (cl + 8 * k) + e] = x[k][e];
-        }
         __syncthreads();
         const int ex = tile_exponent(__builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3])));
         const float inv = pow2i(-ex);
@@ -110,32 +101,17 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
             j.stats[at * 64 + t] = live ? j.lse[(b * a.Hkv * j.G + u * j.G + g) * (j.len / j.G) + i] * kLog2e : INFINITY;
             j.stats[at * 64 + 32 + t] = d;
         }
-        if (j.rows) {
-            char *out = j.rows + at * tile_bytes(DP);
+        char *out = j.out + at * tile_bytes(DP);
 #pragma unroll
-            for (int k = 0; k < PER; k++)
-                if (cl + 8 * k < C) {
+        for (int k = 0; k < PER; k++) {
+            const int c = cl + 8 * k;
+            if (c >= C) continue;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[k][e] *= inv;
-                    const Split8 s = split8(x[k]);
-                    h8 *o = (h8 *)out + (cl + 8 * k) * 32 + row;
-                    o[0] = s.hi;
-                    o[4 * DP] = s.lo;
-                }
-        }
-        if (j.turned) {
-            char *out = j.turned + at * tile_bytes(DP);
-            for (int k = t; k < 4 * DP; k += kAttnB) {  // fragment k / 64, its lane k % 64
-                const int f = k >> 6, lane = k & 63, s = f / (DP / 32), col = 32 * (f % (DP / 32)) + (lane & 31);
-                const float *p = tile + (16 * s + 4 * (lane >> 5)) * LD + col;
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = p[(e < 4 ? e : e + 4) * LD] * inv;
-                const Split8 q = split8(y);
-                h8 *o = (h8 *)out + k;
-                o[0] = q.hi;
-                o[4 * DP] = q.lo;
-            }
+            for (int e = 0; e < 8; e++) x[k][e] *= inv;
+            const Split8 s = split8(x[k]);
+            h8 *o = (h8 *)out + c * 32 + (row ^ (4 * (c & 1)));
+            o[0] = s.hi;
+            o[4 * DP] = s.lo;
         }
     }
 }
@@ -163,14 +139,14 @@ __device__ __forceinline__ float scalar_load(const float *p) {
     return *(const __attribute__((address_space(4))) float *)(uintptr_t)p;
 }
 
-// The order of a block of N steps, each two fragments from LDS and three products: reads two steps ahead of their products.
-template <int N>
+// The order of a block of N steps, each R reads of fragments from LDS and three products: reads two steps ahead of their products.
+template <int N, int R>
 __device__ __forceinline__ void order_steps() {
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * R, 0);
 #pragma unroll
     for (int i = 0; i < N - 2; i++) {
         __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
 }
@@ -188,7 +164,7 @@ __device__ __forceinline__ int64_t xcd_unit(int64_t w, int64_t units) {
 struct FwdArgs {
     AttnArgs a;
     const float *q;
-    const char *kr, *vt;         // packed keys (rows), values (turned)
+    const char *kp, *vp;         // packed keys and values
     const float *kx, *vx;        // their exponents
     const int *key_len;
     float *o, *lse;
@@ -207,11 +183,12 @@ constexpr float kPShift = 10.0f, kPSlack = 4.0f;
 template <int DP, int TPS, int OCC>
 __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
     constexpr int KS = DP / 16, NT = DP / 32;
-    constexpr int TB = 128 * DP;                 // bytes of a packed tile
+    constexpr int TB = 128 * DP, LO = 64 * DP;   // bytes of a packed tile, and of its first piece
     constexpr int STAGE = 2 * TPS * TB;          // keys' tiles, then values'
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ra = row_at(lane), ca = col_at(lane);
     const uint32_t lds = lds_address(smem);
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
@@ -221,14 +198,14 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
         const int64_t pair = rest / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
         const int64_t n = keys_of(a.Lk, f.key_len, b), nt = (n + kTile - 1) / kTile;
         const int64_t t0 = nt * split / f.splits, t1 = nt * (split + 1) / f.splits;
-        const char *kr = f.kr + pair * f.tiles * TB, *vt = f.vt + pair * f.tiles * TB;
+        const char *kp = f.kp + pair * f.tiles * TB, *vp = f.vp + pair * f.tiles * TB;
         const float *kx = f.kx + pair * f.tiles, *vx = f.vx + pair * f.tiles;
 
         auto copy = [&](int64_t t, int buf) {
             const int c = (int)min((int64_t)TPS, t1 - t) * (TB / 1024);
             const uint32_t at = __builtin_amdgcn_readfirstlane(lds + buf * STAGE);
-            stage_copy(kr + t * TB, at, c);
-            stage_copy(vt + t * TB, at + TPS * TB, c);
+            stage_copy(kp + t * TB, at, c);
+            stage_copy(vp + t * TB, at + TPS * TB, c);
         };
         __syncthreads();  // the last unit's stages have been read
         if (t0 < t1) copy(t0, 0);
@@ -278,13 +255,13 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
 #pragma unroll
             for (int x = 0; x < TPS; x++) {
                 if (t + x >= t1) break;
-                const h8 *kf = (const h8 *)(st + x * TB) + lane, *vf = (const h8 *)(st + (TPS + x) * TB) + lane;
+                const char *kt = st + x * TB + ra, *vt = st + (TPS + x) * TB + ca;
                 f16x s;
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[r] = 0.0f;
 #pragma unroll
-                for (int k = 0; k < KS; k++) s = mfma3(kf[64 * k], kf[64 * k + 4 * DP], qh[k], ql[k], s);
-                order_steps<KS>();
+                for (int k = 0; k < KS; k++) s = mfma3(row_frag(kt, k), row_frag(kt + LO, k), qh[k], ql[k], s);
+                order_steps<KS, 2>();
                 const float c = __builtin_fmaxf(cq * pow2i((int)ek[x]), 0x1p-126f);  // -inf * c stays -inf
                 const int left = (int)min(n - (t + x) * kTile, (int64_t)kTile) - 4 * half;
                 if (t + x + 1 == nt) {
@@ -326,9 +303,9 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
                     const Split8 p = split8(y);
 #pragma unroll
                     for (int d = 0; d < NT; d++)
-                        o[d] = mfma3(vf[64 * (k * NT + d)], vf[64 * (k * NT + d) + 4 * DP], p.hi, p.lo, o[d]);
+                        o[d] = mfma3(col_frag(vt, k, d), col_frag(vt + LO, k, d), p.hi, p.lo, o[d]);
                 }
-                order_steps<2 * NT>();
+                order_steps<2 * NT, 4>();
             }
         }
         l = halves_sum(l);
@@ -567,7 +544,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
 // ------------------------------------------------------------------------------------------------
 struct BwdArgs {
     AttnArgs a;
-    const char *kr, *kt, *vr, *qr, *qt, *gr, *gt;  // packed: rows and turned layouts
+    const char *kp, *vp, *qp, *gp;                 // packed
     const float *kx, *vx, *qx, *gx, *stats;
     const int *key_len;
     float *gq, *gk, *gv;                           // the gradients, or the splits' parts [split][...] where there are any
@@ -611,13 +588,14 @@ __device__ __forceinline__ void store_column(float *row, const f16x (&acc)[NT], 
 
 // gk and gv: a wave holds 32 keys as columns and goes over the tiles of queries: s = q k^T and dp = go v^T, whose rows are queries,
 // then gv^T += go^T p and gk^T += q^T ds with p and ds as they lie.  Padded rows of queries have an infinite log-sum-exp: p = 0.
-template <int DP, int STAGES, int OCC>
+template <int DP, int OCC>
 __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
-    constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, STAGE = 4 * TB + 256;
+    constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * TB + 256;
     constexpr bool REG = DP <= 128;  // keys and values stay in registers, else they are read again for every tile
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ra = row_at(lane), ca = col_at(lane);
     const uint32_t lds = lds_address(smem);
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
@@ -626,23 +604,21 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
         const int split = (int)(rest % f.splits);
         const int64_t pair = rest / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
         const int64_t n = keys_of(a.Lk, f.key_len, b);
-        const int64_t kt = (int64_t)kg * kAttnWaves + wave, key = kt * kTile + (lane & 31);
-        const bool any = (int64_t)kg * kAttnWaves * kTile < n, mine = kt * kTile < n, live = key < n;
+        const int64_t k0 = (int64_t)kg * kAttnWaves + wave, key = k0 * kTile + (lane & 31);
+        const bool any = (int64_t)kg * kAttnWaves * kTile < n, mine = k0 * kTile < n, live = key < n;
         const int64_t t0 = any ? f.qtiles * split / f.splits : 0, t1 = any ? f.qtiles * (split + 1) / f.splits : 0;
         const int64_t q0 = pair * f.qtiles;
         auto copy = [&](int64_t t, int buf) {
             const uint32_t at = __builtin_amdgcn_readfirstlane(lds + buf * STAGE);
             const int64_t x = (q0 + t) * TB;
-            stage_copy(f.qr + x, at, TB / 1024);
-            stage_copy(f.gr + x, at + TB, TB / 1024);
-            stage_copy(f.qt + x, at + 2 * TB, TB / 1024);
-            stage_copy(f.gt + x, at + 3 * TB, TB / 1024);
-            if (threadIdx.x < 16) dma16(f.stats + (q0 + t) * 64 + threadIdx.x * 4, at + 4 * TB);
+            stage_copy(f.qp + x, at, TB / 1024);
+            stage_copy(f.gp + x, at + TB, TB / 1024);
+            if (threadIdx.x < 16) dma16(f.stats + (q0 + t) * 64 + threadIdx.x * 4, at + 2 * TB);
         };
         __syncthreads();  // the last unit's stages have been read
-        if (STAGES == 2 && t0 < t1) copy(t0, 0);
-        const int64_t tile = pair * f.ktiles + (mine ? kt : 0);
-        const h8 *kf = (const h8 *)(f.kr + tile * TB) + lane, *vf = (const h8 *)(f.vr + tile * TB) + lane;
+        if (t0 < t1) copy(t0, 0);
+        const int64_t tile = pair * f.ktiles + (mine ? k0 : 0);
+        const char *kt = f.kp + tile * TB + ra, *vt = f.vp + tile * TB + ra;
         h8 kh[REG ? KS : 1], kl[REG ? KS : 1], vh[REG ? KS : 1], vl[REG ? KS : 1];
         float ck = 0.0f, cv = 0.0f;
         if (mine) {
@@ -651,8 +627,8 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
             if constexpr (REG) {
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
-                    kh[s] = kf[64 * s], kl[s] = kf[64 * s + 4 * DP];
-                    vh[s] = vf[64 * s], vl[s] = vf[64 * s + 4 * DP];
+                    kh[s] = row_frag(kt, s), kl[s] = row_frag(kt + LO, s);
+                    vh[s] = row_frag(vt, s), vl[s] = row_frag(vt + LO, s);
                 }
             }
         }
@@ -662,29 +638,23 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
 #pragma unroll
             for (int r = 0; r < 16; r++) dk[t][r] = dv[t][r] = 0.0f;
         float F = 0x1p100f, E = -1000.0f;
-        for (int64_t t = t0, buf = 0; t < t1; t++) {
-            if constexpr (STAGES == 1) {
-                __syncthreads();  // the last tile has been read
-                copy(t, 0);
-            }
+        for (int64_t t = t0, buf = 0; t < t1; t++, buf ^= 1) {
             const float ex = scalar_load(f.gx + q0 + t), eq = scalar_load(f.qx + q0 + t);
             stage_wait();
-            if (STAGES == 2 && t + 1 < t1) copy(t + 1, (int)buf ^ 1);
+            if (t + 1 < t1) copy(t + 1, (int)buf ^ 1);
             const char *st = smem + buf * STAGE;
-            if (STAGES == 2) buf ^= 1;
             if (!mine) continue;
-            const h8 *qf = (const h8 *)st + lane, *gf = (const h8 *)(st + TB) + lane;
-            const h8 *qtf = (const h8 *)(st + 2 * TB) + lane, *gtf = (const h8 *)(st + 3 * TB) + lane;
-            const f4 *rows = (const f4 *)(st + 4 * TB) + half;
+            const char *qt = st + ra, *gt = st + TB + ra, *qc = st + ca, *gc = st + TB + ca;
+            const f4 *rows = (const f4 *)(st + 2 * TB) + half;
             f16x s, dp;
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                s = mfma3(qf[64 * k], qf[64 * k + 4 * DP], REG ? kh[k] : kf[64 * k], REG ? kl[k] : kf[64 * k + 4 * DP], s);
-                dp = mfma3(gf[64 * k], gf[64 * k + 4 * DP], REG ? vh[k] : vf[64 * k], REG ? vl[k] : vf[64 * k + 4 * DP], dp);
+                s = mfma3(row_frag(qt, k), row_frag(qt + LO, k), REG ? kh[k] : row_frag(kt, k), REG ? kl[k] : row_frag(kt + LO, k), s);
+                dp = mfma3(row_frag(gt, k), row_frag(gt + LO, k), REG ? vh[k] : row_frag(vt, k), REG ? vl[k] : row_frag(vt + LO, k), dp);
             }
-            if constexpr (REG) order_steps<2 * KS>();
+            if constexpr (REG) order_steps<2 * KS, 2>();
             if (ex > E) {
                 scale_acc(dv, __builtin_amdgcn_exp2f(E - ex));
                 E = ex;
@@ -716,12 +686,11 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                 const Split8 ps = split8(y), ds = split8(z);
 #pragma unroll
                 for (int d = 0; d < NT; d++) {
-                    const int at = 64 * (k * NT + d);
-                    dv[d] = mfma3(gtf[at], gtf[at + 4 * DP], ps.hi, ps.lo, dv[d]);
-                    dk[d] = mfma3(qtf[at], qtf[at + 4 * DP], ds.hi, ds.lo, dk[d]);
+                    dv[d] = mfma3(col_frag(gc, k, d), col_frag(gc + LO, k, d), ps.hi, ps.lo, dv[d]);
+                    dk[d] = mfma3(col_frag(qc, k, d), col_frag(qc + LO, k, d), ds.hi, ds.lo, dk[d]);
                 }
             }
-            order_steps<4 * NT>();
+            order_steps<4 * NT, 4>();
         }
         if (key < a.Lk) {
             const int64_t at = ((b * a.Lk + key) * a.Hkv + u) * a.D;
@@ -734,12 +703,13 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
 
 // gq: a wave holds 32 rows of queries as columns, as the forward does, and goes over the tiles of keys: s^T = k q^T and
 // dp^T = v go^T, then gq^T += k^T ds^T.
-template <int DP, int STAGES, int OCC>
+template <int DP, int OCC>
 __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
-    constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, STAGE = 3 * TB;
+    constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * TB;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ra = row_at(lane), ca = col_at(lane);
     const uint32_t lds = lds_address(smem);
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
@@ -755,19 +725,18 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
         auto copy = [&](int64_t t, int buf) {
             const uint32_t at = __builtin_amdgcn_readfirstlane(lds + buf * STAGE);
             const int64_t x = (k0 + t) * TB;
-            stage_copy(f.kr + x, at, TB / 1024);
-            stage_copy(f.vr + x, at + TB, TB / 1024);
-            stage_copy(f.kt + x, at + 2 * TB, TB / 1024);
+            stage_copy(f.kp + x, at, TB / 1024);
+            stage_copy(f.vp + x, at + TB, TB / 1024);
         };
         __syncthreads();  // the last unit's stages have been read
-        if (STAGES == 2 && t0 < t1) copy(t0, 0);
+        if (t0 < t1) copy(t0, 0);
         const int64_t tile = pair * f.qtiles + (mine ? qt : 0);
-        const h8 *qf = (const h8 *)(f.qr + tile * TB) + lane, *gf = (const h8 *)(f.gr + tile * TB) + lane;
+        const char *qp = f.qp + tile * TB + ra, *gp = f.gp + tile * TB + ra;
         h8 qh[KS], ql[KS], gh[KS], gl[KS];
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            qh[s] = qf[64 * s], ql[s] = qf[64 * s + 4 * DP];
-            gh[s] = gf[64 * s], gl[s] = gf[64 * s + 4 * DP];
+            qh[s] = row_frag(qp, s), ql[s] = row_frag(qp + LO, s);
+            gh[s] = row_frag(gp, s), gl[s] = row_frag(gp + LO, s);
         }
         const float cq = pow2i((int)f.qx[tile]) * a.scale * kLog2e, cg = pow2i((int)f.gx[tile]);
         const float ls = f.stats[tile * 64 + (lane & 31)], de = f.stats[tile * 64 + 32 + (lane & 31)];
@@ -777,27 +746,22 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
 #pragma unroll
             for (int r = 0; r < 16; r++) dq[t][r] = 0.0f;
         float F = 0x1p100f;
-        for (int64_t t = t0, buf = 0; t < t1; t++) {
-            if constexpr (STAGES == 1) {
-                __syncthreads();  // the last tile has been read
-                copy(t, 0);
-            }
+        for (int64_t t = t0, buf = 0; t < t1; t++, buf ^= 1) {
             const float ek = scalar_load(f.kx + k0 + t), ev = scalar_load(f.vx + k0 + t);
             stage_wait();
-            if (STAGES == 2 && t + 1 < t1) copy(t + 1, (int)buf ^ 1);
+            if (t + 1 < t1) copy(t + 1, (int)buf ^ 1);
             const char *st = smem + buf * STAGE;
-            if (STAGES == 2) buf ^= 1;
             if (!mine) continue;
-            const h8 *kf = (const h8 *)st + lane, *vf = (const h8 *)(st + TB) + lane, *ktf = (const h8 *)(st + 2 * TB) + lane;
+            const char *kt = st + ra, *vt = st + TB + ra, *kc = st + ca;
             f16x s, dp;
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                s = mfma3(kf[64 * k], kf[64 * k + 4 * DP], qh[k], ql[k], s);
-                dp = mfma3(vf[64 * k], vf[64 * k + 4 * DP], gh[k], gl[k], dp);
+                s = mfma3(row_frag(kt, k), row_frag(kt + LO, k), qh[k], ql[k], s);
+                dp = mfma3(row_frag(vt, k), row_frag(vt + LO, k), gh[k], gl[k], dp);
             }
-            order_steps<2 * KS>();
+            order_steps<2 * KS, 2>();
             const float c = cq * pow2i((int)ek), c2 = cg * pow2i((int)ev);
             const int left = (int)min(n - t * kTile, (int64_t)kTile) - 4 * half;
             float most = 0.0f;
@@ -820,11 +784,10 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
                 const Split8 ds = split8(z);
 #pragma unroll
                 for (int d = 0; d < NT; d++) {
-                    const int at = 64 * (k * NT + d);
-                    dq[d] = mfma3(ktf[at], ktf[at + 4 * DP], ds.hi, ds.lo, dq[d]);
+                    dq[d] = mfma3(col_frag(kc, k, d), col_frag(kc + LO, k, d), ds.hi, ds.lo, dq[d]);
                 }
             }
-            order_steps<2 * NT>();
+            order_steps<2 * NT, 4>();
         }
         if (R < f.rows) {
             const int64_t i = R / a.G, h = u * a.G + (R - i * a.G);
@@ -886,7 +849,7 @@ struct FwdPlan {
     bool token;
     int DP, qtiles, splits;
     int64_t rows, tiles, pairs, units;
-    size_t kr, vt, kx, vx, po, pm, total;  // offsets into the workspace
+    size_t kp, vp, kx, vx, po, pm, total;  // offsets into the workspace
 };
 
 static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D) {
@@ -909,8 +872,8 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
         return here;
     };
     if (!p.token) {
-        p.kr = take(pt * tile_bytes(p.DP));
-        p.vt = take(pt * tile_bytes(p.DP));
+        p.kp = take(pt * tile_bytes(p.DP));
+        p.vp = take(pt * tile_bytes(p.DP));
         p.kx = take(pt * 4);
         p.vx = take(pt * 4);
     }
@@ -986,11 +949,11 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     if (Lk && !p.token) {
         PackArgs pk{};
         pk.Lk = Lk, pk.Hkv = Hkv, pk.D = (int)D, pk.key_len = key_len, pk.jobs = 2;
-        pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, 1, w + p.kr, nullptr, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
-        pk.job[1] = {v, sv[0], sv[1], sv[2], Lk, p.tiles, 1, 1, nullptr, w + p.vt, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
+        pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, 1, w + p.kp, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
+        pk.job[1] = {v, sv[0], sv[1], sv[2], Lk, p.tiles, 1, 1, w + p.vp, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
         pack_launch(pk, p.pairs, p.DP, st);
     }
-    FwdArgs f{a, q, w + p.kr, w + p.vt, (float *)(w + p.kx), (float *)(w + p.vx), key_len, o, lse, (float *)(w + p.po), (f2 *)(w + p.pm),
+    FwdArgs f{a, q, w + p.kp, w + p.vp, (float *)(w + p.kx), (float *)(w + p.vx), key_len, o, lse, (float *)(w + p.po), (f2 *)(w + p.pm),
               p.rows, p.tiles, p.units, p.qtiles, p.splits};
     if (p.token)
         token_launch(f, k, v, st);
@@ -1007,7 +970,7 @@ namespace nchip {
 struct BwdPlan {
     int DP, qgroups, kgroups, qsplits, ksplits;  // splits of the keys for gq, of the queries for gk and gv
     int64_t rows, qtiles, ktiles, pairs, nq, nk;
-    size_t kr, kt, vr, qr, qt, gr, gt, kx, vx, qx, gx, stats, pq, pk, pv, total;
+    size_t kp, vp, qp, gp, kx, vx, qx, gx, stats, pq, pk, pv, total;
 };
 
 static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D) {
@@ -1031,8 +994,7 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
         return here;
     };
     const int64_t q = p.pairs * p.qtiles, k = p.pairs * p.ktiles, tb = tile_bytes(p.DP);
-    p.kr = take(k * tb), p.kt = take(k * tb), p.vr = take(k * tb);
-    p.qr = take(q * tb), p.qt = take(q * tb), p.gr = take(q * tb), p.gt = take(q * tb);
+    p.kp = take(k * tb), p.vp = take(k * tb), p.qp = take(q * tb), p.gp = take(q * tb);
     p.kx = take(k * 4), p.vx = take(k * 4), p.qx = take(q * 4), p.gx = take(q * 4), p.stats = take(q * 256);
     if (p.qsplits > 1) p.pq = take(p.qsplits * p.nq * 4);
     if (p.ksplits > 1) p.pk = take(p.ksplits * p.nk * 4), p.pv = take(p.ksplits * p.nk * 4);
@@ -1073,7 +1035,7 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
     char *const w = (char *)ws;
     BwdArgs f{};
     f.a = a;
-    f.kr = w + p.kr, f.kt = w + p.kt, f.vr = w + p.vr, f.qr = w + p.qr, f.qt = w + p.qt, f.gr = w + p.gr, f.gt = w + p.gt;
+    f.kp = w + p.kp, f.vp = w + p.vp, f.qp = w + p.qp, f.gp = w + p.gp;
     f.kx = (float *)(w + p.kx), f.vx = (float *)(w + p.vx), f.qx = (float *)(w + p.qx), f.gx = (float *)(w + p.gx);
     f.stats = (float *)(w + p.stats);
     f.key_len = key_len;
@@ -1082,12 +1044,12 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
     pk.Lk = Lk, pk.Hkv = Hkv, pk.D = (int)D, pk.key_len = key_len;
     const int64_t G = a.G;
     if (Lk) {
-        pk.job[pk.jobs++] = {k, sk[0], sk[1], sk[2], Lk, p.ktiles, 1, 1, w + p.kr, want_q ? w + p.kt : nullptr, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
-        pk.job[pk.jobs++] = {v, sv[0], sv[1], sv[2], Lk, p.ktiles, 1, 1, w + p.vr, nullptr, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {k, sk[0], sk[1], sk[2], Lk, p.ktiles, 1, 1, w + p.kp, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {v, sv[0], sv[1], sv[2], Lk, p.ktiles, 1, 1, w + p.vp, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
     }
     if (Lq) {
-        pk.job[pk.jobs++] = {q, sq[0], sq[1], sq[2], p.rows, p.qtiles, (int)G, 0, w + p.qr, want_k ? w + p.qt : nullptr, (float *)(w + p.qx), 0, nullptr, nullptr, nullptr};
-        pk.job[pk.jobs++] = {go, Lq * Hq * D, Hq * D, D, p.rows, p.qtiles, (int)G, 0, w + p.gr, want_k ? w + p.gt : nullptr, (float *)(w + p.gx), 0, o, lse, (float *)(w + p.stats)};
+        pk.job[pk.jobs++] = {q, sq[0], sq[1], sq[2], p.rows, p.qtiles, (int)G, 0, w + p.qp, (float *)(w + p.qx), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {go, Lq * Hq * D, Hq * D, D, p.rows, p.qtiles, (int)G, 0, w + p.gp, (float *)(w + p.gx), 0, o, lse, (float *)(w + p.stats)};
     }
     pack_launch(pk, p.pairs, p.DP, st);
     if (want_q) {
@@ -1096,8 +1058,7 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
         f.acc_q = cut ? 0 : acc_q;
         f.part_q = p.nq, f.groups = p.qgroups, f.splits = p.qsplits;
         f.units = p.pairs * p.qgroups * p.qsplits;
-        NC_ATTN_DP(p.DP, constexpr int STAGES = DP <= 128 ? 2 : 1; constexpr int OCC = DP <= 64 ? 2 : 1;
-                   attn_launch(&k_attn_dq<DP, STAGES, OCC>, f.units, STAGES * 3 * 128 * DP, st, f));
+        NC_ATTN_DP(p.DP, constexpr int OCC = DP <= 64 ? 2 : 1; attn_launch(&k_attn_dq<DP, OCC>, f.units, 2 * 2 * 128 * DP, st, f));
         if (cut) sum_launch(p.nq, p.qsplits, f.gq, gq, acc_q, st);
     }
     if (want_k) {
@@ -1108,8 +1069,8 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
         f.acc_v = cut ? 0 : acc_v;
         f.part_k = p.nk, f.groups = p.kgroups, f.splits = p.ksplits;
         f.units = p.pairs * p.kgroups * p.ksplits;
-        NC_ATTN_DP(p.DP, constexpr int STAGES = DP <= 128 ? 2 : 1; constexpr int OCC = DP <= 64 ? 2 : 1;
-                   attn_launch(&k_attn_dkv<DP, STAGES, OCC>, f.units, STAGES * (4 * 128 * DP + 256), st, f));
+        NC_ATTN_DP(p.DP, constexpr int OCC = DP <= 64 ? 2 : 1;
+                   attn_launch(&k_attn_dkv<DP, OCC>, f.units, 2 * (2 * 128 * DP + 256), st, f));
         if (cut && gk) sum_launch(p.nk, p.ksplits, f.gk, gk, acc_k, st);
         if (cut && gv) sum_launch(p.nk, p.ksplits, f.gv, gv, acc_v, st);
     }

@@ -6,14 +6,14 @@
 // scale keeps the whole exponent range: values 2^-17 of their tile's largest and up have their 22 bits, smaller ones an absolute
 // error of 2^-40 of that largest.  Three products at the fp16 rate cost a fifth of v_mfma_f32_32x32x2_f32's one.
 //
-// Fragments: lane l of the 32x32x16 product holds row (of A) or column (of B) l % 32 and the eight k of half l / 32; the
-// result's column l % 32 in rows 8 (r / 4) + 4 (l / 32) + r % 4, r < 16.  A tile is stored fragment by fragment, 1 KiB each,
-// lane l's 16 bytes at 16 l, so that a wave's load of one (from LDS, or by direct-to-LDS copies from memory) is contiguous:
-//   rows layout (the columns are summed over): fragment s holds columns 16 s + 8 (l / 32) .. + 7 of row l % 32;
-//   turned layout (the rows are summed over): fragment s * (DP / 32) + t holds rows 16 s + 4 (l / 32) + {0, 1, 2, 3, 8, 9, 10, 11}
+// Fragments: lane l of the 32x32x16 product holds row (of A) or column (of B) l % 32 and eight k, those of half l / 32; the
+// result's column l % 32 in rows 8 (r / 4) + 4 (l / 32) + r % 4, r < 16.  A tile holds the 16 bytes of columns 8 c .. 8 c + 7 of row
+// r at 16 (32 c + (r ^ 4 (c & 1))), first of all hi, then of all lo: 128 DP bytes, DP the columns padded to 32, 64, 96, 128 or
+// 256 with zeros.  From LDS it gives both operands without bank conflicts:
+//   row fragments (the columns are summed over), one 16-byte read: columns 16 s + 8 (l / 32) .. + 7 of row l % 32;
+//   column fragments (the rows are summed over), two transposing 8-byte reads: rows 16 s + 4 (l / 32) + {0, 1, 2, 3, 8, 9, 10, 11}
 //   of column 32 t + l % 32 -- the order in which a result's registers 8 s .. 8 s + 7 hold their rows, so that probabilities
 //   are the next product's operand without leaving their lanes.
-// Each layout has the hi fragments, then the lo ones: 128 DP bytes, DP the columns padded to 32, 64, 96, 128 or 256 with zeros.
 #pragma once
 
 #include "common.hpp"
@@ -46,6 +46,27 @@ __device__ __forceinline__ Split8 split8(const float *x) {
         r.lo[i] = l.x, r.lo[i + 1] = l.y;
     }
     return r;
+}
+
+// a lane's byte offset in a tile for row fragment 0 (s: + 1024 s; lo: + 64 DP), and for column fragment (0, 0)
+__device__ __forceinline__ int row_at(int lane) {
+    const int half = lane >> 5, r = lane & 31;
+    return half * 512 + (r ^ (4 * half)) * 16;
+}
+__device__ __forceinline__ int col_at(int lane) {
+    const int i = lane & 15, g = lane >> 4, b = (i >> 1) & 1;
+    return (2 * (g & 1) + b) * 512 + (((g >> 1) ^ b) * 4 + i / 4) * 16 + 8 * (i & 1);
+}
+__device__ __forceinline__ h8 row_frag(const char *tile, int s) { return *(const h8 *)(tile + 1024 * s); }
+// 16 lanes read four rows of 16 columns, four columns a lane, and get four rows of one column each
+__device__ __forceinline__ h8 col_frag(const char *tile, int s, int t) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    const char *p = tile + 2048 * t + 256 * s;
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 128));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(h8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 }
 
 __device__ __forceinline__ f16x mfma3(const h8 &ah, const h8 &al, const h8 &bh, const h8 &bl, f16x c) {
