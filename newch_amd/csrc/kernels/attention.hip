@@ -9,28 +9,21 @@
 //
 // The products run on the fp16 matrix cores with operands in two pieces (attention.hpp), packed once into a workspace.
 #include "attention.hpp"
+#include "attention_short.hpp"
 
 #include <math.h>
 
 namespace nchip {
 
-constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
-
-struct AttnArgs {
-    int64_t B, Lq, Lk, Hq, Hkv, D, G;  // G: query heads of a key head
-    int64_t sq[3], sk[3], sv[3];
-    float scale;
-};
-
 // ------------------------------------------------------------------------------------------------
 // packing: a workgroup a tile of 32 rows
 // ------------------------------------------------------------------------------------------------
-// Rows of a (sequence, head of keys) pair: queries' row R is token R / G of query head u G + R % G, keys' are tokens (G = 1).
+// Rows of a (sequence, head of keys) pair: queries' row R is token R / G of query head u G + R % G, keys' are tokens.
 struct PackJob {
     const float *src;
     int64_t sb, sl, sh;
     int64_t len, tiles;    // rows and tiles of a pair, before key_len
-    int G, by_len;         // rows are cut by key_len
+    int by_len;            // keys: rows are cut by key_len; else queries
     char *out;             // [pair][tile][128 DP]
     float *exps;           // [pair][tile] exponents of the scales
     int64_t first;         // the job's first workgroup
@@ -40,16 +33,10 @@ struct PackJob {
 struct PackArgs {
     PackJob job[4];
     int jobs;
-    int64_t total, Lk, Hkv;
-    int D;
+    AttnArgs a;
+    int64_t total;
     const int *key_len;
 };
-
-__device__ __forceinline__ int64_t keys_of(int64_t Lk, const int *key_len, int64_t b) {
-    if (!key_len) return Lk;
-    const int64_t n = key_len[b];
-    return n < 0 ? 0 : n < Lk ? n : Lk;
-}
 
 template <int DP>
 __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
@@ -61,13 +48,14 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
         while (jx + 1 < a.jobs && w >= a.job[jx + 1].first) jx++;
         const PackJob &j = a.job[jx];
         const int64_t pair = (w - j.first) / j.tiles, tl = (w - j.first) - pair * j.tiles;
-        const int64_t b = pair / a.Hkv, u = pair - b * a.Hkv;
-        const int64_t n = j.by_len ? keys_of(a.Lk, a.key_len, b) : j.len;
+        const int64_t b = pair / a.a.Hkv, u = pair - b * a.a.Hkv;
+        const int64_t n = j.by_len ? keys_of(a.a.Lk, a.key_len, b) : j.len;
         const int64_t R = tl * kTile + row;
         if (tl * kTile >= n) continue;  // no workgroup reads this tile
         const bool live = R < n;
-        const int64_t i = live ? R / j.G : 0, g = live ? R - i * j.G : 0;
-        const int64_t off = b * j.sb + i * j.sl + (u * j.G + g) * j.sh;
+        int64_t i = live ? R : 0, g = 0;
+        if (!j.by_len) a.a.row(i, i, g);
+        const int64_t h = j.by_len ? u : u * a.a.G + g, off = b * j.sb + i * j.sl + h * j.sh;
         const float *src = j.src + off;
         float x[PER][8], most = 0.0f, dot = 0.0f;
 #pragma unroll
@@ -75,12 +63,12 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; e++) x[k][e] = 0.0f;
             const int c = cl + 8 * k;
-            if (live && c < C) load8(src, 8 * c, a.D, x[k]);
+            if (live && c < C) load8(src, 8 * c, (int)a.a.D, x[k]);
 #pragma unroll
             for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[k][e]));
             if (j.stats && live && c < C) {
                 float y[8];
-                load8(j.o + off, 8 * c, a.D, y);
+                load8(j.o + off, 8 * c, (int)a.a.D, y);
 #pragma unroll
                 for (int e = 0; e < 8; e++) dot = fma_(x[k][e], y[e], dot);
             }
@@ -98,7 +86,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
             float d = dots[0][t];
 #pragma unroll
             for (int e = 1; e < 8; e++) d += dots[e][t];
-            j.stats[at * 64 + t] = live ? j.lse[(b * a.Hkv * j.G + u * j.G + g) * (j.len / j.G) + i] * kLog2e : INFINITY;
+            j.stats[at * 64 + t] = live ? j.lse[(b * a.a.Hq + h) * a.a.Lq + i] * kLog2e : INFINITY;
             j.stats[at * 64 + 32 + t] = d;
         }
         char *out = j.out + at * tile_bytes(DP);
@@ -139,25 +127,6 @@ __device__ __forceinline__ float scalar_load(const float *p) {
     return *(const __attribute__((address_space(4))) float *)(uintptr_t)p;
 }
 
-// The order of a block of N steps, each R reads of fragments from LDS and three products: reads two steps ahead of their products.
-template <int N, int R>
-__device__ __forceinline__ void order_steps() {
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * R, 0);
-#pragma unroll
-    for (int i = 0; i < N - 2; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
-}
-
-// Workgroups are dealt round robin over the 8 XCDs: consecutive units of a launch go to one XCD, which then keeps their
-// keys in its L2.
-__device__ __forceinline__ int64_t xcd_unit(int64_t w, int64_t units) {
-    const int64_t each = units / 8, rest = units % 8, x = w % 8, k = w / 8;
-    return x * each + (x < rest ? x : rest) + k;
-}
-
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
@@ -174,17 +143,9 @@ struct FwdArgs {
     int qtiles, splits;          // groups of 128 rows of a pair, parts its keys are cut into
 };
 
-// A wave holds 32 rows of queries as columns: s^T = k q^T (A: 32 keys), so that a row's scores lie in the registers of two lanes
-// and its maximum, sum and scale are theirs; p^T is then the operand of o^T = v^T p^T as it lies.  One pass over the keys: the
-// reference m a row's exponents are taken from moves only when a score passes it by 2^4, and o and the sum with it; p is held as
-// 2^10 p (at most 2^14) in two fp16, so a p below 2^-13 loses low bits against an absolute 2^-35.
-constexpr float kPShift = 10.0f, kPSlack = 4.0f;
-
 template <int DP, int TPS, int OCC>
 __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
-    constexpr int KS = DP / 16, NT = DP / 32;
-    constexpr int TB = 128 * DP, LO = 64 * DP;   // bytes of a packed tile, and of its first piece
-    constexpr int STAGE = 2 * TPS * TB;          // keys' tiles, then values'
+    constexpr int TB = 128 * DP, STAGE = 2 * TPS * TB;  // bytes of a packed tile; of the keys' and values' of a stage
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -213,125 +174,37 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
         // this lane's row of queries, times scale log2(e), as the second operand
         const int64_t R = ((int64_t)qt * kAttnWaves + wave) * kTile + (lane & 31);
         const bool live = R < f.rows;
-        const int64_t i = live ? R / a.G : 0, g = live ? R - i * a.G : 0, h = u * a.G + g;
-        const float *qrow = f.q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2];
-        h8 qh[KS], ql[KS];
-        float cq;
-        {
-            const float c = live ? a.scale * kLog2e : 0.0f;
-            float most = 0.0f, x[8];
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                load8(qrow, 16 * s + 8 * half, (int)a.D, x);
-#pragma unroll
-                for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[e] * c));
-            }
-            const int e = tile_exponent(halves_max(most));
-            const float inv = pow2i(-e);
-            cq = pow2i(e);
-            asm volatile("" ::: "memory");  // the row is read again (from the caches) rather than held in fp32 as well
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                load8(qrow, 16 * s + 8 * half, (int)a.D, x);
-#pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = live ? x[k] * c * inv : 0.0f;
-                const Split8 p = split8(x);
-                qh[s] = p.hi, ql[s] = p.lo;
-            }
-        }
-        f16x o[NT];
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
-        float m = -INFINITY, l = 0.0f, E = -1000.0f;
+        int64_t i, g;
+        a.row(live ? R : 0, i, g);
+        const int64_t h = u * a.G + g;
+        Query<DP> q;
+        load_query(q, f.q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2], live, a.scale, half, (int)a.D);
+        Sums<DP> sum;
+        sum.clear();
         for (int64_t t = t0, buf = 0; t < t1; t += TPS, buf ^= 1) {
-            float ek[TPS], evs[TPS];
+            float ek[TPS], ev[TPS];
 #pragma unroll
-            for (int x = 0; x < TPS; x++) ek[x] = scalar_load(kx + min(t + x, t1 - 1)), evs[x] = scalar_load(vx + min(t + x, t1 - 1));
+            for (int x = 0; x < TPS; x++) ek[x] = scalar_load(kx + min(t + x, t1 - 1)), ev[x] = scalar_load(vx + min(t + x, t1 - 1));
             stage_wait();
             if (t + TPS < t1) copy(t + TPS, (int)buf ^ 1);
             const char *st = smem + buf * STAGE;
 #pragma unroll
             for (int x = 0; x < TPS; x++) {
                 if (t + x >= t1) break;
-                const char *kt = st + x * TB + ra, *vt = st + (TPS + x) * TB + ca;
-                f16x s;
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; k++) s = mfma3(row_frag(kt, k), row_frag(kt + LO, k), qh[k], ql[k], s);
-                order_steps<KS, 2>();
-                const float c = __builtin_fmaxf(cq * pow2i((int)ek[x]), 0x1p-126f);  // -inf * c stays -inf
-                const int left = (int)min(n - (t + x) * kTile, (int64_t)kTile) - 4 * half;
-                if (t + x + 1 == nt) {
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (8 * (r / 4) + r % 4 >= left) s[r] = -INFINITY;
-                }
-                float top = s[0];
-#pragma unroll
-                for (int r = 1; r < 16; r++) top = __builtin_fmaxf(top, s[r]);
-                top = halves_max(top) * c;
-                const float ev = evs[x];
-                if (__any(top > m + kPSlack) || ev > E) {
-                    const float mn = top > m + kPSlack ? top : m, En = __builtin_fmaxf(E, ev);
-                    const float al = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-                    const float ao = al * __builtin_amdgcn_exp2f(E - En);
-                    l *= al;
-                    m = mn;
-                    E = En;
-#pragma unroll
-                    for (int d = 0; d < NT; d++)
-#pragma unroll
-                        for (int r = 0; r < 16; r++) o[d][r] *= ao;
-                }
-                // values of smaller tiles count through smaller p (no smaller than 2^-60: below what o can show)
-                const float dv = __builtin_fmaxf(ev - E, -60.0f), off = kPShift + dv - m;
-                float sum = 0.0f;
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    s[r] = __builtin_amdgcn_exp2f(fma_(s[r], c, off));
-                    sum += s[r];
-                }
-                l = fma_(sum, __builtin_amdgcn_exp2f(-dv), l);
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) y[e] = s[8 * k + e];
-                    const Split8 p = split8(y);
-#pragma unroll
-                    for (int d = 0; d < NT; d++)
-                        o[d] = mfma3(col_frag(vt, k, d), col_frag(vt + LO, k, d), p.hi, p.lo, o[d]);
-                }
-                order_steps<2 * NT, 4>();
+                attend(sum, q, st + x * TB + ra, st + (TPS + x) * TB + ca, ek[x], ev[x], t + x + 1 == nt,
+                       (int)min(n - (t + x) * kTile, (int64_t)kTile) - 4 * half);
             }
         }
-        l = halves_sum(l);
-        if (!live) continue;
-        if (f.splits == 1) {
-            const float inv = l != 0.0f ? pow2i((int)E) / l : 0.0f;  // no keys: o is zero
-            float *row = f.o + ((b * a.Lq + i) * a.Hq + h) * a.D;
-#pragma unroll
-            for (int d = 0; d < NT; d++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    store4(row, 32 * d + 8 * j + 4 * half, (int)a.D,
-                           f4{o[d][4 * j] * inv, o[d][4 * j + 1] * inv, o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv}, 0);
+        const float l = halves_sum(sum.l);
+        if (live && f.splits == 1) {
+            // no keys: o is zero
+            store_column(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, l != 0.0f, pow2i((int)sum.E) / l, half, (int)a.D, 0);
             if (f.lse && half == 0)
-                f.lse[(b * a.Hq + h) * a.Lq + i] = nt ? fma_(m - kPShift, kLn2, logf(l)) : -INFINITY;
-        } else {
+                f.lse[(b * a.Hq + h) * a.Lq + i] = nt ? fma_(sum.m - kPShift, kLn2, logf(l)) : -INFINITY;
+        } else if (live) {
             const int64_t pr = ((int64_t)split * a.B * a.Hkv + pair) * f.rows + R;
-            const float inv = t0 < t1 ? pow2i((int)E) : 0.0f;
-            float *row = f.po + pr * a.D;
-#pragma unroll
-            for (int d = 0; d < NT; d++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    store4(row, 32 * d + 8 * j + 4 * half, (int)a.D,
-                           f4{o[d][4 * j] * inv, o[d][4 * j + 1] * inv, o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv}, 0);
-            if (half == 0) f.pm[pr] = f2{t0 < t1 ? m - kPShift : -INFINITY, l};
+            store_column(f.po + pr * a.D, sum.o, t0 < t1, pow2i((int)sum.E), half, (int)a.D, 0);
+            if (half == 0) f.pm[pr] = f2{t0 < t1 ? sum.m - kPShift : -INFINITY, l};
         }
     }
 }
@@ -383,7 +256,9 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
         float m[NR], l[NR];
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-            const int64_t R = r < f.rows ? r : 0, i = R / a.G, h = u * a.G + (R - i * a.G);
+            int64_t i, g;
+            a.row(r < f.rows ? r : 0, i, g);
+            const int64_t h = u * a.G + g;
             const float *row = f.q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2];
 #pragma unroll
             for (int x = 0; x < 2; x++) {
@@ -492,7 +367,9 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
                 total = fma_(al, t.y, total);
             }
             if (f.splits == 1) {
-                const int64_t i = r / a.G, h = u * a.G + (r - i * a.G);
+                int64_t i, g;
+                a.row(r, i, g);
+                const int64_t h = u * a.G + g;
                 f.o[((b * a.Lq + i) * a.Hq + h) * a.D + d] = total != 0.0f ? sum / total : 0.0f;
                 if (f.lse && d == 0) f.lse[(b * a.Hq + h) * a.Lq + i] = n ? fma_(top, kLn2, logf(total)) : -INFINITY;
             } else {
@@ -512,7 +389,9 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
     const int lane = threadIdx.x & 63;
     for (int64_t pr = (int64_t)blockIdx.x * kAttnWaves + (threadIdx.x >> 6); pr < all; pr += (int64_t)gridDim.x * kAttnWaves) {
         const int64_t pair = pr / rows, R = pr - pair * rows, b = pair / a.Hkv, u = pair - b * a.Hkv;
-        const int64_t i = R / a.G, h = u * a.G + (R - i * a.G);
+        int64_t i, g;
+            a.row(R, i, g);
+            const int64_t h = u * a.G + g;
         const f2 ml = lane < splits ? pm[lane * all + pr] : f2{-INFINITY, 0.0f};
         const bool nan = __any(ml.x != ml.x);
         const float M = wave_max_nan_skip(ml.x);
@@ -552,39 +431,6 @@ struct BwdArgs {
     int groups, splits;                            // groups of four tiles of a pair, parts the other side is cut into
     int acc_q, acc_k, acc_v;
 };
-
-// The gradients of the scores have no bound to scale them by beforehand: a lane's column (a key, or a query's row) has a power of
-// two F of its own that puts its largest |x| into [2^11, 2^12) when it first shows or passes 2^15, and its sums are brought along.
-__device__ __forceinline__ bool column_scale(float most, float &F, float &by) {
-    by = 1.0f;
-    const bool over = most * F > 32768.0f;
-    if (over) {
-        int e = (int)(__float_as_uint(most) >> 23);
-        e = e < 12 ? 12 : e;
-        const float f = __uint_as_float((uint32_t)(127 + 11 + 127 - e) << 23);
-        by = f / F;
-        F = f;
-    }
-    return __any(over);
-}
-
-template <int NT>
-__device__ __forceinline__ void scale_acc(f16x (&acc)[NT], float by) {
-#pragma unroll
-    for (int d = 0; d < NT; d++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) acc[d][r] *= by;
-}
-
-template <int NT>
-__device__ __forceinline__ void store_column(float *row, const f16x (&acc)[NT], float by, int half, int D, int add) {
-#pragma unroll
-    for (int d = 0; d < NT; d++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            store4(row, 32 * d + 8 * j + 4 * half, D,
-                   f4{acc[d][4 * j] * by, acc[d][4 * j + 1] * by, acc[d][4 * j + 2] * by, acc[d][4 * j + 3] * by}, add);
-}
 
 // gk and gv: a wave holds 32 keys as columns and goes over the tiles of queries: s = q k^T and dp = go v^T, whose rows are queries,
 // then gv^T += go^T p and gk^T += q^T ds with p and ds as they lie.  Padded rows of queries have an infinite log-sum-exp: p = 0.
@@ -695,8 +541,8 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
         if (key < a.Lk) {
             const int64_t at = ((b * a.Lk + key) * a.Hkv + u) * a.D;
             const bool some = live && t0 < t1;
-            if (f.gk) store_column(f.gk + split * f.part_k + at, dk, some ? a.scale / F : 0.0f, half, (int)a.D, f.acc_k);
-            if (f.gv) store_column(f.gv + split * f.part_k + at, dv, some ? __builtin_amdgcn_exp2f(E - 14.0f) : 0.0f, half, (int)a.D, f.acc_v);
+            if (f.gk) store_column(f.gk + split * f.part_k + at, dk, some, a.scale / F, half, (int)a.D, f.acc_k);
+            if (f.gv) store_column(f.gv + split * f.part_k + at, dv, some, __builtin_amdgcn_exp2f(E - 14.0f), half, (int)a.D, f.acc_v);
         }
     }
 }
@@ -790,8 +636,10 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
             order_steps<2 * NT, 4>();
         }
         if (R < f.rows) {
-            const int64_t i = R / a.G, h = u * a.G + (R - i * a.G);
-            store_column(f.gq + split * f.part_q + ((b * a.Lq + i) * a.Hq + h) * a.D, dq, t0 < t1 ? a.scale / F : 0.0f, half, (int)a.D, f.acc_q);
+            int64_t i, g;
+            a.row(R, i, g);
+            const int64_t h = u * a.G + g;
+            store_column(f.gq + split * f.part_q + ((b * a.Lq + i) * a.Hq + h) * a.D, dq, t0 < t1, a.scale / F, half, (int)a.D, f.acc_q);
         }
     }
 }
@@ -813,7 +661,8 @@ static int attn_args(const char *what, AttnArgs &a, int64_t B, int64_t Lq, int64
     if (Lq > INT32_MAX || Lk > INT32_MAX || Hq > INT32_MAX || B > INT32_MAX) return set_error(NC_HIP_ERR_ARG, "%s: sizes past 2^31", what);
     if (!isfinite(scale)) return set_error(NC_HIP_ERR_ARG, "%s: the scale must be finite", what);
     if (!sq || !sk || !sv) return set_error(NC_HIP_ERR_ARG, "%s: strides are needed", what);
-    a = {B, Lq, Lk, Hq, Hkv, D, Hq / Hkv, {sq[0], sq[1], sq[2]}, {sk[0], sk[1], sk[2]}, {sv[0], sv[1], sv[2]}, scale};
+    const int64_t G = Hq / Hkv;
+    a = {B, Lq, Lk, Hq, Hkv, D, G, {sq[0], sq[1], sq[2]}, {sk[0], sk[1], sk[2]}, {sv[0], sv[1], sv[2]}, scale, G * Lq <= INT32_MAX, IntDiv((uint32_t)G)};
     return NC_HIP_OK;
 }
 
@@ -846,7 +695,7 @@ static int attn_splits(int64_t whole, int64_t tiles, int64_t want) {
 constexpr int64_t kTokenRows = 8;  // rows of a pair that k_attn_token takes
 
 struct FwdPlan {
-    bool token;
+    bool token, few;  // k_attn_token; few keys
     int DP, qtiles, splits;
     int64_t rows, tiles, pairs, units;
     size_t kp, vp, kx, vx, po, pm, total;  // offsets into the workspace
@@ -860,6 +709,15 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
     p.tiles = (Lk + kTile - 1) / kTile;
     p.qtiles = (int)((p.rows + kAttnWaves * kTile - 1) / (kAttnWaves * kTile));
     p.token = p.rows <= kTokenRows;
+    p.few = !p.token && Lk <= short_keys_fwd(p.DP);
+    if (p.few) {  // two workgroups a CU, with a tile of queries for each of their eight waves
+        const int64_t tiles = (p.rows + kTile - 1) / kTile;
+        int64_t parts = p.pairs ? 2 * kPlanCUs / p.pairs : 1;
+        if (parts > tiles / 8) parts = tiles / 8;
+        p.splits = (int)(parts < 1 ? 1 : parts);
+        p.units = p.pairs * p.splits;
+        return p;
+    }
     if (p.token) p.qtiles = 1;
     const int64_t whole = p.pairs * p.qtiles;
     p.splits = attn_splits(whole, p.tiles, (p.token ? 8 : 2) * kPlanCUs);
@@ -946,11 +804,16 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
         return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, p.total);
     hipStream_t st = as_stream(stream);
     char *const w = (char *)ws;
+    if (p.few) {
+        const ShortFwd f{a, q, k, v, key_len, o, lse, p.rows, (p.rows + kTile - 1) / kTile, p.units, (int)p.tiles, p.splits};
+        short_fwd(f, p.DP, st);
+        return check_launch(what);
+    }
     if (Lk && !p.token) {
         PackArgs pk{};
-        pk.Lk = Lk, pk.Hkv = Hkv, pk.D = (int)D, pk.key_len = key_len, pk.jobs = 2;
-        pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, 1, w + p.kp, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
-        pk.job[1] = {v, sv[0], sv[1], sv[2], Lk, p.tiles, 1, 1, w + p.vp, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
+        pk.a = a, pk.key_len = key_len, pk.jobs = 2;
+        pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, w + p.kp, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
+        pk.job[1] = {v, sv[0], sv[1], sv[2], Lk, p.tiles, 1, w + p.vp, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
         pack_launch(pk, p.pairs, p.DP, st);
     }
     FwdArgs f{a, q, w + p.kp, w + p.vp, (float *)(w + p.kx), (float *)(w + p.vx), key_len, o, lse, (float *)(w + p.po), (f2 *)(w + p.pm),
@@ -968,6 +831,7 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
 namespace nchip {
 
 struct BwdPlan {
+    bool few;
     int DP, qgroups, kgroups, qsplits, ksplits;  // splits of the keys for gq, of the queries for gk and gv
     int64_t rows, qtiles, ktiles, pairs, nq, nk;
     size_t kp, vp, qp, gp, kx, vx, qx, gx, stats, pq, pk, pv, total;
@@ -987,16 +851,22 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
     p.ksplits = attn_splits(p.pairs * p.kgroups, p.qtiles, want);
     p.nq = B * Lq * Hq * D;
     p.nk = B * Lk * Hkv * D;
+    p.few = Lk <= short_keys_bwd(p.DP);
+    if (p.few) {  // a workgroup of eight waves a CU, or two of four, with two tiles of queries at least
+        int64_t parts = p.pairs ? (p.ktiles <= 4 && p.DP <= 64 ? 2 : 1) * kPlanCUs / p.pairs : 1;
+        if (parts > p.qtiles / 2) parts = p.qtiles / 2;
+        p.ksplits = (int)(parts < 1 ? 1 : parts);
+    }
     size_t at = 0;
     auto take = [&](int64_t bytes) {
         const size_t here = at;
         at += up256((size_t)bytes);
         return here;
     };
-    const int64_t q = p.pairs * p.qtiles, k = p.pairs * p.ktiles, tb = tile_bytes(p.DP);
+    const int64_t q = p.few ? 0 : p.pairs * p.qtiles, k = p.few ? 0 : p.pairs * p.ktiles, tb = tile_bytes(p.DP);
     p.kp = take(k * tb), p.vp = take(k * tb), p.qp = take(q * tb), p.gp = take(q * tb);
     p.kx = take(k * 4), p.vx = take(k * 4), p.qx = take(q * 4), p.gx = take(q * 4), p.stats = take(q * 256);
-    if (p.qsplits > 1) p.pq = take(p.qsplits * p.nq * 4);
+    if (p.qsplits > 1 && !p.few) p.pq = take(p.qsplits * p.nq * 4);
     if (p.ksplits > 1) p.pk = take(p.ksplits * p.nk * 4), p.pv = take(p.ksplits * p.nk * 4);
     p.total = at;
     return p;
@@ -1033,6 +903,15 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
         return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, p.total);
     hipStream_t st = as_stream(stream);
     char *const w = (char *)ws;
+    if (p.few) {
+        const bool cut = p.ksplits > 1;
+        ShortBwd f{a, q, k, v, key_len, o, lse, go, want_q ? gq : nullptr, cut && gk ? (float *)(w + p.pk) : gk, cut && gv ? (float *)(w + p.pv) : gv,
+                   p.rows, p.qtiles, p.pairs * p.ksplits, p.nk, p.ksplits, acc_q, cut ? 0 : acc_k, cut ? 0 : acc_v};
+        short_bwd(f, p.DP, st);
+        if (cut && want_k && gk) sum_launch(p.nk, p.ksplits, f.gk, gk, acc_k, st);
+        if (cut && want_k && gv) sum_launch(p.nk, p.ksplits, f.gv, gv, acc_v, st);
+        return check_launch(what);
+    }
     BwdArgs f{};
     f.a = a;
     f.kp = w + p.kp, f.vp = w + p.vp, f.qp = w + p.qp, f.gp = w + p.gp;
@@ -1041,15 +920,14 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
     f.key_len = key_len;
     f.rows = p.rows, f.qtiles = p.qtiles, f.ktiles = p.ktiles;
     PackArgs pk{};
-    pk.Lk = Lk, pk.Hkv = Hkv, pk.D = (int)D, pk.key_len = key_len;
-    const int64_t G = a.G;
+    pk.a = a, pk.key_len = key_len;
     if (Lk) {
-        pk.job[pk.jobs++] = {k, sk[0], sk[1], sk[2], Lk, p.ktiles, 1, 1, w + p.kp, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
-        pk.job[pk.jobs++] = {v, sv[0], sv[1], sv[2], Lk, p.ktiles, 1, 1, w + p.vp, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {k, sk[0], sk[1], sk[2], Lk, p.ktiles, 1, w + p.kp, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {v, sv[0], sv[1], sv[2], Lk, p.ktiles, 1, w + p.vp, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
     }
     if (Lq) {
-        pk.job[pk.jobs++] = {q, sq[0], sq[1], sq[2], p.rows, p.qtiles, (int)G, 0, w + p.qp, (float *)(w + p.qx), 0, nullptr, nullptr, nullptr};
-        pk.job[pk.jobs++] = {go, Lq * Hq * D, Hq * D, D, p.rows, p.qtiles, (int)G, 0, w + p.gp, (float *)(w + p.gx), 0, o, lse, (float *)(w + p.stats)};
+        pk.job[pk.jobs++] = {q, sq[0], sq[1], sq[2], p.rows, p.qtiles, 0, w + p.qp, (float *)(w + p.qx), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {go, Lq * Hq * D, Hq * D, D, p.rows, p.qtiles, 0, w + p.gp, (float *)(w + p.gx), 0, o, lse, (float *)(w + p.stats)};
     }
     pack_launch(pk, p.pairs, p.DP, st);
     if (want_q) {

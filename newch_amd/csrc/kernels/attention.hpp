@@ -17,12 +17,35 @@
 #pragma once
 
 #include "common.hpp"
+#include "intdiv.hpp"
 
 namespace nchip {
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f16x __attribute__((ext_vector_type(16)));
+
+constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
+
+struct AttnArgs {
+    int64_t B, Lq, Lk, Hq, Hkv, D, G;  // G: query heads of a key head
+    int64_t sq[3], sk[3], sv[3];
+    float scale;
+    bool narrow;   // fewer than 2^31 rows of a pair
+    IntDiv by_g;
+
+    // row R of a pair: token and, among the heads that share the pair's keys, head
+    __device__ __forceinline__ void row(int64_t R, int64_t &i, int64_t &g) const {
+        if (G == 1) {
+            i = R, g = 0;
+        } else if (narrow) {
+            const uint32_t q = by_g.div31((uint32_t)R);
+            i = q, g = (uint32_t)R - q * (uint32_t)G;
+        } else {
+            i = R / G, g = R - i * G;
+        }
+    }
+};
 
 constexpr int kAttnD = 256;       // columns at most
 constexpr int kAttnB = 256;       // lanes of a workgroup
@@ -97,19 +120,32 @@ __device__ __forceinline__ int tile_exponent(float most) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
+// four columns of a row of D >= 4 from d on, zeros from column D on: the row's last four, moved down, where it ends among them
+__device__ __forceinline__ f4 last4(const float *row, int d, int D) {
+    const int o = min(d, D - 4), by = d - o;
+    f4 v = *(const f4u *)(row + o);
+    if (by & 1) v = f4{v[1], v[2], v[3], 0.0f};
+    if (by & 2) v = f4{v[2], v[3], 0.0f, 0.0f};
+    if (by & ~3) v = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    return v;
+}
+
 // eight columns of a row from d on, zeros from column D on
 __device__ __forceinline__ void load8(const float *row, int d, int D, float *x) {
+    f4 p = {0.0f, 0.0f, 0.0f, 0.0f}, q = p;
     if (d + 8 <= D) {
-        const f4 p = *(const f4u *)(row + d), q = *(const f4u *)(row + d + 4);
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = p[i], x[4 + i] = q[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float v = row[d + i < D ? d + i : D - 1];
-            x[i] = d + i < D ? v : 0.0f;
-        }
+        p = *(const f4u *)(row + d);
+        q = *(const f4u *)(row + d + 4);
+    } else if (d < D && D >= 4) {
+        p = last4(row, d, D);
+        q = last4(row, d + 4, D);
+    } else if (d < D) {  // a row of one to three columns
+        p[0] = row[0];
+        if (D > 1) p[1] = row[1];
+        if (D > 2) p[2] = row[2];
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = p[i], x[4 + i] = q[i];
 }
 
 // four columns of a contiguous row from d on, stored or added
@@ -122,6 +158,175 @@ __device__ __forceinline__ void store4(float *row, int d, int D, f4 v, int acc) 
         for (int i = 0; i < 3; i++)
             if (d + i < D) row[d + i] = acc ? row[d + i] + v[i] : v[i];
     }
+}
+
+__device__ __forceinline__ int64_t keys_of(int64_t Lk, const int *key_len, int64_t b) {
+    if (!key_len) return Lk;
+    const int64_t n = key_len[b];
+    return n < 0 ? 0 : n < Lk ? n : Lk;
+}
+
+// The order of a block of N steps, each R reads of fragments from LDS and three products: reads two steps ahead of their products.
+template <int N, int R>
+__device__ __forceinline__ void order_steps() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * R, 0);
+#pragma unroll
+    for (int i = 0; i < N - 2; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+}
+
+// Workgroups are dealt round robin over the 8 XCDs: consecutive units of a launch go to one XCD, which then keeps their
+// keys in its L2.
+__device__ __forceinline__ int64_t xcd_unit(int64_t w, int64_t units) {
+    const int64_t each = units / 8, rest = units % 8, x = w % 8, k = w / 8;
+    return x * each + (x < rest ? x : rest) + k;
+}
+
+// The gradients of the scores have no bound to scale them by beforehand: a lane's column (a key, or a query's row) has a power of
+// two F of its own that puts its largest |x| into [2^11, 2^12) when it first shows or passes 2^15, and its sums are brought along.
+__device__ __forceinline__ bool column_scale(float most, float &F, float &by) {
+    by = 1.0f;
+    const bool over = most * F > 32768.0f;
+    if (over) {
+        int e = (int)(__float_as_uint(most) >> 23);
+        e = e < 12 ? 12 : e;
+        const float f = __uint_as_float((uint32_t)(127 + 11 + 127 - e) << 23);
+        by = f / F;
+        F = f;
+    }
+    return __any(over);
+}
+
+template <int NT>
+__device__ __forceinline__ void scale_acc(f16x (&acc)[NT], float by) {
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[d][r] *= by;
+}
+
+// a lane's column as a row of the output, `by` times; zeros where it holds nothing that counts
+template <int NT>
+__device__ __forceinline__ void store_column(float *row, const f16x (&acc)[NT], bool some, float by, int half, int D, int add) {
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            f4 v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = some ? acc[d][4 * j + e] * by : 0.0f;
+            store4(row, 32 * d + 8 * j + 4 * half, D, v, add);
+        }
+}
+
+// ------------------------------------------------------------------------------------------------
+// forward: a wave's 32 rows of queries against a tile of keys
+// ------------------------------------------------------------------------------------------------
+// A wave holds 32 rows of queries as columns: s^T = k q^T (A: 32 keys), so that a row's scores lie in the registers of two lanes
+// and its maximum, sum and scale are theirs; p^T is then the operand of o^T = v^T p^T as it lies.  One pass over the keys: the
+// reference m a row's exponents are taken from moves only when a score passes it by 2^4, and o and the sum with it; p is held as
+// 2^10 p (at most 2^14) in two fp16, so a p below 2^-13 loses low bits against an absolute 2^-35.
+constexpr float kPShift = 10.0f, kPSlack = 4.0f;
+
+template <int DP>
+struct Query {  // the rows times scale log2(e), as the second operand: column fragments of q^T
+    h8 hi[DP / 16], lo[DP / 16];
+    float c;  // 2^ its exponent
+};
+
+template <int DP>
+__device__ __forceinline__ void load_query(Query<DP> &q, const float *row, bool live, float scale, int half, int D) {
+    const float c = live ? scale * kLog2e : 0.0f;
+    float most = 0.0f, x[8];
+#pragma unroll
+    for (int s = 0; s < DP / 16; s++) {
+        load8(row, 16 * s + 8 * half, D, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[e] * c));
+    }
+    const int e = tile_exponent(halves_max(most));
+    const float inv = pow2i(-e);
+    q.c = pow2i(e);
+    asm volatile("" ::: "memory");  // the row is read again (from the caches) rather than held in fp32 as well
+#pragma unroll
+    for (int s = 0; s < DP / 16; s++) {
+        load8(row, 16 * s + 8 * half, D, x);
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = live ? x[k] * c * inv : 0.0f;
+        const Split8 p = split8(x);
+        q.hi[s] = p.hi, q.lo[s] = p.lo;
+    }
+}
+
+template <int DP>
+struct Sums {
+    f16x o[DP / 32];
+    float m, l, E;  // reference, sum of 2^kPShift p, exponent of o
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
+        m = -INFINITY, l = 0.0f, E = -1000.0f;
+    }
+};
+
+// kt, vt: the tile's keys and values in LDS, at this lane's row_at and col_at; ek, ev: their exponents; left: keys of the tile
+// that count (32 but in the last one), less 4 half
+template <int DP>
+__device__ __forceinline__ void attend(Sums<DP> &a, const Query<DP> &q, const char *kt, const char *vt, float ek, float ev, bool cut,
+                                       int left) {
+    constexpr int KS = DP / 16, NT = DP / 32, LO = 64 * DP;
+    f16x s;
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; k++) s = mfma3(row_frag(kt, k), row_frag(kt + LO, k), q.hi[k], q.lo[k], s);
+    order_steps<KS, 2>();
+    const float c = __builtin_fmaxf(q.c * pow2i((int)ek), 0x1p-126f);  // -inf * c stays -inf
+    if (cut) {
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            if (8 * (r / 4) + r % 4 >= left) s[r] = -INFINITY;
+    }
+    float top = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; r++) top = __builtin_fmaxf(top, s[r]);
+    top = halves_max(top) * c;
+    if (__any(top > a.m + kPSlack) || ev > a.E) {
+        const float mn = top > a.m + kPSlack ? top : a.m, En = __builtin_fmaxf(a.E, ev);
+        const float al = a.m == mn ? 1.0f : __builtin_amdgcn_exp2f(a.m - mn);
+        const float ao = al * __builtin_amdgcn_exp2f(a.E - En);
+        a.l *= al;
+        a.m = mn;
+        a.E = En;
+#pragma unroll
+        for (int d = 0; d < NT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) a.o[d][r] *= ao;
+    }
+    // values of smaller tiles count through smaller p (no smaller than 2^-60: below what o can show)
+    const float dv = __builtin_fmaxf(ev - a.E, -60.0f), off = kPShift + dv - a.m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        s[r] = __builtin_amdgcn_exp2f(fma_(s[r], c, off));
+        sum += s[r];
+    }
+    a.l = fma_(sum, __builtin_amdgcn_exp2f(-dv), a.l);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = s[8 * k + e];
+        const Split8 p = split8(y);
+#pragma unroll
+        for (int d = 0; d < NT; d++) a.o[d] = mfma3(col_frag(vt, k, d), col_frag(vt + LO, k, d), p.hi, p.lo, a.o[d]);
+    }
+    order_steps<2 * NT, 4>();
 }
 
 }  // namespace nchip
