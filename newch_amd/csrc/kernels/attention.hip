@@ -64,8 +64,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
             for (int e = 0; e < 8; e++) x[k][e] = 0.0f;
             const int c = cl + 8 * k;
             if (live && c < C) load8(src, 8 * c, (int)a.a.D, x[k]);
-#pragma unroll
-            for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[k][e]));
+            most = abs_max(x[k], most);
             if (j.stats && live && c < C) {
                 float y[8];
                 load8(j.o + off, 8 * c, (int)a.a.D, y);
@@ -108,9 +107,10 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
 // stages of tiles in LDS
 // ------------------------------------------------------------------------------------------------
 // blocks of 1 KiB dealt over the workgroup's waves, copied straight to LDS; nothing waits for them here
+template <int WAVES = kAttnWaves>
 __device__ __forceinline__ void stage_copy(const char *src, uint32_t lds, int blocks) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    for (int i = wave; i < blocks; i += kAttnWaves) dma16(src + i * 1024 + lane * 16, lds + i * 1024);
+    for (int i = wave; i < blocks; i += WAVES) dma16(src + i * 1024 + lane * 16, lds + i * 1024);
 }
 __device__ __forceinline__ void stage_wait() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's copies and LDS reads
@@ -198,12 +198,12 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
         const float l = halves_sum(sum.l);
         if (live && f.splits == 1) {
             // no keys: o is zero
-            store_column(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, l != 0.0f, pow2i((int)sum.E) / l, half, (int)a.D, 0);
+            store_column<false>(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, true, l != 0.0f ? pow2i((int)sum.E) / l : 0.0f, half, (int)a.D, 0);
             if (f.lse && half == 0)
                 f.lse[(b * a.Hq + h) * a.Lq + i] = nt ? fma_(sum.m - kPShift, kLn2, logf(l)) : -INFINITY;
         } else if (live) {
             const int64_t pr = ((int64_t)split * a.B * a.Hkv + pair) * f.rows + R;
-            store_column(f.po + pr * a.D, sum.o, t0 < t1, pow2i((int)sum.E), half, (int)a.D, 0);
+            store_column<true>(f.po + pr * a.D, sum.o, t0 < t1, pow2i((int)sum.E), half, (int)a.D, 0);
             if (half == 0) f.pm[pr] = f2{t0 < t1 ? sum.m - kPShift : -INFINITY, l};
         }
     }
@@ -381,9 +381,9 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
     }
 }
 
-// The splits' parts of a row joined: a part counts by 2^(its reference - the largest).  A wave a row: lane s has part s's
-// reference and sum, then every lane 64th column.
-__global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t rows, int splits, const float *po, const f2 *pm,
+// The splits' parts of a row joined: a part counts by 2^(its reference - the largest).  A wave a row, where there are few: lane s
+// has part s's reference and sum, then every lane 64th column.
+__global__ __launch_bounds__(kAttnB) void k_attn_join_rows(const AttnArgs a, int64_t rows, int splits, const float *po, const f2 *pm,
                                                       float *o, float *lse) {
     const int64_t all = a.B * a.Hkv * rows;
     const int lane = threadIdx.x & 63;
@@ -418,6 +418,47 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
     }
 }
 
+// the same for many rows in up to eight parts: a lane four columns of a row
+__global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t rows, int splits, const float *po, const f2 *pm,
+                                                      float *o, float *lse) {
+    const int64_t all = a.B * a.Hkv * rows, D4 = (a.D + 3) / 4;
+    for (int64_t x = (int64_t)blockIdx.x * kAttnB + threadIdx.x; x < all * D4; x += (int64_t)gridDim.x * kAttnB) {
+        const int64_t pr = x / D4, pair = pr / rows, R = pr - pair * rows, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int d = (int)(x - pr * D4) * 4;
+        int64_t i, g;
+        a.row(R, i, g);
+        const int64_t h = u * a.G + g;
+        f2 ml[8];
+        f4 p[8];
+        float M = -INFINITY, l = 0.0f;
+        bool nan = false;
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            const int64_t at = min(s, splits - 1) * all + pr;
+            ml[s] = pm[at];
+            p[s] = a.D >= 4 ? last4(po + at * a.D, d, (int)a.D) : f4{po[at * a.D], po[at * a.D + (a.D > 1)], po[at * a.D + a.D - 1], 0.0f};
+        }
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            if (s >= splits) ml[s] = f2{-INFINITY, 0.0f};
+            nan = nan || ml[s].x != ml[s].x;
+            M = __builtin_fmaxf(M, ml[s].x);
+        }
+        f4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            if (ml[s].x == -INFINITY) continue;  // a part without keys
+            const float w = __builtin_amdgcn_exp2f(ml[s].x - M);
+            l = fma_(w, ml[s].y, l);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] = fma_(w, p[s][e], sum[e]);
+        }
+        const float inv = nan ? NAN : l != 0.0f ? 1.0f / l : 0.0f;
+        store4(o + ((b * a.Lq + i) * a.Hq + h) * a.D, d, (int)a.D, sum * inv, 0);
+        if (lse && d == 0) lse[(b * a.Hq + h) * a.Lq + i] = M == -INFINITY ? -INFINITY : fma_(M, kLn2, logf(l));
+    }
+}
+
 // ------------------------------------------------------------------------------------------------
 // backward: two kernels, each with its own recomputed scores, so that every gradient is summed in one place and order
 // ------------------------------------------------------------------------------------------------
@@ -432,17 +473,22 @@ struct BwdArgs {
     int acc_q, acc_k, acc_v;
 };
 
-// gk and gv: a wave holds 32 keys as columns and goes over the tiles of queries: s = q k^T and dp = go v^T, whose rows are queries,
-// then gv^T += go^T p and gk^T += q^T ds with p and ds as they lie.  Padded rows of queries have an infinite log-sum-exp: p = 0.
+// gk and gv: two waves share 32 keys as columns and go over the tiles of queries.  One takes s = q k^T and p, whose rows are queries,
+// hands p over through LDS and sums gv^T += go^T p; the other takes dp = go v^T, makes ds of it and sums gk^T += q^T ds.  Each keeps
+// half of the fragments and of the sums, so that two waves fit a SIMD: one's exponentials run under the other's products (128
+// columns: 0.90 -> XX ms of the 2048 x 4096 backward against one wave that does both).  Padded rows of queries have an infinite
+// log-sum-exp: p = 0.
 template <int DP, int OCC>
-__global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
+__global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * TB + 256;
-    constexpr bool REG = DP <= 128;  // keys and values stay in registers, else they are read again for every tile
+    constexpr bool REG = DP <= 128;  // keys or values stay in registers, else they are read again for every tile
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int which = wave & (kAttnWaves - 1), ds_wave = wave / kAttnWaves;  // tile of keys; 0: p and gv, 1: ds and gk
     const int ra = row_at(lane), ca = col_at(lane);
     const uint32_t lds = lds_address(smem);
+    f4 *const hand = (f4 *)(smem + 2 * STAGE) + which * 256 + lane;  // p's registers 4 j .. 4 j + 3 at 64 j
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
         const int kg = (int)(unit % f.groups);
@@ -450,100 +496,103 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
         const int split = (int)(rest % f.splits);
         const int64_t pair = rest / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
         const int64_t n = keys_of(a.Lk, f.key_len, b);
-        const int64_t k0 = (int64_t)kg * kAttnWaves + wave, key = k0 * kTile + (lane & 31);
+        const int64_t k0 = (int64_t)kg * kAttnWaves + which, key = k0 * kTile + (lane & 31);
         const bool any = (int64_t)kg * kAttnWaves * kTile < n, mine = k0 * kTile < n, live = key < n;
         const int64_t t0 = any ? f.qtiles * split / f.splits : 0, t1 = any ? f.qtiles * (split + 1) / f.splits : 0;
         const int64_t q0 = pair * f.qtiles;
         auto copy = [&](int64_t t, int buf) {
             const uint32_t at = __builtin_amdgcn_readfirstlane(lds + buf * STAGE);
             const int64_t x = (q0 + t) * TB;
-            stage_copy(f.qp + x, at, TB / 1024);
-            stage_copy(f.gp + x, at + TB, TB / 1024);
+            stage_copy<2 * kAttnWaves>(f.qp + x, at, TB / 1024);
+            stage_copy<2 * kAttnWaves>(f.gp + x, at + TB, TB / 1024);
             if (threadIdx.x < 16) dma16(f.stats + (q0 + t) * 64 + threadIdx.x * 4, at + 2 * TB);
         };
         __syncthreads();  // the last unit's stages have been read
         if (t0 < t1) copy(t0, 0);
         const int64_t tile = pair * f.ktiles + (mine ? k0 : 0);
-        const char *kt = f.kp + tile * TB + ra, *vt = f.vp + tile * TB + ra;
-        h8 kh[REG ? KS : 1], kl[REG ? KS : 1], vh[REG ? KS : 1], vl[REG ? KS : 1];
-        float ck = 0.0f, cv = 0.0f;
+        const char *kt = (ds_wave ? f.vp : f.kp) + tile * TB + ra;
+        h8 kh[REG ? KS : 1], kl[REG ? KS : 1];
+        float ck = 0.0f;
         if (mine) {
-            ck = pow2i((int)f.kx[tile]) * a.scale * kLog2e;
-            cv = pow2i((int)f.vx[tile]);
+            ck = ds_wave ? pow2i((int)f.vx[tile]) : pow2i((int)f.kx[tile]) * a.scale * kLog2e;
             if constexpr (REG) {
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    kh[s] = row_frag(kt, s), kl[s] = row_frag(kt + LO, s);
-                    vh[s] = row_frag(vt, s), vl[s] = row_frag(vt + LO, s);
-                }
+                for (int s = 0; s < KS; s++) kh[s] = row_frag(kt, s), kl[s] = row_frag(kt + LO, s);
             }
         }
-        f16x dk[NT], dv[NT];
+        f16x acc[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) dk[t][r] = dv[t][r] = 0.0f;
+            for (int r = 0; r < 16; r++) acc[t][r] = 0.0f;
         float F = 0x1p100f, E = -1000.0f;
         for (int64_t t = t0, buf = 0; t < t1; t++, buf ^= 1) {
             const float ex = scalar_load(f.gx + q0 + t), eq = scalar_load(f.qx + q0 + t);
             stage_wait();
             if (t + 1 < t1) copy(t + 1, (int)buf ^ 1);
             const char *st = smem + buf * STAGE;
-            if (!mine) continue;
-            const char *qt = st + ra, *gt = st + TB + ra, *qc = st + ca, *gc = st + TB + ca;
             const f4 *rows = (const f4 *)(st + 2 * TB) + half;
-            f16x s, dp;
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                s = mfma3(row_frag(qt, k), row_frag(qt + LO, k), REG ? kh[k] : row_frag(kt, k), REG ? kl[k] : row_frag(kt + LO, k), s);
-                dp = mfma3(row_frag(gt, k), row_frag(gt + LO, k), REG ? vh[k] : row_frag(vt, k), REG ? vl[k] : row_frag(vt + LO, k), dp);
-            }
-            if constexpr (REG) order_steps<2 * KS, 2>();
-            if (ex > E) {
-                scale_acc(dv, __builtin_amdgcn_exp2f(E - ex));
-                E = ex;
-            }
             // p as 2^14 p, less for tiles of smaller gradients (no less than 2^-60 times: below what gv can show)
-            const float sh = 14.0f + __builtin_fmaxf(ex - E, -60.0f), base = live ? sh : -INFINITY;
-            const float c = ck * pow2i((int)eq), c2 = cv * pow2i((int)ex);
-            float most = 0.0f;
+            const float En = __builtin_fmaxf(E, ex), sh = 14.0f + __builtin_fmaxf(ex - En, -60.0f);
+            f16x s;
+            if (mine) {
+                const char *rt = st + ds_wave * TB + ra;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const f4 ls = rows[2 * j], de = rows[8 + 2 * j];
+                for (int r = 0; r < 16; r++) s[r] = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int r = 4 * j + e;
-                    s[r] = __builtin_amdgcn_exp2f(fma_(s[r], c, base - ls[e]));
-                    dp[r] = s[r] * fma_(dp[r], c2, -de[e]);
-                    most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
+                for (int k = 0; k < KS; k++)
+                    s = mfma3(row_frag(rt, k), row_frag(rt + LO, k), REG ? kh[k] : row_frag(kt, k), REG ? kl[k] : row_frag(kt + LO, k), s);
+                if constexpr (REG) order_steps<KS, 2>();
+                if (!ds_wave) {
+                    if (ex > E) scale_acc(acc, __builtin_amdgcn_exp2f(E - ex));
+                    const float c = ck * pow2i((int)eq), base = live ? sh : -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const f4 ls = rows[2 * j];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[4 * j + e] = __builtin_amdgcn_exp2f(fma_(s[4 * j + e], c, base - ls[e]));
+                        hand[64 * j] = f4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
+                    }
                 }
             }
-            const float kap = __builtin_amdgcn_exp2f(eq - sh);
-            float by;
-            if (column_scale(halves_max(most) * kap, F, by)) scale_acc(dk, by);
-            const float kF = kap * F;
+            E = En;
+            lds_barrier();  // p is there (the next stage's copies stay on their way)
+            if (!mine) continue;
+            if (ds_wave) {
+                const float c = ck * pow2i((int)ex), kap = __builtin_amdgcn_exp2f(eq - sh);
+                float most = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const f4 p = hand[64 * j], de = rows[8 + 2 * j];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int r = 4 * j + e;
+                        s[r] = p[e] * fma_(s[r], c, -de[e]);
+                        most = __builtin_fmaxf(most, __builtin_fabsf(s[r]));
+                    }
+                }
+                float by;
+                if (column_scale(halves_max(most) * kap, F, by)) scale_acc(acc, by);
+                const float kF = kap * F;
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] *= kF;
+            }
+            const char *ct = st + (ds_wave ? 0 : TB) + ca;
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                float y[8], z[8];
+                float y[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = s[8 * k + e], z[e] = dp[8 * k + e] * kF;
-                const Split8 ps = split8(y), ds = split8(z);
+                for (int e = 0; e < 8; e++) y[e] = s[8 * k + e];
+                const Split8 ps = split8(y);
 #pragma unroll
-                for (int d = 0; d < NT; d++) {
-                    dv[d] = mfma3(col_frag(gc, k, d), col_frag(gc + LO, k, d), ps.hi, ps.lo, dv[d]);
-                    dk[d] = mfma3(col_frag(qc, k, d), col_frag(qc + LO, k, d), ds.hi, ds.lo, dk[d]);
-                }
+                for (int d = 0; d < NT; d++) acc[d] = mfma3(col_frag(ct, k, d), col_frag(ct + LO, k, d), ps.hi, ps.lo, acc[d]);
             }
-            order_steps<4 * NT, 4>();
+            order_steps<2 * NT, 4>();
         }
-        if (key < a.Lk) {
-            const int64_t at = ((b * a.Lk + key) * a.Hkv + u) * a.D;
-            const bool some = live && t0 < t1;
-            if (f.gk) store_column(f.gk + split * f.part_k + at, dk, some, a.scale / F, half, (int)a.D, f.acc_k);
-            if (f.gv) store_column(f.gv + split * f.part_k + at, dv, some, __builtin_amdgcn_exp2f(E - 14.0f), half, (int)a.D, f.acc_v);
-        }
+        float *const out = ds_wave ? f.gk : f.gv;
+        if (out && key < a.Lk)
+            store_column<true>(out + split * f.part_k + ((b * a.Lk + key) * a.Hkv + u) * a.D, acc, live && t0 < t1,
+                               ds_wave ? a.scale / F : __builtin_amdgcn_exp2f(E - 14.0f), half, (int)a.D, ds_wave ? f.acc_k : f.acc_v);
     }
 }
 
@@ -639,17 +688,32 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
             int64_t i, g;
             a.row(R, i, g);
             const int64_t h = u * a.G + g;
-            store_column(f.gq + split * f.part_q + ((b * a.Lq + i) * a.Hq + h) * a.D, dq, t0 < t1, a.scale / F, half, (int)a.D, f.acc_q);
+            store_column<true>(f.gq + split * f.part_q + ((b * a.Lq + i) * a.Hq + h) * a.D, dq, t0 < t1, a.scale / F, half, (int)a.D, f.acc_q);
         }
     }
 }
 
-// out (+)= the splits' parts, in order
-__global__ __launch_bounds__(kAttnB) void k_attn_sum(int64_t n, int splits, const float *part, float *out, int acc) {
-    for (int64_t i = (int64_t)blockIdx.x * kAttnB + threadIdx.x; i < n; i += (int64_t)gridDim.x * kAttnB) {
-        float s = part[i];
-        for (int k = 1; k < splits; k++) s += part[k * n + i];
-        out[i] = acc ? out[i] + s : s;
+// out (+)= the splits' parts [split][n], in order; one or two tensors of one size
+struct SumArgs {
+    const float *part[2];
+    float *out[2];
+    int acc[2];
+    int64_t n;
+    int splits;
+};
+__global__ __launch_bounds__(kAttnB) void k_attn_sum(const SumArgs a) {
+    const float *part = a.part[blockIdx.y];
+    float *out = a.out[blockIdx.y];
+    for (int64_t i = (int64_t)blockIdx.x * kAttnB + threadIdx.x; i < a.n; i += (int64_t)gridDim.x * kAttnB) {
+        float s = 0.0f;
+        for (int k = 0; k < a.splits; k += 8) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = k + e < a.splits ? part[(k + e) * a.n + i] : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) s += x[e];
+        }
+        out[i] = a.acc[blockIdx.y] ? out[i] + s : s;
     }
 }
 
@@ -746,9 +810,9 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
 static unsigned attn_grid(int64_t units) { return (unsigned)(units < kAttnGrid ? units : kAttnGrid); }
 
 template <class F, class A>
-static void attn_launch(F *kernel, int64_t units, size_t lds, hipStream_t st, const A &args) {
+static void attn_launch(F *kernel, int64_t units, size_t lds, hipStream_t st, const A &args, int threads = kAttnB) {
     if (lds > 65536) (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    hipLaunchKernelGGL(kernel, dim3(attn_grid(units)), dim3(kAttnB), lds, st, args);
+    hipLaunchKernelGGL(kernel, dim3(attn_grid(units)), dim3(threads), lds, st, args);
 }
 
 template <int NR, int LPK>
@@ -823,8 +887,12 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     else
         NC_ATTN_DP(p.DP, constexpr int TPS = DP <= 64 ? 2 : 1; constexpr int OCC = DP <= 128 ? 2 : 1;
                    attn_launch(&k_attn_fwd<DP, TPS, OCC>, p.units, 2 * 2 * TPS * 128 * DP, st, f));
-    if (p.splits > 1)
-        hipLaunchKernelGGL(k_attn_join, dim3(attn_grid((p.pairs * p.rows + kAttnWaves - 1) / kAttnWaves)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, o, lse);
+    // a wave a row while that fills the chip at most twice over, or for more than eight parts
+    const int64_t all = p.pairs * p.rows, pieces = all * ((D + 3) / 4);
+    if (p.splits > 8 || (p.splits > 1 && all <= 16 * kPlanCUs))
+        hipLaunchKernelGGL(k_attn_join_rows, dim3(attn_grid((all + kAttnWaves - 1) / kAttnWaves)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, o, lse);
+    else if (p.splits > 1)
+        hipLaunchKernelGGL(k_attn_join, dim3(attn_grid((pieces + kAttnB - 1) / kAttnB)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, o, lse);
     return check_launch(what);
 }
 
@@ -846,9 +914,8 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
     p.ktiles = (Lk + kTile - 1) / kTile;
     p.qgroups = (int)((p.qtiles + kAttnWaves - 1) / kAttnWaves);
     p.kgroups = (int)((p.ktiles + kAttnWaves - 1) / kAttnWaves);
-    const int64_t want = kPlanCUs * (p.DP <= 64 ? 2 : 1);
-    p.qsplits = attn_splits(p.pairs * p.qgroups, p.ktiles, want);
-    p.ksplits = attn_splits(p.pairs * p.kgroups, p.qtiles, want);
+    p.qsplits = attn_splits(p.pairs * p.qgroups, p.ktiles, kPlanCUs * (p.DP <= 128 ? 2 : 1));
+    p.ksplits = attn_splits(p.pairs * p.kgroups, p.qtiles, kPlanCUs * (p.DP <= 64 ? 2 : 1));
     p.nq = B * Lq * Hq * D;
     p.nk = B * Lk * Hkv * D;
     p.few = Lk <= short_keys_bwd(p.DP);
@@ -872,8 +939,9 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
     return p;
 }
 
-static void sum_launch(int64_t n, int splits, const float *part, float *out, int acc, hipStream_t st) {
-    hipLaunchKernelGGL(k_attn_sum, dim3(attn_grid((n + kAttnB - 1) / kAttnB)), dim3(kAttnB), 0, st, n, splits, part, out, acc);
+static void sum_launch(int64_t n, int splits, const float *p0, float *o0, int acc0, const float *p1, float *o1, int acc1, hipStream_t st) {
+    SumArgs s{{o0 ? p0 : p1, p1}, {o0 ? o0 : o1, o1}, {o0 ? acc0 : acc1, acc1}, n, splits};
+    hipLaunchKernelGGL(k_attn_sum, dim3(attn_grid((n + kAttnB - 1) / kAttnB), o0 && o1 ? 2 : 1), dim3(kAttnB), 0, st, s);
 }
 
 }  // namespace nchip
@@ -908,8 +976,7 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
         ShortBwd f{a, q, k, v, key_len, o, lse, go, want_q ? gq : nullptr, cut && gk ? (float *)(w + p.pk) : gk, cut && gv ? (float *)(w + p.pv) : gv,
                    p.rows, p.qtiles, p.pairs * p.ksplits, p.nk, p.ksplits, acc_q, cut ? 0 : acc_k, cut ? 0 : acc_v};
         short_bwd(f, p.DP, st);
-        if (cut && want_k && gk) sum_launch(p.nk, p.ksplits, f.gk, gk, acc_k, st);
-        if (cut && want_k && gv) sum_launch(p.nk, p.ksplits, f.gv, gv, acc_v, st);
+        if (cut && want_k) sum_launch(p.nk, p.ksplits, f.gk, gk, acc_k, f.gv, gv, acc_v, st);
         return check_launch(what);
     }
     BwdArgs f{};
@@ -936,8 +1003,8 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
         f.acc_q = cut ? 0 : acc_q;
         f.part_q = p.nq, f.groups = p.qgroups, f.splits = p.qsplits;
         f.units = p.pairs * p.qgroups * p.qsplits;
-        NC_ATTN_DP(p.DP, constexpr int OCC = DP <= 64 ? 2 : 1; attn_launch(&k_attn_dq<DP, OCC>, f.units, 2 * 2 * 128 * DP, st, f));
-        if (cut) sum_launch(p.nq, p.qsplits, f.gq, gq, acc_q, st);
+        NC_ATTN_DP(p.DP, constexpr int OCC = DP <= 128 ? 2 : 1; attn_launch(&k_attn_dq<DP, OCC>, f.units, 2 * 2 * 128 * DP, st, f));
+        if (cut) sum_launch(p.nq, p.qsplits, f.gq, gq, acc_q, nullptr, nullptr, 0, st);
     }
     if (want_k) {
         const bool cut = p.ksplits > 1;
@@ -947,10 +1014,9 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
         f.acc_v = cut ? 0 : acc_v;
         f.part_k = p.nk, f.groups = p.kgroups, f.splits = p.ksplits;
         f.units = p.pairs * p.kgroups * p.ksplits;
-        NC_ATTN_DP(p.DP, constexpr int OCC = DP <= 64 ? 2 : 1;
-                   attn_launch(&k_attn_dkv<DP, OCC>, f.units, 2 * (2 * 128 * DP + 256), st, f));
-        if (cut && gk) sum_launch(p.nk, p.ksplits, f.gk, gk, acc_k, st);
-        if (cut && gv) sum_launch(p.nk, p.ksplits, f.gv, gv, acc_v, st);
+        NC_ATTN_DP(p.DP, constexpr int OCC = DP <= 64 ? 4 : 2;
+                   attn_launch(&k_attn_dkv<DP, OCC>, f.units, 2 * (2 * 128 * DP + 256) + 16384, st, f, 2 * kAttnB));
+        if (cut) sum_launch(p.nk, p.ksplits, f.gk, gk, acc_k, f.gv, gv, acc_v, st);
     }
     return check_launch(what);
 }

@@ -108,9 +108,18 @@ __device__ __forceinline__ float halves_sum(float v) {
     return __int_as_float(r[0]) + __int_as_float(r[1]);
 }
 
-__device__ __forceinline__ float finite_abs(float x) {
-    const float a = __builtin_fabsf(x);
-    return a < INFINITY ? a : 0.0f;  // NaN too
+// The largest |x| of n values that is finite: NaNs do not count, and where an infinity is met the values are looked at again.
+template <int N>
+__device__ __forceinline__ float abs_max(const float (&x)[N], float most) {
+    float m = most;
+#pragma unroll
+    for (int i = 0; i < N; i++) m = __builtin_fmaxf(m, __builtin_fabsf(x[i]));
+    if (__builtin_expect(m == INFINITY, 0)) {
+        m = most;
+#pragma unroll
+        for (int i = 0; i < N; i++) m = __builtin_fmaxf(m, __builtin_fabsf(x[i]) < INFINITY ? __builtin_fabsf(x[i]) : 0.0f);
+    }
+    return m;
 }
 
 // the exponent e of a scale 2^e that puts `most` (finite, >= 0) into [2^14, 2^15) when values are divided by it
@@ -208,8 +217,8 @@ __device__ __forceinline__ void scale_acc(f16x (&acc)[NT], float by) {
         for (int r = 0; r < 16; r++) acc[d][r] *= by;
 }
 
-// a lane's column as a row of the output, `by` times; zeros where it holds nothing that counts
-template <int NT>
+// a lane's column as a row of the output, `by` times; CHECK: zeros where it holds nothing that counts
+template <bool CHECK, int NT>
 __device__ __forceinline__ void store_column(float *row, const f16x (&acc)[NT], bool some, float by, int half, int D, int add) {
 #pragma unroll
     for (int d = 0; d < NT; d++)
@@ -217,7 +226,7 @@ __device__ __forceinline__ void store_column(float *row, const f16x (&acc)[NT], 
         for (int j = 0; j < 4; j++) {
             f4 v;
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = some ? acc[d][4 * j + e] * by : 0.0f;
+            for (int e = 0; e < 4; e++) v[e] = !CHECK || some ? acc[d][4 * j + e] * by : 0.0f;
             store4(row, 32 * d + 8 * j + 4 * half, D, v, add);
         }
 }
@@ -244,18 +253,17 @@ __device__ __forceinline__ void load_query(Query<DP> &q, const float *row, bool 
 #pragma unroll
     for (int s = 0; s < DP / 16; s++) {
         load8(row, 16 * s + 8 * half, D, x);
-#pragma unroll
-        for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[e] * c));
+        most = abs_max(x, most);
     }
-    const int e = tile_exponent(halves_max(most));
-    const float inv = pow2i(-e);
+    const int e = tile_exponent(halves_max(most) * __builtin_fabsf(c));
+    const float by = c * pow2i(-e);
     q.c = pow2i(e);
     asm volatile("" ::: "memory");  // the row is read again (from the caches) rather than held in fp32 as well
 #pragma unroll
     for (int s = 0; s < DP / 16; s++) {
         load8(row, 16 * s + 8 * half, D, x);
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = live ? x[k] * c * inv : 0.0f;
+        for (int k = 0; k < 8; k++) x[k] *= by;
         const Split8 p = split8(x);
         q.hi[s] = p.hi, q.lo[s] = p.lo;
     }

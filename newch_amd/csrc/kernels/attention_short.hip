@@ -20,10 +20,8 @@ __device__ __forceinline__ float wave_tile(const float *src, int64_t step, int r
     for (int k = 0; k < PER; k++) {
         load8(row, 16 * k + 8 * half, D, x[k]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            x[k][e] = live ? x[k][e] : 0.0f;
-            most = __builtin_fmaxf(most, finite_abs(x[k][e]));
-        }
+        for (int e = 0; e < 8; e++) x[k][e] = live ? x[k][e] : 0.0f;
+        most = abs_max(x[k], most);
     }
     const int ex = tile_exponent(wave_max_nan_skip(most));
     const float inv = pow2i(-ex);
@@ -76,7 +74,7 @@ __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd
                 attend(sum, q, kt + t * TB, vt + t * TB, exps[t], exps[f.tiles + t], t + 1 == nt, min(n - t * kTile, kTile) - 4 * half);
             const float l = halves_sum(sum.l);
             if (live) {
-                store_column(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, l != 0.0f, pow2i((int)sum.E) / l, half, (int)a.D, 0);
+                store_column<false>(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, true, l != 0.0f ? pow2i((int)sum.E) / l : 0.0f, half, (int)a.D, 0);
                 if (f.lse && half == 0)
                     f.lse[(b * a.Hq + h) * a.Lq + i] = nt ? fma_(sum.m - kPShift, kLn2, logf(l)) : -INFINITY;
             }
@@ -102,14 +100,15 @@ __global__ __launch_bounds__(W *kWave, DP <= 64 ? 2 : 1) void k_attn_short_bwd(c
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ra = row_at(lane), ca = col_at(lane), D = (int)a.D;
-    char *const part = parts + wave * PART;
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t pair = w / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
         const int split = (int)(w - pair * f.splits);
         const int n = (int)keys_of(a.Lk, f.key_len, b), nt = (n + kTile - 1) / kTile;
         const int64_t t0 = f.qtiles * split / f.splits, t1 = f.qtiles * (split + 1) / f.splits;
-        const int key = wave * kTile + (lane & 31);
-        const bool mine = wave < nt, live = key < n;
+        // workgroups that share a CU give the first tiles of keys (the only ones of a short sequence) to other waves, so to other SIMDs
+        const int kw = (wave + (int)(w >> 8) * (W / 2)) & (W - 1), key = kw * kTile + (lane & 31);
+        char *const part = parts + kw * PART;
+        const bool mine = kw < nt, live = key < n;
 
         // the next tile's pieces: piece p is columns 8 (p / 32) .. + 7 of row p % 32
         float nq[PER][8], ng[PER][8], no[PER][8], nl = INFINITY;
@@ -135,14 +134,14 @@ __global__ __launch_bounds__(W *kWave, DP <= 64 ? 2 : 1) void k_attn_short_bwd(c
         h8 kh[KS], kl[KS], vh[KS], vl[KS], ch[2][NT], cl[2][NT];
         float ek = 0.0f, ev = 0.0f;
         if (mine) {  // this wave's keys and values, through its part of LDS
-            ek = wave_tile<DP>(f.k + b * a.sk[0] + u * a.sk[2], a.sk[1], wave * kTile, n, D, part);
+            ek = wave_tile<DP>(f.k + b * a.sk[0] + u * a.sk[2], a.sk[1], kw * kTile, n, D, part);
 #pragma unroll
             for (int s = 0; s < KS; s++) kh[s] = row_frag(part + ra, s), kl[s] = row_frag(part + ra + LO, s);
 #pragma unroll
             for (int s = 0; s < 2; s++)
 #pragma unroll
                 for (int t = 0; t < NT; t++) ch[s][t] = col_frag(part + ca, s, t), cl[s][t] = col_frag(part + ca + LO, s, t);
-            ev = wave_tile<DP>(f.v + b * a.sv[0] + u * a.sv[2], a.sv[1], wave * kTile, n, D, part);
+            ev = wave_tile<DP>(f.v + b * a.sv[0] + u * a.sv[2], a.sv[1], kw * kTile, n, D, part);
 #pragma unroll
             for (int s = 0; s < KS; s++) vh[s] = row_frag(part + ra, s), vl[s] = row_frag(part + ra + LO, s);
         }
@@ -160,12 +159,9 @@ __global__ __launch_bounds__(W *kWave, DP <= 64 ? 2 : 1) void k_attn_short_bwd(c
             for (int k = 0; k < PER; k++) {
                 const int p = threadIdx.x + k * THREADS;
                 float dot = 0.0f;
+                mq = abs_max(nq[k], mq), mg = abs_max(ng[k], mg);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    mq = __builtin_fmaxf(mq, finite_abs(nq[k][e]));
-                    mg = __builtin_fmaxf(mg, finite_abs(ng[k][e]));
-                    dot = fma_(ng[k][e], no[k][e], dot);
-                }
+                for (int e = 0; e < 8; e++) dot = fma_(ng[k][e], no[k][e], dot);
                 if (p < UNITS) dots[p] = dot;
             }
             mq = wave_max_nan_skip(mq), mg = wave_max_nan_skip(mg);
@@ -301,8 +297,8 @@ __global__ __launch_bounds__(W *kWave, DP <= 64 ? 2 : 1) void k_attn_short_bwd(c
         if (key < a.Lk) {
             const int64_t at = ((b * a.Lk + key) * a.Hkv + u) * D;
             const bool some = live && t0 < t1;
-            if (f.gk) store_column(f.gk + split * f.part_k + at, dk, some, a.scale / F, half, D, f.acc_k);
-            if (f.gv) store_column(f.gv + split * f.part_k + at, dv, some, __builtin_amdgcn_exp2f(E - 14.0f), half, D, f.acc_v);
+            if (f.gk) store_column<true>(f.gk + split * f.part_k + at, dk, some, a.scale / F, half, D, f.acc_k);
+            if (f.gv) store_column<true>(f.gv + split * f.part_k + at, dv, some, __builtin_amdgcn_exp2f(E - 14.0f), half, D, f.acc_v);
         }
     }
 }
