@@ -539,10 +539,10 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                 const char *rt = st + ds_wave * TB + ra;
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[r] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; k++)
-                    s = mfma3(row_frag(rt, k), row_frag(rt + LO, k), REG ? kh[k] : row_frag(kt, k), REG ? kl[k] : row_frag(kt + LO, k), s);
-                if constexpr (REG) order_steps<KS, 2>();
+                steps<KS>([&](int k) { return Pieces{row_frag(rt, k), row_frag(rt + LO, k)}; },
+                          [&](int k, const Pieces &x) {
+                              s = mfma3(x.hi, x.lo, REG ? kh[k] : row_frag(kt, k), REG ? kl[k] : row_frag(kt + LO, k), s);
+                          });
                 if (!ds_wave) {
                     if (ex > E) scale_acc(acc, __builtin_amdgcn_exp2f(E - ex));
                     const float c = ck * pow2i((int)eq), base = live ? sh : -INFINITY;
@@ -556,6 +556,11 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                 }
             }
             E = En;
+            const char *ct = st + (ds_wave ? 0 : TB) + ca;
+            const auto turned = [&](int k) { return Pieces{col_frag(ct, k / NT, k % NT), col_frag(ct + LO, k / NT, k % NT)}; };
+            Pieces x[3];
+            x[0] = turned(0);
+            x[1] = turned(1);
             lds_barrier();  // p is there (the next stage's copies stay on their way)
             if (!mine) continue;
             if (ds_wave) {
@@ -577,17 +582,8 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[r] *= kF;
             }
-            const char *ct = st + (ds_wave ? 0 : TB) + ca;
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = s[8 * k + e];
-                const Split8 ps = split8(y);
-#pragma unroll
-                for (int d = 0; d < NT; d++) acc[d] = mfma3(col_frag(ct, k, d), col_frag(ct + LO, k, d), ps.hi, ps.lo, acc[d]);
-            }
-            order_steps<2 * NT, 4>();
+            const Split8 y[2] = {split_regs(s, 0), split_regs(s, 8)};
+            steps<2 * NT>(x, turned, [&](int k, const Pieces &v) { acc[k % NT] = mfma3(v.hi, v.lo, y[k / NT].hi, y[k / NT].lo, acc[k % NT]); });
         }
         float *const out = ds_wave ? f.gk : f.gv;
         if (out && key < a.Lk)
@@ -651,12 +647,15 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
             f16x s, dp;
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                s = mfma3(row_frag(kt, k), row_frag(kt + LO, k), qh[k], ql[k], s);
-                dp = mfma3(row_frag(vt, k), row_frag(vt + LO, k), gh[k], gl[k], dp);
-            }
-            order_steps<2 * KS, 2>();
+            steps<2 * KS>([&](int k) { return k % 2 ? Pieces{row_frag(vt, k / 2), row_frag(vt + LO, k / 2)} : Pieces{row_frag(kt, k / 2), row_frag(kt + LO, k / 2)}; },
+                          [&](int k, const Pieces &x) {
+                              if (k % 2) dp = mfma3(x.hi, x.lo, gh[k / 2], gl[k / 2], dp);
+                              else s = mfma3(x.hi, x.lo, qh[k / 2], ql[k / 2], s);
+                          });
+            const auto turned = [&](int k) { return Pieces{col_frag(kc, k / NT, k % NT), col_frag(kc + LO, k / NT, k % NT)}; };
+            Pieces x[3];
+            x[0] = turned(0);
+            x[1] = turned(1);
             const float c = cq * pow2i((int)ek), c2 = cg * pow2i((int)ev);
             const int left = (int)min(n - t * kTile, (int64_t)kTile) - 4 * half;
             float most = 0.0f;
@@ -672,17 +671,9 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
             if (column_scale(halves_max(most) * kap, F, by)) scale_acc(dq, by);
             const float kF = kap * F;
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                float z[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) z[e] = dp[8 * k + e] * kF;
-                const Split8 ds = split8(z);
-#pragma unroll
-                for (int d = 0; d < NT; d++) {
-                    dq[d] = mfma3(col_frag(kc, k, d), col_frag(kc + LO, k, d), ds.hi, ds.lo, dq[d]);
-                }
-            }
-            order_steps<2 * NT, 4>();
+            for (int r = 0; r < 16; r++) dp[r] *= kF;
+            const Split8 y[2] = {split_regs(dp, 0), split_regs(dp, 8)};
+            steps<2 * NT>(x, turned, [&](int k, const Pieces &v) { dq[k % NT] = mfma3(v.hi, v.lo, y[k / NT].hi, y[k / NT].lo, dq[k % NT]); });
         }
         if (R < f.rows) {
             int64_t i, g;

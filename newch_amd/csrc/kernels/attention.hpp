@@ -92,6 +92,14 @@ __device__ __forceinline__ h8 col_frag(const char *tile, int s, int t) {
     return __builtin_bit_cast(h8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 }
 
+// a result's registers r0 .. r0 + 7 as the next product's operand
+__device__ __forceinline__ Split8 split_regs(const f16x &s, int r0) {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = s[r0 + e];
+    return split8(y);
+}
+
 __device__ __forceinline__ f16x mfma3(const h8 &ah, const h8 &al, const h8 &bh, const h8 &bl, f16x c) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c, 0, 0, 0);
@@ -175,16 +183,31 @@ __device__ __forceinline__ int64_t keys_of(int64_t Lk, const int *key_len, int64
     return n < 0 ? 0 : n < Lk ? n : Lk;
 }
 
-// The order of a block of N steps, each R reads of fragments from LDS and three products: reads two steps ahead of their products.
-template <int N, int R>
-__device__ __forceinline__ void order_steps() {
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * R, 0);
+// A block of N steps, each with two fragments from LDS (read(k): its hi and lo) and three products (step(k, pieces)): the
+// fragments are read two steps ahead of their products, which the compiler on its own does not do -- it saves registers and waits
+// for LDS in every step.  `first`: the steps 0 and 1, where they are read earlier still.
+struct Pieces {
+    h8 hi, lo;
+};
+__device__ __forceinline__ void keep_order() {  // LDS reads and products stay where they are; all else may pass
+    __builtin_amdgcn_sched_barrier(0x0002 | 0x0004 | 0x0010 | 0x0020 | 0x0040);
+}
+template <int N, class Read, class Step>
+__device__ __forceinline__ void steps(Pieces (&f)[3], Read &&read, Step &&step) {
+    keep_order();
 #pragma unroll
-    for (int i = 0; i < N - 2; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    for (int k = 0; k < N; k++) {
+        if (k + 2 < N) f[(k + 2) % 3] = read(k + 2);
+        step(k, f[k % 3]);
+        keep_order();
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+}
+template <int N, class Read, class Step>
+__device__ __forceinline__ void steps(Read &&read, Step &&step) {
+    Pieces f[3];
+    f[0] = read(0);
+    f[1] = read(1);
+    steps<N>(f, read, step);
 }
 
 // Workgroups are dealt round robin over the 8 XCDs: consecutive units of a launch go to one XCD, which then keeps their
@@ -291,9 +314,12 @@ __device__ __forceinline__ void attend(Sums<DP> &a, const Query<DP> &q, const ch
     f16x s;
 #pragma unroll
     for (int r = 0; r < 16; r++) s[r] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KS; k++) s = mfma3(row_frag(kt, k), row_frag(kt + LO, k), q.hi[k], q.lo[k], s);
-    order_steps<KS, 2>();
+    steps<KS>([&](int k) { return Pieces{row_frag(kt, k), row_frag(kt + LO, k)}; },
+              [&](int k, const Pieces &f) { s = mfma3(f.hi, f.lo, q.hi[k], q.lo[k], s); });
+    const auto value = [&](int k) { return Pieces{col_frag(vt, k / NT, k % NT), col_frag(vt + LO, k / NT, k % NT)}; };
+    Pieces f[3];
+    f[0] = value(0);
+    f[1] = value(1);
     const float c = __builtin_fmaxf(q.c * pow2i((int)ek), 0x1p-126f);  // -inf * c stays -inf
     if (cut) {
 #pragma unroll
@@ -325,16 +351,8 @@ __device__ __forceinline__ void attend(Sums<DP> &a, const Query<DP> &q, const ch
         sum += s[r];
     }
     a.l = fma_(sum, __builtin_amdgcn_exp2f(-dv), a.l);
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = s[8 * k + e];
-        const Split8 p = split8(y);
-#pragma unroll
-        for (int d = 0; d < NT; d++) a.o[d] = mfma3(col_frag(vt, k, d), col_frag(vt + LO, k, d), p.hi, p.lo, a.o[d]);
-    }
-    order_steps<2 * NT, 4>();
+    const Split8 p[2] = {split_regs(s, 0), split_regs(s, 8)};
+    steps<2 * NT>(f, value, [&](int k, const Pieces &v) { a.o[k % NT] = mfma3(v.hi, v.lo, p[k / NT].hi, p[k / NT].lo, a.o[k % NT]); });
 }
 
 }  // namespace nchip

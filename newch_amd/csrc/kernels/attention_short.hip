@@ -86,7 +86,7 @@ __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd
 // (the next one's on their way meanwhile), and each wave takes its part of gk and gv as k_attn_dkv does, then turns its ds in LDS
 // and multiplies it with its keys; the waves' parts of gq are added in wave order.
 template <int DP, int W>
-__global__ __launch_bounds__(W *kWave, DP <= 64 ? 2 : 1) void k_attn_short_bwd(const ShortBwd f) {
+__global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP;
     constexpr int THREADS = W * kWave, UNITS = 4 * DP, PER = (UNITS + THREADS - 1) / THREADS;  // 8-column pieces of a tile
     constexpr int LD = DP + 4, PART = 32 * LD * 4;  // a wave's part of gq: 32 rows, which also holds ds turned, and at first a tile
@@ -198,12 +198,11 @@ __global__ __launch_bounds__(W *kWave, DP <= 64 ? 2 : 1) void k_attn_short_bwd(c
                 f16x s, dp;
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    s = mfma3(row_frag(qt, k), row_frag(qt + LO, k), kh[k], kl[k], s);
-                    dp = mfma3(row_frag(gt, k), row_frag(gt + LO, k), vh[k], vl[k], dp);
-                }
-                order_steps<2 * KS, 2>();
+                steps<2 * KS>([&](int k) { return k % 2 ? Pieces{row_frag(gt, k / 2), row_frag(gt + LO, k / 2)} : Pieces{row_frag(qt, k / 2), row_frag(qt + LO, k / 2)}; },
+                              [&](int k, const Pieces &x) {
+                                  if (k % 2) dp = mfma3(x.hi, x.lo, vh[k / 2], vl[k / 2], dp);
+                                  else s = mfma3(x.hi, x.lo, kh[k / 2], kl[k / 2], s);
+                              });
                 const float ex = (float)eg;
                 if (ex > E) {
                     scale_acc(dv, __builtin_amdgcn_exp2f(E - ex));
@@ -232,18 +231,18 @@ __global__ __launch_bounds__(W *kWave, DP <= 64 ? 2 : 1) void k_attn_short_bwd(c
                 if (column_scale(halves_max(most) * kap, F, by)) scale_acc(dk, by);
                 const float kF = kap * F;
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    float y[8], z[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) y[e] = s[8 * k + e], z[e] = dp[8 * k + e] * kF;
-                    const Split8 ps = split8(y), ds = split8(z);
-#pragma unroll
-                    for (int d = 0; d < NT; d++) {
-                        dv[d] = mfma3(col_frag(gc, k, d), col_frag(gc + LO, k, d), ps.hi, ps.lo, dv[d]);
-                        dk[d] = mfma3(col_frag(qc, k, d), col_frag(qc + LO, k, d), ds.hi, ds.lo, dk[d]);
-                    }
-                }
-                order_steps<4 * NT, 4>();
+                for (int r = 0; r < 16; r++) dp[r] *= kF;
+                const Split8 ps[2] = {split_regs(s, 0), split_regs(s, 8)}, ds[2] = {split_regs(dp, 0), split_regs(dp, 8)};
+                // steps of 2 NT: go's fragment (s, t), then q's
+                steps<4 * NT>([&](int k) {
+                                  const char *c = k % 2 ? qc : gc;
+                                  return Pieces{col_frag(c, k / 2 / NT, k / 2 % NT), col_frag(c + LO, k / 2 / NT, k / 2 % NT)};
+                              },
+                              [&](int k, const Pieces &x) {
+                                  const int r = k / 2 / NT, d = k / 2 % NT;
+                                  if (k % 2) dk[d] = mfma3(x.hi, x.lo, ds[r].hi, ds[r].lo, dk[d]);
+                                  else dv[d] = mfma3(x.hi, x.lo, ps[r].hi, ps[r].lo, dv[d]);
+                              });
                 // gq^T of this wave's keys: k^T ds^T, a lane a row of queries
                 float x[2][8], top = 0.0f;
                 const float *row = (const float *)part + (lane & 31) * LDS_DS + 4 * half;
@@ -267,9 +266,9 @@ __global__ __launch_bounds__(W *kWave, DP <= 64 ? 2 : 1) void k_attn_short_bwd(c
                 for (int k = 0; k < 2; k++) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) x[k][e] *= Fq;
-                    const Split8 ds = split8(x[k]);
+                    const Split8 y = split8(x[k]);
 #pragma unroll
-                    for (int d = 0; d < NT; d++) dq[d] = mfma3(ch[k][d], cl[k][d], ds.hi, ds.lo, dq[d]);
+                    for (int d = 0; d < NT; d++) dq[d] = mfma3(ch[k][d], cl[k][d], y.hi, y.lo, dq[d]);
                 }
                 const float back = __builtin_amdgcn_exp2f(ek - sh) / Fq * a.scale;
                 float *mypart = (float *)part + (lane & 31) * LD + 4 * half;
@@ -303,8 +302,8 @@ __global__ __launch_bounds__(W *kWave, DP <= 64 ? 2 : 1) void k_attn_short_bwd(c
     }
 }
 
-int short_keys_fwd(int DP) { return DP <= 128 ? 16384 / DP : 0; }
-int short_keys_bwd(int DP) { return DP <= 64 ? 256 : DP <= 128 ? 128 : 0; }
+int short_keys_fwd(int DP) { return DP <= 128 ? 16384 / DP : -1; }
+int short_keys_bwd(int DP) { return DP <= 64 ? 256 : -1; }
 
 template <class F, class A>
 static void launch(F *kernel, int64_t units, int threads, size_t lds, hipStream_t st, const A &args) {
@@ -329,9 +328,7 @@ static void bwd_launch(const ShortBwd &f, hipStream_t st) {
 void short_bwd(const ShortBwd &f, int DP, hipStream_t st) {
     const bool four = f.a.Lk <= 4 * kTile;
     if (DP == 32) four ? bwd_launch<32, 4>(f, st) : bwd_launch<32, 8>(f, st);
-    else if (DP == 64) four ? bwd_launch<64, 4>(f, st) : bwd_launch<64, 8>(f, st);
-    else if (DP == 96) bwd_launch<96, 4>(f, st);
-    else bwd_launch<128, 4>(f, st);
+    else four ? bwd_launch<64, 4>(f, st) : bwd_launch<64, 8>(f, st);
 }
 
 }  // namespace nchip
