@@ -13,6 +13,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace nchip {
 
 // ------------------------------------------------------------------------------------------------
@@ -434,13 +436,14 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
         bool nan = false;
 #pragma unroll
         for (int s = 0; s < 8; s++) {
-            const int64_t at = min(s, splits - 1) * all + pr;
+            ml[s] = f2{-INFINITY, 0.0f};
+            if (s >= splits) continue;
+            const int64_t at = s * all + pr;
             ml[s] = pm[at];
             p[s] = a.D >= 4 ? last4(po + at * a.D, d, (int)a.D) : f4{po[at * a.D], po[at * a.D + (a.D > 1)], po[at * a.D + a.D - 1], 0.0f};
         }
 #pragma unroll
         for (int s = 0; s < 8; s++) {
-            if (s >= splits) ml[s] = f2{-INFINITY, 0.0f};
             nan = nan || ml[s].x != ml[s].x;
             M = __builtin_fmaxf(M, ml[s].x);
         }
@@ -740,10 +743,11 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
         else { constexpr int DP = 256; __VA_ARGS__; }                   \
     } while (0)
 
-// parts so that there are `want` workgroups, of at least four tiles each, 64 parts at most
+// Parts so that there are `want` workgroups, 64 parts at most, of at least four tiles each, or sixteen where the whole ones already
+// fill half the CUs: joining costs more than it gains there (1001 x 333, 3 x 8 heads of 80, forward: XX us in two parts, YY whole).
 static int attn_splits(int64_t whole, int64_t tiles, int64_t want) {
     int64_t s = whole ? want / whole : 1;
-    if (s > tiles / 4) s = tiles / 4;
+    s = std::min(s, tiles / (whole >= kPlanCUs / 2 ? 16 : 4));
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
@@ -765,10 +769,12 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
     p.qtiles = (int)((p.rows + kAttnWaves * kTile - 1) / (kAttnWaves * kTile));
     p.token = p.rows <= kTokenRows;
     p.few = !p.token && Lk <= short_keys_fwd(p.DP);
-    if (p.few) {  // two workgroups a CU, with a tile of queries for each of their eight waves
+    if (p.few) {
+        // two workgroups a CU with a tile of queries for each of their eight waves, or one a CU with two tiles at least (58 rows x
+        // 2 heads against 96 keys, heads of 128, four sequences: 30 us with eight tiles a workgroup, 20 with two)
         const int64_t tiles = (p.rows + kTile - 1) / kTile;
-        int64_t parts = p.pairs ? 2 * kPlanCUs / p.pairs : 1;
-        if (parts > tiles / 8) parts = tiles / 8;
+        const auto cut = [&](int64_t units, int64_t least) { return std::min(p.pairs ? units / p.pairs : 1, tiles / least); };
+        const int64_t parts = std::max(cut(2 * kPlanCUs, 8), cut(kPlanCUs, 2));
         p.splits = (int)(parts < 1 ? 1 : parts);
         p.units = p.pairs * p.splits;
         return p;

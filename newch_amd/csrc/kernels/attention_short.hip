@@ -314,7 +314,7 @@ static void launch(F *kernel, int64_t units, int threads, size_t lds, hipStream_
 void short_fwd(const ShortFwd &f, int DP, hipStream_t st) {
     const size_t lds = (size_t)f.tiles * 2 * tile_bytes(DP) + 2 * f.tiles * sizeof(float);
     if (DP == 32) launch(&k_attn_short_fwd<32, 8, 4>, f.units, 512, lds, st, f);
-    else if (DP == 64) launch(&k_attn_short_fwd<64, 8, 4>, f.units, 512, lds, st, f);
+    else if (DP == 64) launch(&k_attn_short_fwd<64, 8, 2>, f.units, 512, lds, st, f);
     else if (DP == 96) launch(&k_attn_short_fwd<96, 8, 2>, f.units, 512, lds, st, f);
     else launch(&k_attn_short_fwd<128, 8, 2>, f.units, 512, lds, st, f);
 }
