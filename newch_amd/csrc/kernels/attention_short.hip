@@ -63,8 +63,8 @@ __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd
             const int64_t R = qt * kTile + (lane & 31);
             const bool live = R < f.rows;
             int64_t i, g;
-        a.row(live ? R : 0, i, g);
-        const int64_t h = u * a.G + g;
+            a.row(live ? R : 0, i, g);
+            const int64_t h = u * a.G + g;
             Query<DP> q;
             load_query(q, f.q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2], live, a.scale, half, (int)a.D);
             Sums<DP> sum;
@@ -287,8 +287,8 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
                     f4 sum = {0.f, 0.f, 0.f, 0.f};
                     for (int x = 0; x < nt; x++) sum += *(const f4 *)((const float *)(parts + x * PART) + r * LD + d);
                     int64_t i, g;
-            a.row(R, i, g);
-            const int64_t h = u * a.G + g;
+                    a.row(R, i, g);
+                    const int64_t h = u * a.G + g;
                     store4(f.gq + ((b * a.Lq + i) * a.Hq + h) * D, d, D, sum, f.acc_q);
                 }
             }

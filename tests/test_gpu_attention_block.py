@@ -298,6 +298,29 @@ def test_attention_nan_stays_in_its_sequence(K):
         R.within(got[at], ref["o"][0][at], ref["o"][1][at], str(at))
 
 
+# rows of a pair against keys: eight rows read in parts, parts joined by rows, and parts joined by pieces
+@pytest.mark.parametrize("shape", [(1, 1, 3000, 1, 1, 64, None), (1, 20, 3000, 2, 2, 128, None), (1, 3000, 700, 2, 2, 96, None),
+                                   (1, 300, 90, 2, 2, 64, None)], ids=str)
+def test_attention_nan_query_stays_in_its_row(K, shape):
+    """A row of queries that holds a NaN gives NaN, whichever way its keys' parts are joined, and its neighbours their values."""
+    q, k, v, g, lens = attn_inputs(shape, 20)
+    Lq, Hq = shape[1], shape[3]
+    ref = R.attention64(q, k, v, lens, 0.125, None)
+    q[0, Lq // 2, 0, 1] = np.nan
+    o, lse, n = Out(q.shape), Out((1, Hq, Lq)), K.cross_attention_fwd_workspace(*shape[:6])
+    bufs = [place(t) for t in (q, k, v)]
+    src = sum(((p, s) for _, p, s in bufs), ())
+    ws = DeviceBuffer.empty(max(n, 1))
+    K.cross_attention_fwd(*shape[:6], 0.125, *src, None, o.ptr, lse.ptr, ws.ptr, n)
+    synchronize()
+    got, l = o.get(), lse.get()
+    assert np.isnan(got[0, Lq // 2, 0]).all() and np.isnan(l[0, 0, Lq // 2])
+    rest = np.ones((1, Lq, Hq), bool)
+    rest[0, Lq // 2, 0] = False
+    R.within(got[rest], ref["o"][0][rest], ref["o"][1][rest], "o")
+    R.within(l.transpose(0, 2, 1)[rest], *(t.transpose(0, 2, 1)[rest] for t in ref["lse"]), "lse")
+
+
 def test_attention_is_deterministic_and_takes_streams(K):
     """The same bits on another stream, twice, from workspaces that held other bytes."""
     shape = (2, 150, 333, 4, 2, 64, (333, 100))
