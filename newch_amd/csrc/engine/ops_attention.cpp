@@ -265,26 +265,34 @@ static void attn_bwd(nc_node *n) {
     const int32_t *len = c.len ? contig_i32(c.len) : nullptr;
     const bool want_q = needs_grad(c.q), want_k = needs_grad(c.k), want_v = needs_grad(c.v);
     if ((c.len && !len) || (want_q && !grad_buf(c.q)) || (want_k && !grad_buf(c.k)) || (want_v && !grad_buf(c.v))) return;
-    // keys that are the values too have one gradient: the values' part goes through scratch (the kernel writes both at once)
-    const bool shared = want_v && c.k == c.v;
-    const size_t kv_bytes = (size_t)nc_numel(c.v) * sizeof(float);
-    const int acc_q = want_q ? grad_acc(c.q) : 0, acc_k = want_k ? grad_acc(c.k) : 0;
-    const int acc_v = want_v && !shared ? grad_acc(c.v) : 0;
-    float *gq = want_q ? fptr(c.q->grad) : nullptr, *gk = want_k ? fptr(c.k->grad) : nullptr;
-    float *gv = shared ? (float *)arena_alloc(ctx, kv_bytes ? kv_bytes : 1) : want_v ? fptr(c.v->grad) : nullptr;
+    // One tensor as several of the three has one gradient, and the kernels' must not overlap: its later parts go through scratch.
+    nc_tensor *const in[3] = {c.q, c.k, c.v};
+    const bool want[3] = {want_q, want_k, want_v};
+    int first[3], acc[3];
+    float *g[3] = {};
+    for (int i = 0; i < 3; i++) {
+        first[i] = 0;
+        while (in[first[i]] != in[i]) first[i]++;
+        const size_t bytes = (size_t)nc_numel(in[i]) * sizeof(float);
+        acc[i] = want[i] && first[i] == i ? grad_acc(in[i]) : 0;
+        if (want[i]) g[i] = first[i] == i ? fptr(in[i]->grad) : (float *)arena_alloc(ctx, bytes ? bytes : 1);
+        if (want[i] && !g[i]) return;
+    }
     const size_t ws_bytes = nc_hip_cross_attention_bwd_workspace(c.B, c.Lq, c.Lk, c.Hq, c.Hkv, c.D);
     char *ws = ws_bytes ? arena_alloc(ctx, ws_bytes) : nullptr;
-    if ((want_q && !gq) || (want_k && !gk) || (want_v && !gv) || (ws_bytes && !ws)) return;
+    if (ws_bytes && !ws) return;
     if (!hip_layer_ok(ctx,
                       nc_hip_cross_attention_bwd(c.B, c.Lq, c.Lk, c.Hq, c.Hkv, c.D, n->p.f[0], q.p, q.s, k.p, k.s, v.p, v.s, len, o,
-                                                 (const float *)n->saved, go, gq, gk, gv, acc_q, acc_k, acc_v, ws, ws_bytes,
+                                                 (const float *)n->saved, go, g[0], g[1], g[2], acc[0], acc[1], acc[2], ws, ws_bytes,
                                                  stream(ctx)),
                       n->op->name))
         return;
-    if (shared && !hip_layer_ok(ctx, nc_hip_axpy(nc_numel(c.v), 1.0f, gv, gk, stream(ctx)), n->op->name)) return;
-    if (want_q) wrote_dev(c.q->grad);
-    if (want_k) wrote_dev(c.k->grad);
-    if (want_v) wrote_dev(c.v->grad);
+    for (int i = 1; i < 3; i++)
+        if (want[i] && first[i] != i &&
+            !hip_layer_ok(ctx, nc_hip_axpy(nc_numel(in[i]), 1.0f, g[i], g[first[i]], stream(ctx)), n->op->name))
+            return;
+    for (int i = 0; i < 3; i++)
+        if (want[i] && first[i] == i) wrote_dev(in[i]->grad);
 }
 
 static const OpDef op_cross_attention = {"cross_attention", 0, 0, attn_shape, nullptr, attn_fwd, attn_bwd};

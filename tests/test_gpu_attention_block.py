@@ -428,6 +428,26 @@ def test_engine_attention(eng, same):
         R.within(eng.grad(Q), *ref["gq"], "gq")
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("same", ["qk", "qv", "qkv"])
+def test_engine_one_tensor_twice(eng, same, D):
+    """One tensor as queries and keys, queries and values, or all: its gradient is the sum, in both backward kernels."""
+    L = eng.lib
+    B, T, H = 2, 90, 2
+    q, k, v, g, _ = attn_inputs((B, T, T, H, H, D, None), 27)
+    k, v = (q if "k" in same else k), (q if "v" in same else v)
+    ref = R.attention64(q, k, v, None, D ** -0.5, g)
+    Q = eng.param(q)
+    K_, V = Q if "k" in same else eng.param(k), Q if "v" in same else eng.param(v)
+    want, bound = (sum(ref["g" + c][j] for c in same) for j in (0, 1))
+    for times in (1, 2):
+        eng.backward_with(L.nc_cross_attention(Q, K_, V, None, c_float(D ** -0.5)), g)
+        R.within(eng.grad(Q), times * want, times * (bound + 4 * R.U * np.abs(want)), "g of " + same)
+    for c, t in (("k", K_), ("v", V)):
+        if c not in same:
+            R.within(eng.grad(t), 2 * ref["g" + c][0], 3 * ref["g" + c][1], "g" + c)
+
+
 def test_engine_refuses_inputs_written_since(eng):
     L = eng.lib
     q, k, v, g, _ = attn_inputs((1, 4, 6, 2, 2, 16, None), 24)
