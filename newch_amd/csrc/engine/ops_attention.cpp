@@ -37,17 +37,18 @@ static const int32_t *contig_i32(nc_tensor *t) {
     return (const int32_t *)c;
 }
 
-// counts every write to the storage of the inputs from `first` on: the same number means that none was written
-static int64_t generations(const nc_node *n, int first = 0) {
-    uint64_t g = 0;
+// counts every write to the storage of the inputs from `first` on, and of the output where the backward reads it: the same number
+// means that none was written
+static int64_t generations(const nc_node *n, int first = 0, bool output = false) {
+    uint64_t g = output ? owner_of(n->out)->wgen : 0;
     for (int i = first; i < n->n_in; i++) g += owner_of(n->in[i])->wgen;
     return (int64_t)g;
 }
 
-static bool unwritten(const nc_node *n, int64_t then, int first = 0) {
-    if (generations(n, first) == then) return true;
-    error(n->in[0]->ctx, NC_ERR_STATE, "%s: an input was written after the forward (the backward reads it again)",
-          n->op->name);
+static bool unwritten(const nc_node *n, int64_t then, int first = 0, bool output = false) {
+    if (generations(n, first, output) == then) return true;
+    error(n->in[0]->ctx, NC_ERR_STATE, "%s: an input%s was written after the forward (the backward reads it again)",
+          n->op->name, output ? " or the output" : "");
     return false;
 }
 
@@ -251,14 +252,14 @@ static nc_status attn_fwd(nc_node *n) {
                       n->op->name))
         return NC_ERR_STATE;
     wrote_dev(n->out);
-    n->p.i[0] = generations(n);
+    n->p.i[0] = generations(n, 0, true);
     return NC_OK;
 }
 
 static void attn_bwd(nc_node *n) {
     const AttnCall c(n);
     nc_ctx *ctx = c.q->ctx;
-    if (!unwritten(n, n->p.i[0])) return;
+    if (!unwritten(n, n->p.i[0], 0, true)) return;
     Heads q, k, v;
     const float *o = fptr(n->out), *go = fptr(n->out->grad);
     if (!o || !go || !heads_of(c.q, q) || !heads_of(c.k, k) || !heads_of(c.v, v)) return;
