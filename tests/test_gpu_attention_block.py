@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from newch_amd import abi, hip
-from newch_amd.hipmem import DeviceBuffer, Stream, synchronize
+from newch_amd.hipmem import DeviceBuffer, Stream, check, runtime, synchronize
 from tests import attention_ref as R
 from tests.ncdrive import Engine, NcError
 
@@ -240,6 +240,22 @@ def test_attention_kernel(K, shape):
         check_attention(run_attention(K, shape, q, k, v, g, lens, order, shift, gap, old_v), ref, old or 0.0, order)
 
 
+# what the sizes above do not reach: rows of few keys cut among workgroups with heads that do not divide a tile; few keys of two
+# to eight tiles; three to eight rows of odd widths; many parts of keys, or of queries; wide heads over several tiles
+PATH_SHAPES = [(1, 900, 40, 6, 2, 64, (33,)), (2, 130, 200, 4, 2, 64, (200, 131)), (1, 70, 500, 2, 1, 32, (481,)),
+               (1, 700, 150, 2, 2, 96, None), (2, 3, 400, 2, 2, 30, (400, 129)), (1, 2, 300, 8, 2, 250, (299,)),
+               (2, 1, 600, 5, 1, 101, (0, 600)), (1, 1, 900, 3, 3, 255, None), (1, 2000, 50, 1, 1, 128, (45,)),
+               (1, 40, 3000, 1, 1, 64, (2990,)), (1, 300, 290, 2, 1, 200, (285,)), (1, 9, 2100, 3, 3, 48, None),
+               (1, 33, 260, 5, 5, 64, None), (300, 5, 9, 4, 2, 16, None), (1, 4, 4, 64, 1, 64, None)]
+
+
+@pytest.mark.parametrize("shape", PATH_SHAPES, ids=str)
+def test_attention_paths(K, shape):
+    q, k, v, g, lens = attn_inputs(shape, 28)
+    ref = R.attention64(q, k, v, lens, shape[5] ** -0.5, g)
+    check_attention(run_attention(K, shape, q, k, v, g, lens, "bhld", 2, 3), ref)
+
+
 @pytest.mark.parametrize("want", ["q", "k", "v", "qv", ""])
 def test_attention_some_gradients(K, want):
     shape = (2, 70, 45, 4, 2, 64, (45, 3))
@@ -331,6 +347,96 @@ def test_attention_is_deterministic_and_takes_streams(K):
         again = run_attention(K, shape, q, k, v, g, lens, stream=s.handle, poison=poison)
         for name, a in first.items():
             assert (a.view(np.uint32) == again[name].view(np.uint32)).all(), name
+
+
+class Block:
+    """Norm and rotation of the queries, attention to rotated keys, and its backward, on buffers of its own."""
+
+    def __init__(self, K, shape, seed):
+        B, Lq, Lk, Hq, Hkv, D, _ = self.shape = shape
+        self.K, self.sizes = K, shape[:6]
+        self.host = attn_inputs(shape, seed)
+        self.q, self.k, self.v, self.g, self.n = (up(t) for t in self.host)
+        self.wq = up(np.linspace(0.5, 1.5, D, dtype=np.float32))
+        self.pos = up(np.arange(max(Lq, Lk), dtype=np.int32)[:, None])
+        new = lambda *s: DeviceBuffer.from_numpy(np.full(s, np.nan, np.float32))
+        self.x, self.y, self.o, self.lse = new(B, Lq, Hq, D), new(B, Lk, Hkv, D), new(B, Lq, Hq, D), new(B, Hq, Lq)
+        self.gx, self.gk, self.gv, self.gq = new(B, Lq, Hq, D), new(B, Lk, Hkv, D), new(B, Lk, Hkv, D), new(B, Lq, Hq, D)
+        self.gw = new(D)
+        self.n1, self.n2 = K.cross_attention_fwd_workspace(*self.sizes), K.cross_attention_bwd_workspace(*self.sizes)
+        self.n3 = K.qk_norm_rope_bwd_workspace(B, Lq, Hq, D)
+        self.ws = DeviceBuffer.empty(max(self.n1, self.n2, self.n3, 1))
+
+    def run(self, stream):
+        B, Lq, Lk, Hq, Hkv, D = self.sizes
+        sq, sk = (Lq * Hq * D, Hq * D, D), (Lk * Hkv * D, Hkv * D, D)
+        K, rot = self.K, (0, (D // 2 * 2,), 100.0, 0)
+        K.qk_norm_rope_fwd(B, Lq, Hq, D, Hq, self.q.ptr, sq, self.wq.ptr, None, 1e-6, self.pos.ptr, *rot, self.x.ptr, stream=stream)
+        K.rope_fwd(B, Lk, Hkv, D, self.k.ptr, sk, self.pos.ptr, *rot, self.y.ptr, stream=stream)
+        src = (self.x.ptr, sq, self.y.ptr, sk, self.v.ptr, sk, ptr(self.n))
+        K.cross_attention_fwd(*self.sizes, 0.2, *src, self.o.ptr, self.lse.ptr, self.ws.ptr, self.n1, stream=stream)
+        K.cross_attention_bwd(*self.sizes, 0.2, *src, self.o.ptr, self.lse.ptr, self.g.ptr, self.gx.ptr, self.gk.ptr, self.gv.ptr,
+                              self.ws.ptr, self.n2, accumulate=False, stream=stream)
+        K.qk_norm_rope_bwd(B, Lq, Hq, D, Hq, self.q.ptr, sq, self.wq.ptr, None, 1e-6, self.pos.ptr, *rot, self.gx.ptr, self.gq.ptr,
+                           self.gw.ptr, None, self.ws.ptr, self.n3, accumulate=False, stream=stream)
+
+    def results(self):
+        got = [b.to_numpy(np.float32, b.nbytes // 4) for b in (self.x, self.y, self.o, self.lse, self.gx, self.gk, self.gv, self.gq, self.gw)]
+        assert all(np.isfinite(t).all() for t in got)
+        return [t.view(np.uint32) for t in got]
+
+
+BLOCK_SHAPES = [(2, 70, 45, 4, 2, 64, (45, 3)), (1, 1, 700, 4, 4, 64, (650,)), (1, 300, 600, 2, 2, 80, (590,)), (1, 150, 270, 2, 1, 200, None)]
+
+
+@pytest.mark.parametrize("shape", BLOCK_SHAPES, ids=str)
+def test_block_captured_and_replayed(K, shape):
+    """The block as a graph: every replay, with other inputs and eager calls in between, gives the eager run's bits."""
+    rt = runtime()
+    a, other = Block(K, shape, 29), Block(K, shape, 30)
+    a.run(None)
+    other.run(None)
+    synchronize()
+    want, new = a.results(), other.results()
+    s, graph, run = Stream(), ctypes.c_void_p(), ctypes.c_void_p()
+    check(rt.hipStreamBeginCapture(ctypes.c_void_p(s.handle), ctypes.c_int(2)), "begin")  # relaxed: other streams as they are
+    try:
+        a.run(s.handle)
+    finally:
+        check(rt.hipStreamEndCapture(ctypes.c_void_p(s.handle), ctypes.byref(graph)), "end")
+    check(rt.hipGraphInstantiate(ctypes.byref(run), graph, None, None, ctypes.c_size_t(0)), "instantiate")
+    for i in range(4):
+        for b, h in zip((a.q, a.k, a.v, a.g), (other if i % 2 else a).host):
+            b.upload(h)
+        for b in (a.x, a.y, a.o, a.lse, a.gx, a.gk, a.gv, a.gq, a.gw):
+            b.upload(np.full(b.nbytes // 4, np.nan, np.float32))
+        synchronize()
+        check(rt.hipGraphLaunch(run, ctypes.c_void_p(s.handle)), "launch")
+        s.synchronize()
+        other.run(None)
+        synchronize()
+        for x, y in zip(a.results(), new if i % 2 else want):
+            assert (x == y).all(), f"replay {i}"
+        for x, y in zip(other.results(), new):
+            assert (x == y).all(), f"eager after replay {i}"
+    check(rt.hipGraphExecDestroy(run), "destroy")
+    check(rt.hipGraphDestroy(graph), "destroy")
+
+
+def test_blocks_on_two_streams_at_once(K):
+    """Two blocks with workspaces of their own, their calls in flight together, several times over."""
+    blocks = [Block(K, BLOCK_SHAPES[0], 31), Block(K, BLOCK_SHAPES[2], 32)]
+    for b in blocks:
+        b.run(None)
+    synchronize()
+    want, streams = [b.results() for b in blocks], [Stream(), Stream()]
+    for _ in range(5):
+        for b, s in zip(blocks, streams):
+            b.run(s.handle)
+    synchronize()
+    for b, w in zip(blocks, want):
+        for x, y in zip(b.results(), w):
+            assert (x == y).all()
 
 
 def test_attention_long_strides(K):
@@ -446,6 +552,18 @@ def test_engine_one_tensor_twice(eng, same, D):
     for c, t in (("k", K_), ("v", V)):
         if c not in same:
             R.within(eng.grad(t), 2 * ref["g" + c][0], 3 * ref["g" + c][1], "g" + c)
+
+
+def test_engine_refuses_an_output_written_since(eng):
+    L = eng.lib
+    q, k, v, g, _ = attn_inputs((1, 4, 6, 2, 2, 16, None), 24)
+    Q, K_, V = eng.param(q), eng.param(k), eng.param(v)
+    o = L.nc_cross_attention(Q, K_, V, None, c_float(0.25))
+    loss = L.nc_sum(o, abi.ALL_AXES, 0)
+    L.nc_copy_from(o, q.ctypes.data_as(ctypes.c_void_p), q.nbytes)
+    assert L.nc_backward(loss) == abi.ERR_STATE and b"written after the forward" in L.nc_error(eng.ctx)
+    L.nc_clear_error(eng.ctx)
+    eng.step_end()
 
 
 def test_engine_refuses_inputs_written_since(eng):
