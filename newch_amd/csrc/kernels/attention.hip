@@ -145,30 +145,31 @@ struct FwdArgs {
     int qtiles, splits;          // groups of 128 rows of a pair, parts its keys are cut into
 };
 
-template <int DP, int TPS, int OCC>
-__global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
-    constexpr int TB = 128 * DP, STAGE = 2 * TPS * TB;  // bytes of a packed tile; of the keys' and values' of a stage
+template <int DP, int TPS, int OCC, int KG>
+__global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
+    constexpr int TB = 128 * DP, TS = KG * TPS, STAGE = 2 * TS * TB;  // bytes of a packed tile; tiles and bytes of a stage
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = wave_all & (kAttnWaves - 1), kg = wave_all / kAttnWaves;  // tile of queries, group of keys
     const int ra = row_at(lane), ca = col_at(lane);
     const uint32_t lds = lds_address(smem);
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
-        const int qt = (int)(unit % f.qtiles);
         const int64_t rest = unit / f.qtiles;
-        const int split = (int)(rest % f.splits);
+        const int qt = (int)(unit - rest * f.qtiles);
         const int64_t pair = rest / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int split = (int)(rest - pair * f.splits);
         const int64_t n = keys_of(a.Lk, f.key_len, b), nt = (n + kTile - 1) / kTile;
         const int64_t t0 = nt * split / f.splits, t1 = nt * (split + 1) / f.splits;
         const char *kp = f.kp + pair * f.tiles * TB, *vp = f.vp + pair * f.tiles * TB;
         const float *kx = f.kx + pair * f.tiles, *vx = f.vx + pair * f.tiles;
 
         auto copy = [&](int64_t t, int buf) {
-            const int c = (int)min((int64_t)TPS, t1 - t) * (TB / 1024);
+            const int c = (int)min((int64_t)TS, t1 - t) * (TB / 1024);
             const uint32_t at = __builtin_amdgcn_readfirstlane(lds + buf * STAGE);
-            stage_copy(kp + t * TB, at, c);
-            stage_copy(vp + t * TB, at + TPS * TB, c);
+            stage_copy<KG * kAttnWaves>(kp + t * TB, at, c);
+            stage_copy<KG * kAttnWaves>(vp + t * TB, at + TS * TB, c);
         };
         __syncthreads();  // the last unit's stages have been read
         if (t0 < t1) copy(t0, 0);
@@ -183,19 +184,28 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
         load_query(q, f.q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2], live, a.scale, half, (int)a.D);
         Sums<DP> sum;
         sum.clear();
-        for (int64_t t = t0, buf = 0; t < t1; t += TPS, buf ^= 1) {
+        for (int64_t t = t0, buf = 0; t < t1; t += TS, buf ^= 1) {
+            const int64_t tg = t + kg * TPS;  // this group's first tile
             float ek[TPS], ev[TPS];
 #pragma unroll
-            for (int x = 0; x < TPS; x++) ek[x] = scalar_load(kx + min(t + x, t1 - 1)), ev[x] = scalar_load(vx + min(t + x, t1 - 1));
+            for (int x = 0; x < TPS; x++) ek[x] = scalar_load(kx + min(tg + x, t1 - 1)), ev[x] = scalar_load(vx + min(tg + x, t1 - 1));
             stage_wait();
-            if (t + TPS < t1) copy(t + TPS, (int)buf ^ 1);
-            const char *st = smem + buf * STAGE;
+            if (t + TS < t1) copy(t + TS, (int)buf ^ 1);
+            const char *st = smem + buf * STAGE + kg * TPS * TB;
 #pragma unroll
             for (int x = 0; x < TPS; x++) {
-                if (t + x >= t1) break;
-                attend(sum, q, st + x * TB + ra, st + (TPS + x) * TB + ca, ek[x], ev[x], t + x + 1 == nt,
-                       (int)min(n - (t + x) * kTile, (int64_t)kTile) - 4 * half);
+                if (tg + x >= t1) break;
+                attend(sum, q, st + x * TB + ra, st + (TS + x) * TB + ca, ek[x], ev[x], tg + x + 1 == nt,
+                       (int)min(n - (tg + x) * kTile, (int64_t)kTile) - 4 * half);
             }
+        }
+        if constexpr (KG > 1) {  // the second group's sums join the first's through LDS
+            f4 *const hand = (f4 *)smem + wave * (4 * (DP / 32) + 1) * kWave + lane;
+            __syncthreads();  // the last stage has been read
+            if (kg) put(sum, hand);
+            __syncthreads();
+            if (kg) continue;
+            join(sum, hand);
         }
         const float l = halves_sum(sum.l);
         if (live && f.splits == 1) {
@@ -249,8 +259,8 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane % LPK, grp = lane / LPK, D = (int)a.D;
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
-        const int split = (int)(w % f.splits);
         const int64_t pair = w / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int split = (int)(w - pair * f.splits);
         const int64_t n = keys_of(a.Lk, f.key_len, b), nt = (n + kTile - 1) / kTile;
         const int64_t j0 = nt * split / f.splits * kTile, j1 = min(n, nt * (split + 1) / f.splits * kTile);
         const float *kb = k + b * a.sk[0] + u * a.sk[2], *vb = v + b * a.sv[0] + u * a.sv[2];
@@ -494,10 +504,10 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
     f4 *const hand = (f4 *)(smem + 2 * STAGE) + which * 256 + lane;  // p's registers 4 j .. 4 j + 3 at 64 j
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
-        const int kg = (int)(unit % f.groups);
         const int64_t rest = unit / f.groups;
-        const int split = (int)(rest % f.splits);
+        const int kg = (int)(unit - rest * f.groups);
         const int64_t pair = rest / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int split = (int)(rest - pair * f.splits);
         const int64_t n = keys_of(a.Lk, f.key_len, b);
         const int64_t k0 = (int64_t)kg * kAttnWaves + which, key = k0 * kTile + (lane & 31);
         const bool any = (int64_t)kg * kAttnWaves * kTile < n, mine = k0 * kTile < n, live = key < n;
@@ -597,20 +607,21 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
 
 // gq: a wave holds 32 rows of queries as columns, as the forward does, and goes over the tiles of keys: s^T = k q^T and
 // dp^T = v go^T, then gq^T += k^T ds^T.
-template <int DP, int OCC>
-__global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
-    constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * TB;
+template <int DP, int OCC, int KG>
+__global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
+    constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * KG * TB;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = wave_all & (kAttnWaves - 1), kg = wave_all / kAttnWaves;  // tile of queries, group of keys
     const int ra = row_at(lane), ca = col_at(lane);
     const uint32_t lds = lds_address(smem);
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
-        const int qg = (int)(unit % f.groups);
         const int64_t rest = unit / f.groups;
-        const int split = (int)(rest % f.splits);
+        const int qg = (int)(unit - rest * f.groups);
         const int64_t pair = rest / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
+        const int split = (int)(rest - pair * f.splits);
         const int64_t n = keys_of(a.Lk, f.key_len, b), nt = (n + kTile - 1) / kTile;
         const int64_t t0 = nt * split / f.splits, t1 = nt * (split + 1) / f.splits;
         const int64_t qt = (int64_t)qg * kAttnWaves + wave, R = qt * kTile + (lane & 31);
@@ -619,8 +630,9 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
         auto copy = [&](int64_t t, int buf) {
             const uint32_t at = __builtin_amdgcn_readfirstlane(lds + buf * STAGE);
             const int64_t x = (k0 + t) * TB;
-            stage_copy(f.kp + x, at, TB / 1024);
-            stage_copy(f.vp + x, at + TB, TB / 1024);
+            const int c = (int)min((int64_t)KG, t1 - t) * (TB / 1024);
+            stage_copy<KG * kAttnWaves>(f.kp + x, at, c);
+            stage_copy<KG * kAttnWaves>(f.vp + x, at + KG * TB, c);
         };
         __syncthreads();  // the last unit's stages have been read
         if (t0 < t1) copy(t0, 0);
@@ -640,13 +652,14 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
 #pragma unroll
             for (int r = 0; r < 16; r++) dq[t][r] = 0.0f;
         float F = 0x1p100f;
-        for (int64_t t = t0, buf = 0; t < t1; t++, buf ^= 1) {
-            const float ek = scalar_load(f.kx + k0 + t), ev = scalar_load(f.vx + k0 + t);
+        for (int64_t ts = t0, buf = 0; ts < t1; ts += KG, buf ^= 1) {
+            const int64_t t = ts + kg;
+            const float ek = scalar_load(f.kx + k0 + min(t, t1 - 1)), ev = scalar_load(f.vx + k0 + min(t, t1 - 1));
             stage_wait();
-            if (t + 1 < t1) copy(t + 1, (int)buf ^ 1);
-            const char *st = smem + buf * STAGE;
-            if (!mine) continue;
-            const char *kt = st + ra, *vt = st + TB + ra, *kc = st + ca;
+            if (ts + KG < t1) copy(ts + KG, (int)buf ^ 1);
+            const char *st = smem + buf * STAGE + kg * TB;
+            if (!mine || t >= t1) continue;
+            const char *kt = st + ra, *vt = st + KG * TB + ra, *kc = st + ca;
             f16x s, dp;
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
@@ -670,19 +683,41 @@ __global__ __launch_bounds__(kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
                 most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
             }
             const float kap = pow2i((int)ek);
-            float by;
-            if (column_scale(halves_max(most) * kap, F, by)) scale_acc(dq, by);
+            float step;
+            if (column_scale(halves_max(most) * kap, F, step)) scale_acc(dq, step);
             const float kF = kap * F;
 #pragma unroll
             for (int r = 0; r < 16; r++) dp[r] *= kF;
             const Split8 y[2] = {split_regs(dp, 0), split_regs(dp, 8)};
             steps<2 * NT>(x, turned, [&](int k, const Pieces &v) { dq[k % NT] = mfma3(v.hi, v.lo, y[k / NT].hi, y[k / NT].lo, dq[k % NT]); });
         }
+        float by = a.scale / F;
+        if constexpr (KG > 1) {  // the second group's sums are added through LDS
+            f4 *const hand = (f4 *)smem + wave * 4 * NT * kWave + lane;
+            __syncthreads();  // the last stage has been read
+            if (kg) {
+#pragma unroll
+                for (int d = 0; d < NT; d++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) hand[(4 * d + j) * kWave] = f4{dq[d][4 * j], dq[d][4 * j + 1], dq[d][4 * j + 2], dq[d][4 * j + 3]} * by;
+            }
+            __syncthreads();
+            if (kg) continue;
+#pragma unroll
+            for (int d = 0; d < NT; d++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const f4 v = hand[(4 * d + j) * kWave];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) dq[d][4 * j + e] = fma_(dq[d][4 * j + e], by, v[e]);
+                }
+            by = 1.0f;
+        }
         if (R < f.rows) {
             int64_t i, g;
             a.row(R, i, g);
             const int64_t h = u * a.G + g;
-            store_column<true>(f.gq + split * f.part_q + ((b * a.Lq + i) * a.Hq + h) * a.D, dq, t0 < t1, a.scale / F, half, (int)a.D, f.acc_q);
+            store_column<true>(f.gq + split * f.part_q + ((b * a.Lq + i) * a.Hq + h) * a.D, dq, t0 < t1, by, half, (int)a.D, f.acc_q);
         }
     }
 }
@@ -751,11 +786,16 @@ static int attn_splits(int64_t whole, int64_t tiles, int64_t want) {
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
+// Two groups of waves that share a workgroup's rows and take every other tile of keys, joined through LDS: where workgroups of four
+// waves would leave most SIMDs with one wave or none.  (1024 x 1024, 32 heads of 128: forward 75 us, and 96 with one group, forward
+// and backward 307 and 343; 8 heads of 64: 90 and 97.)
+static bool key_groups(int64_t whole, int64_t tiles, int DP) { return DP <= 128 && whole <= kPlanCUs && tiles >= 4; }
+
 constexpr int64_t kTokenRows = 8;  // rows of a pair that k_attn_token takes
 
 struct FwdPlan {
     bool token, few;  // k_attn_token; few keys
-    int DP, qtiles, splits;
+    int DP, qtiles, splits, kg;  // kg: groups of waves that share a workgroup's keys
     int64_t rows, tiles, pairs, units;
     size_t kp, vp, kx, vx, po, pm, total;  // offsets into the workspace
 };
@@ -781,7 +821,8 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
     }
     if (p.token) p.qtiles = 1;
     const int64_t whole = p.pairs * p.qtiles;
-    p.splits = attn_splits(whole, p.tiles, (p.token ? 8 : 2) * kPlanCUs);
+    p.kg = !p.token && key_groups(whole, p.tiles, p.DP);
+    p.splits = attn_splits(whole, p.tiles, (p.token ? 8 : p.kg ? 1 : 2) * kPlanCUs);
     p.units = whole * p.splits;
     const size_t pt = (size_t)(p.pairs * p.tiles);
     size_t at = 0;
@@ -882,8 +923,9 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     if (p.token)
         token_launch(f, k, v, st);
     else
-        NC_ATTN_DP(p.DP, constexpr int TPS = DP <= 64 ? 2 : 1; constexpr int OCC = DP <= 128 ? 2 : 1;
-                   attn_launch(&k_attn_fwd<DP, TPS, OCC>, p.units, 2 * 2 * TPS * 128 * DP, st, f));
+        NC_ATTN_DP(p.DP, constexpr int TPS = DP <= 64 ? 2 : 1; constexpr int OCC = DP <= 128 ? 2 : 1; constexpr int KG = DP <= 128 ? 2 : 1;
+                   if (p.kg) attn_launch(&k_attn_fwd<DP, 1, OCC, KG>, p.units, 2 * 2 * KG * 128 * DP, st, f, KG * kAttnB);
+                   else attn_launch(&k_attn_fwd<DP, TPS, OCC, 1>, p.units, 2 * 2 * TPS * 128 * DP, st, f));
     // a wave a row while that fills the chip at most twice over, or for more than eight parts
     const int64_t all = p.pairs * p.rows, pieces = all * ((D + 3) / 4);
     if (p.splits > 8 || (p.splits > 1 && all <= 16 * kPlanCUs))
@@ -896,7 +938,7 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
 namespace nchip {
 
 struct BwdPlan {
-    bool few;
+    bool few, kg;  // few keys; two groups of waves share a workgroup's keys for gq
     int DP, qgroups, kgroups, qsplits, ksplits;  // splits of the keys for gq, of the queries for gk and gv
     int64_t rows, qtiles, ktiles, pairs, nq, nk;
     size_t kp, vp, qp, gp, kx, vx, qx, gx, stats, pq, pk, pv, total;
@@ -911,7 +953,8 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
     p.ktiles = (Lk + kTile - 1) / kTile;
     p.qgroups = (int)((p.qtiles + kAttnWaves - 1) / kAttnWaves);
     p.kgroups = (int)((p.ktiles + kAttnWaves - 1) / kAttnWaves);
-    p.qsplits = attn_splits(p.pairs * p.qgroups, p.ktiles, kPlanCUs * (p.DP <= 128 ? 2 : 1));
+    p.kg = key_groups(p.pairs * p.qgroups, p.ktiles, p.DP);
+    p.qsplits = attn_splits(p.pairs * p.qgroups, p.ktiles, kPlanCUs * (p.DP <= 128 && !p.kg ? 2 : 1));
     p.ksplits = attn_splits(p.pairs * p.kgroups, p.qtiles, kPlanCUs * (p.DP <= 64 ? 2 : 1));
     p.nq = B * Lq * Hq * D;
     p.nk = B * Lk * Hkv * D;
@@ -1000,7 +1043,9 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
         f.acc_q = cut ? 0 : acc_q;
         f.part_q = p.nq, f.groups = p.qgroups, f.splits = p.qsplits;
         f.units = p.pairs * p.qgroups * p.qsplits;
-        NC_ATTN_DP(p.DP, constexpr int OCC = DP <= 128 ? 2 : 1; attn_launch(&k_attn_dq<DP, OCC>, f.units, 2 * 2 * 128 * DP, st, f));
+        NC_ATTN_DP(p.DP, constexpr int OCC = DP <= 128 ? 2 : 1; constexpr int KG = DP <= 128 ? 2 : 1;
+                   if (p.kg) attn_launch(&k_attn_dq<DP, OCC, KG>, f.units, 2 * 2 * KG * 128 * DP, st, f, KG * kAttnB);
+                   else attn_launch(&k_attn_dq<DP, OCC, 1>, f.units, 2 * 2 * 128 * DP, st, f));
         if (cut) sum_launch(p.nq, p.qsplits, f.gq, gq, acc_q, nullptr, nullptr, 0, st);
     }
     if (want_k) {

@@ -137,14 +137,17 @@ __device__ __forceinline__ int tile_exponent(float most) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
-// four columns of a row of D >= 4 from d on, zeros from column D on: the row's last four, moved down, where it ends among them
-__device__ __forceinline__ f4 last4(const float *row, int d, int D) {
-    const int o = min(d, D - 4), by = d - o;
-    f4 v = *(const f4u *)(row + o);
+__device__ __forceinline__ f4 moved4(f4 v, int by) {  // down by `by` places
     if (by & 1) v = f4{v[1], v[2], v[3], 0.0f};
     if (by & 2) v = f4{v[2], v[3], 0.0f, 0.0f};
     if (by & ~3) v = f4{0.0f, 0.0f, 0.0f, 0.0f};
     return v;
+}
+
+// four columns of a row of D >= 4 from d on, zeros from column D on: the row's last four, moved down, where it ends among them
+__device__ __forceinline__ f4 last4(const float *row, int d, int D) {
+    const int o = min(d, D - 4);
+    return moved4(*(const f4u *)(row + o), d - o);
 }
 
 // eight columns of a row from d on, zeros from column D on
@@ -163,6 +166,39 @@ __device__ __forceinline__ void load8(const float *row, int d, int D, float *x) 
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = p[i], x[4 + i] = q[i];
+}
+
+// N times eight columns of a row, from d0, d0 + step, ... on, zeros from column D on.  All loads are on their way before the first
+// is waited for: addresses are held inside the row rather than branched on (with load8 a wave waits for each in turn: 4096 x 77,
+// 4 x 16 heads of 64, forward: 46 us, and 55 with it).
+template <int N>
+__device__ __forceinline__ void load_chunks(const float *row, int d0, int step, int D, float (&x)[N][8]) {
+    if (D < 4) {  // at most the first chunk's first three
+#pragma unroll
+        for (int k = 0; k < N; k++) load8(row, d0 + k * step, D, x[k]);
+        return;
+    }
+    f4 v[N][2];
+#pragma unroll
+    for (int k = 0; k < N; k++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) v[k][h] = *(const f4u *)(row + min(d0 + k * step + 4 * h, D - 4));
+    if (D % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[k][e] = d0 + k * step + 4 * (e / 4) < D ? v[k][e / 4][e % 4] : 0.0f;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int d = d0 + k * step + 4 * h;
+                const f4 m = moved4(v[k][h], d - min(d, D - 4));
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[k][4 * h + e] = m[e];
+            }
+    }
 }
 
 // four columns of a contiguous row from d on, stored or added
@@ -272,22 +308,18 @@ struct Query {  // the rows times scale log2(e), as the second operand: column f
 template <int DP>
 __device__ __forceinline__ void load_query(Query<DP> &q, const float *row, bool live, float scale, int half, int D) {
     const float c = live ? scale * kLog2e : 0.0f;
-    float most = 0.0f, x[8];
+    float most = 0.0f, x[DP / 16][8];
+    load_chunks(row, 8 * half, 16, D, x);
 #pragma unroll
-    for (int s = 0; s < DP / 16; s++) {
-        load8(row, 16 * s + 8 * half, D, x);
-        most = abs_max(x, most);
-    }
+    for (int s = 0; s < DP / 16; s++) most = abs_max(x[s], most);
     const int e = tile_exponent(halves_max(most) * __builtin_fabsf(c));
     const float by = c * pow2i(-e);
     q.c = pow2i(e);
-    asm volatile("" ::: "memory");  // the row is read again (from the caches) rather than held in fp32 as well
 #pragma unroll
     for (int s = 0; s < DP / 16; s++) {
-        load8(row, 16 * s + 8 * half, D, x);
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] *= by;
-        const Split8 p = split8(x);
+        for (int k = 0; k < 8; k++) x[s][k] *= by;
+        const Split8 p = split8(x[s]);
         q.hi[s] = p.hi, q.lo[s] = p.lo;
     }
 }
@@ -304,6 +336,33 @@ struct Sums {
         m = -INFINITY, l = 0.0f, E = -1000.0f;
     }
 };
+
+// a wave's sums handed to another one through LDS, lane by lane, and joined there to its own
+template <int DP>
+__device__ __forceinline__ void put(const Sums<DP> &a, f4 *to) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) to[(4 * d + j) * kWave] = f4{a.o[d][4 * j], a.o[d][4 * j + 1], a.o[d][4 * j + 2], a.o[d][4 * j + 3]};
+    to[DP / 8 * kWave] = f4{a.m, a.l, a.E, 0.0f};
+}
+template <int DP>
+__device__ __forceinline__ void join(Sums<DP> &a, const f4 *from) {
+    const f4 b = from[DP / 8 * kWave];
+    const float m = __builtin_fmaxf(a.m, b[0]), E = __builtin_fmaxf(a.E, b[2]);
+    const float wa = a.m == m ? 1.0f : __builtin_amdgcn_exp2f(a.m - m), wb = b[0] == m ? 1.0f : __builtin_amdgcn_exp2f(b[0] - m);
+    const float oa = wa * __builtin_amdgcn_exp2f(a.E - E), ob = wb * __builtin_amdgcn_exp2f(b[2] - E);
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const f4 v = from[(4 * d + j) * kWave];
+#pragma unroll
+            for (int e = 0; e < 4; e++) a.o[d][4 * j + e] = fma_(a.o[d][4 * j + e], oa, v[e] * ob);
+        }
+    a.l = fma_(a.l, wa, b[1] * wb);
+    a.m = m, a.E = E;
+}
 
 // kt, vt: the tile's keys and values in LDS, at this lane's row_at and col_at; ek, ev: their exponents; left: keys of the tile
 // that count (32 but in the last one), less 4 half

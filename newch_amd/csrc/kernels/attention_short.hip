@@ -16,9 +16,9 @@ __device__ __forceinline__ float wave_tile(const float *src, int64_t step, int r
     const bool live = row0 + r < n;
     const float *row = src + (live ? row0 + r : 0) * step;
     float x[PER][8], most = 0.0f;
+    load_chunks(row, 8 * half, 16, D, x);
 #pragma unroll
     for (int k = 0; k < PER; k++) {
-        load8(row, 16 * k + 8 * half, D, x[k]);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[k][e] = live ? x[k][e] : 0.0f;
         most = abs_max(x[k], most);
