@@ -82,24 +82,40 @@ __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd
     }
 }
 
+// A lane's place in a packed tile for fragments of the 16x16x32 product whose rows are summed over: 16 lanes take rows 8 (l / 16)
+// .. + 3 and, at the place ^ 64, the next four, of 16 columns (tile t: + 1024 t), without bank conflicts.
+__device__ __forceinline__ int turned_at(int lane) {
+    const int i = lane & 15, odd = (i >> 1) & 1;
+    return 512 * odd + 16 * ((8 * (lane >> 4) + i / 4) ^ (4 * odd)) + 8 * (i & 1);
+}
+__device__ __forceinline__ h8 turned16(const char *first, const char *second) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)first);
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)second);
+    return __builtin_bit_cast(h8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+}
+
+constexpr int kDsTile = 4096;  // bytes of a packed tile of 32 columns
+
 // Backward in one pass over the queries: every wave holds 32 keys, the workgroup splits a tile of queries and output gradients
-// (the next one's on their way meanwhile), and each wave takes its part of gk and gv as k_attn_dkv does, then turns its ds in LDS
-// and multiplies it with its keys; the waves' parts of gq are added in wave order.
+// (the next one's on their way meanwhile), and each wave takes its part of gk and gv as k_attn_dkv does.  It leaves its ds in LDS,
+// and the waves share the blocks of gq^T = k^T ds^T over all keys.
 template <int DP, int W>
 __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP;
     constexpr int THREADS = W * kWave, UNITS = 4 * DP, PER = (UNITS + THREADS - 1) / THREADS;  // 8-column pieces of a tile
-    constexpr int LD = DP + 4, PART = 32 * LD * 4;  // a wave's part of gq: 32 rows, which also holds ds turned, and at first a tile
-    constexpr int LDS_DS = 36;
-    static_assert(PART >= TB && PART >= 32 * LDS_DS * 4, "a wave's part holds a tile and a turned ds");
+    constexpr int BLOCKS = DP / 8, PW = (BLOCKS + W - 1) / W;  // 16 x 16 blocks of a tile's gq, of a wave
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // q's tile, go's tile, the waves' parts, then small tables
-    char *const qs = smem, *const gs = smem + TB, *const parts = smem + 2 * TB;
-    float *const small = (float *)(parts + W * PART);
+    // q's tile, go's tile, the waves' keys, their ds, then small tables
+    char *const qs = smem, *const gs = smem + TB, *const keys = smem + 2 * TB, *const dss = keys + W * TB;
+    float *const small = (float *)(dss + W * kDsTile);
     float *const stats = small, *const dots = small + 64, *const red = dots + (DP / 8) * 32;  // [64], [DP / 8][32], [2][W]
+    f2 *const dsx = (f2 *)(red + 2 * W);  // [W]: the scales of the waves' ds, and of their keys
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int ra = row_at(lane), ca = col_at(lane), D = (int)a.D;
+    const int ra = row_at(lane), ca = col_at(lane), ta = turned_at(lane), D = (int)a.D;
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t pair = w / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
         const int split = (int)(w - pair * f.splits);
@@ -107,7 +123,7 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
         const int64_t t0 = f.qtiles * split / f.splits, t1 = f.qtiles * (split + 1) / f.splits;
         // workgroups that share a CU give the first tiles of keys (the only ones of a short sequence) to other waves, so to other SIMDs
         const int kw = (wave + (int)(w >> 8) * (W / 2)) & (W - 1), key = kw * kTile + (lane & 31);
-        char *const part = parts + kw * PART;
+        char *const kt = keys + kw * TB, *const mine_ds = dss + kw * kDsTile;
         const bool mine = kw < nt, live = key < n;
 
         // the next tile's pieces: piece p is columns 8 (p / 32) .. + 7 of row p % 32
@@ -129,21 +145,17 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
                 if (k == 0) nl = p < 32 && in ? f.lse[(b * a.Hq + h) * a.Lq + i] * kLog2e : INFINITY;
             }
         };
-        __syncthreads();  // the last unit's parts have been read
+        __syncthreads();  // the last unit's keys have been read
         if (t0 < t1) fetch(t0);
-        h8 kh[KS], kl[KS], vh[KS], vl[KS], ch[2][NT], cl[2][NT];
+        h8 kh[KS], kl[KS], vh[KS], vl[KS];
         float ek = 0.0f, ev = 0.0f;
-        if (mine) {  // this wave's keys and values, through its part of LDS
-            ek = wave_tile<DP>(f.k + b * a.sk[0] + u * a.sk[2], a.sk[1], kw * kTile, n, D, part);
+        if (mine) {  // this wave's values, through the place of its keys, and its keys, which stay
+            ev = wave_tile<DP>(f.v + b * a.sv[0] + u * a.sv[2], a.sv[1], kw * kTile, n, D, kt);
 #pragma unroll
-            for (int s = 0; s < KS; s++) kh[s] = row_frag(part + ra, s), kl[s] = row_frag(part + ra + LO, s);
+            for (int s = 0; s < KS; s++) vh[s] = row_frag(kt + ra, s), vl[s] = row_frag(kt + ra + LO, s);
+            ek = wave_tile<DP>(f.k + b * a.sk[0] + u * a.sk[2], a.sk[1], kw * kTile, n, D, kt);
 #pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int t = 0; t < NT; t++) ch[s][t] = col_frag(part + ca, s, t), cl[s][t] = col_frag(part + ca + LO, s, t);
-            ev = wave_tile<DP>(f.v + b * a.sv[0] + u * a.sv[2], a.sv[1], kw * kTile, n, D, part);
-#pragma unroll
-            for (int s = 0; s < KS; s++) vh[s] = row_frag(part + ra, s), vl[s] = row_frag(part + ra + LO, s);
+            for (int s = 0; s < KS; s++) kh[s] = row_frag(kt + ra, s), kl[s] = row_frag(kt + ra + LO, s);
         }
         f16x dk[NT], dv[NT];
 #pragma unroll
@@ -222,10 +234,27 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
                         most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
                     }
                 }
-                // ds, 2^-sh times: for gq as it is, one row of queries after another
-                float *turned = (float *)part + (lane & 31);
+                // ds for gq, in two pieces: a tile of 32 rows of keys, its columns the rows of queries
+                float finite = most;
+                if (__builtin_expect(most == INFINITY, 0)) {  // a row of queries with an infinity leaves the others their scale
+                    finite = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 16; r++) turned[(8 * (r / 4) + 4 * half + r % 4) * LDS_DS] = dp[r];
+                    for (int r = 0; r < 16; r++) finite = __builtin_fmaxf(finite, __builtin_fabsf(dp[r]) < INFINITY ? __builtin_fabsf(dp[r]) : 0.0f);
+                }
+                const int ed = tile_exponent(wave_max_nan_skip(finite));
+                const float id = pow2i(-ed);
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[e] = dp[4 * j + e] * id;
+                    const Split8 x = split8(y);
+                    char *const at = mine_ds + 512 * j + 8 * half;
+                    const int r0 = 16 * (lane & 31), r1 = r0 ^ 64;
+                    *(h4 *)(at + r0) = x.hi.lo, *(h4 *)(at + 512 + r1) = x.hi.hi;
+                    *(h4 *)(at + 2048 + r0) = x.lo.lo, *(h4 *)(at + 2560 + r1) = x.lo.hi;
+                }
+                if (lane == 0) dsx[kw] = f2{__builtin_amdgcn_exp2f((float)ed - sh), pow2i((int)ek) * a.scale};
                 const float kap = __builtin_amdgcn_exp2f((float)eq - sh);
                 float by;
                 if (column_scale(halves_max(most) * kap, F, by)) scale_acc(dk, by);
@@ -243,53 +272,37 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
                                   if (k % 2) dk[d] = mfma3(x.hi, x.lo, ds[r].hi, ds[r].lo, dk[d]);
                                   else dv[d] = mfma3(x.hi, x.lo, ps[r].hi, ps[r].lo, dv[d]);
                               });
-                // gq^T of this wave's keys: k^T ds^T, a lane a row of queries
-                float x[2][8], top = 0.0f;
-                const float *row = (const float *)part + (lane & 31) * LDS_DS + 4 * half;
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const f4 lo = *(const f4 *)(row + 16 * k), hi = *(const f4 *)(row + 16 * k + 8);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[k][e] = lo[e], x[k][4 + e] = hi[e];
-                        top = __builtin_fmaxf(top, __builtin_fmaxf(__builtin_fabsf(lo[e]), __builtin_fabsf(hi[e])));
-                    }
-                }
-                float Fq = 0x1p100f, by_q;
-                column_scale(halves_max(top), Fq, by_q);
-                f16x dq[NT];
-#pragma unroll
-                for (int d = 0; d < NT; d++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) dq[d][r] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[k][e] *= Fq;
-                    const Split8 y = split8(x[k]);
-#pragma unroll
-                    for (int d = 0; d < NT; d++) dq[d] = mfma3(ch[k][d], cl[k][d], y.hi, y.lo, dq[d]);
-                }
-                const float back = __builtin_amdgcn_exp2f(ek - sh) / Fq * a.scale;
-                float *mypart = (float *)part + (lane & 31) * LD + 4 * half;
-#pragma unroll
-                for (int d = 0; d < NT; d++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        *(f4 *)(mypart + 32 * d + 8 * j) = f4{dq[d][4 * j] * back, dq[d][4 * j + 1] * back, dq[d][4 * j + 2] * back, dq[d][4 * j + 3] * back};
             }
             __syncthreads();
-            if (f.gq) {
-                for (int p = threadIdx.x; p < 32 * DP / 4; p += THREADS) {
-                    const int r = p / (DP / 4), d = 4 * (p - r * (DP / 4));
-                    const int64_t R = t * kTile + r;
-                    if (R >= f.rows || d >= D) continue;
-                    f4 sum = {0.f, 0.f, 0.f, 0.f};
-                    for (int x = 0; x < nt; x++) sum += *(const f4 *)((const float *)(parts + x * PART) + r * LD + d);
+            if (f.gq) {  // gq^T = k^T ds^T over all keys, blocks of 16 columns and 16 rows of queries
+                f4 sum[PW];
+#pragma unroll
+                for (int x = 0; x < PW; x++) sum[x] = f4{0.f, 0.f, 0.f, 0.f};
+                for (int y = 0; y < nt; y++) {
+                    const f2 by = dsx[y];
+#pragma unroll
+                    for (int x = 0; x < PW; x++) {
+                        const int block = wave + x * W, c = block % (DP / 16), r = block / (DP / 16);
+                        if (BLOCKS % W && block >= BLOCKS) break;
+                        const char *const kc = keys + y * TB + 1024 * c + ta, *const dc = dss + y * kDsTile + 1024 * r + ta;
+                        const char *const kc2 = keys + y * TB + 1024 * c + (ta ^ 64), *const dc2 = dss + y * kDsTile + 1024 * r + (ta ^ 64);
+                        const h8 ah = turned16(kc, kc2), al = turned16(kc + LO, kc2 + LO), bh = turned16(dc, dc2), bl = turned16(dc + 2048, dc2 + 2048);
+                        f4 v = {0.f, 0.f, 0.f, 0.f};
+                        v = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, v, 0, 0, 0);
+                        v = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, v, 0, 0, 0);
+                        v = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, v, 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sum[x][e] = fma_(v[e] * by.x, by.y, sum[x][e]);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < PW; x++) {
+                    const int block = wave + x * W, c = block % (DP / 16), r = block / (DP / 16);
+                    const int64_t R = t * kTile + 16 * r + (lane & 15);
+                    if (block >= BLOCKS || R >= f.rows) continue;
                     int64_t i, g;
                     a.row(R, i, g);
-                    const int64_t h = u * a.G + g;
-                    store4(f.gq + ((b * a.Lq + i) * a.Hq + h) * D, d, D, sum, f.acc_q);
+                    store4(f.gq + ((b * a.Lq + i) * a.Hq + u * a.G + g) * D, 16 * c + 4 * (lane >> 4), D, sum[x], f.acc_q);
                 }
             }
         }
@@ -321,7 +334,7 @@ void short_fwd(const ShortFwd &f, int DP, hipStream_t st) {
 
 template <int DP, int W>
 static void bwd_launch(const ShortBwd &f, hipStream_t st) {
-    const size_t lds = 2 * 128 * DP + (size_t)W * 32 * (DP + 4) * 4 + (64 + DP / 8 * 32 + 2 * W) * sizeof(float);
+    const size_t lds = 2 * 128 * DP + (size_t)W * (128 * DP + kDsTile) + (64 + DP / 8 * 32 + 4 * W) * sizeof(float);
     launch(&k_attn_short_bwd<DP, W>, f.units, W * kWave, lds, st, f);
 }
 
