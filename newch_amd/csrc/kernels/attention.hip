@@ -7,7 +7,12 @@
 //
 // A sequence without keys gives o = 0, lse = -inf and no gradient.  Keys and values past a sequence's length are not read.
 //
-// The products run on the fp16 matrix cores with operands in two pieces (attention.hpp), packed once into a workspace.
+// A value that counts and is not finite makes the results that meet it NaN.
+//
+// The products run on the fp16 matrix cores with operands in two pieces (attention.hpp), packed once into a workspace, where
+// they bound the time: three products for one reach at most a third of a library's fp16 product of 8192^3, 1.23 PFLOP/s, which
+// is 2.7 times what its fp32 product reaches.  Few rows of queries (k_attn_token) are bound by reading the keys, few keys
+// (attention_short.hip) by the chain of one tile's steps.
 #include "attention.hpp"
 #include "attention_short.hpp"
 
@@ -18,7 +23,7 @@
 namespace nchip {
 
 // ------------------------------------------------------------------------------------------------
-// packing: a workgroup a tile of 32 rows
+// packing: a workgroup a tile of 32 rows; bound by memory (8192 keys and values of 16 heads of 128, 134 MB each way: 57 us, 4.7 TB/s)
 // ------------------------------------------------------------------------------------------------
 // Rows of a (sequence, head of keys) pair: queries' row R is token R / G of query head u G + R % G, keys' are tokens.
 struct PackJob {
@@ -145,6 +150,10 @@ struct FwdArgs {
     int qtiles, splits;          // groups of 128 rows of a pair, parts its keys are cut into
 };
 
+// A workgroup's waves hold 32 rows of queries each, so that a stage of TPS tiles of keys and values comes from L2 once for 128
+// rows, the next one on its way meanwhile.  Two waves a SIMD (what the registers allow) run one's exponentials beside the other's
+// products: from two workgroups, or from KG = 2 groups of waves of one, which take every other stage (key_groups below).  8192 x
+// 8192, 16 heads of 128: 1.50 ms, 1.10 PFLOP/s of fp16 products.
 template <int DP, int TPS, int OCC, int KG>
 __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
     constexpr int TB = 128 * DP, TS = KG * TPS, STAGE = 2 * TS * TB;  // bytes of a packed tile; tiles and bytes of a stage
@@ -227,7 +236,8 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
 // Bound by reading keys and values once.  LPK lanes hold a key's columns, two 16-byte pieces each, for NR rows of queries at once
 // (the query heads that share the keys); each group of LPK lanes keeps its own running maximum, sum and o over the keys that it
 // sees, U of them in flight, and the groups, waves and parts are joined at the end.  All in fp32 on the vector unit: 8 rows of
-// 128 columns still take less time than the keys' way from memory.
+// 128 columns still take less time than the keys' way from memory.  1500 keys, 8 x 12 heads of 64: 16 us (4.5 TB/s) and 4 for the
+// join; up to 16384 keys, 16 x 8 heads of 128, four rows: 215 to 230 us (5.0 to 5.3 TB/s).
 template <int LPK>
 __device__ __forceinline__ float lanes_sum(float v) {  // over LPK neighbours
     v += dpp_f32<kDppXor1>(v, 0.0f);
@@ -489,8 +499,8 @@ struct BwdArgs {
 // gk and gv: two waves share 32 keys as columns and go over the tiles of queries.  One takes s = q k^T and p, whose rows are queries,
 // hands p over through LDS and sums gv^T += go^T p; the other takes dp = go v^T, makes ds of it and sums gk^T += q^T ds.  Each keeps
 // half of the fragments and of the sums, so that two waves fit a SIMD: one's exponentials run under the other's products (128
-// columns, 16 heads, 2048 x 4096 with heads of 128: 0.77 ms, and 0.90 with one wave that does both).  Padded rows of queries have an infinite
-// log-sum-exp: p = 0.
+// columns, 2 x 16 heads on 4, 2048 x 4096: 0.77 ms, and 0.90 with one wave that does both; 0.72 ms with the fragments read ahead,
+// 1.15 PFLOP/s).  Padded rows of queries have an infinite log-sum-exp: p = 0.
 template <int DP, int OCC>
 __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * TB + 256;
@@ -606,7 +616,8 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
 }
 
 // gq: a wave holds 32 rows of queries as columns, as the forward does, and goes over the tiles of keys: s^T = k q^T and
-// dp^T = v go^T, then gq^T += k^T ds^T.
+// dp^T = v go^T, then gq^T += k^T ds^T.  The same sizes: 0.61 ms, 1.02 PFLOP/s (the queries' and gradients' fragments fill the
+// registers, so fewer reads are ahead).
 template <int DP, int OCC, int KG>
 __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * KG * TB;
@@ -722,7 +733,8 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
     }
 }
 
-// out (+)= the splits' parts [split][n], in order; one or two tensors of one size
+// out (+)= the splits' parts [split][n], in order; one or two tensors of one size.  Bound by memory (two parts of 2 x 1.2 million
+// floats: 7 us, 4.1 TB/s).
 struct SumArgs {
     const float *part[2];
     float *out[2];
