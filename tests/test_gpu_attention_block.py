@@ -247,6 +247,7 @@ PATH_SHAPES = [(1, 900, 40, 6, 2, 64, (33,)), (2, 130, 200, 4, 2, 64, (200, 131)
                (2, 1, 600, 5, 1, 101, (0, 600)), (1, 1, 900, 3, 3, 255, None), (1, 2000, 50, 1, 1, 128, (45,)),
                (1, 40, 3000, 1, 1, 64, (2990,)), (1, 300, 290, 2, 1, 200, (285,)), (1, 9, 2100, 3, 3, 48, None),
                (1, 33, 260, 5, 5, 64, None), (300, 5, 9, 4, 2, 16, None), (1, 4, 4, 64, 1, 64, None),
+               (1, 900, 70, 6, 2, 128, (65,)), (2, 100, 128, 2, 2, 90, (128, 31)), (1, 2000, 140, 1, 1, 128, (135,)),
                # more than a workgroup a CU
                (40, 10, 300, 7, 7, 64, tuple(range(290, 250, -1))), (33, 9, 161, 8, 8, 128, tuple(range(0, 165, 5))),
                (260, 9, 520, 1, 1, 30, None), (130, 9, 200, 2, 2, 90, None)]
