@@ -488,6 +488,9 @@ static void launch(F *kernel, int64_t units, int threads, size_t lds, hipStream_
 void short_fwd(const ShortFwd &f, int DP, hipStream_t st) {
     const size_t lds = (size_t)f.tiles * 2 * tile_bytes(DP) + 2 * f.tiles * sizeof(float);
     if (DP == 32) launch(&k_attn_short_fwd<32, 8, 4>, f.units, 512, lds, st, f);
+    // three workgroups of four waves a CU where their keys fit its LDS, else eight waves over one copy (heads of 64, both ways: 4096
+    // x 77, 4 x 16 heads 147 us with four and 153 with eight, 64 x 64, 64 x 8 35 and 39; 197 x 197, 8 x 12 heads 60 and 58)
+    else if (DP == 64 && 3 * lds <= 160 * 1024) launch(&k_attn_short_fwd<64, 4, 3>, f.units, 256, lds, st, f);
     else if (DP == 64) launch(&k_attn_short_fwd<64, 8, 2>, f.units, 512, lds, st, f);
     else if (DP == 96) launch(&k_attn_short_fwd<96, 8, 2>, f.units, 512, lds, st, f);
     else launch(&k_attn_short_fwd<128, 8, 2>, f.units, 512, lds, st, f);
