@@ -38,8 +38,8 @@ __device__ __forceinline__ void tile_split(float (&x)[DP / 16][8], int ex, char 
 }
 
 // Forward: keys and values of a pair stay in LDS, and each wave goes over tiles of queries by itself.  4096 x at most 77, 4 x 16
-// heads of 64: 43 to 46 us for 136 MB (3.1 TB/s) -- a wave reads its rows, multiplies and stores in turn, and two waves a SIMD
-// do not cover all of it.
+// heads of 64: 42 to 44 us for 136 MB (3.2 TB/s) -- a wave reads its rows, multiplies and stores in turn, and the three
+// waves of a SIMD do not cover all of it.
 template <int DP, int W, int OCC>
 __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd f) {
     constexpr int TB = 128 * DP;
@@ -239,7 +239,7 @@ __device__ __forceinline__ void gq_blocks(const ShortBwd &f, int64_t b, int64_t 
 
 // Backward in one pass over the queries: every wave holds 32 keys, the workgroup splits a tile of queries and output gradients
 // (the next one's on their way meanwhile), and each wave takes its part of gk and gv as k_attn_dkv does.  It leaves its ds in LDS,
-// and the waves share the blocks of gq^T = k^T ds^T over all keys.  The same sizes: 100 to 105 us, and 120 to 125 with every
+// and the waves share the blocks of gq^T = k^T ds^T over all keys.  The same sizes: 97 to 104 us, and 120 to 125 with every
 // wave's part of gq added in LDS; memory would take 57.  A tile's steps follow each other (read, split, scores, gradients, store), two
 // workgroups a CU, by the registers, which hold heads of 64 columns and no more.
 template <int DP, int W>

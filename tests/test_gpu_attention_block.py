@@ -260,11 +260,38 @@ def test_attention_paths(K, shape):
     check_attention(run_attention(K, shape, q, k, v, g, lens, "bhld", 2, 3), ref)
 
 
+@pytest.mark.parametrize("shape", [(2, 70, 45, 4, 2, 64, (45, 3)), (1, 300, 100, 2, 2, 128, (70,)), (1, 90, 400, 2, 1, 96, None)], ids=str)
 @pytest.mark.parametrize("want", ["q", "k", "v", "qv", ""])
-def test_attention_some_gradients(K, want):
-    shape = (2, 70, 45, 4, 2, 64, (45, 3))
+def test_attention_some_gradients(K, want, shape):
     q, k, v, g, lens = attn_inputs(shape, 12)
-    check_attention(run_attention(K, shape, q, k, v, g, lens, want=want), R.attention64(q, k, v, lens, 0.125, g))
+    check_attention(run_attention(K, shape, q, k, v, g, lens, want=want), R.attention64(q, k, v, lens, shape[5] ** -0.5, g))
+
+
+@pytest.mark.parametrize("value", [np.inf, np.nan])
+@pytest.mark.parametrize("shape", [(1, 70, 45, 2, 2, 64, None), (1, 70, 45, 2, 2, 128, None), (1, 70, 300, 2, 2, 64, None)], ids=str)
+def test_attention_infinite_gradient_stays_in_its_row(K, shape, value):
+    """An output gradient that is not finite leaves the other rows' gradients of the queries, and other heads', as they are."""
+    q, k, v, g, lens = attn_inputs(shape, 33)
+    g[0, 5, 0] = 0
+    ref = R.attention64(q, k, v, lens, shape[5] ** -0.5, g)
+    g[0, 5, 0] = value
+    B, Lq, Lk, Hq, Hkv, D, _ = shape
+    Q, K_, V, G = (up(t) for t in (q, k, v, g))
+    src = (Q.ptr, (Lq * Hq * D, Hq * D, D), K_.ptr, (Lk * Hkv * D, Hkv * D, D), V.ptr, (Lk * Hkv * D, Hkv * D, D), None)
+    o, lse, outs = Out(q.shape), Out((B, Hq, Lq)), [Out(t.shape) for t in (q, k, v)]
+    n1, n2 = K.cross_attention_fwd_workspace(*shape[:6]), K.cross_attention_bwd_workspace(*shape[:6])
+    ws = DeviceBuffer.empty(max(n1, n2, 1))
+    K.cross_attention_fwd(*shape[:6], D ** -0.5, *src, o.ptr, lse.ptr, ws.ptr, n1)
+    K.cross_attention_bwd(*shape[:6], D ** -0.5, *src, o.ptr, lse.ptr, G.ptr, *(t.ptr for t in outs), ws.ptr, n2, accumulate=False)
+    synchronize()
+    gq, gk, gv = (t.get() for t in outs)
+    rest = np.ones(gq.shape[:3], bool)
+    rest[0, 5, 0] = False
+    assert not np.isfinite(gq[0, 5, 0]).any()
+    R.within(gq[rest], ref["gq"][0][rest], ref["gq"][1][rest], "gq")
+    for name, t in (("gk", gk), ("gv", gv)):
+        R.within(t[:, :, 1], ref[name][0][:, :, 1], ref[name][1][:, :, 1], name)
+        assert not np.isfinite(t[0, :, 0]).any()
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
