@@ -914,8 +914,8 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     if (B == 0 || Lq == 0) return NC_HIP_OK;
     if (!q || !o || (Lk && (!k || !v))) return set_error(NC_HIP_ERR_ARG, "%s: q, k, v and o are needed", what);
     const FwdPlan p = fwd_plan(B, Lq, Lk, Hq, Hkv, D);
-    if (p.total && (!ws || ws_bytes < p.total))
-        return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, p.total);
+    if (p.total && (!ws || ws_bytes < p.total || (uintptr_t)ws % 16))
+        return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, 16-byte aligned", what, p.total);
     hipStream_t st = as_stream(stream);
     char *const w = (char *)ws;
     if (p.few) {
@@ -1019,8 +1019,8 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
     const bool want_q = gq && Lq, want_k = (gk || gv) && Lk;
     if (!want_q && !want_k) return NC_HIP_OK;
     const BwdPlan p = bwd_plan(B, Lq, Lk, Hq, Hkv, D);
-    if (p.total && (!ws || ws_bytes < p.total))
-        return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, p.total);
+    if (p.total && (!ws || ws_bytes < p.total || (uintptr_t)ws % 16))
+        return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, 16-byte aligned", what, p.total);
     hipStream_t st = as_stream(stream);
     char *const w = (char *)ws;
     if (p.few) {

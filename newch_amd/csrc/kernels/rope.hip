@@ -491,8 +491,8 @@ extern "C" NC_HIP_API int nc_hip_qk_norm_rope_bwd(int64_t B, int64_t L, int64_t 
     const bool cols = gwq || gwk, empty = a.tokens == 0 || H == 0;
     if (!empty && (!x || !sx || !gy || !gx)) return set_error(NC_HIP_ERR_ARG, "%s: x, sx, gy and gx are needed", what);
     const size_t need = cols ? nc_hip_qk_norm_rope_bwd_workspace(B, L, H, D) : 0;
-    if (need && (!ws || ws_bytes < need))
-        return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+    if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 16))
+        return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, 16-byte aligned", what, need);
     int n = 0;
     if (!empty) {
         a.q_heads = (int)q_heads;

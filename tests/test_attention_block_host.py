@@ -141,6 +141,16 @@ def test_kernel_layer_refusals():
     no("are needed", attn, k=None)
     no("are needed", K.cross_attention_bwd, 1, 1, 1, 2, 1, 8, 1.0, p, s, p, s, p, s, None, p, None, p, p, p, p)
     attn(Lq=0, q=None)
+    # a workspace that is too small, or not at a multiple of 16 bytes
+    sizes = (1, 40, 600, 2, 2, 64)
+    for name, need, args in (("fwd", K.cross_attention_fwd_workspace(*sizes), (None, p, None)),
+                             ("bwd", K.cross_attention_bwd_workspace(*sizes), (None, p, p, p, p, p, p))):
+        assert need > 0
+        call = getattr(K, "cross_attention_" + name)
+        for ws, n in ((p, need - 1), (p + 8, need), (None, need)):
+            no("workspace of .* 16-byte", call, *sizes, 1.0, p, s, p, s, p, s, *args, ws, n)
+    need = K.qk_norm_rope_bwd_workspace(1, 1, 2, 8)
+    no("workspace of .* 16-byte", K.qk_norm_rope_bwd, 1, 1, 2, 8, 1, p, s, p, p, 0.0, p, 0, (8,), 1e4, 0, p, p, p, p, p + 8, need)
 
 
 # ---- the references themselves -----------------------------------------------------------------------------------
