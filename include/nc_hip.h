@@ -331,8 +331,8 @@ NC_HIP_API int nc_hip_qk_norm_rope_bwd(int64_t B, int64_t L, int64_t H, int64_t 
  * keys; lse [B, Hq, Lq] (may be NULL): log sum exp of the scaled products, for the backward.
  * Backward, from the forward's inputs, o and lse: gq [B, Lq, Hq, D], gk and gv [B, Lk, Hkv, D] (contiguous, not overlapping, each
  * may be NULL) (+)= ..., zeros for keys that do not count; sums in a fixed order.  A value that counts and is not finite makes the
- * results that meet it NaN.  Outputs do not overlap inputs; the workspace is 16-byte aligned; calls that may overlap need workspaces of their own.  No counterpart
- * in the reference (its attention is bmm, masked_fill, softmax and bmm). */
+ * results that meet it NaN.  Outputs do not overlap inputs; the workspace is 16-byte aligned; calls that may overlap need workspaces
+ * of their own.  No counterpart in the reference (its attention is bmm, masked_fill, softmax and bmm). */
 NC_HIP_API size_t nc_hip_cross_attention_fwd_workspace(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv,
                                                        int64_t D);
 NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D,
