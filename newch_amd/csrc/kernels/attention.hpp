@@ -313,7 +313,8 @@ __device__ __forceinline__ void load_query(Query<DP> &q, const float *row, bool 
     load_chunks(row, 8 * half, 16, D, x);
 #pragma unroll
     for (int s = 0; s < DP / 16; s++) most = abs_max(x[s], most);
-    const int e = tile_exponent(halves_max(most) * __builtin_fabsf(c));
+    // c 2^-e stays finite where the row is all but zero
+    const int e = max(tile_exponent(halves_max(most) * __builtin_fabsf(c)), tile_exponent(__builtin_fabsf(c)) - 98);
     const float by = c * pow2i(-e);
     q.c = pow2i(e);
 #pragma unroll

@@ -302,6 +302,16 @@ def test_attention_scales_and_sharp_rows(K, scale):
     check_attention(run_attention(K, shape, q, k, v, g, lens, scale=scale), R.attention64(q, k, v, lens, scale, g))
 
 
+@pytest.mark.parametrize("shape", [(1, 40, 90, 2, 2, 64, None), (1, 40, 300, 2, 2, 64, None), (1, 2, 90, 1, 1, 64, None)], ids=str)
+@pytest.mark.parametrize("scale", [300.0, 1e6])
+def test_attention_large_scale_and_rows_of_zeros(K, shape, scale):
+    """A query of zeros weighs its keys alike whatever the scale; the others hold what the scale takes."""
+    q, k, v, g, lens = attn_inputs(shape, 34)
+    q *= np.float32(0.125 / scale)
+    q[0, 1] = 0
+    check_attention(run_attention(K, shape, q, k, v, g, lens, scale=scale), R.attention64(q, k, v, lens, scale, g))
+
+
 @pytest.mark.parametrize("mag", [1e-12, 1e12])
 def test_attention_magnitudes(K, mag):
     """Values and gradients of any magnitude, keys and queries whose magnitudes cancel: the pieces' scales follow them."""
