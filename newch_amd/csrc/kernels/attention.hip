@@ -549,6 +549,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[t][r] = 0.0f;
         float F = 0x1p100f, E = -1000.0f;
+        const ScaleParts parts(a.scale);
         for (int64_t t = t0, buf = 0; t < t1; t++, buf ^= 1) {
             const float ex = scalar_load(f.gx + q0 + t), eq = scalar_load(f.qx + q0 + t);
             stage_wait();
@@ -587,7 +588,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
             lds_barrier();  // p is there (the next stage's copies stay on their way)
             if (!mine) continue;
             if (ds_wave) {
-                const float c = ck * pow2i((int)ex), kap = __builtin_amdgcn_exp2f(eq - sh);
+                const float c = ck * pow2i((int)ex), kap = parts.times(eq - sh);
                 float most = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -600,8 +601,8 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                     }
                 }
                 float by;
-                if (column_scale(halves_max(most) * kap, F, by)) scale_acc(acc, by);
-                const float kF = kap * F;
+                if (column_scale(halves_max(most) * __builtin_fabsf(kap), F, by)) scale_acc(acc, by);
+                const float kF = finite_product(kap, F);
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[r] *= kF;
             }
@@ -611,7 +612,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
         float *const out = ds_wave ? f.gk : f.gv;
         if (out && key < a.Lk)
             store_column<true>(out + split * f.part_k + ((b * a.Lk + key) * a.Hkv + u) * a.D, acc, live && t0 < t1,
-                               ds_wave ? a.scale / F : __builtin_amdgcn_exp2f(E - 14.0f), half, (int)a.D, ds_wave ? f.acc_k : f.acc_v);
+                               ds_wave ? 1.0f / F : __builtin_amdgcn_exp2f(E - 14.0f), half, (int)a.D, ds_wave ? f.acc_k : f.acc_v);
     }
 }
 
@@ -663,6 +664,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
 #pragma unroll
             for (int r = 0; r < 16; r++) dq[t][r] = 0.0f;
         float F = 0x1p100f;
+        const ScaleParts parts(a.scale);
         for (int64_t ts = t0, buf = 0; ts < t1; ts += KG, buf ^= 1) {
             const int64_t t = ts + kg;
             const float ek = scalar_load(f.kx + k0 + min(t, t1 - 1)), ev = scalar_load(f.vx + k0 + min(t, t1 - 1));
@@ -693,16 +695,16 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
                 dp[r] = p * fma_(dp[r], c2, -de);
                 most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
             }
-            const float kap = pow2i((int)ek);
+            const float kap = parts.times(ek);
             float step;
-            if (column_scale(halves_max(most) * kap, F, step)) scale_acc(dq, step);
-            const float kF = kap * F;
+            if (column_scale(halves_max(most) * __builtin_fabsf(kap), F, step)) scale_acc(dq, step);
+            const float kF = finite_product(kap, F);
 #pragma unroll
             for (int r = 0; r < 16; r++) dp[r] *= kF;
             const Split8 y[2] = {split_regs(dp, 0), split_regs(dp, 8)};
             steps<2 * NT>(x, turned, [&](int k, const Pieces &v) { dq[k % NT] = mfma3(v.hi, v.lo, y[k / NT].hi, y[k / NT].lo, dq[k % NT]); });
         }
-        float by = a.scale / F;
+        float by = 1.0f / F;
         if constexpr (KG > 1) {  // the second group's sums are added through LDS
             f4 *const hand = (f4 *)smem + wave * 4 * NT * kWave + lane;
             __syncthreads();  // the last stage has been read

@@ -269,6 +269,20 @@ __device__ __forceinline__ bool column_scale(float most, float &F, float &by) {
     return __any(over);
 }
 
+// The scale of the scores times 2^e, e far outside a float's exponents where the scale is: it goes into the scores' gradients before
+// their column scale, which would lose them else.
+struct ScaleParts {
+    float m, k;  // m 2^k
+    __device__ __forceinline__ explicit ScaleParts(float scale) {
+        const int e = (int)((__float_as_uint(scale) >> 23) & 255) - 127;
+        k = (float)e;
+        m = e > 126 ? scale * 0.5f * pow2i(1 - e) : scale * pow2i(-e);
+    }
+    __device__ __forceinline__ float times(float e) const { return m * __builtin_amdgcn_exp2f(e + k); }
+};
+// kap F, held finite: where it is not, every gradient of the tile is zero, or past a float's range
+__device__ __forceinline__ float finite_product(float kap, float F) { return __builtin_fminf(__builtin_fmaxf(kap * F, -0x1p127f), 0x1p127f); }
+
 template <int NT>
 __device__ __forceinline__ void scale_acc(f16x (&acc)[NT], float by) {
 #pragma unroll

@@ -286,6 +286,7 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
 #pragma unroll
             for (int r = 0; r < 16; r++) dk[t][r] = dv[t][r] = 0.0f;
         float F = 0x1p100f, E = -1000.0f;
+        const ScaleParts parts(a.scale);
         const float ck = pow2i((int)ek) * a.scale * kLog2e, cv = pow2i((int)ev);
         for (int64_t t = t0; t < t1; t++) {
             int eq, eg;
@@ -323,10 +324,10 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
                 }
                 const int ed = put_ds(dp, most, mine_ds);
                 if (lane == 0) dsx[kw] = f2{__builtin_amdgcn_exp2f((float)ed - sh), pow2i((int)ek) * a.scale};
-                const float kap = __builtin_amdgcn_exp2f((float)eq - sh);
+                const float kap = parts.times((float)eq - sh);
                 float by;
-                if (column_scale(halves_max(most) * kap, F, by)) scale_acc(dk, by);
-                const float kF = kap * F;
+                if (column_scale(halves_max(most) * __builtin_fabsf(kap), F, by)) scale_acc(dk, by);
+                const float kF = finite_product(kap, F);
 #pragma unroll
                 for (int r = 0; r < 16; r++) dp[r] *= kF;
                 const Split8 ps[2] = {split_regs(s, 0), split_regs(s, 8)}, ds[2] = {split_regs(dp, 0), split_regs(dp, 8)};
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
         if (key < a.Lk) {
             const int64_t at = ((b * a.Lk + key) * a.Hkv + u) * D;
             const bool some = live && t0 < t1;
-            if (f.gk) store_column<true>(f.gk + split * f.part_k + at, dk, some, a.scale / F, half, D, f.acc_k);
+            if (f.gk) store_column<true>(f.gk + split * f.part_k + at, dk, some, 1.0f / F, half, D, f.acc_k);
             if (f.gv) store_column<true>(f.gv + split * f.part_k + at, dv, some, __builtin_amdgcn_exp2f(E - 14.0f), half, D, f.acc_v);
         }
     }
@@ -409,6 +410,7 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[t][r] = 0.0f;
         float F = 0x1p100f, E = -1000.0f;
+        const ScaleParts parts(a.scale);
         const float ck = ds_wave ? pow2i(ek) : pow2i(ek) * a.scale * kLog2e;
         for (int64_t t = t0; t < t1; t++) {
             int eq, eg;
@@ -441,7 +443,7 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
             lds_barrier();  // p is there
             if (mine) {
                 if (ds_wave) {
-                    const float c = ck * pow2i(eg), kap = __builtin_amdgcn_exp2f((float)eq - sh);
+                    const float c = ck * pow2i(eg), kap = parts.times((float)eq - sh);
                     float most = 0.0f;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
@@ -456,8 +458,8 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
                     const int ed = put_ds(s, most, hand);  // where p was
                     if (lane == 0) dsx[kw].x = __builtin_amdgcn_exp2f((float)ed - sh);
                     float by;
-                    if (column_scale(halves_max(most) * kap, F, by)) scale_acc(acc, by);
-                    const float kF = kap * F;
+                    if (column_scale(halves_max(most) * __builtin_fabsf(kap), F, by)) scale_acc(acc, by);
+                    const float kF = finite_product(kap, F);
 #pragma unroll
                     for (int r = 0; r < 16; r++) s[r] *= kF;
                 }
@@ -472,7 +474,7 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
         float *const out = ds_wave ? f.gk : f.gv;
         if (out && key < a.Lk)
             store_column<true>(out + split * f.part_k + ((b * a.Lk + key) * a.Hkv + u) * D, acc, live && t0 < t1,
-                               ds_wave ? a.scale / F : __builtin_amdgcn_exp2f(E - 14.0f), half, D, ds_wave ? f.acc_k : f.acc_v);
+                               ds_wave ? 1.0f / F : __builtin_amdgcn_exp2f(E - 14.0f), half, D, ds_wave ? f.acc_k : f.acc_v);
     }
 }
 

@@ -303,13 +303,28 @@ def test_attention_scales_and_sharp_rows(K, scale):
 
 
 @pytest.mark.parametrize("shape", [(1, 40, 90, 2, 2, 64, None), (1, 40, 300, 2, 2, 64, None), (1, 2, 90, 1, 1, 64, None)], ids=str)
-@pytest.mark.parametrize("scale", [300.0, 1e6])
+@pytest.mark.parametrize("scale", [300.0, 1e6, 1e30])
 def test_attention_large_scale_and_rows_of_zeros(K, shape, scale):
     """A query of zeros weighs its keys alike whatever the scale; the others hold what the scale takes."""
     q, k, v, g, lens = attn_inputs(shape, 34)
     q *= np.float32(0.125 / scale)
     q[0, 1] = 0
     check_attention(run_attention(K, shape, q, k, v, g, lens, scale=scale), R.attention64(q, k, v, lens, scale, g))
+
+
+@pytest.mark.parametrize("shape", [(1, 40, 1, 2, 2, 64, None), (1, 40, 90, 2, 2, 128, None), (1, 40, 300, 2, 2, 64, None)], ids=str)
+def test_attention_huge_queries_without_gradient(K, shape):
+    """Scores without gradients (one key: but for roundings; or none of the output) against queries of 1e25: no NaN."""
+    q, k, v, g, lens = attn_inputs(shape, 35)
+    q *= np.float32(1e25)
+    k *= np.float32(1e-25)
+    if shape[2] > 1:
+        g[:] = 0
+    got = run_attention(K, shape, q, k, v, g, lens, scale=0.125)
+    if shape[2] > 1:
+        assert all((got[i] == 0).all() for i in ("gq", "gk", "gv"))
+    else:
+        check_attention(got, R.attention64(q, k, v, lens, 0.125, g))
 
 
 @pytest.mark.parametrize("mag", [1e-12, 1e12])
