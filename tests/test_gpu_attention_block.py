@@ -495,22 +495,24 @@ def test_blocks_on_two_streams_at_once(K):
             assert (x == y).all()
 
 
-def test_attention_long_strides(K):
-    """Keys and values whose rows lie over 2^31 floats apart from first to last."""
-    B, Lq, Lk, H, D = 1, 2, 5, 1, 32
-    q, k, v, g, _ = attn_inputs((B, Lq, Lk, H, H, D, None), 19)
-    step = (1 << 29) + 12
+# read by rows, split by each workgroup, packed
+@pytest.mark.parametrize("Lq,Lk,D,step", [(2, 5, 32, (1 << 29) + 12), (20, 5, 32, (1 << 29) + 12), (20, 300, 128, (1 << 23) + 4)])
+def test_attention_long_strides(K, Lq, Lk, D, step):
+    """Keys whose rows lie over 2^31 floats apart from first to last, forward and backward."""
+    sizes = (1, Lq, Lk, 1, 1, D)
+    q, k, v, g, _ = attn_inputs((*sizes, None), 19)
     big = DeviceBuffer.empty(4 * (step * (Lk - 1) + D))
     for j in range(Lk):
-        for t, at in ((k, 0),):
-            big.upload(np.ascontiguousarray(t[0, j, 0]), 4 * (j * step + at))
-    Q, V, o = up(q), up(v), Out(q.shape)
-    n = K.cross_attention_fwd_workspace(B, Lq, Lk, H, H, D)
-    ws = DeviceBuffer.empty(n)
-    K.cross_attention_fwd(B, Lq, Lk, H, H, D, 0.2, Q.ptr, (64, 32, 32), big.ptr, (0, step, 0), V.ptr, (160, 32, 32), None,
-                          o.ptr, None, ws.ptr, n)
+        big.upload(np.ascontiguousarray(k[0, j, 0]), 4 * j * step)
+    Q, V, G, o, lse, outs = up(q), up(v), up(g), Out(q.shape), Out((1, 1, Lq)), [Out(t.shape) for t in (q, k, v)]
+    src = (Q.ptr, (Lq * D, D, D), big.ptr, (0, step, 0), V.ptr, (Lk * D, D, D), None)
+    n1, n2 = K.cross_attention_fwd_workspace(*sizes), K.cross_attention_bwd_workspace(*sizes)
+    ws = DeviceBuffer.empty(max(n1, n2, 1))
+    K.cross_attention_fwd(*sizes, 0.2, *src, o.ptr, lse.ptr, ws.ptr, n1)
+    K.cross_attention_bwd(*sizes, 0.2, *src, o.ptr, lse.ptr, G.ptr, *(t.ptr for t in outs), ws.ptr, n2, accumulate=False)
     synchronize()
-    R.within(o.get(), *R.attention64(q, k, v, None, 0.2)["o"], "o")
+    got = {"o": o.get(), "lse": lse.get(), **{"g" + c: t.get() for c, t in zip("qkv", outs)}}
+    check_attention(got, R.attention64(q, k, v, None, 0.2, g))
 
 
 # ---- through the engine ----------------------------------------------------------------------------------------------------
