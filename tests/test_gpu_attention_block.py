@@ -248,6 +248,7 @@ PATH_SHAPES = [(1, 900, 40, 6, 2, 64, (33,)), (2, 130, 200, 4, 2, 64, (200, 131)
                (1, 40, 3000, 1, 1, 64, (2990,)), (1, 300, 290, 2, 1, 200, (285,)), (1, 9, 2100, 3, 3, 48, None),
                (1, 33, 260, 5, 5, 64, None), (300, 5, 9, 4, 2, 16, None), (1, 4, 4, 64, 1, 64, None),
                (1, 900, 70, 6, 2, 128, (65,)), (2, 100, 128, 2, 2, 90, (128, 31)), (1, 2000, 140, 1, 1, 128, (135,)),
+               (1, 12, 0, 2, 1, 128, None), (2, 30, 0, 2, 2, 200, None), (2, 4, 0, 2, 2, 64, None),
                # more than a workgroup a CU
                (40, 10, 300, 7, 7, 64, tuple(range(290, 250, -1))), (33, 9, 161, 8, 8, 128, tuple(range(0, 165, 5))),
                (260, 9, 520, 1, 1, 30, None), (130, 9, 200, 2, 2, 90, None)]
@@ -403,6 +404,23 @@ def test_attention_is_deterministic_and_takes_streams(K):
         again = run_attention(K, shape, q, k, v, g, lens, stream=s.handle, poison=poison)
         for name, a in first.items():
             assert (a.view(np.uint32) == again[name].view(np.uint32)).all(), name
+
+
+@pytest.mark.parametrize("shape", [(2, 0, 5, 2, 1, 64), (1, 0, 300, 2, 1, 64), (1, 0, 5, 2, 2, 128), (1, 0, 40, 2, 2, 200)], ids=str)
+def test_attention_without_queries(K, shape):
+    """No queries: nothing forward, gradients of the keys and values that are zero, or stay where they are added to."""
+    B, Lq, Lk, Hq, Hkv, D = shape
+    k, v = up(np.ones((B, Lk, Hkv, D), np.float32)), up(np.ones((B, Lk, Hkv, D), np.float32))
+    s = (Lk * Hkv * D, Hkv * D, D)
+    src = (None, (0, Hq * D, D), k.ptr, s, v.ptr, s, None)
+    n = K.cross_attention_bwd_workspace(*shape)
+    ws = DeviceBuffer.empty(max(n, 1))
+    K.cross_attention_fwd(*shape, 0.1, *src, None, None)
+    for old in (None, 0.5):
+        gk, gv = (Out((B, Lk, Hkv, D), fill=np.nan if old is None else np.float32(old)) for _ in "kv")
+        K.cross_attention_bwd(*shape, 0.1, *src, None, None, None, None, gk.ptr, gv.ptr, ws.ptr, n, accumulate=old is not None)
+        synchronize()
+        assert (gk.get() == (old or 0)).all() and (gv.get() == (old or 0)).all()
 
 
 class Block:
