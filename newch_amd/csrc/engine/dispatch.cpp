@@ -158,17 +158,44 @@ class BackwardPass {
         if (!seed()) return ctx_->status;
         for (nc_node *n : live_) {
             if (!n->out->grad) continue;  // nothing reached this node's output
+            Untouched untouched(n);
             {
                 Scratch scratch(ctx_);
                 n->op->backward(n);
             }
-            if (ctx_->status != NC_OK) return ctx_->status;
+            if (ctx_->status != NC_OK) {
+                untouched.mark_fresh();
+                return ctx_->status;
+            }
             release(n);
         }
         return ctx_->status;
     }
 
   private:
+    // The gradients of a node's inputs that held nothing before its backward.  A backward takes their fresh mark (grad_acc) before
+    // its kernel has written them: where it fails in between (out of memory for a workspace, say), they hold nothing still, and the
+    // next backward must store there, not add.
+    struct Untouched {
+        nc_node *n;
+        bool empty[kMaxInputs];
+        uint64_t wgen[kMaxInputs];
+
+        explicit Untouched(nc_node *node) : n(node) {
+            for (int i = 0; i < n->n_in; i++) {
+                const nc_tensor *g = n->in[i]->grad;
+                empty[i] = !g || (g->flags & TF_GRAD_FRESH);
+                wgen[i] = g ? g->wgen : 0;
+            }
+        }
+        void mark_fresh() {
+            for (int i = 0; i < n->n_in; i++) {
+                nc_tensor *g = n->in[i]->grad;
+                if (g && empty[i] && g->wgen == wgen[i]) g->flags |= TF_GRAD_FRESH;
+            }
+        }
+    };
+
     bool loss_ok() {
         if (nc_numel(loss_) != 1 || loss_->dtype != NC_F32) {
             error(ctx_, NC_ERR_SHAPE, "backward: loss must be a single f32 element");
