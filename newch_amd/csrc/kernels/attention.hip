@@ -7,7 +7,8 @@
 //
 // A sequence without keys gives o = 0, lse = -inf and no gradient.  Keys and values past a sequence's length are not read.
 //
-// A value that counts and is not finite makes the results that meet it NaN.
+// A value that counts and is not finite makes the results that meet it NaN: pieces of an infinity are NaN (inf - inf), and the
+// kernel that reads plain fp32 (k_attn_token) looks at the operands of scores that are not finite.
 //
 // The products run on the fp16 matrix cores with operands in two pieces (attention.hpp), packed once into a workspace, where
 // they bound the time: three products for one reach at most a third of a library's fp16 product of 8192^3, 1.23 PFLOP/s, which
@@ -261,6 +262,10 @@ __device__ __forceinline__ f4 row_piece(const float *row, int c, int D) {
     }
 }
 
+// a row whose probabilities sum to zero: without keys `none`, else all its scores are -inf
+__device__ __forceinline__ float without_sum(int64_t keys, float none = 0.0f) { return keys ? NAN : none; }
+__device__ __forceinline__ float nan_if_infinite(float v) { return v + (v - v); }
+
 template <int NR, int LPK, int U, bool D4>
 __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const float *k, const float *v) {
     constexpr int NG = kWave / LPK, KEYS = kAttnWaves * U * NG;  // groups of a wave; keys of a round
@@ -292,6 +297,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
             }
             m[r] = -INFINITY, l[r] = 0.0f;
         }
+        float low = 0.0f;  // -inf where a score was: it would count nothing (other scores that are not finite give NaN by themselves)
         for (int64_t j = j0; j < j1; j += KEYS) {
             f4 kk[U][2], vv[U][2];
 #pragma unroll
@@ -301,6 +307,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
 #pragma unroll
                 for (int y = 0; y < 2; y++) kk[x][y] = row_piece<D4>(kr, ln + y * LPK, D), vv[x][y] = row_piece<D4>(vr, ln + y * LPK, D);
             }
+            __builtin_amdgcn_sched_barrier(0);  // all loads are on their way before the first is waited for
             float s[NR][U];
 #pragma unroll
             for (int x = 0; x < U; x++) {
@@ -313,6 +320,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
 #pragma unroll
                         for (int e = 0; e < 4; e++) t = fma_(q[r][y][e], kk[x][y][e], t);
                     t = lanes_sum<LPK>(t);
+                    low = __builtin_fminf(low, t);
                     s[r][x] = in ? t : -INFINITY;
                 }
             }
@@ -336,6 +344,32 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[r][y][e] = fma_(p, vv[x][y][e], o[r][y][e]);
                 }
+            }
+        }
+        if (__builtin_expect(__any(low == -INFINITY), 0)) {
+            // NaN where a key or the query is not finite; finite ones' scores are what they are (below a float's range: they count
+            // nothing).  The wave reads its keys again: a branch in the loop costs every call (1500 keys, 8 x 12 heads of 64: 17.9
+            // us, and 15.9).
+            for (int64_t j = j0 + wave * U * NG + grp; j < j1; j += KEYS)
+                for (int64_t key = j; key < min(j + U * NG, j1); key += NG) {
+                    float z = 0.0f;
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        const f4 again = row_piece<D4>(kb + key * a.sk[1], ln + y * LPK, D);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) z = fma_(again[e], 0.0f, z);
+                    }
+#pragma unroll
+                    for (int r = 0; r < NR; r++) l[r] += z;
+                }
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                float z = 0.0f;
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) z = fma_(q[r][y][e], 0.0f, z);
+                l[r] = lanes_sum<LPK>(l[r] + z) * (1.0f / LPK);  // the group's lanes hold one l: NaN in one of them is all of theirs
             }
         }
         // the wave's groups, then the waves
@@ -392,8 +426,9 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
                 int64_t i, g;
                 a.row(r, i, g);
                 const int64_t h = u * a.G + g;
-                f.o[((b * a.Lq + i) * a.Hq + h) * a.D + d] = total != 0.0f ? sum / total : 0.0f;
-                if (f.lse && d == 0) f.lse[(b * a.Hq + h) * a.Lq + i] = n ? fma_(top, kLn2, logf(total)) : -INFINITY;
+                f.o[((b * a.Lq + i) * a.Hq + h) * a.D + d] = nan_if_infinite(total != 0.0f ? sum / total : without_sum(n));
+                if (f.lse && d == 0)
+                    f.lse[(b * a.Hq + h) * a.Lq + i] = total != 0.0f ? fma_(top, kLn2, logf(total)) : without_sum(n, -INFINITY);
             } else {
                 const int64_t pr = ((int64_t)split * a.B * a.Hkv + pair) * f.rows + r;
                 f.po[pr * D + d] = sum;
@@ -406,7 +441,7 @@ __global__ __launch_bounds__(kAttnB) void k_attn_token(const FwdArgs f, const fl
 // The splits' parts of a row joined: a part counts by 2^(its reference - the largest).  A wave a row, where there are few: lane s
 // has part s's reference and sum, then every lane 64th column.
 __global__ __launch_bounds__(kAttnB) void k_attn_join_rows(const AttnArgs a, int64_t rows, int splits, const float *po, const f2 *pm,
-                                                      float *o, float *lse) {
+                                                      const int *key_len, float *o, float *lse) {
     const int64_t all = a.B * a.Hkv * rows;
     const int lane = threadIdx.x & 63;
     for (int64_t pr = (int64_t)blockIdx.x * kAttnWaves + (threadIdx.x >> 6); pr < all; pr += (int64_t)gridDim.x * kAttnWaves) {
@@ -419,7 +454,8 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join_rows(const AttnArgs a, int
         const float M = wave_max_nan_skip(ml.x);
         const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
         const float l = wave_sum(w * ml.y);
-        const float wn = nan ? NAN : l != 0.0f ? w / l : 0.0f;
+        const int64_t n = keys_of(a.Lk, key_len, b);
+        const float wn = nan ? NAN : l != 0.0f ? w / l : without_sum(n);
         for (int64_t d0 = 0; d0 < a.D; d0 += kWave) {
             const int64_t d = d0 + lane;
             const float *p = po + pr * a.D + (d < a.D ? d : 0);
@@ -434,15 +470,15 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join_rows(const AttnArgs a, int
                     sum = ws != 0.0f ? fma_(ws, x[s], sum) : sum;
                 }
             }
-            if (d < a.D) o[((b * a.Lq + i) * a.Hq + h) * a.D + d] = sum;
+            if (d < a.D) o[((b * a.Lq + i) * a.Hq + h) * a.D + d] = nan_if_infinite(sum);
         }
-        if (lse && lane == 0) lse[(b * a.Hq + h) * a.Lq + i] = l == 0.0f ? -INFINITY : fma_(M, kLn2, logf(l));
+        if (lse && lane == 0) lse[(b * a.Hq + h) * a.Lq + i] = l == 0.0f ? without_sum(n, -INFINITY) : fma_(M, kLn2, logf(l));
     }
 }
 
 // the same for many rows in up to eight parts: a lane four columns of a row
 __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t rows, int splits, const float *po, const f2 *pm,
-                                                      float *o, float *lse) {
+                                                      const int *key_len, float *o, float *lse) {
     const int64_t all = a.B * a.Hkv * rows, D4 = (a.D + 3) / 4;
     for (int64_t x = (int64_t)blockIdx.x * kAttnB + threadIdx.x; x < all * D4; x += (int64_t)gridDim.x * kAttnB) {
         const int64_t pr = x / D4, pair = pr / rows, R = pr - pair * rows, b = pair / a.Hkv, u = pair - b * a.Hkv;
@@ -476,9 +512,12 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
 #pragma unroll
             for (int e = 0; e < 4; e++) sum[e] = fma_(w, p[s][e], sum[e]);
         }
-        const float inv = nan ? NAN : l != 0.0f ? 1.0f / l : 0.0f;
-        store4(o + ((b * a.Lq + i) * a.Hq + h) * a.D, d, (int)a.D, sum * inv, 0);
-        if (lse && d == 0) lse[(b * a.Hq + h) * a.Lq + i] = l == 0.0f ? -INFINITY : fma_(M, kLn2, logf(l));
+        const int64_t n = keys_of(a.Lk, key_len, b);
+        const float inv = nan ? NAN : l != 0.0f ? 1.0f / l : without_sum(n);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[e] = nan_if_infinite(sum[e] * inv);
+        store4(o + ((b * a.Lq + i) * a.Hq + h) * a.D, d, (int)a.D, sum, 0);
+        if (lse && d == 0) lse[(b * a.Hq + h) * a.Lq + i] = l == 0.0f ? without_sum(n, -INFINITY) : fma_(M, kLn2, logf(l));
     }
 }
 
@@ -943,9 +982,9 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     // a wave a row while that fills the chip at most twice over, or for more than eight parts
     const int64_t all = p.pairs * p.rows, pieces = all * ((D + 3) / 4);
     if (p.splits > 8 || (p.splits > 1 && all <= 16 * kPlanCUs))
-        hipLaunchKernelGGL(k_attn_join_rows, dim3(attn_grid((all + kAttnWaves - 1) / kAttnWaves)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, o, lse);
+        hipLaunchKernelGGL(k_attn_join_rows, dim3(attn_grid((all + kAttnWaves - 1) / kAttnWaves)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, key_len, o, lse);
     else if (p.splits > 1)
-        hipLaunchKernelGGL(k_attn_join, dim3(attn_grid((pieces + kAttnB - 1) / kAttnB)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, o, lse);
+        hipLaunchKernelGGL(k_attn_join, dim3(attn_grid((pieces + kAttnB - 1) / kAttnB)), dim3(kAttnB), 0, st, a, p.rows, p.splits, f.po, f.pm, key_len, o, lse);
     return check_launch(what);
 }
 
