@@ -33,7 +33,8 @@ struct PackJob {
     int64_t len, tiles;    // rows and tiles of a pair, before key_len
     int by_len;            // keys: rows are cut by key_len; else queries
     char *out;             // [pair][tile][128 DP]
-    float *exps;           // [pair][tile] exponents of the scales
+    int *exps;             // [pair][tile] exponents of the scales
+    float *rows;           // [pair][tile][32] rows' exponents below it, where they have their own; or none are wanted
     int64_t first;         // the job's first workgroup
     const float *o, *lse;  // the output gradient's job: o (laid out as src), the rows' log-sum-exps [B, Hq, Lq]
     float *stats;          // [pair][tile][64]: log2-sum-exps (infinite past the rows), src . o of the tile's rows
@@ -49,7 +50,7 @@ struct PackArgs {
 template <int DP>
 __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
     constexpr int C = DP / 8, PER = (C + 7) / 8;  // chunks of a row; of a lane
-    __shared__ float red[kAttnWaves], dots[8][kTile];
+    __shared__ float tops[8][kTile], dots[8][kTile];
     const int t = threadIdx.x, row = t & 31, cl = t >> 5;
     for (int64_t w = blockIdx.x; w < a.total; w += gridDim.x) {
         int jx = 0;
@@ -80,15 +81,20 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
                 for (int e = 0; e < 8; e++) dot = fma_(x[k][e], y[e], dot);
             }
         }
-        most = wave_max_nan_skip(most);
         __syncthreads();  // the last tile has been read
         if (j.stats) dots[cl][row] = dot;
-        if ((t & 63) == 0) red[t >> 6] = most;
+        tops[cl][row] = most;
         __syncthreads();
-        const int ex = tile_exponent(__builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3])));
-        const float inv = pow2i(-ex);
+#pragma unroll
+        for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, tops[e][row]);
+        const float top = wave_max_nan_skip(most);
+        const int ex = tile_exponent(top);
+        const bool own = j.rows && rows_unlike(most, top);
+        const int er = own ? row_exponent(most, ex) : ex;
+        const float inv = pow2i(-er);
         const int64_t at = pair * j.tiles + tl;
-        if (t == 0) j.exps[at] = (float)ex;
+        if (t == 0) j.exps[at] = own ? ex + kOwnRows : ex;
+        if (own && t < kTile) j.rows[at * kTile + t] = (float)(er - ex);
         if (j.stats && t < kTile) {
             float d = dots[0][t];
 #pragma unroll
@@ -131,9 +137,7 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 
 // A value that the launch does not write, through the scalar cache: a vector load here would wait behind the next stage's
 // copies, which share its counter.
-__device__ __forceinline__ float scalar_load(const float *p) {
-    return *(const __attribute__((address_space(4))) float *)(uintptr_t)p;
-}
+__device__ __forceinline__ int scalar_load(const int *p) { return *(const __attribute__((address_space(4))) int *)(uintptr_t)p; }
 
 // ------------------------------------------------------------------------------------------------
 // forward
@@ -142,7 +146,8 @@ struct FwdArgs {
     AttnArgs a;
     const float *q;
     const char *kp, *vp;         // packed keys and values
-    const float *kx, *vx;        // their exponents
+    const int *kx, *vx;          // their exponents
+    const float *kr, *vr;        // and their rows'
     const int *key_len;
     float *o, *lse;
     float *po;                   // splits: [split][pair][row][D] sums, and {reference, sum} of each row
@@ -173,7 +178,8 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
         const int64_t n = keys_of(a.Lk, f.key_len, b), nt = (n + kTile - 1) / kTile;
         const int64_t t0 = nt * split / f.splits, t1 = nt * (split + 1) / f.splits;
         const char *kp = f.kp + pair * f.tiles * TB, *vp = f.vp + pair * f.tiles * TB;
-        const float *kx = f.kx + pair * f.tiles, *vx = f.vx + pair * f.tiles;
+        const int *kx = f.kx + pair * f.tiles, *vx = f.vx + pair * f.tiles;
+        const float *kr = f.kr + pair * f.tiles * kTile + 4 * half, *vr = f.vr + pair * f.tiles * kTile + 4 * half;
 
         auto copy = [&](int64_t t, int buf) {
             const int c = (int)min((int64_t)TS, t1 - t) * (TB / 1024);
@@ -196,7 +202,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
         sum.clear();
         for (int64_t t = t0, buf = 0; t < t1; t += TS, buf ^= 1) {
             const int64_t tg = t + kg * TPS;  // this group's first tile
-            float ek[TPS], ev[TPS];
+            int ek[TPS], ev[TPS];
 #pragma unroll
             for (int x = 0; x < TPS; x++) ek[x] = scalar_load(kx + min(tg + x, t1 - 1)), ev[x] = scalar_load(vx + min(tg + x, t1 - 1));
             stage_wait();
@@ -205,8 +211,8 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
 #pragma unroll
             for (int x = 0; x < TPS; x++) {
                 if (tg + x >= t1) break;
-                attend(sum, q, st + x * TB + ra, st + (TS + x) * TB + ca, ek[x], ev[x], tg + x + 1 == nt,
-                       (int)min(n - (tg + x) * kTile, (int64_t)kTile) - 4 * half);
+                attend(sum, q, st + x * TB + ra, st + (TS + x) * TB + ca, ek[x], ev[x], kr + (tg + x) * kTile, vr + (tg + x) * kTile,
+                       tg + x + 1 == nt, (int)min(n - (tg + x) * kTile, (int64_t)kTile) - 4 * half);
             }
         }
         if constexpr (KG > 1) {  // the second group's sums join the first's through LDS
@@ -220,13 +226,13 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
         const float l = halves_sum(sum.l);
         if (live && f.splits == 1) {
             // no keys: o is zero
-            store_column<false>(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, true, l != 0.0f ? pow2i((int)sum.E) / l : 0.0f, half, (int)a.D, 0);
+            store_column<false>(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, true, l != 0.0f ? unit_of(sum.U) / l : 0.0f, half, (int)a.D, 0);
             if (f.lse && half == 0)
-                f.lse[(b * a.Hq + h) * a.Lq + i] = nt ? fma_(sum.m - kPShift, kLn2, logf(l)) : -INFINITY;
+                f.lse[(b * a.Hq + h) * a.Lq + i] = nt ? fma_(sum.m, kLn2, logf(l)) : -INFINITY;
         } else if (live) {
             const int64_t pr = ((int64_t)split * a.B * a.Hkv + pair) * f.rows + R;
-            store_column<true>(f.po + pr * a.D, sum.o, t0 < t1, pow2i((int)sum.E), half, (int)a.D, 0);
-            if (half == 0) f.pm[pr] = f2{t0 < t1 ? sum.m - kPShift : -INFINITY, l};
+            store_column<true>(f.po + pr * a.D, sum.o, t0 < t1, unit_of(sum.U), half, (int)a.D, 0);
+            if (half == 0) f.pm[pr] = f2{t0 < t1 ? sum.m : -INFINITY, l};
         }
     }
 }
@@ -527,7 +533,8 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
 struct BwdArgs {
     AttnArgs a;
     const char *kp, *vp, *qp, *gp;                 // packed
-    const float *kx, *vx, *qx, *gx, *stats;
+    const int *kx, *vx, *qx, *gx;
+    const float *stats;
     const int *key_len;
     float *gq, *gk, *gv;                           // the gradients, or the splits' parts [split][...] where there are any
     int64_t rows, qtiles, ktiles, units, part_q, part_k;  // rows of a pair, tiles, units; floats of a part
@@ -576,7 +583,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
         h8 kh[REG ? KS : 1], kl[REG ? KS : 1];
         float ck = 0.0f;
         if (mine) {
-            ck = ds_wave ? pow2i((int)f.vx[tile]) : pow2i((int)f.kx[tile]) * a.scale * kLog2e;
+            ck = ds_wave ? pow2i(f.vx[tile]) : pow2i(f.kx[tile]) * a.scale * kLog2e;
             if constexpr (REG) {
 #pragma unroll
                 for (int s = 0; s < KS; s++) kh[s] = row_frag(kt, s), kl[s] = row_frag(kt + LO, s);
@@ -590,13 +597,13 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
         float F = 0x1p100f, E = -1000.0f;
         const ScaleParts parts(a.scale);
         for (int64_t t = t0, buf = 0; t < t1; t++, buf ^= 1) {
-            const float ex = scalar_load(f.gx + q0 + t), eq = scalar_load(f.qx + q0 + t);
+            const int eg = scalar_load(f.gx + q0 + t), eq = scalar_load(f.qx + q0 + t);
             stage_wait();
             if (t + 1 < t1) copy(t + 1, (int)buf ^ 1);
             const char *st = smem + buf * STAGE;
             const f4 *rows = (const f4 *)(st + 2 * TB) + half;
             // p as 2^14 p, less for tiles of smaller gradients (no less than 2^-60 times: below what gv can show)
-            const float En = __builtin_fmaxf(E, ex), sh = 14.0f + __builtin_fmaxf(ex - En, -60.0f);
+            const float ex = (float)eg, En = __builtin_fmaxf(E, ex), sh = 14.0f + __builtin_fmaxf(ex - En, -60.0f);
             f16x s;
             if (mine) {
                 const char *rt = st + ds_wave * TB + ra;
@@ -608,7 +615,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                           });
                 if (!ds_wave) {
                     if (ex > E) scale_acc(acc, __builtin_amdgcn_exp2f(E - ex));
-                    const float c = ck * pow2i((int)eq), base = live ? sh : -INFINITY;
+                    const float c = ck * pow2i(eq), base = live ? sh : -INFINITY;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const f4 ls = rows[2 * j];
@@ -627,7 +634,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
             lds_barrier();  // p is there (the next stage's copies stay on their way)
             if (!mine) continue;
             if (ds_wave) {
-                const float c = ck * pow2i((int)ex), kap = parts.times(eq - sh);
+                const float c = ck * pow2i(eg), kap = parts.times((float)eq - sh);
                 float most = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -695,7 +702,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
             qh[s] = row_frag(qp, s), ql[s] = row_frag(qp + LO, s);
             gh[s] = row_frag(gp, s), gl[s] = row_frag(gp + LO, s);
         }
-        const float cq = pow2i((int)f.qx[tile]) * a.scale * kLog2e, cg = pow2i((int)f.gx[tile]);
+        const float cq = pow2i(f.qx[tile]) * a.scale * kLog2e, cg = pow2i(f.gx[tile]);
         const float ls = f.stats[tile * 64 + (lane & 31)], de = f.stats[tile * 64 + 32 + (lane & 31)];
         f16x dq[NT];
 #pragma unroll
@@ -706,7 +713,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
         const ScaleParts parts(a.scale);
         for (int64_t ts = t0, buf = 0; ts < t1; ts += KG, buf ^= 1) {
             const int64_t t = ts + kg;
-            const float ek = scalar_load(f.kx + k0 + min(t, t1 - 1)), ev = scalar_load(f.vx + k0 + min(t, t1 - 1));
+            const int ek = scalar_load(f.kx + k0 + min(t, t1 - 1)), ev = scalar_load(f.vx + k0 + min(t, t1 - 1));
             stage_wait();
             if (ts + KG < t1) copy(ts + KG, (int)buf ^ 1);
             const char *st = smem + buf * STAGE + kg * TB;
@@ -724,7 +731,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
             Pieces x[3];
             x[0] = turned(0);
             x[1] = turned(1);
-            const float c = cq * pow2i((int)ek), c2 = cg * pow2i((int)ev);
+            const float c = cq * pow2i(ek), c2 = cg * pow2i(ev);
             const int left = (int)min(n - t * kTile, (int64_t)kTile) - 4 * half;
             float most = 0.0f;
 #pragma unroll
@@ -734,7 +741,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
                 dp[r] = p * fma_(dp[r], c2, -de);
                 most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
             }
-            const float kap = parts.times(ek);
+            const float kap = parts.times((float)ek);
             float step;
             if (column_scale(halves_max(most) * __builtin_fabsf(kap), F, step)) scale_acc(dq, step);
             const float kF = finite_product(kap, F);
@@ -850,7 +857,7 @@ struct FwdPlan {
     bool token, few;  // k_attn_token; few keys
     int DP, qtiles, splits, kg;  // kg: groups of waves that share a workgroup's keys
     int64_t rows, tiles, pairs, units;
-    size_t kp, vp, kx, vx, po, pm, total;  // offsets into the workspace
+    size_t kp, vp, kx, vx, kr, vr, po, pm, total;  // offsets into the workspace
 };
 
 static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D) {
@@ -889,6 +896,8 @@ static FwdPlan fwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
         p.vp = take(pt * tile_bytes(p.DP));
         p.kx = take(pt * 4);
         p.vx = take(pt * 4);
+        p.kr = take(pt * 4 * kTile);
+        p.vr = take(pt * 4 * kTile);
     }
     if (p.splits > 1) {
         p.po = take((size_t)p.splits * p.pairs * p.rows * D * 4);
@@ -967,11 +976,11 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_fwd(int64_t B, int64_t Lq, int6
     if (Lk && !p.token) {
         PackArgs pk{};
         pk.a = a, pk.key_len = key_len, pk.jobs = 2;
-        pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, w + p.kp, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
-        pk.job[1] = {v, sv[0], sv[1], sv[2], Lk, p.tiles, 1, w + p.vp, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
+        pk.job[0] = {k, sk[0], sk[1], sk[2], Lk, p.tiles, 1, w + p.kp, (int *)(w + p.kx), (float *)(w + p.kr), 0, nullptr, nullptr, nullptr};
+        pk.job[1] = {v, sv[0], sv[1], sv[2], Lk, p.tiles, 1, w + p.vp, (int *)(w + p.vx), (float *)(w + p.vr), 0, nullptr, nullptr, nullptr};
         pack_launch(pk, p.pairs, p.DP, st);
     }
-    FwdArgs f{a, q, w + p.kp, w + p.vp, (float *)(w + p.kx), (float *)(w + p.vx), key_len, o, lse, (float *)(w + p.po), (f2 *)(w + p.pm),
+    FwdArgs f{a, q, w + p.kp, w + p.vp, (int *)(w + p.kx), (int *)(w + p.vx), (float *)(w + p.kr), (float *)(w + p.vr), key_len, o, lse, (float *)(w + p.po), (f2 *)(w + p.pm),
               p.rows, p.tiles, p.units, p.qtiles, p.splits};
     if (p.token)
         token_launch(f, k, v, st);
@@ -1075,19 +1084,19 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
     BwdArgs f{};
     f.a = a;
     f.kp = w + p.kp, f.vp = w + p.vp, f.qp = w + p.qp, f.gp = w + p.gp;
-    f.kx = (float *)(w + p.kx), f.vx = (float *)(w + p.vx), f.qx = (float *)(w + p.qx), f.gx = (float *)(w + p.gx);
+    f.kx = (int *)(w + p.kx), f.vx = (int *)(w + p.vx), f.qx = (int *)(w + p.qx), f.gx = (int *)(w + p.gx);
     f.stats = (float *)(w + p.stats);
     f.key_len = key_len;
     f.rows = p.rows, f.qtiles = p.qtiles, f.ktiles = p.ktiles;
     PackArgs pk{};
     pk.a = a, pk.key_len = key_len;
     if (Lk) {
-        pk.job[pk.jobs++] = {k, sk[0], sk[1], sk[2], Lk, p.ktiles, 1, w + p.kp, (float *)(w + p.kx), 0, nullptr, nullptr, nullptr};
-        pk.job[pk.jobs++] = {v, sv[0], sv[1], sv[2], Lk, p.ktiles, 1, w + p.vp, (float *)(w + p.vx), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {k, sk[0], sk[1], sk[2], Lk, p.ktiles, 1, w + p.kp, (int *)(w + p.kx), nullptr, 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {v, sv[0], sv[1], sv[2], Lk, p.ktiles, 1, w + p.vp, (int *)(w + p.vx), nullptr, 0, nullptr, nullptr, nullptr};
     }
     if (Lq) {
-        pk.job[pk.jobs++] = {q, sq[0], sq[1], sq[2], p.rows, p.qtiles, 0, w + p.qp, (float *)(w + p.qx), 0, nullptr, nullptr, nullptr};
-        pk.job[pk.jobs++] = {go, Lq * Hq * D, Hq * D, D, p.rows, p.qtiles, 0, w + p.gp, (float *)(w + p.gx), 0, o, lse, (float *)(w + p.stats)};
+        pk.job[pk.jobs++] = {q, sq[0], sq[1], sq[2], p.rows, p.qtiles, 0, w + p.qp, (int *)(w + p.qx), nullptr, 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {go, Lq * Hq * D, Hq * D, D, p.rows, p.qtiles, 0, w + p.gp, (int *)(w + p.gx), nullptr, 0, o, lse, (float *)(w + p.stats)};
     }
     pack_launch(pk, p.pairs, p.DP, st);
     if (want_q) {

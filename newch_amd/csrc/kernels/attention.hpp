@@ -1,10 +1,12 @@
 // Shared pieces of the attention kernels (attention.hip): fp32 operands as pairs of fp16 on the matrix cores.
 //
-// A 32-row tile of an operand is scaled by a power of two that puts its largest finite value into [2^14, 2^15), and every value
-// is cut into x = hi + lo, fp16 each (rounded to nearest: |x - hi| <= 2^-11 |x|, |x - hi - lo| <= 2^-22 |x|).  A product is
-// hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16, which sums in fp32: the part left out, lo lo, is at most 2^-22 of it.  The
-// scale keeps the whole exponent range: values 2^-17 of their tile's largest and up have their 22 bits, smaller ones an absolute
-// error of 2^-40 of that largest.  Three products at the fp16 rate cost a fifth of v_mfma_f32_32x32x2_f32's one.
+// A 32-row tile of an operand is scaled by a power of two that puts its largest finite value into [2^14, 2^15), or, where its rows are
+// unlike (kOwnRows), each row by one of its own; and every value is cut into x = hi + lo, fp16 each (rounded to nearest: |x - hi| <=
+// 2^-11 |x|, |x - hi - lo| <= 2^-22 |x|).  A product is hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16, which sums in fp32: the
+// part left out, lo lo, is at most 2^-22 of it.  Values 2^-17 of what they are scaled by and up have their 22 bits, smaller ones
+// an absolute error of 2^-40 of it, so no more than 2^-34 of their row's largest.  Where rows are summed over, the other operand takes
+// the rows' powers of two, and its own scale follows the products' size, not that of the tiles.  Three products at the fp16 rate cost
+// three eighths of v_mfma_f32_32x32x2_f32's one.
 //
 // Fragments: lane l of the 32x32x16 product holds row (of A) or column (of B) l % 32 and eight k, those of half l / 32; the
 // result's column l % 32 in rows 8 (r / 4) + 4 (l / 32) + r % 4, r < 16.  A tile holds the 16 bytes of columns 8 c .. 8 c + 7 of row
@@ -137,6 +139,18 @@ __device__ __forceinline__ int tile_exponent(float most) {
     return e < -120 ? -120 : e;
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+
+// A tile whose rows are unlike -- the largest of one, zeros aside, below 2^-6 of the tile's -- is scaled row by row.  Its exponent, the
+// largest row's, is stored with kOwnRows added, and how far each row's lies below it (0 to -100) beside it.
+constexpr int kOwnRows = 1024;
+__device__ __forceinline__ bool own_rows(int code) { return code >= kOwnRows / 2; }
+__device__ __forceinline__ int exponent_of(int code) { return own_rows(code) ? code - kOwnRows : code; }
+__device__ __forceinline__ bool rows_unlike(float row_most, float tile_most) {  // of a wave that has all rows
+    return __any(row_most > 0.0f && row_most < tile_most * 0x1p-6f);
+}
+__device__ __forceinline__ int row_exponent(float row_most, int tile_ex) {
+    return row_most > 0.0f ? max(tile_exponent(row_most), tile_ex - 100) : tile_ex;
+}
 
 __device__ __forceinline__ f4 moved4(f4 v, int by) {  // down by `by` places
     if (by & 1) v = f4{v[1], v[2], v[3], 0.0f};
@@ -283,6 +297,16 @@ struct ScaleParts {
 // kap F, held finite: where it is not, every gradient of the tile is zero, or past a float's range
 __device__ __forceinline__ float finite_product(float kap, float F) { return __builtin_fminf(__builtin_fmaxf(kap * F, -0x1p127f), 0x1p127f); }
 
+// a result's rows 8 (r / 4) + 4 half + r % 4 times 2^ their own exponents, which are given from 4 half on
+__device__ __forceinline__ void scale_rows(f16x &s, const float *rows) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const f4 e = *(const f4 *)(rows + 8 * j);
+#pragma unroll
+        for (int x = 0; x < 4; x++) s[4 * j + x] *= __builtin_amdgcn_exp2f(e[x]);
+    }
+}
+
 template <int NT>
 __device__ __forceinline__ void scale_acc(f16x (&acc)[NT], float by) {
 #pragma unroll
@@ -309,10 +333,12 @@ __device__ __forceinline__ void store_column(float *row, const f16x (&acc)[NT], 
 // forward: a wave's 32 rows of queries against a tile of keys
 // ------------------------------------------------------------------------------------------------
 // A wave holds 32 rows of queries as columns: s^T = k q^T (A: 32 keys), so that a row's scores lie in the registers of two lanes
-// and its maximum, sum and scale are theirs; p^T is then the operand of o^T = v^T p^T as it lies.  One pass over the keys: the
-// reference m a row's exponents are taken from moves only when a score passes it by 2^4, and o and the sum with it; p is held as
-// 2^10 p (at most 2^14) in two fp16, so a p below 2^-13 loses low bits against an absolute 2^-35.
-constexpr float kPShift = 10.0f, kPSlack = 4.0f;
+// and its maximum, sum and scale are theirs; p^T is then the operand of o^T = v^T p^T as it lies.  One pass over the keys.  p = 2^(s - m)
+// for a reference m, a whole number that moves when a score passes it by 2^4.  What is cut into pieces is p 2^(e - U): e the
+// exponent of the tile's values, U that of o's unit, a row's own, which is raised so that its largest product -- p and value
+// together -- lies at 2^10 when it passes 2^14, and falls as m rises.  So a value that is large and does not count leaves the
+// others their bits, and a product below 2^-24 of a row's largest loses low bits against an absolute 2^-35 of it.
+constexpr float kPTop = 10.0f, kPSlack = 4.0f;
 
 template <int DP>
 struct Query {  // the rows times scale log2(e), as the second operand: column fragments of q^T
@@ -340,16 +366,18 @@ __device__ __forceinline__ void load_query(Query<DP> &q, const float *row, bool 
     }
 }
 
+__device__ __forceinline__ float unit_of(float U) { return __builtin_amdgcn_ldexpf(1.0f, (int)__builtin_fmaxf(U, -1000.0f)); }
+
 template <int DP>
 struct Sums {
     f16x o[DP / 32];
-    float m, l, E;  // reference, sum of 2^kPShift p, exponent of o
+    float m, l, U;  // reference, sum of p, exponent of o's unit
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int t = 0; t < DP / 32; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
-        m = -INFINITY, l = 0.0f, E = -1000.0f;
+        m = -INFINITY, l = 0.0f, U = -INFINITY;
     }
 };
 
@@ -360,14 +388,14 @@ __device__ __forceinline__ void put(const Sums<DP> &a, f4 *to) {
     for (int d = 0; d < DP / 32; d++)
 #pragma unroll
         for (int j = 0; j < 4; j++) to[(4 * d + j) * kWave] = f4{a.o[d][4 * j], a.o[d][4 * j + 1], a.o[d][4 * j + 2], a.o[d][4 * j + 3]};
-    to[DP / 8 * kWave] = f4{a.m, a.l, a.E, 0.0f};
+    to[DP / 8 * kWave] = f4{a.m, a.l, a.U, 0.0f};
 }
 template <int DP>
 __device__ __forceinline__ void join(Sums<DP> &a, const f4 *from) {
     const f4 b = from[DP / 8 * kWave];
-    const float m = __builtin_fmaxf(a.m, b[0]), E = __builtin_fmaxf(a.E, b[2]);
-    const float wa = a.m == m ? 1.0f : __builtin_amdgcn_exp2f(a.m - m), wb = b[0] == m ? 1.0f : __builtin_amdgcn_exp2f(b[0] - m);
-    const float oa = wa * __builtin_amdgcn_exp2f(a.E - E), ob = wb * __builtin_amdgcn_exp2f(b[2] - E);
+    const float m = __builtin_fmaxf(a.m, b[0]), da = a.m == m ? 0.0f : a.m - m, db = b[0] == m ? 0.0f : b[0] - m;
+    const float ua = a.U + da, ub = b[2] + db, U = __builtin_fmaxf(ua, ub);
+    const float oa = ua == U ? 1.0f : __builtin_amdgcn_exp2f(ua - U), ob = ub == U ? 1.0f : __builtin_amdgcn_exp2f(ub - U);
 #pragma unroll
     for (int d = 0; d < DP / 32; d++)
 #pragma unroll
@@ -376,15 +404,15 @@ __device__ __forceinline__ void join(Sums<DP> &a, const f4 *from) {
 #pragma unroll
             for (int e = 0; e < 4; e++) a.o[d][4 * j + e] = fma_(a.o[d][4 * j + e], oa, v[e] * ob);
         }
-    a.l = fma_(a.l, wa, b[1] * wb);
-    a.m = m, a.E = E;
+    a.l = fma_(a.l, __builtin_amdgcn_exp2f(da), b[1] * __builtin_amdgcn_exp2f(db));
+    a.m = m, a.U = U;
 }
 
-// kt, vt: the tile's keys and values in LDS, at this lane's row_at and col_at; ek, ev: their exponents; left: keys of the tile
-// that count (32 but in the last one), less 4 half
+// kt, vt: the tile's keys and values in LDS, at this lane's row_at and col_at; ek, ev: their exponents, kr, vr: their rows', from 4
+// half on, read where they have their own; left: keys of the tile that count (32 but in the last one), less 4 half
 template <int DP>
-__device__ __forceinline__ void attend(Sums<DP> &a, const Query<DP> &q, const char *kt, const char *vt, float ek, float ev, bool cut,
-                                       int left) {
+__device__ __forceinline__ void attend(Sums<DP> &a, const Query<DP> &q, const char *kt, const char *vt, int ek, int ev, const float *kr,
+                                       const float *vr, bool cut, int left) {
     constexpr int KS = DP / 16, NT = DP / 32, LO = 64 * DP;
     f16x s;
 #pragma unroll
@@ -395,37 +423,65 @@ __device__ __forceinline__ void attend(Sums<DP> &a, const Query<DP> &q, const ch
     Pieces f[3];
     f[0] = value(0);
     f[1] = value(1);
-    const float c = __builtin_fmaxf(q.c * pow2i((int)ek), 0x1p-126f);  // -inf * c stays -inf
-    if (cut) {
+    float c = __builtin_fmaxf(q.c * pow2i(exponent_of(ek)), 0x1p-126f);  // -inf * c stays -inf
+    if (cut || own_rows(ek)) {
+        if (own_rows(ek)) scale_rows(s, kr);
+        if (cut) {
 #pragma unroll
-        for (int r = 0; r < 16; r++)
-            if (8 * (r / 4) + r % 4 >= left) s[r] = -INFINITY;
+            for (int r = 0; r < 16; r++)
+                if (8 * (r / 4) + r % 4 >= left) s[r] = -INFINITY;
+        }
     }
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < 16; r++) top = __builtin_fmaxf(top, s[r]);
     top = halves_max(top) * c;
-    if (__any(top > a.m + kPSlack) || ev > a.E) {
-        const float mn = top > a.m + kPSlack ? top : a.m, En = __builtin_fmaxf(a.E, ev);
-        const float al = a.m == mn ? 1.0f : __builtin_amdgcn_exp2f(a.m - mn);
-        const float ao = al * __builtin_amdgcn_exp2f(a.E - En);
-        a.l *= al;
+    const float e = (float)exponent_of(ev);
+    const bool own = own_rows(ev);
+    float dv = e - a.U;
+    if (__any(top - a.m > kPSlack || top - a.m + dv > kPTop + kPSlack) || own) {
+        const float mn = top - a.m > kPSlack ? __builtin_rintf(top) : a.m, down = a.m == mn ? 0.0f : a.m - mn;
+        a.l *= __builtin_amdgcn_exp2f(down);
+        a.U += down;
         a.m = mn;
-        a.E = En;
+        if (own) {  // p's sum, then p times 2^ its value's own exponent in p's place
+            float sum = 0.0f;
+            top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const f4 er = *(const f4 *)(vr + 8 * j);
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int r = 4 * j + x;
+                    sum += __builtin_amdgcn_exp2f(fma_(s[r], c, -mn));
+                    s[r] = fma_(s[r], c, er[x]);
+                    top = __builtin_fmaxf(top, s[r]);
+                }
+            }
+            top = halves_max(top);
+            c = 1.0f;
+            a.l += sum;
+        }
+        const float over = top - mn;
+        const float Un = over + (e - a.U) > kPTop + kPSlack ? __builtin_ceilf(over) + (e - kPTop) : a.U;
+        const float by = a.U == Un ? 1.0f : __builtin_amdgcn_exp2f(a.U - Un);
+        a.U = Un;
+        dv = e - Un;
 #pragma unroll
         for (int d = 0; d < NT; d++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) a.o[d][r] *= ao;
+            for (int r = 0; r < 16; r++) a.o[d][r] *= by;
     }
-    // values of smaller tiles count through smaller p (no smaller than 2^-60: below what o can show)
-    const float dv = __builtin_fmaxf(ev - a.E, -60.0f), off = kPShift + dv - a.m;
+    // no smaller than 2^-60: far below what o can show, and p's sum keeps its bits
+    dv = __builtin_fmaxf(dv, -60.0f);
+    const float off = dv - a.m;
     float sum = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; r++) {
         s[r] = __builtin_amdgcn_exp2f(fma_(s[r], c, off));
         sum += s[r];
     }
-    a.l = fma_(sum, __builtin_amdgcn_exp2f(-dv), a.l);
+    a.l = fma_(sum, own ? 0.0f : __builtin_amdgcn_exp2f(-dv), a.l);
     const Split8 p[2] = {split_regs(s, 0), split_regs(s, 8)};
     steps<2 * NT>(f, value, [&](int k, const Pieces &v) { a.o[k % NT] = mfma3(v.hi, v.lo, p[k / NT].hi, p[k / NT].lo, a.o[k % NT]); });
 }

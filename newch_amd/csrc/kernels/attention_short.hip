@@ -8,9 +8,10 @@
 
 namespace nchip {
 
-// A wave reads 32 rows of `src` (from `row0` on, n in all, `step` floats apart): the tile's exponent; and splits them into LDS.
+// A wave reads 32 rows of `src` (from `row0` on, n in all, `step` floats apart): the tile's exponent, with kOwnRows added where its rows
+// have their own (wanted: own is given, this lane's row's); and splits them into LDS.
 template <int DP>
-__device__ __forceinline__ int tile_load(const float *src, int64_t step, int row0, int n, int D, float (&x)[DP / 16][8]) {
+__device__ __forceinline__ int tile_load(const float *src, int64_t step, int row0, int n, int D, float (&x)[DP / 16][8], int *own = nullptr) {
     const int lane = threadIdx.x & 63, half = lane >> 5, r = lane & 31;
     const bool live = row0 + r < n;
     float most = 0.0f;
@@ -21,7 +22,13 @@ __device__ __forceinline__ int tile_load(const float *src, int64_t step, int row
         for (int e = 0; e < 8; e++) x[k][e] = live ? x[k][e] : 0.0f;
         most = abs_max(x[k], most);
     }
-    return tile_exponent(wave_max_nan_skip(most));
+    const float top = wave_max_nan_skip(most);
+    const int ex = tile_exponent(top);
+    if (!own) return ex;
+    most = halves_max(most);
+    const bool unlike = rows_unlike(most, top);
+    *own = unlike ? row_exponent(most, ex) : ex;
+    return unlike ? ex + kOwnRows : ex;
 }
 template <int DP>
 __device__ __forceinline__ void tile_split(float (&x)[DP / 16][8], int ex, char *tile) {
@@ -46,7 +53,8 @@ __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    float *const exps = (float *)(smem + 2 * f.tiles * TB);
+    float *const rows = (float *)(smem + 2 * f.tiles * TB);  // [2][tiles][32], then the tiles' exponents
+    int *const exps = (int *)(rows + 2 * f.tiles * kTile);
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t pair = w / f.splits, b = pair / a.Hkv, u = pair - b * a.Hkv;
         const int split = (int)(w - pair * f.splits);
@@ -58,9 +66,11 @@ __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd
             const int k = val ? t - nt : t;
             const float *src = val ? f.v + b * a.sv[0] + u * a.sv[2] : f.k + b * a.sk[0] + u * a.sk[2];
             float x[DP / 16][8];
-            const int e = tile_load<DP>(src, val ? a.sv[1] : a.sk[1], k * kTile, n, (int)a.D, x);
-            tile_split<DP>(x, e, smem + (val ? f.tiles + k : k) * TB);
-            if (lane == 0) exps[val ? f.tiles + k : k] = (float)e;
+            int er;
+            const int at = val ? f.tiles + k : k, e = tile_load<DP>(src, val ? a.sv[1] : a.sk[1], k * kTile, n, (int)a.D, x, &er);
+            tile_split<DP>(x, er, smem + at * TB);
+            if (lane == 0) exps[at] = e;
+            if (own_rows(e) && half == 0) rows[at * kTile + lane] = (float)(er - exponent_of(e));
         }
         __syncthreads();
         for (int64_t qt = t0 + wave; qt < t1; qt += W) {
@@ -75,12 +85,13 @@ __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd
             sum.clear();
             const char *kt = smem + row_at(lane), *vt = smem + f.tiles * TB + col_at(lane);
             for (int t = 0; t < nt; t++)
-                attend(sum, q, kt + t * TB, vt + t * TB, exps[t], exps[f.tiles + t], t + 1 == nt, min(n - t * kTile, kTile) - 4 * half);
+                attend(sum, q, kt + t * TB, vt + t * TB, __builtin_amdgcn_readfirstlane(exps[t]), __builtin_amdgcn_readfirstlane(exps[f.tiles + t]),
+                       rows + t * kTile + 4 * half, rows + (f.tiles + t) * kTile + 4 * half, t + 1 == nt, min(n - t * kTile, kTile) - 4 * half);
             const float l = halves_sum(sum.l);
             if (live) {
-                store_column<false>(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, true, l != 0.0f ? pow2i((int)sum.E) / l : 0.0f, half, (int)a.D, 0);
+                store_column<false>(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, true, l != 0.0f ? unit_of(sum.U) / l : 0.0f, half, (int)a.D, 0);
                 if (f.lse && half == 0)
-                    f.lse[(b * a.Hq + h) * a.Lq + i] = nt ? fma_(sum.m - kPShift, kLn2, logf(l)) : -INFINITY;
+                    f.lse[(b * a.Hq + h) * a.Lq + i] = nt ? fma_(sum.m, kLn2, logf(l)) : -INFINITY;
             }
         }
     }
@@ -488,7 +499,7 @@ static void launch(F *kernel, int64_t units, int threads, size_t lds, hipStream_
 }
 
 void short_fwd(const ShortFwd &f, int DP, hipStream_t st) {
-    const size_t lds = (size_t)f.tiles * 2 * tile_bytes(DP) + 2 * f.tiles * sizeof(float);
+    const size_t lds = (size_t)f.tiles * 2 * (tile_bytes(DP) + (kTile + 1) * sizeof(float));
     if (DP == 32) launch(&k_attn_short_fwd<32, 8, 4>, f.units, 512, lds, st, f);
     // three workgroups of four waves a CU where their keys fit its LDS, else eight waves over one copy (heads of 64, both ways: 4096
     // x 77, 4 x 16 heads 147 us with four and 153 with eight, 64 x 64, 64 x 8 35 and 39; 197 x 197, 8 x 12 heads 60 and 58)
