@@ -33,11 +33,14 @@ struct PackJob {
     int64_t len, tiles;    // rows and tiles of a pair, before key_len
     int by_len;            // keys: rows are cut by key_len; else queries
     char *out;             // [pair][tile][128 DP]
-    int *exps;             // [pair][tile] exponents of the scales
-    float *rows;           // [pair][tile][32] rows' exponents below it, where they have their own; or none are wanted
+    int *exps;             // [pair][tile] exponents of the scales, kOwnRows added where `rows` counts, or with stats where a row is `loose`
+    float *rows;           // [pair][tile][32] rows' exponents below it, where they have their own; none: they are in stats
     int64_t first;         // the job's first workgroup
     const float *o, *lse;  // the output gradient's job: o (laid out as src), the rows' log-sum-exps [B, Hq, Lq]
-    float *stats;          // [pair][tile][64]: log2-sum-exps (infinite past the rows), src . o of the tile's rows
+    // [pair][tile][64]: log2-sum-exps (infinite past the rows), src . o of the tile's rows.  Where the rows have their own exponents,
+    // d below the tile's (d <= 0), log2-sum-exps less d, and 2^-d src . o: the scores' gradients p (go . v - go . o) come out
+    // of p 2^d and the row's pieces' products with v as if the rows had the tile's.
+    float *stats;
 };
 struct PackArgs {
     PackJob job[4];
@@ -89,18 +92,21 @@ __global__ __launch_bounds__(kAttnB) void k_attn_pack(const PackArgs a) {
         for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, tops[e][row]);
         const float top = wave_max_nan_skip(most);
         const int ex = tile_exponent(top);
-        const bool own = j.rows && rows_unlike(most, top);
+        const bool own = rows_unlike(most, top);
         const int er = own ? row_exponent(most, ex) : ex;
         const float inv = pow2i(-er);
         const int64_t at = pair * j.tiles + tl;
-        if (t == 0) j.exps[at] = own ? ex + kOwnRows : ex;
-        if (own && t < kTile) j.rows[at * kTile + t] = (float)(er - ex);
+        float log_sum = INFINITY;
+        if (j.stats && live) log_sum = j.lse[(b * a.a.Hq + h) * a.a.Lq + i] * kLog2e;
+        const bool marked = (own && j.rows) || __any(loose(log_sum));
+        if (t == 0) j.exps[at] = marked ? ex + kOwnRows : ex;
+        if (own && j.rows && t < kTile) j.rows[at * kTile + t] = (float)(er - ex);
         if (j.stats && t < kTile) {
             float d = dots[0][t];
 #pragma unroll
             for (int e = 1; e < 8; e++) d += dots[e][t];
-            j.stats[at * 64 + t] = live ? j.lse[(b * a.a.Hq + h) * a.a.Lq + i] * kLog2e : INFINITY;
-            j.stats[at * 64 + 32 + t] = d;
+            j.stats[at * 64 + t] = log_sum - (float)(er - ex);
+            j.stats[at * 64 + 32 + t] = d * pow2i(ex - er);
         }
         char *out = j.out + at * tile_bytes(DP);
 #pragma unroll
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
         const int64_t t0 = nt * split / f.splits, t1 = nt * (split + 1) / f.splits;
         const char *kp = f.kp + pair * f.tiles * TB, *vp = f.vp + pair * f.tiles * TB;
         const int *kx = f.kx + pair * f.tiles, *vx = f.vx + pair * f.tiles;
-        const float *kr = f.kr + pair * f.tiles * kTile + 4 * half, *vr = f.vr + pair * f.tiles * kTile + 4 * half;
+        const float *kr = f.kr + pair * f.tiles * kTile, *vr = f.vr + pair * f.tiles * kTile;
 
         auto copy = [&](int64_t t, int buf) {
             const int c = (int)min((int64_t)TS, t1 - t) * (TB / 1024);
@@ -530,10 +536,17 @@ __global__ __launch_bounds__(kAttnB) void k_attn_join(const AttnArgs a, int64_t 
 // ------------------------------------------------------------------------------------------------
 // backward: two kernels, each with its own recomputed scores, so that every gradient is summed in one place and order
 // ------------------------------------------------------------------------------------------------
+// 2^ the exponent of this lane's row of a packed tile
+__device__ __forceinline__ float column_exponent(const int *exps, const float *rows, int64_t tile) {
+    const int e = exps[tile];
+    return pow2i(own_rows(e) ? exponent_of(e) + (int)rows[tile * kTile + (threadIdx.x & 31)] : e);
+}
+
 struct BwdArgs {
     AttnArgs a;
     const char *kp, *vp, *qp, *gp;                 // packed
-    const int *kx, *vx, *qx, *gx;
+    const int *kx, *vx, *qx, *gx;                  // their exponents
+    const float *kr, *vr, *qr;                     // and their rows'
     const float *stats;
     const int *key_len;
     float *gq, *gk, *gv;                           // the gradients, or the splits' parts [split][...] where there are any
@@ -546,7 +559,8 @@ struct BwdArgs {
 // hands p over through LDS and sums gv^T += go^T p; the other takes dp = go v^T, makes ds of it and sums gk^T += q^T ds.  Each keeps
 // half of the fragments and of the sums, so that two waves fit a SIMD: one's exponentials run under the other's products (128
 // columns, 2 x 16 heads on 4, 2048 x 4096: 0.77 ms, and 0.90 with one wave that does both; 0.72 ms with the fragments read ahead,
-// 1.15 PFLOP/s).  Padded rows of queries have an infinite log-sum-exp: p = 0.
+// 1.15 PFLOP/s).  Padded rows of queries have an infinite log-sum-exp: p = 0.  gv's unit follows p times the gradients' size, as o's
+// does in the forward.
 template <int DP, int OCC>
 __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * TB + 256;
@@ -557,7 +571,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
     const int which = wave & (kAttnWaves - 1), ds_wave = wave / kAttnWaves;  // tile of keys; 0: p and gv, 1: ds and gk
     const int ra = row_at(lane), ca = col_at(lane);
     const uint32_t lds = lds_address(smem);
-    f4 *const hand = (f4 *)(smem + 2 * STAGE) + which * 256 + lane;  // p's registers 4 j .. 4 j + 3 at 64 j
+    f4 *const hand = (f4 *)(smem + 2 * STAGE) + which * 320 + lane;  // p's registers 4 j .. 4 j + 3 at 64 j
     for (int64_t w = blockIdx.x; w < f.units; w += gridDim.x) {
         const int64_t unit = xcd_unit(w, f.units);
         const int64_t rest = unit / f.groups;
@@ -583,7 +597,8 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
         h8 kh[REG ? KS : 1], kl[REG ? KS : 1];
         float ck = 0.0f;
         if (mine) {
-            ck = ds_wave ? pow2i(f.vx[tile]) : pow2i(f.kx[tile]) * a.scale * kLog2e;
+            ck = column_exponent(ds_wave ? f.vx : f.kx, ds_wave ? f.vr : f.kr, tile);
+            if (!ds_wave) ck *= a.scale * kLog2e;
             if constexpr (REG) {
 #pragma unroll
                 for (int s = 0; s < KS; s++) kh[s] = row_frag(kt, s), kl[s] = row_frag(kt + LO, s);
@@ -594,7 +609,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[t][r] = 0.0f;
-        float F = 0x1p100f, E = -1000.0f;
+        float scale = ds_wave ? 0x1p100f : live ? kNoUnit : -kNoUnit;
         const ScaleParts parts(a.scale);
         for (int64_t t = t0, buf = 0; t < t1; t++, buf ^= 1) {
             const int eg = scalar_load(f.gx + q0 + t), eq = scalar_load(f.qx + q0 + t);
@@ -602,8 +617,8 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
             if (t + 1 < t1) copy(t + 1, (int)buf ^ 1);
             const char *st = smem + buf * STAGE;
             const f4 *rows = (const f4 *)(st + 2 * TB) + half;
-            // p as 2^14 p, less for tiles of smaller gradients (no less than 2^-60 times: below what gv can show)
-            const float ex = (float)eg, En = __builtin_fmaxf(E, ex), sh = 14.0f + __builtin_fmaxf(ex - En, -60.0f);
+            const float *qr = f.qr + (q0 + t) * kTile;
+            const int xq = exponent_of(eq), xg = exponent_of(eg);
             f16x s;
             if (mine) {
                 const char *rt = st + ds_wave * TB + ra;
@@ -614,18 +629,19 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                               s = mfma3(x.hi, x.lo, REG ? kh[k] : row_frag(kt, k), REG ? kl[k] : row_frag(kt + LO, k), s);
                           });
                 if (!ds_wave) {
-                    if (ex > E) scale_acc(acc, __builtin_amdgcn_exp2f(E - ex));
-                    const float c = ck * pow2i(eq), base = live ? sh : -INFINITY;
+                    if (own_rows(eq)) scale_rows(s, qr);
+                    const float c = ck * pow2i(xq), off = live ? first_shift((float)xg, scale) : -INFINITY;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const f4 ls = rows[2 * j];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[4 * j + e] = __builtin_amdgcn_exp2f(fma_(s[4 * j + e], c, base - ls[e]));
-                        hand[64 * j] = f4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
+                        for (int e = 0; e < 4; e++) s[4 * j + e] = __builtin_amdgcn_exp2f(fma_(s[4 * j + e], c, off - ls[e]));
                     }
+                    hand[256].x = column_unit(s, (float)xg, own_rows(eg), scale, acc);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) hand[64 * j] = f4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
                 }
             }
-            E = En;
             const char *ct = st + (ds_wave ? 0 : TB) + ca;
             const auto turned = [&](int k) { return Pieces{col_frag(ct, k / NT, k % NT), col_frag(ct + LO, k / NT, k % NT)}; };
             Pieces x[3];
@@ -634,7 +650,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
             lds_barrier();  // p is there (the next stage's copies stay on their way)
             if (!mine) continue;
             if (ds_wave) {
-                const float c = ck * pow2i(eg), kap = parts.times((float)eq - sh);
+                const float c = ck * pow2i(xg), kap = parts.times((float)xq - hand[256].x);
                 float most = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -646,9 +662,13 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                         most = __builtin_fmaxf(most, __builtin_fabsf(s[r]));
                     }
                 }
+                if (own_rows(eq)) {
+                    scale_rows(s, qr);
+                    most = largest(s);
+                }
                 float by;
-                if (column_scale(halves_max(most) * __builtin_fabsf(kap), F, by)) scale_acc(acc, by);
-                const float kF = finite_product(kap, F);
+                if (column_scale(halves_max(most) * __builtin_fabsf(kap), scale, by)) scale_acc(acc, by);
+                const float kF = finite_product(kap, scale);
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[r] *= kF;
             }
@@ -658,7 +678,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
         float *const out = ds_wave ? f.gk : f.gv;
         if (out && key < a.Lk)
             store_column<true>(out + split * f.part_k + ((b * a.Lk + key) * a.Hkv + u) * a.D, acc, live && t0 < t1,
-                               ds_wave ? 1.0f / F : __builtin_amdgcn_exp2f(E - 14.0f), half, (int)a.D, ds_wave ? f.acc_k : f.acc_v);
+                               ds_wave ? 1.0f / scale : unit_of(scale), half, (int)a.D, ds_wave ? f.acc_k : f.acc_v);
     }
 }
 
@@ -702,7 +722,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
             qh[s] = row_frag(qp, s), ql[s] = row_frag(qp + LO, s);
             gh[s] = row_frag(gp, s), gl[s] = row_frag(gp + LO, s);
         }
-        const float cq = pow2i(f.qx[tile]) * a.scale * kLog2e, cg = pow2i(f.gx[tile]);
+        const float cq = column_exponent(f.qx, f.qr, tile) * a.scale * kLog2e, cg = pow2i(exponent_of(f.gx[tile]));
         const float ls = f.stats[tile * 64 + (lane & 31)], de = f.stats[tile * 64 + 32 + (lane & 31)];
         f16x dq[NT];
 #pragma unroll
@@ -731,17 +751,27 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
             Pieces x[3];
             x[0] = turned(0);
             x[1] = turned(1);
-            const float c = cq * pow2i(ek), c2 = cg * pow2i(ev);
+            const float *kr = f.kr + (k0 + t) * kTile;
+            if (own_rows(max(ek, ev))) {
+                if (own_rows(ek)) scale_rows(s, kr);
+                if (own_rows(ev)) scale_rows(dp, f.vr + (k0 + t) * kTile);
+            }
+            const float c = cq * pow2i(exponent_of(ek)), c2 = cg * pow2i(exponent_of(ev));
             const int left = (int)min(n - t * kTile, (int64_t)kTile) - 4 * half;
             float most = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                float p = __builtin_amdgcn_exp2f(fma_(s[r], c, -ls));
+                // roundings of large scores and of their sum may put p above 1: far above, it is held there (a NaN shows in o, so in de)
+                float p = __builtin_amdgcn_exp2f(__builtin_fminf(fma_(s[r], c, -ls), 0.0f));
                 p = 8 * (r / 4) + r % 4 < left ? p : 0.0f;
                 dp[r] = p * fma_(dp[r], c2, -de);
                 most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
             }
-            const float kap = parts.times((float)ek);
+            if (own_rows(ek)) {
+                scale_rows(dp, kr);
+                most = largest(dp);
+            }
+            const float kap = parts.times((float)exponent_of(ek));
             float step;
             if (column_scale(halves_max(most) * __builtin_fabsf(kap), F, step)) scale_acc(dq, step);
             const float kF = finite_product(kap, F);
@@ -1003,7 +1033,7 @@ struct BwdPlan {
     bool few, kg;  // few keys; two groups of waves share a workgroup's keys for gq
     int DP, qgroups, kgroups, qsplits, ksplits;  // splits of the keys for gq, of the queries for gk and gv
     int64_t rows, qtiles, ktiles, pairs, nq, nk;
-    size_t kp, vp, qp, gp, kx, vx, qx, gx, stats, pq, pk, pv, total;
+    size_t kp, vp, qp, gp, kx, vx, qx, gx, kr, vr, qr, stats, pq, pk, pv, total;
 };
 
 static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t Hkv, int64_t D) {
@@ -1035,6 +1065,7 @@ static BwdPlan bwd_plan(int64_t B, int64_t Lq, int64_t Lk, int64_t Hq, int64_t H
     const int64_t q = p.few ? 0 : p.pairs * p.qtiles, k = p.few ? 0 : p.pairs * p.ktiles, tb = tile_bytes(p.DP);
     p.kp = take(k * tb), p.vp = take(k * tb), p.qp = take(q * tb), p.gp = take(q * tb);
     p.kx = take(k * 4), p.vx = take(k * 4), p.qx = take(q * 4), p.gx = take(q * 4), p.stats = take(q * 256);
+    p.kr = take(k * 4 * kTile), p.vr = take(k * 4 * kTile), p.qr = take(q * 4 * kTile);
     if (p.qsplits > 1 && !p.few) p.pq = take(p.qsplits * p.nq * 4);
     if (p.ksplits > 1) p.pk = take(p.ksplits * p.nk * 4), p.pv = take(p.ksplits * p.nk * 4);
     p.total = at;
@@ -1085,17 +1116,18 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
     f.a = a;
     f.kp = w + p.kp, f.vp = w + p.vp, f.qp = w + p.qp, f.gp = w + p.gp;
     f.kx = (int *)(w + p.kx), f.vx = (int *)(w + p.vx), f.qx = (int *)(w + p.qx), f.gx = (int *)(w + p.gx);
+    f.kr = (float *)(w + p.kr), f.vr = (float *)(w + p.vr), f.qr = (float *)(w + p.qr);
     f.stats = (float *)(w + p.stats);
     f.key_len = key_len;
     f.rows = p.rows, f.qtiles = p.qtiles, f.ktiles = p.ktiles;
     PackArgs pk{};
     pk.a = a, pk.key_len = key_len;
     if (Lk) {
-        pk.job[pk.jobs++] = {k, sk[0], sk[1], sk[2], Lk, p.ktiles, 1, w + p.kp, (int *)(w + p.kx), nullptr, 0, nullptr, nullptr, nullptr};
-        pk.job[pk.jobs++] = {v, sv[0], sv[1], sv[2], Lk, p.ktiles, 1, w + p.vp, (int *)(w + p.vx), nullptr, 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {k, sk[0], sk[1], sk[2], Lk, p.ktiles, 1, w + p.kp, (int *)(w + p.kx), (float *)(w + p.kr), 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {v, sv[0], sv[1], sv[2], Lk, p.ktiles, 1, w + p.vp, (int *)(w + p.vx), (float *)(w + p.vr), 0, nullptr, nullptr, nullptr};
     }
     if (Lq) {
-        pk.job[pk.jobs++] = {q, sq[0], sq[1], sq[2], p.rows, p.qtiles, 0, w + p.qp, (int *)(w + p.qx), nullptr, 0, nullptr, nullptr, nullptr};
+        pk.job[pk.jobs++] = {q, sq[0], sq[1], sq[2], p.rows, p.qtiles, 0, w + p.qp, (int *)(w + p.qx), (float *)(w + p.qr), 0, nullptr, nullptr, nullptr};
         pk.job[pk.jobs++] = {go, Lq * Hq * D, Hq * D, D, p.rows, p.qtiles, 0, w + p.gp, (int *)(w + p.gx), nullptr, 0, o, lse, (float *)(w + p.stats)};
     }
     pack_launch(pk, p.pairs, p.DP, st);
@@ -1119,7 +1151,7 @@ extern "C" NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int6
         f.part_k = p.nk, f.groups = p.kgroups, f.splits = p.ksplits;
         f.units = p.pairs * p.kgroups * p.ksplits;
         NC_ATTN_DP(p.DP, constexpr int OCC = DP <= 64 ? 4 : 2;
-                   attn_launch(&k_attn_dkv<DP, OCC>, f.units, 2 * (2 * 128 * DP + 256) + 16384, st, f, 2 * kAttnB));
+                   attn_launch(&k_attn_dkv<DP, OCC>, f.units, 2 * (2 * 128 * DP + 256) + 4 * 320 * 16, st, f, 2 * kAttnB));
         if (cut) sum_launch(p.nk, p.ksplits, f.gk, gk, acc_k, f.gv, gv, acc_v, st);
     }
     return check_launch(what);

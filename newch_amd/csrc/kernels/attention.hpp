@@ -283,6 +283,61 @@ __device__ __forceinline__ bool column_scale(float most, float &F, float &by) {
     return __any(over);
 }
 
+// a result's rows 8 (r / 4) + 4 (lane / 32) + r % 4 times 2^ the exponents of a tile's 32 rows
+__device__ __forceinline__ void scale_rows(f16x &s, const float *rows) {
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const f4 e = *(const f4 *)(rows + 4 * half + 8 * j);
+#pragma unroll
+        for (int x = 0; x < 4; x++) s[4 * j + x] *= __builtin_amdgcn_exp2f(e[x]);
+    }
+}
+__device__ __forceinline__ float largest(const f16x &s) {
+    float most = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; r++) most = __builtin_fmaxf(most, __builtin_fabsf(s[r]));
+    return most;
+}
+
+// gv's sums: a lane's column (a key) has a unit 2^U of its own, for products of probabilities and gradients of 2^e.  Probabilities
+// are taken as p 2^first_shift; where one of 1 would pass 2^14 in the unit, or the tile is `loose`, column_unit looks at the column's
+// largest: the unit is raised so that 1 is 2^14 where the key is counted by 2^-16 and up, else so that this largest product is 2^10.
+// So a tile of large gradients whose rows do not count a key leaves it its bits, and a key that is hardly counted by any row has
+// its own.  Returns the shift of the probabilities as they are left, e - U.
+constexpr float kPTop = 10.0f, kPSlack = 4.0f, kNoUnit = -1000.0f;
+__device__ __forceinline__ float first_shift(float e, float U) {  // no less than -60: far below what gv can show
+    return __builtin_fminf(__builtin_fmaxf(e - U, -60.0f), kPTop + kPSlack);
+}
+template <int NT>
+__device__ __forceinline__ float column_unit(f16x &p, float e, bool loose, float &U, f16x (&acc)[NT]) {
+    constexpr float most = kPTop + kPSlack;
+    float shift = first_shift(e, U);
+    if (__any(e - U > most) || loose) {
+        float top = 0.0f;
+        const float one = __builtin_amdgcn_ldexpf(1.0f, (int)shift);
+#pragma unroll
+        for (int r = 0; r < 16; r++) p[r] = p[r] > one ? one : p[r], top = __builtin_fmaxf(top, p[r]);
+        top = halves_max(top);
+        const float log_top = (float)((int)(__float_as_uint(top) >> 23) - 126) - shift;  // rounded up; far below where there is none
+        const float need = log_top >= -16.0f ? e - most : __builtin_fmaxf(log_top + (e - kPTop), e - 100.0f);
+        const float Un = e - U > most ? __builtin_fmaxf(U, need) : U, left = __builtin_fmaxf(e - Un, -60.0f);
+        const float by = __builtin_amdgcn_exp2f(U - Un), to = __builtin_amdgcn_exp2f(left - shift);
+        U = Un;
+        shift = left;
+#pragma unroll
+        for (int r = 0; r < 16; r++) p[r] *= to;
+#pragma unroll
+        for (int d = 0; d < NT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[d][r] *= by;
+    }
+    return shift;
+}
+// A probability taken from scores and their sum past 2^20 may come out above 1, far past 2^24: a tile with such rows is marked.
+__device__ __forceinline__ bool loose(float log_sum) { return __builtin_fabsf(log_sum) > 0x1p20f && log_sum < INFINITY; }
+__device__ __forceinline__ float unit_of(float U) { return __builtin_amdgcn_ldexpf(1.0f, (int)__builtin_fmaxf(U, -1000.0f)); }
+
 // The scale of the scores times 2^e, e far outside a float's exponents where the scale is: it goes into the scores' gradients before
 // their column scale, which would lose them else.
 struct ScaleParts {
@@ -296,16 +351,6 @@ struct ScaleParts {
 };
 // kap F, held finite: where it is not, every gradient of the tile is zero, or past a float's range
 __device__ __forceinline__ float finite_product(float kap, float F) { return __builtin_fminf(__builtin_fmaxf(kap * F, -0x1p127f), 0x1p127f); }
-
-// a result's rows 8 (r / 4) + 4 half + r % 4 times 2^ their own exponents, which are given from 4 half on
-__device__ __forceinline__ void scale_rows(f16x &s, const float *rows) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const f4 e = *(const f4 *)(rows + 8 * j);
-#pragma unroll
-        for (int x = 0; x < 4; x++) s[4 * j + x] *= __builtin_amdgcn_exp2f(e[x]);
-    }
-}
 
 template <int NT>
 __device__ __forceinline__ void scale_acc(f16x (&acc)[NT], float by) {
@@ -338,8 +383,6 @@ __device__ __forceinline__ void store_column(float *row, const f16x (&acc)[NT], 
 // exponent of the tile's values, U that of o's unit, a row's own, which is raised so that its largest product -- p and value
 // together -- lies at 2^10 when it passes 2^14, and falls as m rises.  So a value that is large and does not count leaves the
 // others their bits, and a product below 2^-24 of a row's largest loses low bits against an absolute 2^-35 of it.
-constexpr float kPTop = 10.0f, kPSlack = 4.0f;
-
 template <int DP>
 struct Query {  // the rows times scale log2(e), as the second operand: column fragments of q^T
     h8 hi[DP / 16], lo[DP / 16];
@@ -365,8 +408,6 @@ __device__ __forceinline__ void load_query(Query<DP> &q, const float *row, bool 
         q.hi[s] = p.hi, q.lo[s] = p.lo;
     }
 }
-
-__device__ __forceinline__ float unit_of(float U) { return __builtin_amdgcn_ldexpf(1.0f, (int)__builtin_fmaxf(U, -1000.0f)); }
 
 template <int DP>
 struct Sums {
@@ -408,8 +449,8 @@ __device__ __forceinline__ void join(Sums<DP> &a, const f4 *from) {
     a.m = m, a.U = U;
 }
 
-// kt, vt: the tile's keys and values in LDS, at this lane's row_at and col_at; ek, ev: their exponents, kr, vr: their rows', from 4
-// half on, read where they have their own; left: keys of the tile that count (32 but in the last one), less 4 half
+// kt, vt: the tile's keys and values in LDS, at this lane's row_at and col_at; ek, ev: their exponents; kr, vr: their rows', read where
+// they have their own; left: keys of the tile that count (32 but in the last one), less 4 half
 template <int DP>
 __device__ __forceinline__ void attend(Sums<DP> &a, const Query<DP> &q, const char *kt, const char *vt, int ek, int ev, const float *kr,
                                        const float *vr, bool cut, int left) {
@@ -445,11 +486,12 @@ __device__ __forceinline__ void attend(Sums<DP> &a, const Query<DP> &q, const ch
         a.U += down;
         a.m = mn;
         if (own) {  // p's sum, then p times 2^ its value's own exponent in p's place
+            const int half = (threadIdx.x >> 5) & 1;
             float sum = 0.0f;
             top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const f4 er = *(const f4 *)(vr + 8 * j);
+                const f4 er = *(const f4 *)(vr + 4 * half + 8 * j);
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
                     const int r = 4 * j + x;

@@ -9,9 +9,9 @@
 namespace nchip {
 
 // A wave reads 32 rows of `src` (from `row0` on, n in all, `step` floats apart): the tile's exponent, with kOwnRows added where its rows
-// have their own (wanted: own is given, this lane's row's); and splits them into LDS.
+// have their own, and this lane's row's; and splits them into LDS.
 template <int DP>
-__device__ __forceinline__ int tile_load(const float *src, int64_t step, int row0, int n, int D, float (&x)[DP / 16][8], int *own = nullptr) {
+__device__ __forceinline__ int tile_load(const float *src, int64_t step, int row0, int n, int D, float (&x)[DP / 16][8], int &own) {
     const int lane = threadIdx.x & 63, half = lane >> 5, r = lane & 31;
     const bool live = row0 + r < n;
     float most = 0.0f;
@@ -24,10 +24,9 @@ __device__ __forceinline__ int tile_load(const float *src, int64_t step, int row
     }
     const float top = wave_max_nan_skip(most);
     const int ex = tile_exponent(top);
-    if (!own) return ex;
     most = halves_max(most);
     const bool unlike = rows_unlike(most, top);
-    *own = unlike ? row_exponent(most, ex) : ex;
+    own = unlike ? row_exponent(most, ex) : ex;
     return unlike ? ex + kOwnRows : ex;
 }
 template <int DP>
@@ -67,7 +66,7 @@ __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd
             const float *src = val ? f.v + b * a.sv[0] + u * a.sv[2] : f.k + b * a.sk[0] + u * a.sk[2];
             float x[DP / 16][8];
             int er;
-            const int at = val ? f.tiles + k : k, e = tile_load<DP>(src, val ? a.sv[1] : a.sk[1], k * kTile, n, (int)a.D, x, &er);
+            const int at = val ? f.tiles + k : k, e = tile_load<DP>(src, val ? a.sv[1] : a.sk[1], k * kTile, n, (int)a.D, x, er);
             tile_split<DP>(x, er, smem + at * TB);
             if (lane == 0) exps[at] = e;
             if (own_rows(e) && half == 0) rows[at * kTile + lane] = (float)(er - exponent_of(e));
@@ -86,7 +85,7 @@ __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd
             const char *kt = smem + row_at(lane), *vt = smem + f.tiles * TB + col_at(lane);
             for (int t = 0; t < nt; t++)
                 attend(sum, q, kt + t * TB, vt + t * TB, __builtin_amdgcn_readfirstlane(exps[t]), __builtin_amdgcn_readfirstlane(exps[f.tiles + t]),
-                       rows + t * kTile + 4 * half, rows + (f.tiles + t) * kTile + 4 * half, t + 1 == nt, min(n - t * kTile, kTile) - 4 * half);
+                       rows + t * kTile, rows + (f.tiles + t) * kTile, t + 1 == nt, min(n - t * kTile, kTile) - 4 * half);
             const float l = halves_sum(sum.l);
             if (live) {
                 store_column<false>(f.o + ((b * a.Lq + i) * a.Hq + h) * a.D, sum.o, true, l != 0.0f ? unit_of(sum.U) / l : 0.0f, half, (int)a.D, 0);
@@ -115,105 +114,213 @@ __device__ __forceinline__ h8 turned16(const char *first, const char *second) {
 constexpr int kDsTile = 4096;  // bytes of a packed tile of 32 columns
 
 // The backward's way in: the workgroup's W waves read a tile of 32 rows of queries, output gradients and outputs, one tile ahead,
-// and split it.  Piece p is columns 8 (p / 32) .. + 7 of row p % 32.
+// and split it, a piece a lane: piece p is columns 8 (p / 32) .. + 7 of row p % 32.  A tile whose rows are unlike (rows_unlike, of queries
+// or of gradients) is taken in several passes, each with the rows that are alike and zeros in the others' places.
+template <int DP, int W>
+struct FeedTables {  // in LDS
+    float stats[64];                // the rows' log2-sum-exps (infinite: not in this pass) and go . o
+    float dots[DP / 8][kTile];      // scratch
+    float red[2][W];
+    uint32_t masks[W][4];
+    uint32_t loose_rows, unused[3];
+};
+struct FeedPass {
+    int eq, eg;       // exponents of the tile's queries and gradients
+    uint32_t rows;    // that are in this pass; none: the tile takes several, or has a row that is loose
+    bool last, hold;  // the tile's last; a row may be loose
+};
 template <int DP, int W>
 struct Feed {
-    static constexpr int THREADS = W * kWave, UNITS = 4 * DP, PER = (UNITS + THREADS - 1) / THREADS;
-    float q[PER][8], go[PER][8], o[PER][8], lse;
+    static constexpr int UNITS = 4 * DP;
+    static_assert(UNITS <= W * kWave, "a piece a lane");
+    float q[8], go[8], o[8], lse;
 
     __device__ __forceinline__ void fetch(const ShortBwd &f, int64_t b, int64_t u, int64_t t) {
         const AttnArgs &a = f.a;
-        const int D = (int)a.D;
-#pragma unroll
-        for (int k = 0; k < PER; k++) {
-            const int p = threadIdx.x + k * THREADS;
-            const int64_t R = t * kTile + (p & 31);
-            const bool in = p < UNITS && R < f.rows;
-            int64_t i, g;
-            a.row(in ? R : 0, i, g);
-            const int64_t h = u * a.G + g;
-            const int64_t at = ((b * a.Lq + i) * a.Hq + h) * D;
-            const int d = in ? 8 * (p >> 5) : D;  // nothing is read from column D on
-            load8(f.q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2], d, D, q[k]);
-            load8(f.go + at, d, D, go[k]);
-            load8(f.o + at, d, D, o[k]);
-            if (k == 0) lse = p < 32 && in ? f.lse[(b * a.Hq + h) * a.Lq + i] * kLog2e : INFINITY;
-        }
+        const int D = (int)a.D, p = threadIdx.x;
+        const int64_t R = t * kTile + (p & 31);
+        const bool in = p < UNITS && R < f.rows;
+        int64_t i, g;
+        a.row(in ? R : 0, i, g);
+        const int64_t h = u * a.G + g;
+        const int64_t at = ((b * a.Lq + i) * a.Hq + h) * D;
+        const int d = in ? 8 * (p >> 5) : D;  // nothing is read from column D on
+        load8(f.q + b * a.sq[0] + i * a.sq[1] + h * a.sq[2], d, D, q);
+        load8(f.go + at, d, D, go);
+        load8(f.o + at, d, D, o);
+        lse = p < 32 && in ? f.lse[(b * a.Hq + h) * a.Lq + i] * kLog2e : INFINITY;
     }
 
-    // into the tiles qs and gs, with stats[64]: the rows' log2-sum-exps and go . o; dots [DP / 8][32] and red [2][W] are scratch
-    __device__ __forceinline__ void split(char *qs, char *gs, float *stats, float *dots, float *red, int &eq, int &eg) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        float mq = 0.0f, mg = 0.0f;
+    // this lane's piece under 2^ex, or zeros
+    static __device__ __forceinline__ void put(const float (&x)[8], int ex, bool in, char *tile) {
+        const int p = threadIdx.x, c = p >> 5, at = 16 * (32 * c + ((p & 31) ^ (4 * (c & 1))));
+        if (p >= UNITS) return;
+        const float by = pow2i(-ex);
+        float y[8];
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            const int p = threadIdx.x + k * THREADS;
-            float dot = 0.0f;
-            mq = abs_max(q[k], mq), mg = abs_max(go[k], mg);
-#pragma unroll
-            for (int e = 0; e < 8; e++) dot = fma_(go[k][e], o[k][e], dot);
-            if (p < UNITS) dots[p] = dot;
-        }
-        mq = wave_max_nan_skip(mq), mg = wave_max_nan_skip(mg);
-        if (lane == 0) red[wave] = mq, red[W + wave] = mg;
+        for (int e = 0; e < 8; e++) y[e] = in ? x[e] * by : 0.0f;
+        const Split8 s = split8(y);
+        *(h8 *)(tile + at) = s.hi, *(h8 *)(tile + 64 * DP + at) = s.lo;
+    }
+    // the largest of this lane's row; all lanes of the workgroup
+    static __device__ __forceinline__ float of_row(float piece, FeedTables<DP, W> &t) {
+        const int p = threadIdx.x;
+        __syncthreads();  // dots have been read
+        if (p < UNITS) t.dots[p >> 5][p & 31] = piece;
         __syncthreads();
-        mq = red[0], mg = red[W];
+        float most = t.dots[0][p & 31];
+        for (int c = 1; c < DP / 8; c++) most = __builtin_fmaxf(most, t.dots[c][p & 31]);
+        return most;
+    }
+
+    // into the tiles qs and gs, and the tables
+    __device__ __forceinline__ FeedPass split(char *qs, char *gs, FeedTables<DP, W> &t) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p = threadIdx.x;
+        const float mq = abs_max(q, 0.0f), mg = abs_max(go, 0.0f);
+        float dot = 0.0f;
 #pragma unroll
-        for (int x = 1; x < W; x++) mq = __builtin_fmaxf(mq, red[x]), mg = __builtin_fmaxf(mg, red[W + x]);
-        eq = tile_exponent(mq), eg = tile_exponent(mg);
-        const float iq = pow2i(-eq), ig = pow2i(-eg);
+        for (int e = 0; e < 8; e++) dot = fma_(go[e], o[e], dot);
+        if (p < UNITS) t.dots[p >> 5][p & 31] = dot;
+        float tq = wave_max_nan_skip(mq), tg = wave_max_nan_skip(mg);
+        if (lane == 0) t.red[0][wave] = tq, t.red[1][wave] = tg;
+        __syncthreads();
+        tq = t.red[0][0], tg = t.red[1][0];
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            const int p = threadIdx.x + k * THREADS, c = p >> 5;
-            if (p >= UNITS) continue;
+        for (int x = 1; x < W; x++) tq = __builtin_fmaxf(tq, t.red[0][x]), tg = __builtin_fmaxf(tg, t.red[1][x]);
+        const int eq = tile_exponent(tq), eg = tile_exponent(tg);
+        // rows that hold something, and rows that hold something of 2^-6 of the tile's largest and up
+        const auto rows_of = [](bool v) {
+            const uint64_t m = __ballot(v);
+            return (uint32_t)m | (uint32_t)(m >> 32);
+        };
+        const uint32_t some_q = rows_of(mq > 0.0f), large_q = rows_of(mq >= tq * 0x1p-6f);
+        const uint32_t some_g = rows_of(mg > 0.0f), large_g = rows_of(mg >= tg * 0x1p-6f), loose_rows = rows_of(loose(lse));
+        if (lane == 0) t.masks[wave][0] = some_q, t.masks[wave][1] = large_q, t.masks[wave][2] = some_g, t.masks[wave][3] = large_g;
+        if (p == 0) t.loose_rows = loose_rows;  // the first wave has all rows' log-sum-exps
+        put(q, eq, true, qs);
+        put(go, eg, true, gs);
+        if (p < kTile) {
+            float d = t.dots[0][p];
 #pragma unroll
-            for (int e = 0; e < 8; e++) q[k][e] *= iq, go[k][e] *= ig;
-            const int at = 16 * (32 * c + ((p & 31) ^ (4 * (c & 1))));
-            const Split8 x = split8(q[k]), y = split8(go[k]);
-            *(h8 *)(qs + at) = x.hi, *(h8 *)(qs + 64 * DP + at) = x.lo;
-            *(h8 *)(gs + at) = y.hi, *(h8 *)(gs + 64 * DP + at) = y.lo;
-        }
-        if (threadIdx.x < 32) {
-            float d = dots[threadIdx.x];
-#pragma unroll
-            for (int c = 1; c < DP / 8; c++) d += dots[32 * c + threadIdx.x];
-            stats[threadIdx.x] = lse;
-            stats[32 + threadIdx.x] = d;
+            for (int c = 1; c < DP / 8; c++) d += t.dots[c][p];
+            t.stats[p] = lse;
+            t.stats[32 + p] = d;
         }
         __syncthreads();
+        uint32_t m[4] = {};
+#pragma unroll
+        for (int w = 0; w < W; w++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) m[x] |= t.masks[w][x];
+        const uint32_t unlike = __builtin_amdgcn_readfirstlane((m[0] & ~m[1]) | (m[2] & ~m[3]) | t.loose_rows);
+        return {eq, eg, unlike ? 0u : ~0u, true, false};
+    }
+
+    // the same for those rows of `todo` that are like the one of the largest queries, and among them like the one of the largest gradients
+    __device__ __forceinline__ FeedPass split_alike(char *qs, char *gs, FeedTables<DP, W> &t, uint32_t todo) {
+        const int p = threadIdx.x;
+        const float row_q = of_row(abs_max(q, 0.0f), t), row_g = of_row(abs_max(go, 0.0f), t);
+        bool in = (todo >> (p & 31)) & 1;
+        const float tq = wave_max_nan_skip(in ? row_q : 0.0f);
+        in = in && (row_q == 0.0f || row_q >= tq * 0x1p-6f);
+        const float tg = wave_max_nan_skip(in ? row_g : 0.0f);
+        in = in && (row_g == 0.0f || row_g >= tg * 0x1p-6f);
+        const uint32_t rows = (uint32_t)__ballot(in);
+        float dot = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) dot = fma_(go[e], o[e], dot);
+        __syncthreads();  // dots have been read
+        if (p < UNITS) t.dots[p >> 5][p & 31] = dot;
+        const int eq = tile_exponent(tq), eg = tile_exponent(tg);
+        put(q, eq, in, qs);
+        put(go, eg, in, gs);
+        __syncthreads();
+        if (p < kTile) {
+            float d = t.dots[0][p];
+            for (int c = 1; c < DP / 8; c++) d += t.dots[c][p];
+            t.stats[p] = in ? lse : INFINITY;
+            t.stats[32 + p] = in ? d : 0.0f;
+        }
+        __syncthreads();
+        return {eq, eg, rows, (todo & ~rows) == 0, true};
+    }
+
+    // The next pass, of tile t, with the next tile's rows on their way.  The rows of a tile that takes several are read again for each:
+    // kept, they would cost the others' registers.
+    __device__ __forceinline__ FeedPass pass(const ShortBwd &f, int64_t b, int64_t u, int64_t &t, int64_t t1, uint32_t &todo, char *qs, char *gs,
+                                             FeedTables<DP, W> &tables) {
+        FeedPass r;
+        r.rows = 0;
+        if (todo == ~0u) {
+            r = split(qs, gs, tables);
+            if (t + 1 < t1) fetch(f, b, u, t + 1);
+        }
+        if (__builtin_expect(r.rows == 0, 0)) {
+            fetch(f, b, u, t);
+            r = split_alike(qs, gs, tables, todo);
+            todo = r.last ? ~0u : todo & ~r.rows;
+            if (r.last && t + 1 < t1) fetch(f, b, u, t + 1);
+        }
+        t += r.last;
+        return r;
     }
 };
 
-// A wave's ds (32 rows of queries as a result's rows, its keys the columns; `most` its lane's largest) in two pieces as a packed
-// tile of 32 rows of keys, whose columns are the rows of queries; returns the tile's exponent.
-__device__ __forceinline__ int put_ds(const f16x &ds, float most, char *tile) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    float finite = most;
-    if (__builtin_expect(most == INFINITY, 0)) {  // a row of queries with an infinity leaves the others their scale
-        finite = 0.0f;
+// The largest of each of a result's 16 rows over its 32 columns, a lane's times f, in magnitude: lane l gets register (l / 2) % 16's.
+// Each step halves the registers and the lanes that have to be joined.
+__device__ __forceinline__ float largest_of_rows(const f16x &x, float f) {
+    const int lane = threadIdx.x & 63;
+    float a[8];
 #pragma unroll
-        for (int r = 0; r < 16; r++) finite = __builtin_fmaxf(finite, __builtin_fabsf(ds[r]) < INFINITY ? __builtin_fabsf(ds[r]) : 0.0f);
+    for (int r = 0; r < 8; r++) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_int(x[r] * f), __float_as_int(x[r + 8] * f), false, false);
+        a[r] = __builtin_fmaxf(__builtin_fabsf(__int_as_float(s[0])), __builtin_fabsf(__int_as_float(s[1])));
     }
-    const int ed = tile_exponent(wave_max_nan_skip(finite));
-    const float id = pow2i(-ed);
+    const auto halve = [&](int n, bool upper, auto from) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if (r >= n) break;
+            const float keep = upper ? a[r + n] : a[r], give = upper ? a[r] : a[r + n];
+            a[r] = __builtin_fmaxf(keep, from(give));
+        }
+    };
+    halve(4, lane & 8, [](float v) { return dpp_f32<kDppRor8>(v, 0.0f); });
+    halve(2, lane & 4, [](float v) { return dpp_f32<kDppHalfMirror>(v, 0.0f); });
+    halve(1, lane & 2, [](float v) { return dpp_f32<kDppXor2>(v, 0.0f); });
+    return __builtin_fmaxf(a[0], dpp_f32<kDppXor1>(a[0], 0.0f));
+}
+
+// A wave's ds (32 rows of queries as a result's rows, its keys the columns), a lane's times f, in two pieces as a packed tile of 32 rows
+// of keys, whose columns are the rows of queries.  Each row of queries has a scale of its own, its gradients being small or large with
+// the values and gradients that it meets: scale [2][32], 2^(its exponent - 14), and its inverse less the 14.
+__device__ __forceinline__ void put_ds(const f16x &ds, float f, char *tile, float *scale) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, r = (lane >> 1) & 15;
+    const int er = tile_exponent(largest_of_rows(ds, f)), at = 8 * (r / 4) + 4 * half + r % 4;
+    scale[at] = pow2i(max(er - 14, -126));
+    scale[kTile + at] = pow2i(-er);
+    asm volatile("" ::: "memory");  // a wave's LDS accesses are in order
 #pragma unroll
     for (int j = 0; j < 4; j += 2) {
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = ds[4 * j + e] * id;
-        const Split8 x = split8(y);
-        char *const at = tile + 512 * j + 8 * half;
+        for (int h = 0; h < 2; h++) {
+            const f4 inv = *(const f4 *)(scale + kTile + 4 * half + 8 * (j + h));
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[4 * h + e] = ds[4 * (j + h) + e] * f * inv[e];
+        }
+        const Split8 s = split8(y);
+        char *const to = tile + 512 * j + 8 * half;
         const int r0 = 16 * (lane & 31), r1 = r0 ^ 64;
-        *(h4 *)(at + r0) = x.hi.lo, *(h4 *)(at + 512 + r1) = x.hi.hi;
-        *(h4 *)(at + 2048 + r0) = x.lo.lo, *(h4 *)(at + 2560 + r1) = x.lo.hi;
+        *(h4 *)(to + r0) = s.hi.lo, *(h4 *)(to + 512 + r1) = s.hi.hi;
+        *(h4 *)(to + 2048 + r0) = s.lo.lo, *(h4 *)(to + 2560 + r1) = s.lo.hi;
     }
-    return ed;
 }
 
-// gq^T = k^T ds^T over all nt tiles of keys, blocks of 16 columns and 16 rows of queries dealt over the W waves; scale[y]: the
-// scales of tile y's ds, and of its keys
+// gq^T = k^T ds^T over all nt tiles of keys, blocks of 16 columns and 16 rows of queries dealt over the W waves; rows
+// [nt][2][32] and keys_by [nt]: the scales of a tile's ds, and of its keys; in: the rows of queries that are stored
 template <int DP, int W>
-__device__ __forceinline__ void gq_blocks(const ShortBwd &f, int64_t b, int64_t u, int64_t t, int nt, const char *keys, const char *dss, const f2 *scale) {
+__device__ __forceinline__ void gq_blocks(const ShortBwd &f, int64_t b, int64_t u, int64_t t, int nt, const char *keys, const char *dss, const float *rows,
+                                          const float *keys_by, uint32_t in) {
     constexpr int TB = 128 * DP, LO = 64 * DP, BLOCKS = DP / 8, PW = (BLOCKS + W - 1) / W;
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ta = turned_at(lane);
@@ -221,7 +328,7 @@ __device__ __forceinline__ void gq_blocks(const ShortBwd &f, int64_t b, int64_t 
 #pragma unroll
     for (int x = 0; x < PW; x++) sum[x] = f4{0.f, 0.f, 0.f, 0.f};
     for (int y = 0; y < nt; y++) {
-        const f2 by = scale[y];
+        const float by_keys = keys_by[y];
 #pragma unroll
         for (int x = 0; x < PW; x++) {
             const int block = wave + x * W, c = block % (DP / 16), r = block / (DP / 16);
@@ -229,19 +336,20 @@ __device__ __forceinline__ void gq_blocks(const ShortBwd &f, int64_t b, int64_t 
             const char *const kc = keys + y * TB + 1024 * c + ta, *const dc = dss + y * kDsTile + 1024 * r + ta;
             const char *const kc2 = keys + y * TB + 1024 * c + (ta ^ 64), *const dc2 = dss + y * kDsTile + 1024 * r + (ta ^ 64);
             const h8 ah = turned16(kc, kc2), al = turned16(kc + LO, kc2 + LO), bh = turned16(dc, dc2), bl = turned16(dc + 2048, dc2 + 2048);
+            const float by = rows[2 * y * kTile + 16 * r + (lane & 15)];
             f4 v = {0.f, 0.f, 0.f, 0.f};
             v = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, v, 0, 0, 0);
             v = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, v, 0, 0, 0);
             v = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, v, 0, 0, 0);
 #pragma unroll
-            for (int e = 0; e < 4; e++) sum[x][e] = fma_(v[e] * by.x, by.y, sum[x][e]);
+            for (int e = 0; e < 4; e++) sum[x][e] = fma_(v[e] * by, by_keys, sum[x][e]);
         }
     }
 #pragma unroll
     for (int x = 0; x < PW; x++) {
         const int block = wave + x * W, c = block % (DP / 16), r = block / (DP / 16);
         const int64_t R = t * kTile + 16 * r + (lane & 15);
-        if (block >= BLOCKS || R >= f.rows) continue;
+        if (block >= BLOCKS || R >= f.rows || !((in >> (16 * r + (lane & 15))) & 1)) continue;
         int64_t i, g;
         a.row(R, i, g);
         store4(f.gq + ((b * a.Lq + i) * a.Hq + u * a.G + g) * a.D, 16 * c + 4 * (lane >> 4), (int)a.D, sum[x], f.acc_q);
@@ -256,12 +364,12 @@ __device__ __forceinline__ void gq_blocks(const ShortBwd &f, int64_t b, int64_t 
 template <int DP, int W>
 __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP;
+    constexpr bool REG = DP <= 32;  // keys stay in registers, else they are read from LDS for every tile, where they are anyway
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     // q's tile, go's tile, the waves' keys, their ds, then small tables
     char *const qs = smem, *const gs = smem + TB, *const keys = smem + 2 * TB, *const dss = keys + W * TB;
-    float *const small = (float *)(dss + W * kDsTile);
-    float *const stats = small, *const dots = small + 64, *const red = dots + (DP / 8) * 32;  // [64], [DP / 8][32], [2][W]
-    f2 *const dsx = (f2 *)(red + 2 * W);  // [W]: the scales of the waves' ds, and of their keys
+    FeedTables<DP, W> &tables = *(FeedTables<DP, W> *)(dss + W * kDsTile);
+    float *const ds_by = (float *)(&tables + 1), *const keys_by = ds_by + 2 * W * kTile;  // [W][2][32], [W]: the scales of the waves' ds and of their keys
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ra = row_at(lane), ca = col_at(lane), D = (int)a.D;
@@ -278,64 +386,65 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
         Feed<DP, W> next;
         __syncthreads();  // the last unit's keys have been read
         if (t0 < t1) next.fetch(f, b, u, t0);
-        h8 kh[KS], kl[KS], vh[KS], vl[KS];
-        float ek = 0.0f, ev = 0.0f;
+        h8 kh[REG ? KS : 1], kl[REG ? KS : 1], vh[KS], vl[KS];
+        int ek = 0, own_k = 0, own_v = 0;  // the keys' tile's exponent, this lane's key's and value's
         if (mine) {  // this wave's values, through the place of its keys, and its keys, which stay
             float x[KS][8];
-            ev = (float)tile_load<DP>(f.v + b * a.sv[0] + u * a.sv[2], a.sv[1], kw * kTile, n, D, x);
-            tile_split<DP>(x, (int)ev, kt);
+            (void)tile_load<DP>(f.v + b * a.sv[0] + u * a.sv[2], a.sv[1], kw * kTile, n, D, x, own_v);
+            tile_split<DP>(x, own_v, kt);
 #pragma unroll
             for (int s = 0; s < KS; s++) vh[s] = row_frag(kt + ra, s), vl[s] = row_frag(kt + ra + LO, s);
-            ek = (float)tile_load<DP>(f.k + b * a.sk[0] + u * a.sk[2], a.sk[1], kw * kTile, n, D, x);
-            tile_split<DP>(x, (int)ek, kt);
+            ek = exponent_of(tile_load<DP>(f.k + b * a.sk[0] + u * a.sk[2], a.sk[1], kw * kTile, n, D, x, own_k));
+            tile_split<DP>(x, own_k, kt);
+            if constexpr (REG) {
 #pragma unroll
-            for (int s = 0; s < KS; s++) kh[s] = row_frag(kt + ra, s), kl[s] = row_frag(kt + ra + LO, s);
+                for (int s = 0; s < KS; s++) kh[s] = row_frag(kt + ra, s), kl[s] = row_frag(kt + ra + LO, s);
+            }
+            if (lane == 0) keys_by[kw] = pow2i(ek) * a.scale;
         }
         f16x dk[NT], dv[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) dk[t][r] = dv[t][r] = 0.0f;
-        float F = 0x1p100f, E = -1000.0f;
+        float F = 0x1p100f, U = live ? kNoUnit : -kNoUnit;
         const ScaleParts parts(a.scale);
-        const float ck = pow2i((int)ek) * a.scale * kLog2e, cv = pow2i((int)ev);
-        for (int64_t t = t0; t < t1; t++) {
-            int eq, eg;
-            next.split(qs, gs, stats, dots, red, eq, eg);
-            if (t + 1 < t1) next.fetch(f, b, u, t + 1);
+        const float ck = pow2i(own_k) * a.scale * kLog2e, cv = pow2i(own_v), key_below = (float)(own_k - ek);
+        uint32_t todo = ~0u;  // rows of a tile that no pass had
+        for (int64_t t = t0, tn = t0; t < t1; t = tn) {
+            const FeedPass pass = next.pass(f, b, u, tn, t1, todo, qs, gs, tables);
             if (mine) {
                 const char *qt = qs + ra, *gt = gs + ra, *qc = qs + ca, *gc = gs + ca;
-                const f4 *rows = (const f4 *)stats + half;
+                const f4 *rows = (const f4 *)tables.stats + half;
                 f16x s, dp;
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.0f;
                 steps<2 * KS>([&](int k) { return k % 2 ? Pieces{row_frag(gt, k / 2), row_frag(gt + LO, k / 2)} : Pieces{row_frag(qt, k / 2), row_frag(qt + LO, k / 2)}; },
                               [&](int k, const Pieces &x) {
                                   if (k % 2) dp = mfma3(x.hi, x.lo, vh[k / 2], vl[k / 2], dp);
-                                  else s = mfma3(x.hi, x.lo, kh[k / 2], kl[k / 2], s);
+                                  else s = mfma3(x.hi, x.lo, REG ? kh[k / 2] : row_frag(kt + ra, k / 2), REG ? kl[k / 2] : row_frag(kt + ra + LO, k / 2), s);
                               });
-                const float ex = (float)eg;
-                if (ex > E) {
-                    scale_acc(dv, __builtin_amdgcn_exp2f(E - ex));
-                    E = ex;
-                }
-                const float sh = 14.0f + __builtin_fmaxf(ex - E, -60.0f), base = live ? sh : -INFINITY;
-                const float c = ck * pow2i(eq), c2 = cv * pow2i(eg);
+                const float c = ck * pow2i(pass.eq), c2 = cv * pow2i(pass.eg), xg = (float)pass.eg, off = live ? first_shift(xg, U) : -INFINITY;
                 float most = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const f4 ls = rows[2 * j], de = rows[8 + 2 * j];
+                    const f4 ls = rows[2 * j];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[4 * j + e] = __builtin_amdgcn_exp2f(fma_(s[4 * j + e], c, off - ls[e]));
+                }
+                const float sh = column_unit(s, xg, pass.hold, U, dv);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const f4 de = rows[8 + 2 * j];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int r = 4 * j + e;
-                        s[r] = __builtin_amdgcn_exp2f(fma_(s[r], c, base - ls[e]));
                         dp[r] = s[r] * fma_(dp[r], c2, -de[e]);
                         most = __builtin_fmaxf(most, __builtin_fabsf(dp[r]));
                     }
                 }
-                const int ed = put_ds(dp, most, mine_ds);
-                if (lane == 0) dsx[kw] = f2{__builtin_amdgcn_exp2f((float)ed - sh), pow2i((int)ek) * a.scale};
-                const float kap = parts.times((float)eq - sh);
+                put_ds(dp, __builtin_amdgcn_exp2f(key_below + 14.0f - sh), mine_ds, ds_by + 2 * kw * kTile);
+                const float kap = parts.times((float)pass.eq - sh);
                 float by;
                 if (column_scale(halves_max(most) * __builtin_fabsf(kap), F, by)) scale_acc(dk, by);
                 const float kF = finite_product(kap, F);
@@ -354,13 +463,13 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
                               });
             }
             __syncthreads();
-            if (f.gq) gq_blocks<DP, W>(f, b, u, t, nt, keys, dss, dsx);
+            if (f.gq) gq_blocks<DP, W>(f, b, u, t, nt, keys, dss, ds_by, keys_by, pass.rows);
         }
         if (key < a.Lk) {
             const int64_t at = ((b * a.Lk + key) * a.Hkv + u) * D;
             const bool some = live && t0 < t1;
             if (f.gk) store_column<true>(f.gk + split * f.part_k + at, dk, some, 1.0f / F, half, D, f.acc_k);
-            if (f.gv) store_column<true>(f.gv + split * f.part_k + at, dv, some, __builtin_amdgcn_exp2f(E - 14.0f), half, D, f.acc_v);
+            if (f.gv) store_column<true>(f.gv + split * f.part_k + at, dv, some, unit_of(U), half, D, f.acc_v);
         }
     }
 }
@@ -376,9 +485,9 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     // q's tile, go's tile, the tiles of keys, p and then ds of each, then small tables
     char *const qs = smem, *const gs = smem + TB, *const keys = smem + 2 * TB, *const dss = keys + KT * TB;
-    float *const small = (float *)(dss + KT * kDsTile);
-    float *const stats = small, *const dots = small + 64, *const red = dots + (DP / 8) * 32;  // [64], [DP / 8][32], [2][W]
-    f2 *const dsx = (f2 *)(red + 2 * W);  // [KT]: the scales of the tiles' ds, and of their keys
+    FeedTables<DP, W> &tables = *(FeedTables<DP, W> *)(dss + KT * kDsTile);
+    float *const ds_by = (float *)(&tables + 1), *const keys_by = ds_by + 2 * KT * kTile;  // [KT][2][32], [KT]: the scales of the tiles' ds and of their keys
+    float *const shift = keys_by + KT, *const below = shift + KT * kWave;  // [KT][64]: p is handed over as 2^shift p; the keys' own exponents
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ra = row_at(lane), ca = col_at(lane), D = (int)a.D;
@@ -397,22 +506,23 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
         __syncthreads();  // the last unit's keys have been read
         // this wave's keys or values as row fragments: the values go through the place of the keys, which stay there
         h8 kh[KS], kl[KS];
-        int ek = 0;
+        int own = 0;  // this lane's key's or value's exponent
         if (mine && ds_wave) {
             float x[KS][8];
-            ek = tile_load<DP>(f.v + b * a.sv[0] + u * a.sv[2], a.sv[1], kw * kTile, n, D, x);
-            tile_split<DP>(x, ek, kt);
+            (void)tile_load<DP>(f.v + b * a.sv[0] + u * a.sv[2], a.sv[1], kw * kTile, n, D, x, own);
+            tile_split<DP>(x, own, kt);
 #pragma unroll
             for (int s = 0; s < KS; s++) kh[s] = row_frag(kt + ra, s), kl[s] = row_frag(kt + ra + LO, s);
         }
         __syncthreads();
         if (mine && !ds_wave) {
             float x[KS][8];
-            ek = tile_load<DP>(f.k + b * a.sk[0] + u * a.sk[2], a.sk[1], kw * kTile, n, D, x);
-            tile_split<DP>(x, ek, kt);
+            const int ek = exponent_of(tile_load<DP>(f.k + b * a.sk[0] + u * a.sk[2], a.sk[1], kw * kTile, n, D, x, own));
+            tile_split<DP>(x, own, kt);
 #pragma unroll
             for (int s = 0; s < KS; s++) kh[s] = row_frag(kt + ra, s), kl[s] = row_frag(kt + ra + LO, s);
-            if (lane == 0) dsx[kw].y = pow2i(ek) * a.scale;
+            if (lane == 0) keys_by[kw] = pow2i(ek) * a.scale;
+            below[kw * kWave + lane] = (float)(own - ek);
         }
         if (t0 < t1) next.fetch(f, b, u, t0);
         f16x acc[NT];
@@ -420,17 +530,15 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[t][r] = 0.0f;
-        float F = 0x1p100f, E = -1000.0f;
+        float F = 0x1p100f, U = live ? kNoUnit : -kNoUnit;
         const ScaleParts parts(a.scale);
-        const float ck = ds_wave ? pow2i(ek) : pow2i(ek) * a.scale * kLog2e;
-        for (int64_t t = t0; t < t1; t++) {
-            int eq, eg;
-            next.split(qs, gs, stats, dots, red, eq, eg);
-            if (t + 1 < t1) next.fetch(f, b, u, t + 1);
-            const f4 *const rows = (const f4 *)stats + half;
+        const float ck = ds_wave ? pow2i(own) : pow2i(own) * a.scale * kLog2e;
+        uint32_t todo = ~0u;  // rows of a tile that no pass had
+        for (int64_t t = t0, tn = t0; t < t1; t = tn) {
+            const FeedPass pass = next.pass(f, b, u, tn, t1, todo, qs, gs, tables);
+            const f4 *const rows = (const f4 *)tables.stats + half;
             f4 *const ph = (f4 *)hand + lane;  // p's registers 4 j .. 4 j + 3 at 64 j
-            // p as 2^14 p, less for tiles of smaller gradients (no less than 2^-60 times: below what gv can show)
-            const float ex = (float)eg, En = __builtin_fmaxf(E, ex), sh = 14.0f + __builtin_fmaxf(ex - En, -60.0f);
+            const float xg = (float)pass.eg;
             f16x s;
             if (mine) {
                 const char *rt = (ds_wave ? gs : qs) + ra;
@@ -439,22 +547,22 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
                 steps<KS>([&](int k) { return Pieces{row_frag(rt, k), row_frag(rt + LO, k)}; },
                           [&](int k, const Pieces &x) { s = mfma3(x.hi, x.lo, kh[k], kl[k], s); });
                 if (!ds_wave) {
-                    if (ex > E) scale_acc(acc, __builtin_amdgcn_exp2f(E - ex));
-                    const float c = ck * pow2i(eq), base = live ? sh : -INFINITY;
+                    const float c = ck * pow2i(pass.eq), off = live ? first_shift(xg, U) : -INFINITY;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const f4 ls = rows[2 * j];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[4 * j + e] = __builtin_amdgcn_exp2f(fma_(s[4 * j + e], c, base - ls[e]));
-                        ph[64 * j] = f4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
+                        for (int e = 0; e < 4; e++) s[4 * j + e] = __builtin_amdgcn_exp2f(fma_(s[4 * j + e], c, off - ls[e]));
                     }
+                    shift[kw * kWave + lane] = column_unit(s, xg, pass.hold, U, acc);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) ph[64 * j] = f4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
                 }
             }
-            E = En;
             lds_barrier();  // p is there
             if (mine) {
                 if (ds_wave) {
-                    const float c = ck * pow2i(eg), kap = parts.times((float)eq - sh);
+                    const float sh = shift[kw * kWave + lane], c = ck * pow2i(pass.eg), kap = parts.times((float)pass.eq - sh);
                     float most = 0.0f;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
@@ -466,8 +574,7 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
                             most = __builtin_fmaxf(most, __builtin_fabsf(s[r]));
                         }
                     }
-                    const int ed = put_ds(s, most, hand);  // where p was
-                    if (lane == 0) dsx[kw].x = __builtin_amdgcn_exp2f((float)ed - sh);
+                    put_ds(s, __builtin_amdgcn_exp2f(below[kw * kWave + lane] + 14.0f - sh), hand, ds_by + 2 * kw * kTile);  // where p was
                     float by;
                     if (column_scale(halves_max(most) * __builtin_fabsf(kap), F, by)) scale_acc(acc, by);
                     const float kF = finite_product(kap, F);
@@ -480,12 +587,12 @@ __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const
                               [&](int k, const Pieces &v) { acc[k % NT] = mfma3(v.hi, v.lo, y[k / NT].hi, y[k / NT].lo, acc[k % NT]); });
             }
             lds_barrier();
-            if (f.gq) gq_blocks<DP, W>(f, b, u, t, nt, keys, dss, dsx);
+            if (f.gq) gq_blocks<DP, W>(f, b, u, t, nt, keys, dss, ds_by, keys_by, pass.rows);
         }
         float *const out = ds_wave ? f.gk : f.gv;
         if (out && key < a.Lk)
             store_column<true>(out + split * f.part_k + ((b * a.Lk + key) * a.Hkv + u) * D, acc, live && t0 < t1,
-                               ds_wave ? 1.0f / F : __builtin_amdgcn_exp2f(E - 14.0f), half, D, ds_wave ? f.acc_k : f.acc_v);
+                               ds_wave ? 1.0f / F : unit_of(U), half, D, ds_wave ? f.acc_k : f.acc_v);
     }
 }
 
@@ -511,7 +618,8 @@ void short_fwd(const ShortFwd &f, int DP, hipStream_t st) {
 
 template <int DP, int W, int KT, class F>
 static void bwd_launch(F *kernel, const ShortBwd &f, hipStream_t st) {  // W waves, KT tiles of keys
-    const size_t lds = 2 * 128 * DP + (size_t)KT * (128 * DP + kDsTile) + (64 + DP / 8 * 32 + 2 * W + 2 * KT) * sizeof(float);
+    const size_t lds = 2 * 128 * DP + (size_t)KT * (128 * DP + kDsTile) + sizeof(FeedTables<DP, W>) +
+                       KT * (2 * kTile + 1 + (W > KT ? 2 * kWave : 0)) * sizeof(float);
     launch(kernel, f.units, W * kWave, lds, st, f);
 }
 

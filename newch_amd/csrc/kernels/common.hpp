@@ -199,7 +199,7 @@ __device__ __forceinline__ double lane63_f64(double v) {
 }
 // DPP steps: quad_perm [1,0,3,2], quad_perm [2,3,0,1], row_half_mirror, row_mirror, then
 // row_bcast:15 into rows 1 and 3 and row_bcast:31 into rows 2 and 3
-enum : int { kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140, kDppBcast15 = 0x142,
+enum : int { kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140, kDppRor8 = 0x128, kDppBcast15 = 0x142,
              kDppBcast31 = 0x143 };
 
 __device__ __forceinline__ double wave_sum(double v) {

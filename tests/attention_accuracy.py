@@ -8,9 +8,9 @@ the whole, is left out; roundings of sums and of exp2's argument are fp32's.  Ta
   a probability: that, exp2's argument at up to 16 (2^-21 ln 2 / sqrt(3) = 2e-7) and its sum's: 1e-6 relative;
   an output or a gradient: a probability's, the other factor's 2^-22 and its sum's: 1.2e-6 of its norm, less where many keys share it.
 WHOLE, of a tensor's norm, allows three times that; an operand that lost its low piece is off by 2^-11 / sqrt(12) = 1.4e-4.
-ROW is for every row by itself, of the norm of the magnitudes that it adds up: p |v|, p |go|, and p (|go . v| + |go . o| + the root of
-the sum of go . v's squared terms) |k| or |q| -- a row's gradient may cancel far below them (one key that takes nearly all), in
-any arithmetic.  It allows twice WHOLE: a row has no other rows to average with, and its scores go to ten units.
+ROW is for every row by itself, of the norm of the magnitudes that it adds up: p |v|, p |go|, and p (|go . v| + |go . o| + the roots of
+the sums of go . v's squared terms and of go . o's, with p |v| for o) |k| or |q| -- a row's gradient may cancel far below them
+(one key that takes nearly all; go . o of values that cancel), in any arithmetic.  It allows twice WHOLE: a row has no other rows to average with, and its scores go to ten units.
 """
 import numpy as np
 
@@ -55,8 +55,9 @@ def forward_backward(q, k, v, lens, scale, go, cut=None):
             out["gq"][b, :, h] = part("gq", "ds", ds) @ part("gq", "k", K)
             out["gk"][b, :n, u] += part("gk", "ds", ds).T @ part("gk", "q", Q)
             out["gv"][b, :n, u] += part("gv", "p", p).T @ part("gv", "go", G)
-            mds = p * (np.abs(dp) + np.abs(delta) + np.sqrt((G * G) @ (V * V).T)) * abs(float(np.float32(scale)))
-            mag["o"][b, :, h] = p @ np.abs(V)
+            mag["o"][b, :, h] = mo = p @ np.abs(V)
+            rough = np.sqrt((G * G) @ (V * V).T) + np.sqrt((G * G * mo * mo).sum(1, keepdims=True))
+            mds = p * (np.abs(dp) + np.abs(delta) + rough) * abs(float(np.float32(scale)))
             mag["gq"][b, :, h] = mds @ np.abs(K)
             mag["gk"][b, :n, u] += mds.T @ np.abs(Q)
             mag["gv"][b, :n, u] += p.T @ np.abs(G)
@@ -78,7 +79,7 @@ def check(got, want, what="", names=("o", "gq", "gk", "gv"), pick=None, skip=0, 
             r = np.linalg.norm(g - w) / np.linalg.norm(w)
             assert r <= WHOLE, f"{what} {name}: off by {r:.3g} of its norm, {WHOLE:.3g} allowed"
         err, top = np.linalg.norm(g - w, axis=-1), np.linalg.norm(m, axis=-1)
-        over = err > ROW * top
+        over = err > ROW * top + 2.0 ** -120  # what a float can hold at all
         if over.any():
             i = np.unravel_index(int(np.argmax(err - ROW * top)), err.shape)
             raise AssertionError(f"{what} {name}: {int(over.sum())} rows of {err.size} off; row {tuple(int(x) for x in i)} off by "
@@ -115,8 +116,8 @@ def up(a):
     return None if a is None else DeviceBuffer.from_numpy(np.asarray(a))
 
 
-def run(K, q, k, v, g, lens, scale, backward=True):
-    """Forward, and backward, on contiguous buffers; outputs begin as NaN."""
+def run(K, q, k, v, g, lens, scale, backward=True, old=None):
+    """Forward, and backward, on contiguous buffers; outputs begin as NaN, or, old, gradients as that and are added to."""
     B, Lq, Hq, D = q.shape
     Lk, Hkv = k.shape[1:3]
     sizes, sq, sk = (B, Lq, Lk, Hq, Hkv, D), (Lq * Hq * D, Hq * D, D), (Lk * Hkv * D, Hkv * D, D)
@@ -128,8 +129,10 @@ def run(K, q, k, v, g, lens, scale, backward=True):
     ws = DeviceBuffer.from_numpy(np.full(max(n1, n2, 16), 0xFF, np.uint8))
     K.cross_attention_fwd(*sizes, scale, *src, out["o"].ptr, out["lse"].ptr, ws.ptr, n1)
     if backward:
-        out.update(gq=new(*q.shape), gk=new(*k.shape), gv=new(*v.shape))
-        K.cross_attention_bwd(*sizes, scale, *src, out["o"].ptr, out["lse"].ptr, G.ptr, *(out["g" + c].ptr for c in "qkv"), ws.ptr, n2)
+        begin = new if old is None else lambda *shape: DeviceBuffer.from_numpy(np.full(shape, old, np.float32))
+        out.update(gq=begin(*q.shape), gk=begin(*k.shape), gv=begin(*v.shape))
+        K.cross_attention_bwd(*sizes, scale, *src, out["o"].ptr, out["lse"].ptr, G.ptr, *(out["g" + c].ptr for c in "qkv"), ws.ptr, n2,
+                              accumulate=old is not None)
     synchronize()
     like = {"o": q, "gq": q, "gk": k, "gv": v}
     return {i: t.to_numpy(np.float32, like[i].shape if i in like else (B, Hq, Lq)) for i, t in out.items()}

@@ -29,8 +29,7 @@ def test_random_inputs(K, shape):
     print("random", shape, flush=True)
     q, k, v, g, _ = A.random_inputs((*shape, None), 51)
     # a few queries' errors do not average: rows alone
-    A.check(A.run(K, q, k, v, g, None, shape[5] ** -0.5, backward=False), A.forward_backward(q, k, v, None, shape[5] ** -0.5, g), str(shape),
-            names=("o",), whole=shape[1] > 8)
+    A.check(A.run(K, q, k, v, g, None, shape[5] ** -0.5), A.forward_backward(q, k, v, None, shape[5] ** -0.5, g), str(shape), whole=shape[1] > 8)
 
 
 def members(n, where):
@@ -52,9 +51,9 @@ def test_far_larger_values_that_a_row_does_not_count(K, shape, where):
         big, far = v.copy(), g.copy()
         big[:, fk] *= np.float32(2.0 ** e)
         far[:, fq] *= np.float32(2.0 ** e)
-        got, want = A.run(K, q, k, big, far, None, scale, backward=False), A.forward_backward(q, k, big, None, scale, far)
-        A.check(got, want, f"2^{e} near", pick={"o": ~fq, "gq": ~fq, "gk": ~fk, "gv": ~fk}, skip=2, whole=False, names=("o",))
-        A.check(got, want, f"2^{e} far", pick={"o": fq, "gq": fq, "gk": fk, "gv": fk}, skip=2, whole=False, names=("o",))
+        got, want = A.run(K, q, k, big, far, None, scale), A.forward_backward(q, k, big, None, scale, far)
+        A.check(got, want, f"2^{e} near", pick={"o": ~fq, "gq": ~fq, "gk": ~fk, "gv": ~fk}, skip=2, whole=False)
+        A.check(got, want, f"2^{e} far", pick={"o": fq, "gq": fq, "gk": fk, "gv": fk}, skip=2, whole=False)
 
 
 @pytest.mark.parametrize("shape", [s for s in SHAPES if s[1] > 1], ids=str)
@@ -97,7 +96,42 @@ def test_far_larger_keys_or_queries(K, shape, where, which):
         q2, k2 = q.copy(), k.copy()
         q2[:, fq] *= np.float32(2.0 ** e)
         k2[:, fk] *= np.float32(2.0 ** e)
-        got, want = A.run(K, q2, k2, v, g, None, scale, backward=False), A.forward_backward(q2, k2, v, None, scale, g)
-        A.check(got, want, f"{which} 2^{e}", pick={"o": ~fq, "gq": ~fq, "gk": ~fk, "gv": ~fk}, skip=1, whole=False, names=("o",))
+        got, want = A.run(K, q2, k2, v, g, None, scale), A.forward_backward(q2, k2, v, None, scale, g)
+        A.check(got, want, f"{which} 2^{e}", pick={"o": ~fq, "gq": ~fq, "gk": ~fk, "gv": ~fk}, skip=1, whole=False)
         lse = np.abs(got["lse"] - want["lse"])[:, :, ~fq]
         assert lse.max() <= 2.0 ** -17 * max(1.0, np.abs(want["lse"][:, :, ~fq]).max()), lse.max()
+
+
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[1] > 1], ids=str)
+def test_rows_of_every_magnitude(K, shape):
+    """Values, output gradients and keys from 2^-20 to 2^20 of each other row by row, stored and added: each row keeps its bits."""
+    B, Lq, Lk, Hq, Hkv, D = shape
+    q, k, v, g, _ = A.random_inputs((*shape, None), 61)
+    rng = np.random.default_rng(62)
+    v *= np.exp2(rng.integers(-20, 21, v.shape[:3])).astype(np.float32)[..., None]
+    g *= np.exp2(rng.integers(-20, 21, g.shape[:3])).astype(np.float32)[..., None]
+    q *= np.exp2(rng.integers(-20, 1, q.shape[:3])).astype(np.float32)[..., None]
+    k *= np.exp2(rng.integers(-20, 1, k.shape[:3])).astype(np.float32)[..., None]
+    print("magnitudes", shape, flush=True)
+    want = A.forward_backward(q, k, v, None, D ** -0.5, g)
+    got = A.run(K, q, k, v, g, None, D ** -0.5)
+    A.check(got, want, str(shape), whole=False)
+    added = A.run(K, q, k, v, g, None, D ** -0.5, old=0.0)
+    for i in ("gq", "gk", "gv"):
+        assert (added[i] == got[i]).all(), i
+
+
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[1] > 1], ids=str)
+def test_keys_that_are_hardly_counted(K, shape):
+    """Keys whose probabilities are 2^-20 to 2^-60 in every row: their gradients are small, not rough.  Their scores are 42 units below
+    the others' at most, whose roundings are 42 / 2.3 times the size."""
+    B, Lq, Lk, Hq, Hkv, D = shape
+    q, k, v, g, _ = A.random_inputs((*shape, None), 63)
+    e = np.where(np.arange(Lk) % 3 == 1, np.linspace(20, 60, Lk), 0.0)
+    a = np.float32(np.sqrt(np.log(2.0) * np.sqrt(D)))
+    q[..., 0], k[..., 0] = a, (-e * a)[None, :, None]
+    print("hardly", shape, flush=True)
+    got, want = A.run(K, q, k, v, g, None, D ** -0.5), A.forward_backward(q, k, v, None, D ** -0.5, g)
+    for i in ("gk", "gv"):
+        err, top = (np.linalg.norm(t[..., 1:], axis=-1) for t in (got[i] - want[i], want["mag"][i]))
+        assert (err <= 18 * A.ROW * top).all(), (i, (err / top).max())

@@ -51,6 +51,34 @@ def test_a_value_that_is_not_finite_gives_nan_where_it_counts(K, shape, operand,
     assert (np.linalg.norm(err, axis=-1) <= A.ROW * np.linalg.norm(want["mag"]["o"], axis=-1)).all()
 
 
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan], ids=str)
+@pytest.mark.parametrize("operand", ["q", "k", "v"])
+@pytest.mark.parametrize("shape", FINITE_SHAPES, ids=str)
+def test_gradients_that_meet_a_value_that_is_not_finite(K, shape, operand, value):
+    """In a query: its own gradient and those of its head's keys and values.  In a key or a value: the gradients of all that share the
+    head.  Other heads' are as they are."""
+    B, Lq, Lk, Hq, Hkv, D = shape
+    q, k, v, g, _ = A.random_inputs((*shape, None), 60)
+    want = A.forward_backward(q, k, v, None, D ** -0.5, g)
+    rows = np.zeros((1, Lq, Hq), bool)
+    if operand == "q":
+        q[0, Lq // 2, 0, 1] = value
+        rows[0, Lq // 2, 0] = True
+    else:
+        (k if operand == "k" else v)[0, Lk // 3, 0, 1] = value
+        rows[0, :, : Hq // Hkv] = True
+    print("gradients", shape, operand, value, flush=True)
+    got = A.run(K, q, k, v, g, None, D ** -0.5)
+    assert np.isnan(got["gq"][rows]).all()
+    assert np.isnan(got["gk"][:, :, 0]).all()
+    if operand != "v":
+        assert np.isnan(got["gv"][:, :, 0]).all()
+    for i, rest in (("gq", ~rows), ("gk", np.arange(Hkv) > 0), ("gv", np.arange(Hkv) > 0)):
+        pick = rest if i == "gq" else np.broadcast_to(rest, (1, Lk, Hkv))
+        err, top = (np.linalg.norm(t[pick], axis=-1) for t in (got[i] - want[i], want["mag"][i]))
+        assert (err <= A.ROW * top).all(), i
+
+
 @pytest.mark.parametrize("shape", FINITE_SHAPES, ids=str)
 def test_scores_that_are_all_infinite_are_not_no_keys(K, shape):
     """A query of +inf in a column where every key is negative: every score is -inf, and the row is NaN, not the zeros of no keys."""
