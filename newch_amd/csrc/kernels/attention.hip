@@ -565,6 +565,8 @@ template <int DP, int OCC>
 __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * TB + 256;
     constexpr bool REG = DP <= 128;  // keys or values stay in registers, else they are read again for every tile
+    // the last products' first fragments are read before p is there, but where that spills (2048 x 2048, 16 heads of 64: 542 us, and 570)
+    constexpr bool EARLY = OCC == 2 && DP <= 128;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const AttnArgs &a = f.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -645,8 +647,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
             const char *ct = st + (ds_wave ? 0 : TB) + ca;
             const auto turned = [&](int k) { return Pieces{col_frag(ct, k / NT, k % NT), col_frag(ct + LO, k / NT, k % NT)}; };
             Pieces x[3];
-            x[0] = turned(0);
-            x[1] = turned(1);
+            if constexpr (EARLY) x[0] = turned(0), x[1] = turned(1);
             lds_barrier();  // p is there (the next stage's copies stay on their way)
             if (!mine) continue;
             if (ds_wave) {
@@ -673,6 +674,7 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
                 for (int r = 0; r < 16; r++) s[r] *= kF;
             }
             const Split8 y[2] = {split_regs(s, 0), split_regs(s, 8)};
+            if constexpr (!EARLY) x[0] = turned(0), x[1] = turned(1);
             steps<2 * NT>(x, turned, [&](int k, const Pieces &v) { acc[k % NT] = mfma3(v.hi, v.lo, y[k / NT].hi, y[k / NT].lo, acc[k % NT]); });
         }
         float *const out = ds_wave ? f.gk : f.gv;
@@ -749,8 +751,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
                           });
             const auto turned = [&](int k) { return Pieces{col_frag(kc, k / NT, k % NT), col_frag(kc + LO, k / NT, k % NT)}; };
             Pieces x[3];
-            x[0] = turned(0);
-            x[1] = turned(1);
+            if constexpr (DP <= 128) x[0] = turned(0), x[1] = turned(1);  // wider: 1024 x 1024, 8 heads of 256 152 us, and 190 with the spills
             const float *kr = f.kr + (k0 + t) * kTile;
             if (own_rows(max(ek, ev))) {
                 if (own_rows(ek)) scale_rows(s, kr);
@@ -778,6 +779,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
 #pragma unroll
             for (int r = 0; r < 16; r++) dp[r] *= kF;
             const Split8 y[2] = {split_regs(dp, 0), split_regs(dp, 8)};
+            if constexpr (DP > 128) x[0] = turned(0), x[1] = turned(1);
             steps<2 * NT>(x, turned, [&](int k, const Pieces &v) { dq[k % NT] = mfma3(v.hi, v.lo, y[k / NT].hi, y[k / NT].lo, dq[k % NT]); });
         }
         float by = 1.0f / F;
