@@ -70,6 +70,7 @@ struct nc_tensor {
     size_t bytes;     // storage bytes
     uint32_t res;     // RES_DEV | RES_HOST: which copies are current
     uint64_t wgen;    // write generation: bumped by every device write and every host pointer handed out for writing
+    uint64_t hgen;    // of those, the host pointers handed out to the caller (nc_data_f32, nc_data_i32), who may only have read
     nc_tensor *grad;  // contiguous, same logical shape
     nc_node *node;
     nc_tensor *owner;  // views: the storage owner

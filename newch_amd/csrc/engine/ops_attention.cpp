@@ -37,18 +37,16 @@ static const int32_t *contig_i32(nc_tensor *t) {
     return (const int32_t *)c;
 }
 
-// counts every write to the storage of the inputs from `first` on, and of the output where the backward reads it: the same number
-// means that none was written
-static int64_t generations(const nc_node *n, int first = 0, bool output = false) {
-    uint64_t g = output ? owner_of(n->out)->wgen : 0;
+// counts every write to the storage of the inputs from `first` on: the same number means that none was written
+static int64_t generations(const nc_node *n, int first = 0) {
+    uint64_t g = 0;
     for (int i = first; i < n->n_in; i++) g += owner_of(n->in[i])->wgen;
     return (int64_t)g;
 }
 
-static bool unwritten(const nc_node *n, int64_t then, int first = 0, bool output = false) {
-    if (generations(n, first, output) == then) return true;
-    error(n->in[0]->ctx, NC_ERR_STATE, "%s: an input%s was written after the forward (the backward reads it again)",
-          n->op->name, output ? " or the output" : "");
+static bool unwritten(const nc_node *n, int64_t then, int first = 0) {
+    if (generations(n, first) == then) return true;
+    error(n->in[0]->ctx, NC_ERR_STATE, "%s: an input was written after the forward (the backward reads it again)", n->op->name);
     return false;
 }
 
@@ -252,20 +250,48 @@ static nc_status attn_fwd(nc_node *n) {
                       n->op->name))
         return NC_ERR_STATE;
     wrote_dev(n->out);
-    n->p.i[0] = generations(n, 0, true);
+    const nc_tensor *out = owner_of(n->out);
+    n->p.i[0] = generations(n);
+    n->p.i[1] = (int64_t)out->wgen, n->p.i[2] = (int64_t)out->hgen;
     return NC_OK;
+}
+
+// The output as the forward left it: its own storage, or, where the caller had a host pointer to it since (and may have written
+// through that), the forward once more into scratch.  An output that a call wrote is refused.
+static const float *output_of(const nc_node *n, const AttnCall &c, const Heads &q, const Heads &k, const Heads &v, const int32_t *len) {
+    nc_ctx *ctx = c.q->ctx;
+    const nc_tensor *out = owner_of(n->out);
+    const uint64_t writes = out->wgen - (uint64_t)n->p.i[1], pointers = out->hgen - (uint64_t)n->p.i[2];
+    if (writes == 0) return fptr(n->out);
+    if (writes != pointers) {
+        error(ctx, NC_ERR_STATE, "%s: the output was written after the forward (the backward reads it again)", n->op->name);
+        return nullptr;
+    }
+    const size_t bytes = (size_t)nc_numel(n->out) * sizeof(float), ws_bytes = nc_hip_cross_attention_fwd_workspace(c.B, c.Lq, c.Lk, c.Hq, c.Hkv, c.D);
+    float *o = (float *)arena_alloc(ctx, bytes ? bytes : 1);
+    char *ws = ws_bytes ? arena_alloc(ctx, ws_bytes) : nullptr;
+    if (!o || (ws_bytes && !ws)) return nullptr;
+    return hip_layer_ok(ctx,
+                        nc_hip_cross_attention_fwd(c.B, c.Lq, c.Lk, c.Hq, c.Hkv, c.D, n->p.f[0], q.p, q.s, k.p, k.s, v.p, v.s, len, o, nullptr,
+                                                   ws, ws_bytes, stream(ctx)),
+                        n->op->name)
+               ? o
+               : nullptr;
 }
 
 static void attn_bwd(nc_node *n) {
     const AttnCall c(n);
     nc_ctx *ctx = c.q->ctx;
-    if (!unwritten(n, n->p.i[0], 0, true)) return;
+    if (!unwritten(n, n->p.i[0])) return;
     Heads q, k, v;
-    const float *o = fptr(n->out), *go = fptr(n->out->grad);
-    if (!o || !go || !heads_of(c.q, q) || !heads_of(c.k, k) || !heads_of(c.v, v)) return;
+    const float *go = fptr(n->out->grad);
+    if (!go || !heads_of(c.q, q) || !heads_of(c.k, k) || !heads_of(c.v, v)) return;
     const int32_t *len = c.len ? contig_i32(c.len) : nullptr;
+    if (c.len && !len) return;
+    const float *o = output_of(n, c, q, k, v, len);
+    if (!o) return;
     const bool want_q = needs_grad(c.q), want_k = needs_grad(c.k), want_v = needs_grad(c.v);
-    if ((c.len && !len) || (want_q && !grad_buf(c.q)) || (want_k && !grad_buf(c.k)) || (want_v && !grad_buf(c.v))) return;
+    if ((want_q && !grad_buf(c.q)) || (want_k && !grad_buf(c.k)) || (want_v && !grad_buf(c.v))) return;
     // One tensor as several of the three has one gradient, and the kernels' must not overlap: its later parts go through scratch.
     nc_tensor *const in[3] = {c.q, c.k, c.v};
     const bool want[3] = {want_q, want_k, want_v};

@@ -478,11 +478,13 @@ int nc_is_contiguous(const nc_tensor *t) {
 
 float *nc_data_f32(nc_tensor *t) {
     if (!t || t->dtype != NC_F32 || !nc_is_contiguous(t)) return nullptr;
+    owner_of(t)->hgen++;
     return (float *)hptr(t, true);
 }
 
 int32_t *nc_data_i32(nc_tensor *t) {
     if (!t || t->dtype != NC_I32 || !nc_is_contiguous(t)) return nullptr;
+    owner_of(t)->hgen++;
     return (int32_t *)hptr(t, true);
 }
 

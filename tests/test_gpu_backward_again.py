@@ -1,4 +1,6 @@
-"""A backward that fails for memory between taking a gradient and writing it leaves nothing behind: after nc_clear_error the next one
+"""Backwards after something went between: a failure, a look at an output.
+
+A backward that fails for memory between taking a gradient and writing it leaves nothing behind: after nc_clear_error the next one
 stores where nothing was written, and gives what it gives without the failure."""
 import ctypes
 from ctypes import c_float, c_int64
@@ -87,3 +89,31 @@ def test_the_next_backward_stores_what_the_failed_one_did_not(monkeypatch, op, h
             assert (e.grad(t).view(np.uint32) == w.view(np.uint32)).all()
         e.close()
     assert failures
+
+
+@pytest.mark.parametrize("Lk", [40, 300])
+@pytest.mark.parametrize("write", [False, True])
+def test_an_output_that_the_host_looked_at(write, Lk):
+    """nc_data_f32 on attention's output, or on a view of it, between the forward and the backward, to read it or to write: the
+    backward is the one of the forward that ran."""
+    with Engine(lib=abi.load(abi.LIB_PATH)) as e:
+        L, rng = e.lib, np.random.default_rng(6)
+        q, k, v = (e.param(rng.standard_normal((2, n, 2, 64))) for n in (50, Lk, Lk))
+        g = rng.standard_normal((2, 50, 2, 64)).astype(np.float32)
+        grads = []
+        for look in (False, True):
+            for t in (q, k, v):
+                L.nc_zero_grad(t)
+            o = L.nc_cross_attention(q, k, v, e.tensor(np.array([Lk, 7], np.int32)), c_float(0.125))
+            e.check()
+            if look:
+                was = e.read(o)
+                p = ctypes.cast(L.nc_data_f32(L.nc_slice(o, 1, 0, 50, 1) if Lk == 300 else o), ctypes.POINTER(c_float))
+                assert p and p[5] == was.reshape(-1)[5]
+                if write:
+                    p[5] = 1e9
+            e.backward_with(o, g)
+            grads.append([e.grad(t) for t in (q, k, v)])
+        for a, b in zip(*grads):
+            assert (a.view(np.uint32) == b.view(np.uint32)).all()
+        e.step_end()
