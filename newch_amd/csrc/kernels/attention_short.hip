@@ -120,9 +120,9 @@ template <int DP, int W>
 struct FeedTables {  // in LDS
     float stats[64];                // the rows' log2-sum-exps (infinite: not in this pass) and go . o
     float dots[DP / 8][kTile];      // scratch
+    float tops[2][DP / 8][kTile];   // the largest of the pieces of queries, of gradients
     float red[2][W];
-    uint32_t masks[W][4];
-    uint32_t loose_rows, unused[3];
+    int several[4];                 // a row is loose, rows are unlike
 };
 struct FeedPass {
     int eq, eg;       // exponents of the tile's queries and gradients
@@ -180,7 +180,7 @@ struct Feed {
         float dot = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) dot = fma_(go[e], o[e], dot);
-        if (p < UNITS) t.dots[p >> 5][p & 31] = dot;
+        if (p < UNITS) t.dots[p >> 5][p & 31] = dot, t.tops[0][p >> 5][p & 31] = mq, t.tops[1][p >> 5][p & 31] = mg;
         float tq = wave_max_nan_skip(mq), tg = wave_max_nan_skip(mg);
         if (lane == 0) t.red[0][wave] = tq, t.red[1][wave] = tg;
         __syncthreads();
@@ -188,32 +188,32 @@ struct Feed {
 #pragma unroll
         for (int x = 1; x < W; x++) tq = __builtin_fmaxf(tq, t.red[0][x]), tg = __builtin_fmaxf(tg, t.red[1][x]);
         const int eq = tile_exponent(tq), eg = tile_exponent(tg);
-        // rows that hold something, and rows that hold something of 2^-6 of the tile's largest and up
-        const auto rows_of = [](bool v) {
-            const uint64_t m = __ballot(v);
-            return (uint32_t)m | (uint32_t)(m >> 32);
-        };
-        const uint32_t some_q = rows_of(mq > 0.0f), large_q = rows_of(mq >= tq * 0x1p-6f);
-        const uint32_t some_g = rows_of(mg > 0.0f), large_g = rows_of(mg >= tg * 0x1p-6f), loose_rows = rows_of(loose(lse));
-        if (lane == 0) t.masks[wave][0] = some_q, t.masks[wave][1] = large_q, t.masks[wave][2] = some_g, t.masks[wave][3] = large_g;
-        if (p == 0) t.loose_rows = loose_rows;  // the first wave has all rows' log-sum-exps
+        // the first wave sums the rows' pieces of go . o, the second takes the rows' largest: queries' in the one half, gradients' in the other
+        float row[DP / 8];
+        if (wave < 2) {
+            const float *const from = (wave == 0 ? t.dots[0] : t.tops[lane >> 5][0]) + (lane & 31);
+#pragma unroll
+            for (int c = 0; c < DP / 8; c++) row[c] = from[c * kTile];
+        }
         put(q, eq, true, qs);
         put(go, eg, true, gs);
-        if (p < kTile) {
-            float d = t.dots[0][p];
+        if (wave == 0) {
+            float d = row[0];
 #pragma unroll
-            for (int c = 1; c < DP / 8; c++) d += t.dots[c][p];
-            t.stats[p] = lse;
-            t.stats[32 + p] = d;
+            for (int c = 1; c < DP / 8; c++) d += row[c];
+            if (lane < kTile) t.stats[lane] = lse, t.stats[32 + lane] = d;
+            const bool some = __any(loose(lse));
+            if (lane == 0) t.several[0] = some;
+        } else if (wave == 1) {
+            float most = row[0];
+#pragma unroll
+            for (int c = 1; c < DP / 8; c++) most = __builtin_fmaxf(most, row[c]);
+            const bool some = rows_unlike(most, lane < kTile ? tq : tg);
+            if (lane == 0) t.several[1] = some;
         }
         __syncthreads();
-        uint32_t m[4] = {};
-#pragma unroll
-        for (int w = 0; w < W; w++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) m[x] |= t.masks[w][x];
-        const uint32_t unlike = __builtin_amdgcn_readfirstlane((m[0] & ~m[1]) | (m[2] & ~m[3]) | t.loose_rows);
-        return {eq, eg, unlike ? 0u : ~0u, true, false};
+        const int several = __builtin_amdgcn_readfirstlane(t.several[0] | t.several[1]);
+        return {eq, eg, several ? 0u : ~0u, true, false};
     }
 
     // the same for those rows of `todo` that are like the one of the largest queries, and among them like the one of the largest gradients
