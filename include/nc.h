@@ -271,7 +271,8 @@ NC_API nc_tensor *nc_qk_norm_rope(nc_tensor *x, int64_t q_heads, nc_tensor *q_we
                                   int interleaved);
 /* softmax(scale q k^T) v of q [B, Lq, Hq, D] over k and v [B, Lk, Hkv, D], Hq a multiple of Hkv (heads of keys are shared), D <=
  * 256, no causal mask.  key_lengths i32 [B] or NULL: how many of each sequence's keys count; a sequence without keys
- * gives zeros and no gradient.  One tensor may be several of the three.  The backwards of these three read their inputs again
+ * gives zeros and no gradient.  A value that counts and is not finite makes the results that meet it NaN.  Operands are held in 22 bits,
+ * but for the forward of at most 8 rows a head of keys, and summed in fp32 (nc_hip_cross_attention_fwd says more).  One tensor may be several of the three.  The backwards of these three read their inputs again
  * (attention: its output too) and fail with NC_ERR_STATE where the storage of one was written since the forward; taking a pointer
  * for writing to an input (nc_data_f32) counts as a write, to attention's output it does not. */
 NC_API nc_tensor *nc_cross_attention(nc_tensor *q, nc_tensor *k, nc_tensor *v, nc_tensor *key_lengths, float scale);

@@ -24,7 +24,7 @@
 namespace nchip {
 
 // ------------------------------------------------------------------------------------------------
-// packing: a workgroup a tile of 32 rows; bound by memory (8192 keys and values of 16 heads of 128, 134 MB each way: 57 us, 4.7 TB/s)
+// packing: a workgroup a tile of 32 rows; bound by memory (8192 keys and values of 16 heads of 128, 134 MB each way: 58 us, 4.6 TB/s)
 // ------------------------------------------------------------------------------------------------
 // Rows of a (sequence, head of keys) pair: queries' row R is token R / G of query head u G + R % G, keys' are tokens.
 struct PackJob {
@@ -165,7 +165,8 @@ struct FwdArgs {
 // A workgroup's waves hold 32 rows of queries each, so that a stage of TPS tiles of keys and values comes from L2 once for 128
 // rows, the next one on its way meanwhile.  Two waves a SIMD (what the registers allow) run one's exponentials beside the other's
 // products: from two workgroups, or from KG = 2 groups of waves of one, which take every other stage (key_groups below).  8192 x
-// 8192, 16 heads of 128: 1.50 ms, 1.10 PFLOP/s of fp16 products.
+// 8192, 16 heads of 128: 1.45 to 1.54 ms from card to card, 1.07 to 1.14 PFLOP/s of fp16 products.  Heads of up to 128 columns hold
+// everything in registers; those of 129 to 256 spill 78.
 template <int DP, int TPS, int OCC, int KG>
 __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
     constexpr int TB = 128 * DP, TS = KG * TPS, STAGE = 2 * TS * TB;  // bytes of a packed tile; tiles and bytes of a stage
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_fwd(const FwdArgs f) {
 // (the query heads that share the keys); each group of LPK lanes keeps its own running maximum, sum and o over the keys that it
 // sees, U of them in flight, and the groups, waves and parts are joined at the end.  All in fp32 on the vector unit: 8 rows of
 // 128 columns still take less time than the keys' way from memory.  1500 keys, 8 x 12 heads of 64: 16 us (4.5 TB/s) and 4 for the
-// join; up to 16384 keys, 16 x 8 heads of 128, four rows: 215 to 230 us (5.0 to 5.3 TB/s).
+// join; up to 16384 keys, 16 x 8 heads of 128, four rows: 203 to 206 us (5.5 TB/s).
 template <int LPK>
 __device__ __forceinline__ float lanes_sum(float v) {  // over LPK neighbours
     v += dpp_f32<kDppXor1>(v, 0.0f);
@@ -558,8 +559,9 @@ struct BwdArgs {
 // gk and gv: two waves share 32 keys as columns and go over the tiles of queries.  One takes s = q k^T and p, whose rows are queries,
 // hands p over through LDS and sums gv^T += go^T p; the other takes dp = go v^T, makes ds of it and sums gk^T += q^T ds.  Each keeps
 // half of the fragments and of the sums, so that two waves fit a SIMD: one's exponentials run under the other's products (128
-// columns, 2 x 16 heads on 4, 2048 x 4096: 0.77 ms, and 0.90 with one wave that does both; 0.72 ms with the fragments read ahead,
-// 1.15 PFLOP/s).  Padded rows of queries have an infinite log-sum-exp: p = 0.  gv's unit follows p times the gradients' size, as o's
+// columns, 2 x 16 heads on 4, 2048 x 4096: 0.77 ms, and 0.90 with one wave that does both, before the fragments were read ahead; since
+// then 0.72 to 0.77 ms from card to card, 1.07 to 1.15 PFLOP/s).  Heads of 33 to 64 columns, four waves a SIMD, spill 37 registers, of
+// up to 32 two, of 129 to 256 17.  Padded rows of queries have an infinite log-sum-exp: p = 0.  gv's unit follows p times the gradients' size, as o's
 // does in the forward.
 template <int DP, int OCC>
 __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
@@ -685,8 +687,8 @@ __global__ __launch_bounds__(2 * kAttnB, OCC) void k_attn_dkv(const BwdArgs f) {
 }
 
 // gq: a wave holds 32 rows of queries as columns, as the forward does, and goes over the tiles of keys: s^T = k q^T and
-// dp^T = v go^T, then gq^T += k^T ds^T.  The same sizes: 0.61 ms, 1.02 PFLOP/s (the queries' and gradients' fragments fill the
-// registers, so fewer reads are ahead).
+// dp^T = v go^T, then gq^T += k^T ds^T.  The same sizes: 0.61 to 0.64 ms, 0.97 to 1.02 PFLOP/s (the queries' and gradients' fragments
+// fill the registers: heads of 97 to 128 columns spill 34, of 129 to 256 113, so fewer reads are ahead than in k_attn_dkv).
 template <int DP, int OCC, int KG>
 __global__ __launch_bounds__(KG *kAttnB, OCC) void k_attn_dq(const BwdArgs f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, STAGE = 2 * KG * TB;
@@ -871,7 +873,8 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
     } while (0)
 
 // Parts so that there are `want` workgroups, 64 parts at most, of at least four tiles each, or sixteen where the whole ones already
-// fill half the CUs: joining costs more than it gains there (1001 x 333, 3 x 8 heads of 80, forward: 36 us in two parts, 25 whole).
+// fill half the CUs: joining costs as much as it gains there, or more (1024 rows, 16 heads of 128, forward, whole and in two parts:
+// against 300 keys 33 and 41 us, 600 keys 46 both, 1000 keys 55 both; 1000 x 400, 4 x 6 heads of 256 77 and 110).
 static int attn_splits(int64_t whole, int64_t tiles, int64_t want) {
     int64_t s = whole ? want / whole : 1;
     s = std::min(s, tiles / (whole >= kPlanCUs / 2 ? 16 : 4));
@@ -879,11 +882,14 @@ static int attn_splits(int64_t whole, int64_t tiles, int64_t want) {
 }
 
 // Two groups of waves that share a workgroup's rows and take every other tile of keys, joined through LDS: where workgroups of four
-// waves would leave most SIMDs with one wave or none.  (1024 x 1024, 32 heads of 128: forward 75 us, and 96 with one group, forward
-// and backward 307 and 343; 8 heads of 64: 90 and 97.)
+// waves would leave most SIMDs with one wave or none.  (1024 x 1024, 32 heads of 128: forward 78 us, and 90 with one group, forward
+// and backward 300 and 335; 8 heads of 64: 95 and 99.)
 static bool key_groups(int64_t whole, int64_t tiles, int DP) { return DP <= 128 && whole <= kPlanCUs && tiles >= 4; }
 
-constexpr int64_t kTokenRows = 8;  // rows of a pair that k_attn_token takes
+// Rows of a pair that k_attn_token takes; more go through the pack, which costs the keys' bytes twice more.  8 x 8 heads of keys of 128
+// columns, four rows, eight, and 9 to 32: 4096 keys 61, 78 and 169 us, 16384 keys 204, 220 and 652 (four and eight rows packed: 169
+// and 647).
+constexpr int64_t kTokenRows = 8;
 
 struct FwdPlan {
     bool token, few;  // k_attn_token; few keys

@@ -44,8 +44,8 @@ __device__ __forceinline__ void tile_split(float (&x)[DP / 16][8], int ex, char 
 }
 
 // Forward: keys and values of a pair stay in LDS, and each wave goes over tiles of queries by itself.  4096 x at most 77, 4 x 16
-// heads of 64: 42 to 44 us for 136 MB (3.2 TB/s) -- a wave reads its rows, multiplies and stores in turn, and the three
-// waves of a SIMD do not cover all of it.
+// heads of 64: 38 to 43 us for 136 MB (3.2 to 3.6 TB/s) -- a wave reads its rows, multiplies and stores in turn, and the three
+// waves of a SIMD do not cover all of it.  Heads of 97 to 128 columns spill seven registers.
 template <int DP, int W, int OCC>
 __global__ __launch_bounds__(W *kWave, OCC) void k_attn_short_fwd(const ShortFwd f) {
     constexpr int TB = 128 * DP;
@@ -358,8 +358,9 @@ __device__ __forceinline__ void gq_blocks(const ShortBwd &f, int64_t b, int64_t 
 
 // Backward in one pass over the queries: every wave holds 32 keys, the workgroup splits a tile of queries and output gradients
 // (the next one's on their way meanwhile), and each wave takes its part of gk and gv as k_attn_dkv does.  It leaves its ds in LDS,
-// and the waves share the blocks of gq^T = k^T ds^T over all keys.  The same sizes: 97 to 104 us, and 120 to 125 with every
-// wave's part of gq added in LDS; memory would take 57.  A tile's steps follow each other (read, split, scores, gradients, store), two
+// and the waves share the blocks of gq^T = k^T ds^T over all keys.  The same sizes: 105 to 108 us, of which the look
+// at the rows, the units of gv's columns and the scales of ds's rows are 8, and 23 more with every wave's part of gq added in LDS; memory
+// would take 57.  A tile's steps follow each other (read, split, scores, gradients, store), two
 // workgroups a CU, by the registers, which hold heads of 64 columns and no more.
 template <int DP, int W>
 __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f) {
@@ -477,8 +478,8 @@ __global__ __launch_bounds__(W *kWave, 2) void k_attn_short_bwd(const ShortBwd f
 // Backward in one pass over the queries: two waves share 32 keys, and the workgroup splits a tile of queries and output gradients
 // (the next one's on their way meanwhile).  As in k_attn_dkv one wave takes the scores, p and gv, the other makes ds of p and takes
 // gk; it leaves ds in LDS, and all waves share the blocks of gq^T = k^T ds^T over all keys.  Half the registers for each wave's
-// keys: heads of up to 128 columns, a workgroup a CU.  4096 x 77, 4 x 16 heads, forward and backward: of 128 columns 320 us, and 487
-// through packed tiles and k_attn_dkv, k_attn_dq; of 80, 258 and 319; of 64, 204 where the kernel above takes 150.
+// keys: heads of up to 128 columns, a workgroup a CU.  4096 x 77, 4 x 16 heads, forward and backward: of 128 columns 332 us (39
+// registers spill), and 491 through packed tiles and k_attn_dkv, k_attn_dq; of 80, 268 and 326; of 64, 216 where the kernel above takes 161.
 template <int DP, int KT>
 __global__ __launch_bounds__(2 * KT *kWave, 2) void k_attn_short_bwd_pairs(const ShortBwd f) {
     constexpr int KS = DP / 16, NT = DP / 32, TB = 128 * DP, LO = 64 * DP, W = 2 * KT;
@@ -609,7 +610,7 @@ void short_fwd(const ShortFwd &f, int DP, hipStream_t st) {
     const size_t lds = (size_t)f.tiles * 2 * (tile_bytes(DP) + (kTile + 1) * sizeof(float));
     if (DP == 32) launch(&k_attn_short_fwd<32, 8, 4>, f.units, 512, lds, st, f);
     // three workgroups of four waves a CU where their keys fit its LDS, else eight waves over one copy (heads of 64, both ways: 4096
-    // x 77, 4 x 16 heads 147 us with four and 153 with eight, 64 x 64, 64 x 8 35 and 39; 197 x 197, 8 x 12 heads 60 and 58)
+    // x 77, 4 x 16 heads 161 us with four and 165 with eight, 64 x 64, 64 x 8 38 and 42; 197 x 197, 8 x 12 heads 65 and 63)
     else if (DP == 64 && 3 * lds <= 160 * 1024) launch(&k_attn_short_fwd<64, 4, 3>, f.units, 256, lds, st, f);
     else if (DP == 64) launch(&k_attn_short_fwd<64, 8, 2>, f.units, 512, lds, st, f);
     else if (DP == 96) launch(&k_attn_short_fwd<96, 8, 2>, f.units, 512, lds, st, f);
