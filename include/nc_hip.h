@@ -334,8 +334,8 @@ NC_HIP_API int nc_hip_qk_norm_rope_bwd(int64_t B, int64_t L, int64_t H, int64_t 
  * results that meet it NaN, be its probability zero.  A finite score below a float's range counts nothing; a row of such scores alone is
  * NaN.
  * Precision: the forward of at most 8 rows (Hq / Hkv * Lq) is plain fp32.  All else holds q, k, v and go in two fp16 pieces, 22 bits, under
- * a power of two of the row (32 rows share one where their largest values are within 2^6): a value below 2^-17 of what it is scaled by
- * is held to 2^-34 of its row's largest.  Products are summed in fp32.  Errors are up to 1.5 times a plain fp32 attention's.  Rows, values
+ * a power of two of the row (32 rows share one where their largest values are within 2^12): a value below 2^-17 of what it is scaled by
+ * is held to 2^-28 of its row's largest.  Products are summed in fp32.  Errors are up to 1.5 times a plain fp32 attention's.  Rows, values
  * and gradients far larger than the ones that a result counts cost it nothing, within 2^100 of each other in a tile of 32 rows and values
  * of 2^-100 to 2^100.  Outputs do not overlap inputs; the workspace is 16-byte aligned; calls that may overlap need workspaces
  * of their own.  No counterpart in the reference (its attention is bmm, masked_fill, softmax and bmm). */

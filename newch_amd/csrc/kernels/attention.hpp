@@ -4,7 +4,7 @@
 // unlike (kOwnRows), each row by one of its own; and every value is cut into x = hi + lo, fp16 each (rounded to nearest: |x - hi| <=
 // 2^-11 |x|, |x - hi - lo| <= 2^-22 |x|).  A product is hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16, which sums in fp32: the
 // part left out, lo lo, is at most 2^-22 of it.  Values 2^-17 of what they are scaled by and up have their 22 bits, smaller ones
-// an absolute error of 2^-40 of it, so no more than 2^-34 of their row's largest.  Where rows are summed over, the other operand takes
+// an absolute error of 2^-40 of it, so no more than 2^-28 of their row's largest.  Where rows are summed over, the other operand takes
 // the rows' powers of two, and its own scale follows the products' size, not that of the tiles.  Three products at the fp16 rate cost
 // three eighths of v_mfma_f32_32x32x2_f32's one.
 //
@@ -140,13 +140,15 @@ __device__ __forceinline__ int tile_exponent(float most) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
-// A tile whose rows are unlike -- the largest of one, zeros aside, below 2^-6 of the tile's -- is scaled row by row.  Its exponent, the
-// largest row's, is stored with kOwnRows added, and how far each row's lies below it (0 to -100) beside it.
+// A tile whose rows are unlike -- the largest of one, zeros aside, below 2^-12 of the tile's -- is scaled row by row: rows above keep 22
+// bits of values down to 2^-5 of their own largest.  (A limit of 2^-6 was met by gradients of 2^(2 N(0, 1)): with few keys, where unlike
+// rows cost another pass, 287 us where 145 do, 4096 x 77, 4 x 16 heads of 64.)  The tile's exponent, the largest row's, is stored with kOwnRows added, and how far each row's lies below it (0 to -100) beside it.
 constexpr int kOwnRows = 1024;
+constexpr float kAlike = 0x1p-12f;
 __device__ __forceinline__ bool own_rows(int code) { return code >= kOwnRows / 2; }
 __device__ __forceinline__ int exponent_of(int code) { return own_rows(code) ? code - kOwnRows : code; }
 __device__ __forceinline__ bool rows_unlike(float row_most, float tile_most) {  // of a wave that has all rows
-    return __any(row_most > 0.0f && row_most < tile_most * 0x1p-6f);
+    return __any(row_most > 0.0f && row_most < tile_most * kAlike);
 }
 __device__ __forceinline__ int row_exponent(float row_most, int tile_ex) {
     return row_most > 0.0f ? max(tile_exponent(row_most), tile_ex - 100) : tile_ex;

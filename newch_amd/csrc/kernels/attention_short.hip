@@ -114,11 +114,12 @@ __device__ __forceinline__ h8 turned16(const char *first, const char *second) {
 constexpr int kDsTile = 4096;  // bytes of a packed tile of 32 columns
 
 // The backward's way in: the workgroup's W waves read a tile of 32 rows of queries, output gradients and outputs, one tile ahead,
-// and split it, a piece a lane: piece p is columns 8 (p / 32) .. + 7 of row p % 32.  A tile whose rows are unlike (rows_unlike, of queries
-// or of gradients) is taken in several passes, each with the rows that are alike and zeros in the others' places.
+// and split it, a piece a lane: piece p is columns 8 (p / 32) .. + 7 of row p % 32.  Gradients of unlike rows have a scale for each row,
+// which goes into the rows' statistics as in PackJob; queries of unlike rows are taken in several passes, each with rows that are alike and
+// zeros in the others' places.
 template <int DP, int W>
 struct FeedTables {  // in LDS
-    float stats[64];                // the rows' log2-sum-exps (infinite: not in this pass) and go . o
+    float stats[64];                // the rows' log2-sum-exps (infinite: not in this pass) and go . o, as in PackJob
     float dots[DP / 8][kTile];      // scratch
     float tops[2][DP / 8][kTile];   // the largest of the pieces of queries, of gradients
     float red[2][W];
@@ -126,7 +127,7 @@ struct FeedTables {  // in LDS
 };
 struct FeedPass {
     int eq, eg;       // exponents of the tile's queries and gradients
-    uint32_t rows;    // that are in this pass; none: the tile takes several, or has a row that is loose
+    uint32_t rows;    // that are in this pass; none: rows are unlike, or one is loose
     bool last, hold;  // the tile's last; a row may be loose
 };
 template <int DP, int W>
@@ -216,37 +217,35 @@ struct Feed {
         return {eq, eg, several ? 0u : ~0u, true, false};
     }
 
-    // the same for those rows of `todo` that are like the one of the largest queries, and among them like the one of the largest gradients
-    __device__ __forceinline__ FeedPass split_alike(char *qs, char *gs, FeedTables<DP, W> &t, uint32_t todo) {
+    // the same for those rows of `todo` whose queries are like the largest, gradients by their rows' own scales
+    __device__ __forceinline__ FeedPass split_rows(char *qs, char *gs, FeedTables<DP, W> &t, uint32_t todo) {
         const int p = threadIdx.x;
         const float row_q = of_row(abs_max(q, 0.0f), t), row_g = of_row(abs_max(go, 0.0f), t);
         bool in = (todo >> (p & 31)) & 1;
         const float tq = wave_max_nan_skip(in ? row_q : 0.0f);
-        in = in && (row_q == 0.0f || row_q >= tq * 0x1p-6f);
-        const float tg = wave_max_nan_skip(in ? row_g : 0.0f);
-        in = in && (row_g == 0.0f || row_g >= tg * 0x1p-6f);
+        in = in && (row_q == 0.0f || row_q >= tq * kAlike);
+        const int eq = tile_exponent(tq), eg = tile_exponent(wave_max_nan_skip(in ? row_g : 0.0f)), own = row_exponent(row_g, eg);
         const uint32_t rows = (uint32_t)__ballot(in);
         float dot = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) dot = fma_(go[e], o[e], dot);
         __syncthreads();  // dots have been read
         if (p < UNITS) t.dots[p >> 5][p & 31] = dot;
-        const int eq = tile_exponent(tq), eg = tile_exponent(tg);
         put(q, eq, in, qs);
-        put(go, eg, in, gs);
+        put(go, own, in, gs);
         __syncthreads();
         if (p < kTile) {
             float d = t.dots[0][p];
             for (int c = 1; c < DP / 8; c++) d += t.dots[c][p];
-            t.stats[p] = in ? lse : INFINITY;
-            t.stats[32 + p] = in ? d : 0.0f;
+            t.stats[p] = in ? lse - (float)(own - eg) : INFINITY;
+            t.stats[32 + p] = in ? d * pow2i(eg - own) : 0.0f;
         }
         __syncthreads();
         return {eq, eg, rows, (todo & ~rows) == 0, true};
     }
 
-    // The next pass, of tile t, with the next tile's rows on their way.  The rows of a tile that takes several are read again for each:
-    // kept, they would cost the others' registers.
+    // The next pass, of tile t, with the next tile's rows on their way.  The rows of a tile that is cut again are read again: kept, they would
+    // hold up the next tile's (4096 x 77, 4 x 16 heads of 64, rows alike: 136 us, and 148), or cost the passes' registers.
     __device__ __forceinline__ FeedPass pass(const ShortBwd &f, int64_t b, int64_t u, int64_t &t, int64_t t1, uint32_t &todo, char *qs, char *gs,
                                              FeedTables<DP, W> &tables) {
         FeedPass r;
@@ -257,7 +256,7 @@ struct Feed {
         }
         if (__builtin_expect(r.rows == 0, 0)) {
             fetch(f, b, u, t);
-            r = split_alike(qs, gs, tables, todo);
+            r = split_rows(qs, gs, tables, todo);
             todo = r.last ? ~0u : todo & ~r.rows;
             if (r.last && t + 1 < t1) fetch(f, b, u, t + 1);
         }

@@ -46,7 +46,7 @@ def test_far_larger_values_that_a_row_does_not_count(K, shape, where):
     fq, fk = members(Lq, where), members(Lk, where)
     q, k, v, g = A.two_groups((*shape, None), 52, fq, fk)
     scale = D ** -0.5
-    for e in (7, 16, 20, 30, 40, 50):
+    for e in (7, 11, 13, 16, 20, 30, 40, 50):
         print("values", shape, where, e, flush=True)
         big, far = v.copy(), g.copy()
         big[:, fk] *= np.float32(2.0 ** e)
@@ -91,7 +91,7 @@ def test_far_larger_keys_or_queries(K, shape, where, which):
     else:
         fq = members(Lq, where)
         g[:, fq] = 0
-    for e in (7, 16, 30, 60):
+    for e in (7, 11, 13, 16, 30, 60):
         print(which, shape, where, e, flush=True)
         q2, k2 = q.copy(), k.copy()
         q2[:, fq] *= np.float32(2.0 ** e)
