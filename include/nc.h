@@ -277,6 +277,22 @@ NC_API nc_tensor *nc_qk_norm_rope(nc_tensor *x, int64_t q_heads, nc_tensor *q_we
  * for writing to an input (nc_data_f32) counts as a write, to attention's output it does not. */
 NC_API nc_tensor *nc_cross_attention(nc_tensor *q, nc_tensor *k, nc_tensor *v, nc_tensor *key_lengths, float scale);
 
+/* ---- a language model's two ends (additive; the reference's index_select, dropout and cross_entropy copy rows, keep the mask and
+ * read stored logits) ---- */
+/* scale * weight[tokens]: weight f32 [V, D], tokens i32 of at most 5 dims; the output has one dim of D more.  A token outside [0, V) fails
+ * the call with NC_ERR_ARG.  The gradient of the weight sums over each token's positions in a fixed order; `padding` (negative:
+ * none) is a token without one. */
+NC_API nc_tensor *nc_embedding(nc_tensor *weight, nc_tensor *tokens, float scale, int32_t padding);
+/* x with each value kept and divided by 1 - p, or made 0 with probability p, plus residual (of x's shape; NULL: none).  The mask is a
+ * function of (seed, offset) and the value's place alone and is never stored (nc_hip_dropout_fwd has the generator): the same pair
+ * gives the same mask, so every call of a step and every step takes an offset of its own.  p in [0, 1]. */
+NC_API nc_tensor *nc_dropout_seeded(nc_tensor *x, nc_tensor *residual, double p, uint64_t seed, uint64_t offset);
+/* The cross entropy of x weight^T + bias (x [.., D], weight [V, D], bias [V] or NULL) against labels (i32, x's shape without its last
+ * dim) without keeping the products: the mean, or the sum, over the rows whose label is not `ignore` (a mean over none is NaN).  Rows that
+ * do not count may hold anything.  A label outside [0, V) that is not `ignore` fails the call with NC_ERR_ARG.  Where an input
+ * needs a gradient the forward takes it and keeps it for the backward, which scales it: inputs may be written in between. */
+NC_API nc_tensor *nc_linear_cross_entropy(nc_tensor *x, nc_tensor *weight, nc_tensor *bias, nc_tensor *labels, int32_t ignore, int sum);
+
 #ifdef __cplusplus
 }
 #endif

@@ -354,6 +354,44 @@ NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int64_t Lk, int
                                           float *gv, int acc_q, int acc_k, int acc_v, void *ws, size_t ws_bytes,
                                           void *stream);
 
+/* A language model's two ends and the regulariser between them; no counterparts in the reference's device-free engine, whose
+ * index_select, dropout and cross_entropy copy rows, keep masks and keep logits.
+ *
+ * Embedding: y[i] = scale * w[tokens[i]], tokens i32 [N], w [V, D] with rows ldw apart, y [N, D] contiguous.  A token outside [0, V)
+ * gives a row of zeros; where bad (8 bytes, device or device-mapped host memory; NULL: not looked for) is set it receives the first such
+ * one as (i << 32) | (uint32)token, or all ones.  Backward: gw [V, D] contiguous (+)= scale * the sum of g [N, D] over the positions of each
+ * token, in a fixed order; tokens outside [0, V) and the token `padding` (negative: none) have no gradient, and g is not read at their
+ * positions.  Rows whose token does not occur become zero where gw is stored and stay where it is added to.  gw does not overlap g; the
+ * workspace is 16-byte aligned.  N <= 2^30, V < 2^31. */
+NC_HIP_API int nc_hip_embedding_fwd(int64_t N, int64_t V, int64_t D, const float *w, int64_t ldw, const int32_t *tokens, float scale,
+                                    float *y, uint64_t *bad, void *stream);
+NC_HIP_API size_t nc_hip_embedding_bwd_workspace(int64_t N, int64_t V, int64_t D);
+NC_HIP_API int nc_hip_embedding_bwd(int64_t N, int64_t V, int64_t D, const int32_t *tokens, int32_t padding, float scale, const float *g,
+                                    float *gw, int accumulate, void *ws, size_t ws_bytes, void *stream);
+/* Dropout with a mask made from (seed, offset) wherever it is needed: value i of n stays where word i % 4 of Philox 4x32-10's block
+ * (key seed, counter (i / 4, offset + *offset_dev)) is at least p 2^32, rounded to even.  y = x / (1 - p) where it stays, else 0,
+ * plus the residual (NULL: none); a value that is dropped counts as 0 whatever it holds.  Backward: gx (+)= gy / (1 - p) where the
+ * value stays.  offset_dev (NULL: 0) is device memory that is read when the kernel runs, so that a captured call draws another mask
+ * at each replay whose owner has changed it.  One offset is one mask: calls that need unlike masks take unlike offsets.  y may
+ * be x or the residual, gx may be gy.  0 <= p <= 1. */
+NC_HIP_API int nc_hip_dropout_fwd(int64_t n, double p, uint64_t seed, uint64_t offset, const uint64_t *offset_dev, const float *x,
+                                  const float *residual, float *y, void *stream);
+NC_HIP_API int nc_hip_dropout_bwd(int64_t n, double p, uint64_t seed, uint64_t offset, const uint64_t *offset_dev, const float *gy,
+                                  float *gx, int accumulate, void *stream);
+/* Cross entropy of z = x w^T + bias against labels, and its gradients, without keeping z: x [N, D] (rows ldx apart), w [V, D] (rows ldw
+ * apart), bias [V] or NULL, labels i32 [N].  A row whose label is `ignore` does not count, whatever its x holds: no loss, a gradient of zeros.
+ * Neither does one whose label is outside [0, V); `bad` receives the first such row as in nc_hip_cross_entropy_fwd (NULL: not asked
+ * for).  *loss is the mean of the rows that count (NaN where none does) or their sum; row_loss [N] (NULL: not asked for) each row's.
+ * gx [N, D], gw [V, D] and gb [V] (contiguous, each may be NULL: the loss alone) are stored or, with their acc, added to: the gradients of
+ * *gout * loss (gout: one float in device memory; NULL: 1).  Sums in a fixed order.  Outputs overlap neither inputs nor each other.
+ * The workspace (16-byte aligned) is for the gradients that are asked for; its contents count only within a call.
+ * N < 2^31, D <= 2^20, V <= 2^26. */
+NC_HIP_API size_t nc_hip_linear_cross_entropy_workspace(int64_t N, int64_t D, int64_t V, int want_x, int want_w, int want_b);
+NC_HIP_API int nc_hip_linear_cross_entropy(int64_t N, int64_t D, int64_t V, const float *x, int64_t ldx, const float *w, int64_t ldw,
+                                           const float *bias, const int32_t *labels, int32_t ignore, int sum, const float *gout,
+                                           float *loss, float *row_loss, uint64_t *bad, float *gx, float *gw, float *gb, int acc_x,
+                                           int acc_w, int acc_b, void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

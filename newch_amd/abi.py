@@ -15,7 +15,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64,
+                    c_void_p)
 from pathlib import Path
 
 F32, I32, F16, I8, U8 = 0, 1, 2, 3, 4
@@ -181,6 +182,13 @@ NC_ATTENTION_SIGNATURES: dict[str, tuple] = {
     "nc_cross_attention": (P, [P, P, P, P, c_float]),
 }
 
+# A language model's two ends in this engine (not in the reference ABI).
+NC_LANGUAGE_SIGNATURES: dict[str, tuple] = {
+    "nc_embedding": (P, [P, P, c_float, c_int32]),
+    "nc_dropout_seeded": (P, [P, P, c_double, c_uint64, c_uint64]),
+    "nc_linear_cross_entropy": (P, [P, P, P, P, c_int32, c_int]),
+}
+
 
 def bind(lib: ctypes.CDLL, strict: bool = True) -> ctypes.CDLL:
     """Sets restype/argtypes for every nc.h function (raises AttributeError on a missing one when
@@ -193,7 +201,7 @@ def bind(lib: ctypes.CDLL, strict: bool = True) -> ctypes.CDLL:
                 raise
             continue
         fn.restype, fn.argtypes = res, args
-    for name, (res, args) in (NC_DEVICE_SIGNATURES | NC_ATTENTION_SIGNATURES).items():
+    for name, (res, args) in (NC_DEVICE_SIGNATURES | NC_ATTENTION_SIGNATURES | NC_LANGUAGE_SIGNATURES).items():
         if hasattr(lib, name):
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args

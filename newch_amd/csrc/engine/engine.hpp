@@ -276,6 +276,20 @@ nc_tensor *apply(const OpDef *op, nc_tensor **in, int n_in, const Params *p);
 // activation by a FREE_GRAPH backward, at once when the call is not recorded, else at step end.
 void *save_state(nc_node *n, size_t bytes);
 
+// A kernel's report of the first label or token that is out of range, (position << 32) | value or all ones, read back before
+// the call returns (ops_nn.cpp).
+struct IndexCheck {
+    uint64_t *bad = nullptr;  // where the kernel writes it
+    uint64_t key = 0;
+    bool mapped = false;  // host memory that the host watches
+
+    bool begin(nc_ctx *ctx);
+    bool read(nc_ctx *ctx, const char *what);
+    bool ok() const { return key == ~(uint64_t)0; }
+    long long at() const { return (long long)(key >> 32); }
+    int32_t value() const { return (int32_t)(uint32_t)key; }
+};
+
 inline bool needs_grad(const nc_tensor *t) { return (t->flags & TF_REQUIRES_GRAD) != 0; }
 inline hipStream_t stream(const nc_ctx *ctx) { return ctx->stream; }
 

@@ -151,7 +151,7 @@ static nc_status loss_shape(nc_node *n, OutSpec &out) {
     return NC_OK;
 }
 
-// The loss forwards' bad-label key lands in a pinned, coherent host word the kernel stores to at system scope (mapped into the
+// The key lands in a pinned, coherent host word the kernel stores to at system scope (mapped into the
 // device's address space), so the host sees it while the stream still runs, with no device-to-host copy: the
 // reference's error is a synchronous one.  Null when the host allocation is refused: the key then goes through arena memory
 // and a copy.
@@ -174,7 +174,7 @@ static uint64_t *loss_flag_dev(nc_ctx *ctx) {
 }
 
 // The mapped word holds kLossPending (no key: rows are numbered from 0 in 32 bits, and this one's label is valid) until
-// the forward's last kernel writes it, so the host sees the key as soon as it is written; the stream's own
+// the kernel writes it, so the host sees the key as soon as it is written; the stream's own
 // synchronization comes back later, while the GPU waits for the next launch (loss and gradient of small logits 26.5 -> 22 us, a
 // classifier's step at batch 64 98 -> 70).  After 2 ms of looking it is
 // left to that, which also reports a kernel that failed.
@@ -188,6 +188,23 @@ static bool poll_loss_flag(const nc_ctx *ctx, uint64_t &key) {
         if (k % 64 == 0 && std::chrono::steady_clock::now() - t0 > std::chrono::milliseconds(2)) return false;
         __builtin_ia32_pause();
     }
+}
+
+bool IndexCheck::begin(nc_ctx *ctx) {
+    uint64_t *const m = loss_flag_dev(ctx);
+    mapped = m != nullptr;
+    bad = m ? m : (uint64_t *)arena_alloc(ctx, sizeof(uint64_t));
+    if (mapped) __atomic_store_n(ctx->loss_flag, kLossPending, __ATOMIC_RELEASE);
+    return bad != nullptr;
+}
+
+bool IndexCheck::read(nc_ctx *ctx, const char *what) {
+    if (!mapped && !hip_ok(ctx, hipMemcpyAsync(&key, bad, sizeof key, hipMemcpyDeviceToHost, stream(ctx)), what)) return false;
+    if (!mapped || !poll_loss_flag(ctx, key)) {
+        if (!hip_ok(ctx, hipStreamSynchronize(stream(ctx)), what)) return false;
+        if (mapped) key = *(volatile const uint64_t *)ctx->loss_flag;
+    }
+    return true;
 }
 
 static nc_status loss_fwd(nc_node *n) {
@@ -204,28 +221,19 @@ static nc_status loss_fwd(nc_node *n) {
     char *saved = (char *)save_state(n, sbytes);
     const size_t ws_bytes = nc_hip_loss_workspace(N, C);
     char *ws = arena_alloc(ctx, ws_bytes ? ws_bytes : 8);
-    uint64_t *const mapped = loss_flag_dev(ctx);
-    uint64_t *bad = mapped ? mapped : (uint64_t *)arena_alloc(ctx, sizeof(uint64_t));
-    if (!saved || !ws || !bad) return NC_ERR_STATE;
-    if (mapped) __atomic_store_n(ctx->loss_flag, kLossPending, __ATOMIC_RELEASE);
+    IndexCheck check;
+    if (!saved || !ws || !check.begin(ctx)) return NC_ERR_STATE;
     float *stats = ce ? (float *)saved : nullptr;
     int32_t *lab = (int32_t *)(saved + pbytes);
     if (N > 0 && !hip_layer_ok(ctx, nc_hip_copy_strided(4, 1, yt->shape, labels, yt->stride, lab, stream(ctx)),
                                n->op->name))
         return NC_ERR_STATE;
-    const int rc = ce ? nc_hip_cross_entropy_fwd(N, C, x, lab, stats, loss, bad, ws, ws_bytes, stream(ctx))
-                      : nc_hip_nll_loss_fwd(N, C, x, lab, (int)n->p.i[0], loss, bad, ws, ws_bytes, stream(ctx));
+    const int rc = ce ? nc_hip_cross_entropy_fwd(N, C, x, lab, stats, loss, check.bad, ws, ws_bytes, stream(ctx))
+                      : nc_hip_nll_loss_fwd(N, C, x, lab, (int)n->p.i[0], loss, check.bad, ws, ws_bytes, stream(ctx));
     if (!hip_layer_ok(ctx, rc, n->op->name)) return NC_ERR_STATE;
-    uint64_t hb = 0;
-    if (!mapped && !hip_ok(ctx, hipMemcpyAsync(&hb, bad, sizeof hb, hipMemcpyDeviceToHost, stream(ctx)), n->op->name))
-        return NC_ERR_STATE;
-    if (!mapped || !poll_loss_flag(ctx, hb)) {
-        if (!hip_ok(ctx, hipStreamSynchronize(stream(ctx)), n->op->name)) return NC_ERR_STATE;
-        if (mapped) hb = *(volatile const uint64_t *)ctx->loss_flag;
-    }
-    if (hb != ~(uint64_t)0) {
-        error(ctx, NC_ERR_ARG, "%s: label %d at row %lld outside [0, %lld)", n->op->name, (int32_t)(uint32_t)hb,
-              (long long)(hb >> 32), (long long)C);
+    if (!check.read(ctx, n->op->name)) return NC_ERR_STATE;
+    if (!check.ok()) {
+        error(ctx, NC_ERR_ARG, "%s: label %d at row %lld outside [0, %lld)", n->op->name, check.value(), check.at(), (long long)C);
         return NC_ERR_ARG;
     }
     wrote_dev(n->out);

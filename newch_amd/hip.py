@@ -10,7 +10,8 @@ message when a call returns an error code; nothing here falls back to the host.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import (POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64,
+                    c_void_p)
 
 from . import abi
 
@@ -107,6 +108,14 @@ SIGNATURES = {
     "nc_hip_cross_attention_bwd": (c_int, [c_int64] * 6 + [c_float, P, I64P, P, I64P, P, I64P, P, P, P, P, P, P, P, c_int,
                                                            c_int, c_int, P, c_size_t, P]),
     "nc_hip_linear_int8": (c_int, [c_int64, c_int64, c_int64, P, P, P, P, P, P, c_size_t, P]),
+    "nc_hip_embedding_fwd": (c_int, [c_int64, c_int64, c_int64, P, c_int64, P, c_float, P, P, P]),
+    "nc_hip_embedding_bwd_workspace": (c_size_t, [c_int64, c_int64, c_int64]),
+    "nc_hip_embedding_bwd": (c_int, [c_int64, c_int64, c_int64, P, c_int32, c_float, P, P, c_int, P, c_size_t, P]),
+    "nc_hip_dropout_fwd": (c_int, [c_int64, c_double, c_uint64, c_uint64, P, P, P, P, P]),
+    "nc_hip_dropout_bwd": (c_int, [c_int64, c_double, c_uint64, c_uint64, P, P, P, c_int, P]),
+    "nc_hip_linear_cross_entropy_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
+    "nc_hip_linear_cross_entropy": (c_int, [c_int64, c_int64, c_int64, P, c_int64, P, c_int64, P, P, c_int32, c_int, P, P, P, P, P,
+                                            P, P, c_int, c_int, c_int, P, c_size_t, P]),
 }
 
 
@@ -359,3 +368,34 @@ class Kernels:
         self._ok(self.lib.nc_hip_cross_attention_bwd(B, Lq, Lk, Hq, Hkv, D, scale, q, _i64(sq), k, _i64(sk), v, _i64(sv),
                                                      key_len, o, lse, go, gq, gk, gv, int(aq), int(ak), int(av), ws,
                                                      ws_bytes, stream), "cross_attention_bwd")
+
+    def embedding_fwd(self, N, V, D, w, ldw, tokens, scale, y, bad=None, stream=None):
+        """bad: 8 bytes that receive the first token outside [0, V) as (position << 32) | token, or all ones."""
+        self._ok(self.lib.nc_hip_embedding_fwd(N, V, D, w, ldw, tokens, scale, y, bad, stream), "embedding_fwd")
+
+    def embedding_bwd_workspace(self, N, V, D):
+        return self.lib.nc_hip_embedding_bwd_workspace(N, V, D)
+
+    def embedding_bwd(self, N, V, D, tokens, padding, scale, g, gw, ws=None, ws_bytes=0, accumulate=True, stream=None):
+        """padding: a token without a gradient, or -1."""
+        self._ok(self.lib.nc_hip_embedding_bwd(N, V, D, tokens, padding, scale, g, gw, int(accumulate), ws, ws_bytes, stream),
+                 "embedding_bwd")
+
+    def dropout_fwd(self, n, p, seed, offset, x, residual, y, offset_ptr=None, stream=None):
+        """offset_ptr: 8 bytes of device memory added to the offset when the kernel runs."""
+        self._ok(self.lib.nc_hip_dropout_fwd(n, p, seed, offset, offset_ptr, x, residual, y, stream), "dropout_fwd")
+
+    def dropout_bwd(self, n, p, seed, offset, gy, gx, offset_ptr=None, accumulate=True, stream=None):
+        self._ok(self.lib.nc_hip_dropout_bwd(n, p, seed, offset, offset_ptr, gy, gx, int(accumulate), stream), "dropout_bwd")
+
+    def linear_cross_entropy_workspace(self, N, D, V, gx=False, gw=False, gb=False):
+        return self.lib.nc_hip_linear_cross_entropy_workspace(N, D, V, int(gx), int(gw), int(gb))
+
+    def linear_cross_entropy(self, N, D, V, x, ldx, w, ldw, bias, labels, loss, ws, ws_bytes, ignore=-100, sum=False, gout=None,
+                             rows=None, bad=None, gx=None, gw=None, gb=None, accumulate=False, stream=None):
+        """rows: each row's loss; gradients stored (or, accumulate, added: one flag, or one each for gx, gw and gb) where
+        their address is given."""
+        ax, aw, ab = accumulate if isinstance(accumulate, tuple) else (accumulate,) * 3
+        self._ok(self.lib.nc_hip_linear_cross_entropy(N, D, V, x, ldx, w, ldw, bias, labels, ignore, int(sum), gout, loss, rows,
+                                                      bad, gx, gw, gb, int(ax), int(aw), int(ab), ws, ws_bytes, stream),
+                 "linear_cross_entropy")
