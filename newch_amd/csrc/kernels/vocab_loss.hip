@@ -8,25 +8,11 @@
 //
 // A row's own entry of G is -(1 - p_l) = -others / (others + e_l), with the exponentials of the other words summed by
 // themselves: p_l - 1 would lose the bits of a word that is all but certain.
-#include "common.hpp"
-
-#include <algorithm>
+#include "vocab_loss.hpp"
 
 namespace nchip {
 
-constexpr int kVlB = 256;
 constexpr size_t kVlPiece = size_t(1) << 30;  // bytes of z held at a time
-
-// the head of the workspace
-struct VlHead {
-    int64_t count;  // rows that count
-};
-
-struct VlRow {
-    float m, ls;  // the row's maximum and log sum exp(z - m)
-    float own;    // p_l - 1
-    float pad;
-};
 
 struct VlArgs {
     int64_t N, V, ldz;
@@ -69,8 +55,6 @@ __global__ __launch_bounds__(1024) void k_vl_count(const int32_t *__restrict__ l
     }
 }
 
-__device__ __forceinline__ bool vl_counts(int32_t label, int32_t ignore, int64_t V) { return label != ignore && label >= 0 && label < V; }
-
 // x with zeros for the rows that do not count
 __global__ __launch_bounds__(kVlB) void k_vl_rows(const float *__restrict__ x, int64_t ldx, const int32_t *__restrict__ labels, int32_t ignore,
                                                   int64_t N, int64_t D, int64_t V, float *__restrict__ out) {
@@ -78,17 +62,6 @@ __global__ __launch_bounds__(kVlB) void k_vl_rows(const float *__restrict__ x, i
         const bool on = vl_counts(labels[i], ignore, V);
         for (int64_t d = threadIdx.x; d < D; d += kVlB) out[i * D + d] = on ? x[i * ldx + d] : 0.0f;
     }
-}
-
-__device__ __forceinline__ double wg_sum(double v, double *sh) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x / kWave] = v;
-    __syncthreads();
-    double t = 0.0;
-#pragma unroll
-    for (int i = 0; i < kVlB / kWave; i++) t += sh[i];
-    return t;
 }
 
 // A workgroup's row: its statistics, its loss, and, GRAD, its row of G in place of z.
@@ -119,7 +92,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_softmax(VlArgs p) {
         for (int k = 0; k < kVlB / kWave; k++) m = __builtin_fmaxf(m, shm[k]);
         double s = 0.0;
         for (int64_t v = threadIdx.x; v < p.V; v += kVlB) s += v == l ? 0.0 : (double)exp_sum_term(z[v] - m);
-        const double others = wg_sum(s, sh);
+        const double others = vl_wg_sum(s, sh);
         const float zl = z[l] - m;
         const double own = (double)exp8_nonpos(zl), total = others + own;
         const double ls = zl == 0.0f ? log1p(others) : log(total);
@@ -153,15 +126,13 @@ __global__ __launch_bounds__(kVlB) void k_vl_finish(const double *__restrict__ r
     __shared__ double sh[kVlB / kWave];
     double t = 0.0;
     for (int64_t i = threadIdx.x; i < N; i += kVlB) t += row_loss[i];
-    t = wg_sum(t, sh);
+    t = vl_wg_sum(t, sh);
     if (threadIdx.x == 0) *loss = sum ? (float)t : head->count ? (float)(t / (double)head->count) : __builtin_nanf("");
 }
 
 __global__ __launch_bounds__(kVlB) void k_vl_zero(float *__restrict__ p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * kVlB + threadIdx.x; i < n; i += (int64_t)gridDim.x * kVlB) p[i] = 0.0f;
 }
-
-static size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // the workspace: [head][row losses][x without the rows that do not count][z of a piece]
 struct VlPlan {
@@ -175,8 +146,8 @@ static VlPlan vl_plan(int64_t N, int64_t D, int64_t V, bool want_w) {
     const int64_t most = std::max<int64_t>(64, (int64_t)(kVlPiece / 4) / p.ldz / 64 * 64);
     p.piece = std::min(N, most);
     p.losses = 256;
-    p.rows = p.losses + round256((size_t)N * 8);
-    p.z = p.rows + (want_w ? round256((size_t)(N * D) * 4) : 0);
+    p.rows = p.losses + vl_round256((size_t)N * 8);
+    p.z = p.rows + (want_w ? vl_round256((size_t)(N * D) * 4) : 0);
     p.total = p.z + (size_t)(p.piece * p.ldz) * 4;
     return p;
 }
@@ -193,8 +164,8 @@ static const char *vl_size_error(int64_t N, int64_t D, int64_t V) {
 using namespace nchip;
 
 extern "C" NC_HIP_API size_t nc_hip_linear_cross_entropy_workspace(int64_t N, int64_t D, int64_t V, int want_x, int want_w, int want_b) {
-    (void)want_x, (void)want_b;
     if (vl_size_error(N, D, V)) return 0;
+    if (vl_split_pays(N, D, V, want_x || want_w || want_b)) return vl_split_workspace(N, D, V, want_x != 0, want_w != 0, want_b != 0);
     return vl_plan(N, D, V, want_w != 0).total;
 }
 
@@ -208,15 +179,19 @@ extern "C" NC_HIP_API int nc_hip_linear_cross_entropy(int64_t N, int64_t D, int6
     if (!loss || !w || (N > 0 && (!x || !labels))) return set_error(NC_HIP_ERR_ARG, "%s: NULL pointer", what);
     if (ldx < D || ldw < D) return set_error(NC_HIP_ERR_ARG, "%s: rows closer than their %lld columns", what, (long long)D);
     if (((uintptr_t)bad & 7u) != 0) return set_error(NC_HIP_ERR_ARG, "%s: bad is not 8-byte aligned", what);
-    const VlPlan plan = vl_plan(N, D, V, gw != nullptr);
-    if (!ws || ws_bytes < plan.total) return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, plan.total);
+    const size_t need = nc_hip_linear_cross_entropy_workspace(N, D, V, gx != nullptr, gw != nullptr, gb != nullptr);
+    if (!ws || ws_bytes < need) return set_error(NC_HIP_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
     if (((uintptr_t)ws & 15u) != 0) return set_error(NC_HIP_ERR_ARG, "%s: the workspace is not 16-byte aligned", what);
     hipStream_t st = as_stream(stream);
+    const bool grad = gx || gw || gb;
+    if (vl_split_pays(N, D, V, grad))
+        return vl_split_run({N, D, V, x, ldx, w, ldw, bias, labels, ignore, sum, gout, loss, row_loss, (unsigned long long *)bad, gx, gw, gb,
+                             acc_x, acc_w, acc_b, (char *)ws, st}, what);
+    const VlPlan plan = vl_plan(N, D, V, gw != nullptr);
     char *base = (char *)ws;
     VlHead *head = (VlHead *)base;
     double *losses = (double *)(base + plan.losses);
     float *clean = (float *)(base + plan.rows), *z = (float *)(base + plan.z);
-    const bool grad = gx || gw || gb;
     hipLaunchKernelGGL(k_vl_count, 1, 1024, 0, st, labels, N, V, ignore, head, (unsigned long long *)bad);
     if (N > 0 && gw) hipLaunchKernelGGL(k_vl_rows, (unsigned)std::min<int64_t>(N, 1 << 16), kVlB, 0, st, x, ldx, labels, ignore, N, D, V, clean);
     for (int64_t r0 = 0; r0 < N; r0 += plan.piece) {

@@ -1,0 +1,57 @@
+// Shared pieces of the vocabulary loss: vocab_loss.hip (entry points, the form on fp32 products) and vocab_split.hip (the form whose
+// products run on the fp16 matrix cores).
+#pragma once
+
+#include "common.hpp"
+
+#include <algorithm>
+
+namespace nchip {
+
+constexpr int kVlB = 256;
+
+// the head of the workspace
+struct VlHead {
+    int64_t count;  // rows that count
+};
+
+// one call's arguments
+struct VlCall {
+    int64_t N, D, V;
+    const float *x;
+    int64_t ldx;
+    const float *w;
+    int64_t ldw;
+    const float *bias;
+    const int32_t *labels;
+    int32_t ignore;
+    int sum;
+    const float *gout;
+    float *loss, *row_loss;
+    unsigned long long *bad;
+    float *gx, *gw, *gb;
+    int acc_x, acc_w, acc_b;
+    char *ws;
+    hipStream_t st;
+};
+
+__device__ __forceinline__ bool vl_counts(int32_t label, int32_t ignore, int64_t V) { return label != ignore && label >= 0 && label < V; }
+
+__device__ __forceinline__ double vl_wg_sum(double v, double *sh) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x / kWave] = v;
+    __syncthreads();
+    double t = 0.0;
+    for (int i = 0; i < (int)blockDim.x / kWave; i++) t += sh[i];
+    return t;
+}
+
+inline size_t vl_round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// whether the products of a call are worth cutting into pieces, the workspace that takes, and the call itself
+bool vl_split_pays(int64_t N, int64_t D, int64_t V, bool grads);
+size_t vl_split_workspace(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w, bool want_b);
+int vl_split_run(const VlCall &c, const char *what);
+
+}  // namespace nchip
