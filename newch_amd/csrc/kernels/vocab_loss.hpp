@@ -13,6 +13,7 @@ constexpr int kVlB = 256;
 // the head of the workspace
 struct VlHead {
     int64_t count;  // rows that count
+    int slices;     // of the words in gx
 };
 
 // one call's arguments

@@ -24,14 +24,23 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f16x __attribute__((ext_vector_type(16)));
 typedef int i4v __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 256;       // rows and columns of a workgroup's product
-constexpr int kMmB = 512;        // its lanes: 8 waves, 2 over the rows and 4 over the columns
-constexpr int kStages = 4;       // blocks of 16 k in LDS
-constexpr int kStage = 2 * kTile * 16 * 4;  // bytes of one: both operands' 256 rows, two pieces
-constexpr size_t kMmLds = (size_t)kStages * kStage;
+// A workgroup's product: 256 rows by 64 columns for each of its WN pairs of waves, WN 2 or 4; kStages blocks of 16 k in LDS.
+constexpr int kTileM = 256, kTileMost = 256;
+constexpr int kStages = 3;
+template <int WN>
+struct Tile {
+    static constexpr int kN = 64 * WN, kLanes = 128 * WN;
+    static constexpr uint32_t kStageA = kTileM * 16 * 4, kStage = (kTileM + kN) * 16 * 4;  // bytes: the rows of A, all
+    static constexpr int kLds = kStages * kStage;
+    static constexpr int kA = 4 / WN;                // row blocks of A that a wave brings, besides one of B
+    static constexpr int kLoads = 2 * (kA + 1);      // and the KiB that these are
+};
 constexpr int64_t kZBytes = int64_t(4) << 30;  // of z and of the turned G, both together, held at a time
 constexpr int64_t kScored = int64_t(1) << 36;  // products of a launch that leaves no z
 constexpr int64_t kPieceRows = 1 << 20;
+constexpr int64_t kPartBytes = int64_t(512) << 20;  // of the parts of gx
+constexpr int kSizeBlocks = 8;   // of 32 rows that a workgroup looks at for their sizes, at most
+constexpr int kPackCols = 128;
 constexpr int kStatWords = 128;  // words of one partial statistic
 
 struct VlRow {
@@ -72,8 +81,8 @@ enum { MM_Z = 0, MM_GX = 1, MM_GW = 2 };
 struct MmArgs {
     const char *A, *B;      // packed; blocks of a row block follow each other
     int64_t step_a, step_b;  // bytes from a row block to the next
-    int tiles_m, tiles_n, slices;
-    int kblocks;            // of 16 k, all slices together: an even number, as each slice's is
+    int tiles_m, tiles_n;   // at most
+    int kblocks;            // of 16 k: an even number, as each slice's is
     const VlHead *head;
     int64_t row0;           // of this piece, among the rows that count
     int64_t V, D;
@@ -158,64 +167,83 @@ __device__ __forceinline__ void z_out(const MmArgs &p, f16x (&acc)[4][2], int64_
     }
 }
 
-template <int WHAT>
-__global__ __launch_bounds__(kMmB, 2) void k_vl_product(MmArgs p) {
+// How many parts the words are cut into for gx: of few tiles' products, as many as make the rounds of workgroups full.  In units of a
+// block of 16 k of a tile (a round costs its blocks and some 24 to start and to leave): rounds x blocks + the parts' way through memory.
+__device__ __forceinline__ int gx_slices(int64_t left, int tiles_n, int kblocks, int most, int at_once) {
+    const int64_t tiles = (left + kTileM - 1) / kTileM * tiles_n;
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int s = 1; s <= most; s++) {
+        const int64_t rounds = (tiles * s + at_once - 1) / at_once;
+        const int64_t cost = rounds * ((kblocks + s - 1) / s + 24) + tiles * s / 24;
+        if (cost < least) least = cost, best = s;
+    }
+    return best;
+}
+
+// WN 2: two workgroups a CU, so that one multiplies while the other starts or leaves, and fewer that wait for the last.  WN 4: one, which
+// brings three quarters as much for a product.
+template <int WHAT, int WN>
+__global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
+    using T = Tile<WN>;
+    constexpr uint32_t kStage = T::kStage;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wm = wave & 1, wn = wave >> 1;
-    // XCD x runs the workgroups b with b % 8 == x: it gets the x-th of 8 runs of tiles, in groups of 8 tile rows
-    const uint32_t nblk = gridDim.x, xcd = blockIdx.x & 7, per = nblk >> 3, rem = nblk & 7;
-    const uint32_t id = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
-    const uint32_t tiles = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;
-    const int slice = (int)(id / tiles), tile = (int)(id % tiles);
-    const int per_group = 8 * p.tiles_n, group = tile / per_group, in_group = tile % per_group;
-    const int gsize = min(p.tiles_m - group * 8, 8);
-    const int tm = group * 8 + in_group % gsize, tn = in_group / gsize;
-
     const int64_t left = p.head->count - p.row0;  // rows of this piece and behind it
+    const int slices = WHAT == MM_GX ? p.head->slices : 1;
+    const uint32_t tiles_m = WHAT == MM_GX ? (uint32_t)(left > 0 ? (min(left, p.rows) + kTileM - 1) / kTileM : 0) : (uint32_t)p.tiles_m;
+    const uint32_t tiles_n = WHAT == MM_Z ? (uint32_t)(left > 0 ? (min(left, p.rows) + T::kN - 1) / T::kN : 0) : (uint32_t)p.tiles_n;
+    const uint32_t tiles = tiles_m * tiles_n, nblk = tiles * (uint32_t)slices;
+    if (blockIdx.x >= nblk) return;
+    // XCD x runs the workgroups b with b % 8 == x: it gets the x-th of 8 runs of tiles, in groups of 8 tile rows
+    const uint32_t xcd = blockIdx.x & 7, per = nblk >> 3, rem = nblk & 7;
+    const uint32_t id = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
+    const int slice = (int)(id / tiles), tile = (int)(id % tiles);
+    const int per_group = 8 * (int)tiles_n, group = tile / per_group, in_group = tile % per_group;
+    const int gsize = min((int)tiles_m - group * 8, 8);
+    const int tm = group * 8 + in_group % gsize, tn = in_group / gsize;
     int k0 = 0, k1 = p.kblocks;
-    if (WHAT == MM_Z && (int64_t)tn * kTile >= left) return;
     if (WHAT == MM_GX) {
-        if ((int64_t)tm * kTile >= left) return;
         const int64_t pairs = p.kblocks / 2;
-        k0 = 2 * (int)(pairs * slice / p.slices), k1 = 2 * (int)(pairs * (slice + 1) / p.slices);
+        k0 = 2 * (int)(pairs * slice / slices), k1 = 2 * (int)(pairs * (slice + 1) / slices);
     }
     if (WHAT == MM_GW) {
         k1 = (int)min((int64_t)p.kblocks, left > 0 ? (left + 31) / 32 * 2 : 0);
         if (k1 == 0 && p.acc) return;
     }
     const int nk = k1 - k0;
+    const int64_t m0 = (int64_t)tm * kTileM + 128 * wm, n0 = (int64_t)tn * T::kN + 64 * wn;
+    // a wave whose columns no result has only brings its share
+    const bool works = n0 < (WHAT == MM_Z ? left : p.D);
 
-    // wave w brings four of a stage's 32 KiB: pieces of row blocks 2 (w % 4) and the next, of A (w < 4) or B
-    const char *src;
-    int64_t next;
-    {
-        const bool b = wave >= 4;
-        const int64_t rb = (int64_t)(b ? tn : tm) * (kTile / 32) + 2 * (wave & 3);
-        next = b ? p.step_b : p.step_a;
-        src = (b ? p.B : p.A) + rb * next + (int64_t)k0 * 2048 + lane * 16;
-    }
+    // each wave brings its share of a stage: the pieces of kA row blocks of A and of one of B
+    const char *src_a = p.A + ((int64_t)tm * (kTileM / 32) + T::kA * wave) * p.step_a + (int64_t)k0 * 2048 + lane * 16;
+    const char *src_b = p.B + ((int64_t)tn * (T::kN / 32) + wave) * p.step_b + (int64_t)k0 * 2048 + lane * 16;
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    const uint32_t to = base + (uint32_t)wave * 4096;
-    auto bring = [&](int kt) {
-        const uint32_t at = __builtin_amdgcn_readfirstlane(to + (uint32_t)(kt & (kStages - 1)) * kStage);
-        const char *s = src + (int64_t)kt * 2048;
-        dma16(s, at);
-        dma16(s + 1024, at + 1024);
-        dma16(s + next, at + 2048);
-        dma16(s + next + 1024, at + 3072);
+    const uint32_t to_a = base + (uint32_t)wave * (2048 * T::kA), to_b = base + T::kStageA + (uint32_t)wave * 2048;
+    auto bring = [&](uint32_t stage) {
+        const uint32_t a = __builtin_amdgcn_readfirstlane(to_a + stage), b = __builtin_amdgcn_readfirstlane(to_b + stage);
+#pragma unroll
+        for (int i = 0; i < T::kA; i++) {
+            dma16(src_a + i * p.step_a, a + 2048 * i);
+            dma16(src_a + i * p.step_a + 1024, a + 2048 * i + 1024);
+        }
+        dma16(src_b, b);
+        dma16(src_b + 1024, b + 1024);
+        src_a += 2048, src_b += 2048;
     };
-    auto fetch = [&](int kt, Frags &f) {
-        const char *s = lds + (kt & (kStages - 1)) * kStage + lane * 16;
+    const char *const my_a = lds + wm * 8192 + lane * 16, *const my_b = lds + T::kStageA + wn * 4096 + lane * 16;
+    auto fetch = [&](uint32_t stage, Frags &f) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            f.a[i][0] = *(const h8 *)(s + (4 * wm + i) * 2048);
-            f.a[i][1] = *(const h8 *)(s + (4 * wm + i) * 2048 + 1024);
+            f.a[i][0] = *(const h8 *)(my_a + stage + i * 2048);
+            f.a[i][1] = *(const h8 *)(my_a + stage + i * 2048 + 1024);
         }
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            f.b[j][0] = *(const h8 *)(s + kStage / 2 + (2 * wn + j) * 2048);
-            f.b[j][1] = *(const h8 *)(s + kStage / 2 + (2 * wn + j) * 2048 + 1024);
+            f.b[j][0] = *(const h8 *)(my_b + stage + j * 2048);
+            f.b[j][1] = *(const h8 *)(my_b + stage + j * 2048 + 1024);
         }
     };
     f16x acc[4][2];
@@ -237,38 +265,52 @@ __global__ __launch_bounds__(kMmB, 2) void k_vl_product(MmArgs p) {
 #pragma unroll
             for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.a[i][0], f.b[j][0], acc[i][j], 0, 0, 0);
     };
-    // At the barrier before block kt every wave's share of block kt + 1 is in LDS, and every wave has read block kt and with it left block
-    // kt - 1, whose stage then takes block kt + 3.  A wave reads block kt + 1 into registers while it multiplies block kt.
+    // At the barrier before block kt every wave's share of block kt + 1 is in LDS and every wave holds block kt in registers, so its
+    // stage takes block kt + 3.  A wave reads block kt + 1 into registers while it multiplies block kt.
     auto wait = [&](int kt) {  // this wave's loads of block kt + 1 have landed; those of kt + 2 may be on their way
-        if (kt + 2 < nk) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        if (kt + 2 < nk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::kLoads) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();
     };
     if (nk > 0) {
-        for (int kt = 0; kt < 3 && kt < nk; kt++) bring(kt);
-        if (nk >= 3) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        bring(0);
+        bring(kStage);
+        if (nk > 2) bring(2 * kStage);
+        if (nk > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * T::kLoads) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();
         Frags f0, f1;
-        fetch(0, f0);
-        for (int kt = 0; kt < nk; kt += 2) {  // behind the last block a stage is read again, for nothing
-            wait(kt);
-            if (kt + 3 < nk) bring(kt + 3);
-            fetch(kt + 1, f1);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(f0);
-            wait(kt + 1);
-            if (kt + 4 < nk) bring(kt + 4);
-            fetch(kt + 2, f0);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(f1);
+        uint32_t here = 0;  // the stage of block kt
+        auto after = [](uint32_t stage) { return stage == 2 * kStage ? 0u : stage + kStage; };
+        if (works) {
+            fetch(0, f0);
+            for (int kt = 0; kt < nk; kt += 2) {  // behind the last block a stage is read again, for nothing
+                const uint32_t next = after(here), next2 = after(next);
+                wait(kt);
+                if (kt + 3 < nk) bring(here);
+                fetch(next, f1);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(f0);
+                wait(kt + 1);
+                if (kt + 4 < nk) bring(next);
+                fetch(next2, f0);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(f1);
+                here = next2;
+            }
+        } else {
+            for (int kt = 0; kt < nk; kt++) {
+                wait(kt);
+                if (kt + 3 < nk) bring(here);
+                here = after(here);
+            }
         }
     }
+    if (!works) return;
 
     // what the results need is computed behind the products, whose registers it would take
     int at = lane;
     asm volatile("" : "+v"(at)::"memory");
-    const int64_t m0 = (int64_t)tm * kTile + 128 * wm, n0 = (int64_t)tn * kTile + 64 * wn;
     if constexpr (WHAT == MM_Z) {
         z_out(p, acc, m0, n0, at);
     } else if constexpr (WHAT == MM_GX) {
@@ -286,35 +328,58 @@ __global__ __launch_bounds__(kMmB, 2) void k_vl_product(MmArgs p) {
         float *out = p.out + m1 * p.D + d;
         const bool in0 = d < p.D, in1 = d + 32 < p.D;
         const int ed0 = piece_exponent(in0 ? p.most_b[d] : 0.0f), ed1 = piece_exponent(in1 ? p.most_b[d + 32] : 0.0f);
-        auto put = [&](float *o, float v, int e) {
-            v = __builtin_amdgcn_ldexpf(v, e);
-            *o = p.acc ? fma_(v, c, *o) : v * c;
-        };
+        // the old values of 16 rows are asked for together
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4; i++) {
+            float old[2][16];
+            if (p.acc) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int dm = 32 * i + 8 * (r / 4) + r % 4;
+                    const float *o = out + (int64_t)dm * p.D;
+                    old[0][r] = m1 + dm < p.V && in0 ? o[0] : 0.0f;
+                    old[1][r] = m1 + dm < p.V && in1 ? o[32] : 0.0f;
+                }
+            }
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int dm = 32 * i + 8 * (r / 4) + r % 4;
                 if (m1 + dm >= p.V) continue;
                 const int em = piece_exponent(p.most_a[m1 + dm]);
                 float *o = out + (int64_t)dm * p.D;
-                if (in0) put(o, acc[i][0][r], ed0 + em);
-                if (in1) put(o + 32, acc[i][1][r], ed1 + em);
+                const float v0 = __builtin_amdgcn_ldexpf(acc[i][0][r], ed0 + em), v1 = __builtin_amdgcn_ldexpf(acc[i][1][r], ed1 + em);
+                if (in0) o[0] = p.acc ? fma_(v0, c, old[0][r]) : v0 * c;
+                if (in1) o[32] = p.acc ? fma_(v1, c, old[1][r]) : v1 * c;
             }
+        }
     }
 }
 
 // ---- which rows count ----------------------------------------------------------------------------------------------------
-// Lists the rows that count and their labels (-1 behind the last), and looks for the first label that is neither a word nor `ignore`.
-__global__ __launch_bounds__(1024) void k_vl_list(const int32_t *__restrict__ labels, int64_t N, int64_t padded, int64_t V, int32_t ignore,
-                                                  VlHead *head, int32_t *__restrict__ from, int32_t *__restrict__ list, unsigned long long *bad) {
-    constexpr int kWaves = 1024 / kWave;
+// Workgroup 0 lists the rows that count and their labels (-1 behind the last), and looks for the first label that is neither a word
+// nor `ignore`; the others clear what starts at zero: `zeros`, the losses and gradients of the rows that do not count.
+__global__ __launch_bounds__(1024) void k_vl_begin(const int32_t *__restrict__ labels, int64_t N, int64_t padded, int64_t D, int64_t V,
+                                                   int32_t ignore, VlHead *head, int32_t *__restrict__ from, int32_t *__restrict__ list,
+                                                   unsigned long long *bad, float *__restrict__ zeros, int64_t n_zeros,
+                                                   float *__restrict__ row_loss, float *__restrict__ gx) {
+    constexpr int kB = 1024, kWaves = kB / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    if (blockIdx.x > 0) {
+        const int64_t block = blockIdx.x - 1, blocks = gridDim.x - 1;
+        for (int64_t i = block * kB + threadIdx.x; i < n_zeros; i += blocks * kB) zeros[i] = 0.0f;
+        for (int64_t i = block * kWaves + wave; i < N; i += blocks * kWaves) {
+            if (vl_counts(labels[i], ignore, V)) continue;
+            if (row_loss && lane == 0) row_loss[i] = 0.0f;
+            if (gx)
+                for (int64_t d = lane; d < D; d += kWave) gx[i * D + d] = 0.0f;
+        }
+        return;
+    }
     __shared__ unsigned long long shk[kWaves];
     __shared__ int shn[kWaves];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     unsigned long long k = ~0ull;
     int64_t count = 0;
-    for (int64_t i0 = 0; i0 < N; i0 += 1024) {
+    for (int64_t i0 = 0; i0 < N; i0 += kB) {
         const int64_t i = i0 + threadIdx.x;
         const int32_t l = i < N ? labels[i] : ignore;
         const bool on = i < N && vl_counts(l, ignore, V);
@@ -334,7 +399,7 @@ __global__ __launch_bounds__(1024) void k_vl_list(const int32_t *__restrict__ la
             list[at] = l;
         }
     }
-    for (int64_t i = count + threadIdx.x; i < padded; i += 1024) {
+    for (int64_t i = count + threadIdx.x; i < padded; i += kB) {
         from[i] = -1;
         list[i] = -1;
     }
@@ -349,116 +414,152 @@ __global__ __launch_bounds__(1024) void k_vl_list(const int32_t *__restrict__ la
     }
 }
 
-// no loss and no gradient for the rows that do not count
-__global__ __launch_bounds__(kVlB) void k_vl_off(const int32_t *__restrict__ labels, int64_t N, int64_t D, int64_t V, int32_t ignore,
-                                                 float *__restrict__ row_loss, float *__restrict__ gx) {
-    for (int64_t i = blockIdx.x; i < N; i += gridDim.x) {
-        if (vl_counts(labels[i], ignore, V)) continue;
-        if (row_loss && threadIdx.x == 0) row_loss[i] = 0.0f;
-        if (gx)
-            for (int64_t d = threadIdx.x; d < D; d += kVlB) gx[i * D + d] = 0.0f;
-    }
-}
-
-__global__ __launch_bounds__(kVlB) void k_vl_clear(float *__restrict__ p, int64_t n) {
-    for (int64_t i = (int64_t)blockIdx.x * kVlB + threadIdx.x; i < n; i += (int64_t)gridDim.x * kVlB) p[i] = 0.0f;
-}
-
 // ---- operands in pieces ----------------------------------------------------------------------------------------------------
+// A matrix to be packed by its rows (summed over by columns) and, where `turned` is set, by its columns.
 struct PackArgs {
     const float *s;
     int64_t ld, rows, cols;
     const int32_t *from;  // the rows' places, or none: as they lie
     const VlHead *head;   // counts the rows where they are listed
-    char *out;
-    int64_t step;         // bytes from a row block to the next
-    int kblocks;
-    int *e;               // by rows: their exponents
-    int64_t slice;        // rows of a workgroup that looks for the columns' largest
-    float *most;          // by columns: their largest sizes
+    int *e;               // the rows' exponents
+    float *most;          // the columns' largest sizes, or none
+    float *group_most;    // of each group of rows, [groups][padded columns]
+    char *by_rows, *by_columns;  // by_columns: or none
+    int64_t step, step_c;  // bytes from a block of 32 rows (columns) to the next
+    int64_t padded;       // rows, padded
+    int blocks;           // of 32 rows that a workgroup looks at for their sizes
+    int groups;           // workgroups that look at sizes
+    int regions;          // of 64 columns
+    bool as_registers;    // the k of by_columns in the order that z's registers have
+};
+struct PackPair {
+    PackArgs a[2];  // x, W
 };
 
-// A workgroup's 32 rows, summed over by columns: each row's exponent, then its pieces.
-__global__ __launch_bounds__(kVlB) void k_vl_pack_rows(PackArgs p) {
-    __shared__ float sh[kVlB / 32][32];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, half = lane >> 5;
-    const int64_t rb = blockIdx.x, r = rb * 32 + (lane & 31);
-    const int64_t rows = p.from ? p.head->count : p.rows;
-    const bool on = r < rows;
-    const float *row = p.s + (on ? (p.from ? (int64_t)p.from[r] : r) : 0) * p.ld;
-    auto load = [&](int kb, float (&x)[8]) {
-        const int64_t k = 16 * (int64_t)kb + 8 * half;
+__device__ __forceinline__ int64_t row_count(const PackArgs &p) { return p.from ? p.head->count : p.rows; }
+
+// The largest sizes of rows and columns: a wave takes 256 columns at a time and goes down its workgroup's rows.
+__global__ __launch_bounds__(kVlB) void k_vl_sizes(PackPair pp) {
+    __shared__ float sh[kVlB / kWave][32 * kSizeBlocks];
+    const bool second = (int)blockIdx.x >= pp.a[0].groups;
+    const PackArgs &p = pp.a[second];
+    const int64_t group = blockIdx.x - (second ? pp.a[0].groups : 0), first = group * p.blocks * 32;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, all = p.blocks * 32;
+    const int64_t rows = row_count(p);
+    const int here = (int)max(int64_t(0), min((int64_t)all, rows - first));
+    for (int i = lane; i < all; i += kWave) sh[wave][i] = 0.0f;
+    for (int64_t c0 = wave * 256; c0 < p.cols; c0 += kVlB / kWave * 256) {
+        const int64_t c = c0 + 4 * lane;
+        f4 most = {};
+        for (int r = 0; r < here; r += 8) {
+            f4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                v[u] = f4{};
+                if (r + u < here && c < p.cols) {
+                    const float *row = p.s + (p.from ? (int64_t)p.from[first + r + u] : first + r + u) * p.ld + c;
+                    if (c + 4 <= p.cols) v[u] = *(const f4u *)row;
+                    else
+                        for (int e = 0; e < (int)(p.cols - c); e++) v[u][e] = row[e];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                float m = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float x = finite_abs(v[u][e]);
+                    most[e] = __builtin_fmaxf(most[e], x);
+                    m = __builtin_fmaxf(m, x);
+                }
+                m = wave_max_nan_skip(m);
+                if (lane == 0) sh[wave][r + u] = __builtin_fmaxf(sh[wave][r + u], m);
+            }
+        }
+        if (p.most && c < p.cols) *(f4 *)(p.group_most + group * p.step / 32 + c) = most;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < all && first + i < p.padded; i += kVlB) {
+        float m = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kVlB / kWave; w++) m = __builtin_fmaxf(m, sh[w][i]);
+        p.e[first + i] = piece_exponent(m);
+    }
+}
+
+// The columns' largest sizes of all groups: 64 columns a workgroup, 16 lanes each.
+__global__ __launch_bounds__(1024) void k_vl_sizes_join(PackPair pp) {
+    __shared__ float sh[16][64];
+    const PackArgs &p = pp.a[blockIdx.y];
+    if (!p.most) return;
+    const int col = threadIdx.x & 63, sub = threadIdx.x / 64;
+    const int64_t d = (int64_t)blockIdx.x * 64 + col;
+    float m = 0.0f;
+    if (d < p.cols)
+#pragma unroll 8
+        for (int g = sub; g < p.groups; g += 16) m = __builtin_fmaxf(m, p.group_most[g * (p.step / 32) + d]);
+    sh[sub][col] = m;
+    __syncthreads();
+    if (sub == 0 && d < p.cols) {
+#pragma unroll
+        for (int i = 1; i < 16; i++) m = __builtin_fmaxf(m, sh[i][col]);
+        p.most[d] = m;
+    }
+}
+
+// A region of 64 rows by kPackCols columns in pieces: by rows, then by columns (the caches have it by then).
+__global__ __launch_bounds__(kVlB) void k_vl_pack(PackPair pp) {
+    const int64_t of_first = pp.a[0].padded / 64 * pp.a[0].regions;
+    const bool second = (int64_t)blockIdx.x >= of_first;
+    const PackArgs &p = pp.a[second];
+    const uint32_t id = (uint32_t)(blockIdx.x - (second ? of_first : 0));
+    const int64_t r0 = (int64_t)(id / (uint32_t)p.regions) * 64, c0 = (int64_t)(id % (uint32_t)p.regions) * kPackCols;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, half = lane >> 5, col = lane & 31;
+    const int64_t rows = row_count(p);
+    auto store = [&](char *o, const Pieces &c) {
+        *(h8 *)(o + lane * 16) = c.hi;
+        *(h8 *)(o + lane * 16 + 1024) = c.lo;
+    };
+    constexpr int kTasks = 2 * kPackCols / 16;  // of either kind
+#pragma unroll 2
+    for (int t = wave; t < kTasks; t += kVlB / kWave) {
+        const int64_t r = r0 + 32 * (t & 1) + col, k = c0 + 16 * (t >> 1) + 8 * half;
+        if (c0 + 16 * (t >> 1) >= p.step / 128) continue;  // behind the padded columns
+        float x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = 0.0f;
-        if (!on || k >= p.cols) return;
-        if (k + 8 <= p.cols) {
-            const f4 a = *(const f4u *)(row + k), b = *(const f4u *)(row + k + 4);
+        if (r < rows && k < p.cols) {
+            const float *row = p.s + (p.from ? (int64_t)p.from[r] : r) * p.ld + k;
+            if (k + 8 <= p.cols) {
+                const f4 a = *(const f4u *)row, b = *(const f4u *)(row + 4);
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = a[e], x[4 + e] = b[e];
-        } else {
+                for (int e = 0; e < 4; e++) x[e] = a[e], x[4 + e] = b[e];
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (k + e < p.cols) x[e] = row[k + e];
+                for (int e = 0; e < 8; e++)
+                    if (k + e < p.cols) x[e] = row[e];
+            }
         }
-    };
-    float most = 0.0f, x[8];
-    for (int kb = wave; kb < p.kblocks; kb += kVlB / kWave) {
-        load(kb, x);
-#pragma unroll
-        for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[e]));
+        store(p.by_rows + (r0 / 32 + (t & 1)) * p.step + (c0 / 16 + (t >> 1)) * 2048, cut(x, power(-p.e[r])));
     }
-    sh[threadIdx.x / 32][lane & 31] = most;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kVlB / 32; i++) most = __builtin_fmaxf(most, sh[i][lane & 31]);
-    const int ex = piece_exponent(most);
-    if (threadIdx.x < 32) p.e[r] = ex;
-    const float scale = power(-ex);
-    for (int kb = wave; kb < p.kblocks; kb += kVlB / kWave) {
-        load(kb, x);
-        const Pieces c = cut(x, scale);
-        char *o = p.out + rb * p.step + (int64_t)kb * 2048 + lane * 16;
-        *(h8 *)o = c.hi;
-        *(h8 *)(o + 1024) = c.lo;
-    }
-}
-
-// the columns' largest sizes
-__global__ __launch_bounds__(kVlB) void k_vl_most(PackArgs p) {
-    const int64_t d = (int64_t)blockIdx.x * kVlB + threadIdx.x;
-    const int64_t rows = p.from ? p.head->count : p.rows;
-    const int64_t r0 = (int64_t)blockIdx.y * p.slice, r1 = min(rows, r0 + p.slice);
-    if (d >= p.cols || r0 >= r1) return;
-    float most = 0.0f;
-    for (int64_t r = r0; r < r1; r++) most = __builtin_fmaxf(most, finite_abs(p.s[(p.from ? (int64_t)p.from[r] : r) * p.ld + d]));
-    atomicMax((unsigned int *)p.most + d, __float_as_uint(most));
-}
-
-// Columns as rows, summed over by rows; a wave's block of 32 columns by 16 rows.  TURNED: the k in the order that z's registers have.
-template <bool TURNED>
-__global__ __launch_bounds__(kVlB) void k_vl_pack_columns(PackArgs p) {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, half = lane >> 5;
-    const int64_t db = (int64_t)blockIdx.y * (kVlB / kWave) + wave, d = db * 32 + (lane & 31);
-    const int64_t rows = p.from ? p.head->count : p.rows;
-    if (db * 32 >= p.cols) return;
-    const float scale = d < p.cols ? power(-piece_exponent(p.most[d])) : 0.0f;
-    for (int kb = blockIdx.x; kb < p.kblocks; kb += gridDim.x) {
+    if (!p.by_columns) return;
+#pragma unroll 2
+    for (int t = wave; t < kTasks; t += kVlB / kWave) {
+        const int64_t kb = r0 / 16 + (t & 3), db = c0 / 32 + (t >> 2), d = db * 32 + col;
+        if (db * 32 >= p.cols) continue;
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const int64_t k = 16 * (int64_t)kb + (TURNED ? 4 * half + (e & 3) + 8 * (e >> 2) : 8 * half + e);
+            const int64_t k = 16 * kb + (p.as_registers ? 4 * half + (e & 3) + 8 * (e >> 2) : 8 * half + e);
             x[e] = d < p.cols && k < rows ? p.s[(p.from ? (int64_t)p.from[k] : k) * p.ld + d] : 0.0f;
         }
-        const Pieces c = cut(x, scale);
-        char *o = p.out + db * p.step + (int64_t)kb * 2048 + lane * 16;
-        *(h8 *)o = c.hi;
-        *(h8 *)(o + 1024) = c.lo;
+        store(p.by_columns + db * p.step_c + kb * 2048, cut(x, d < p.cols ? power(-piece_exponent(p.most[d])) : 0.0f));
     }
 }
 
 // ---- the rows' statistics and G ---------------------------------------------------------------------------------------------
 struct GradArgs {
-    const VlHead *head;
+    VlHead *head;
     int64_t row0, rows;  // of this piece: the first, how many (padded)
     int64_t V, words;    // words, padded
     const f2 *part;
@@ -471,25 +572,33 @@ struct GradArgs {
     char *turned;
     int64_t turned_step;
     float *most;         // of every word of this piece
-    double *column;      // [slices][words], or none
-    int slices;
+    float *column;       // [rows / 32][words], or none
+    int slices;          // of the rows where the words' largest are looked for
+    int tiles_n, slices_most, at_once;  // of gx: tiles over the columns, parts at most, workgroups that the chip holds
 };
 
-// lanes over 32 rows, eight of them over the partial statistics of each
-__global__ __launch_bounds__(kVlB) void k_vl_stats(GradArgs p) {
-    __shared__ double sh[kVlB / 32][32];
-    __shared__ float shm[kVlB / 32][32];
+// lanes over 32 rows, 32 of them over the partial statistics of each; and what the next steps of this piece need
+__global__ __launch_bounds__(1024) void k_vl_stats(GradArgs p) {
+    constexpr int kSubs = 1024 / 32;
+    __shared__ double sh[kSubs][32];
+    __shared__ float shm[kSubs][32];
+    if (p.most && p.row0 > 0)  // the first piece finds them clear
+        for (int64_t v = (int64_t)blockIdx.x * 1024 + threadIdx.x; v < p.words; v += (int64_t)gridDim.x * 1024) p.most[v] = 0.0f;
+    const int64_t left = p.head->count - p.row0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.head->slices = gx_slices(min(p.rows, left), p.tiles_n, (int)(p.words / 16), p.slices_most, p.at_once);
     const int sub = threadIdx.x / 32, col = threadIdx.x & 31;
     const int64_t n = (int64_t)blockIdx.x * 32 + col;
     const int64_t parts = p.words / kStatWords;
     float m = -__builtin_inff();
-    for (int64_t i = sub; i < parts; i += kVlB / 32) m = __builtin_fmaxf(m, p.part[i * p.rows + n].x);
+#pragma unroll 4
+    for (int64_t i = sub; i < parts; i += kSubs) m = __builtin_fmaxf(m, p.part[i * p.rows + n].x);
     shm[sub][col] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kVlB / 32; i++) m = __builtin_fmaxf(m, shm[i][col]);
+    for (int i = 0; i < kSubs; i++) m = __builtin_fmaxf(m, shm[i][col]);
     double s = 0.0;
-    for (int64_t i = sub; i < parts; i += kVlB / 32) {
+#pragma unroll 4
+    for (int64_t i = sub; i < parts; i += kSubs) {
         const f2 v = p.part[i * p.rows + n];
         s += (double)v.y * (double)(v.x == m ? 1.0f : exp8_nonpos(v.x - m));
     }
@@ -498,10 +607,10 @@ __global__ __launch_bounds__(kVlB) void k_vl_stats(GradArgs p) {
     if (sub != 0) return;
     double others = 0.0;
 #pragma unroll
-    for (int i = 0; i < kVlB / 32; i++) others += sh[i][col];
+    for (int i = 0; i < kSubs; i++) others += sh[i][col];
     const int label = p.labels[n];
     VlRow row = {0.0f, 0.0f, 0.0f, -1};
-    if (p.row0 + n < p.head->count) {
+    if (n < left) {
         const float zl = p.label_z[n] - m;
         const double total = others + (double)exp8_nonpos(zl);
         const double ls = zl == 0.0f ? log1p(others) : log(total), loss = ls - (double)zl;
@@ -518,19 +627,15 @@ __device__ __forceinline__ float g_entry(float z, int64_t v, const VlRow &row) {
     return v == row.label ? row.own : p;
 }
 
-// Every word's largest entry of G in this piece and, SUM, the sum of them.  A wave takes 32 words and goes over its slice of the rows.
-template <bool SUM>
+// Every word's largest entry of G in this piece.  A wave takes 32 words and goes over its slice of the rows.
 __global__ __launch_bounds__(kVlB) void k_vl_words(GradArgs p) {
     const int lane = threadIdx.x & (kWave - 1), half = lane >> 5;
     const int64_t vb = (int64_t)blockIdx.x * (kVlB / kWave) + threadIdx.x / kWave, zwords = p.words / 32;
     const int64_t left = min(p.rows, p.head->count - p.row0), blocks = left > 0 ? (left + 31) / 32 : 0;
     const int64_t b0 = blocks * blockIdx.y / p.slices, b1 = blocks * (blockIdx.y + 1) / p.slices;
-    float most[16];
-    double sum[SUM ? 16 : 1];
+    float most[16];  // logarithms: the exponential of the largest is the largest
 #pragma unroll
     for (int r = 0; r < 16; r++) most[r] = -__builtin_inff();
-#pragma unroll
-    for (int r = 0; r < (SUM ? 16 : 1); r++) sum[r] = 0.0;
     for (int64_t nb = b0; nb < b1; nb++) {
         const VlRow row = p.row[nb * 32 + (lane & 31)];
         const float *z = p.z + (nb * zwords + vb) * 1024 + lane * 4;
@@ -540,15 +645,8 @@ __global__ __launch_bounds__(kVlB) void k_vl_words(GradArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const bool own = vb * 32 + 8 * q + 4 * half + e == row.label;
-                if constexpr (SUM) {
-                    const float g = row.label < 0 ? 0.0f : g_entry(v[e], vb * 32 + 8 * q + 4 * half + e, row);
-                    most[4 * q + e] = __builtin_fmaxf(most[4 * q + e], __builtin_fabsf(g));
-                    sum[4 * q + e] += (double)g;
-                } else {
-                    // logarithms: the exponential of the largest is the largest
-                    const float t = own ? 0.0f : (v[e] - row.m) - row.ls;
-                    most[4 * q + e] = __builtin_fmaxf(most[4 * q + e], row.label < 0 ? -__builtin_inff() : t);
-                }
+                const float t = own ? 0.0f : (v[e] - row.m) - row.ls;
+                most[4 * q + e] = __builtin_fmaxf(most[4 * q + e], row.label < 0 ? -__builtin_inff() : t);
             }
         }
     }
@@ -561,29 +659,24 @@ __global__ __launch_bounds__(kVlB) void k_vl_words(GradArgs p) {
         m = __builtin_fmaxf(m, __shfl_xor(m, 8));
         m = __builtin_fmaxf(m, __shfl_xor(m, 16));
         const int64_t v = vb * 32 + 8 * (r / 4) + 4 * half + r % 4;
-        if (!SUM) m = exp8_nonpos(m);
-        else m = m > 0.0f ? m : 0.0f;
-        if ((lane & 31) == 0) atomicMax((unsigned int *)p.most + v, __float_as_uint(m));
-        if constexpr (SUM) {
-            double s = sum[r];
-            for (int d = 1; d < 32; d *= 2) s += __shfl_xor(s, d);
-            if ((lane & 31) == 0) p.column[(int64_t)blockIdx.y * p.words + v] = s;
-        }
+        if ((lane & 31) == 0) atomicMax((unsigned int *)p.most + v, __float_as_uint(exp8_nonpos(m)));
     }
 }
 
-// gb (+)= the slices' sums
-__global__ __launch_bounds__(kVlB) void k_vl_bias(const double *__restrict__ column, int slices, int64_t words, int64_t V, const VlHead *head,
-                                                  const float *gout, int sum, float *__restrict__ gb, int acc) {
+// gb (+)= the sums of the columns of G, which k_vl_grad left for every 32 rows
+__global__ __launch_bounds__(kVlB) void k_vl_bias(GradArgs p, const float *gout, int sum, float *__restrict__ gb, int acc) {
     const int64_t v = (int64_t)blockIdx.x * kVlB + threadIdx.x;
-    if (v >= V) return;
+    if (v >= p.V) return;
+    const int64_t left = min(p.rows, p.head->count - p.row0), blocks = left > 0 ? (left + 31) / 32 : 0;
     double s = 0.0;
-    for (int i = 0; i < slices; i++) s += column[(int64_t)i * words + v];
-    const float c = vl_coef(head, gout, sum);
-    gb[v] = head->count == 0 ? (acc ? gb[v] : 0.0f) : (acc ? fma_((float)s, c, gb[v]) : (float)s * c);
+#pragma unroll 8
+    for (int64_t i = 0; i < blocks; i++) s += (double)p.column[i * p.words + v];
+    const float c = blocks ? vl_coef(p.head, gout, sum) : 0.0f;
+    gb[v] = acc ? fma_((float)s, c, gb[v]) : (float)s * c;
 }
 
-// G of a block of 32 rows by 32 words, in pieces: under the rows' exponents in z's place (X), and turned, under the words' (W).
+// G of a block of 32 rows by 32 words, in pieces: under the rows' exponents in z's place (X), and turned, under the words' (W),
+// with the sums of its columns where gb wants them.
 template <bool X, bool W>
 __global__ __launch_bounds__(kVlB) void k_vl_grad(GradArgs p) {
     __shared__ float turn[W ? kVlB / kWave : 1][32][33];
@@ -620,25 +713,31 @@ __global__ __launch_bounds__(kVlB) void k_vl_grad(GradArgs p) {
         // the wave's own part of LDS: it reads what it wrote
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         const float scale = power(-piece_exponent(p.most[vb * 32 + col]));
+        float sum = 0.0f;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = turn[wave][col][16 * s + 8 * half + e];
+            for (int e = 0; e < 8; e++) sum += x[e] = turn[wave][col][16 * s + 8 * half + e];
             const Pieces c = cut(x, scale);
             char *o = p.turned + vb * p.turned_step + (nb * 2 + s) * 2048 + lane * 16;
             *(h8 *)o = c.hi;
             *(h8 *)(o + 1024) = c.lo;
         }
+        if (p.column) {
+            sum += __shfl_xor(sum, 32);
+            if (half == 0) p.column[nb * p.words + vb * 32 + col] = sum;
+        }
     }
 }
 
 // gx (+)= the parts' sum, at the rows' places
-__global__ __launch_bounds__(kVlB) void k_vl_gx(const float *__restrict__ parts, int slices, int64_t rows, int64_t cols, const VlHead *head,
+__global__ __launch_bounds__(kVlB) void k_vl_gx(const float *__restrict__ parts, int64_t rows, int64_t cols, const VlHead *head,
                                                 int64_t row0, const int32_t *__restrict__ from, const VlRow *__restrict__ row,
                                                 const float *__restrict__ most, int64_t D, const float *gout, int sum, float *__restrict__ gx,
                                                 int acc) {
     const int64_t left = min(rows, head->count - row0);
+    const int slices = head->slices;
     const float c = vl_coef(head, gout, sum);
     for (int64_t n = blockIdx.x; n < left; n += gridDim.x) {
         const int en = piece_exponent(finite_abs(row[n].own));
@@ -667,22 +766,23 @@ struct SplitPlan {
     int64_t n, d, v;   // rows, columns and words, padded to tiles
     int64_t dk;        // columns, padded to two blocks of k
     int64_t piece;     // rows of a piece, padded
-    int slices;        // of the words in gx
-    int columns;       // slices of the rows in gb and the words' largest
-    size_t from, list, losses, row, label_z, part, ew, ex, most_w, most_x, most_g, column, x1, x3, w1, w2, z, turned, parts, total;
+    int slices;        // of the words in gx, at most
+    int columns;       // slices of the rows where the words' largest are looked for
+    size_t from, list, losses, row, label_z, part, ew, ex, most_w, most_x, most_g, group_w, group_x, column, x1, x3, w1, w2, z, turned, parts, total;
 };
 
 static int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
+// row blocks of a group: some 1024 groups
+static int size_blocks(int64_t padded) { return (int)std::max<int64_t>(1, std::min<int64_t>(kSizeBlocks, padded / 32 / 1024)); }
+
 static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w, bool want_b) {
     SplitPlan p{};
     const bool grad = want_x || want_w || want_b;
-    p.n = up_to(N, kTile), p.d = up_to(D, kTile), p.v = up_to(V, kTile), p.dk = up_to(D, 32);
+    p.n = up_to(N, kTileM), p.d = up_to(D, kTileMost), p.v = up_to(V, kTileM), p.dk = up_to(D, 32);
     const int64_t most = grad ? kZBytes / (8 * p.v) : kScored / p.v;
-    p.piece = std::max<int64_t>(kTile, std::min(std::min(p.n, kPieceRows), most / kTile * kTile));
-    // enough parts of gx for four rounds of workgroups, none with fewer than 64 blocks of k
-    const int64_t tiles = p.piece / kTile * (p.d / kTile);
-    p.slices = (int)std::max<int64_t>(1, std::min((4 * kPlanCUs + tiles - 1) / tiles, p.v / 16 / 64));
+    p.piece = std::max<int64_t>(kTileM, std::min(std::min(p.n, kPieceRows), most / kTileM * kTileM));
+    p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(64, kPartBytes / (p.piece * p.d * 4)));
     p.columns = (int)std::max<int64_t>(1, std::min(p.piece / 32, (4096 + p.v / 32 - 1) / (p.v / 32)));
     size_t at = 256;
     auto take = [&](bool wanted, int64_t bytes) {
@@ -701,13 +801,15 @@ static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool w
     p.most_w = take(want_x, p.d * 4);
     p.most_x = take(want_w, p.d * 4);
     p.most_g = take(want_w || want_b, p.v * 4);
-    p.column = take(want_b, p.columns * p.v * 8);
+    p.group_w = take(want_x, (p.v / 32 / size_blocks(p.v) + 1) * p.dk * 4);
+    p.group_x = take(want_w, (p.n / 32 / size_blocks(p.n) + 1) * p.dk * 4);
+    p.column = take(want_b, p.piece / 32 * p.v * 4);
     p.x1 = take(true, p.n * p.dk * 4);
     p.x3 = take(want_w, p.d * p.n * 4);
     p.w1 = take(true, p.v * p.dk * 4);
     p.w2 = take(want_x, p.d * p.v * 4);
     p.z = take(grad, p.piece * p.v * 4);
-    p.turned = take(want_w, p.piece * p.v * 4);
+    p.turned = take(want_w || want_b, p.piece * p.v * 4);
     p.parts = take(want_x, p.slices * p.piece * p.d * 4);
     p.total = at;
     return p;
@@ -722,6 +824,15 @@ size_t vl_split_workspace(int64_t N, int64_t D, int64_t V, bool want_x, bool wan
     return split_plan(N, D, V, want_x, want_w, want_b).total;
 }
 
+// Whether a product runs on tiles of 256 columns.  z and gW: unless tiles of 128, two a CU, take fewer rounds, by more than the
+// 4% that they are slower at the same number (gW of 128000 x 4096 x 2048: 5.5 ms, 6.3 with tiles of 128; 50021 x 700 x 770: 257 us, 239).
+// gx, whose words are cut to fill the rounds: where more than 128 columns are there.
+static bool wide_tiles(int64_t tiles_m, int64_t cols, bool cut) {
+    if (cut) return cols > 128;
+    const int64_t wide = tiles_m * ((cols + 255) / 256), narrow = tiles_m * ((cols + 127) / 128);
+    return 25 * ((wide + kPlanCUs - 1) / kPlanCUs) <= 26 * ((narrow + 2 * kPlanCUs - 1) / (2 * kPlanCUs));
+}
+
 int vl_split_run(const VlCall &c, const char *what) {
     const SplitPlan pl = split_plan(c.N, c.D, c.V, c.gx, c.gw, c.gb);
     const bool grad = c.gx || c.gw || c.gb;
@@ -729,78 +840,89 @@ int vl_split_run(const VlCall &c, const char *what) {
     VlHead *head = (VlHead *)c.ws;
     int32_t *from = (int32_t *)at(pl.from), *list = (int32_t *)at(pl.list);
     double *losses = (double *)at(pl.losses);
-    hipLaunchKernelGGL(k_vl_list, 1, 1024, 0, c.st, c.labels, c.N, pl.n, c.V, c.ignore, head, from, list, c.bad);
-    if (c.row_loss || (c.gx && !c.acc_x))
-        hipLaunchKernelGGL(k_vl_off, (unsigned)std::min<int64_t>(c.N, 1 << 14), kVlB, 0, c.st, c.labels, c.N, c.D, c.V, c.ignore, c.row_loss,
-                           c.acc_x ? nullptr : c.gx);
+    float *const gx_off = c.acc_x ? nullptr : c.gx;
+    const int64_t zeros = c.gw || c.gb ? pl.v : 0;
+    const int64_t helpers = std::min<int64_t>(1024, (std::max(zeros / 4, c.row_loss || gx_off ? c.N : 0) + 255) / 256);
+    hipLaunchKernelGGL(k_vl_begin, (unsigned)(1 + helpers), 1024, 0, c.st, c.labels, c.N, pl.n, c.D, c.V, c.ignore, head, from, list, c.bad,
+                       (float *)at(pl.most_g), zeros, c.row_loss, gx_off);
+    PackPair pp{};
+    for (int i = 0; i < 2; i++) {
+        PackArgs &a = pp.a[i];
+        a.s = i ? c.w : c.x, a.ld = i ? c.ldw : c.ldx, a.rows = i ? c.V : c.N, a.cols = c.D, a.from = i ? nullptr : from, a.head = head;
+        a.e = (int *)at(i ? pl.ew : pl.ex);
+        a.by_rows = at(i ? pl.w1 : pl.x1), a.step = pl.dk * 128, a.padded = i ? pl.v : pl.n;
+        if (i ? c.gx : c.gw) {
+            a.most = (float *)at(i ? pl.most_w : pl.most_x);
+            a.by_columns = at(i ? pl.w2 : pl.x3), a.step_c = a.padded * 128, a.as_registers = i == 1;
+        }
+        a.blocks = size_blocks(a.padded);
+        a.groups = (int)((a.padded / 32 + a.blocks - 1) / a.blocks);
+        a.group_most = (float *)at(i ? pl.group_w : pl.group_x);
+        a.regions = (int)((pl.dk + kPackCols - 1) / kPackCols);
+    }
+    hipLaunchKernelGGL(k_vl_sizes, (unsigned)(pp.a[0].groups + pp.a[1].groups), kVlB, 0, c.st, pp);
+    if (c.gx || c.gw) hipLaunchKernelGGL(k_vl_sizes_join, dim3((unsigned)((c.D + 63) / 64), 2), 1024, 0, c.st, pp);
+    hipLaunchKernelGGL(k_vl_pack, (unsigned)((pl.n + pl.v) / 64 * pp.a[0].regions), kVlB, 0, c.st, pp);
 
-    PackArgs x{c.x, c.ldx, c.N, c.D, from, head, at(pl.x1), pl.dk * 128, (int)(pl.dk / 16), (int *)at(pl.ex), 0, nullptr};
-    PackArgs w{c.w, c.ldw, c.V, c.D, nullptr, head, at(pl.w1), pl.dk * 128, (int)(pl.dk / 16), (int *)at(pl.ew), 0, nullptr};
-    hipLaunchKernelGGL(k_vl_pack_rows, (unsigned)(pl.n / 32), kVlB, 0, c.st, x);
-    hipLaunchKernelGGL(k_vl_pack_rows, (unsigned)(pl.v / 32), kVlB, 0, c.st, w);
-    auto columns = [&](PackArgs a, size_t most, size_t out, int64_t k, bool turned) {
-        a.most = (float *)at(most), a.out = at(out), a.step = k * 128, a.kblocks = (int)(k / 16);
-        hipLaunchKernelGGL(k_vl_clear, (unsigned)((pl.d + kVlB - 1) / kVlB), kVlB, 0, c.st, a.most, pl.d);
-        a.slice = std::max<int64_t>(256, (a.rows + 4095) / 4096);
-        const dim3 g1((unsigned)((c.D + kVlB - 1) / kVlB), (unsigned)((a.rows + a.slice - 1) / a.slice));
-        hipLaunchKernelGGL(k_vl_most, g1, kVlB, 0, c.st, a);
-        const dim3 g2((unsigned)std::min<int64_t>(k / 16, 1 << 16), (unsigned)((c.D + 127) / 128));
-        if (turned) hipLaunchKernelGGL(k_vl_pack_columns<true>, g2, kVlB, 0, c.st, a);
-        else hipLaunchKernelGGL(k_vl_pack_columns<false>, g2, kVlB, 0, c.st, a);
+    auto launch = [&](auto kernel, int lanes, int lds, int64_t groups, const MmArgs &m) {
+        (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        hipLaunchKernelGGL(kernel, (unsigned)groups, lanes, lds, c.st, m);
     };
-    if (c.gw) columns(x, pl.most_x, pl.x3, pl.n, false);
-    if (c.gx) columns(w, pl.most_w, pl.w2, pl.v, true);
-
-    auto product = [&](auto kernel, const MmArgs &m) {
-        (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kMmLds);
-        hipLaunchKernelGGL(kernel, (unsigned)(m.tiles_m * m.tiles_n * m.slices), kMmB, kMmLds, c.st, m);
+    auto product = [&](auto what, MmArgs m, int64_t cols, int slices) {
+        constexpr int W = decltype(what)::value;
+        const bool wide = wide_tiles(m.tiles_m, cols, W == MM_GX);
+        m.tiles_n = (int)((cols + (wide ? 255 : 127)) / (wide ? 256 : 128));
+        const int64_t groups = (int64_t)m.tiles_m * m.tiles_n * slices;
+        if (wide) launch(k_vl_product<W, 4>, Tile<4>::kLanes, Tile<4>::kLds, groups, m);
+        else launch(k_vl_product<W, 2>, Tile<2>::kLanes, Tile<2>::kLds, groups, m);
     };
     for (int64_t r0 = 0; r0 < pl.n; r0 += pl.piece) {
         const int64_t rows = std::min(pl.piece, pl.n - r0);
         MmArgs m{};
         m.A = at(pl.w1), m.step_a = pl.dk * 128, m.B = at(pl.x1) + r0 / 32 * (pl.dk * 128), m.step_b = pl.dk * 128;
-        m.tiles_m = (int)(pl.v / kTile), m.tiles_n = (int)(rows / kTile), m.slices = 1, m.kblocks = (int)(pl.dk / 16);
+        m.tiles_m = (int)(pl.v / kTileM), m.kblocks = (int)(pl.dk / 16);
         m.head = head, m.row0 = r0, m.V = c.V, m.D = c.D;
         m.ew = (const int *)at(pl.ew), m.ex = (const int *)at(pl.ex) + r0, m.bias = c.bias, m.labels = list + r0;
         m.z = grad ? (float *)at(pl.z) : nullptr, m.zwords = pl.v / 32, m.part = (f2 *)at(pl.part), m.label_z = (float *)at(pl.label_z);
         m.rows = pl.piece;
-        product(k_vl_product<MM_Z>, m);
+        product(std::integral_constant<int, MM_Z>{}, m, rows, 1);
 
         GradArgs g{};
         g.head = head, g.row0 = r0, g.rows = pl.piece, g.V = c.V, g.words = pl.v, g.part = m.part, g.label_z = m.label_z;
         g.labels = list + r0, g.from = from + r0, g.row = (VlRow *)at(pl.row), g.losses = losses, g.row_loss = c.row_loss;
-        g.z = m.z, g.turned = at(pl.turned), g.turned_step = pl.piece * 128, g.most = (float *)at(pl.most_g), g.column = (double *)at(pl.column);
-        g.slices = pl.columns;
-        hipLaunchKernelGGL(k_vl_stats, (unsigned)(rows / 32), kVlB, 0, c.st, g);
+        g.z = m.z, g.turned = at(pl.turned), g.turned_step = pl.piece * 128, g.most = (float *)at(pl.most_g), g.column = c.gb ? (float *)at(pl.column) : nullptr;
+        g.slices = pl.columns, g.slices_most = pl.slices;
+        const bool wide = wide_tiles(rows / kTileM, c.D, true);
+        g.tiles_n = (int)((c.D + (wide ? 255 : 127)) / (wide ? 256 : 128)), g.at_once = wide ? kPlanCUs : 2 * kPlanCUs;
+        if (!(c.gw || c.gb)) g.most = nullptr;
+        hipLaunchKernelGGL(k_vl_stats, (unsigned)(rows / 32), 1024, 0, c.st, g);
         if (!grad) continue;
         if (c.gw || c.gb) {
-            hipLaunchKernelGGL(k_vl_clear, (unsigned)((pl.v + kVlB - 1) / kVlB), kVlB, 0, c.st, g.most, pl.v);
             const dim3 gw((unsigned)(pl.v / 32 / (kVlB / kWave)), (unsigned)pl.columns);
-            if (c.gb) hipLaunchKernelGGL(k_vl_words<true>, gw, kVlB, 0, c.st, g);
-            else hipLaunchKernelGGL(k_vl_words<false>, gw, kVlB, 0, c.st, g);
-            if (c.gb)
-                hipLaunchKernelGGL(k_vl_bias, (unsigned)((c.V + kVlB - 1) / kVlB), kVlB, 0, c.st, g.column, pl.columns, pl.v, c.V, head, c.gout,
-                                   c.sum, c.gb, c.acc_b || r0);
+            hipLaunchKernelGGL(k_vl_words, gw, kVlB, 0, c.st, g);
         }
         const dim3 gg((unsigned)(pl.v / 32 / (kVlB / kWave)), (unsigned)(rows / 32));
-        if (c.gx && c.gw) hipLaunchKernelGGL((k_vl_grad<true, true>), gg, kVlB, 0, c.st, g);
+        const bool turn = c.gw || c.gb;
+        if (c.gx && turn) hipLaunchKernelGGL((k_vl_grad<true, true>), gg, kVlB, 0, c.st, g);
         else if (c.gx) hipLaunchKernelGGL((k_vl_grad<true, false>), gg, kVlB, 0, c.st, g);
-        else if (c.gw) hipLaunchKernelGGL((k_vl_grad<false, true>), gg, kVlB, 0, c.st, g);
+        else hipLaunchKernelGGL((k_vl_grad<false, true>), gg, kVlB, 0, c.st, g);
+        if (c.gb)
+            hipLaunchKernelGGL(k_vl_bias, (unsigned)((c.V + kVlB - 1) / kVlB), kVlB, 0, c.st, g, c.gout, c.sum, c.gb, c.acc_b || r0);
         if (c.gx) {
             MmArgs a = m;
             a.A = (const char *)m.z, a.step_a = pl.v * 128, a.B = at(pl.w2), a.step_b = pl.v * 128;
-            a.tiles_m = (int)(rows / kTile), a.tiles_n = (int)(pl.d / kTile), a.slices = pl.slices, a.kblocks = (int)(pl.v / 16);
+            a.tiles_m = (int)(rows / kTileM), a.kblocks = (int)(pl.v / 16);
             a.parts = (float *)at(pl.parts), a.cols = pl.d;
-            product(k_vl_product<MM_GX>, a);
-            hipLaunchKernelGGL(k_vl_gx, (unsigned)std::min<int64_t>(rows, 1 << 14), kVlB, 0, c.st, a.parts, pl.slices, pl.piece, pl.d, head, r0,
+            product(std::integral_constant<int, MM_GX>{}, a, c.D, pl.slices);
+            hipLaunchKernelGGL(k_vl_gx, (unsigned)std::min<int64_t>(rows, 1 << 14), kVlB, 0, c.st, a.parts, pl.piece, pl.d, head, r0,
                                from + r0, g.row, (const float *)at(pl.most_w), c.D, c.gout, c.sum, c.gx, c.acc_x);
         }
         if (c.gw) {
             MmArgs a = m;
             a.A = g.turned, a.step_a = g.turned_step, a.B = at(pl.x3) + r0 / 16 * 2048, a.step_b = pl.n * 128;
-            a.tiles_m = (int)(pl.v / kTile), a.tiles_n = (int)(pl.d / kTile), a.kblocks = (int)(rows / 16);
+            a.tiles_m = (int)(pl.v / kTileM), a.kblocks = (int)(rows / 16);
             a.most_a = g.most, a.most_b = (const float *)at(pl.most_x), a.gout = c.gout, a.out = c.gw, a.sum = c.sum, a.acc = c.acc_w || r0;
-            product(k_vl_product<MM_GW>, a);
+            product(std::integral_constant<int, MM_GW>{}, a, c.D, 1);
         }
     }
     hipLaunchKernelGGL(k_vl_total, 1, 1024, 0, c.st, losses, head, c.sum, c.loss);
