@@ -1,7 +1,7 @@
 // Rows of a table looked up by token and scaled, and the table's gradient: y[i] = s W[t_i], gW[v] (+)= s sum over t_i = v of g[i].  No
 // counterpart in the reference on the device (its index_select copies rows on the host).
 //
-// The gradient sums in a fixed order without atomics.  Positions are sorted by (token, position); blocks of kSortedBlock sorted
+// The gradient sums in a fixed order without atomics.  Positions are sorted by (token, position); blocks of 8 or 32 sorted
 // positions are summed by a lane for every four columns.  A token whose positions lie within one block has its row written there; one
 // that goes over blocks leaves a part with each (at most two a block: one of a token that began before it, one of a token that goes on
 // behind it), which a second kernel adds in the blocks' order, in fp64.  Rows of tokens that do not occur are cleared by workgroups of
@@ -15,9 +15,10 @@
 namespace nchip {
 
 constexpr int kEmbB = 256;
-constexpr int kSortedBlock = 32;  // sorted positions that one workgroup's lane sums
 constexpr int kClearRows = 32;    // rows of the table that one workgroup clears, or as many as it has side by side
-constexpr int kRankB = 1024, kRankWaves = kRankB / kWave;
+constexpr int kRankB = 1024, kRankMost = 8192;  // tokens whose places are counted, at most
+constexpr int kDigitBits = 10, kChunk = 1024;   // of the others' sort
+constexpr int kSumChunks = 256;  // chunks whose counts each workgroup adds up itself, at most; more are summed by a launch of its own
 constexpr int64_t kMaxTokens = int64_t(1) << 30;
 constexpr int64_t kMaxRows = int64_t(1) << 31;
 
@@ -93,28 +94,175 @@ __global__ __launch_bounds__(1024) void k_embed_check(const int32_t *__restrict_
 }
 
 // ---- the order of the positions -----------------------------------------------------------------------------
-// A position's place is the number of those before it: tokens that are less, and equal ones at earlier positions.  A workgroup
-// counts for 64 positions, a sixteenth of all tokens in each wave.  Tokens compare as unsigned, so those in the table come first.
-__global__ __launch_bounds__(kRankB) void k_embed_rank(const uint32_t *__restrict__ tokens, int N, uint32_t *__restrict__ sorted,
+// A position's place is the number of those that come before it by (token, position).  Tokens compare as unsigned, so those outside the
+// table come last, in whatever order.
+//
+// Few tokens: every place by counting, in one launch.  A workgroup has 32 positions, all tokens in LDS, and counts with each half of its
+// 16 waves over a thirty-second of them: 8192 tokens take two instructions a pair, 7 us.
+__device__ __forceinline__ uint32_t sort_key(int32_t t) { return min((uint32_t)t, 0xfffffffeu); }  // a key has one above it
+
+__global__ __launch_bounds__(kRankB) void k_embed_rank(const int32_t *__restrict__ tokens, int N, uint32_t *__restrict__ sorted,
                                                        int32_t *__restrict__ from) {
-    __shared__ int counts[kRankWaves][kWave];
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int first = blockIdx.x * kWave, i = first + lane;
-    const uint32_t t = i < N ? tokens[i] : 0;
-    const int per = (N + kRankWaves - 1) / kRankWaves;
-    const int a = min(N, wave * per), b = min(N, a + per);
-    int n = 0;
-    for (int j = a; j < min(b, first); j++) n += tokens[j] <= t;
-    for (int j = max(a, first); j < min(b, first + kWave); j++) n += tokens[j] < t || (tokens[j] == t && j < i);
-    for (int j = max(a, first + kWave); j < b; j++) n += tokens[j] < t;
-    counts[wave][lane] = n;
+    __shared__ __attribute__((aligned(16))) uint32_t keys[kRankMost];
+    __shared__ int counts[kRankB / 32][32];
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const int padded = (N + 127) / 128 * 128;  // a multiple of four keys for each of the 32 groups
+    for (int j = threadIdx.x; j < padded; j += kRankB) keys[j] = j < N ? sort_key(tokens[j]) : 0xffffffffu;  // behind all others
     __syncthreads();
-    if (wave == 0 && i < N) {
+    const int col = threadIdx.x & 31, group = threadIdx.x / 32;
+    const int first = blockIdx.x * 32, i = first + col;
+    const uint32_t t = i < N ? keys[i] : 0;
+    const int per = padded / 32, a = group * per, b = a + per;
+    auto count = [&](int from_j, int to_j, uint32_t bound) {
+        int n = 0;
+#pragma unroll 4
+        for (int j = from_j; j < to_j; j += 4) {
+            const u4 k = *(const u4 *)(keys + j);
+            n += (k.x < bound) + (k.y < bound) + (k.z < bound) + (k.w < bound);
+        }
+        return n;
+    };
+    int n = count(a, min(b, first), t + 1);                      // equal ones before the workgroup's positions come first,
+    for (int j = max(a, first); j < min(b, first + 32); j++) n += keys[j] < t + (j < i);
+    n += count(max(a, first + 32), b, t);                        // those behind them do not
+    counts[group][col] = n;
+    __syncthreads();
+    if (group == 0 && i < N) {
         n = 0;
 #pragma unroll
-        for (int k = 0; k < kRankWaves; k++) n += counts[k][lane];
+        for (int k = 0; k < kRankB / 32; k++) n += counts[k][col];
         sorted[n] = t;
         from[n] = i;
+    }
+}
+
+// Many: digits of up to kDigitBits from the last to the first, two launches each.  A workgroup has kChunk positions in order.
+struct Digits {
+    const uint32_t *key_in;  // or none: the tokens themselves, and positions as they lie
+    const int32_t *tokens, *from_in;
+    uint32_t *key_out;
+    int32_t *from_out;
+    int *counts;  // [chunks][bins]; summed: of the chunks before, and of all in one more row
+    bool summed;
+    int N, chunks, bins, shift;
+    uint32_t top;  // the key of all tokens outside the table: the number of its rows
+
+    __device__ __forceinline__ uint32_t key(int i) const { return key_in ? key_in[i] : min((uint32_t)tokens[i], top); }
+    __device__ __forceinline__ int digit(uint32_t k) const { return (int)(k >> shift) & (bins - 1); }
+};
+
+__global__ __launch_bounds__(kEmbB) void k_embed_digits(Digits p) {
+    __shared__ int bin[1 << kDigitBits];
+    for (int b = threadIdx.x; b < p.bins; b += kEmbB) bin[b] = 0;
+    __syncthreads();
+    const int i0 = blockIdx.x * kChunk;
+#pragma unroll
+    for (int u = 0; u < kChunk / kEmbB; u++) {
+        const int i = i0 + u * kEmbB + threadIdx.x;
+        if (i < p.N) atomicAdd(&bin[p.digit(p.key(i))], 1);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < p.bins; b += kEmbB) p.counts[(int64_t)blockIdx.x * p.bins + b] = bin[b];
+}
+
+// counts of the chunks before each, and of all
+__global__ __launch_bounds__(kWave) void k_embed_sum(Digits p) {
+    constexpr int U = 16;
+    const int b = blockIdx.x * kWave + threadIdx.x;
+    if (b >= p.bins) return;
+    int sum = 0;
+    for (int c0 = 0; c0 < p.chunks; c0 += U) {
+        int n[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) n[u] = c0 + u < p.chunks ? p.counts[(int64_t)(c0 + u) * p.bins + b] : 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (c0 + u < p.chunks) p.counts[(int64_t)(c0 + u) * p.bins + b] = sum;
+            sum += n[u];
+        }
+    }
+    p.counts[(int64_t)p.chunks * p.bins + b] = sum;
+}
+
+// Each wave has a quarter of the chunk, in order: its positions of a digit go behind those of smaller digits, of earlier chunks and of
+// the waves before it, and among themselves in their order.
+__global__ __launch_bounds__(kEmbB) void k_embed_place(Digits p) {
+    constexpr int kWaves = kEmbB / kWave, kEach = kChunk / kWaves, kBinsEach = (1 << kDigitBits) / kEmbB;
+    __shared__ int at[kWaves][1 << kDigitBits];
+    __shared__ int wave_total[kWaves];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    for (int b = threadIdx.x; b < kWaves << kDigitBits; b += kEmbB) (&at[0][0])[b] = 0;
+    __syncthreads();
+    const int i0 = blockIdx.x * kChunk + wave * kEach;
+    uint32_t key[kEach / kWave];
+    int from[kEach / kWave];
+#pragma unroll
+    for (int u = 0; u < kEach / kWave; u++) {
+        const int i = i0 + u * kWave + lane;
+        key[u] = i < p.N ? p.key(i) : 0;
+        from[u] = i < p.N ? (p.key_in ? p.from_in[i] : i) : -1;
+        if (from[u] >= 0) atomicAdd(&at[wave][p.digit(key[u])], 1);
+    }
+    __syncthreads();
+    // this lane's kBinsEach digits, one after the other: how many in all, and in chunks before this one
+    int total[kBinsEach], before[kBinsEach], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kBinsEach; e++) {
+        const int b = threadIdx.x * kBinsEach + e;
+        total[e] = before[e] = 0;
+        if (b < p.bins && p.summed) {
+            before[e] = p.counts[(int64_t)blockIdx.x * p.bins + b];
+            total[e] = p.counts[(int64_t)p.chunks * p.bins + b];
+        } else if (b < p.bins)
+#pragma unroll 8
+            for (int c = 0; c < p.chunks; c++) {
+                const int n = p.counts[(int64_t)c * p.bins + b];
+                total[e] += n;
+                before[e] += c < (int)blockIdx.x ? n : 0;
+            }
+        sum += total[e];
+    }
+    int up = sum;  // of this lane and those below it in the wave
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int v = __shfl_up(up, d);
+        if (lane >= d) up += v;
+    }
+    if (lane == kWave - 1) wave_total[wave] = up;
+    __syncthreads();
+    int start = up - sum;
+    for (int w = 0; w < wave; w++) start += wave_total[w];
+#pragma unroll
+    for (int e = 0; e < kBinsEach; e++) {
+        const int b = threadIdx.x * kBinsEach + e;
+        if (b < p.bins) {
+            int here = start + before[e];
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                const int n = at[w][b];
+                at[w][b] = here;
+                here += n;
+            }
+        }
+        start += total[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kEach / kWave; u++) {
+        const bool on = from[u] >= 0;
+        const int d = p.digit(key[u]);
+        unsigned long long same = __ballot(on);
+        for (int bit = 0; (1 << bit) < p.bins; bit++) {
+            const unsigned long long m = __ballot((d >> bit) & 1);
+            same &= (d >> bit) & 1 ? m : ~m;
+        }
+        if (on) {
+            const int to = at[wave][d] + __popcll(same & ((1ull << lane) - 1));
+            p.key_out[to] = key[u];
+            p.from_out[to] = from[u];
+            // the digit's last lane moves its place on; the wave's lanes have read it
+            if (same >> lane == 1) at[wave][d] = to + 1;
+        }
     }
 }
 
@@ -125,7 +273,7 @@ struct EmbGrad {
     const float *g;
     float *gw, *parts;  // parts: [blocks][2][4 pieces]
     int64_t N, V;
-    int64_t blocks;      // of sorted positions
+    int64_t blocks;      // of S sorted positions
     unsigned sum_groups;  // workgroups that sum; the others clear
     uint32_t padding;    // a token without a gradient (>= V: none)
     float scale;
@@ -154,10 +302,10 @@ __device__ __forceinline__ float *part_at(const EmbGrad &p, int64_t block, int s
     return p.parts + (block * 2 + slot) * ((p.l.D + 3) / 4 * 4) + c;
 }
 
-template <bool AL>
+template <bool AL, int S>
 __device__ __forceinline__ void sum_block(const EmbGrad &p, int64_t block, int64_t c) {
     constexpr int U = 8;
-    const int64_t k0 = block * kSortedBlock, k1 = min(p.N, k0 + kSortedBlock);
+    const int64_t k0 = block * S, k1 = min(p.N, k0 + S);
     uint32_t cur = p.sorted[k0];
     bool before = k0 > 0 && p.sorted[k0 - 1] == cur;  // the token began before this block
     f4 sum = {};
@@ -192,11 +340,12 @@ template <bool AL>
 __device__ __forceinline__ void clear_rows(const EmbGrad &p, int64_t r0, int count, int64_t c) {
     __shared__ int used[kEmbB];
     used[threadIdx.x] = 0;
-    int64_t lo = 0, hi = p.N;  // the first sorted position of row r0 or later
+    int64_t lo = 0, hi = p.N;  // the first sorted position of row r0 or later: 64 places at a time
     while (lo < hi) {
-        const int64_t mid = (lo + hi) / 2;
-        if (p.sorted[mid] < r0) lo = mid + 1;
-        else hi = mid;
+        const int64_t step = (hi - lo + kWave - 1) / kWave, k = lo + (int64_t)(threadIdx.x & (kWave - 1)) * step;
+        const int less = __popcll(__ballot(k < hi && p.sorted[min(k, hi - 1)] < r0));
+        hi = min(hi, lo + less * step);
+        if (less) lo += (less - 1) * step + 1;
     }
     __syncthreads();
     for (int64_t k = lo + threadIdx.x; k < p.N; k += kEmbB) {
@@ -210,7 +359,7 @@ __device__ __forceinline__ void clear_rows(const EmbGrad &p, int64_t r0, int cou
         if (r0 + r < p.V && !used[r]) put<AL>(p.gw + (r0 + r) * p.l.D, c, p.l.D, f4{});
 }
 
-template <bool AL>
+template <bool AL, int S>
 __global__ __launch_bounds__(kEmbB) void k_embed_grad(EmbGrad p) {
     const int64_t c = 4 * (((int64_t)blockIdx.y << p.l.shift) + (threadIdx.x & ((1 << p.l.shift) - 1)));
     if (blockIdx.x >= p.sum_groups) {
@@ -218,23 +367,23 @@ __global__ __launch_bounds__(kEmbB) void k_embed_grad(EmbGrad p) {
         return;
     }
     const int64_t block = (int64_t)blockIdx.x * (kEmbB >> p.l.shift) + (threadIdx.x >> p.l.shift);
-    if (c < p.l.D && block < p.blocks) sum_block<AL>(p, block, c);
+    if (c < p.l.D && block < p.blocks) sum_block<AL, S>(p, block, c);
 }
 
 // The rows of tokens that go over blocks, where each begins.
-template <bool AL>
+template <bool AL, int S>
 __global__ __launch_bounds__(kEmbB) void k_embed_join(EmbGrad p) {
     constexpr int U = 8;
     const int64_t c = 4 * (((int64_t)blockIdx.y << p.l.shift) + (threadIdx.x & ((1 << p.l.shift) - 1)));
     const int64_t block = (int64_t)blockIdx.x * (kEmbB >> p.l.shift) + (threadIdx.x >> p.l.shift);
-    const int64_t end = (block + 1) * kSortedBlock;
+    const int64_t end = (block + 1) * S;
     if (c >= p.l.D || end >= p.N) return;
     const uint32_t t = p.sorted[end];
     if (!p.counts(t) || p.sorted[end - 1] != t) return;
-    const int64_t begin = block * kSortedBlock;
+    const int64_t begin = block * S;
     if (begin > 0 && p.sorted[begin - 1] == t) return;  // it began before
     int64_t last = block + 1;  // the block it ends in
-    while ((last + 1) * kSortedBlock < p.N && p.sorted[(last + 1) * kSortedBlock] == t) last++;
+    while ((last + 1) * S < p.N && p.sorted[(last + 1) * S] == t) last++;
     const f4 head = *(const f4 *)part_at(p, block, 1, c);
     double sum[4] = {head[0], head[1], head[2], head[3]};
     for (int64_t b = block + 1; b <= last; b += U) {
@@ -250,6 +399,32 @@ __global__ __launch_bounds__(kEmbB) void k_embed_join(EmbGrad p) {
 }
 
 static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+// Sorted positions of a block: 8 where blocks of 32 would leave most of the chip idle, at the cost of more parts of tokens that
+// occur often (2331 tokens of 250 columns: 28 -> 11 us).
+static int sorted_block(int64_t N, int64_t D) { return (N + 31) / 32 * ((D + 3) / 4) < 65536 ? 8 : 32; }
+
+// the workspace: [tokens in order][their positions], where digits are sorted the same again and the digits' counts, [parts]
+struct SortPlan {
+    int passes, bits, chunks;
+    size_t list, counts, parts;
+};
+static SortPlan sort_plan(int64_t N, int64_t V) {
+    SortPlan s{};
+    s.list = round16((size_t)N * 4);
+    if (N > kRankMost) {
+        int bits = 1;
+        while (bits < 31 && (int64_t(1) << bits) <= V) bits++;  // V itself is a key
+        s.passes = (bits + kDigitBits - 1) / kDigitBits;
+        s.bits = (bits + s.passes - 1) / s.passes;
+        s.chunks = (int)((N + kChunk - 1) / kChunk);
+        s.counts = 4 * s.list;
+        s.parts = s.counts + round16(((size_t)(s.chunks + 1) << s.bits) * 4);
+    } else {
+        s.parts = 2 * s.list;
+    }
+    return s;
+}
 
 static const char *size_error(int64_t N, int64_t V, int64_t D) {
     if (N < 0 || N > kMaxTokens) return "0 to 2^30 tokens";
@@ -288,8 +463,8 @@ extern "C" NC_HIP_API int nc_hip_embedding_fwd(int64_t N, int64_t V, int64_t D, 
 
 extern "C" NC_HIP_API size_t nc_hip_embedding_bwd_workspace(int64_t N, int64_t V, int64_t D) {
     if (size_error(N, V, D) || N == 0) return 0;
-    const int64_t blocks = (N + kSortedBlock - 1) / kSortedBlock;
-    return 2 * round16((size_t)N * 4) + (size_t)blocks * 2 * (size_t)((D + 3) / 4 * 4) * sizeof(float);
+    const int S = sorted_block(N, D);
+    return sort_plan(N, V).parts + (size_t)((N + S - 1) / S) * 2 * (size_t)((D + 3) / 4 * 4) * sizeof(float);
 }
 
 extern "C" NC_HIP_API int nc_hip_embedding_bwd(int64_t N, int64_t V, int64_t D, const int32_t *tokens, int32_t padding, float scale,
@@ -304,29 +479,44 @@ extern "C" NC_HIP_API int nc_hip_embedding_bwd(int64_t N, int64_t V, int64_t D, 
     hipStream_t st = as_stream(stream);
     EmbGrad p{};
     p.l = lay_of(D);
-    p.sorted = (uint32_t *)ws;
-    p.from = (int32_t *)((char *)ws + round16((size_t)N * 4));
-    p.parts = (float *)((char *)ws + 2 * round16((size_t)N * 4));
+    const SortPlan sp = sort_plan(N, V);
+    const int S = sorted_block(N, D);
+    uint32_t *sorted = (uint32_t *)ws;
+    int32_t *from = (int32_t *)((char *)ws + sp.list);
+    p.sorted = sorted, p.from = from, p.parts = (float *)((char *)ws + sp.parts);
     p.g = g, p.gw = gw, p.N = N, p.V = V, p.scale = scale, p.acc = accumulate != 0;
     p.padding = padding >= 0 ? (uint32_t)padding : ~0u;
-    p.blocks = (N + kSortedBlock - 1) / kSortedBlock;
+    p.blocks = (N + S - 1) / S;
     const int64_t groups = (p.blocks + p.l.rows() - 1) / p.l.rows();
     p.sum_groups = (unsigned)groups;
     p.clear_rows = p.l.clear_rows();
     const int64_t clear = accumulate ? 0 : (V + p.clear_rows - 1) / p.clear_rows;
-    if ((groups + clear) * p.l.slices() * kEmbB > kMaxLanes || N * kRankWaves > kMaxLanes)
+    if ((groups + clear) * p.l.slices() * kEmbB > kMaxLanes)
         return set_error(NC_HIP_ERR_ARG, "%s: bad size, no launch holds it", what);
     const bool al = D % 4 == 0 && aligned16(g) && aligned16(gw);
-    if (N > 0)
-        hipLaunchKernelGGL(k_embed_rank, (unsigned)((N + kWave - 1) / kWave), kRankB, 0, st, (const uint32_t *)tokens, (int)N,
-                           (uint32_t *)p.sorted, (int32_t *)p.from);
-    const dim3 grid((unsigned)(groups + clear), (unsigned)p.l.slices());
-    if (al) hipLaunchKernelGGL(k_embed_grad<true>, grid, kEmbB, 0, st, p);
-    else hipLaunchKernelGGL(k_embed_grad<false>, grid, kEmbB, 0, st, p);
+    if (N > kRankMost) {
+        // the last digit's places are the workspace's first lists: an odd number of digits starts there, an even one in the others
+        uint32_t *keys[2] = {sorted, (uint32_t *)((char *)ws + 2 * sp.list)};
+        int32_t *places[2] = {from, (int32_t *)((char *)ws + 3 * sp.list)};
+        Digits d{nullptr, tokens, nullptr, nullptr, nullptr, (int *)((char *)ws + sp.counts), sp.chunks > kSumChunks, (int)N, sp.chunks, 1 << sp.bits, 0, (uint32_t)V};
+        for (int i = 0; i < sp.passes; i++) {
+            const int to = (sp.passes - 1 - i) & 1;
+            d.key_out = keys[to], d.from_out = places[to], d.shift = i * sp.bits;
+            hipLaunchKernelGGL(k_embed_digits, (unsigned)sp.chunks, kEmbB, 0, st, d);
+            if (d.summed) hipLaunchKernelGGL(k_embed_sum, (unsigned)((d.bins + kWave - 1) / kWave), kWave, 0, st, d);
+            hipLaunchKernelGGL(k_embed_place, (unsigned)sp.chunks, kEmbB, 0, st, d);
+            d.key_in = d.key_out, d.from_in = d.from_out;
+        }
+    } else if (N > 0) {
+        hipLaunchKernelGGL(k_embed_rank, (unsigned)((N + 31) / 32), kRankB, 0, st, tokens, (int)N, sorted, from);
+    }
+    const dim3 grid((unsigned)(groups + clear), (unsigned)p.l.slices()), joins((unsigned)groups, (unsigned)p.l.slices());
+    auto run = [&](auto kernel, dim3 g) { hipLaunchKernelGGL(kernel, g, kEmbB, 0, st, p); };
+    if (S == 8) al ? run(k_embed_grad<true, 8>, grid) : run(k_embed_grad<false, 8>, grid);
+    else al ? run(k_embed_grad<true, 32>, grid) : run(k_embed_grad<false, 32>, grid);
     if (p.blocks > 1) {
-        const dim3 joins((unsigned)groups, (unsigned)p.l.slices());
-        if (al) hipLaunchKernelGGL(k_embed_join<true>, joins, kEmbB, 0, st, p);
-        else hipLaunchKernelGGL(k_embed_join<false>, joins, kEmbB, 0, st, p);
+        if (S == 8) al ? run(k_embed_join<true, 8>, joins) : run(k_embed_join<false, 8>, joins);
+        else al ? run(k_embed_join<true, 32>, joins) : run(k_embed_join<false, 32>, joins);
     }
     return check_launch(what);
 }
