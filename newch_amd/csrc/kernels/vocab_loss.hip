@@ -13,25 +13,43 @@
 namespace nchip {
 
 constexpr size_t kVlPiece = size_t(1) << 30;  // bytes of z held at a time
+constexpr int64_t kVlRows = 32768;            // and rows
+
+constexpr int kVlChunk = 2048;  // words of a row that a workgroup takes, where a row is shared by several
+constexpr int kVlShort = 4096;  // words of a row that one workgroup takes alone, at most
 
 struct VlArgs {
     int64_t N, V, ldz;
     int64_t row0, rows;  // the rows of this piece
+    int chunks;          // of a row
     const int32_t *labels;
     int32_t ignore;
     int sum;
     const VlHead *head;
     const float *gout;
-    float *z;         // [rows][ldz]: the products, then G
+    float *z;          // [rows][ldz]: the products, then G
+    f2 *part;          // [rows][chunks] {maximum, sum of exponentials}, the label's left out of the sum
+    float *label_z;    // [rows]
     double *row_loss;  // [N]
-    float *row_out;   // [N] or none
+    float *row_out;    // [N] or none
 };
 
-// rows that count, and the first label that is neither a word nor `ignore`, as (row << 32) | label, or all ones
-__global__ __launch_bounds__(1024) void k_vl_count(const int32_t *__restrict__ labels, int64_t N, int64_t V, int32_t ignore, VlHead *head,
-                                                   unsigned long long *bad) {
-    __shared__ unsigned long long shk[1024 / kWave];
-    __shared__ double shn[1024 / kWave];
+// Workgroup 0: rows that count, and the first label that is neither a word nor `ignore`, as (row << 32) | label, or all ones.  The
+// others copy x with zeros for the rows that do not count, where gW wants it.
+__global__ __launch_bounds__(1024) void k_vl_count(const int32_t *__restrict__ labels, int64_t N, int64_t D, int64_t V, int32_t ignore,
+                                                   VlHead *head, unsigned long long *bad, const float *__restrict__ x, int64_t ldx,
+                                                   float *__restrict__ clean) {
+    constexpr int kWaves = 1024 / kWave;
+    if (blockIdx.x > 0) {
+        const int lane = threadIdx.x & (kWave - 1);
+        for (int64_t i = (int64_t)(blockIdx.x - 1) * kWaves + threadIdx.x / kWave; i < N; i += (int64_t)(gridDim.x - 1) * kWaves) {
+            const bool on = vl_counts(labels[i], ignore, V);
+            for (int64_t d = lane; d < D; d += kWave) clean[i * D + d] = on ? x[i * ldx + d] : 0.0f;
+        }
+        return;
+    }
+    __shared__ unsigned long long shk[kWaves];
+    __shared__ double shn[kWaves];
     unsigned long long k = ~0ull;
     double n = 0.0;
     for (int64_t i = threadIdx.x; i < N; i += 1024) {
@@ -45,7 +63,7 @@ __global__ __launch_bounds__(1024) void k_vl_count(const int32_t *__restrict__ l
     if ((threadIdx.x & (kWave - 1)) == 0) shk[threadIdx.x / kWave] = k, shn[threadIdx.x / kWave] = n;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < 1024 / kWave; i++) {
+        for (int i = 1; i < kWaves; i++) {
             k = shk[i] < k ? shk[i] : k;
             n += shn[i];
         }
@@ -55,13 +73,25 @@ __global__ __launch_bounds__(1024) void k_vl_count(const int32_t *__restrict__ l
     }
 }
 
-// x with zeros for the rows that do not count
-__global__ __launch_bounds__(kVlB) void k_vl_rows(const float *__restrict__ x, int64_t ldx, const int32_t *__restrict__ labels, int32_t ignore,
-                                                  int64_t N, int64_t D, int64_t V, float *__restrict__ out) {
-    for (int64_t i = blockIdx.x; i < N; i += gridDim.x) {
-        const bool on = vl_counts(labels[i], ignore, V);
-        for (int64_t d = threadIdx.x; d < D; d += kVlB) out[i * D + d] = on ? x[i * ldx + d] : 0.0f;
+// what a row's G is made from
+struct VlStat {
+    float m, ls, own, coef;
+};
+
+__device__ __forceinline__ VlStat vl_stat(const VlArgs &p, int64_t i, float m, double others, float zl, bool first) {
+    const double own = (double)exp8_nonpos(zl), total = others + own;
+    const double ls = zl == 0.0f ? log1p(others) : log(total);
+    if (first) {
+        const double loss = ls - (double)zl;
+        p.row_loss[i] = loss;
+        if (p.row_out) p.row_out[i] = (float)loss;
     }
+    const float c = p.gout ? *p.gout : 1.0f;
+    return {m, (float)ls, (float)(-others / total), p.sum ? c : c / (float)p.head->count};
+}
+
+__device__ __forceinline__ float vl_entry(float z, int64_t v, int32_t label, const VlStat &s) {
+    return (v == label ? s.own : exp8_nonpos((z - s.m) - s.ls)) * s.coef;
 }
 
 // A workgroup's row: its statistics, its loss, and, GRAD, its row of G in place of z.
@@ -93,31 +123,106 @@ __global__ __launch_bounds__(kVlB) void k_vl_softmax(VlArgs p) {
         double s = 0.0;
         for (int64_t v = threadIdx.x; v < p.V; v += kVlB) s += v == l ? 0.0 : (double)exp_sum_term(z[v] - m);
         const double others = vl_wg_sum(s, sh);
-        const float zl = z[l] - m;
-        const double own = (double)exp8_nonpos(zl), total = others + own;
-        const double ls = zl == 0.0f ? log1p(others) : log(total);
-        if (threadIdx.x == 0) {
-            const double loss = ls - (double)zl;
-            p.row_loss[i] = loss;
-            if (p.row_out) p.row_out[i] = (float)loss;
-        }
+        const VlStat st = vl_stat(p, i, m, others, z[l] - m, threadIdx.x == 0);
         if (GRAD) {
-            float c = p.gout ? *p.gout : 1.0f;
-            if (!p.sum) c = c / (float)p.head->count;
-            const float g_own = (float)(-others / total), lf = (float)ls;
             __syncthreads();  // z[l] has been read
-            for (int64_t v = threadIdx.x; v < p.V; v += kVlB) z[v] = (v == l ? g_own : exp8_nonpos((z[v] - m) - lf)) * c;
+            for (int64_t v = threadIdx.x; v < p.V; v += kVlB) z[v] = vl_entry(z[v], v, l, st);
         }
     }
 }
 
-// gb (+)= column sums of G, rows in order
+// The same of long rows, whose chunks are workgroups of their own: first each chunk's maximum and sum,
+__global__ __launch_bounds__(kVlB) void k_vl_part(VlArgs p) {
+    constexpr int kEach = kVlChunk / kVlB;
+    __shared__ double sh[kVlB / kWave];
+    __shared__ float shm[kVlB / kWave];
+    const int64_t r = blockIdx.y, v0 = (int64_t)blockIdx.x * kVlChunk;
+    const int32_t l = p.labels[p.row0 + r];
+    if (!vl_counts(l, p.ignore, p.V)) return;
+    const float *z = p.z + r * p.ldz;
+    float x[kEach], m = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+        const int64_t v = v0 + k * kVlB + threadIdx.x;
+        x[k] = v < p.V ? z[v] : -__builtin_inff();
+        m = __builtin_fmaxf(m, x[k]);
+        if (v == l) {
+            p.label_z[r] = x[k];
+            x[k] = -__builtin_inff();
+        }
+    }
+    m = wave_max_nan_skip(m);
+    if ((threadIdx.x & (kWave - 1)) == 0) shm[threadIdx.x / kWave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kVlB / kWave; k++) m = __builtin_fmaxf(m, shm[k]);
+    double s = 0.0;
+    const float base = m == -__builtin_inff() ? 0.0f : m;  // words that are all -inf have no part in the row's sum
+#pragma unroll
+    for (int k = 0; k < kEach; k++) s += (double)exp_sum_term(x[k] - base);
+    s = vl_wg_sum(s, sh);
+    if (threadIdx.x == 0) p.part[r * p.chunks + blockIdx.x] = f2{m, (float)s};
+}
+
+// then, from those of its row, a chunk of G.
+template <bool GRAD>
+__global__ __launch_bounds__(kVlB) void k_vl_chunk(VlArgs p) {
+    __shared__ double sh[kVlB / kWave];
+    __shared__ float shm[kVlB / kWave];
+    const int64_t r = blockIdx.y, i = p.row0 + r, v0 = (int64_t)blockIdx.x * kVlChunk;
+    const int32_t l = p.labels[i];
+    float *z = p.z + r * p.ldz;
+    if (!vl_counts(l, p.ignore, p.V)) {
+        if (threadIdx.x == 0 && blockIdx.x == 0) {
+            p.row_loss[i] = 0.0;
+            if (p.row_out) p.row_out[i] = 0.0f;
+        }
+        if (GRAD)
+            for (int64_t v = v0 + threadIdx.x; v < min(p.V, v0 + kVlChunk); v += kVlB) z[v] = 0.0f;
+        return;
+    }
+    const f2 *part = p.part + r * p.chunks;
+    float m = -__builtin_inff();
+    for (int k = threadIdx.x; k < p.chunks; k += kVlB) m = __builtin_fmaxf(m, part[k].x);
+    m = wave_max_nan_skip(m);
+    if ((threadIdx.x & (kWave - 1)) == 0) shm[threadIdx.x / kWave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kVlB / kWave; k++) m = __builtin_fmaxf(m, shm[k]);
+    double s = 0.0;
+    for (int k = threadIdx.x; k < p.chunks; k += kVlB) s += (double)part[k].y * (double)(part[k].x == m ? 1.0f : exp8_nonpos(part[k].x - m));
+    const double others = vl_wg_sum(s, sh);
+    const VlStat st = vl_stat(p, i, m, others, p.label_z[r] - m, blockIdx.x == 0 && threadIdx.x == 0);
+    if (GRAD)
+        for (int64_t v = v0 + threadIdx.x; v < min(p.V, v0 + kVlChunk); v += kVlB) z[v] = vl_entry(z[v], v, l, st);
+}
+
+// gx (+)= the parts' sum
+__global__ __launch_bounds__(kVlB) void k_vl_parts(const float *__restrict__ parts, int slices, int64_t n, float *__restrict__ gx, int acc) {
+    for (int64_t i = (int64_t)blockIdx.x * kVlB + threadIdx.x; i < n; i += (int64_t)gridDim.x * kVlB) {
+        double s = acc ? (double)gx[i] : 0.0;
+#pragma unroll 8
+        for (int k = 0; k < slices; k++) s += (double)parts[k * n + i];
+        gx[i] = (float)s;
+    }
+}
+
+// gb (+)= column sums of G: 64 columns a workgroup, a quarter of the rows in each wave
 __global__ __launch_bounds__(kVlB) void k_vl_columns(const float *__restrict__ g, int64_t ldz, int64_t rows, int64_t V, float *gb, int acc) {
-    const int64_t v = (int64_t)blockIdx.x * kVlB + threadIdx.x;
-    if (v >= V) return;
-    double s = acc ? (double)gb[v] : 0.0;
-    for (int64_t r = 0; r < rows; r++) s += (double)g[r * ldz + v];
-    gb[v] = (float)s;
+    constexpr int kWaves = kVlB / kWave;
+    __shared__ double sh[kWaves][kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int64_t v = (int64_t)blockIdx.x * kWave + lane;
+    double s = 0.0;
+    if (v < V)
+#pragma unroll 8
+        for (int64_t r = wave; r < rows; r += kWaves) s += (double)g[r * ldz + v];
+    sh[wave][lane] = s;
+    __syncthreads();
+    if (wave != 0 || v >= V) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) s += sh[w][lane];
+    gb[v] = (float)(acc ? (double)gb[v] + s : s);
 }
 
 // the loss of no rows is NaN, as a mean over nothing is (a sum: 0)
@@ -134,21 +239,32 @@ __global__ __launch_bounds__(kVlB) void k_vl_zero(float *__restrict__ p, int64_t
     for (int64_t i = (int64_t)blockIdx.x * kVlB + threadIdx.x; i < n; i += (int64_t)gridDim.x * kVlB) p[i] = 0.0f;
 }
 
-// the workspace: [head][row losses][x without the rows that do not count][z of a piece]
+// the workspace: [head][row losses][labels' products][chunks' statistics][x without the rows that do not count][z of a piece][parts of gx]
 struct VlPlan {
     int64_t ldz, piece;
-    size_t losses, rows, z, total;
+    int chunks, slices;
+    int64_t slice;  // words of a part of gx
+    size_t losses, label_z, part, rows, z, parts, total;
 };
 
-static VlPlan vl_plan(int64_t N, int64_t D, int64_t V, bool want_w) {
+static VlPlan vl_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w) {
     VlPlan p{};
     p.ldz = (V + 15) / 16 * 16;
     const int64_t most = std::max<int64_t>(64, (int64_t)(kVlPiece / 4) / p.ldz / 64 * 64);
-    p.piece = std::min(N, most);
+    p.piece = std::min(std::min(N, most), kVlRows);
+    p.chunks = V > kVlShort ? (int)((V + kVlChunk - 1) / kVlChunk) : 1;
+    // gx of few rows: its words in parts, as many as give the chip's CUs two tiles of 64 x 64 each, of at least 512 words
+    const int64_t tiles = (p.piece + 63) / 64 * ((D + 63) / 64);
+    const int64_t cut = std::max<int64_t>(1, std::min((2 * kPlanCUs + tiles - 1) / std::max<int64_t>(tiles, 1), V / 512));
+    p.slice = cut > 1 ? ((V + cut - 1) / cut + 31) / 32 * 32 : V;
+    p.slices = (int)((V + p.slice - 1) / p.slice);
     p.losses = 256;
-    p.rows = p.losses + vl_round256((size_t)N * 8);
+    p.label_z = p.losses + vl_round256((size_t)N * 8);
+    p.part = p.label_z + vl_round256((size_t)p.piece * 4);
+    p.rows = p.part + vl_round256((size_t)p.piece * p.chunks * sizeof(f2));
     p.z = p.rows + (want_w ? vl_round256((size_t)(N * D) * 4) : 0);
-    p.total = p.z + (size_t)(p.piece * p.ldz) * 4;
+    p.parts = p.z + vl_round256((size_t)(p.piece * p.ldz) * 4);
+    p.total = p.parts + (want_x && p.slices > 1 ? (size_t)p.slices * p.piece * D * 4 : 0);
     return p;
 }
 
@@ -166,7 +282,7 @@ using namespace nchip;
 extern "C" NC_HIP_API size_t nc_hip_linear_cross_entropy_workspace(int64_t N, int64_t D, int64_t V, int want_x, int want_w, int want_b) {
     if (vl_size_error(N, D, V)) return 0;
     if (vl_split_pays(N, D, V, want_x || want_w || want_b)) return vl_split_workspace(N, D, V, want_x != 0, want_w != 0, want_b != 0);
-    return vl_plan(N, D, V, want_w != 0).total;
+    return vl_plan(N, D, V, want_x != 0, want_w != 0).total;
 }
 
 extern "C" NC_HIP_API int nc_hip_linear_cross_entropy(int64_t N, int64_t D, int64_t V, const float *x, int64_t ldx, const float *w,
@@ -187,25 +303,44 @@ extern "C" NC_HIP_API int nc_hip_linear_cross_entropy(int64_t N, int64_t D, int6
     if (vl_split_pays(N, D, V, grad))
         return vl_split_run({N, D, V, x, ldx, w, ldw, bias, labels, ignore, sum, gout, loss, row_loss, (unsigned long long *)bad, gx, gw, gb,
                              acc_x, acc_w, acc_b, (char *)ws, st}, what);
-    const VlPlan plan = vl_plan(N, D, V, gw != nullptr);
+    const VlPlan plan = vl_plan(N, D, V, gx != nullptr, gw != nullptr);
     char *base = (char *)ws;
     VlHead *head = (VlHead *)base;
     double *losses = (double *)(base + plan.losses);
-    float *clean = (float *)(base + plan.rows), *z = (float *)(base + plan.z);
-    hipLaunchKernelGGL(k_vl_count, 1, 1024, 0, st, labels, N, V, ignore, head, (unsigned long long *)bad);
-    if (N > 0 && gw) hipLaunchKernelGGL(k_vl_rows, (unsigned)std::min<int64_t>(N, 1 << 16), kVlB, 0, st, x, ldx, labels, ignore, N, D, V, clean);
+    float *clean = (float *)(base + plan.rows), *z = (float *)(base + plan.z), *parts = (float *)(base + plan.parts);
+    const unsigned copies = gw ? (unsigned)std::min<int64_t>((N + 15) / 16, 1024) : 0;
+    hipLaunchKernelGGL(k_vl_count, 1 + copies, 1024, 0, st, labels, N, D, V, ignore, head, (unsigned long long *)bad, x, ldx, clean);
     for (int64_t r0 = 0; r0 < N; r0 += plan.piece) {
-        VlArgs a{N, V, plan.ldz, r0, std::min(plan.piece, N - r0), labels, ignore, sum, head, gout, z, losses, row_loss};
+        VlArgs a{N, V, plan.ldz, r0, std::min(plan.piece, N - r0), plan.chunks, labels, ignore, sum, head, gout, z, (f2 *)(base + plan.part),
+                 (float *)(base + plan.label_z), losses, row_loss};
         int rc = nc_hip_gemm_f32_bias(0, 1, a.rows, V, D, 1.0f, x + r0 * ldx, ldx, w, ldw, bias, z, plan.ldz, stream);
         if (rc) return rc;
-        const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 1 << 16);
-        if (grad) hipLaunchKernelGGL(k_vl_softmax<true>, grid, kVlB, 0, st, a);
-        else hipLaunchKernelGGL(k_vl_softmax<false>, grid, kVlB, 0, st, a);
-        if (gx) rc = nc_hip_gemm_f32(0, 0, a.rows, D, V, 1.0f, z, plan.ldz, w, ldw, acc_x ? 1.0f : 0.0f, gx + r0 * D, D, stream);
+        if (plan.chunks > 1) {
+            const dim3 grid((unsigned)plan.chunks, (unsigned)a.rows);
+            hipLaunchKernelGGL(k_vl_part, grid, kVlB, 0, st, a);
+            if (grad) hipLaunchKernelGGL(k_vl_chunk<true>, grid, kVlB, 0, st, a);
+            else hipLaunchKernelGGL(k_vl_chunk<false>, dim3(1, (unsigned)a.rows), kVlB, 0, st, a);
+        } else if (grad) {
+            hipLaunchKernelGGL(k_vl_softmax<true>, (unsigned)a.rows, kVlB, 0, st, a);
+        } else {
+            hipLaunchKernelGGL(k_vl_softmax<false>, (unsigned)a.rows, kVlB, 0, st, a);
+        }
+        if (gx && plan.slices > 1) {
+            const int64_t whole = V / plan.slice, rest = V - whole * plan.slice, part = a.rows * D;
+            const int64_t shape = whole, sa = plan.slice, sb = plan.slice * ldw;
+            rc = nc_hip_gemm_f32_bmm(0, 0, a.rows, D, plan.slice, z, plan.ldz, w, ldw, 0.0f, parts, D, 1, &shape, &sa, &sb, &part, nullptr, 0, stream);
+            if (!rc && rest)
+                rc = nc_hip_gemm_f32(0, 0, a.rows, D, rest, 1.0f, z + whole * plan.slice, plan.ldz, w + whole * sb, ldw, 0.0f,
+                                     parts + whole * part, D, stream);
+            if (!rc)
+                hipLaunchKernelGGL(k_vl_parts, stream_grid(part, kVlB), kVlB, 0, st, parts, plan.slices, part, gx + r0 * D, acc_x != 0);
+        } else if (gx) {
+            rc = nc_hip_gemm_f32(0, 0, a.rows, D, V, 1.0f, z, plan.ldz, w, ldw, acc_x ? 1.0f : 0.0f, gx + r0 * D, D, stream);
+        }
         if (!rc && gw)
             rc = nc_hip_gemm_f32(1, 0, V, D, a.rows, 1.0f, z, plan.ldz, clean + r0 * D, D, acc_w || r0 ? 1.0f : 0.0f, gw, D, stream);
         if (rc) return rc;
-        if (gb) hipLaunchKernelGGL(k_vl_columns, (unsigned)((V + kVlB - 1) / kVlB), kVlB, 0, st, z, plan.ldz, a.rows, V, gb, acc_b || r0);
+        if (gb) hipLaunchKernelGGL(k_vl_columns, (unsigned)((V + kWave - 1) / kWave), kVlB, 0, st, z, plan.ldz, a.rows, V, gb, acc_b || r0);
     }
     if (N == 0) {
         if (gw && !acc_w) hipLaunchKernelGGL(k_vl_zero, stream_grid(V * D, kVlB), kVlB, 0, st, gw, V * D);

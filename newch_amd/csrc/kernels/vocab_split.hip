@@ -157,11 +157,11 @@ __device__ __forceinline__ void z_out(const MmArgs &p, f16x (&acc)[4][2], int64_
                     }
         }
         float s = 0.0f;
+        const float base = m == -__builtin_inff() ? 0.0f : m;  // words that are all -inf have no part in the row's sum
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) s += exp_sum_term(acc[i][j][r] - m);
-        if (m == -__builtin_inff()) s = s == s ? s : 0.0f;
+            for (int r = 0; r < 16; r++) s += exp_sum_term(acc[i][j][r] - base);
         s += __shfl_xor(s, 32);
         if (half == 0) p.part[(v0 / kStatWords) * p.rows + n] = f2{m, s};
     }
