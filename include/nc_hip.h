@@ -385,7 +385,12 @@ NC_HIP_API int nc_hip_dropout_bwd(int64_t n, double p, uint64_t seed, uint64_t o
  * gx [N, D], gw [V, D] and gb [V] (contiguous, each may be NULL: the loss alone) are stored or, with their acc, added to: the gradients of
  * *gout * loss (gout: one float in device memory; NULL: 1).  Sums in a fixed order.  Outputs overlap neither inputs nor each other.
  * The workspace (16-byte aligned) is for the gradients that are asked for; its contents count only within a call.
- * N < 2^31, D <= 2^20, V <= 2^26. */
+ * N < 2^31, D <= 2^20, V <= 2^26.
+ * Precision: few rows or words run on plain fp32 products.  Where it pays, operands (x and w by rows and by columns, and the
+ * gradient of z by both) are held in two fp16 pieces, 22 bits, under a power of two of their row or column: a value below 2^-17 of the
+ * largest of its row (column) is held to 2^-40 of it; an infinity that counts gives NaN.  Products are summed in fp32 either way.
+ * Test hooks: NC_HIP_VOCAB_FORM=fp32 or split chooses the form, NC_HIP_VOCAB_ROWS=n the rows whose z is held at a time (the
+ * workspace's size follows both). */
 NC_HIP_API size_t nc_hip_linear_cross_entropy_workspace(int64_t N, int64_t D, int64_t V, int want_x, int want_w, int want_b);
 NC_HIP_API int nc_hip_linear_cross_entropy(int64_t N, int64_t D, int64_t V, const float *x, int64_t ldx, const float *w, int64_t ldw,
                                            const float *bias, const int32_t *labels, int32_t ignore, int sum, const float *gout,

@@ -251,7 +251,7 @@ static VlPlan vl_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w)
     VlPlan p{};
     p.ldz = (V + 15) / 16 * 16;
     const int64_t most = std::max<int64_t>(64, (int64_t)(kVlPiece / 4) / p.ldz / 64 * 64);
-    p.piece = std::min(std::min(N, most), kVlRows);
+    p.piece = std::min(std::min(N, most), vl_piece_rows(kVlRows));
     p.chunks = V > kVlShort ? (int)((V + kVlChunk - 1) / kVlChunk) : 1;
     // gx of few rows: its words in parts, as many as give the chip's CUs two tiles of 64 x 64 each, of at least 512 words
     const int64_t tiles = (p.piece + 63) / 64 * ((D + 63) / 64);

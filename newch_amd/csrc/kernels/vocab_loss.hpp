@@ -13,7 +13,7 @@ constexpr int kVlB = 256;
 // the head of the workspace
 struct VlHead {
     int64_t count;  // rows that count
-    int slices;     // of the words in gx
+    int slices_x, slices_w;  // parts of gx and gW
 };
 
 // one call's arguments
@@ -49,6 +49,15 @@ __device__ __forceinline__ double vl_wg_sum(double v, double *sh) {
 }
 
 inline size_t vl_round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// rows of a piece at most: `most`, or what the test hook NC_HIP_VOCAB_ROWS says
+inline int64_t vl_piece_rows(int64_t most) {
+    if (const char *e = getenv("NC_HIP_VOCAB_ROWS")) {
+        const long long v = atoll(e);
+        if (v > 0 && v < most) return v;
+    }
+    return most;
+}
 
 // whether the products of a call are worth cutting into pieces, the workspace that takes, and the call itself
 bool vl_split_pays(int64_t N, int64_t D, int64_t V, bool grads);

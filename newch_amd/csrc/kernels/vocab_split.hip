@@ -39,7 +39,6 @@ constexpr int64_t kZBytes = int64_t(4) << 30;  // of z and of the turned G, both
 constexpr int64_t kScored = int64_t(1) << 36;  // products of a launch that leaves no z
 constexpr int64_t kPieceRows = 1 << 20;
 constexpr int64_t kPartBytes = int64_t(512) << 20;  // of the parts of gx
-constexpr int kSizeBlocks = 8;   // of 32 rows that a workgroup looks at for their sizes, at most
 constexpr int kPackCols = 128;
 constexpr int kStatWords = 128;  // words of one partial statistic
 
@@ -76,7 +75,7 @@ __device__ __forceinline__ Pieces cut(const float (&x)[8], float scale) {
 }
 
 // ---- the product ------------------------------------------------------------------------------------------------------
-enum { MM_Z = 0, MM_GX = 1, MM_GW = 2 };
+enum { MM_Z = 0, MM_GX = 1, MM_GW = 2, MM_GW_PARTS = 3 };
 
 struct MmArgs {
     const char *A, *B;      // packed; blocks of a row block follow each other
@@ -95,9 +94,9 @@ struct MmArgs {
     f2 *part;               // [words / kStatWords][rows]
     float *label_z;         // [rows]
     int64_t rows;           // of a piece, padded
-    // MM_GX: A the rows, B the columns
-    float *parts;           // [slices][rows][columns]
-    int64_t cols;           // columns, padded
+    // MM_GX: A the rows, B the columns; MM_GW_PARTS: A the words
+    float *parts;           // [slices][rows or words][columns]
+    int64_t part_rows, cols;  // rows or words, and columns, padded
     // MM_GW: A the words, B the columns
     const float *most_a, *most_b;
     const float *gout;
@@ -167,18 +166,15 @@ __device__ __forceinline__ void z_out(const MmArgs &p, f16x (&acc)[4][2], int64_
     }
 }
 
-// How many parts the words are cut into for gx: of few tiles' products, as many as make the rounds of workgroups full.  In units of a
-// block of 16 k of a tile (a round costs its blocks and some 24 to start and to leave): rounds x blocks + the parts' way through memory.
-__device__ __forceinline__ int gx_slices(int64_t left, int tiles_n, int kblocks, int most, int at_once) {
-    const int64_t tiles = (left + kTileM - 1) / kTileM * tiles_n;
-    int best = 1;
-    int64_t least = INT64_MAX;
-    for (int s = 1; s <= most; s++) {
-        const int64_t rounds = (tiles * s + at_once - 1) / at_once;
-        const int64_t cost = rounds * ((kblocks + s - 1) / s + 24) + tiles * s / 24;
-        if (cost < least) least = cost, best = s;
-    }
-    return best;
+// How many parts a sum is cut into, of 64 at most: of few tiles' products, as many as make the rounds of workgroups full.  A wave's lanes
+// try one number each.  In units of a block of 16 k of a tile: a round costs its blocks and some 24 to start and to leave, and a part of a
+// tile an eighth of one on its way through memory.
+__device__ __forceinline__ int parts_of(int64_t tiles, int kblocks, int most, int at_once) {
+    const int s = (int)(threadIdx.x & (kWave - 1)) + 1;
+    const int64_t rounds = (tiles * s + at_once - 1) / at_once;
+    const int64_t cost = rounds * ((kblocks + s - 1) / s + 24) + tiles * s * kPlanCUs / (8 * at_once);
+    const unsigned long long key = s <= most ? (unsigned long long)cost << 8 | (unsigned)s : ~0ull;
+    return (int)max(1ull, wave_min_u64(key) & 0xff) & 0x7f;
 }
 
 // WN 2: two workgroups a CU, so that one multiplies while the other starts or leaves, and fewer that wait for the last.  WN 4: one, which
@@ -191,7 +187,7 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wm = wave & 1, wn = wave >> 1;
     const int64_t left = p.head->count - p.row0;  // rows of this piece and behind it
-    const int slices = WHAT == MM_GX ? p.head->slices : 1;
+    const int slices = WHAT == MM_GX ? p.head->slices_x : WHAT == MM_GW_PARTS ? p.head->slices_w : 1;
     const uint32_t tiles_m = WHAT == MM_GX ? (uint32_t)(left > 0 ? (min(left, p.rows) + kTileM - 1) / kTileM : 0) : (uint32_t)p.tiles_m;
     const uint32_t tiles_n = WHAT == MM_Z ? (uint32_t)(left > 0 ? (min(left, p.rows) + T::kN - 1) / T::kN : 0) : (uint32_t)p.tiles_n;
     const uint32_t tiles = tiles_m * tiles_n, nblk = tiles * (uint32_t)slices;
@@ -204,13 +200,11 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
     const int gsize = min((int)tiles_m - group * 8, 8);
     const int tm = group * 8 + in_group % gsize, tn = in_group / gsize;
     int k0 = 0, k1 = p.kblocks;
-    if (WHAT == MM_GX) {
-        const int64_t pairs = p.kblocks / 2;
+    if (WHAT == MM_GW || WHAT == MM_GW_PARTS) k1 = (int)min((int64_t)p.kblocks, left > 0 ? (left + 31) / 32 * 2 : 0);
+    if (WHAT == MM_GW && k1 == 0 && p.acc) return;
+    if (WHAT == MM_GX || WHAT == MM_GW_PARTS) {
+        const int64_t pairs = k1 / 2;
         k0 = 2 * (int)(pairs * slice / slices), k1 = 2 * (int)(pairs * (slice + 1) / slices);
-    }
-    if (WHAT == MM_GW) {
-        k1 = (int)min((int64_t)p.kblocks, left > 0 ? (left + 31) / 32 * 2 : 0);
-        if (k1 == 0 && p.acc) return;
     }
     const int nk = k1 - k0;
     const int64_t m0 = (int64_t)tm * kTileM + 128 * wm, n0 = (int64_t)tn * T::kN + 64 * wn;
@@ -313,9 +307,9 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
     asm volatile("" : "+v"(at)::"memory");
     if constexpr (WHAT == MM_Z) {
         z_out(p, acc, m0, n0, at);
-    } else if constexpr (WHAT == MM_GX) {
+    } else if constexpr (WHAT == MM_GX || WHAT == MM_GW_PARTS) {
         // a store instruction writes 32 columns of two rows
-        float *out = p.parts + ((int64_t)slice * p.rows + m0 + 4 * (at >> 5)) * p.cols + n0 + (at & 31);
+        float *out = p.parts + ((int64_t)slice * p.part_rows + m0 + 4 * (at >> 5)) * p.cols + n0 + (at & 31);
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -427,7 +421,6 @@ struct PackArgs {
     char *by_rows, *by_columns;  // by_columns: or none
     int64_t step, step_c;  // bytes from a block of 32 rows (columns) to the next
     int64_t padded;       // rows, padded
-    int blocks;           // of 32 rows that a workgroup looks at for their sizes
     int groups;           // workgroups that look at sizes
     int regions;          // of 64 columns
     bool as_registers;    // the k of by_columns in the order that z's registers have
@@ -438,26 +431,35 @@ struct PackPair {
 
 __device__ __forceinline__ int64_t row_count(const PackArgs &p) { return p.from ? p.head->count : p.rows; }
 
-// The largest sizes of rows and columns: a wave takes 256 columns at a time and goes down its workgroup's rows.
+// The largest sizes of rows and columns: a wave goes down 8 BATCHES rows, 256 columns at a time, and the columns' sizes of the four
+// waves meet in LDS.
+template <int BATCHES>
 __global__ __launch_bounds__(kVlB) void k_vl_sizes(PackPair pp) {
-    __shared__ float sh[kVlB / kWave][32 * kSizeBlocks];
+    constexpr int kWaves = kVlB / kWave;
+    __shared__ f4 sh[2][kWaves][kWave];
     const bool second = (int)blockIdx.x >= pp.a[0].groups;
     const PackArgs &p = pp.a[second];
-    const int64_t group = blockIdx.x - (second ? pp.a[0].groups : 0), first = group * p.blocks * 32;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, all = p.blocks * 32;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int64_t group = blockIdx.x - (second ? pp.a[0].groups : 0), first = (group * kWaves + wave) * (8 * BATCHES);
     const int64_t rows = row_count(p);
-    const int here = (int)max(int64_t(0), min((int64_t)all, rows - first));
-    for (int i = lane; i < all; i += kWave) sh[wave][i] = 0.0f;
-    for (int64_t c0 = wave * 256; c0 < p.cols; c0 += kVlB / kWave * 256) {
+    float most_r[BATCHES][8];
+#pragma unroll
+    for (int t = 0; t < BATCHES; t++)
+#pragma unroll
+        for (int u = 0; u < 8; u++) most_r[t][u] = 0.0f;
+    int turn = 0;
+    for (int64_t c0 = 0; c0 < p.cols; c0 += 256, turn ^= 1) {
         const int64_t c = c0 + 4 * lane;
         f4 most = {};
-        for (int r = 0; r < here; r += 8) {
+#pragma unroll
+        for (int t = 0; t < BATCHES; t++) {
             f4 v[8];
 #pragma unroll
             for (int u = 0; u < 8; u++) {
+                const int64_t r = first + 8 * t + u;
                 v[u] = f4{};
-                if (r + u < here && c < p.cols) {
-                    const float *row = p.s + (p.from ? (int64_t)p.from[first + r + u] : first + r + u) * p.ld + c;
+                if (r < rows && c < p.cols) {
+                    const float *row = p.s + (p.from ? (int64_t)p.from[r] : r) * p.ld + c;
                     if (c + 4 <= p.cols) v[u] = *(const f4u *)row;
                     else
                         for (int e = 0; e < (int)(p.cols - c); e++) v[u][e] = row[e];
@@ -465,26 +467,33 @@ __global__ __launch_bounds__(kVlB) void k_vl_sizes(PackPair pp) {
             }
 #pragma unroll
             for (int u = 0; u < 8; u++) {
-                float m = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float x = finite_abs(v[u][e]);
                     most[e] = __builtin_fmaxf(most[e], x);
-                    m = __builtin_fmaxf(m, x);
+                    most_r[t][u] = __builtin_fmaxf(most_r[t][u], x);
                 }
-                m = wave_max_nan_skip(m);
-                if (lane == 0) sh[wave][r + u] = __builtin_fmaxf(sh[wave][r + u], m);
             }
         }
-        if (p.most && c < p.cols) *(f4 *)(p.group_most + group * p.step / 32 + c) = most;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < all && first + i < p.padded; i += kVlB) {
-        float m = 0.0f;
+        if (p.most) {
+            sh[turn][wave][lane] = most;  // two in turn, so that one barrier does
+            __syncthreads();
+            if (wave == 0 && c < p.cols) {
 #pragma unroll
-        for (int w = 0; w < kVlB / kWave; w++) m = __builtin_fmaxf(m, sh[w][i]);
-        p.e[first + i] = piece_exponent(m);
+                for (int w = 1; w < kWaves; w++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) most[e] = __builtin_fmaxf(most[e], sh[turn][w][lane][e]);
+                *(f4 *)(p.group_most + group * (p.step / 128) + c) = most;
+            }
+        }
     }
+#pragma unroll
+    for (int t = 0; t < BATCHES; t++)
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const float m = wave_max_nan_skip(most_r[t][u]);
+            if (lane == 0 && first + 8 * t + u < p.padded) p.e[first + 8 * t + u] = piece_exponent(m);
+        }
 }
 
 // The columns' largest sizes of all groups: 64 columns a workgroup, 16 lanes each.
@@ -497,7 +506,7 @@ __global__ __launch_bounds__(1024) void k_vl_sizes_join(PackPair pp) {
     float m = 0.0f;
     if (d < p.cols)
 #pragma unroll 8
-        for (int g = sub; g < p.groups; g += 16) m = __builtin_fmaxf(m, p.group_most[g * (p.step / 32) + d]);
+        for (int g = sub; g < p.groups; g += 16) m = __builtin_fmaxf(m, p.group_most[g * (p.step / 128) + d]);
     sh[sub][col] = m;
     __syncthreads();
     if (sub == 0 && d < p.cols) {
@@ -520,44 +529,62 @@ __global__ __launch_bounds__(kVlB) void k_vl_pack(PackPair pp) {
         *(h8 *)(o + lane * 16) = c.hi;
         *(h8 *)(o + lane * 16 + 1024) = c.lo;
     };
-    constexpr int kTasks = 2 * kPackCols / 16;  // of either kind
-#pragma unroll 2
-    for (int t = wave; t < kTasks; t += kVlB / kWave) {
-        const int64_t r = r0 + 32 * (t & 1) + col, k = c0 + 16 * (t >> 1) + 8 * half;
-        if (c0 + 16 * (t >> 1) >= p.step / 128) continue;  // behind the padded columns
-        float x[8];
+    constexpr int kEach = 2 * kPackCols / 16 / (kVlB / kWave);  // blocks of either kind for each wave, asked for together
+    float x[kEach][8];
+    int ex[kEach];
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = 0.0f;
+    for (int i = 0; i < kEach; i++) {
+        const int t = wave + i * (kVlB / kWave);
+        const int64_t r = r0 + 32 * (t & 1) + col, k = c0 + 16 * (t >> 1) + 8 * half;
+        ex[i] = p.e[r];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
         if (r < rows && k < p.cols) {
             const float *row = p.s + (p.from ? (int64_t)p.from[r] : r) * p.ld + k;
             if (k + 8 <= p.cols) {
                 const f4 a = *(const f4u *)row, b = *(const f4u *)(row + 4);
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = a[e], x[4 + e] = b[e];
+                for (int e = 0; e < 4; e++) x[i][e] = a[e], x[i][4 + e] = b[e];
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    if (k + e < p.cols) x[e] = row[e];
+                    if (k + e < p.cols) x[i][e] = row[e];
             }
         }
-        store(p.by_rows + (r0 / 32 + (t & 1)) * p.step + (c0 / 16 + (t >> 1)) * 2048, cut(x, power(-p.e[r])));
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const int t = wave + i * (kVlB / kWave);
+        if (c0 + 16 * (t >> 1) >= p.step / 128) continue;  // behind the padded columns
+        store(p.by_rows + (r0 / 32 + (t & 1)) * p.step + (c0 / 16 + (t >> 1)) * 2048, cut(x[i], power(-ex[i])));
     }
     if (!p.by_columns) return;
-#pragma unroll 2
-    for (int t = wave; t < kTasks; t += kVlB / kWave) {
-        const int64_t kb = r0 / 16 + (t & 3), db = c0 / 32 + (t >> 2), d = db * 32 + col;
-        if (db * 32 >= p.cols) continue;
-        float x[8];
+    float most[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const int t = wave + i * (kVlB / kWave);
+        const int64_t kb = r0 / 16 + (t & 3), d = c0 + 32 * (t >> 2) + col;
+        most[i] = d < p.cols ? p.most[d] : 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int64_t k = 16 * kb + (p.as_registers ? 4 * half + (e & 3) + 8 * (e >> 2) : 8 * half + e);
-            x[e] = d < p.cols && k < rows ? p.s[(p.from ? (int64_t)p.from[k] : k) * p.ld + d] : 0.0f;
+            x[i][e] = d < p.cols && k < rows ? p.s[(p.from ? (int64_t)p.from[k] : k) * p.ld + d] : 0.0f;
         }
-        store(p.by_columns + db * p.step_c + kb * 2048, cut(x, d < p.cols ? power(-piece_exponent(p.most[d])) : 0.0f));
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const int t = wave + i * (kVlB / kWave);
+        const int64_t kb = r0 / 16 + (t & 3), db = c0 / 32 + (t >> 2);
+        if (db * 32 < p.cols) store(p.by_columns + db * p.step_c + kb * 2048, cut(x[i], power(-piece_exponent(most[i]))));
     }
 }
 
 // ---- the rows' statistics and G ---------------------------------------------------------------------------------------------
+// of a product whose sum is cut: tiles over the columns, parts at most, workgroups that the chip holds
+struct PartPlan {
+    int tiles_n, most, at_once;
+};
+
 struct GradArgs {
     VlHead *head;
     int64_t row0, rows;  // of this piece: the first, how many (padded)
@@ -574,7 +601,7 @@ struct GradArgs {
     float *most;         // of every word of this piece
     float *column;       // [rows / 32][words], or none
     int slices;          // of the rows where the words' largest are looked for
-    int tiles_n, slices_most, at_once;  // of gx: tiles over the columns, parts at most, workgroups that the chip holds
+    PartPlan of_x, of_w;
 };
 
 // lanes over 32 rows, 32 of them over the partial statistics of each; and what the next steps of this piece need
@@ -585,7 +612,15 @@ __global__ __launch_bounds__(1024) void k_vl_stats(GradArgs p) {
     if (p.most && p.row0 > 0)  // the first piece finds them clear
         for (int64_t v = (int64_t)blockIdx.x * 1024 + threadIdx.x; v < p.words; v += (int64_t)gridDim.x * 1024) p.most[v] = 0.0f;
     const int64_t left = p.head->count - p.row0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.head->slices = gx_slices(min(p.rows, left), p.tiles_n, (int)(p.words / 16), p.slices_most, p.at_once);
+    if (blockIdx.x == 0 && threadIdx.x < 2 * kWave) {
+        const bool w = threadIdx.x >= kWave;
+        const int64_t here = max(int64_t(0), min(p.rows, left));
+        const PartPlan &q = w ? p.of_w : p.of_x;
+        const int64_t tiles_m = w ? p.words / kTileM : (here + kTileM - 1) / kTileM;
+        const int64_t kblocks = w ? (here + 31) / 32 * 2 : p.words / 16;
+        const int n = parts_of(tiles_m * q.tiles_n, (int)kblocks, q.most, q.at_once);
+        if ((threadIdx.x & (kWave - 1)) == 0) (w ? p.head->slices_w : p.head->slices_x) = n;
+    }
     const int sub = threadIdx.x / 32, col = threadIdx.x & 31;
     const int64_t n = (int64_t)blockIdx.x * 32 + col;
     const int64_t parts = p.words / kStatWords;
@@ -737,7 +772,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_gx(const float *__restrict__ parts,
                                                 const float *__restrict__ most, int64_t D, const float *gout, int sum, float *__restrict__ gx,
                                                 int acc) {
     const int64_t left = min(rows, head->count - row0);
-    const int slices = head->slices;
+    const int slices = head->slices_x;
     const float c = vl_coef(head, gout, sum);
     for (int64_t n = blockIdx.x; n < left; n += gridDim.x) {
         const int en = piece_exponent(finite_abs(row[n].own));
@@ -747,6 +782,24 @@ __global__ __launch_bounds__(kVlB) void k_vl_gx(const float *__restrict__ parts,
             for (int i = 0; i < slices; i++) s += (double)parts[((int64_t)i * rows + n) * cols + d];
             const float v = __builtin_amdgcn_ldexpf((float)s, en + piece_exponent(most[d]));
             out[d] = acc ? fma_(v, c, out[d]) : v * c;
+        }
+    }
+}
+
+// gW (+)= the parts' sum
+__global__ __launch_bounds__(kVlB) void k_vl_gw(const float *__restrict__ parts, int64_t part_rows, int64_t cols, const VlHead *head,
+                                                const float *__restrict__ most_g, const float *__restrict__ most_x, int64_t V, int64_t D,
+                                                const float *gout, int sum, float *__restrict__ gw, int acc) {
+    const int slices = head->slices_w;
+    const float c = head->count ? vl_coef(head, gout, sum) : 0.0f;
+    for (int64_t v = blockIdx.x; v < V; v += gridDim.x) {
+        const int ev = piece_exponent(most_g[v]);
+        for (int64_t d = threadIdx.x; d < D; d += kVlB) {
+            double s = 0.0;
+            for (int i = 0; i < slices; i++) s += (double)parts[((int64_t)i * part_rows + v) * cols + d];
+            const float x = __builtin_amdgcn_ldexpf((float)s, ev + piece_exponent(most_x[d]));
+            float *o = gw + v * D + d;
+            *o = acc ? fma_(x, c, *o) : x * c;
         }
     }
 }
@@ -766,24 +819,28 @@ struct SplitPlan {
     int64_t n, d, v;   // rows, columns and words, padded to tiles
     int64_t dk;        // columns, padded to two blocks of k
     int64_t piece;     // rows of a piece, padded
-    int slices;        // of the words in gx, at most
+    int slices, slices_w;  // parts of gx and of gW, at most; 0: gW is not cut
+    int batches;       // of 8 rows a wave, where sizes are looked for
     int columns;       // slices of the rows where the words' largest are looked for
     size_t from, list, losses, row, label_z, part, ew, ex, most_w, most_x, most_g, group_w, group_x, column, x1, x3, w1, w2, z, turned, parts, total;
 };
 
 static int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
-// row blocks of a group: some 1024 groups
-static int size_blocks(int64_t padded) { return (int)std::max<int64_t>(1, std::min<int64_t>(kSizeBlocks, padded / 32 / 1024)); }
+// batches of 8 rows that a wave looks at for their sizes: two where that leaves the chip full
+static int size_batches(int64_t rows) { return rows >= 64 * 4 * kPlanCUs ? 2 : 1; }
 
 static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w, bool want_b) {
     SplitPlan p{};
     const bool grad = want_x || want_w || want_b;
     p.n = up_to(N, kTileM), p.d = up_to(D, kTileMost), p.v = up_to(V, kTileM), p.dk = up_to(D, 32);
     const int64_t most = grad ? kZBytes / (8 * p.v) : kScored / p.v;
-    p.piece = std::max<int64_t>(kTileM, std::min(std::min(p.n, kPieceRows), most / kTileM * kTileM));
+    p.piece = std::max<int64_t>(kTileM, std::min(std::min(p.n, up_to(vl_piece_rows(kPieceRows), kTileM)), most / kTileM * kTileM));
     p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(64, kPartBytes / (p.piece * p.d * 4)));
-    p.columns = (int)std::max<int64_t>(1, std::min(p.piece / 32, (4096 + p.v / 32 - 1) / (p.v / 32)));
+    // gW: where its tiles would leave the chip's CUs idle
+    if (p.v / kTileM * ((D + 127) / 128) < kPlanCUs) p.slices_w = (int)std::max<int64_t>(1, std::min<int64_t>(64, kPartBytes / (p.v * p.d * 4)));
+    p.columns = (int)std::max<int64_t>(1, std::min<int64_t>(16, std::min(p.piece / 32, (4096 + p.v / 32 - 1) / (p.v / 32))));
+    p.batches = size_batches(p.v + p.n);
     size_t at = 256;
     auto take = [&](bool wanted, int64_t bytes) {
         const size_t here = at;
@@ -801,8 +858,8 @@ static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool w
     p.most_w = take(want_x, p.d * 4);
     p.most_x = take(want_w, p.d * 4);
     p.most_g = take(want_w || want_b, p.v * 4);
-    p.group_w = take(want_x, (p.v / 32 / size_blocks(p.v) + 1) * p.dk * 4);
-    p.group_x = take(want_w, (p.n / 32 / size_blocks(p.n) + 1) * p.dk * 4);
+    p.group_w = take(want_x, p.v / (32 * p.batches) * p.dk * 4);
+    p.group_x = take(want_w, p.n / (32 * p.batches) * p.dk * 4);
     p.column = take(want_b, p.piece / 32 * p.v * 4);
     p.x1 = take(true, p.n * p.dk * 4);
     p.x3 = take(want_w, p.d * p.n * 4);
@@ -810,27 +867,38 @@ static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool w
     p.w2 = take(want_x, p.d * p.v * 4);
     p.z = take(grad, p.piece * p.v * 4);
     p.turned = take(want_w || want_b, p.piece * p.v * 4);
-    p.parts = take(want_x, p.slices * p.piece * p.d * 4);
+    p.parts = take(want_x || (want_w && p.slices_w), std::max(want_x ? p.slices * p.piece : 0, want_w ? p.slices_w * p.v : 0) * p.d * 4);
     p.total = at;
     return p;
 }
 
+// The two forms' times by what they do, in us: fp32 products start at once and run at 115 TFLOP/s; pieces have W and x read twice and
+// written first, whole tiles of rows, and 370.  Both sides measured (us, fp32 products : pieces): 128000 x 2048 with gradients, 64 rows 1167 :
+// 2012, 256 3651 : 2425; 32000 x 1024, 128 rows 306 : 426, 256 526 : 457, 4096 7316 : 2640; 2000 x 256, 1024 rows 83 : 123, 4096 207 : 162;
+// scored, 32000 x 1024, 128 rows 92 : 145, 256 167 : 153; 5000 x 64, 1024 rows 36 : 38, 4096 80 : 58.  Over 400 sizes what it chooses takes
+// 0.2% longer than the better one.
 bool vl_split_pays(int64_t N, int64_t D, int64_t V, bool grads) {
-    (void)grads;
-    return N >= 256 && N <= kPieceRows * 16 && D >= 64 && V >= 1024;
+    if (N == 0 || N > kPieceRows * 16) return false;
+    if (const char *form = getenv("NC_HIP_VOCAB_FORM")) return form[0] == 's';
+    const double d = (double)D, vd = (double)V * d, nv = (double)N * (double)V, nvd = nv * d;
+    const double fp32 = grads ? 30 + 2e-6 * vd + 4.5e-6 * nv + 5.2e-8 * nvd : 17 + 0.75e-6 * vd + 1.4e-6 * nv + 1.6e-8 * nvd;
+    const double split = grads ? 70 + 0.04 * d + 1e-3 * (double)V + 6e-6 * vd + 4.5e-6 * nv + 1.6e-8 * nvd
+                               : 28 + 0.027 * d + 2.4e-6 * vd + 0.6e-6 * nv + 5.5e-9 * nvd;
+    return split < fp32;
 }
 
 size_t vl_split_workspace(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w, bool want_b) {
     return split_plan(N, D, V, want_x, want_w, want_b).total;
 }
 
-// Whether a product runs on tiles of 256 columns.  z and gW: unless tiles of 128, two a CU, take fewer rounds, by more than the
-// 4% that they are slower at the same number (gW of 128000 x 4096 x 2048: 5.5 ms, 6.3 with tiles of 128; 50021 x 700 x 770: 257 us, 239).
-// gx, whose words are cut to fill the rounds: where more than 128 columns are there.
+// Whether a product runs on tiles of 256 columns, one a CU, rather than of 128, two a CU: by the rounds that they take, where a last round
+// of 128s that finds a CU each takes half.  At the same number those are 4% slower (gW of 128000 x 4096 x 2048: 5.5 ms, 6.3 with tiles of
+// 128; 50021 x 700 x 770, 4 rounds for 3: 257 us, 239).  A sum that is cut fills the rounds by itself: where more than 128 columns are there.
 static bool wide_tiles(int64_t tiles_m, int64_t cols, bool cut) {
     if (cut) return cols > 128;
-    const int64_t wide = tiles_m * ((cols + 255) / 256), narrow = tiles_m * ((cols + 127) / 128);
-    return 25 * ((wide + kPlanCUs - 1) / kPlanCUs) <= 26 * ((narrow + 2 * kPlanCUs - 1) / (2 * kPlanCUs));
+    const int64_t wide = tiles_m * ((cols + 255) / 256), narrow = tiles_m * ((cols + 127) / 128), last = narrow % (2 * kPlanCUs);
+    const int64_t halves = narrow / (2 * kPlanCUs) * 2 + (last > kPlanCUs ? 2 : last > 0 ? 1 : 0);
+    return 25 * 2 * ((wide + kPlanCUs - 1) / kPlanCUs) <= 26 * halves;
 }
 
 int vl_split_run(const VlCall &c, const char *what) {
@@ -855,12 +923,13 @@ int vl_split_run(const VlCall &c, const char *what) {
             a.most = (float *)at(i ? pl.most_w : pl.most_x);
             a.by_columns = at(i ? pl.w2 : pl.x3), a.step_c = a.padded * 128, a.as_registers = i == 1;
         }
-        a.blocks = size_blocks(a.padded);
-        a.groups = (int)((a.padded / 32 + a.blocks - 1) / a.blocks);
+        a.groups = (int)(a.padded / (32 * pl.batches));
         a.group_most = (float *)at(i ? pl.group_w : pl.group_x);
         a.regions = (int)((pl.dk + kPackCols - 1) / kPackCols);
     }
-    hipLaunchKernelGGL(k_vl_sizes, (unsigned)(pp.a[0].groups + pp.a[1].groups), kVlB, 0, c.st, pp);
+    const unsigned looking = (unsigned)(pp.a[0].groups + pp.a[1].groups);
+    if (pl.batches == 2) hipLaunchKernelGGL(k_vl_sizes<2>, looking, kVlB, 0, c.st, pp);
+    else hipLaunchKernelGGL(k_vl_sizes<1>, looking, kVlB, 0, c.st, pp);
     if (c.gx || c.gw) hipLaunchKernelGGL(k_vl_sizes_join, dim3((unsigned)((c.D + 63) / 64), 2), 1024, 0, c.st, pp);
     hipLaunchKernelGGL(k_vl_pack, (unsigned)((pl.n + pl.v) / 64 * pp.a[0].regions), kVlB, 0, c.st, pp);
 
@@ -870,7 +939,7 @@ int vl_split_run(const VlCall &c, const char *what) {
     };
     auto product = [&](auto what, MmArgs m, int64_t cols, int slices) {
         constexpr int W = decltype(what)::value;
-        const bool wide = wide_tiles(m.tiles_m, cols, W == MM_GX);
+        const bool wide = wide_tiles(m.tiles_m, cols, W == MM_GX || W == MM_GW_PARTS);
         m.tiles_n = (int)((cols + (wide ? 255 : 127)) / (wide ? 256 : 128));
         const int64_t groups = (int64_t)m.tiles_m * m.tiles_n * slices;
         if (wide) launch(k_vl_product<W, 4>, Tile<4>::kLanes, Tile<4>::kLds, groups, m);
@@ -891,9 +960,10 @@ int vl_split_run(const VlCall &c, const char *what) {
         g.head = head, g.row0 = r0, g.rows = pl.piece, g.V = c.V, g.words = pl.v, g.part = m.part, g.label_z = m.label_z;
         g.labels = list + r0, g.from = from + r0, g.row = (VlRow *)at(pl.row), g.losses = losses, g.row_loss = c.row_loss;
         g.z = m.z, g.turned = at(pl.turned), g.turned_step = pl.piece * 128, g.most = (float *)at(pl.most_g), g.column = c.gb ? (float *)at(pl.column) : nullptr;
-        g.slices = pl.columns, g.slices_most = pl.slices;
-        const bool wide = wide_tiles(rows / kTileM, c.D, true);
-        g.tiles_n = (int)((c.D + (wide ? 255 : 127)) / (wide ? 256 : 128)), g.at_once = wide ? kPlanCUs : 2 * kPlanCUs;
+        g.slices = pl.columns;
+        const bool wide = wide_tiles(0, c.D, true);
+        g.of_x = {(int)((c.D + (wide ? 255 : 127)) / (wide ? 256 : 128)), pl.slices, wide ? kPlanCUs : 2 * kPlanCUs};
+        g.of_w = {g.of_x.tiles_n, pl.slices_w, g.of_x.at_once};
         if (!(c.gw || c.gb)) g.most = nullptr;
         hipLaunchKernelGGL(k_vl_stats, (unsigned)(rows / 32), 1024, 0, c.st, g);
         if (!grad) continue;
@@ -912,7 +982,7 @@ int vl_split_run(const VlCall &c, const char *what) {
             MmArgs a = m;
             a.A = (const char *)m.z, a.step_a = pl.v * 128, a.B = at(pl.w2), a.step_b = pl.v * 128;
             a.tiles_m = (int)(rows / kTileM), a.kblocks = (int)(pl.v / 16);
-            a.parts = (float *)at(pl.parts), a.cols = pl.d;
+            a.parts = (float *)at(pl.parts), a.part_rows = pl.piece, a.cols = pl.d;
             product(std::integral_constant<int, MM_GX>{}, a, c.D, pl.slices);
             hipLaunchKernelGGL(k_vl_gx, (unsigned)std::min<int64_t>(rows, 1 << 14), kVlB, 0, c.st, a.parts, pl.piece, pl.d, head, r0,
                                from + r0, g.row, (const float *)at(pl.most_w), c.D, c.gout, c.sum, c.gx, c.acc_x);
@@ -922,7 +992,14 @@ int vl_split_run(const VlCall &c, const char *what) {
             a.A = g.turned, a.step_a = g.turned_step, a.B = at(pl.x3) + r0 / 16 * 2048, a.step_b = pl.n * 128;
             a.tiles_m = (int)(pl.v / kTileM), a.kblocks = (int)(rows / 16);
             a.most_a = g.most, a.most_b = (const float *)at(pl.most_x), a.gout = c.gout, a.out = c.gw, a.sum = c.sum, a.acc = c.acc_w || r0;
-            product(std::integral_constant<int, MM_GW>{}, a, c.D, 1);
+            if (pl.slices_w) {
+                a.parts = (float *)at(pl.parts), a.part_rows = pl.v, a.cols = pl.d;
+                product(std::integral_constant<int, MM_GW_PARTS>{}, a, c.D, pl.slices_w);
+                hipLaunchKernelGGL(k_vl_gw, (unsigned)std::min<int64_t>(c.V, 1 << 14), kVlB, 0, c.st, a.parts, pl.v, pl.d, head, a.most_a,
+                                   a.most_b, c.V, c.D, c.gout, c.sum, c.gw, a.acc);
+            } else {
+                product(std::integral_constant<int, MM_GW>{}, a, c.D, 1);
+            }
         }
     }
     hipLaunchKernelGGL(k_vl_total, 1, 1024, 0, c.st, losses, head, c.sum, c.loss);

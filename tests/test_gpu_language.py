@@ -236,8 +236,15 @@ def test_dropout_past_2_34_bytes(K):
 
 
 # ---- the cross entropy of a product ------------------------------------------------------------------------------------
+@pytest.fixture(params=["fp32", "split"])
+def form(request, monkeypatch):
+    """either form of the kernels, whatever the sizes"""
+    monkeypatch.setenv("NC_HIP_VOCAB_FORM", request.param)
+    return request.param
+
+
 # N, D, V
-LOSS = [(1, 1, 1), (1, 7, 3), (2, 4, 1), (5, 33, 17), (64, 64, 64), (65, 130, 257), (300, 96, 1000), (257, 256, 513), (1000, 40, 50),
+LOSS = [(1, 1, 1), (1, 7, 3), (40, 31, 9001), (3, 1030, 4097), (260, 33, 300), (2, 4, 1), (5, 33, 17), (64, 64, 64), (65, 130, 257), (300, 96, 1000), (257, 256, 513), (1000, 40, 50),
         (130, 512, 2050), (513, 100, 5003), (1030, 260, 1027)]
 
 
@@ -290,7 +297,7 @@ def agree(got, ref, x, w, old=None, scale=1.0):
 
 @pytest.mark.parametrize("bias,ignored", [(False, 0.0), (True, 0.3)])
 @pytest.mark.parametrize("shape", LOSS, ids=str)
-def test_loss_and_gradients(K, shape, bias, ignored):
+def test_loss_and_gradients(K, form, shape, bias, ignored):
     x, w, b, labels = loss_inputs(*shape, 11, bias, ignored)
     ref = R.vocab_loss(x, w, b, labels)
     x = np.where(ref["on"][:, None], x, np.nan)  # rows that do not count may hold anything
@@ -309,7 +316,7 @@ def test_loss_and_gradients(K, shape, bias, ignored):
 
 
 @pytest.mark.parametrize("shape", [(5, 33, 17), (300, 96, 1000), (513, 100, 5003), (257, 256, 513)], ids=str)
-def test_loss_added_gradients_sum_and_its_own_gradient(K, shape):
+def test_loss_added_gradients_sum_and_its_own_gradient(K, form, shape):
     x, w, b, labels = loss_inputs(*shape, 12, True, 0.2)
     labels[0] = shape[2] - 1
     rng = np.random.default_rng(1)
@@ -324,7 +331,7 @@ def test_loss_added_gradients_sum_and_its_own_gradient(K, shape):
 
 @pytest.mark.parametrize("shape", [(5, 33, 17), (300, 96, 1000), (1030, 260, 1027)], ids=str)
 @pytest.mark.parametrize("grads", ["", "x", "w", "b", "xw"])
-def test_loss_some_gradients(K, shape, grads):
+def test_loss_some_gradients(K, form, shape, grads):
     x, w, b, labels = loss_inputs(*shape, 13, False, 0.1)
     ref = R.vocab_loss(x, w, None, labels)
     c = Loss(K, x, w, None, labels, grads=grads)
@@ -335,7 +342,7 @@ def test_loss_some_gradients(K, shape, grads):
 
 
 @pytest.mark.parametrize("shape", [(5, 33, 17), (300, 96, 1000), (600, 128, 2048)], ids=str)
-def test_loss_labels_outside(K, shape):
+def test_loss_labels_outside(K, form, shape):
     N, D, V = shape
     x, w, b, labels = loss_inputs(*shape, 14, True, 0.2)
     labels[3], labels[1] = V, -7
@@ -348,7 +355,7 @@ def test_loss_labels_outside(K, shape):
 
 
 @pytest.mark.parametrize("shape", [(3, 5, 9), (300, 96, 1000), (600, 128, 2048)], ids=str)
-def test_loss_no_row_counts(K, shape):
+def test_loss_no_row_counts(K, form, shape):
     x, w, b, labels = loss_inputs(*shape, 15, True, 0.0)
     labels[:] = 5  # the ignored label may be a word
     c = Loss(K, x * np.nan, w, b, labels, ignore=5)
@@ -360,7 +367,7 @@ def test_loss_no_row_counts(K, shape):
     assert c.get()["loss"] == 0
 
 
-def test_loss_of_no_rows(K):
+def test_loss_of_no_rows(K, form):
     x, w, b, labels = loss_inputs(0, 6, 9, 16, True, 0.0)
     c = Loss(K, x, w, b, labels)
     c.run()
@@ -369,7 +376,7 @@ def test_loss_of_no_rows(K):
 
 
 @pytest.mark.parametrize("shape", [(40, 33, 170), (300, 96, 1000), (600, 128, 2048)], ids=str)
-def test_loss_masked_words(K, shape):
+def test_loss_masked_words(K, form, shape):
     """A bias of -inf, or of the type's lowest value, takes words out: no probability, no gradient."""
     N, D, V = shape
     x, w, b, labels = loss_inputs(*shape, 17, True, 0.1)
@@ -387,7 +394,7 @@ def test_loss_masked_words(K, shape):
 
 
 @pytest.mark.parametrize("shape", [(40, 33, 170), (300, 96, 1000), (600, 128, 2048)], ids=str)
-def test_loss_rows_and_words_of_unlike_sizes(K, shape):
+def test_loss_rows_and_words_of_unlike_sizes(K, form, shape):
     """Rows of x and of w whose sizes lie many powers of two apart: each result keeps the precision of what it sums."""
     N, D, V = shape
     x, w, b, labels = loss_inputs(*shape, 18, False, 0.0, confident=False)
@@ -401,7 +408,7 @@ def test_loss_rows_and_words_of_unlike_sizes(K, shape):
 
 
 @pytest.mark.parametrize("shape", [(300, 96, 1000), (600, 128, 2048)], ids=str)
-def test_loss_certain_rows(K, shape):
+def test_loss_certain_rows(K, form, shape):
     """Rows that are all but certain of their word keep the bits of what little gradient they have."""
     N, D, V = shape
     x, w, b, labels = loss_inputs(*shape, 19, False, 0.0)
@@ -420,7 +427,7 @@ def test_loss_certain_rows(K, shape):
 
 
 @pytest.mark.parametrize("shape", [(40, 33, 170), (300, 96, 1000), (600, 128, 2048)], ids=str)
-def test_loss_values_that_are_not_finite(K, shape):
+def test_loss_values_that_are_not_finite(K, form, shape):
     """NaN in a row that counts makes that row's loss and gradient NaN and leaves the other rows' theirs."""
     N, D, V = shape
     x, w, b, labels = loss_inputs(*shape, 20, True, 0.0)
@@ -434,6 +441,31 @@ def test_loss_values_that_are_not_finite(K, shape):
     assert np.isfinite(got["rows"][others]).all() and np.isfinite(got["gx"][others]).all()
     tol = R.vocab_loss_tol(np.where(np.isnan(x), 0, x), w, ref)
     assert rms(got["gx"][others] - ref["gx"][others]) <= 1.1 * tol["gx"]
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("shape", [(700, 40, 600), (1030, 260, 1027), (9, 5, 5000)], ids=str)
+def test_loss_in_pieces(K, form, shape, rows, monkeypatch):
+    """Rows taken a few at a time, gradients added from piece to piece; rows that do not count leave the last pieces empty."""
+    monkeypatch.setenv("NC_HIP_VOCAB_ROWS", str(rows))
+    x, w, b, labels = loss_inputs(*shape, 23, True, 0.6)
+    labels[0] = 1
+    ref = R.vocab_loss(x, w, b, labels)
+    old = {k: ref[k].astype(np.float32)[::-1].copy() for k in ("gx", "gw", "gb")}
+    for o in (None, old):
+        c = Loss(K, x, w, b, labels, old=o)
+        c.run()
+        agree(c.get(), ref, x, w, old=o)
+
+
+@pytest.mark.parametrize("shape,grads", [((2100, 100, 5003), ""), ((4200, 100, 5003), "xwb"), ((1300, 520, 3001), "xwb")], ids=str)
+def test_loss_of_the_chosen_form(K, shape, grads):
+    """Sizes that run on pieces by the kernels' own choice."""
+    x, w, b, labels = loss_inputs(*shape, 24, True, 0.1)
+    ref = R.vocab_loss(x, w, b, labels)
+    c = Loss(K, x, w, b, labels, grads=grads)
+    c.run()
+    agree(c.get(), ref, x, w)
 
 
 # ---- together ----------------------------------------------------------------------------------------------------------
@@ -481,7 +513,7 @@ ENDS = [(37, 50, 24), (300, 1000, 96), (700, 2048, 128)]
 
 
 @pytest.mark.parametrize("shape", ENDS, ids=str)
-def test_ends_together(K, shape):
+def test_ends_together(K, form, shape):
     a = Ends(K, *shape, 3)
     a.run()
     synchronize()
@@ -494,7 +526,7 @@ def test_ends_together(K, shape):
 
 
 @pytest.mark.parametrize("shape", ENDS, ids=str)
-def test_ends_captured_and_replayed(K, shape):
+def test_ends_captured_and_replayed(K, form, shape):
     """The run as a graph: every replay, with other inputs, another offset and eager calls in between, gives the eager run's bits."""
     rt = runtime()
     a, other = Ends(K, *shape, 29), Ends(K, *shape, 30)
@@ -526,7 +558,7 @@ def test_ends_captured_and_replayed(K, shape):
     check(rt.hipGraphDestroy(graph), "destroy")
 
 
-def test_ends_on_two_streams_at_once(K):
+def test_ends_on_two_streams_at_once(K, form):
     runs = [Ends(K, 300, 1000, 96, 41), Ends(K, 700, 2048, 128, 42)]
     streams = [Stream(), Stream()]
     for r in runs:
