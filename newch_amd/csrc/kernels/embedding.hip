@@ -48,7 +48,7 @@ __device__ __forceinline__ f4 piece(const float *row, int64_t c, int64_t D) {
 
 template <bool AL>
 __device__ __forceinline__ void put(float *row, int64_t c, int64_t D, f4 v) {
-    if (AL) *(f4 *)(row + c) = v;
+    if (AL) __builtin_nontemporal_store(v, (f4 *)(row + c));
     else if (c + 4 <= D) *(f4u *)(row + c) = v;
     else
         for (int e = 0; e < (int)(D - c); e++) row[c + e] = v[e];
