@@ -1,20 +1,25 @@
 // The vocabulary loss with its three products on the fp16 matrix cores: z = x W^T, gx = G W, gW = G^T x.
 //
-// A library's fp32 product of 8192^3 reaches an eighth of what its fp16 one does, so every operand is cut into two fp16 pieces under
-// a power of two of its row (the index that is not summed over): x = 2^e (hi + lo), the row's largest finite value in [2^14, 2^15)
-// after the scaling, hi and lo rounded to nearest: 22 bits of every value down to 2^-17 of its row's largest, an absolute error of
-// 2^-40 of that below.  A product is hi hi + hi lo + lo hi, summed in fp32; lo lo, at most 2^-22 of a term, is left out.
+// A library's fp32 product of 8192^3 reaches an eighth of what its fp16 one does, so operands are cut into two fp16 pieces under a
+// power of two of their row: x = 2^e (hi + lo), the row's largest finite value in [2^14, 2^15) after the scaling, hi and lo rounded to
+// nearest: 22 bits of every value down to 2^-17 of its row's largest, an absolute error of 2^-40 of that below.  A product is hi hi +
+// hi lo + lo hi, summed in fp32; lo lo, at most 2^-22 of a term, is left out.
 //
-// Packed operands.  A block of 32 rows by 16 k is 2 KiB: its hi pieces, then its lo pieces, each as a wave holds them for
-// v_mfma_f32_32x32x16_f16 -- lane l has row l % 32 and eight k of half l / 32 in 16 bytes.  So a block is loaded into LDS as it lies, a
-// KiB an instruction, and read from there as it lies, without bank conflicts.  z is left by the first product in the registers' order,
-// 4 KiB a block of 32 rows n by 32 words v: lane l has n = l % 32 and v = 8 q + 4 (l / 32) + e, q and e < 4.  Quads 2 s and 2 s + 1 are then
-// eight k of a block of 16 words, in the order 4 (l / 32) + {0, 1, 2, 3, 8, 9, 10, 11}, which the packed W that they meet has too.
+// x and W are packed once, by rows.  gx and gW sum over those rows, so G takes their powers of two: gx_n = sum_v (G_nv 2^e_v) pieces of W_v,
+// where the row n of G 2^e has the power of its own largest entry, which is that of the largest term that gx_n sums; gW in
+// the same way.  So rows of x or W far larger than those that a result counts leave those their bits.
 //
-// Steps of a call: labels that count are listed (rows that do not count take part in nothing); x and W are packed, by rows and by
-// columns; then for pieces of the rows z (with each row's maximum and sum of exponentials over every 128 words), the rows' statistics,
-// G's largest entry of every word, G in pieces for both products (in z's place, and turned for gW), gx in parts over the words and their
-// sum, gW.  Scoring ends with the rows' statistics and leaves no z.
+// A packed block, 32 rows by 16 k, is 2 KiB: for each half of the rows 256 bytes of hi of k 0 .. 7, of hi of k 8 .. 15, and of lo of both;
+// a row's eight k are 16 bytes, at place r % 16 ^ 8 (k / 8).  Blocks go into LDS as they lie, a KiB an instruction, and give
+// v_mfma_f32_32x32x16_f16's fragments from there: rows that are not summed over by one 16-byte read of a lane (row l % 32, k of half
+// l / 32), rows that are by two transposing 8-byte reads (column l % 32 of 32, rows 4 (l / 32) + {0, 1, 2, 3, 8, 9, 10, 11} of a half).
+// That is the order in which a result's registers hold rows, so z's blocks are left as the registers hold them -- 32 rows n by 32 words v
+// in 4 KiB, lane l with n = l % 32 and v = 8 q + 4 (l / 32) + e, q and e < 4 -- and G's pieces take z's place without leaving their lanes.
+//
+// Steps of a call: labels that count are listed (rows that do not count take part in nothing); x and W are packed; then for pieces of the
+// rows z, with each row's maximum, sum of exponentials and largest term of gx over every 128 words; the rows' statistics; the largest
+// terms of gW of every word; G in pieces for both products (in z's place, and turned for gW); gx in parts over the words and their
+// sum; gW.  Scoring ends with the rows' statistics and leaves no z.
 #include "vocab_loss.hpp"
 
 namespace nchip {
@@ -39,13 +44,21 @@ constexpr int64_t kZBytes = int64_t(4) << 30;  // of z and of the turned G, both
 constexpr int64_t kScored = int64_t(1) << 36;  // products of a launch that leaves no z
 constexpr int64_t kPieceRows = 1 << 20;
 constexpr int64_t kPartBytes = int64_t(512) << 20;  // of the parts of gx
-constexpr int kPackCols = 128;
 constexpr int kStatWords = 128;  // words of one partial statistic
+
+constexpr float kLog2e = 1.44269504088896341f;
 
 struct VlRow {
     float m, ls;  // the row's maximum and log sum exp(z - m)
-    float own;    // p_l - 1, the largest of its row of G
-    int label;
+    float own;    // p_l - 1
+    int label;    // -1: no row
+    int e;        // the power of two of its row of G 2^e_v
+    int ex;       // of its row of x
+    int pad[2];
+};
+// of 128 words of a row: the maximum, the sum of exponentials from there, the largest term of gx (a base-2 logarithm from there)
+struct VlPart {
+    float m, s, c;
 };
 
 // the exponent e that puts `most` (finite, >= 0) into [2^14, 2^15) when values are divided by 2^e
@@ -58,6 +71,11 @@ __device__ __forceinline__ float finite_abs(float x) {
     const float a = __builtin_fabsf(x);
     return a < __builtin_inff() ? a : 0.0f;
 }
+
+// The largest of a word's or a row's terms is kept as the whole part of its base-2 logarithm; kNoTerm: there is none.
+constexpr int kNoTerm = -400;
+__device__ __forceinline__ int term_exponent(float log2) { return log2 > (float)kNoTerm ? (int)__builtin_floorf(__builtin_fminf(log2, 400.0f)) : kNoTerm; }
+__device__ __forceinline__ int word_exponent(int term) { return term - 14; }
 
 struct Pieces {
     h8 hi, lo;
@@ -72,6 +90,17 @@ __device__ __forceinline__ Pieces cut(const float (&x)[8], float scale) {
         r.lo[i] = (_Float16)(v - (float)h);
     }
     return r;
+}
+
+// a lane's place in a packed block: row l % 32, k of half l / 32
+__device__ __forceinline__ int block_at(int lane) {
+    const int half = lane >> 5, r = lane & 31;
+    return (r >> 4) * 1024 + half * 256 + ((r & 15) ^ (8 * half)) * 16;
+}
+__device__ __forceinline__ void store_block(char *block, int lane, const Pieces &c) {
+    char *o = block + block_at(lane);
+    *(h8 *)o = c.hi;
+    *(h8 *)(o + 512) = c.lo;
 }
 
 // ---- the product ------------------------------------------------------------------------------------------------------
@@ -91,14 +120,14 @@ struct MmArgs {
     const int32_t *labels;  // of this piece's rows
     float *z;               // or none
     int64_t zwords;         // blocks of 32 words of a row block
-    f2 *part;               // [words / kStatWords][rows]
+    VlPart *part;           // [words / kStatWords][rows]
     float *label_z;         // [rows]
     int64_t rows;           // of a piece, padded
-    // MM_GX: A the rows, B the columns; MM_GW_PARTS: A the words
-    float *parts;           // [slices][rows or words][columns]
+    // MM_GX: A the rows, B the words; MM_GW: A the words, B the rows; of B the columns, `blocks` of 16
+    int blocks;
+    float *parts;           // MM_GX, MM_GW_PARTS: [slices][rows or words][columns]
     int64_t part_rows, cols;  // rows or words, and columns, padded
-    // MM_GW: A the words, B the columns
-    const float *most_a, *most_b;
+    const int *eg;          // MM_GW: the largest terms' exponents of the words
     const float *gout;
     float *out;
     int sum, acc;
@@ -155,14 +184,24 @@ __device__ __forceinline__ void z_out(const MmArgs &p, f16x (&acc)[4][2], int64_
                         acc[i][j][r] = -__builtin_inff();
                     }
         }
-        float s = 0.0f;
+        float s = 0.0f, c = -__builtin_inff();
         const float base = m == -__builtin_inff() ? 0.0f : m;  // words that are all -inf have no part in the row's sum
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) s += exp_sum_term(acc[i][j][r] - base);
+            for (int q = 0; q < 4; q++) {
+                i4v ew = {};
+                if (p.z) ew = *(const i4v *)(p.ew + v0 + 32 * i + 8 * q + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float t = (acc[i][j][4 * q + e] - base) * kLog2e;
+                    s += __builtin_amdgcn_exp2f(t);
+                    if (p.z) c = __builtin_fmaxf(c, t + (float)ew[e]);
+                }
+            }
         s += __shfl_xor(s, 32);
-        if (half == 0) p.part[(v0 / kStatWords) * p.rows + n] = f2{m, s};
+        c = __builtin_fmaxf(c, __shfl_xor(c, 32));
+        if (half == 0) p.part[(v0 / kStatWords) * p.rows + n] = {m, s, c};
     }
 }
 
@@ -213,7 +252,15 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
 
     // each wave brings its share of a stage: the pieces of kA row blocks of A and of one of B
     const char *src_a = p.A + ((int64_t)tm * (kTileM / 32) + T::kA * wave) * p.step_a + (int64_t)k0 * 2048 + lane * 16;
-    const char *src_b = p.B + ((int64_t)tn * (T::kN / 32) + wave) * p.step_b + (int64_t)k0 * 2048 + lane * 16;
+    // of B: its row block's 2 KiB, or, where B's rows are summed over, half a block, 16 rows, of two blocks of columns (behind the
+    // last columns the last block again)
+    constexpr bool kTurned = WHAT != MM_Z;
+    const int db = min(p.blocks - 1, tn * (T::kN / 16) + 2 * wave), db1 = min(p.blocks - 1, db + 1);
+    const char *src_b = kTurned ? p.B + k0 / 2 * p.step_b + db * 2048 + lane * 16
+                                : p.B + ((int64_t)tn * (T::kN / 32) + wave) * p.step_b + (int64_t)k0 * 2048 + lane * 16;
+    const int next_b = kTurned ? (db1 - db) * 2048 : 1024;
+    const int64_t odd_b = kTurned ? p.step_b - 1024 : 2048, even_b = kTurned ? 1024 : 2048;
+    int brought = 0;
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     const uint32_t to_a = base + (uint32_t)wave * (2048 * T::kA), to_b = base + T::kStageA + (uint32_t)wave * 2048;
     auto bring = [&](uint32_t stage) {
@@ -224,21 +271,35 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
             dma16(src_a + i * p.step_a + 1024, a + 2048 * i + 1024);
         }
         dma16(src_b, b);
-        dma16(src_b + 1024, b + 1024);
-        src_a += 2048, src_b += 2048;
+        dma16(src_b + next_b, b + 1024);
+        src_a += 2048, src_b += brought++ & 1 ? odd_b : even_b;
     };
-    const char *const my_a = lds + wm * 8192 + lane * 16, *const my_b = lds + T::kStageA + wn * 4096 + lane * 16;
+    const char *const my_a = lds + wm * 8192 + block_at(lane), *const my_b = lds + T::kStageA + wn * 4096;
+    // the transposing reads' places: 16 lanes bring four rows of 16 columns, four columns a lane
+    const int u = (lane >> 1) & 1, row = 4 * (lane >> 5) + (lane & 15) / 4;
+    const int turned = ((lane >> 4) & 1) * 1024 + u * 256 + (row + 8 * u) * 16 + 8 * (lane & 1);
     auto fetch = [&](uint32_t stage, Frags &f) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             f.a[i][0] = *(const h8 *)(my_a + stage + i * 2048);
-            f.a[i][1] = *(const h8 *)(my_a + stage + i * 2048 + 1024);
+            f.a[i][1] = *(const h8 *)(my_a + stage + i * 2048 + 512);
         }
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            f.b[j][0] = *(const h8 *)(my_b + stage + j * 2048);
-            f.b[j][1] = *(const h8 *)(my_b + stage + j * 2048 + 1024);
-        }
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                if constexpr (kTurned) {
+                    typedef short s4 __attribute__((ext_vector_type(4)));
+                    typedef short s8 __attribute__((ext_vector_type(8)));
+                    typedef __attribute__((address_space(3))) s4 lds_s4;
+                    const char *q = my_b + stage + j * 2048 + t * 512 + turned;
+                    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(q));
+                    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(q + 128 - 256 * u));
+                    f.b[j][t] = __builtin_bit_cast(h8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+                } else {
+                    f.b[j][t] = *(const h8 *)(my_b + stage + j * 2048 + t * 512 + block_at(lane));
+                }
+            }
     };
     f16x acc[4][2];
 #pragma unroll
@@ -321,7 +382,6 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
         const int64_t m1 = m0 + 4 * (at >> 5), d = n0 + (at & 31);
         float *out = p.out + m1 * p.D + d;
         const bool in0 = d < p.D, in1 = d + 32 < p.D;
-        const int ed0 = piece_exponent(in0 ? p.most_b[d] : 0.0f), ed1 = piece_exponent(in1 ? p.most_b[d + 32] : 0.0f);
         // the old values of 16 rows are asked for together
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -339,9 +399,9 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
             for (int r = 0; r < 16; r++) {
                 const int dm = 32 * i + 8 * (r / 4) + r % 4;
                 if (m1 + dm >= p.V) continue;
-                const int em = piece_exponent(p.most_a[m1 + dm]);
+                const int em = word_exponent(p.eg[m1 + dm]);
                 float *o = out + (int64_t)dm * p.D;
-                const float v0 = __builtin_amdgcn_ldexpf(acc[i][0][r], ed0 + em), v1 = __builtin_amdgcn_ldexpf(acc[i][1][r], ed1 + em);
+                const float v0 = __builtin_amdgcn_ldexpf(acc[i][0][r], em), v1 = __builtin_amdgcn_ldexpf(acc[i][1][r], em);
                 if (in0) o[0] = p.acc ? fma_(v0, c, old[0][r]) : v0 * c;
                 if (in1) o[32] = p.acc ? fma_(v1, c, old[1][r]) : v1 * c;
             }
@@ -351,16 +411,16 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
 
 // ---- which rows count ----------------------------------------------------------------------------------------------------
 // Workgroup 0 lists the rows that count and their labels (-1 behind the last), and looks for the first label that is neither a word
-// nor `ignore`; the others clear what starts at zero: `zeros`, the losses and gradients of the rows that do not count.
+// nor `ignore`; the others set what grows from nothing: the words' largest terms, the losses and gradients of the rows that do not count.
 __global__ __launch_bounds__(1024) void k_vl_begin(const int32_t *__restrict__ labels, int64_t N, int64_t padded, int64_t D, int64_t V,
                                                    int32_t ignore, VlHead *head, int32_t *__restrict__ from, int32_t *__restrict__ list,
-                                                   unsigned long long *bad, float *__restrict__ zeros, int64_t n_zeros,
+                                                   unsigned long long *bad, int *__restrict__ terms, int64_t n_terms,
                                                    float *__restrict__ row_loss, float *__restrict__ gx) {
     constexpr int kB = 1024, kWaves = kB / kWave;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     if (blockIdx.x > 0) {
         const int64_t block = blockIdx.x - 1, blocks = gridDim.x - 1;
-        for (int64_t i = block * kB + threadIdx.x; i < n_zeros; i += blocks * kB) zeros[i] = 0.0f;
+        for (int64_t i = block * kB + threadIdx.x; i < n_terms; i += blocks * kB) terms[i] = kNoTerm;
         for (int64_t i = block * kWaves + wave; i < N; i += blocks * kWaves) {
             if (vl_counts(labels[i], ignore, V)) continue;
             if (row_loss && lane == 0) row_loss[i] = 0.0f;
@@ -409,173 +469,73 @@ __global__ __launch_bounds__(1024) void k_vl_begin(const int32_t *__restrict__ l
 }
 
 // ---- operands in pieces ----------------------------------------------------------------------------------------------------
-// A matrix to be packed by its rows (summed over by columns) and, where `turned` is set, by its columns.
 struct PackArgs {
     const float *s;
     int64_t ld, rows, cols;
     const int32_t *from;  // the rows' places, or none: as they lie
     const VlHead *head;   // counts the rows where they are listed
     int *e;               // the rows' exponents
-    float *most;          // the columns' largest sizes, or none
-    float *group_most;    // of each group of rows, [groups][padded columns]
-    char *by_rows, *by_columns;  // by_columns: or none
-    int64_t step, step_c;  // bytes from a block of 32 rows (columns) to the next
-    int64_t padded;       // rows, padded
-    int groups;           // workgroups that look at sizes
-    int regions;          // of 64 columns
-    bool as_registers;    // the k of by_columns in the order that z's registers have
+    char *out;
+    int groups;           // of 32 rows, padded
 };
 struct PackPair {
     PackArgs a[2];  // x, W
+    int kblocks;
 };
 
-__device__ __forceinline__ int64_t row_count(const PackArgs &p) { return p.from ? p.head->count : p.rows; }
-
-// The largest sizes of rows and columns: a wave goes down 8 BATCHES rows, 256 columns at a time, and the columns' sizes of the four
-// waves meet in LDS.
-template <int BATCHES>
-__global__ __launch_bounds__(kVlB) void k_vl_sizes(PackPair pp) {
-    constexpr int kWaves = kVlB / kWave;
-    __shared__ f4 sh[2][kWaves][kWave];
+// A workgroup's 32 rows.  A lane has eight k of its row in every eighth block, up to NB of them in registers (NB 0: more, read again once
+// the rows' largest values are known).
+template <int NB>
+__global__ __launch_bounds__(512) void k_vl_pack(PackPair pp) {
+    constexpr int kWaves = 8, kHold = NB ? NB : 4;
+    __shared__ float sh[2 * kWaves][32];
     const bool second = (int)blockIdx.x >= pp.a[0].groups;
     const PackArgs &p = pp.a[second];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int64_t group = blockIdx.x - (second ? pp.a[0].groups : 0), first = (group * kWaves + wave) * (8 * BATCHES);
-    const int64_t rows = row_count(p);
-    float most_r[BATCHES][8];
-#pragma unroll
-    for (int t = 0; t < BATCHES; t++)
-#pragma unroll
-        for (int u = 0; u < 8; u++) most_r[t][u] = 0.0f;
-    int turn = 0;
-    for (int64_t c0 = 0; c0 < p.cols; c0 += 256, turn ^= 1) {
-        const int64_t c = c0 + 4 * lane;
-        f4 most = {};
-#pragma unroll
-        for (int t = 0; t < BATCHES; t++) {
-            f4 v[8];
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const int64_t r = first + 8 * t + u;
-                v[u] = f4{};
-                if (r < rows && c < p.cols) {
-                    const float *row = p.s + (p.from ? (int64_t)p.from[r] : r) * p.ld + c;
-                    if (c + 4 <= p.cols) v[u] = *(const f4u *)row;
-                    else
-                        for (int e = 0; e < (int)(p.cols - c); e++) v[u][e] = row[e];
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float x = finite_abs(v[u][e]);
-                    most[e] = __builtin_fmaxf(most[e], x);
-                    most_r[t][u] = __builtin_fmaxf(most_r[t][u], x);
-                }
-            }
-        }
-        if (p.most) {
-            sh[turn][wave][lane] = most;  // two in turn, so that one barrier does
-            __syncthreads();
-            if (wave == 0 && c < p.cols) {
-#pragma unroll
-                for (int w = 1; w < kWaves; w++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) most[e] = __builtin_fmaxf(most[e], sh[turn][w][lane][e]);
-                *(f4 *)(p.group_most + group * (p.step / 128) + c) = most;
-            }
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < BATCHES; t++)
-#pragma unroll
-        for (int u = 0; u < 8; u++) {
-            const float m = wave_max_nan_skip(most_r[t][u]);
-            if (lane == 0 && first + 8 * t + u < p.padded) p.e[first + 8 * t + u] = piece_exponent(m);
-        }
-}
-
-// The columns' largest sizes of all groups: 64 columns a workgroup, 16 lanes each.
-__global__ __launch_bounds__(1024) void k_vl_sizes_join(PackPair pp) {
-    __shared__ float sh[16][64];
-    const PackArgs &p = pp.a[blockIdx.y];
-    if (!p.most) return;
-    const int col = threadIdx.x & 63, sub = threadIdx.x / 64;
-    const int64_t d = (int64_t)blockIdx.x * 64 + col;
-    float m = 0.0f;
-    if (d < p.cols)
-#pragma unroll 8
-        for (int g = sub; g < p.groups; g += 16) m = __builtin_fmaxf(m, p.group_most[g * (p.step / 128) + d]);
-    sh[sub][col] = m;
-    __syncthreads();
-    if (sub == 0 && d < p.cols) {
-#pragma unroll
-        for (int i = 1; i < 16; i++) m = __builtin_fmaxf(m, sh[i][col]);
-        p.most[d] = m;
-    }
-}
-
-// A region of 64 rows by kPackCols columns in pieces: by rows, then by columns (the caches have it by then).
-__global__ __launch_bounds__(kVlB) void k_vl_pack(PackPair pp) {
-    const int64_t of_first = pp.a[0].padded / 64 * pp.a[0].regions;
-    const bool second = (int64_t)blockIdx.x >= of_first;
-    const PackArgs &p = pp.a[second];
-    const uint32_t id = (uint32_t)(blockIdx.x - (second ? of_first : 0));
-    const int64_t r0 = (int64_t)(id / (uint32_t)p.regions) * 64, c0 = (int64_t)(id % (uint32_t)p.regions) * kPackCols;
+    const int64_t rb = blockIdx.x - (second ? pp.a[0].groups : 0);
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, half = lane >> 5, col = lane & 31;
-    const int64_t rows = row_count(p);
-    auto store = [&](char *o, const Pieces &c) {
-        *(h8 *)(o + lane * 16) = c.hi;
-        *(h8 *)(o + lane * 16 + 1024) = c.lo;
+    const int64_t r = rb * 32 + col;
+    const bool on = r < (p.from ? p.head->count : p.rows);
+    const float *row = p.s + (on ? (p.from ? (int64_t)p.from[r] : r) : 0) * p.ld;
+    auto load = [&](int kb, float (&x)[8]) {
+        const int64_t k = 16 * (int64_t)kb + 8 * half;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = 0.0f;
+        if (!on || k >= p.cols) return;
+        if (k + 8 <= p.cols) {
+            const f4 a = *(const f4u *)(row + k), b = *(const f4u *)(row + k + 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = a[e], x[4 + e] = b[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (k + e < p.cols) x[e] = row[k + e];
+        }
     };
-    constexpr int kEach = 2 * kPackCols / 16 / (kVlB / kWave);  // blocks of either kind for each wave, asked for together
-    float x[kEach][8];
-    int ex[kEach];
+    float x[kHold][8], most = 0.0f;
+    for (int k0 = 0; k0 < (NB ? 1 : pp.kblocks); k0 += kHold * kWaves) {
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        const int t = wave + i * (kVlB / kWave);
-        const int64_t r = r0 + 32 * (t & 1) + col, k = c0 + 16 * (t >> 1) + 8 * half;
-        ex[i] = p.e[r];
+        for (int i = 0; i < kHold; i++) load(k0 + wave + i * kWaves, x[i]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
-        if (r < rows && k < p.cols) {
-            const float *row = p.s + (p.from ? (int64_t)p.from[r] : r) * p.ld + k;
-            if (k + 8 <= p.cols) {
-                const f4 a = *(const f4u *)row, b = *(const f4u *)(row + 4);
+        for (int i = 0; i < kHold; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[i][e] = a[e], x[i][4 + e] = b[e];
-            } else {
+            for (int e = 0; e < 8; e++) most = __builtin_fmaxf(most, finite_abs(x[i][e]));
+    }
+    sh[threadIdx.x / 32][col] = most;
+    __syncthreads();
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (k + e < p.cols) x[i][e] = row[e];
-            }
+    for (int i = 0; i < 2 * kWaves; i++) most = __builtin_fmaxf(most, sh[i][col]);
+    const int ex = piece_exponent(most);
+    if (threadIdx.x < 32) p.e[r] = ex;
+    const float scale = power(-ex);
+    char *out = p.out + rb * pp.kblocks * 2048;
+    for (int k0 = 0; k0 < (NB ? 1 : pp.kblocks); k0 += kHold * kWaves) {
+#pragma unroll
+        for (int i = 0; i < kHold; i++) {
+            const int kb = k0 + wave + i * kWaves;
+            if (kb >= pp.kblocks) break;
+            if (!NB) load(kb, x[i]);
+            store_block(out + (int64_t)kb * 2048, lane, cut(x[i], scale));
         }
-    }
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        const int t = wave + i * (kVlB / kWave);
-        if (c0 + 16 * (t >> 1) >= p.step / 128) continue;  // behind the padded columns
-        store(p.by_rows + (r0 / 32 + (t & 1)) * p.step + (c0 / 16 + (t >> 1)) * 2048, cut(x[i], power(-ex[i])));
-    }
-    if (!p.by_columns) return;
-    float most[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        const int t = wave + i * (kVlB / kWave);
-        const int64_t kb = r0 / 16 + (t & 3), d = c0 + 32 * (t >> 2) + col;
-        most[i] = d < p.cols ? p.most[d] : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int64_t k = 16 * kb + (p.as_registers ? 4 * half + (e & 3) + 8 * (e >> 2) : 8 * half + e);
-            x[i][e] = d < p.cols && k < rows ? p.s[(p.from ? (int64_t)p.from[k] : k) * p.ld + d] : 0.0f;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        const int t = wave + i * (kVlB / kWave);
-        const int64_t kb = r0 / 16 + (t & 3), db = c0 / 32 + (t >> 2);
-        if (db * 32 < p.cols) store(p.by_columns + db * p.step_c + kb * 2048, cut(x[i], power(-piece_exponent(most[i]))));
     }
 }
 
@@ -589,16 +549,17 @@ struct GradArgs {
     VlHead *head;
     int64_t row0, rows;  // of this piece: the first, how many (padded)
     int64_t V, words;    // words, padded
-    const f2 *part;
+    const VlPart *part;
     const float *label_z;
     const int32_t *labels, *from;  // of this piece's rows
+    const int *ex, *ew;  // the exponents of this piece's rows, of the words
     VlRow *row;
     double *losses;      // by place in the list
     float *row_loss;
     float *z;
     char *turned;
     int64_t turned_step;
-    float *most;         // of every word of this piece
+    int *term;           // of every word of this piece, or none
     float *column;       // [rows / 32][words], or none
     int slices;          // of the rows where the words' largest are looked for
     PartPlan of_x, of_w;
@@ -609,8 +570,8 @@ __global__ __launch_bounds__(1024) void k_vl_stats(GradArgs p) {
     constexpr int kSubs = 1024 / 32;
     __shared__ double sh[kSubs][32];
     __shared__ float shm[kSubs][32];
-    if (p.most && p.row0 > 0)  // the first piece finds them clear
-        for (int64_t v = (int64_t)blockIdx.x * 1024 + threadIdx.x; v < p.words; v += (int64_t)gridDim.x * 1024) p.most[v] = 0.0f;
+    if (p.term && p.row0 > 0)  // the first piece finds them set
+        for (int64_t v = (int64_t)blockIdx.x * 1024 + threadIdx.x; v < p.words; v += (int64_t)gridDim.x * 1024) p.term[v] = kNoTerm;
     const int64_t left = p.head->count - p.row0;
     if (blockIdx.x == 0 && threadIdx.x < 2 * kWave) {
         const bool w = threadIdx.x >= kWave;
@@ -626,32 +587,41 @@ __global__ __launch_bounds__(1024) void k_vl_stats(GradArgs p) {
     const int64_t parts = p.words / kStatWords;
     float m = -__builtin_inff();
 #pragma unroll 4
-    for (int64_t i = sub; i < parts; i += kSubs) m = __builtin_fmaxf(m, p.part[i * p.rows + n].x);
+    for (int64_t i = sub; i < parts; i += kSubs) m = __builtin_fmaxf(m, p.part[i * p.rows + n].m);
     shm[sub][col] = m;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kSubs; i++) m = __builtin_fmaxf(m, shm[i][col]);
     double s = 0.0;
+    float c = -__builtin_inff();
 #pragma unroll 4
     for (int64_t i = sub; i < parts; i += kSubs) {
-        const f2 v = p.part[i * p.rows + n];
-        s += (double)v.y * (double)(v.x == m ? 1.0f : exp8_nonpos(v.x - m));
+        const VlPart v = p.part[i * p.rows + n];
+        s += (double)v.s * (double)(v.m == m ? 1.0f : exp8_nonpos(v.m - m));
+        c = __builtin_fmaxf(c, v.m == m ? v.c : v.c + (v.m - m) * kLog2e);
     }
+    __syncthreads();
     sh[sub][col] = s;
+    shm[sub][col] = c;
     __syncthreads();
     if (sub != 0) return;
     double others = 0.0;
 #pragma unroll
-    for (int i = 0; i < kSubs; i++) others += sh[i][col];
+    for (int i = 0; i < kSubs; i++) {
+        others += sh[i][col];
+        c = __builtin_fmaxf(c, shm[i][col]);
+    }
     const int label = p.labels[n];
-    VlRow row = {0.0f, 0.0f, 0.0f, -1};
+    VlRow row = {0.0f, 0.0f, 0.0f, -1, 0, p.ex[n], {}};
     if (n < left) {
         const float zl = p.label_z[n] - m;
         const double total = others + (double)exp8_nonpos(zl);
         const double ls = zl == 0.0f ? log1p(others) : log(total), loss = ls - (double)zl;
         p.losses[p.row0 + n] = loss;
         if (p.row_loss) p.row_loss[p.from[n]] = (float)loss;
-        row = {m, (float)ls, (float)(-others / total), label};
+        row.m = m, row.ls = (float)ls, row.own = (float)(-others / total), row.label = label;
+        const float term = __builtin_fmaxf(c - row.ls * kLog2e, __builtin_log2f(__builtin_fabsf(row.own)) + (float)p.ew[label]);
+        row.e = word_exponent(term_exponent(term));
     }
     p.row[n] = row;
 }
@@ -662,26 +632,27 @@ __device__ __forceinline__ float g_entry(float z, int64_t v, const VlRow &row) {
     return v == row.label ? row.own : p;
 }
 
-// Every word's largest entry of G in this piece.  A wave takes 32 words and goes over its slice of the rows.
+// Every word's largest term of gW in this piece.  A wave takes 32 words and goes over its slice of the rows.
 __global__ __launch_bounds__(kVlB) void k_vl_words(GradArgs p) {
     const int lane = threadIdx.x & (kWave - 1), half = lane >> 5;
     const int64_t vb = (int64_t)blockIdx.x * (kVlB / kWave) + threadIdx.x / kWave, zwords = p.words / 32;
     const int64_t left = min(p.rows, p.head->count - p.row0), blocks = left > 0 ? (left + 31) / 32 : 0;
     const int64_t b0 = blocks * blockIdx.y / p.slices, b1 = blocks * (blockIdx.y + 1) / p.slices;
-    float most[16];  // logarithms: the exponential of the largest is the largest
+    float most[16];  // logarithms of the terms' sizes
 #pragma unroll
     for (int r = 0; r < 16; r++) most[r] = -__builtin_inff();
     for (int64_t nb = b0; nb < b1; nb++) {
         const VlRow row = p.row[nb * 32 + (lane & 31)];
         const float *z = p.z + (nb * zwords + vb) * 1024 + lane * 4;
+        const float e = row.label < 0 ? -__builtin_inff() : (float)row.ex;
+        const float of_own = __builtin_log2f(__builtin_fabsf(row.own));
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const f4 v = *(const f4 *)(z + q * 256);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const bool own = vb * 32 + 8 * q + 4 * half + e == row.label;
-                const float t = own ? 0.0f : (v[e] - row.m) - row.ls;
-                most[4 * q + e] = __builtin_fmaxf(most[4 * q + e], row.label < 0 ? -__builtin_inff() : t);
+            for (int k = 0; k < 4; k++) {
+                const float t = ((v[k] - row.m) - row.ls) * kLog2e;
+                most[4 * q + k] = __builtin_fmaxf(most[4 * q + k], (vb * 32 + 8 * q + 4 * half + k == row.label ? of_own : t) + e);
             }
         }
     }
@@ -694,7 +665,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_words(GradArgs p) {
         m = __builtin_fmaxf(m, __shfl_xor(m, 8));
         m = __builtin_fmaxf(m, __shfl_xor(m, 16));
         const int64_t v = vb * 32 + 8 * (r / 4) + 4 * half + r % 4;
-        if ((lane & 31) == 0) atomicMax((unsigned int *)p.most + v, __float_as_uint(exp8_nonpos(m)));
+        if ((lane & 31) == 0) atomicMax(p.term + v, term_exponent(m));
     }
 }
 
@@ -710,7 +681,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_bias(GradArgs p, const float *gout,
     gb[v] = acc ? fma_((float)s, c, gb[v]) : (float)s * c;
 }
 
-// G of a block of 32 rows by 32 words, in pieces: under the rows' exponents in z's place (X), and turned, under the words' (W),
+// G of a block of 32 rows by 32 words, in pieces: under the rows' powers in z's place (X), and turned, under the words' (W),
 // with the sums of its columns where gb wants them.
 template <bool X, bool W>
 __global__ __launch_bounds__(kVlB) void k_vl_grad(GradArgs p) {
@@ -720,6 +691,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_grad(GradArgs p) {
     if (p.row0 + nb * 32 >= p.head->count) {
         return;  // gW does not read what lies behind the rows' last 32
     }
+    __shared__ int exs[W ? kVlB / kWave : 1][32];
     const VlRow row = p.row[nb * 32 + col];
     float *z = p.z + (nb * zwords + vb) * 1024;
     float g[16];
@@ -730,34 +702,37 @@ __global__ __launch_bounds__(kVlB) void k_vl_grad(GradArgs p) {
         for (int e = 0; e < 4; e++) g[4 * q + e] = row.label < 0 ? 0.0f : g_entry(v[e], vb * 32 + 8 * q + 4 * half + e, row);
     }
     if constexpr (X) {
-        const float scale = power(-piece_exponent(finite_abs(row.own)));
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = g[8 * s + e];
-            const Pieces c = cut(x, scale);
-            char *o = (char *)z + s * 2048 + lane * 16;
-            *(h8 *)o = c.hi;
-            *(h8 *)(o + 1024) = c.lo;
+            for (int t = 0; t < 2; t++) {
+                const i4v ew = *(const i4v *)(p.ew + vb * 32 + 8 * (2 * s + t) + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[4 * t + e] = __builtin_amdgcn_ldexpf(g[8 * s + 4 * t + e], ew[e] - row.e);
+            }
+            store_block((char *)z + s * 2048, lane, cut(x, 1.0f));
         }
     }
     if constexpr (W) {
 #pragma unroll
         for (int r = 0; r < 16; r++) turn[wave][8 * (r / 4) + 4 * half + r % 4][col] = g[r];
+        if (half == 0) exs[wave][col] = row.ex;
         // the wave's own part of LDS: it reads what it wrote
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const float scale = power(-piece_exponent(p.most[vb * 32 + col]));
+        const int ev = word_exponent(p.term[vb * 32 + col]);
         float sum = 0.0f;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) sum += x[e] = turn[wave][col][16 * s + 8 * half + e];
-            const Pieces c = cut(x, scale);
-            char *o = p.turned + vb * p.turned_step + (nb * 2 + s) * 2048 + lane * 16;
-            *(h8 *)o = c.hi;
-            *(h8 *)(o + 1024) = c.lo;
+            for (int e = 0; e < 8; e++) {
+                const int k = 16 * s + 4 * half + (e & 3) + 8 * (e >> 2);
+                const float v = turn[wave][col][k];
+                sum += v;
+                x[e] = __builtin_amdgcn_ldexpf(v, exs[wave][k] - ev);
+            }
+            store_block(p.turned + vb * p.turned_step + (nb * 2 + s) * 2048, lane, cut(x, 1.0f));
         }
         if (p.column) {
             sum += __shfl_xor(sum, 32);
@@ -769,18 +744,17 @@ __global__ __launch_bounds__(kVlB) void k_vl_grad(GradArgs p) {
 // gx (+)= the parts' sum, at the rows' places
 __global__ __launch_bounds__(kVlB) void k_vl_gx(const float *__restrict__ parts, int64_t rows, int64_t cols, const VlHead *head,
                                                 int64_t row0, const int32_t *__restrict__ from, const VlRow *__restrict__ row,
-                                                const float *__restrict__ most, int64_t D, const float *gout, int sum, float *__restrict__ gx,
-                                                int acc) {
+                                                int64_t D, const float *gout, int sum, float *__restrict__ gx, int acc) {
     const int64_t left = min(rows, head->count - row0);
     const int slices = head->slices_x;
     const float c = vl_coef(head, gout, sum);
     for (int64_t n = blockIdx.x; n < left; n += gridDim.x) {
-        const int en = piece_exponent(finite_abs(row[n].own));
+        const int en = row[n].e;
         float *out = gx + (int64_t)from[n] * D;
         for (int64_t d = threadIdx.x; d < D; d += kVlB) {
             double s = 0.0;
             for (int i = 0; i < slices; i++) s += (double)parts[((int64_t)i * rows + n) * cols + d];
-            const float v = __builtin_amdgcn_ldexpf((float)s, en + piece_exponent(most[d]));
+            const float v = __builtin_amdgcn_ldexpf((float)s, en);
             out[d] = acc ? fma_(v, c, out[d]) : v * c;
         }
     }
@@ -788,16 +762,15 @@ __global__ __launch_bounds__(kVlB) void k_vl_gx(const float *__restrict__ parts,
 
 // gW (+)= the parts' sum
 __global__ __launch_bounds__(kVlB) void k_vl_gw(const float *__restrict__ parts, int64_t part_rows, int64_t cols, const VlHead *head,
-                                                const float *__restrict__ most_g, const float *__restrict__ most_x, int64_t V, int64_t D,
-                                                const float *gout, int sum, float *__restrict__ gw, int acc) {
+                                                const int *__restrict__ term, int64_t V, int64_t D, const float *gout, int sum, float *__restrict__ gw, int acc) {
     const int slices = head->slices_w;
     const float c = head->count ? vl_coef(head, gout, sum) : 0.0f;
     for (int64_t v = blockIdx.x; v < V; v += gridDim.x) {
-        const int ev = piece_exponent(most_g[v]);
+        const int ev = word_exponent(term[v]);
         for (int64_t d = threadIdx.x; d < D; d += kVlB) {
             double s = 0.0;
             for (int i = 0; i < slices; i++) s += (double)parts[((int64_t)i * part_rows + v) * cols + d];
-            const float x = __builtin_amdgcn_ldexpf((float)s, ev + piece_exponent(most_x[d]));
+            const float x = __builtin_amdgcn_ldexpf((float)s, ev);
             float *o = gw + v * D + d;
             *o = acc ? fma_(x, c, *o) : x * c;
         }
@@ -820,15 +793,11 @@ struct SplitPlan {
     int64_t dk;        // columns, padded to two blocks of k
     int64_t piece;     // rows of a piece, padded
     int slices, slices_w;  // parts of gx and of gW, at most; 0: gW is not cut
-    int batches;       // of 8 rows a wave, where sizes are looked for
     int columns;       // slices of the rows where the words' largest are looked for
-    size_t from, list, losses, row, label_z, part, ew, ex, most_w, most_x, most_g, group_w, group_x, column, x1, x3, w1, w2, z, turned, parts, total;
+    size_t from, list, losses, row, label_z, part, ew, ex, term, column, x, w, z, turned, parts, total;
 };
 
 static int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
-
-// batches of 8 rows that a wave looks at for their sizes: two where that leaves the chip full
-static int size_batches(int64_t rows) { return rows >= 64 * 4 * kPlanCUs ? 2 : 1; }
 
 static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w, bool want_b) {
     SplitPlan p{};
@@ -840,7 +809,6 @@ static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool w
     // gW: where its tiles would leave the chip's CUs idle
     if (p.v / kTileM * ((D + 127) / 128) < kPlanCUs) p.slices_w = (int)std::max<int64_t>(1, std::min<int64_t>(64, kPartBytes / (p.v * p.d * 4)));
     p.columns = (int)std::max<int64_t>(1, std::min<int64_t>(16, std::min(p.piece / 32, (4096 + p.v / 32 - 1) / (p.v / 32))));
-    p.batches = size_batches(p.v + p.n);
     size_t at = 256;
     auto take = [&](bool wanted, int64_t bytes) {
         const size_t here = at;
@@ -852,19 +820,13 @@ static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool w
     p.losses = take(true, p.n * 8);
     p.row = take(true, p.piece * (int64_t)sizeof(VlRow));
     p.label_z = take(true, p.piece * 4);
-    p.part = take(true, p.v / kStatWords * p.piece * 8);
+    p.part = take(true, p.v / kStatWords * p.piece * (int64_t)sizeof(VlPart));
     p.ew = take(true, p.v * 4);
     p.ex = take(true, p.n * 4);
-    p.most_w = take(want_x, p.d * 4);
-    p.most_x = take(want_w, p.d * 4);
-    p.most_g = take(want_w || want_b, p.v * 4);
-    p.group_w = take(want_x, p.v / (32 * p.batches) * p.dk * 4);
-    p.group_x = take(want_w, p.n / (32 * p.batches) * p.dk * 4);
+    p.term = take(want_w || want_b, p.v * 4);
     p.column = take(want_b, p.piece / 32 * p.v * 4);
-    p.x1 = take(true, p.n * p.dk * 4);
-    p.x3 = take(want_w, p.d * p.n * 4);
-    p.w1 = take(true, p.v * p.dk * 4);
-    p.w2 = take(want_x, p.d * p.v * 4);
+    p.x = take(true, p.n * p.dk * 4);
+    p.w = take(true, p.v * p.dk * 4);
     p.z = take(grad, p.piece * p.v * 4);
     p.turned = take(want_w || want_b, p.piece * p.v * 4);
     p.parts = take(want_x || (want_w && p.slices_w), std::max(want_x ? p.slices * p.piece : 0, want_w ? p.slices_w * p.v : 0) * p.d * 4);
@@ -909,29 +871,19 @@ int vl_split_run(const VlCall &c, const char *what) {
     int32_t *from = (int32_t *)at(pl.from), *list = (int32_t *)at(pl.list);
     double *losses = (double *)at(pl.losses);
     float *const gx_off = c.acc_x ? nullptr : c.gx;
-    const int64_t zeros = c.gw || c.gb ? pl.v : 0;
-    const int64_t helpers = std::min<int64_t>(1024, (std::max(zeros / 4, c.row_loss || gx_off ? c.N : 0) + 255) / 256);
+    const int64_t terms = c.gw || c.gb ? pl.v : 0;
+    const int64_t helpers = std::min<int64_t>(1024, (std::max(terms / 4, c.row_loss || gx_off ? c.N : 0) + 255) / 256);
     hipLaunchKernelGGL(k_vl_begin, (unsigned)(1 + helpers), 1024, 0, c.st, c.labels, c.N, pl.n, c.D, c.V, c.ignore, head, from, list, c.bad,
-                       (float *)at(pl.most_g), zeros, c.row_loss, gx_off);
+                       (int *)at(pl.term), terms, c.row_loss, gx_off);
     PackPair pp{};
-    for (int i = 0; i < 2; i++) {
-        PackArgs &a = pp.a[i];
-        a.s = i ? c.w : c.x, a.ld = i ? c.ldw : c.ldx, a.rows = i ? c.V : c.N, a.cols = c.D, a.from = i ? nullptr : from, a.head = head;
-        a.e = (int *)at(i ? pl.ew : pl.ex);
-        a.by_rows = at(i ? pl.w1 : pl.x1), a.step = pl.dk * 128, a.padded = i ? pl.v : pl.n;
-        if (i ? c.gx : c.gw) {
-            a.most = (float *)at(i ? pl.most_w : pl.most_x);
-            a.by_columns = at(i ? pl.w2 : pl.x3), a.step_c = a.padded * 128, a.as_registers = i == 1;
-        }
-        a.groups = (int)(a.padded / (32 * pl.batches));
-        a.group_most = (float *)at(i ? pl.group_w : pl.group_x);
-        a.regions = (int)((pl.dk + kPackCols - 1) / kPackCols);
-    }
-    const unsigned looking = (unsigned)(pp.a[0].groups + pp.a[1].groups);
-    if (pl.batches == 2) hipLaunchKernelGGL(k_vl_sizes<2>, looking, kVlB, 0, c.st, pp);
-    else hipLaunchKernelGGL(k_vl_sizes<1>, looking, kVlB, 0, c.st, pp);
-    if (c.gx || c.gw) hipLaunchKernelGGL(k_vl_sizes_join, dim3((unsigned)((c.D + 63) / 64), 2), 1024, 0, c.st, pp);
-    hipLaunchKernelGGL(k_vl_pack, (unsigned)((pl.n + pl.v) / 64 * pp.a[0].regions), kVlB, 0, c.st, pp);
+    pp.a[0] = {c.x, c.ldx, c.N, c.D, from, head, (int *)at(pl.ex), at(pl.x), (int)(pl.n / 32)};
+    pp.a[1] = {c.w, c.ldw, c.V, c.D, nullptr, head, (int *)at(pl.ew), at(pl.w), (int)(pl.v / 32)};
+    pp.kblocks = (int)(pl.dk / 16);
+    const unsigned packing = (unsigned)(pp.a[0].groups + pp.a[1].groups);
+    if (pp.kblocks <= 32) hipLaunchKernelGGL(k_vl_pack<4>, packing, 512, 0, c.st, pp);
+    else if (pp.kblocks <= 64) hipLaunchKernelGGL(k_vl_pack<8>, packing, 512, 0, c.st, pp);
+    else if (pp.kblocks <= 128) hipLaunchKernelGGL(k_vl_pack<16>, packing, 512, 0, c.st, pp);
+    else hipLaunchKernelGGL(k_vl_pack<0>, packing, 512, 0, c.st, pp);
 
     auto launch = [&](auto kernel, int lanes, int lds, int64_t groups, const MmArgs &m) {
         (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -948,23 +900,23 @@ int vl_split_run(const VlCall &c, const char *what) {
     for (int64_t r0 = 0; r0 < pl.n; r0 += pl.piece) {
         const int64_t rows = std::min(pl.piece, pl.n - r0);
         MmArgs m{};
-        m.A = at(pl.w1), m.step_a = pl.dk * 128, m.B = at(pl.x1) + r0 / 32 * (pl.dk * 128), m.step_b = pl.dk * 128;
+        m.A = at(pl.w), m.step_a = pl.dk * 128, m.B = at(pl.x) + r0 / 32 * (pl.dk * 128), m.step_b = pl.dk * 128;
         m.tiles_m = (int)(pl.v / kTileM), m.kblocks = (int)(pl.dk / 16);
         m.head = head, m.row0 = r0, m.V = c.V, m.D = c.D;
         m.ew = (const int *)at(pl.ew), m.ex = (const int *)at(pl.ex) + r0, m.bias = c.bias, m.labels = list + r0;
-        m.z = grad ? (float *)at(pl.z) : nullptr, m.zwords = pl.v / 32, m.part = (f2 *)at(pl.part), m.label_z = (float *)at(pl.label_z);
-        m.rows = pl.piece;
+        m.z = grad ? (float *)at(pl.z) : nullptr, m.zwords = pl.v / 32, m.part = (VlPart *)at(pl.part), m.label_z = (float *)at(pl.label_z);
+        m.rows = pl.piece, m.blocks = (int)(pl.dk / 16);
         product(std::integral_constant<int, MM_Z>{}, m, rows, 1);
 
         GradArgs g{};
         g.head = head, g.row0 = r0, g.rows = pl.piece, g.V = c.V, g.words = pl.v, g.part = m.part, g.label_z = m.label_z;
         g.labels = list + r0, g.from = from + r0, g.row = (VlRow *)at(pl.row), g.losses = losses, g.row_loss = c.row_loss;
-        g.z = m.z, g.turned = at(pl.turned), g.turned_step = pl.piece * 128, g.most = (float *)at(pl.most_g), g.column = c.gb ? (float *)at(pl.column) : nullptr;
+        g.z = m.z, g.turned = at(pl.turned), g.turned_step = pl.piece * 128, g.term = c.gw || c.gb ? (int *)at(pl.term) : nullptr, g.column = c.gb ? (float *)at(pl.column) : nullptr;
         g.slices = pl.columns;
         const bool wide = wide_tiles(0, c.D, true);
         g.of_x = {(int)((c.D + (wide ? 255 : 127)) / (wide ? 256 : 128)), pl.slices, wide ? kPlanCUs : 2 * kPlanCUs};
         g.of_w = {g.of_x.tiles_n, pl.slices_w, g.of_x.at_once};
-        if (!(c.gw || c.gb)) g.most = nullptr;
+        g.ex = m.ex, g.ew = m.ew;
         hipLaunchKernelGGL(k_vl_stats, (unsigned)(rows / 32), 1024, 0, c.st, g);
         if (!grad) continue;
         if (c.gw || c.gb) {
@@ -980,23 +932,23 @@ int vl_split_run(const VlCall &c, const char *what) {
             hipLaunchKernelGGL(k_vl_bias, (unsigned)((c.V + kVlB - 1) / kVlB), kVlB, 0, c.st, g, c.gout, c.sum, c.gb, c.acc_b || r0);
         if (c.gx) {
             MmArgs a = m;
-            a.A = (const char *)m.z, a.step_a = pl.v * 128, a.B = at(pl.w2), a.step_b = pl.v * 128;
+            a.A = (const char *)m.z, a.step_a = pl.v * 128, a.B = at(pl.w), a.step_b = pl.dk * 128;
             a.tiles_m = (int)(rows / kTileM), a.kblocks = (int)(pl.v / 16);
             a.parts = (float *)at(pl.parts), a.part_rows = pl.piece, a.cols = pl.d;
             product(std::integral_constant<int, MM_GX>{}, a, c.D, pl.slices);
             hipLaunchKernelGGL(k_vl_gx, (unsigned)std::min<int64_t>(rows, 1 << 14), kVlB, 0, c.st, a.parts, pl.piece, pl.d, head, r0,
-                               from + r0, g.row, (const float *)at(pl.most_w), c.D, c.gout, c.sum, c.gx, c.acc_x);
+                               from + r0, g.row, c.D, c.gout, c.sum, c.gx, c.acc_x);
         }
         if (c.gw) {
             MmArgs a = m;
-            a.A = g.turned, a.step_a = g.turned_step, a.B = at(pl.x3) + r0 / 16 * 2048, a.step_b = pl.n * 128;
+            a.A = g.turned, a.step_a = g.turned_step;
             a.tiles_m = (int)(pl.v / kTileM), a.kblocks = (int)(rows / 16);
-            a.most_a = g.most, a.most_b = (const float *)at(pl.most_x), a.gout = c.gout, a.out = c.gw, a.sum = c.sum, a.acc = c.acc_w || r0;
+            a.eg = g.term, a.gout = c.gout, a.out = c.gw, a.sum = c.sum, a.acc = c.acc_w || r0;
             if (pl.slices_w) {
                 a.parts = (float *)at(pl.parts), a.part_rows = pl.v, a.cols = pl.d;
                 product(std::integral_constant<int, MM_GW_PARTS>{}, a, c.D, pl.slices_w);
-                hipLaunchKernelGGL(k_vl_gw, (unsigned)std::min<int64_t>(c.V, 1 << 14), kVlB, 0, c.st, a.parts, pl.v, pl.d, head, a.most_a,
-                                   a.most_b, c.V, c.D, c.gout, c.sum, c.gw, a.acc);
+                hipLaunchKernelGGL(k_vl_gw, (unsigned)std::min<int64_t>(c.V, 1 << 14), kVlB, 0, c.st, a.parts, pl.v, pl.d, head, g.term,
+                                   c.V, c.D, c.gout, c.sum, c.gw, a.acc);
             } else {
                 product(std::integral_constant<int, MM_GW>{}, a, c.D, 1);
             }
