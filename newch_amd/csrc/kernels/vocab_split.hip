@@ -104,7 +104,7 @@ __device__ __forceinline__ void store_block(char *block, int lane, const Pieces 
 }
 
 // ---- the product ------------------------------------------------------------------------------------------------------
-enum { MM_Z = 0, MM_GX = 1, MM_GW = 2, MM_GW_PARTS = 3 };
+enum { MM_Z = 0, MM_GX = 1, MM_GW = 2, MM_GW_PARTS = 3, MM_SCORE = 4 };  // MM_SCORE: z, not kept
 
 struct MmArgs {
     const char *A, *B;      // packed; blocks of a row block follow each other
@@ -118,7 +118,7 @@ struct MmArgs {
     const int *ew, *ex;
     const float *bias;
     const int32_t *labels;  // of this piece's rows
-    float *z;               // or none
+    float *z;               // MM_Z
     int64_t zwords;         // blocks of 32 words of a row block
     VlPart *part;           // [words / kStatWords][rows]
     float *label_z;         // [rows]
@@ -143,29 +143,40 @@ __device__ __forceinline__ float vl_coef(const VlHead *head, const float *gout, 
 }
 
 // The wave's 128 words by 64 rows of z, out of its accumulators.
+template <bool KEEP>
 __device__ __forceinline__ void z_out(const MmArgs &p, f16x (&acc)[4][2], int64_t v0, int64_t n0, int lane) {
-    const int half = lane >> 5;
+    const int half = lane >> 5, ex[2] = {p.ex[n0 + (lane & 31)], p.ex[n0 + 32 + (lane & 31)]};
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const int64_t n = n0 + 32 * j + (lane & 31);
-        const int ex = p.ex[n];
+    for (int i = 0; i < 4; i++) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int q = 0; q < 4; q++) {
+            const int64_t v = v0 + 32 * i + 8 * q + 4 * half;
+            const i4v ew = *(const i4v *)(p.ew + v);
+            f4 b = {};
+            if (p.bias) {
+                if (v + 4 <= p.V) b = *(const f4u *)(p.bias + v);
+                else
+                    for (int e = 0; e < 3; e++)
+                        if (v + e < p.V) b[e] = p.bias[v + e];
+            }
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int64_t v = v0 + 32 * i + 8 * q + 4 * half;
-                const i4v ew = *(const i4v *)(p.ew + v);
+            for (int j = 0; j < 2; j++) {
                 f4 z;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float b = p.bias && v + e < p.V ? p.bias[v + e] : 0.0f;
-                    z[e] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + e], ew[e] + ex) + b;
+                    z[e] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + e], ew[e] + ex[j]) + b[e];
                     z[e] = v + e < p.V ? z[e] : -__builtin_inff();
                     acc[i][j][4 * q + e] = z[e];
                 }
-                if (p.z) *(f4 *)(p.z + ((n0 / 32 + j) * p.zwords + v0 / 32 + i) * 1024 + q * 256 + lane * 4) = z;
+                if (KEEP) *(f4 *)(p.z + ((n0 / 32 + j) * p.zwords + v0 / 32 + i) * 1024 + q * 256 + lane * 4) = z;
             }
         }
+        // a block of words at a time: the accumulators leave no registers to load ahead
+        asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1])::"memory");
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int64_t n = n0 + 32 * j + (lane & 31);
         float m = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -191,12 +202,12 @@ __device__ __forceinline__ void z_out(const MmArgs &p, f16x (&acc)[4][2], int64_
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 i4v ew = {};
-                if (p.z) ew = *(const i4v *)(p.ew + v0 + 32 * i + 8 * q + 4 * half);
+                if (KEEP) ew = *(const i4v *)(p.ew + v0 + 32 * i + 8 * q + 4 * half);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float t = (acc[i][j][4 * q + e] - base) * kLog2e;
                     s += __builtin_amdgcn_exp2f(t);
-                    if (p.z) c = __builtin_fmaxf(c, t + (float)ew[e]);
+                    if (KEEP) c = __builtin_fmaxf(c, t + (float)ew[e]);
                 }
             }
         s += __shfl_xor(s, 32);
@@ -222,13 +233,14 @@ template <int WHAT, int WN>
 __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
     using T = Tile<WN>;
     constexpr uint32_t kStage = T::kStage;
+    constexpr bool kZ = WHAT == MM_Z || WHAT == MM_SCORE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wm = wave & 1, wn = wave >> 1;
     const int64_t left = p.head->count - p.row0;  // rows of this piece and behind it
     const int slices = WHAT == MM_GX ? p.head->slices_x : WHAT == MM_GW_PARTS ? p.head->slices_w : 1;
     const uint32_t tiles_m = WHAT == MM_GX ? (uint32_t)(left > 0 ? (min(left, p.rows) + kTileM - 1) / kTileM : 0) : (uint32_t)p.tiles_m;
-    const uint32_t tiles_n = WHAT == MM_Z ? (uint32_t)(left > 0 ? (min(left, p.rows) + T::kN - 1) / T::kN : 0) : (uint32_t)p.tiles_n;
+    const uint32_t tiles_n = kZ ? (uint32_t)(left > 0 ? (min(left, p.rows) + T::kN - 1) / T::kN : 0) : (uint32_t)p.tiles_n;
     const uint32_t tiles = tiles_m * tiles_n, nblk = tiles * (uint32_t)slices;
     if (blockIdx.x >= nblk) return;
     // XCD x runs the workgroups b with b % 8 == x: it gets the x-th of 8 runs of tiles, in groups of 8 tile rows
@@ -248,13 +260,13 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
     const int nk = k1 - k0;
     const int64_t m0 = (int64_t)tm * kTileM + 128 * wm, n0 = (int64_t)tn * T::kN + 64 * wn;
     // a wave whose columns no result has only brings its share
-    const bool works = n0 < (WHAT == MM_Z ? left : p.D);
+    const bool works = n0 < (kZ ? left : p.D);
 
     // each wave brings its share of a stage: the pieces of kA row blocks of A and of one of B
     const char *src_a = p.A + ((int64_t)tm * (kTileM / 32) + T::kA * wave) * p.step_a + (int64_t)k0 * 2048 + lane * 16;
     // of B: its row block's 2 KiB, or, where B's rows are summed over, half a block, 16 rows, of two blocks of columns (behind the
     // last columns the last block again)
-    constexpr bool kTurned = WHAT != MM_Z;
+    constexpr bool kTurned = !kZ;
     const int db = min(p.blocks - 1, tn * (T::kN / 16) + 2 * wave), db1 = min(p.blocks - 1, db + 1);
     const char *src_b = kTurned ? p.B + k0 / 2 * p.step_b + db * 2048 + lane * 16
                                 : p.B + ((int64_t)tn * (T::kN / 32) + wave) * p.step_b + (int64_t)k0 * 2048 + lane * 16;
@@ -366,8 +378,8 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
     // what the results need is computed behind the products, whose registers it would take
     int at = lane;
     asm volatile("" : "+v"(at)::"memory");
-    if constexpr (WHAT == MM_Z) {
-        z_out(p, acc, m0, n0, at);
+    if constexpr (kZ) {
+        z_out<WHAT == MM_Z>(p, acc, m0, n0, at);
     } else if constexpr (WHAT == MM_GX || WHAT == MM_GW_PARTS) {
         // a store instruction writes 32 columns of two rows
         float *out = p.parts + ((int64_t)slice * p.part_rows + m0 + 4 * (at >> 5)) * p.cols + n0 + (at & 31);
@@ -906,7 +918,8 @@ int vl_split_run(const VlCall &c, const char *what) {
         m.ew = (const int *)at(pl.ew), m.ex = (const int *)at(pl.ex) + r0, m.bias = c.bias, m.labels = list + r0;
         m.z = grad ? (float *)at(pl.z) : nullptr, m.zwords = pl.v / 32, m.part = (VlPart *)at(pl.part), m.label_z = (float *)at(pl.label_z);
         m.rows = pl.piece, m.blocks = (int)(pl.dk / 16);
-        product(std::integral_constant<int, MM_Z>{}, m, rows, 1);
+        if (grad) product(std::integral_constant<int, MM_Z>{}, m, rows, 1);
+        else product(std::integral_constant<int, MM_SCORE>{}, m, rows, 1);
 
         GradArgs g{};
         g.head = head, g.row0 = r0, g.rows = pl.piece, g.V = c.V, g.words = pl.v, g.part = m.part, g.label_z = m.label_z;
