@@ -765,6 +765,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_gx(const float *__restrict__ parts,
         float *out = gx + (int64_t)from[n] * D;
         for (int64_t d = threadIdx.x; d < D; d += kVlB) {
             double s = 0.0;
+#pragma unroll 8
             for (int i = 0; i < slices; i++) s += (double)parts[((int64_t)i * rows + n) * cols + d];
             const float v = __builtin_amdgcn_ldexpf((float)s, en);
             out[d] = acc ? fma_(v, c, out[d]) : v * c;
@@ -781,6 +782,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_gw(const float *__restrict__ parts,
         const int ev = word_exponent(term[v]);
         for (int64_t d = threadIdx.x; d < D; d += kVlB) {
             double s = 0.0;
+#pragma unroll 8
             for (int i = 0; i < slices; i++) s += (double)parts[((int64_t)i * part_rows + v) * cols + d];
             const float x = __builtin_amdgcn_ldexpf((float)s, ev);
             float *o = gw + v * D + d;
