@@ -98,6 +98,7 @@ def test_kernel_layer_refusals(lib):
     bad("NULL", K.embedding_fwd, 1, 5, 4, P, 4, None, 1.0, P)
     bad("NULL", K.embedding_fwd, 1, 5, 4, P, 4, P, 1.0, None)
     bad("8-byte", K.embedding_fwd, 1, 5, 4, P, 4, P, 1.0, P, bad=P + 4)
+    bad("rows closer", K.embedding_fwd, 1, 5, 4, P, 3, P, 1.0, P)
     n = K.embedding_bwd_workspace(100, 5, 4)
     assert n > 0 and K.embedding_bwd_workspace(0, 5, 4) == 0
     bad("workspace of", K.embedding_bwd, 100, 5, 4, P, -1, 1.0, P, P, P, n - 1)
