@@ -94,41 +94,48 @@ __device__ __forceinline__ float vl_entry(float z, int64_t v, int32_t label, con
     return (v == label ? s.own : exp8_nonpos((z - s.m) - s.ls)) * s.coef;
 }
 
-// A workgroup's row: its statistics, its loss, and, GRAD, its row of G in place of z.
+// A workgroup's row of up to kVlShort words, in registers: its statistics, its loss, and, GRAD, its row of G in place of z.
 template <bool GRAD>
 __global__ __launch_bounds__(kVlB) void k_vl_softmax(VlArgs p) {
+    constexpr int kEach = kVlShort / kVlB;
     __shared__ double sh[kVlB / kWave];
-    __shared__ float shm[kVlB / kWave];
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const int64_t i = p.row0 + r;
-        float *z = p.z + r * p.ldz;
-        const int32_t l = p.labels[i];
-        if (!vl_counts(l, p.ignore, p.V)) {
-            if (threadIdx.x == 0) {
-                p.row_loss[i] = 0.0;
-                if (p.row_out) p.row_out[i] = 0.0f;
-            }
-            if (GRAD)
-                for (int64_t v = threadIdx.x; v < p.V; v += kVlB) z[v] = 0.0f;
-            continue;
+    __shared__ float shm[kVlB / kWave], own;
+    const int64_t r = blockIdx.x, i = p.row0 + r;
+    const int V = (int)p.V;
+    float *z = p.z + r * p.ldz;
+    const int32_t l = p.labels[i];
+    if (!vl_counts(l, p.ignore, p.V)) {
+        if (threadIdx.x == 0) {
+            p.row_loss[i] = 0.0;
+            if (p.row_out) p.row_out[i] = 0.0f;
         }
-        float m = -__builtin_inff();
-        for (int64_t v = threadIdx.x; v < p.V; v += kVlB) m = __builtin_fmaxf(m, z[v]);
-        m = wave_max_nan_skip(m);
-        __syncthreads();
-        if ((threadIdx.x & (kWave - 1)) == 0) shm[threadIdx.x / kWave] = m;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kVlB / kWave; k++) m = __builtin_fmaxf(m, shm[k]);
-        double s = 0.0;
-        for (int64_t v = threadIdx.x; v < p.V; v += kVlB) s += v == l ? 0.0 : (double)exp_sum_term(z[v] - m);
-        const double others = vl_wg_sum(s, sh);
-        const VlStat st = vl_stat(p, i, m, others, z[l] - m, threadIdx.x == 0);
-        if (GRAD) {
-            __syncthreads();  // z[l] has been read
-            for (int64_t v = threadIdx.x; v < p.V; v += kVlB) z[v] = vl_entry(z[v], v, l, st);
-        }
+        if (GRAD)
+            for (int v = threadIdx.x; v < V; v += kVlB) z[v] = 0.0f;
+        return;
     }
+    float x[kEach], m = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < kEach; k++) x[k] = k * kVlB + (int)threadIdx.x < V ? z[k * kVlB + threadIdx.x] : -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+        m = __builtin_fmaxf(m, x[k]);
+        if (k * kVlB + (int)threadIdx.x == l) own = x[k];
+    }
+    m = wave_max_nan_skip(m);
+    if ((threadIdx.x & (kWave - 1)) == 0) shm[threadIdx.x / kWave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kVlB / kWave; k++) m = __builtin_fmaxf(m, shm[k]);
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < kEach; k++)
+        if (k * kVlB < V) s += k * kVlB + (int)threadIdx.x == l || k * kVlB + (int)threadIdx.x >= V ? 0.0 : (double)exp_sum_term(x[k] - m);
+    const double others = vl_wg_sum(s, sh);
+    const VlStat st = vl_stat(p, i, m, others, own - m, threadIdx.x == 0);
+    if (GRAD)
+#pragma unroll
+        for (int k = 0; k < kEach; k++)
+            if (k * kVlB + (int)threadIdx.x < V) z[k * kVlB + threadIdx.x] = vl_entry(x[k], k * kVlB + threadIdx.x, l, st);
 }
 
 // The same of long rows, whose chunks are workgroups of their own: first each chunk's maximum and sum,

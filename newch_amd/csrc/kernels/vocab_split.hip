@@ -848,18 +848,19 @@ static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool w
     return p;
 }
 
-// The two forms' times by what they do, in us: fp32 products start at once and run at 115 TFLOP/s; pieces have W and x read twice and
-// written first, whole tiles of rows, and 370.  Both sides measured (us, fp32 products : pieces): 128000 x 2048 with gradients, 64 rows 1167 :
-// 2012, 256 3651 : 2425; 32000 x 1024, 128 rows 306 : 426, 256 526 : 457, 4096 7316 : 2640; 2000 x 256, 1024 rows 83 : 123, 4096 207 : 162;
-// scored, 32000 x 1024, 128 rows 92 : 145, 256 167 : 153; 5000 x 64, 1024 rows 36 : 38, 4096 80 : 58.  Over 400 sizes what it chooses takes
-// 0.2% longer than the better one.
+// The two forms' times by what they do, in us.  fp32 products start at once and run at 115 TFLOP/s; pieces have x and W read and written
+// first, whole tiles of rows, and some 370 TFLOP/s.  Both sides measured (us, fp32 products : pieces): 128000 x 2048 with gradients, 64
+// rows 1136 : 1456, 256 3655 : 1828; 32000 x 1024, 64 rows 186 : 257, 128 294 : 277, 4096 7262 : 2517; 2000 x 256, 1024 rows 83 : 104, 4096
+// 200 : 141; scored, 32000 x 1024, 64 rows 57 : 102, 128 90 : 105, 256 167 : 113; 5000 x 64, 512 rows 25 : 28, 1024 36 : 29.  Over the 400
+// sizes that the numbers are fitted to (1 to 4096 rows, 64 to 2048 columns, 500 to 128000 words) what it chooses takes 0.2% longer in the
+// mean than the better one, 13% at most.
 bool vl_split_pays(int64_t N, int64_t D, int64_t V, bool grads) {
     if (N == 0 || N > kPieceRows * 16) return false;
     if (const char *form = getenv("NC_HIP_VOCAB_FORM")) return form[0] == 's';
     const double d = (double)D, vd = (double)V * d, nv = (double)N * (double)V, nvd = nv * d;
     const double fp32 = grads ? 30 + 2e-6 * vd + 4.5e-6 * nv + 5.2e-8 * nvd : 17 + 0.75e-6 * vd + 1.4e-6 * nv + 1.6e-8 * nvd;
-    const double split = grads ? 70 + 0.04 * d + 1e-3 * (double)V + 6e-6 * vd + 4.5e-6 * nv + 1.6e-8 * nvd
-                               : 28 + 0.027 * d + 2.4e-6 * vd + 0.6e-6 * nv + 5.5e-9 * nvd;
+    const double split = grads ? 52 + 0.043 * d + 0.8e-3 * (double)V + 4e-6 * vd + 4e-6 * nv + 1e-8 * nvd
+                               : 20 + 0.036 * d + 2.1e-6 * vd + 0.4e-6 * nv + 3.5e-9 * nvd;
     return split < fp32;
 }
 
