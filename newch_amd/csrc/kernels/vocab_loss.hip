@@ -15,6 +15,9 @@ namespace nchip {
 constexpr size_t kVlPiece = size_t(1) << 30;  // bytes of z held at a time
 constexpr int64_t kVlRows = 32768;            // and rows
 
+// Rows whose count the workgroup of every short row takes for itself, at most, in place of a launch: 64 and 256 rows over 1000 words are
+// 1.6 us faster by it, 2000 no more, 4000 to 8000 4 to 20 us slower.
+constexpr int64_t kVlCountMost = 1024;
 constexpr int kVlChunk = 2048;  // words of a row that a workgroup takes, where a row is shared by several
 constexpr int kVlShort = 4096;  // words of a row that one workgroup takes alone, at most
 
@@ -25,8 +28,13 @@ struct VlArgs {
     const int32_t *labels;
     int32_t ignore;
     int sum;
-    const VlHead *head;
+    bool count_here;  // the rows that count are counted here, not by k_vl_count
+    VlHead *head;
+    unsigned long long *bad;
     const float *gout;
+    const float *x;
+    int64_t ldx, D;
+    float *clean;      // [N][D], x with zeros for the rows that do not count, or none
     float *z;          // [rows][ldz]: the products, then G
     f2 *part;          // [rows][chunks] {maximum, sum of exponentials}, the label's left out of the sum
     float *label_z;    // [rows]
@@ -34,43 +42,43 @@ struct VlArgs {
     float *row_out;    // [N] or none
 };
 
-// Workgroup 0: rows that count, and the first label that is neither a word nor `ignore`, as (row << 32) | label, or all ones.  The
-// others copy x with zeros for the rows that do not count, where gW wants it.
-__global__ __launch_bounds__(1024) void k_vl_count(const int32_t *__restrict__ labels, int64_t N, int64_t D, int64_t V, int32_t ignore,
-                                                   VlHead *head, unsigned long long *bad, const float *__restrict__ x, int64_t ldx,
-                                                   float *__restrict__ clean) {
-    constexpr int kWaves = 1024 / kWave;
-    if (blockIdx.x > 0) {
-        const int lane = threadIdx.x & (kWave - 1);
-        for (int64_t i = (int64_t)(blockIdx.x - 1) * kWaves + threadIdx.x / kWave; i < N; i += (int64_t)(gridDim.x - 1) * kWaves) {
-            const bool on = vl_counts(labels[i], ignore, V);
-            for (int64_t d = lane; d < D; d += kWave) clean[i * D + d] = on ? x[i * ldx + d] : 0.0f;
-        }
-        return;
-    }
-    __shared__ unsigned long long shk[kWaves];
-    __shared__ double shn[kWaves];
+// Rows that count, and, SAY, for the head and the caller, the first label that is neither a word nor `ignore`, as (row << 32) | label, or
+// all ones.
+template <int B, bool SAY>
+__device__ __forceinline__ int64_t vl_count(const VlArgs &p, double *sh) {
+    __shared__ unsigned long long shk[B / kWave];
     unsigned long long k = ~0ull;
     double n = 0.0;
-    for (int64_t i = threadIdx.x; i < N; i += 1024) {
-        const int32_t l = labels[i];
-        if (l == ignore) continue;
-        if (l >= 0 && l < V) n += 1.0;
-        else if (k == ~0ull) k = ((unsigned long long)i << 32) | (uint32_t)l;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < p.N; i += B) {
+        const int32_t l = p.labels[i];
+        if (vl_counts(l, p.ignore, p.V)) n += 1.0;
+        else if (SAY && l != p.ignore && k == ~0ull) k = ((unsigned long long)i << 32) | (uint32_t)l;
     }
-    k = wave_min_u64(k);
-    n = wave_sum(n);
-    if ((threadIdx.x & (kWave - 1)) == 0) shk[threadIdx.x / kWave] = k, shn[threadIdx.x / kWave] = n;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < kWaves; i++) {
-            k = shk[i] < k ? shk[i] : k;
-            n += shn[i];
-        }
-        head->count = (int64_t)n;
+    if (SAY) {
+        k = wave_min_u64(k);
+        if ((threadIdx.x & (kWave - 1)) == 0) shk[threadIdx.x / kWave] = k;
+    }
+    n = vl_wg_sum(n, sh);
+    if (SAY && threadIdx.x == 0) {
+        for (int i = 1; i < B / kWave; i++) k = shk[i] < k ? shk[i] : k;
+        p.head->count = (int64_t)n;
         // at system scope: *bad may be host memory that the host watches while the kernel runs
-        if (bad) __hip_atomic_store(bad, k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        if (p.bad) __hip_atomic_store(p.bad, k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     }
+    return (int64_t)n;
+}
+
+__global__ __launch_bounds__(1024) void k_vl_count(VlArgs p) {
+    __shared__ double sh[1024 / kWave];
+    vl_count<1024, true>(p, sh);
+}
+
+// this workgroup's share, part of parts, of row i of the x that gW takes
+__device__ __forceinline__ void vl_clean(const VlArgs &p, int64_t i, bool on, int part, int parts) {
+    if (p.clean)
+        for (int64_t d = (int64_t)part * kVlB + threadIdx.x; d < p.D; d += (int64_t)parts * kVlB)
+            p.clean[i * p.D + d] = on ? p.x[i * p.ldx + d] : 0.0f;
 }
 
 // what a row's G is made from
@@ -78,7 +86,7 @@ struct VlStat {
     float m, ls, own, coef;
 };
 
-__device__ __forceinline__ VlStat vl_stat(const VlArgs &p, int64_t i, float m, double others, float zl, bool first) {
+__device__ __forceinline__ VlStat vl_stat(const VlArgs &p, int64_t i, float m, double others, float zl, int64_t count, bool first) {
     const double own = (double)exp8_nonpos(zl), total = others + own;
     const double ls = zl == 0.0f ? log1p(others) : log(total);
     if (first) {
@@ -87,7 +95,7 @@ __device__ __forceinline__ VlStat vl_stat(const VlArgs &p, int64_t i, float m, d
         if (p.row_out) p.row_out[i] = (float)loss;
     }
     const float c = p.gout ? *p.gout : 1.0f;
-    return {m, (float)ls, (float)(-others / total), p.sum ? c : c / (float)p.head->count};
+    return {m, (float)ls, (float)(-others / total), p.sum ? c : c / (float)count};
 }
 
 __device__ __forceinline__ float vl_entry(float z, int64_t v, int32_t label, const VlStat &s) {
@@ -104,7 +112,10 @@ __global__ __launch_bounds__(kVlB) void k_vl_softmax(VlArgs p) {
     const int V = (int)p.V;
     float *z = p.z + r * p.ldz;
     const int32_t l = p.labels[i];
-    if (!vl_counts(l, p.ignore, p.V)) {
+    const bool on = vl_counts(l, p.ignore, p.V);
+    if (GRAD) vl_clean(p, i, on, 0, 1);
+    if (p.count_here && r == 0) vl_count<kVlB, true>(p, sh);
+    if (!on) {
         if (threadIdx.x == 0) {
             p.row_loss[i] = 0.0;
             if (p.row_out) p.row_out[i] = 0.0f;
@@ -116,6 +127,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_softmax(VlArgs p) {
     float x[kEach], m = -__builtin_inff();
 #pragma unroll
     for (int k = 0; k < kEach; k++) x[k] = k * kVlB + (int)threadIdx.x < V ? z[k * kVlB + threadIdx.x] : -__builtin_inff();
+    const int64_t count = !GRAD || p.sum ? 0 : p.count_here ? vl_count<kVlB, false>(p, sh) : p.head->count;
 #pragma unroll
     for (int k = 0; k < kEach; k++) {
         m = __builtin_fmaxf(m, x[k]);
@@ -131,19 +143,24 @@ __global__ __launch_bounds__(kVlB) void k_vl_softmax(VlArgs p) {
     for (int k = 0; k < kEach; k++)
         if (k * kVlB < V) s += k * kVlB + (int)threadIdx.x == l || k * kVlB + (int)threadIdx.x >= V ? 0.0 : (double)exp_sum_term(x[k] - m);
     const double others = vl_wg_sum(s, sh);
-    const VlStat st = vl_stat(p, i, m, others, own - m, threadIdx.x == 0);
+    const VlStat st = vl_stat(p, i, m, others, own - m, count, threadIdx.x == 0);
     if (GRAD)
 #pragma unroll
         for (int k = 0; k < kEach; k++)
             if (k * kVlB + (int)threadIdx.x < V) z[k * kVlB + threadIdx.x] = vl_entry(x[k], k * kVlB + threadIdx.x, l, st);
 }
 
-// The same of long rows, whose chunks are workgroups of their own: first each chunk's maximum and sum,
+// The same of long rows, whose chunks are workgroups of their own: first each chunk's maximum and sum, and, by one workgroup behind
+// them, the count,
 __global__ __launch_bounds__(kVlB) void k_vl_part(VlArgs p) {
     constexpr int kEach = kVlChunk / kVlB;
     __shared__ double sh[kVlB / kWave];
     __shared__ float shm[kVlB / kWave];
     const int64_t r = blockIdx.y, v0 = (int64_t)blockIdx.x * kVlChunk;
+    if (r == p.rows) {
+        if (blockIdx.x == 0) vl_count<kVlB, true>(p, sh);
+        return;
+    }
     const int32_t l = p.labels[p.row0 + r];
     if (!vl_counts(l, p.ignore, p.V)) return;
     const float *z = p.z + r * p.ldz;
@@ -179,7 +196,9 @@ __global__ __launch_bounds__(kVlB) void k_vl_chunk(VlArgs p) {
     const int64_t r = blockIdx.y, i = p.row0 + r, v0 = (int64_t)blockIdx.x * kVlChunk;
     const int32_t l = p.labels[i];
     float *z = p.z + r * p.ldz;
-    if (!vl_counts(l, p.ignore, p.V)) {
+    const bool on = vl_counts(l, p.ignore, p.V);
+    if (GRAD) vl_clean(p, i, on, blockIdx.x, p.chunks);
+    if (!on) {
         if (threadIdx.x == 0 && blockIdx.x == 0) {
             p.row_loss[i] = 0.0;
             if (p.row_out) p.row_out[i] = 0.0f;
@@ -199,47 +218,58 @@ __global__ __launch_bounds__(kVlB) void k_vl_chunk(VlArgs p) {
     double s = 0.0;
     for (int k = threadIdx.x; k < p.chunks; k += kVlB) s += (double)part[k].y * (double)(part[k].x == m ? 1.0f : exp8_nonpos(part[k].x - m));
     const double others = vl_wg_sum(s, sh);
-    const VlStat st = vl_stat(p, i, m, others, p.label_z[r] - m, blockIdx.x == 0 && threadIdx.x == 0);
+    const VlStat st = vl_stat(p, i, m, others, p.label_z[r] - m, GRAD && !p.sum ? p.head->count : 0, blockIdx.x == 0 && threadIdx.x == 0);
     if (GRAD)
         for (int64_t v = v0 + threadIdx.x; v < min(p.V, v0 + kVlChunk); v += kVlB) z[v] = vl_entry(z[v], v, l, st);
 }
 
-// gx (+)= the parts' sum
-__global__ __launch_bounds__(kVlB) void k_vl_parts(const float *__restrict__ parts, int slices, int64_t n, float *__restrict__ gx, int acc) {
-    for (int64_t i = (int64_t)blockIdx.x * kVlB + threadIdx.x; i < n; i += (int64_t)gridDim.x * kVlB) {
-        double s = acc ? (double)gx[i] : 0.0;
-#pragma unroll 8
-        for (int k = 0; k < slices; k++) s += (double)parts[k * n + i];
-        gx[i] = (float)s;
-    }
-}
+// What is left of a piece, in one launch: gx (+)= the sum of its parts; gb (+)= the column sums of G, 64 columns a workgroup, a quarter
+// of the rows in each wave; and at the last the loss, which of no rows is NaN, as a mean over nothing is (a sum: 0).
+struct VlTail {
+    const float *parts;
+    int slices;
+    int64_t n;  // words of a part
+    float *gx;
+    int acc_x;
+    unsigned joins, columns;  // workgroups
+    const float *g;
+    int64_t ldz, rows, V;
+    float *gb;
+    int acc_b;
+    const double *row_loss;
+    int64_t N;
+    const VlHead *head;
+    int sum;
+    float *loss;
+};
 
-// gb (+)= column sums of G: 64 columns a workgroup, a quarter of the rows in each wave
-__global__ __launch_bounds__(kVlB) void k_vl_columns(const float *__restrict__ g, int64_t ldz, int64_t rows, int64_t V, float *gb, int acc) {
+__global__ __launch_bounds__(kVlB) void k_vl_tail(VlTail p) {
     constexpr int kWaves = kVlB / kWave;
-    __shared__ double sh[kWaves][kWave];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int64_t v = (int64_t)blockIdx.x * kWave + lane;
-    double s = 0.0;
-    if (v < V)
+    __shared__ double sh[kWaves * kWave];
+    if (blockIdx.x < p.joins) {
+        for (int64_t i = (int64_t)blockIdx.x * kVlB + threadIdx.x; i < p.n; i += (int64_t)p.joins * kVlB) {
+            double s = p.acc_x ? (double)p.gx[i] : 0.0;
 #pragma unroll 8
-        for (int64_t r = wave; r < rows; r += kWaves) s += (double)g[r * ldz + v];
-    sh[wave][lane] = s;
-    __syncthreads();
-    if (wave != 0 || v >= V) return;
+            for (int k = 0; k < p.slices; k++) s += (double)p.parts[k * p.n + i];
+            p.gx[i] = (float)s;
+        }
+    } else if (blockIdx.x - p.joins < p.columns) {
+        const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+        const int64_t v = (int64_t)(blockIdx.x - p.joins) * kWave + lane;
+        double s = 0.0;
+        if (v < p.V)
+#pragma unroll 8
+            for (int64_t r = wave; r < p.rows; r += kWaves) s += (double)p.g[r * p.ldz + v];
+        sh[threadIdx.x] = s;
+        __syncthreads();
+        if (wave != 0 || v >= p.V) return;
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) s += sh[w][lane];
-    gb[v] = (float)(acc ? (double)gb[v] + s : s);
-}
-
-// the loss of no rows is NaN, as a mean over nothing is (a sum: 0)
-__global__ __launch_bounds__(kVlB) void k_vl_finish(const double *__restrict__ row_loss, int64_t N, const VlHead *__restrict__ head, int sum,
-                                                    float *__restrict__ loss) {
-    __shared__ double sh[kVlB / kWave];
-    double t = 0.0;
-    for (int64_t i = threadIdx.x; i < N; i += kVlB) t += row_loss[i];
-    t = vl_wg_sum(t, sh);
-    if (threadIdx.x == 0) *loss = sum ? (float)t : head->count ? (float)(t / (double)head->count) : __builtin_nanf("");
+        for (int w = 1; w < kWaves; w++) s += sh[w * kWave + lane];
+        p.gb[v] = (float)(p.acc_b ? (double)p.gb[v] + s : s);
+    } else {
+        const double t = vl_wg_sum(vl_lane_sum(p.row_loss, p.N), sh);
+        if (threadIdx.x == 0) *p.loss = p.sum ? (float)t : p.head->count ? (float)(t / (double)p.head->count) : __builtin_nanf("");
+    }
 }
 
 __global__ __launch_bounds__(kVlB) void k_vl_zero(float *__restrict__ p, int64_t n) {
@@ -315,44 +345,52 @@ extern "C" NC_HIP_API int nc_hip_linear_cross_entropy(int64_t N, int64_t D, int6
     VlHead *head = (VlHead *)base;
     double *losses = (double *)(base + plan.losses);
     float *clean = (float *)(base + plan.rows), *z = (float *)(base + plan.z), *parts = (float *)(base + plan.parts);
-    const unsigned copies = gw ? (unsigned)std::min<int64_t>((N + 15) / 16, 1024) : 0;
-    hipLaunchKernelGGL(k_vl_count, 1 + copies, 1024, 0, st, labels, N, D, V, ignore, head, (unsigned long long *)bad, x, ldx, clean);
+    VlArgs a{};
+    a.N = N, a.V = V, a.ldz = plan.ldz, a.chunks = plan.chunks, a.labels = labels, a.ignore = ignore, a.sum = sum;
+    a.head = head, a.bad = (unsigned long long *)bad, a.gout = gout, a.x = x, a.ldx = ldx, a.D = D, a.clean = gw ? clean : nullptr;
+    a.z = z, a.part = (f2 *)(base + plan.part), a.label_z = (float *)(base + plan.label_z), a.row_loss = losses, a.row_out = row_loss;
+    VlTail t{};
+    t.parts = parts, t.slices = plan.slices, t.acc_x = acc_x, t.g = z, t.ldz = plan.ldz, t.V = V, t.gb = gb;
+    t.row_loss = losses, t.N = N, t.head = head, t.sum = sum, t.loss = loss;
+    const bool count_here = N > 0 && (plan.chunks > 1 || N <= kVlCountMost);
+    if (!count_here) hipLaunchKernelGGL(k_vl_count, 1, 1024, 0, st, a);
     for (int64_t r0 = 0; r0 < N; r0 += plan.piece) {
-        VlArgs a{N, V, plan.ldz, r0, std::min(plan.piece, N - r0), plan.chunks, labels, ignore, sum, head, gout, z, (f2 *)(base + plan.part),
-                 (float *)(base + plan.label_z), losses, row_loss};
+        a.row0 = r0, a.rows = std::min(plan.piece, N - r0), a.count_here = count_here && r0 == 0;
         int rc = nc_hip_gemm_f32_bias(0, 1, a.rows, V, D, 1.0f, x + r0 * ldx, ldx, w, ldw, bias, z, plan.ldz, stream);
         if (rc) return rc;
         if (plan.chunks > 1) {
             const dim3 grid((unsigned)plan.chunks, (unsigned)a.rows);
-            hipLaunchKernelGGL(k_vl_part, grid, kVlB, 0, st, a);
+            hipLaunchKernelGGL(k_vl_part, dim3(grid.x, grid.y + a.count_here), kVlB, 0, st, a);
             if (grad) hipLaunchKernelGGL(k_vl_chunk<true>, grid, kVlB, 0, st, a);
-            else hipLaunchKernelGGL(k_vl_chunk<false>, dim3(1, (unsigned)a.rows), kVlB, 0, st, a);
+            else hipLaunchKernelGGL(k_vl_chunk<false>, dim3(1, grid.y), kVlB, 0, st, a);
         } else if (grad) {
             hipLaunchKernelGGL(k_vl_softmax<true>, (unsigned)a.rows, kVlB, 0, st, a);
         } else {
             hipLaunchKernelGGL(k_vl_softmax<false>, (unsigned)a.rows, kVlB, 0, st, a);
         }
-        if (gx && plan.slices > 1) {
+        const bool cut = gx && plan.slices > 1;
+        if (cut) {
             const int64_t whole = V / plan.slice, rest = V - whole * plan.slice, part = a.rows * D;
             const int64_t shape = whole, sa = plan.slice, sb = plan.slice * ldw;
             rc = nc_hip_gemm_f32_bmm(0, 0, a.rows, D, plan.slice, z, plan.ldz, w, ldw, 0.0f, parts, D, 1, &shape, &sa, &sb, &part, nullptr, 0, stream);
             if (!rc && rest)
                 rc = nc_hip_gemm_f32(0, 0, a.rows, D, rest, 1.0f, z + whole * plan.slice, plan.ldz, w + whole * sb, ldw, 0.0f,
                                      parts + whole * part, D, stream);
-            if (!rc)
-                hipLaunchKernelGGL(k_vl_parts, stream_grid(part, kVlB), kVlB, 0, st, parts, plan.slices, part, gx + r0 * D, acc_x != 0);
         } else if (gx) {
             rc = nc_hip_gemm_f32(0, 0, a.rows, D, V, 1.0f, z, plan.ldz, w, ldw, acc_x ? 1.0f : 0.0f, gx + r0 * D, D, stream);
         }
         if (!rc && gw)
             rc = nc_hip_gemm_f32(1, 0, V, D, a.rows, 1.0f, z, plan.ldz, clean + r0 * D, D, acc_w || r0 ? 1.0f : 0.0f, gw, D, stream);
         if (rc) return rc;
-        if (gb) hipLaunchKernelGGL(k_vl_columns, (unsigned)((V + kWave - 1) / kWave), kVlB, 0, st, z, plan.ldz, a.rows, V, gb, acc_b || r0);
+        t.rows = a.rows, t.n = a.rows * D, t.gx = cut ? gx + r0 * D : nullptr, t.acc_b = acc_b || r0;
+        t.joins = cut ? stream_grid(t.n, kVlB) : 0, t.columns = gb ? (unsigned)((V + kWave - 1) / kWave) : 0;
+        const unsigned last = r0 + a.rows == N;
+        if (t.joins + t.columns + last) hipLaunchKernelGGL(k_vl_tail, t.joins + t.columns + last, kVlB, 0, st, t);
     }
     if (N == 0) {
         if (gw && !acc_w) hipLaunchKernelGGL(k_vl_zero, stream_grid(V * D, kVlB), kVlB, 0, st, gw, V * D);
         if (gb && !acc_b) hipLaunchKernelGGL(k_vl_zero, stream_grid(V, kVlB), kVlB, 0, st, gb, V);
+        hipLaunchKernelGGL(k_vl_tail, 1, kVlB, 0, st, t);
     }
-    hipLaunchKernelGGL(k_vl_finish, 1, kVlB, 0, st, losses, N, head, sum, loss);
     return check_launch(what);
 }

@@ -681,18 +681,6 @@ __global__ __launch_bounds__(kVlB) void k_vl_words(GradArgs p) {
     }
 }
 
-// gb (+)= the sums of the columns of G, which k_vl_grad left for every 32 rows
-__global__ __launch_bounds__(kVlB) void k_vl_bias(GradArgs p, const float *gout, int sum, float *__restrict__ gb, int acc) {
-    const int64_t v = (int64_t)blockIdx.x * kVlB + threadIdx.x;
-    if (v >= p.V) return;
-    const int64_t left = min(p.rows, p.head->count - p.row0), blocks = left > 0 ? (left + 31) / 32 : 0;
-    double s = 0.0;
-#pragma unroll 8
-    for (int64_t i = 0; i < blocks; i++) s += (double)p.column[i * p.words + v];
-    const float c = blocks ? vl_coef(p.head, gout, sum) : 0.0f;
-    gb[v] = acc ? fma_((float)s, c, gb[v]) : (float)s * c;
-}
-
 // G of a block of 32 rows by 32 words, in pieces: under the rows' powers in z's place (X), and turned, under the words' (W),
 // with the sums of its columns where gb wants them.
 template <bool X, bool W>
@@ -753,52 +741,67 @@ __global__ __launch_bounds__(kVlB) void k_vl_grad(GradArgs p) {
     }
 }
 
-// gx (+)= the parts' sum, at the rows' places
-__global__ __launch_bounds__(kVlB) void k_vl_gx(const float *__restrict__ parts, int64_t rows, int64_t cols, const VlHead *head,
-                                                int64_t row0, const int32_t *__restrict__ from, const VlRow *__restrict__ row,
-                                                int64_t D, const float *gout, int sum, float *__restrict__ gx, int acc) {
-    const int64_t left = min(rows, head->count - row0);
-    const int slices = head->slices_x;
-    const float c = vl_coef(head, gout, sum);
-    for (int64_t n = blockIdx.x; n < left; n += gridDim.x) {
-        const int en = row[n].e;
-        float *out = gx + (int64_t)from[n] * D;
-        for (int64_t d = threadIdx.x; d < D; d += kVlB) {
-            double s = 0.0;
-#pragma unroll 8
-            for (int i = 0; i < slices; i++) s += (double)parts[((int64_t)i * rows + n) * cols + d];
-            const float v = __builtin_amdgcn_ldexpf((float)s, en);
-            out[d] = acc ? fma_(v, c, out[d]) : v * c;
-        }
-    }
-}
+// What is left of a piece, in one launch: gx (+)= its parts' sum, at the rows' places; gW (+)= its parts' sum; gb (+)= the sums of the
+// columns of G, which k_vl_grad left for every 32 rows; and at the last the loss, which of no rows is NaN, as a mean over nothing is
+// (a sum: 0).
+struct TailArgs {
+    unsigned gx, gw, gb;  // workgroups
+    VlHead *head;
+    const float *gout;
+    int sum;
+    int64_t row0, rows, V, D, words, cols;
+    const int32_t *from;  // of this piece's rows
+    const VlRow *row;
+    const int *term;
+    const float *parts_x, *parts_w, *column;
+    float *out_x, *out_w, *out_b;
+    int acc_x, acc_w, acc_b;
+    const double *losses;
+    float *loss;
+};
 
-// gW (+)= the parts' sum
-__global__ __launch_bounds__(kVlB) void k_vl_gw(const float *__restrict__ parts, int64_t part_rows, int64_t cols, const VlHead *head,
-                                                const int *__restrict__ term, int64_t V, int64_t D, const float *gout, int sum, float *__restrict__ gw, int acc) {
-    const int slices = head->slices_w;
-    const float c = head->count ? vl_coef(head, gout, sum) : 0.0f;
-    for (int64_t v = blockIdx.x; v < V; v += gridDim.x) {
-        const int ev = word_exponent(term[v]);
-        for (int64_t d = threadIdx.x; d < D; d += kVlB) {
-            double s = 0.0;
+__global__ __launch_bounds__(kVlB) void k_vl_ends(TailArgs p) {
+    __shared__ double sh[kVlB / kWave];
+    const int64_t count = p.head->count, left = min(p.rows, count - p.row0);
+    const float c = count ? vl_coef(p.head, p.gout, p.sum) : 0.0f;
+    unsigned b = blockIdx.x;
+    if (b < p.gx) {
+        const int slices = p.head->slices_x;
+        for (int64_t n = b; n < left; n += p.gx) {
+            const int en = p.row[n].e;
+            float *out = p.out_x + (int64_t)p.from[n] * p.D;
+            for (int64_t d = threadIdx.x; d < p.D; d += kVlB) {
+                double s = 0.0;
 #pragma unroll 8
-            for (int i = 0; i < slices; i++) s += (double)parts[((int64_t)i * part_rows + v) * cols + d];
-            const float x = __builtin_amdgcn_ldexpf((float)s, ev);
-            float *o = gw + v * D + d;
-            *o = acc ? fma_(x, c, *o) : x * c;
+                for (int i = 0; i < slices; i++) s += (double)p.parts_x[((int64_t)i * p.rows + n) * p.cols + d];
+                const float v = __builtin_amdgcn_ldexpf((float)s, en);
+                out[d] = p.acc_x ? fma_(v, c, out[d]) : v * c;
+            }
         }
+    } else if ((b -= p.gx) < p.gw) {
+        const int slices = p.head->slices_w;
+        for (int64_t v = b; v < p.V; v += p.gw) {
+            const int ev = word_exponent(p.term[v]);
+            for (int64_t d = threadIdx.x; d < p.D; d += kVlB) {
+                double s = 0.0;
+#pragma unroll 8
+                for (int i = 0; i < slices; i++) s += (double)p.parts_w[((int64_t)i * p.words + v) * p.cols + d];
+                const float x = __builtin_amdgcn_ldexpf((float)s, ev);
+                float *o = p.out_w + v * p.D + d;
+                *o = p.acc_w ? fma_(x, c, *o) : x * c;
+            }
+        }
+    } else if ((b -= p.gw) < p.gb) {
+        const int64_t v = (int64_t)b * kVlB + threadIdx.x, blocks = left > 0 ? (left + 31) / 32 : 0;
+        if (v >= p.V) return;
+        double s = 0.0;
+#pragma unroll 8
+        for (int64_t i = 0; i < blocks; i++) s += (double)p.column[i * p.words + v];
+        p.out_b[v] = p.acc_b ? fma_((float)s, c, p.out_b[v]) : (float)s * c;
+    } else {
+        const double t = vl_wg_sum(vl_lane_sum(p.losses, count), sh);
+        if (threadIdx.x == 0) *p.loss = p.sum ? (float)t : count ? (float)(t / (double)count) : __builtin_nanf("");
     }
-}
-
-// the loss of no rows is NaN, as a mean over nothing is (a sum: 0)
-__global__ __launch_bounds__(1024) void k_vl_total(const double *__restrict__ losses, const VlHead *__restrict__ head, int sum,
-                                                   float *__restrict__ loss) {
-    __shared__ double sh[1024 / kWave];
-    double t = 0.0;
-    for (int64_t i = threadIdx.x; i < head->count; i += 1024) t += losses[i];
-    t = vl_wg_sum(t, sh);
-    if (threadIdx.x == 0) *loss = sum ? (float)t : head->count ? (float)(t / (double)head->count) : __builtin_nanf("");
 }
 
 // ---- one call -----------------------------------------------------------------------------------------------------------------
@@ -808,7 +811,7 @@ struct SplitPlan {
     int64_t piece;     // rows of a piece, padded
     int slices, slices_w;  // parts of gx and of gW, at most; 0: gW is not cut
     int columns;       // slices of the rows where the words' largest are looked for
-    size_t from, list, losses, row, label_z, part, ew, ex, term, column, x, w, z, turned, parts, total;
+    size_t from, list, losses, row, label_z, part, ew, ex, term, column, x, w, z, turned, parts_x, parts_w, total;
 };
 
 static int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
@@ -843,17 +846,18 @@ static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool w
     p.w = take(true, p.v * p.dk * 4);
     p.z = take(grad, p.piece * p.v * 4);
     p.turned = take(want_w || want_b, p.piece * p.v * 4);
-    p.parts = take(want_x || (want_w && p.slices_w), std::max(want_x ? p.slices * p.piece : 0, want_w ? p.slices_w * p.v : 0) * p.d * 4);
+    p.parts_x = take(want_x, p.slices * p.piece * p.d * 4);
+    p.parts_w = take(want_w && p.slices_w, p.slices_w * p.v * p.d * 4);
     p.total = at;
     return p;
 }
 
 // The two forms' times by what they do, in us.  fp32 products start at once and run at 115 TFLOP/s; pieces have x and W read and written
 // first, whole tiles of rows, and some 370 TFLOP/s.  Both sides measured (us, fp32 products : pieces): 128000 x 2048 with gradients, 64
-// rows 1136 : 1456, 256 3655 : 1828; 32000 x 1024, 64 rows 186 : 257, 128 294 : 277, 4096 7262 : 2517; 2000 x 256, 1024 rows 83 : 104, 4096
-// 200 : 141; scored, 32000 x 1024, 64 rows 57 : 102, 128 90 : 105, 256 167 : 113; 5000 x 64, 512 rows 25 : 28, 1024 36 : 29.  Over the 400
-// sizes that the numbers are fitted to (1 to 4096 rows, 64 to 2048 columns, 500 to 128000 words) what it chooses takes 0.2% longer in the
-// mean than the better one, 13% at most.
+// rows 1148 : 1480, 256 3630 : 1872; 32000 x 1024, 64 rows 175 : 266, 128 283 : 289, 4096 7299 : 2540; 2000 x 256, 1024 rows 74 : 96, 4096
+// 189 : 135; scored, 32000 x 1024, 64 rows 55 : 102, 128 88 : 106, 256 165 : 115; 5000 x 64, 512 rows 23 : 28, 1024 34 : 29.  Over the 400
+// sizes that the numbers are fitted to (1 to 4096 rows, 64 to 2048 columns, 500 to 128000 words) what it chooses takes 0.1% longer in the
+// mean than the better one, 11% at most.
 bool vl_split_pays(int64_t N, int64_t D, int64_t V, bool grads) {
     if (N == 0 || N > kPieceRows * 16) return false;
     if (const char *form = getenv("NC_HIP_VOCAB_FORM")) return form[0] == 's';
@@ -934,26 +938,28 @@ int vl_split_run(const VlCall &c, const char *what) {
         g.of_w = {g.of_x.tiles_n, pl.slices_w, g.of_x.at_once};
         g.ex = m.ex, g.ew = m.ew;
         hipLaunchKernelGGL(k_vl_stats, (unsigned)(rows / 32), 1024, 0, c.st, g);
-        if (!grad) continue;
-        if (c.gw || c.gb) {
+        const bool turn = c.gw || c.gb;
+        if (turn) {
             const dim3 gw((unsigned)(pl.v / 32 / (kVlB / kWave)), (unsigned)pl.columns);
             hipLaunchKernelGGL(k_vl_words, gw, kVlB, 0, c.st, g);
         }
         const dim3 gg((unsigned)(pl.v / 32 / (kVlB / kWave)), (unsigned)(rows / 32));
-        const bool turn = c.gw || c.gb;
         if (c.gx && turn) hipLaunchKernelGGL((k_vl_grad<true, true>), gg, kVlB, 0, c.st, g);
         else if (c.gx) hipLaunchKernelGGL((k_vl_grad<true, false>), gg, kVlB, 0, c.st, g);
-        else hipLaunchKernelGGL((k_vl_grad<false, true>), gg, kVlB, 0, c.st, g);
-        if (c.gb)
-            hipLaunchKernelGGL(k_vl_bias, (unsigned)((c.V + kVlB - 1) / kVlB), kVlB, 0, c.st, g, c.gout, c.sum, c.gb, c.acc_b || r0);
+        else if (turn) hipLaunchKernelGGL((k_vl_grad<false, true>), gg, kVlB, 0, c.st, g);
+        TailArgs t{};
+        t.head = head, t.gout = c.gout, t.sum = c.sum, t.row0 = r0, t.rows = pl.piece, t.V = c.V, t.D = c.D, t.words = pl.v, t.cols = pl.d;
+        t.from = g.from, t.row = g.row, t.term = g.term, t.column = g.column, t.losses = losses, t.loss = c.loss;
+        t.parts_x = (float *)at(pl.parts_x), t.parts_w = (float *)at(pl.parts_w), t.out_x = c.gx, t.out_w = c.gw, t.out_b = c.gb;
+        t.acc_x = c.acc_x, t.acc_w = c.acc_w || r0, t.acc_b = c.acc_b || r0;
+        t.gb = c.gb ? (unsigned)((c.V + kVlB - 1) / kVlB) : 0;
         if (c.gx) {
             MmArgs a = m;
             a.A = (const char *)m.z, a.step_a = pl.v * 128, a.B = at(pl.w), a.step_b = pl.dk * 128;
             a.tiles_m = (int)(rows / kTileM), a.kblocks = (int)(pl.v / 16);
-            a.parts = (float *)at(pl.parts), a.part_rows = pl.piece, a.cols = pl.d;
+            a.parts = (float *)at(pl.parts_x), a.part_rows = pl.piece, a.cols = pl.d;
             product(std::integral_constant<int, MM_GX>{}, a, c.D, pl.slices);
-            hipLaunchKernelGGL(k_vl_gx, (unsigned)std::min<int64_t>(rows, 1 << 14), kVlB, 0, c.st, a.parts, pl.piece, pl.d, head, r0,
-                               from + r0, g.row, c.D, c.gout, c.sum, c.gx, c.acc_x);
+            t.gx = (unsigned)std::min<int64_t>(rows, 1 << 14);
         }
         if (c.gw) {
             MmArgs a = m;
@@ -961,16 +967,17 @@ int vl_split_run(const VlCall &c, const char *what) {
             a.tiles_m = (int)(pl.v / kTileM), a.kblocks = (int)(rows / 16);
             a.eg = g.term, a.gout = c.gout, a.out = c.gw, a.sum = c.sum, a.acc = c.acc_w || r0;
             if (pl.slices_w) {
-                a.parts = (float *)at(pl.parts), a.part_rows = pl.v, a.cols = pl.d;
+                a.parts = (float *)at(pl.parts_w), a.part_rows = pl.v, a.cols = pl.d;
                 product(std::integral_constant<int, MM_GW_PARTS>{}, a, c.D, pl.slices_w);
-                hipLaunchKernelGGL(k_vl_gw, (unsigned)std::min<int64_t>(c.V, 1 << 14), kVlB, 0, c.st, a.parts, pl.v, pl.d, head, g.term,
-                                   c.V, c.D, c.gout, c.sum, c.gw, a.acc);
+                t.gw = (unsigned)std::min<int64_t>(c.V, 1 << 14);
             } else {
                 product(std::integral_constant<int, MM_GW>{}, a, c.D, 1);
             }
         }
+        const unsigned last = r0 + pl.piece >= pl.n;
+        const unsigned groups = t.gx + t.gw + t.gb + last;
+        if (groups) hipLaunchKernelGGL(k_vl_ends, groups, kVlB, 0, c.st, t);
     }
-    hipLaunchKernelGGL(k_vl_total, 1, 1024, 0, c.st, losses, head, c.sum, c.loss);
     return check_launch(what);
 }
 
