@@ -17,7 +17,7 @@ namespace nchip {
 constexpr int kEmbB = 256;
 constexpr int kClearRows = 32;    // rows of the table that one workgroup clears, or as many as it has side by side
 constexpr int kRankB = 1024, kRankMost = 8192;  // tokens whose places are counted, at most
-constexpr int kFewMost = 1024;                  // tokens whose rows are summed without a sort, at most
+constexpr int kFewMost = 2560;                  // tokens whose rows are summed without a sort, at most
 constexpr int kDigitBits = 10, kChunk = 1024;   // of the others' sort
 constexpr int kSumChunks = 256;  // chunks whose counts each workgroup adds up itself, at most; more are summed by a launch of its own
 constexpr int64_t kMaxTokens = int64_t(1) << 30;
@@ -378,18 +378,18 @@ __global__ __launch_bounds__(kEmbB) void k_embed_grad(EmbGrad p) {
 
 // Few tokens, in one launch and unsorted: a workgroup for every position, which goes on if its token has none earlier, lists the token's
 // positions and sums their rows, 16 at a time and these in fp64; the workgroups behind them clear rows.
-template <bool AL>
+template <bool AL, int MOST>
 __global__ __launch_bounds__(kEmbB) void k_embed_few(EmbGrad p, const int32_t *__restrict__ tokens) {
     constexpr int U = 16;
-    __shared__ uint32_t token[kFewMost];
-    __shared__ int list[kFewMost];
-    __shared__ unsigned long long masks[kFewMost / kWave];
+    __shared__ uint32_t token[MOST];
+    __shared__ uint16_t list[MOST];
+    __shared__ unsigned long long masks[MOST / kWave];
     __shared__ double part[4][kEmbB];
     const int N = (int)p.N, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int64_t c = 4 * (((int64_t)blockIdx.y << p.l.shift) + (threadIdx.x & ((1 << p.l.shift) - 1)));
     const int R = kEmbB >> p.l.shift, group = threadIdx.x >> p.l.shift;
 #pragma unroll
-    for (int u = 0; u < kFewMost / kEmbB; u++) {
+    for (int u = 0; u < MOST / kEmbB; u++) {
         const int j = u * kEmbB + threadIdx.x;
         token[j] = j < N ? (uint32_t)tokens[j] : ~0u;
     }
@@ -410,26 +410,33 @@ __global__ __launch_bounds__(kEmbB) void k_embed_few(EmbGrad p, const int32_t *_
     const uint32_t t = token[blockIdx.x];
     if (!p.counts(t)) return;
 #pragma unroll
-    for (int u = 0; u < kFewMost / kEmbB; u++) {
+    for (int u = 0; u < MOST / kEmbB; u++) {
         const unsigned long long m = __ballot(token[u * kEmbB + threadIdx.x] == t);
         if (lane == 0) masks[u * (kEmbB / kWave) + wave] = m;
     }
     __syncthreads();
-    int count = 0, first = -1;
-    for (int k = 0; k < kFewMost / kWave; k++) {
-        const unsigned long long m = masks[k];
-        if (first < 0 && m) first = k * kWave + __builtin_ctzll(m);
-        if (k % (kEmbB / kWave) == wave && (m >> lane & 1)) list[count + __popcll(m & ((1ull << lane) - 1))] = k * kWave + lane;
-        count += __popcll(m);
+    const unsigned long long mine = lane < MOST / kWave ? masks[lane] : 0;
+    int upto = __popcll(mine);  // the token's positions up to this lane's mask
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int below = __shfl_up(upto, d);
+        if (lane >= d) upto += below;
     }
-    if (first != (int)blockIdx.x) return;
+    const int count = __shfl(upto, kWave - 1), k_first = __builtin_ctzll(__ballot(mine != 0));
+    if (k_first * kWave + __builtin_ctzll(masks[k_first]) != (int)blockIdx.x) return;
+#pragma unroll
+    for (int u = 0; u < MOST / kEmbB; u++) {
+        const int k = u * (kEmbB / kWave) + wave, before = __shfl(upto, k);
+        const unsigned long long m = masks[k];
+        if (m >> lane & 1) list[before - __popcll(m >> lane)] = (uint16_t)(k * kWave + lane);
+    }
     __syncthreads();
     double sum[4] = {};
     if (c < p.l.D)
         for (int k0 = group; k0 < count; k0 += U * R) {
             f4 v[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) v[u] = k0 + u * R < count ? piece<AL>(p.g + list[k0 + u * R] * p.l.D, c, p.l.D) : f4{};
+            for (int u = 0; u < U; u++) v[u] = k0 + u * R < count ? piece<AL>(p.g + (int64_t)list[k0 + u * R] * p.l.D, c, p.l.D) : f4{};
 #pragma unroll
             for (int d = 1; d < U; d *= 2)
 #pragma unroll
@@ -482,8 +489,9 @@ __global__ __launch_bounds__(kEmbB) void k_embed_join(EmbGrad p) {
 
 static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
-// Without a sort: 17 -> 12 us at 800 tokens of 100 columns, 20 -> 14 at 1024 of 2048.  A token that all positions have is one workgroup's
-// and slice's, so long rows of many tokens are sorted all the same (1024 times the same of 512: 38 -> 46 us, of 2048: 42 -> 91).
+// Without a sort: 17 -> 12 us at 800 tokens of 100 columns, 19 -> 16 at 2331 of 256, 20 -> 18 at 3000.  A token that all positions have
+// is one workgroup's and slice's, so long rows of many tokens are sorted all the same (1024 times the same of 2048: 27 us sorted, 91
+// unsorted; of 512: 45 unsorted, 2331 times of 256: 33 sorted, 50 unsorted).
 static bool sums_unsorted(int64_t N, int64_t D) { return N <= kFewMost && N * D <= int64_t(1) << 20; }
 
 // Sorted positions of a block: 8 where blocks of 32 would leave most of the chip idle, at the cost of more parts of tokens that
@@ -584,8 +592,9 @@ extern "C" NC_HIP_API int nc_hip_embedding_bwd(int64_t N, int64_t V, int64_t D, 
     const bool al = D % 4 == 0 && aligned16(g) && aligned16(gw);
     const dim3 grid((unsigned)(groups + clear), (unsigned)p.l.slices()), joins((unsigned)groups, (unsigned)p.l.slices());
     if (few) {
-        if (al) hipLaunchKernelGGL(k_embed_few<true>, grid, kEmbB, 0, st, p, tokens);
-        else hipLaunchKernelGGL(k_embed_few<false>, grid, kEmbB, 0, st, p, tokens);
+        auto sum = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, kEmbB, 0, st, p, tokens); };
+        if (N <= 1024) al ? sum(k_embed_few<true, 1024>) : sum(k_embed_few<false, 1024>);
+        else al ? sum(k_embed_few<true, kFewMost>) : sum(k_embed_few<false, kFewMost>);
         return check_launch(what);
     }
     if (N > kRankMost) {

@@ -83,7 +83,7 @@ EMBED = [(1, 1, 1, "even"), (1, 5, 4, "even"), (2, 3, 2, "even"), (7, 5, 3, "eve
          (1500, 40, 260, "one"), (4097, 2000, 33, "rank"), (5000, 70000, 12, "rank"), (3, 100, 5001, "even"), (257, 31, 4, "outside"),
          (20001, 3000, 20, "rank"), (40000, 7, 9, "even"), (70000, 100003, 5, "rank"),
          (8192, 31, 3, "rank"), (8193, 1023, 4, "rank"), (8200, 1024, 6, "even"), (9000, 1 << 20, 1, "even"), (10000, 50, 7, "outside"),
-         (300000, 5000, 3, "rank"), (1024, 1000, 40, "rank"), (1024, 3, 1030, "one"), (1023, 700, 5, "outside"), (1025, 100, 33, "one"), (300, 9, 2000, "even"), (263000, 2, 2, "one"), (33000, 1500, 300, "rank")]
+         (300000, 5000, 3, "rank"), (1024, 1000, 40, "rank"), (1024, 3, 1030, "one"), (1023, 700, 5, "outside"), (1025, 100, 33, "one"), (300, 9, 2000, "even"), (2560, 1009, 131, "rank"), (2560, 20, 409, "outside"), (2561, 300, 64, "even"), (2561, 300, 410, "one"), (263000, 2, 2, "one"), (33000, 1500, 300, "rank")]
 
 
 def some_tokens(rng, N, V, how):

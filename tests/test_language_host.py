@@ -99,13 +99,13 @@ def test_kernel_layer_refusals(lib):
     bad("NULL", K.embedding_fwd, 1, 5, 4, P, 4, P, 1.0, None)
     bad("8-byte", K.embedding_fwd, 1, 5, 4, P, 4, P, 1.0, P, bad=P + 4)
     bad("rows closer", K.embedding_fwd, 1, 5, 4, P, 3, P, 1.0, P)
-    n = K.embedding_bwd_workspace(2000, 5, 4)
+    n = K.embedding_bwd_workspace(9000, 5, 4)
     assert n > 0 and K.embedding_bwd_workspace(0, 5, 4) == 0
-    bad("workspace of", K.embedding_bwd, 2000, 5, 4, P, -1, 1.0, P, P, P, n - 1)
-    bad("workspace of", K.embedding_bwd, 2000, 5, 4, P, -1, 1.0, P, P, None, n)
-    bad("16-byte", K.embedding_bwd, 2000, 5, 4, P, -1, 1.0, P, P, P + 4, n)
-    bad("NULL", K.embedding_bwd, 2000, 5, 4, P, -1, 1.0, None, P, P, n)
-    bad("NULL", K.embedding_bwd, 2000, 5, 4, P, -1, 1.0, P, None, P, n)
+    bad("workspace of", K.embedding_bwd, 9000, 5, 4, P, -1, 1.0, P, P, P, n - 1)
+    bad("workspace of", K.embedding_bwd, 9000, 5, 4, P, -1, 1.0, P, P, None, n)
+    bad("16-byte", K.embedding_bwd, 9000, 5, 4, P, -1, 1.0, P, P, P + 4, n)
+    bad("NULL", K.embedding_bwd, 9000, 5, 4, P, -1, 1.0, None, P, P, n)
+    bad("NULL", K.embedding_bwd, 9000, 5, 4, P, -1, 1.0, P, None, P, n)
     for p in (-0.01, 1.01, float("nan")):
         bad("p must be", K.dropout_fwd, 4, p, 1, 2, P, None, P)
         bad("p must be", K.dropout_bwd, 4, p, 1, 2, P, P)
