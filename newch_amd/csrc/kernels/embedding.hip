@@ -1,11 +1,11 @@
 // Rows of a table looked up by token and scaled, and the table's gradient: y[i] = s W[t_i], gW[v] (+)= s sum over t_i = v of g[i].  No
 // counterpart in the reference on the device (its index_select copies rows on the host).
 //
-// The gradient sums in a fixed order without atomics.  Positions are sorted by (token, position); blocks of 8 or 32 sorted
-// positions are summed by a lane for every four columns.  A token whose positions lie within one block has its row written there; one
-// that goes over blocks leaves a part with each (at most two a block: one of a token that began before it, one of a token that goes on
-// behind it), which a second kernel adds in the blocks' order, in fp64.  Rows of tokens that do not occur are cleared by workgroups of
-// the same launch that look their rows up in the sorted tokens, so a stored gradient is written once.
+// The gradient sums in a fixed order without atomics.  Of few tokens a workgroup for each sums its token's rows (k_embed_few).  Positions of
+// more are sorted by (token, position); blocks of 8 or 32 sorted positions are summed by a lane for every four columns.  A token whose
+// positions lie within one block has its row written there; one that goes over blocks leaves a part with each (at most two a block: one
+// of a token that began before it, one of a token that goes on behind it), which a second kernel adds in the blocks' order, in fp64.
+// Rows of tokens that do not occur are cleared by workgroups of the same launch, so a stored gradient is written once.
 //
 // Bound by memory: reads 4 N D bytes of g, writes 4 V D (what is stored) or reads and writes the rows that occur (what is added).
 #include "common.hpp"
@@ -15,7 +15,8 @@
 namespace nchip {
 
 constexpr int kEmbB = 256;
-constexpr int kClearRows = 32;    // rows of the table that one workgroup clears, or as many as it has side by side
+constexpr int kClearMost = 32768;  // words of the table that one workgroup clears, at most
+constexpr int kClearFew = 4096;    // and without a sort
 constexpr int kRankB = 1024, kRankMost = 8192;  // tokens whose places are counted, at most
 constexpr int kFewMost = 2560;                  // tokens whose rows are summed without a sort, at most
 constexpr int kDigitBits = 10, kChunk = 1024;   // of the others' sort
@@ -30,7 +31,6 @@ struct Lay {
     int pieces() const { return (int)((D + 3) / 4); }
     int slices() const { return (pieces() + (1 << shift) - 1) >> shift; }
     int rows() const { return kEmbB >> shift; }
-    int clear_rows() const { return rows() > kClearRows ? rows() : kClearRows; }
 };
 
 static Lay lay_of(int64_t D) {
@@ -284,7 +284,8 @@ struct EmbGrad {
     uint32_t padding;    // a token without a gradient (>= V: none)
     float scale;
     int acc;
-    int clear_rows;      // of a workgroup that clears
+    int clear_words;     // of a workgroup that clears, a multiple of 4 kEmbB
+    int clear_shift;     // words by which gw lies behind a 16-byte boundary
     Lay l;
 
     __device__ __forceinline__ bool counts(uint32_t t) const { return t < V && t != padding; }
@@ -341,35 +342,77 @@ __device__ __forceinline__ void sum_block(const EmbGrad &p, int64_t block, int64
     flush(k1 < p.N && p.sorted[k1] == cur);
 }
 
-// of `count` rows of the table from r0 on, those whose tokens do not occur
-template <bool AL>
-__device__ __forceinline__ void clear_rows(const EmbGrad &p, int64_t r0, int count, int64_t c) {
-    __shared__ int used[kEmbB];
-    used[threadIdx.x] = 0;
-    int64_t lo = 0, hi = p.N;  // the first sorted position of row r0 or later: 64 places at a time
-    while (lo < hi) {
-        const int64_t step = (hi - lo + kWave - 1) / kWave, k = lo + (int64_t)(threadIdx.x & (kWave - 1)) * step;
-        const int less = __popcll(__ballot(k < hi && p.sorted[min(k, hi - 1)] < r0));
-        hi = min(hi, lo + less * step);
-        if (less) lo += (less - 1) * step + 1;
-    }
+// A workgroup's words of the table, whatever rows they are of: cleared where the row's token does not occur.  By whole 16 bytes at their
+// boundaries, since rows of odd lengths begin anywhere (84 tokens of 90560 x 2889, both ways: 306 us with rows stored as they begin, 180
+// so).  Without a sort a workgroup clears 4096 words, since 32768 leave the memory idle at the end (213 us).  `find` marks the tokens that occur among rows r0 to r1.
+template <class F>
+__device__ __forceinline__ void clear_words(const EmbGrad &p, F find) {
+    __shared__ uint32_t used[kClearMost / 32 + 1];
+    __shared__ int any;
+    const int64_t D = p.l.D, all = p.V * D;
+    const int64_t chunk = (int64_t)blockIdx.y * (gridDim.x - p.sum_groups) + (blockIdx.x - p.sum_groups);
+    const int64_t first = chunk * p.clear_words - p.clear_shift;  // 16-byte aligned, and before the table for the first chunk
+    const int64_t f0 = max(first, int64_t(0)), f1 = min(first + p.clear_words, all);
+    if (f0 >= f1) return;
+    const int64_t r0 = f0 / D, r1 = (f1 - 1) / D;
+    for (int k = threadIdx.x; k <= (int)(r1 - r0) / 32; k += kEmbB) used[k] = 0;
+    if (threadIdx.x == 0) any = 0;
     __syncthreads();
-    for (int64_t k = lo + threadIdx.x; k < p.N; k += kEmbB) {
-        const uint32_t t = p.sorted[k];
-        if (t >= r0 + count) break;
-        if (p.counts(t)) used[t - r0] = 1;
-    }
+    find(r0, r1, [&](uint32_t t) {
+        const int k = (int)((int64_t)t - r0);
+        atomicOr(used + k / 32, 1u << (k & 31));
+        any = 1;
+    });
     __syncthreads();
-    if (c >= p.l.D) return;
-    for (int r = threadIdx.x >> p.l.shift; r < count; r += kEmbB >> p.l.shift)
-        if (r0 + r < p.V && !used[r]) put<AL>(p.gw + (r0 + r) * p.l.D, c, p.l.D, f4{});
+    const bool some = any;
+    const float per = 1.0f / (float)D;
+    const int64_t start = r0 * D;
+    for (int k = threadIdx.x * 4; k < p.clear_words; k += 4 * kEmbB) {
+        const int64_t i = first + k;
+        if (i >= f0 && i + 4 <= f1 && !some) {
+            __builtin_nontemporal_store(f4{}, (f4 *)(p.gw + i));
+            continue;
+        }
+        if (i + 4 <= f0 || i >= f1) continue;
+        const int64_t from = max(i, f0), rel = from - start;
+        int r = (int)((float)rel * per);  // at most one off
+        r += (int64_t)(r + 1) * D <= rel ? 1 : (int64_t)r * D > rel ? -1 : 0;
+        const bool left = (int64_t)(r + 1) * D < i + 4 - start || i < f0 || i + 4 > f1;  // more than one row, or not whole
+        if (!left) {
+            if (!(used[r / 32] >> (r & 31) & 1)) __builtin_nontemporal_store(f4{}, (f4 *)(p.gw + i));
+            continue;
+        }
+        int64_t next = (int64_t)(r + 1) * D;
+        for (int64_t j = from; j < min(i + 4, f1); j++) {
+            if (j - start >= next) r++, next += D;
+            if (!(used[r / 32] >> (r & 31) & 1)) p.gw[j] = 0.0f;
+        }
+    }
+}
+
+// clear_words by the sorted tokens: 64 places at a time for the first of row r0 or later
+__device__ __forceinline__ void clear_sorted(const EmbGrad &p) {
+    clear_words(p, [&](int64_t r0, int64_t r1, auto mark) {
+        int64_t lo = 0, hi = p.N;
+        while (lo < hi) {
+            const int64_t step = (hi - lo + kWave - 1) / kWave, k = lo + (int64_t)(threadIdx.x & (kWave - 1)) * step;
+            const int less = __popcll(__ballot(k < hi && p.sorted[min(k, hi - 1)] < r0));
+            hi = min(hi, lo + less * step);
+            if (less) lo += (less - 1) * step + 1;
+        }
+        for (int64_t k = lo + threadIdx.x; k < p.N; k += kEmbB) {
+            const uint32_t t = p.sorted[k];
+            if (t > r1) break;
+            if (p.counts(t)) mark(t);
+        }
+    });
 }
 
 template <bool AL, int S>
 __global__ __launch_bounds__(kEmbB) void k_embed_grad(EmbGrad p) {
     const int64_t c = 4 * (((int64_t)blockIdx.y << p.l.shift) + (threadIdx.x & ((1 << p.l.shift) - 1)));
     if (blockIdx.x >= p.sum_groups) {
-        clear_rows<AL>(p, (int64_t)(blockIdx.x - p.sum_groups) * p.clear_rows, p.clear_rows, c);
+        clear_sorted(p);
         return;
     }
     const int64_t block = (int64_t)blockIdx.x * (kEmbB >> p.l.shift) + (threadIdx.x >> p.l.shift);
@@ -388,25 +431,22 @@ __global__ __launch_bounds__(kEmbB) void k_embed_few(EmbGrad p, const int32_t *_
     const int N = (int)p.N, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int64_t c = 4 * (((int64_t)blockIdx.y << p.l.shift) + (threadIdx.x & ((1 << p.l.shift) - 1)));
     const int R = kEmbB >> p.l.shift, group = threadIdx.x >> p.l.shift;
+    if (blockIdx.x >= p.sum_groups) {
+        clear_words(p, [&](int64_t r0, int64_t r1, auto mark) {
+#pragma unroll 4
+            for (int j = threadIdx.x; j < N; j += kEmbB) {
+                const uint32_t t = (uint32_t)tokens[j];
+                if (p.counts(t) && t >= r0 && t <= r1) mark(t);
+            }
+        });
+        return;
+    }
 #pragma unroll
     for (int u = 0; u < MOST / kEmbB; u++) {
         const int j = u * kEmbB + threadIdx.x;
         token[j] = j < N ? (uint32_t)tokens[j] : ~0u;
     }
     __syncthreads();
-    if (blockIdx.x >= p.sum_groups) {
-        __shared__ int used[kEmbB];
-        const int64_t r0 = (int64_t)(blockIdx.x - p.sum_groups) * p.clear_rows;
-        used[threadIdx.x] = 0;
-        __syncthreads();
-        for (int j = threadIdx.x; j < N; j += kEmbB)
-            if (p.counts(token[j]) && token[j] >= r0 && token[j] < r0 + p.clear_rows) used[token[j] - r0] = 1;
-        __syncthreads();
-        if (c >= p.l.D) return;
-        for (int r = group; r < p.clear_rows; r += R)
-            if (r0 + r < p.V && !used[r]) put<AL>(p.gw + (r0 + r) * p.l.D, c, p.l.D, f4{});
-        return;
-    }
     const uint32_t t = token[blockIdx.x];
     if (!p.counts(t)) return;
 #pragma unroll
@@ -585,12 +625,15 @@ extern "C" NC_HIP_API int nc_hip_embedding_bwd(int64_t N, int64_t V, int64_t D, 
     const bool few = sums_unsorted(N, D);
     const int64_t groups = few ? N : (p.blocks + p.l.rows() - 1) / p.l.rows();
     p.sum_groups = (unsigned)groups;
-    p.clear_rows = p.l.clear_rows();
-    const int64_t clear = accumulate ? 0 : (V + p.clear_rows - 1) / p.clear_rows;
-    if ((groups + clear) * p.l.slices() * kEmbB > kMaxLanes)
+    const int64_t slices = p.l.slices(), words = V * D;
+    p.clear_words = (int)std::max<int64_t>(4 * kEmbB, std::min<int64_t>(few ? kClearFew : kClearMost, words / 4096 / (4 * kEmbB) * (4 * kEmbB)));
+    p.clear_shift = (int)((uintptr_t)gw / 4 & 3u);
+    const int64_t chunks = (words + p.clear_shift + p.clear_words - 1) / p.clear_words;
+    const int64_t clear = accumulate ? 0 : (chunks + slices - 1) / slices;
+    if ((groups + clear) * slices * kEmbB > kMaxLanes)
         return set_error(NC_HIP_ERR_ARG, "%s: bad size, no launch holds it", what);
     const bool al = D % 4 == 0 && aligned16(g) && aligned16(gw);
-    const dim3 grid((unsigned)(groups + clear), (unsigned)p.l.slices()), joins((unsigned)groups, (unsigned)p.l.slices());
+    const dim3 grid((unsigned)(groups + clear), (unsigned)slices), joins((unsigned)groups, (unsigned)slices);
     if (few) {
         auto sum = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, kEmbB, 0, st, p, tokens); };
         if (N <= 1024) al ? sum(k_embed_few<true, 1024>) : sum(k_embed_few<false, 1024>);

@@ -83,7 +83,7 @@ EMBED = [(1, 1, 1, "even"), (1, 5, 4, "even"), (2, 3, 2, "even"), (7, 5, 3, "eve
          (1500, 40, 260, "one"), (4097, 2000, 33, "rank"), (5000, 70000, 12, "rank"), (3, 100, 5001, "even"), (257, 31, 4, "outside"),
          (20001, 3000, 20, "rank"), (40000, 7, 9, "even"), (70000, 100003, 5, "rank"),
          (8192, 31, 3, "rank"), (8193, 1023, 4, "rank"), (8200, 1024, 6, "even"), (9000, 1 << 20, 1, "even"), (10000, 50, 7, "outside"),
-         (300000, 5000, 3, "rank"), (1024, 1000, 40, "rank"), (1024, 3, 1030, "one"), (1023, 700, 5, "outside"), (1025, 100, 33, "one"), (300, 9, 2000, "even"), (2560, 1009, 131, "rank"), (2560, 20, 409, "outside"), (2561, 300, 64, "even"), (2561, 300, 410, "one"), (263000, 2, 2, "one"), (33000, 1500, 300, "rank")]
+         (300000, 5000, 3, "rank"), (1024, 1000, 40, "rank"), (1024, 3, 1030, "one"), (1023, 700, 5, "outside"), (1025, 100, 33, "one"), (300, 9, 2000, "even"), (6, 9001, 1001, "even"), (3, 1501, 2889, "outside"), (9000, 70000, 37, "rank"), (2560, 1009, 131, "rank"), (2560, 20, 409, "outside"), (2561, 300, 64, "even"), (2561, 300, 410, "one"), (263000, 2, 2, "one"), (33000, 1500, 300, "rank")]
 
 
 def some_tokens(rng, N, V, how):
@@ -145,6 +145,25 @@ def test_embedding_gradient(K, shape, accumulate):
         assert (got[untouched] == old[untouched]).all()
         runs.append(got)
     assert (runs[0] == runs[2]).all(), "the same call twice"
+
+
+@pytest.mark.parametrize("D", [1, 2, 3, 5, 66, 1023])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+@pytest.mark.parametrize("N", [0, 3, 3001])
+def test_embedding_gradient_clears(K, N, shift, D):
+    """Rows of all tokens that do not occur, however the table lies and however few they are."""
+    for V in (1, 2, 37, 40000 // D + 1, 200000 // D + 3):
+        rng = np.random.default_rng(V)
+        tokens = (rng.integers(0, V, N) // 7 * 7).astype(np.int32)
+        gp, _g = up(np.ones((max(N, 1), D), np.float32))
+        tok, _t = up(tokens if N else np.zeros(1, np.int32))
+        n = K.embedding_bwd_workspace(N, V, D)
+        ws = DeviceBuffer.from_numpy(np.zeros(max(n, 16), np.uint8))
+        gw = Out((V, D), shift=shift)
+        K.embedding_bwd(N, V, D, tok, -1, 1.0, gp, gw.ptr, ws.ptr, n, accumulate=False)
+        synchronize()
+        count = np.bincount(tokens, minlength=V).astype(np.float32)
+        assert (gw.get() == count[:, None]).all()
 
 
 def test_embedding_of_nothing(K):
