@@ -281,8 +281,14 @@ struct VlPlan {
     int64_t ldz, piece;
     int chunks, slices;
     int64_t slice;  // words of a part of gx
+    bool few_x, few_w;  // gx and gW by vocab_few.hip
     size_t losses, label_z, part, rows, z, parts, total;
 };
+
+// Whether gx and gW are vocab_few.hip's (rows over words x columns, us without : with): 23 over 54997 x 1712 389 : 283, 8 over 4000 x 1024
+// 38 : 31, 23 over 4000 x 256 31 : 31, 1000 x 1024 24 : 31; gW alone, 60 over 54997 x 1712 517 : 440; gx of more than 32 rows takes longer
+// (60: 163 : 188).  Rows that are no whole 16 bytes are written at half the rate.
+static bool vl_few_pays(int64_t D, int64_t V) { return D % 4 == 0 && D >= 128 && V * D >= int64_t(1) << 21; }
 
 static VlPlan vl_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w) {
     VlPlan p{};
@@ -293,7 +299,9 @@ static VlPlan vl_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w)
     // gx of few rows: its words in parts, as many as give the chip's CUs two tiles of 64 x 64 each, of at least 512 words
     const int64_t tiles = (p.piece + 63) / 64 * ((D + 63) / 64);
     const int64_t cut = std::max<int64_t>(1, std::min((2 * kPlanCUs + tiles - 1) / std::max<int64_t>(tiles, 1), V / 512));
-    p.slice = cut > 1 ? ((V + cut - 1) / cut + 31) / 32 * 32 : V;
+    const bool few = vl_few_pays(D, V) && p.piece == N;
+    p.few_x = few && N <= 32, p.few_w = few && N <= 64;
+    p.slice = p.few_x ? vl_few_slice(D, V) : cut > 1 ? ((V + cut - 1) / cut + 31) / 32 * 32 : V;
     p.slices = (int)((V + p.slice - 1) / p.slice);
     p.losses = 256;
     p.label_z = p.losses + vl_round256((size_t)N * 8);
@@ -301,7 +309,7 @@ static VlPlan vl_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w)
     p.rows = p.part + vl_round256((size_t)p.piece * p.chunks * sizeof(f2));
     p.z = p.rows + (want_w ? vl_round256((size_t)(N * D) * 4) : 0);
     p.parts = p.z + vl_round256((size_t)(p.piece * p.ldz) * 4);
-    p.total = p.parts + (want_x && p.slices > 1 ? (size_t)p.slices * p.piece * D * 4 : 0);
+    p.total = p.parts + (want_x && (p.few_x || p.slices > 1) ? (size_t)p.slices * p.piece * D * 4 : 0);
     return p;
 }
 
@@ -356,6 +364,7 @@ extern "C" NC_HIP_API int nc_hip_linear_cross_entropy(int64_t N, int64_t D, int6
     if (!count_here) hipLaunchKernelGGL(k_vl_count, 1, 1024, 0, st, a);
     for (int64_t r0 = 0; r0 < N; r0 += plan.piece) {
         a.row0 = r0, a.rows = std::min(plan.piece, N - r0), a.count_here = count_here && r0 == 0;
+        const VlFew few{N, D, V, w, ldw, z, plan.ldz, clean, parts, plan.slice, gw, acc_w};
         int rc = nc_hip_gemm_f32_bias(0, 1, a.rows, V, D, 1.0f, x + r0 * ldx, ldx, w, ldw, bias, z, plan.ldz, stream);
         if (rc) return rc;
         if (plan.chunks > 1) {
@@ -368,8 +377,10 @@ extern "C" NC_HIP_API int nc_hip_linear_cross_entropy(int64_t N, int64_t D, int6
         } else {
             hipLaunchKernelGGL(k_vl_softmax<false>, (unsigned)a.rows, kVlB, 0, st, a);
         }
-        const bool cut = gx && plan.slices > 1;
-        if (cut) {
+        const bool cut = gx && (plan.few_x || plan.slices > 1);
+        if (plan.few_x && gx) {
+            vl_few_gx(few, st);
+        } else if (cut) {
             const int64_t whole = V / plan.slice, rest = V - whole * plan.slice, part = a.rows * D;
             const int64_t shape = whole, sa = plan.slice, sb = plan.slice * ldw;
             rc = nc_hip_gemm_f32_bmm(0, 0, a.rows, D, plan.slice, z, plan.ldz, w, ldw, 0.0f, parts, D, 1, &shape, &sa, &sb, &part, nullptr, 0, stream);
@@ -379,7 +390,8 @@ extern "C" NC_HIP_API int nc_hip_linear_cross_entropy(int64_t N, int64_t D, int6
         } else if (gx) {
             rc = nc_hip_gemm_f32(0, 0, a.rows, D, V, 1.0f, z, plan.ldz, w, ldw, acc_x ? 1.0f : 0.0f, gx + r0 * D, D, stream);
         }
-        if (!rc && gw)
+        if (gw && plan.few_w && aligned16(gw)) vl_few_gw(few, st);
+        else if (!rc && gw)
             rc = nc_hip_gemm_f32(1, 0, V, D, a.rows, 1.0f, z, plan.ldz, clean + r0 * D, D, acc_w || r0 ? 1.0f : 0.0f, gw, D, stream);
         if (rc) return rc;
         t.rows = a.rows, t.n = a.rows * D, t.gx = cut ? gx + r0 * D : nullptr, t.acc_b = acc_b || r0;

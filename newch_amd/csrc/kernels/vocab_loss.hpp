@@ -73,6 +73,23 @@ inline int64_t vl_piece_rows(int64_t most) {
     return most;
 }
 
+// gx and gW of few rows (vocab_few.hip); D a multiple of 4, gw and z's rows 16-byte aligned
+struct VlFew {
+    int64_t N, D, V;
+    const float *w;
+    int64_t ldw;
+    const float *z;  // G [N][ldz]
+    int64_t ldz;
+    const float *clean;  // [N][D]
+    float *parts;   // [slices][N][D]
+    int64_t slice;  // words of a part of gx
+    float *gw;
+    int acc_w;
+};
+int64_t vl_few_slice(int64_t D, int64_t V);
+void vl_few_gx(const VlFew &p, hipStream_t st);
+void vl_few_gw(const VlFew &p, hipStream_t st);
+
 // whether the products of a call are worth cutting into pieces, the workspace that takes, and the call itself
 bool vl_split_pays(int64_t N, int64_t D, int64_t V, bool grads);
 size_t vl_split_workspace(int64_t N, int64_t D, int64_t V, bool want_x, bool want_w, bool want_b);

@@ -264,7 +264,8 @@ def form(request, monkeypatch):
 
 # N, D, V
 LOSS = [(1, 1, 1), (1, 7, 3), (40, 31, 9001), (3, 1030, 4097), (260, 33, 300), (2, 4, 1), (5, 33, 17), (64, 64, 64), (65, 130, 257), (300, 96, 1000), (257, 256, 513), (1000, 40, 50),
-        (130, 512, 2050), (513, 100, 5003), (1030, 260, 1027)]
+        (130, 512, 2050), (513, 100, 5003), (1030, 260, 1027),
+        (1, 128, 20000), (5, 512, 4099), (31, 1028, 2050), (32, 260, 8191), (33, 132, 16000), (64, 1164, 2050)]
 
 
 def loss_inputs(N, D, V, seed, bias, ignored, confident=True):
