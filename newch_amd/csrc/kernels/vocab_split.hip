@@ -854,8 +854,8 @@ static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool w
 
 // The two forms' times by what they do, in us.  fp32 products start at once and run at 115 TFLOP/s; pieces have x and W read and written
 // first, whole tiles of rows, and some 370 TFLOP/s.  Both sides measured (us, fp32 products : pieces): 128000 x 2048 with gradients, 64
-// rows 1148 : 1480, 256 3630 : 1872; 32000 x 1024, 64 rows 175 : 266, 128 283 : 289, 4096 7299 : 2540; 2000 x 256, 1024 rows 74 : 96, 4096
-// 189 : 135; scored, 32000 x 1024, 64 rows 55 : 102, 128 88 : 106, 256 165 : 115; 5000 x 64, 512 rows 23 : 28, 1024 34 : 29.  Over the 400
+// rows 1172 : 1418, 256 3632 : 1865; 32000 x 1024, 64 rows 172 : 265, 128 300 : 288, 4096 7284 : 2542; 2000 x 256, 1024 rows 73 : 96, 4096
+// 192 : 136; scored, 32000 x 1024, 64 rows 55 : 102, 128 88 : 106, 256 165 : 115; 5000 x 64, 512 rows 23 : 28, 1024 34 : 29.  Over the 400
 // sizes that the numbers are fitted to (1 to 4096 rows, 64 to 2048 columns, 500 to 128000 words) what it chooses takes 0.1% longer in the
 // mean than the better one, 11% at most.
 bool vl_split_pays(int64_t N, int64_t D, int64_t V, bool grads) {
