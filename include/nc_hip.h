@@ -362,7 +362,7 @@ NC_HIP_API int nc_hip_cross_attention_bwd(int64_t B, int64_t Lq, int64_t Lk, int
  * one as (i << 32) | (uint32)token, or all ones.  Backward: gw [V, D] contiguous (+)= scale * the sum of g [N, D] over the positions of each
  * token, in a fixed order; tokens outside [0, V) and the token `padding` (negative: none) have no gradient, and g is not read at their
  * positions.  Rows whose token does not occur become zero where gw is stored and stay where it is added to.  gw does not overlap g; the
- * workspace is 16-byte aligned.  N <= 2^30, V < 2^31. */
+ * workspace is 16-byte aligned (few tokens need none).  N <= 2^30, V < 2^31. */
 NC_HIP_API int nc_hip_embedding_fwd(int64_t N, int64_t V, int64_t D, const float *w, int64_t ldw, const int32_t *tokens, float scale,
                                     float *y, uint64_t *bad, void *stream);
 NC_HIP_API size_t nc_hip_embedding_bwd_workspace(int64_t N, int64_t V, int64_t D);
