@@ -534,9 +534,10 @@ static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 // unsorted; of 512: 45 unsorted, 2331 times of 256: 33 sorted, 50 unsorted).
 static bool sums_unsorted(int64_t N, int64_t D) { return N <= kFewMost && N * D <= int64_t(1) << 20; }
 
-// Sorted positions of a block: 8 where blocks of 32 would leave most of the chip idle, at the cost of more parts of tokens that
-// occur often (2331 tokens of 250 columns: 28 -> 11 us).
-static int sorted_block(int64_t N, int64_t D) { return (N + 31) / 32 * ((D + 3) / 4) < 65536 ? 8 : 32; }
+// Sorted positions of a block: 8 where blocks of 32 would leave most of the chip idle (4378 tokens of 254 columns 46 -> 34 us, 4300 of 736
+// 57 -> 54, 16245 of 256 alike), but of many tokens 32, since those that occur often go over many blocks (words' frequencies as one over
+// their rank; 17000 of 64: 48 -> 46, 65536 of 64: 112 -> 78; 64 at a time take 97 with 100000 words, 76 with 300).
+static int sorted_block(int64_t N, int64_t D) { return N < 16384 && (N + 31) / 32 * ((D + 3) / 4) < 65536 ? 8 : 32; }
 
 // the workspace: [tokens in order][their positions], where digits are sorted the same again and the digits' counts, [parts]
 struct SortPlan {
