@@ -39,25 +39,45 @@ static Lay lay_of(int64_t D) {
     return l;
 }
 
-template <bool AL>
-__device__ __forceinline__ f4 piece(const float *row, int64_t c, int64_t D) {
-    if (AL || c + 4 <= D) return AL ? *(const f4 *)(row + c) : (f4) * (const f4u *)(row + c);
-    f4 v = {};
-    for (int e = 0; e < (int)(D - c); e++) v[e] = row[c + e];
-    return v;
+// How rows are read and written: by aligned 16 bytes; by 16 bytes anywhere; rows of less than 16 bytes.
+enum { ROWS_SHORT, ROWS_ANYWHERE, ROWS_ALIGNED };
+
+// Four columns of a row from c on: loaded without a branch, since a lane that waits for a row's end of its own waits for each row, and behind
+// the last four columns moved from those, by a step of its own that comes after the loads of all rows (885 tokens of 774 columns, both ways:
+// 34 us by branches, 22 moved at once, 13 so).  What lies behind the row's end is anything.
+template <int M>
+__device__ __forceinline__ f4 load4(const float *row, int64_t c, int64_t D) {
+    if (M == ROWS_ALIGNED) return *(const f4 *)(row + c);
+    if (M == ROWS_SHORT) return f4{row[0], row[min(int64_t(1), D - 1)], row[D - 1], 0.0f};
+    return *(const f4u *)(row + min(c, D - 4));
 }
 
-template <bool AL>
+template <int M>
+__device__ __forceinline__ f4 moved(f4 v, int64_t c, int64_t D) {
+    if (M != ROWS_ANYWHERE || c <= D - 4) return v;
+    const int by = (int)(c - (D - 4));
+    return by == 1 ? f4{v[1], v[2], v[3], 0.0f} : by == 2 ? f4{v[2], v[3], 0.0f, 0.0f} : f4{v[3], 0.0f, 0.0f, 0.0f};
+}
+
+template <int M>
 __device__ __forceinline__ void put(float *row, int64_t c, int64_t D, f4 v) {
-    if (AL) __builtin_nontemporal_store(v, (f4 *)(row + c));
+    if (M == ROWS_ALIGNED) __builtin_nontemporal_store(v, (f4 *)(row + c));
     else if (c + 4 <= D) *(f4u *)(row + c) = v;
     else
         for (int e = 0; e < (int)(D - c); e++) row[c + e] = v[e];
 }
 
+// runs a call made for each of the three
+template <class F>
+static void by_rows(bool al, int64_t D, F run) {
+    if (al) run(std::integral_constant<int, ROWS_ALIGNED>{});
+    else if (D >= 4) run(std::integral_constant<int, ROWS_ANYWHERE>{});
+    else run(std::integral_constant<int, ROWS_SHORT>{});
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------
 // tokens outside the table give rows of zeros
-template <bool AL, int U>
+template <int M, int U>
 __global__ __launch_bounds__(kEmbB) void k_embed(const float *__restrict__ w, int64_t ldw, const int32_t *__restrict__ tokens, float scale,
                                                  float *__restrict__ y, int64_t N, int64_t V, Lay l) {
     const int64_t c = 4 * (((int64_t)blockIdx.y << l.shift) + (threadIdx.x & ((1 << l.shift) - 1)));
@@ -69,10 +89,10 @@ __global__ __launch_bounds__(kEmbB) void k_embed(const float *__restrict__ w, in
 #pragma unroll
     for (int u = 0; u < U; u++) t[u] = i0 + u * rows < N ? tokens[i0 + u * rows] : -1;
 #pragma unroll
-    for (int u = 0; u < U; u++) v[u] = (uint32_t)t[u] < V ? piece<AL>(w + t[u] * ldw, c, l.D) : f4{};
+    for (int u = 0; u < U; u++) v[u] = (uint32_t)t[u] < V ? load4<M>(w + t[u] * ldw, c, l.D) : f4{};
 #pragma unroll
     for (int u = 0; u < U; u++)
-        if (i0 + u * rows < N) put<AL>(y + (i0 + u * rows) * l.D, c, l.D, v[u] * scale);
+        if (i0 + u * rows < N) put<M>(y + (i0 + u * rows) * l.D, c, l.D, moved<M>(v[u], c, l.D) * scale);
 }
 
 // the first token outside the table as (position << 32) | token, or all ones
@@ -291,17 +311,17 @@ struct EmbGrad {
     __device__ __forceinline__ bool counts(uint32_t t) const { return t < V && t != padding; }
 };
 
-template <bool AL>
+template <int M>
 __device__ __forceinline__ void put_row(const EmbGrad &p, uint32_t t, int64_t c, f4 sum) {
     float *row = p.gw + (int64_t)t * p.l.D;
     if (p.acc) {
-        const f4 old = piece<AL>(row, c, p.l.D);
+        const f4 old = moved<M>(load4<M>(row, c, p.l.D), c, p.l.D);
         f4 v;
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = fma_(p.scale, sum[e], old[e]);
-        put<AL>(row, c, p.l.D, v);
+        put<M>(row, c, p.l.D, v);
     } else {
-        put<AL>(row, c, p.l.D, sum * p.scale);
+        put<M>(row, c, p.l.D, sum * p.scale);
     }
 }
 
@@ -309,7 +329,7 @@ __device__ __forceinline__ float *part_at(const EmbGrad &p, int64_t block, int s
     return p.parts + (block * 2 + slot) * ((p.l.D + 3) / 4 * 4) + c;
 }
 
-template <bool AL, int S>
+template <int M, int S>
 __device__ __forceinline__ void sum_block(const EmbGrad &p, int64_t block, int64_t c) {
     constexpr int U = 8;
     const int64_t k0 = block * S, k1 = min(p.N, k0 + S);
@@ -320,7 +340,7 @@ __device__ __forceinline__ void sum_block(const EmbGrad &p, int64_t block, int64
         if (!p.counts(cur)) return;
         if (before) *(f4 *)part_at(p, block, 0, c) = sum;
         else if (goes_on) *(f4 *)part_at(p, block, 1, c) = sum;
-        else put_row<AL>(p, cur, c, sum);
+        else put_row<M>(p, cur, c, sum);
     };
     for (int64_t k = k0; k < k1; k += U) {
         uint32_t t[U];
@@ -328,7 +348,7 @@ __device__ __forceinline__ void sum_block(const EmbGrad &p, int64_t block, int64
 #pragma unroll
         for (int u = 0; u < U; u++) t[u] = k + u < k1 ? p.sorted[k + u] : ~0u;
 #pragma unroll
-        for (int u = 0; u < U; u++) v[u] = k + u < k1 && p.counts(t[u]) ? piece<AL>(p.g + p.from[k + u] * p.l.D, c, p.l.D) : f4{};
+        for (int u = 0; u < U; u++) v[u] = k + u < k1 && p.counts(t[u]) ? load4<M>(p.g + p.from[k + u] * p.l.D, c, p.l.D) : f4{};
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (k + u >= k1) break;
@@ -336,7 +356,7 @@ __device__ __forceinline__ void sum_block(const EmbGrad &p, int64_t block, int64
                 flush(false);
                 cur = t[u], before = false, sum = f4{};
             }
-            sum = sum + v[u];
+            sum = sum + moved<M>(v[u], c, p.l.D);
         }
     }
     flush(k1 < p.N && p.sorted[k1] == cur);
@@ -408,7 +428,7 @@ __device__ __forceinline__ void clear_sorted(const EmbGrad &p) {
     });
 }
 
-template <bool AL, int S>
+template <int M, int S>
 __global__ __launch_bounds__(kEmbB) void k_embed_grad(EmbGrad p) {
     const int64_t c = 4 * (((int64_t)blockIdx.y << p.l.shift) + (threadIdx.x & ((1 << p.l.shift) - 1)));
     if (blockIdx.x >= p.sum_groups) {
@@ -416,12 +436,12 @@ __global__ __launch_bounds__(kEmbB) void k_embed_grad(EmbGrad p) {
         return;
     }
     const int64_t block = (int64_t)blockIdx.x * (kEmbB >> p.l.shift) + (threadIdx.x >> p.l.shift);
-    if (c < p.l.D && block < p.blocks) sum_block<AL, S>(p, block, c);
+    if (c < p.l.D && block < p.blocks) sum_block<M, S>(p, block, c);
 }
 
 // Few tokens, in one launch and unsorted: a workgroup for every position, which goes on if its token has none earlier, lists the token's
 // positions and sums their rows, 16 at a time and these in fp64; the workgroups behind them clear rows.
-template <bool AL, int MOST>
+template <int M, int MOST>
 __global__ __launch_bounds__(kEmbB) void k_embed_few(EmbGrad p, const int32_t *__restrict__ tokens) {
     constexpr int U = 16;
     __shared__ uint32_t token[MOST];
@@ -476,13 +496,13 @@ __global__ __launch_bounds__(kEmbB) void k_embed_few(EmbGrad p, const int32_t *_
         for (int k0 = group; k0 < count; k0 += U * R) {
             f4 v[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) v[u] = k0 + u * R < count ? piece<AL>(p.g + (int64_t)list[k0 + u * R] * p.l.D, c, p.l.D) : f4{};
+            for (int u = 0; u < U; u++) v[u] = k0 + u * R < count ? load4<M>(p.g + (int64_t)list[k0 + u * R] * p.l.D, c, p.l.D) : f4{};
 #pragma unroll
             for (int d = 1; d < U; d *= 2)
 #pragma unroll
                 for (int u = 0; u < U; u += 2 * d) v[u] = v[u] + v[u + d];
 #pragma unroll
-            for (int e = 0; e < 4; e++) sum[e] += (double)v[0][e];
+            for (int e = 0; e < 4; e++) sum[e] += (double)moved<M>(v[0], c, p.l.D)[e];
         }
     if (R > 1) {
 #pragma unroll
@@ -493,11 +513,11 @@ __global__ __launch_bounds__(kEmbB) void k_embed_few(EmbGrad p, const int32_t *_
 #pragma unroll
             for (int e = 0; e < 4; e++) sum[e] += part[e][(r << p.l.shift) + threadIdx.x];
     }
-    if (c < p.l.D) put_row<AL>(p, t, c, f4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]});
+    if (c < p.l.D) put_row<M>(p, t, c, f4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]});
 }
 
 // The rows of tokens that go over blocks, where each begins.
-template <bool AL, int S>
+template <int M, int S>
 __global__ __launch_bounds__(kEmbB) void k_embed_join(EmbGrad p) {
     constexpr int U = 16;
     const int64_t c = 4 * (((int64_t)blockIdx.y << p.l.shift) + (threadIdx.x & ((1 << p.l.shift) - 1)));
@@ -524,7 +544,7 @@ __global__ __launch_bounds__(kEmbB) void k_embed_join(EmbGrad p) {
 #pragma unroll
             for (int e = 0; e < 4; e++) sum[e] += (double)v[u][e];
     }
-    put_row<AL>(p, t, c, f4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]});
+    put_row<M>(p, t, c, f4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]});
 }
 
 static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
@@ -591,8 +611,10 @@ extern "C" NC_HIP_API int nc_hip_embedding_fwd(int64_t N, int64_t V, int64_t D, 
         if (groups * l.slices() * kEmbB > kMaxLanes) return set_error(NC_HIP_ERR_ARG, "%s: bad size, no launch holds it", what);
         const dim3 grid((unsigned)groups, (unsigned)l.slices());
         auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, kEmbB, 0, st, w, ldw, tokens, scale, y, N, V, l); };
-        if (U == 4) al ? run(k_embed<true, 4>) : run(k_embed<false, 4>);
-        else al ? run(k_embed<true, 1>) : run(k_embed<false, 1>);
+        by_rows(al, D, [&](auto m) {
+            constexpr int M = decltype(m)::value;
+            U == 4 ? run(k_embed<M, 4>) : run(k_embed<M, 1>);
+        });
     }
     return check_launch(what);
 }
@@ -637,8 +659,10 @@ extern "C" NC_HIP_API int nc_hip_embedding_bwd(int64_t N, int64_t V, int64_t D, 
     const dim3 grid((unsigned)(groups + clear), (unsigned)slices), joins((unsigned)groups, (unsigned)slices);
     if (few) {
         auto sum = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, kEmbB, 0, st, p, tokens); };
-        if (N <= 1024) al ? sum(k_embed_few<true, 1024>) : sum(k_embed_few<false, 1024>);
-        else al ? sum(k_embed_few<true, kFewMost>) : sum(k_embed_few<false, kFewMost>);
+        by_rows(al, D, [&](auto m) {
+            constexpr int M = decltype(m)::value;
+            N <= 1024 ? sum(k_embed_few<M, 1024>) : sum(k_embed_few<M, kFewMost>);
+        });
         return check_launch(what);
     }
     if (N > kRankMost) {
@@ -658,11 +682,10 @@ extern "C" NC_HIP_API int nc_hip_embedding_bwd(int64_t N, int64_t V, int64_t D, 
         hipLaunchKernelGGL(k_embed_rank, (unsigned)((N + 31) / 32), kRankB, 0, st, tokens, (int)N, sorted, from);
     }
     auto run = [&](auto kernel, dim3 g) { hipLaunchKernelGGL(kernel, g, kEmbB, 0, st, p); };
-    if (S == 8) al ? run(k_embed_grad<true, 8>, grid) : run(k_embed_grad<false, 8>, grid);
-    else al ? run(k_embed_grad<true, 32>, grid) : run(k_embed_grad<false, 32>, grid);
-    if (p.blocks > 1) {
-        if (S == 8) al ? run(k_embed_join<true, 8>, joins) : run(k_embed_join<false, 8>, joins);
-        else al ? run(k_embed_join<true, 32>, joins) : run(k_embed_join<false, 32>, joins);
-    }
+    by_rows(al, D, [&](auto m) {
+        constexpr int M = decltype(m)::value;
+        S == 8 ? run(k_embed_grad<M, 8>, grid) : run(k_embed_grad<M, 32>, grid);
+        if (p.blocks > 1) S == 8 ? run(k_embed_join<M, 8>, joins) : run(k_embed_join<M, 32>, joins);
+    });
     return check_launch(what);
 }
