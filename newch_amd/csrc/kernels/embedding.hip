@@ -16,7 +16,7 @@ namespace nchip {
 
 constexpr int kEmbB = 256;
 constexpr int kClearMost = 32768;  // words of the table that one workgroup clears, at most
-constexpr int kClearFew = 4096;    // and without a sort
+constexpr int kClearFew = 4096;    // and, always as many, without a sort
 constexpr int kRankB = 1024, kRankMost = 8192;  // tokens whose places are counted, at most
 constexpr int kFewMost = 2560;                  // tokens whose rows are summed without a sort, at most
 constexpr int kDigitBits = 10, kChunk = 1024;   // of the others' sort
@@ -440,14 +440,15 @@ __global__ __launch_bounds__(kEmbB) void k_embed_grad(EmbGrad p) {
 }
 
 // Few tokens, in one launch and unsorted: a workgroup for every position, which goes on if its token has none earlier, lists the token's
-// positions and sums their rows, 16 at a time and these in fp64; the workgroups behind them clear rows.
+// positions and sums their rows, 8 at a time and these in fp64; the workgroups behind them clear rows.
 template <int M, int MOST>
 __global__ __launch_bounds__(kEmbB) void k_embed_few(EmbGrad p, const int32_t *__restrict__ tokens) {
-    constexpr int U = 16;
-    __shared__ uint32_t token[MOST];
+    constexpr int U = 8;
+    // the tokens, and behind the last look at them the groups' sums: 2000 tokens of 512 columns 21.5 -> 18.9 us by the room it leaves
+    __shared__ __attribute__((aligned(16))) uint32_t token[MOST > 8 * kEmbB ? MOST : 8 * kEmbB];
+    double(*part)[kEmbB] = (double(*)[kEmbB])token;
     __shared__ uint16_t list[MOST];
     __shared__ unsigned long long masks[MOST / kWave];
-    __shared__ double part[4][kEmbB];
     const int N = (int)p.N, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int64_t c = 4 * (((int64_t)blockIdx.y << p.l.shift) + (threadIdx.x & ((1 << p.l.shift) - 1)));
     const int R = kEmbB >> p.l.shift, group = threadIdx.x >> p.l.shift;
@@ -549,9 +550,9 @@ __global__ __launch_bounds__(kEmbB) void k_embed_join(EmbGrad p) {
 
 static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
-// Without a sort: 17 -> 12 us at 800 tokens of 100 columns, 19 -> 16 at 2331 of 256, 20 -> 18 at 3000.  A token that all positions have
+// Without a sort: 17 -> 12 us at 800 tokens of 100 columns, 19 -> 13 at 2331 of 256.  A token that all positions have
 // is one workgroup's and slice's, so long rows of many tokens are sorted all the same (1024 times the same of 2048: 27 us sorted, 91
-// unsorted; of 512: 45 unsorted, 2331 times of 256: 33 sorted, 50 unsorted).
+// unsorted; of 512: 47 unsorted, 2331 times of 256: 33 sorted, 50 unsorted).
 static bool sums_unsorted(int64_t N, int64_t D) { return N <= kFewMost && N * D <= int64_t(1) << 20; }
 
 // Sorted positions of a block: 8 where blocks of 32 would leave most of the chip idle (4378 tokens of 254 columns 46 -> 34 us, 4300 of 736
@@ -649,7 +650,7 @@ extern "C" NC_HIP_API int nc_hip_embedding_bwd(int64_t N, int64_t V, int64_t D, 
     const int64_t groups = few ? N : (p.blocks + p.l.rows() - 1) / p.l.rows();
     p.sum_groups = (unsigned)groups;
     const int64_t slices = p.l.slices(), words = V * D;
-    p.clear_words = (int)std::max<int64_t>(4 * kEmbB, std::min<int64_t>(few ? kClearFew : kClearMost, words / 4096 / (4 * kEmbB) * (4 * kEmbB)));
+    p.clear_words = few ? kClearFew : (int)std::max<int64_t>(4 * kEmbB, std::min<int64_t>(kClearMost, words / 4096 / (4 * kEmbB) * (4 * kEmbB)));
     p.clear_shift = (int)((uintptr_t)gw / 4 & 3u);
     const int64_t chunks = (words + p.clear_shift + p.clear_words - 1) / p.clear_words;
     const int64_t clear = accumulate ? 0 : (chunks + slices - 1) / slices;
