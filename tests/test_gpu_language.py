@@ -335,7 +335,7 @@ def test_loss_and_gradients(K, form, shape, bias, ignored):
         assert all((again[k].view(np.uint32) == got[k].view(np.uint32)).all() for k in c.g), "the same call twice"
 
 
-@pytest.mark.parametrize("shape", [(5, 33, 17), (300, 96, 1000), (513, 100, 5003), (257, 256, 513)], ids=str)
+@pytest.mark.parametrize("shape", [(5, 33, 17), (300, 96, 1000), (513, 100, 5003), (257, 256, 513), (7, 512, 4099), (40, 516, 4099)], ids=str)
 def test_loss_added_gradients_sum_and_its_own_gradient(K, form, shape):
     x, w, b, labels = loss_inputs(*shape, 12, True, 0.2)
     labels[0] = shape[2] - 1
@@ -349,7 +349,7 @@ def test_loss_added_gradients_sum_and_its_own_gradient(K, form, shape):
         agree(c.get(), ref, x, w, old=old)
 
 
-@pytest.mark.parametrize("shape", [(5, 33, 17), (300, 96, 1000), (1030, 260, 1027)], ids=str)
+@pytest.mark.parametrize("shape", [(5, 33, 17), (300, 96, 1000), (1030, 260, 1027), (7, 512, 4099), (40, 516, 4099)], ids=str)
 @pytest.mark.parametrize("grads", ["", "x", "w", "b", "xw"])
 def test_loss_some_gradients(K, form, shape, grads):
     x, w, b, labels = loss_inputs(*shape, 13, False, 0.1)
@@ -361,7 +361,7 @@ def test_loss_some_gradients(K, form, shape, grads):
     agree(got, ref, x, w)
 
 
-@pytest.mark.parametrize("shape", [(5, 33, 17), (300, 96, 1000), (600, 128, 2048)], ids=str)
+@pytest.mark.parametrize("shape", [(5, 33, 17), (300, 96, 1000), (600, 128, 2048), (7, 512, 4099), (40, 516, 4099)], ids=str)
 def test_loss_labels_outside(K, form, shape):
     N, D, V = shape
     x, w, b, labels = loss_inputs(*shape, 14, True, 0.2)
@@ -374,7 +374,7 @@ def test_loss_labels_outside(K, form, shape):
     assert c.bad.to_numpy(np.uint64, 1)[0] == (np.uint64(1) << np.uint64(32)) | np.uint64(np.uint32(-7 % 2 ** 32))
 
 
-@pytest.mark.parametrize("shape", [(3, 5, 9), (300, 96, 1000), (600, 128, 2048)], ids=str)
+@pytest.mark.parametrize("shape", [(3, 5, 9), (300, 96, 1000), (600, 128, 2048), (7, 512, 4099), (40, 516, 4099)], ids=str)
 def test_loss_no_row_counts(K, form, shape):
     x, w, b, labels = loss_inputs(*shape, 15, True, 0.0)
     labels[:] = 5  # the ignored label may be a word
@@ -395,7 +395,7 @@ def test_loss_of_no_rows(K, form):
     assert np.isnan(got["loss"]) and (got["gw"] == 0).all() and (got["gb"] == 0).all()
 
 
-@pytest.mark.parametrize("shape", [(40, 33, 170), (300, 96, 1000), (600, 128, 2048)], ids=str)
+@pytest.mark.parametrize("shape", [(40, 33, 170), (300, 96, 1000), (600, 128, 2048), (7, 512, 4099), (40, 516, 4099)], ids=str)
 def test_loss_masked_words(K, form, shape):
     """A bias of -inf, or of the type's lowest value, takes words out: no probability, no gradient."""
     N, D, V = shape
@@ -413,7 +413,7 @@ def test_loss_masked_words(K, form, shape):
         assert (got["gw"][out] == 0).all() and (got["gb"][out] == 0).all()
 
 
-@pytest.mark.parametrize("shape", [(40, 33, 170), (300, 96, 1000), (600, 128, 2048)], ids=str)
+@pytest.mark.parametrize("shape", [(40, 33, 170), (300, 96, 1000), (600, 128, 2048), (7, 512, 4099), (40, 516, 4099)], ids=str)
 def test_loss_rows_and_words_of_unlike_sizes(K, form, shape):
     """Rows of x and of w whose sizes lie many powers of two apart: each result keeps the precision of what it sums."""
     N, D, V = shape
@@ -446,7 +446,7 @@ def test_loss_certain_rows(K, form, shape):
     assert (err <= (2 * dz + HALF * (20 + np.sqrt(V))) * spread).all()
 
 
-@pytest.mark.parametrize("shape", [(40, 33, 170), (300, 96, 1000), (600, 128, 2048)], ids=str)
+@pytest.mark.parametrize("shape", [(40, 33, 170), (300, 96, 1000), (600, 128, 2048), (9, 512, 4099), (40, 516, 4099)], ids=str)
 def test_loss_values_that_are_not_finite(K, form, shape):
     """NaN in a row that counts makes that row's loss and gradient NaN and leaves the other rows' theirs."""
     N, D, V = shape
@@ -464,7 +464,7 @@ def test_loss_values_that_are_not_finite(K, form, shape):
 
 
 @pytest.mark.parametrize("rows", [1, 300])
-@pytest.mark.parametrize("shape", [(700, 40, 600), (1030, 260, 1027), (9, 5, 5000)], ids=str)
+@pytest.mark.parametrize("shape", [(700, 40, 600), (1030, 260, 1027), (9, 5, 5000), (40, 516, 4099)], ids=str)
 def test_loss_in_pieces(K, form, shape, rows, monkeypatch):
     """Rows taken a few at a time, gradients added from piece to piece; rows that do not count leave the last pieces empty."""
     monkeypatch.setenv("NC_HIP_VOCAB_ROWS", str(rows))
