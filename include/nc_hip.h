@@ -386,9 +386,11 @@ NC_HIP_API int nc_hip_dropout_bwd(int64_t n, double p, uint64_t seed, uint64_t o
  * *gout * loss (gout: one float in device memory; NULL: 1).  Sums in a fixed order.  Outputs overlap neither inputs nor each other.
  * The workspace (16-byte aligned) is for the gradients that are asked for; its contents count only within a call.
  * N < 2^31, D <= 2^20, V <= 2^26.
- * Precision: few rows or words run on plain fp32 products.  Where it pays, operands (x and w by rows and by columns, and the
- * gradient of z by both) are held in two fp16 pieces, 22 bits, under a power of two of their row or column: a value below 2^-17 of the
- * largest of its row (column) is held to 2^-40 of it; an infinity that counts gives NaN.  Products are summed in fp32 either way.
+ * Precision: few rows or words run on plain fp32 products, others, by the sizes alone, on products of operands in two fp16 pieces, 22
+ * bits, under powers of two; either way products are summed in fp32.  x and w have the power of each row's largest value: in z a value down to
+ * 2^-22 of that has its 22 bits and one below is held to 2^-44 of it; in gx (values of w) and gw (values of x) it is 2^-28 and 2^-50.  The
+ * gradient of z has the power of the largest term that a row of gx or gw sums; terms below 2^-17 of that are held to 2^-39 of it.
+ * An infinity in x or w that counts gives NaN in pieces.
  * Test hooks: NC_HIP_VOCAB_FORM=fp32 or split chooses the form, NC_HIP_VOCAB_ROWS=n the rows whose z is held at a time (the
  * workspace's size follows both). */
 NC_HIP_API size_t nc_hip_linear_cross_entropy_workspace(int64_t N, int64_t D, int64_t V, int want_x, int want_w, int want_b);

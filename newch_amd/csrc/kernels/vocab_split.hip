@@ -2,8 +2,13 @@
 //
 // A library's fp32 product of 8192^3 reaches an eighth of what its fp16 one does, so operands are cut into two fp16 pieces under a
 // power of two of their row: x = 2^e (hi + lo), the row's largest finite value in [2^14, 2^15) after the scaling, hi and lo rounded to
-// nearest: 22 bits of every value down to 2^-17 of its row's largest, an absolute error of 2^-40 of that below.  A product is hi hi +
-// hi lo + lo hi, summed in fp32; lo lo, at most 2^-22 of a term, is left out.
+// nearest.  A product is hi hi + hi lo + lo hi, summed in fp32; lo lo, at most 2^-22 of a term, is left out.
+//
+// fp16 has its 11 bits down to 2^-14 only, and steps of 2^-24 below.  So x and W keep lo as 2^11 lo, and the factors 2^-11 that their
+// products then need are taken out of fragments in registers.  gx and gW: out of G's hi, so that every value of W and x has its 22 bits down to
+// 2^-28 of its row's largest (an absolute error of 2^-50 of that below), and a column that is small in all rows its gradient's bits.  z:
+// halves of it out of all four pieces, 22 bits down to 2^-22 and 2^-44 below, so that columns which x and W scale oppositely cost
+// nothing.  G's own lo is kept as it is: what is below 2^-17 of the largest term of a sum, and so held to 2^-39 of it, is lost in that sum.
 //
 // x and W are packed once, by rows.  gx and gW sum over those rows, so G takes their powers of two: gx_n = sum_v (G_nv 2^e_v) pieces of W_v,
 // where the row n of G 2^e has the power of its own largest entry, which is that of the largest term that gx_n sums; gW in
@@ -80,6 +85,8 @@ __device__ __forceinline__ int word_exponent(int term) { return term - 14; }
 struct Pieces {
     h8 hi, lo;
 };
+constexpr int kLow = 11;  // x and W keep 2^kLow lo
+template <int LOW>
 __device__ __forceinline__ Pieces cut(const float (&x)[8], float scale) {
     Pieces r;
 #pragma unroll
@@ -87,7 +94,7 @@ __device__ __forceinline__ Pieces cut(const float (&x)[8], float scale) {
         const float v = x[i] * scale;
         const _Float16 h = (_Float16)v;
         r.hi[i] = h;
-        r.lo[i] = (_Float16)(v - (float)h);
+        r.lo[i] = (_Float16)((v - (float)h) * (float)(1 << LOW));
     }
     return r;
 }
@@ -318,19 +325,26 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 2; j++) acc[i][j] = f16x{};
-    auto multiply = [&](const Frags &f) {
+    // hi hi, then the pieces scaled in place, then hi lo and lo hi
+    auto product = [&](const Frags &f, int a, int b) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.a[i][1], f.b[j][0], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.a[i][a], f.b[j][b], acc[i][j], 0, 0, 0);
+    };
+    auto multiply = [&](Frags &f) {
+        constexpr _Float16 kHalf = (_Float16)(1.0f / (1 << kLow / 2)), kRest = (_Float16)(1.0f / (1 << (kLow - kLow / 2)));
+        product(f, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4; i++) {
+            f.a[i][0] *= kZ ? kHalf : (_Float16)(1.0f / (1 << kLow));
+            if (kZ) f.a[i][1] *= kRest;
+        }
 #pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.a[i][0], f.b[j][1], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.a[i][0], f.b[j][0], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < 2; j++)
+            if (kZ) f.b[j][0] *= kHalf, f.b[j][1] *= kRest;
+        product(f, 0, 1);
+        product(f, 1, 0);
     };
     // At the barrier before block kt every wave's share of block kt + 1 is in LDS and every wave holds block kt in registers, so its
     // stage takes block kt + 3.  A wave reads block kt + 1 into registers while it multiplies block kt.
@@ -546,7 +560,7 @@ __global__ __launch_bounds__(512) void k_vl_pack(PackPair pp) {
             const int kb = k0 + wave + i * kWaves;
             if (kb >= pp.kblocks) break;
             if (!NB) load(kb, x[i]);
-            store_block(out + (int64_t)kb * 2048, lane, cut(x[i], scale));
+            store_block(out + (int64_t)kb * 2048, lane, cut<kLow>(x[i], scale));
         }
     }
 }
@@ -711,7 +725,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_grad(GradArgs p) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[4 * t + e] = __builtin_amdgcn_ldexpf(g[8 * s + 4 * t + e], ew[e] - row.e);
             }
-            store_block((char *)z + s * 2048, lane, cut(x, 1.0f));
+            store_block((char *)z + s * 2048, lane, cut<0>(x, 1.0f));
         }
     }
     if constexpr (W) {
@@ -732,7 +746,7 @@ __global__ __launch_bounds__(kVlB) void k_vl_grad(GradArgs p) {
                 sum += v;
                 x[e] = __builtin_amdgcn_ldexpf(v, exs[wave][k] - ev);
             }
-            store_block(p.turned + vb * p.turned_step + (nb * 2 + s) * 2048, lane, cut(x, 1.0f));
+            store_block(p.turned + vb * p.turned_step + (nb * 2 + s) * 2048, lane, cut<0>(x, 1.0f));
         }
         if (p.column) {
             sum += __shfl_xor(sum, 32);
