@@ -144,9 +144,15 @@ struct Frags {
     h8 a[4][2], b[2][2];
 };
 
-__device__ __forceinline__ float vl_coef(const VlHead *head, const float *gout, int sum) {
-    const float c = gout ? *gout : 1.0f;
-    return sum ? c : c / (float)head->count;
+// What the sums of gx, gW and gb are multiplied by, as m 2^e with 1 <= |m| < 2: the sums are in pieces' powers, and with 2^e taken
+// into those no step passes a float's range unless the result does (gW sums N rows, of which the mean may be all that is a float).
+struct VlCoef {
+    float m;
+    int e;
+};
+__device__ __forceinline__ VlCoef vl_coef(const VlHead *head, const float *gout, int sum) {
+    const float c = gout ? *gout : 1.0f, v = sum ? c : c / (float)head->count;
+    return {2.0f * __builtin_amdgcn_frexp_mantf(v), __builtin_amdgcn_frexp_expf(v) - 1};
 }
 
 // The wave's 128 words by 64 rows of z, out of its accumulators.
@@ -404,7 +410,7 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) out[(32 * i + 8 * (r / 4) + r % 4) * p.cols + 32 * j] = acc[i][j][r];
     } else {
-        const float c = nk > 0 ? vl_coef(p.head, p.gout, p.sum) : 0.0f;
+        const VlCoef c = nk > 0 ? vl_coef(p.head, p.gout, p.sum) : VlCoef{0.0f, 0};
         const int64_t m1 = m0 + 4 * (at >> 5), d = n0 + (at & 31);
         float *out = p.out + m1 * p.D + d;
         const bool in0 = d < p.D, in1 = d + 32 < p.D;
@@ -425,11 +431,11 @@ __global__ __launch_bounds__(Tile<WN>::kLanes, 2) void k_vl_product(MmArgs p) {
             for (int r = 0; r < 16; r++) {
                 const int dm = 32 * i + 8 * (r / 4) + r % 4;
                 if (m1 + dm >= p.V) continue;
-                const int em = word_exponent(p.eg[m1 + dm]);
+                const int em = word_exponent(p.eg[m1 + dm]) + c.e;
                 float *o = out + (int64_t)dm * p.D;
                 const float v0 = __builtin_amdgcn_ldexpf(acc[i][0][r], em), v1 = __builtin_amdgcn_ldexpf(acc[i][1][r], em);
-                if (in0) o[0] = p.acc ? fma_(v0, c, old[0][r]) : v0 * c;
-                if (in1) o[32] = p.acc ? fma_(v1, c, old[1][r]) : v1 * c;
+                if (in0) o[0] = p.acc ? fma_(v0, c.m, old[0][r]) : v0 * c.m;
+                if (in1) o[32] = p.acc ? fma_(v1, c.m, old[1][r]) : v1 * c.m;
             }
         }
     }
@@ -777,32 +783,32 @@ struct TailArgs {
 __global__ __launch_bounds__(kVlB) void k_vl_ends(TailArgs p) {
     __shared__ double sh[kVlB / kWave];
     const int64_t count = p.head->count, left = min(p.rows, count - p.row0);
-    const float c = count ? vl_coef(p.head, p.gout, p.sum) : 0.0f;
+    const VlCoef c = count ? vl_coef(p.head, p.gout, p.sum) : VlCoef{0.0f, 0};
     unsigned b = blockIdx.x;
     if (b < p.gx) {
         const int slices = p.head->slices_x;
         for (int64_t n = b; n < left; n += p.gx) {
-            const int en = p.row[n].e;
+            const int en = p.row[n].e + c.e;
             float *out = p.out_x + (int64_t)p.from[n] * p.D;
             for (int64_t d = threadIdx.x; d < p.D; d += kVlB) {
                 double s = 0.0;
 #pragma unroll 8
                 for (int i = 0; i < slices; i++) s += (double)p.parts_x[((int64_t)i * p.rows + n) * p.cols + d];
                 const float v = __builtin_amdgcn_ldexpf((float)s, en);
-                out[d] = p.acc_x ? fma_(v, c, out[d]) : v * c;
+                out[d] = p.acc_x ? fma_(v, c.m, out[d]) : v * c.m;
             }
         }
     } else if ((b -= p.gx) < p.gw) {
         const int slices = p.head->slices_w;
         for (int64_t v = b; v < p.V; v += p.gw) {
-            const int ev = word_exponent(p.term[v]);
+            const int ev = word_exponent(p.term[v]) + c.e;
             for (int64_t d = threadIdx.x; d < p.D; d += kVlB) {
                 double s = 0.0;
 #pragma unroll 8
                 for (int i = 0; i < slices; i++) s += (double)p.parts_w[((int64_t)i * p.words + v) * p.cols + d];
                 const float x = __builtin_amdgcn_ldexpf((float)s, ev);
                 float *o = p.out_w + v * p.D + d;
-                *o = p.acc_w ? fma_(x, c, *o) : x * c;
+                *o = p.acc_w ? fma_(x, c.m, *o) : x * c.m;
             }
         }
     } else if ((b -= p.gw) < p.gb) {
@@ -811,7 +817,8 @@ __global__ __launch_bounds__(kVlB) void k_vl_ends(TailArgs p) {
         double s = 0.0;
 #pragma unroll 8
         for (int64_t i = 0; i < blocks; i++) s += (double)p.column[i * p.words + v];
-        p.out_b[v] = p.acc_b ? fma_((float)s, c, p.out_b[v]) : (float)s * c;
+        const float x = __builtin_amdgcn_ldexpf((float)s, c.e);
+        p.out_b[v] = p.acc_b ? fma_(x, c.m, p.out_b[v]) : x * c.m;
     } else {
         const double t = vl_wg_sum(vl_lane_sum(p.losses, count), sh);
         if (threadIdx.x == 0) *p.loss = p.sum ? (float)t : count ? (float)(t / (double)count) : __builtin_nanf("");

@@ -41,7 +41,8 @@ def bounds(x, w, ref, gout=1.0):
         """A B summed over K: A's error, the products' roundings, B's floor and A's"""
         term = (A * lB).max(-1, keepdims=True)
         return (dA @ np.abs(B) + rel(K) * np.sqrt((A ** 2) @ (B ** 2)) + SUM_FLOOR * np.sqrt(((A * lB) ** 2).sum(-1, keepdims=True))
-                + G_FLOOR * term * l2((B / safe(lB)[:, None]).T))
+                + G_FLOOR * term * l2((B / safe(lB)[:, None]).T)
+                + 2 * K * 2.0 ** -150)  # where terms are below a float's normal range each product and each addition rounds to steps of 2^-149
 
     rows = (2 * worst + 4 * HALF)[:, 0] * on + 4 * HALF * np.abs(ref["rows"])
     return {"gx": product(dG, aG, w64, lw, V), "gw": product(dG.T, aG.T, x64, lx, N), "rows": rows}
