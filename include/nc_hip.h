@@ -390,7 +390,10 @@ NC_HIP_API int nc_hip_dropout_bwd(int64_t n, double p, uint64_t seed, uint64_t o
  * bits, under powers of two; either way products are summed in fp32.  x and w have the power of each row's largest value: in z a value down to
  * 2^-22 of that has its 22 bits and one below is held to 2^-44 of it; in gx (values of w) and gw (values of x) it is 2^-28 and 2^-50.  The
  * gradient of z has the power of the largest term that a row of gx or gw sums; terms below 2^-17 of that are held to 2^-39 of it.
- * An infinity in x or w that counts gives NaN in pieces.
+ * Values that are not finite: a row of x that holds one and counts has no finite loss or gradient, and neither have gw and gb; the other rows
+ * have theirs.  NaN in w or the bias, or +inf in the bias, leaves no row a loss; -inf in the bias takes its word out.  An infinity in w
+ * leaves none in pieces, and on fp32 products those of the rows that it gives -inf.  Where w is not finite no gradient need be, those of
+ * rows that do not count among them.
  * Test hooks: NC_HIP_VOCAB_FORM=fp32 or split chooses the form, NC_HIP_VOCAB_ROWS=n the rows whose z is held at a time (the
  * workspace's size follows both). */
 NC_HIP_API size_t nc_hip_linear_cross_entropy_workspace(int64_t N, int64_t D, int64_t V, int want_x, int want_w, int want_b);
