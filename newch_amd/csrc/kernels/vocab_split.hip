@@ -46,9 +46,8 @@ struct Tile {
     static constexpr int kLoads = 2 * (kA + 1);      // and the KiB that these are
 };
 constexpr int64_t kZBytes = int64_t(4) << 30;  // of z and of the turned G, both together, held at a time
-constexpr int64_t kScored = int64_t(1) << 36;  // products of a launch that leaves no z
 constexpr int64_t kPieceRows = 1 << 20;
-constexpr int64_t kPartBytes = int64_t(512) << 20;  // of the parts of gx
+constexpr int64_t kPartBytes = int64_t(512) << 20;  // of the parts of gx; of those of gW; of the statistics where no z is held
 constexpr int kStatWords = 128;  // words of one partial statistic
 
 constexpr float kLog2e = 1.44269504088896341f;
@@ -841,7 +840,8 @@ static SplitPlan split_plan(int64_t N, int64_t D, int64_t V, bool want_x, bool w
     SplitPlan p{};
     const bool grad = want_x || want_w || want_b;
     p.n = up_to(N, kTileM), p.d = up_to(D, kTileMost), p.v = up_to(V, kTileM), p.dk = up_to(D, 32);
-    const int64_t most = grad ? kZBytes / (8 * p.v) : kScored / p.v;
+    int64_t most = grad ? kZBytes / (8 * p.v) : kPartBytes / (p.v / kStatWords * (int64_t)sizeof(VlPart));
+    if (want_x) most = std::min(most, kPartBytes / (p.d * 4));
     p.piece = std::max<int64_t>(kTileM, std::min(std::min(p.n, up_to(vl_piece_rows(kPieceRows), kTileM)), most / kTileM * kTileM));
     p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(64, kPartBytes / (p.piece * p.d * 4)));
     // gW: where its tiles would leave the chip's CUs idle
