@@ -550,7 +550,10 @@ __global__ __launch_bounds__(kEmbB) void k_embed_join(EmbGrad p) {
 
 static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
-// Without a sort: 17 -> 12 us at 800 tokens of 100 columns, 19 -> 13 at 2331 of 256.  A token that all positions have
+// Without a sort: 17 -> 12 us at 800 tokens of 100 columns, 19 -> 13 at 2331 of 256.  Every workgroup looks at all tokens, so its lead
+// is gone from some number of them on, which depends on the words (us, unsorted : sorted; 10007 and 50000 rows): even ones over rows of 250
+// and 256 columns 1536 14 : 17, 2304 18 : 18, 2560 23 : 21, 4096 31 : 23; of 16 to 128 columns 2560 14 : 16, 3088 15 : 16, 3584 17 : 17, 4096
+// 20 : 17; frequencies as one over their rank 2560 16 : 23, 3584 29 : 28, 4096 33 : 30.  2560 lies between.  A token that all positions have
 // is one workgroup's and slice's, so long rows of many tokens are sorted all the same (1024 times the same of 2048: 27 us sorted, 91
 // unsorted; of 512: 47 unsorted, 2331 times of 256: 33 sorted, 50 unsorted).
 static bool sums_unsorted(int64_t N, int64_t D) { return N <= kFewMost && N * D <= int64_t(1) << 20; }
