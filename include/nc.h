@@ -290,7 +290,8 @@ NC_API nc_tensor *nc_dropout_seeded(nc_tensor *x, nc_tensor *residual, double p,
 /* The cross entropy of x weight^T + bias (x [.., D], weight [V, D], bias [V] or NULL) against labels (i32, x's shape without its last
  * dim) without keeping the products: the mean, or the sum, over the rows whose label is not `ignore` (a mean over none is NaN).  Rows that
  * do not count may hold anything.  A label outside [0, V) that is not `ignore` fails the call with NC_ERR_ARG.  Where an input
- * needs a gradient the forward takes it and keeps it for the backward, which scales it: inputs may be written in between. */
+ * needs a gradient the forward takes it and keeps it for the backward, which scales it: inputs may be written in between.  Large
+ * products hold their operands in 22 bits (nc_hip_linear_cross_entropy has the bounds) and sum in fp32. */
 NC_API nc_tensor *nc_linear_cross_entropy(nc_tensor *x, nc_tensor *weight, nc_tensor *bias, nc_tensor *labels, int32_t ignore, int sum);
 
 #ifdef __cplusplus
